@@ -2,10 +2,13 @@
 // argument validation, kernel selection and the device fault word.
 #include <cmath>
 #include <cstdio>
+#include <cstdlib>
+#include <cstring>
 #include <mutex>
 
 #include "common.cuh"
 #include "decode.cuh"
+#include "int4.cuh"
 #include "int8.cuh"
 #include "kv_cache.cuh"
 #include "rope.cuh"
@@ -106,6 +109,7 @@ const char* ts_attn_strerror(int status) {
     case TS_ERR_LAUNCH: return "CUDA kernel launch or driver call failed";
     case TS_ERR_DEVICE_TIMEOUT: return "a bounded wait inside an engine kernel gave up";
     case TS_ERR_CAPACITY: return "KV-cache capacity exceeded or empty append";
+    case TS_ERR_PAGE: return "a page table entry outside its pool";
   }
   return "unknown status";
 }
@@ -320,6 +324,193 @@ int ts_attn_decode_int8(const ts_attn_params* p, const float* key_scales, const 
                                             workspace_bytes, fault_ptr(), as_stream(stream)));
 }
 
+}  // extern "C"
+
+namespace {
+
+bool int4_shape_ok(int head_dim, int page_size) {
+  return head_dim > 0 && head_dim <= 256 && head_dim % 32 == 0 &&
+         (page_size == 16 || page_size == 32 || page_size == 64);
+}
+
+int check_int4_cache(const ts_kv4_cache* c) {
+  if (!c || !c->pool || !c->table || reinterpret_cast<uintptr_t>(c->pool) % 16) return TS_ERR_INVALID_ARGUMENT;
+  if (c->batch <= 0 || c->slots <= 0 || c->pages <= 0 || c->kv_heads <= 0) return TS_ERR_INVALID_ARGUMENT;
+  if (!int4_shape_ok(c->head_dim, c->page_size)) return TS_ERR_UNSUPPORTED;
+  if (c->page_stride % 16 ||
+      c->page_stride < (int64_t)c->kv_heads * tsa::int4_block_bytes(c->head_dim, c->page_size))
+    return TS_ERR_INVALID_ARGUMENT;
+  return TS_OK;
+}
+
+bool int4_dtype_ok(int d) { return d == TS_F32 || d == TS_F16 || d == TS_BF16; }
+
+int check_int4_attn(const ts_attn_params* p, const ts_kv4_cache* c) {
+  if (!p) return TS_ERR_INVALID_ARGUMENT;
+  const int st = check_int4_cache(c);
+  if (st != TS_OK) return st;
+  if (!int4_dtype_ok(p->dtype) || p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
+  if (p->batch != c->batch || p->kv_heads != c->kv_heads || p->head_dim != c->head_dim ||
+      p->value_dim != c->head_dim)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (p->q_heads <= 0 || p->q_len <= 0 || p->kv_len <= 0 || p->q_heads % p->kv_heads) return TS_ERR_INVALID_ARGUMENT;
+  if (p->kv_len > (int64_t)c->slots * c->page_size) return TS_ERR_INVALID_ARGUMENT;
+  if (!p->q.data || !p->o.data || !p->kv_lens) return TS_ERR_INVALID_ARGUMENT;
+  if (!(p->scale == p->scale) || p->scale > 1.0e300 || p->scale < -1.0e300) return TS_ERR_INVALID_ARGUMENT;
+  if ((int64_t)p->q_heads / p->kv_heads * p->q_len > 0x40000000) return TS_ERR_UNSUPPORTED;
+  return TS_OK;
+}
+
+// Bytes of the dequantised keys (and of the values after them) the prefill route works on.
+size_t int4_prefill_half(const ts_attn_params& p) {
+  return (size_t)p.batch * p.kv_heads * p.kv_len * p.head_dim * 2;
+}
+
+// The same problem over contiguous keys and values of q's type at `ws`.
+ts_attn_params int4_prefill_params(const ts_attn_params& p, void* ws) {
+  ts_attn_params d = p;
+  const int64_t row = p.head_dim, head = row * p.kv_len;
+  d.k = ts_view4{ws, {head * p.kv_heads, head, row, 1}};
+  d.v = ts_view4{reinterpret_cast<unsigned char*>(ws) + int4_prefill_half(p), {head * p.kv_heads, head, row, 1}};
+  d.causal_offset = 0;
+  return d;
+}
+
+// Query columns of a KV head (group x tokens) from which dequantising the pages and running the
+// prefill kernel is faster than attending over the pages.
+constexpr int kInt4PrefillColumns = 64;
+
+bool int4_prefill(const ts_attn_params& p) {
+  if (!int4_dtype_ok(p.dtype) || p.dtype == TS_F32) return false;
+  alignas(16) static unsigned char aligned[16];  // stands for the workspace, which must be 16-byte aligned
+  if (!tsa::tc_fwd_supported(int4_prefill_params(p, aligned))) return false;
+  const char* force = std::getenv("TS_INT4_KERNEL");
+  if (force && !std::strcmp(force, "pages")) return false;
+  if (force && !std::strcmp(force, "prefill")) return true;
+  return (int64_t)p.q_heads / p.kv_heads * p.q_len >= kInt4PrefillColumns;
+}
+
+int check_page_pool(const ts_page_pool* p) {
+  if (!p || !p->data || p->layers <= 0 || p->pages <= 0 || p->page_bytes <= 0) return TS_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(p->data) % 16 || p->page_bytes % 16 || p->page_stride % 16 ||
+      p->layer_stride % 16 || p->page_stride < p->page_bytes)
+    return TS_ERR_INVALID_ARGUMENT;
+  return TS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ts_kv4_block_bytes(int32_t head_dim, int32_t page_size) {
+  return int4_shape_ok(head_dim, page_size) ? (size_t)tsa::int4_block_bytes(head_dim, page_size) : 0;
+}
+
+int ts_kv_append_int4(ts_view4 key, ts_view4 value, int32_t dtype, int32_t steps, const ts_kv4_cache* cache,
+                      int64_t position, const int32_t* positions, int32_t* positions_out, void* stream) {
+  const int st = check_int4_cache(cache);
+  if (st != TS_OK) return st;
+  if (!int4_dtype_ok(dtype)) return TS_ERR_UNSUPPORTED;
+  if (!key.data || !value.data) return TS_ERR_INVALID_ARGUMENT;
+  if (steps <= 0) return TS_ERR_CAPACITY;
+  if (!positions && (position < 0 || position + steps > (int64_t)cache->slots * cache->page_size))
+    return TS_ERR_CAPACITY;
+  return from_cuda(tsa::kv_append_int4(key, value, dtype, steps, *cache, position, positions, positions_out,
+                                       fault_ptr(), as_stream(stream)));
+}
+
+int ts_kv_gather_int4(const ts_kv4_cache* cache, const int32_t* starts, const int32_t* lens, ts_view4 key,
+                      ts_view4 value, int32_t dtype, int32_t length, void* stream) {
+  const int st = check_int4_cache(cache);
+  if (st != TS_OK) return st;
+  if (!int4_dtype_ok(dtype)) return TS_ERR_UNSUPPORTED;
+  if (!key.data || !value.data || length < 0) return TS_ERR_INVALID_ARGUMENT;
+  if (!starts && length > (int64_t)cache->slots * cache->page_size) return TS_ERR_INVALID_ARGUMENT;
+  return from_cuda(tsa::kv_gather_int4(*cache, starts, lens, key, value, dtype, length, fault_ptr(),
+                                       as_stream(stream)));
+}
+
+int ts_attn_int4_path(const ts_attn_params* p, const ts_kv4_cache* cache) {
+  const int st = check_int4_attn(p, cache);
+  if (st != TS_OK) return st;
+  return int4_prefill(*p) ? TS_PATH_TCGEN05 : TS_PATH_DECODE;
+}
+
+size_t ts_attn_int4_workspace_size(const ts_attn_params* p, const ts_kv4_cache* cache) {
+  if (check_int4_attn(p, cache) != TS_OK) return 0;
+  return int4_prefill(*p) ? 2 * int4_prefill_half(*p) : tsa::attn_int4_workspace(*p, *cache);
+}
+
+int ts_attn_int4(const ts_attn_params* p, const ts_kv4_cache* cache, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  const int st = check_int4_attn(p, cache);
+  if (st != TS_OK) return st;
+  const bool prefill = int4_prefill(*p);
+  const size_t need = prefill ? 2 * int4_prefill_half(*p) : tsa::attn_int4_workspace(*p, *cache);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return TS_ERR_WORKSPACE;
+  if (!prefill)
+    return from_cuda(tsa::attn_int4_forward(*p, *cache, workspace, workspace_bytes, fault_ptr(), as_stream(stream)));
+  const ts_attn_params d = int4_prefill_params(*p, workspace);
+  const cudaError_t e = tsa::kv_gather_int4(*cache, nullptr, p->kv_lens, d.k, d.v, p->dtype, p->kv_len, fault_ptr(),
+                                            as_stream(stream));
+  if (e != cudaSuccess) return from_cuda(e);
+  return from_cuda(tsa::tc_forward(d, fault_ptr(), as_stream(stream)));
+}
+
+int ts_kv_pages_copy(const ts_page_pool* src, const ts_page_pool* dst, const int32_t* from, const int32_t* to,
+                     int32_t count, void* stream) {
+  if (check_page_pool(src) != TS_OK || check_page_pool(dst) != TS_OK) return TS_ERR_INVALID_ARGUMENT;
+  if (src->page_bytes != dst->page_bytes || src->layers != dst->layers || count < 0 || (count && (!from || !to)))
+    return TS_ERR_INVALID_ARGUMENT;
+  return from_cuda(tsa::kv_pages_copy(*src, *dst, from, to, count, as_stream(stream)));
+}
+
+int ts_kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lens, int32_t rows,
+                     const int32_t* index, int32_t* table_out, int64_t table_out_stride, int32_t* lens_out,
+                     int32_t rows_out, int32_t slots, int32_t page_size, int32_t* refs, int32_t pages,
+                     int32_t* counters, void* stream) {
+  if (!table || !lens || !index || !table_out || !lens_out || !refs || !counters || table == table_out ||
+      lens == lens_out)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (rows <= 0 || rows_out <= 0 || slots <= 0 || page_size <= 0 || pages <= 0) return TS_ERR_INVALID_ARGUMENT;
+  return from_cuda(tsa::kv_pages_fork(table, table_stride, lens, rows, index, table_out, table_out_stride, lens_out,
+                                      rows_out, slots, page_size, refs, pages, counters, as_stream(stream)));
+}
+
+size_t ts_kv_pages_reserve_workspace_size(int32_t pages, int32_t rows) {
+  return pages > 0 && rows > 0 ? tsa::kv_pages_reserve_workspace(pages, rows) : 0;
+}
+
+int ts_kv_pages_reserve(const ts_page_pool* pool, int32_t* table, int64_t table_stride, const int32_t* lens,
+                        int32_t rows, int32_t slots, int32_t page_size, int32_t steps, const int32_t* row_steps,
+                        int32_t* refs, int32_t* counters, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_page_pool(pool);
+  if (st != TS_OK) return st;
+  if (!table || !lens || !refs || !counters || rows <= 0 || slots <= 0 || page_size <= 0 || steps < 0)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < tsa::kv_pages_reserve_workspace(pool->pages, rows)) return TS_ERR_WORKSPACE;
+  return from_cuda(tsa::kv_pages_reserve(*pool, table, table_stride, lens, rows, slots, page_size, steps, row_steps,
+                                         refs, counters, workspace, as_stream(stream)));
+}
+
+size_t ts_kv_pages_compact_workspace_size(int32_t pages) {
+  return pages > 0 ? tsa::kv_pages_compact_workspace(pages) : 0;
+}
+
+int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* table, int64_t table_stride, int32_t* table_out,
+                        int64_t table_out_stride, int32_t rows, int32_t slots, const int32_t* refs,
+                        int32_t* refs_out, int32_t* counters, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const int st = check_page_pool(pool);
+  if (st != TS_OK) return st;
+  if (!table || !table_out || !refs || !refs_out || !counters || rows <= 0 || slots <= 0)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < tsa::kv_pages_compact_workspace(pool->pages)) return TS_ERR_WORKSPACE;
+  return from_cuda(tsa::kv_pages_compact(*pool, table, table_out, rows, slots, table_stride, table_out_stride, refs,
+                                         refs_out, counters, workspace, as_stream(stream)));
+}
+
 int ts_attn_device_status(void* stream, uint32_t* info) {
   uint32_t* f = fault_ptr();
   if (!f) return TS_ERR_LAUNCH;
@@ -333,7 +524,7 @@ int ts_attn_device_status(void* stream, uint32_t* info) {
     if (cudaMemcpyAsync(f, &zero, sizeof(uint32_t), cudaMemcpyHostToDevice, s) != cudaSuccess ||
         cudaStreamSynchronize(s) != cudaSuccess)
       return TS_ERR_LAUNCH;
-    return TS_ERR_DEVICE_TIMEOUT;
+    return host == tsa::FAULT_PAGE ? TS_ERR_PAGE : TS_ERR_DEVICE_TIMEOUT;
   }
   return TS_OK;
 }

@@ -63,6 +63,7 @@ enum FaultSite : uint32_t {
   FAULT_FWD_DRAIN = 0x107,
   FAULT_DEC_FULL = 0x201,
   FAULT_DEC_EMPTY = 0x202,
+  FAULT_PAGE = 0x301,  // a page table entry outside its pool
 };
 
 __device__ __forceinline__ void record_fault(uint32_t* fault, uint32_t site) {

@@ -49,6 +49,7 @@ ERR_WORKSPACE = -3
 ERR_LAUNCH = -4
 ERR_DEVICE_TIMEOUT = -5
 ERR_CAPACITY = -6
+ERR_PAGE = -7
 
 # Fixed device scratch of ts_attn_decode_noalloc (TS_ATTN_NOALLOC_SCRATCH_BYTES).
 NOALLOC_SCRATCH_BYTES = 8 << 20
@@ -112,6 +113,32 @@ class KvAppendParams(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("slots", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("layer_stride", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        ("page_bytes", ctypes.c_int64),
+        ("layers", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/ts_attn.h declares, with its ctypes signature.
 SIGNATURES = {
     "ts_attn_abi_version": (ctypes.c_int, []),
@@ -168,6 +195,48 @@ SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(AttnParams), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
          ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ts_kv4_block_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "ts_kv_append_int4": (
+        ctypes.c_int,
+        [View4, View4, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(Kv4Cache), ctypes.c_int64, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "ts_kv_gather_int4": (
+        ctypes.c_int,
+        [ctypes.POINTER(Kv4Cache), ctypes.c_void_p, ctypes.c_void_p, View4, View4, ctypes.c_int32, ctypes.c_int32,
+         ctypes.c_void_p],
+    ),
+    "ts_attn_int4_path": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache)]),
+    "ts_attn_int4_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache)]),
+    "ts_attn_int4": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ts_kv_pages_copy": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagePool), ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+         ctypes.c_void_p],
+    ),
+    "ts_kv_pages_fork": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+         ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "ts_kv_pages_reserve_workspace_size": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "ts_kv_pages_reserve": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+         ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ts_kv_pages_compact_workspace_size": (ctypes.c_size_t, [ctypes.c_int32]),
+    "ts_kv_pages_compact": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+         ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+         ctypes.c_void_p],
     ),
     "ts_attn_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "ts_attn_source_digest": (ctypes.c_char_p, []),

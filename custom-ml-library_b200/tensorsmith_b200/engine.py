@@ -417,6 +417,293 @@ def decode_int8(q, k8, v8, key_scales, value_scales, *, is_causal=True, scale=No
     return out, (lse if need_lse else None)
 
 
+# -- the paged 4-bit cache ----------------------------------------------------
+
+
+def int4_block_bytes(head_dim: int, page_size: int) -> int:
+    """Bytes of one page and KV head, keys and values: 4.5 bits a value (ts_kv4_block_bytes)."""
+    size = int(_lib.lib().ts_kv4_block_bytes(int(head_dim), int(page_size)))
+    if not size:
+        raise ValueError("a 4-bit cache takes head dimensions that are multiples of 32 up to 256 and pages of "
+                         "16, 32 or 64 tokens")
+    return size
+
+
+def int4_pool(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64, layers: int | None = None,
+              device="cuda") -> torch.Tensor:
+    """An empty pool: uint8 [num_pages, kv_heads, block], or [layers, num_pages, kv_heads, block]."""
+    shape = (num_pages, kv_heads, int4_block_bytes(head_dim, page_size))
+    if min(num_pages, kv_heads) <= 0 or (layers is not None and layers <= 0):
+        raise ValueError("a pool needs at least one page, head and layer")
+    return torch.empty(shape if layers is None else (layers,) + shape, dtype=torch.uint8, device=device)
+
+
+def _int32_vector(t, name: str, size: int, device) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] != size or t.device != device:
+        raise ValueError(f"{name} must be a contiguous int32 vector of {size} on the pool's device")
+    return t
+
+
+def _page_table(t, device) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.device != device or min(t.shape) <= 0:
+        raise ValueError("a page table must be int32 [rows, slots] with contiguous rows on the pool's device")
+    return t
+
+
+def _int4_cache(pool, page_table, page_size: int, head_dim: int) -> _lib.Kv4Cache:
+    _require_cuda(pool)
+    if pool.dtype != torch.uint8 or pool.dim() != 3:
+        raise TypeError("a 4-bit pool must be uint8 [pages, kv heads, block]")
+    pages, heads, block = pool.shape
+    if block != int4_block_bytes(head_dim, page_size) or pool.stride(2) != 1 or pool.stride(1) != block:
+        raise ValueError("the pool's blocks do not match the head dimension and page size")
+    _page_table(page_table, pool.device)
+    rows, slots = page_table.shape
+    return _lib.Kv4Cache(pool.data_ptr(), pool.stride(0), page_table.data_ptr(), page_table.stride(0), rows, slots,
+                         pages, heads, head_dim, page_size)
+
+
+def _int4_rows(t, cache, what: str) -> None:
+    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[1] != cache.kv_heads or t.shape[3] != cache.head_dim:
+        raise ValueError(f"{what} must be [rows, kv heads, tokens, head dimension] of the cache")
+
+
+def kv_append_int4(key, value, pool, page_table, *, page_size, position=0, positions=None, positions_out=None):
+    """Quantise a [B, Hkv, steps, D] chunk into the pages of its rows, at token ``position`` (or per-row
+    ``positions``).  The table must hold a page for every token written (``kv_pages_reserve``)."""
+    _require_cuda(key, value)
+    cache = _int4_cache(pool, page_table, page_size, key.shape[-1])
+    _int4_rows(key, cache, "key")
+    if value.shape != key.shape:
+        raise ValueError("key and value must have the same shape")
+    if value.dtype != key.dtype:
+        raise TypeError("key/value must share a dtype")
+    for name, t in (("positions", positions), ("positions_out", positions_out)):
+        if t is not None:
+            _int32_vector(t, name, cache.batch, pool.device)
+    _lib.check(
+        _lib.lib().ts_kv_append_int4(view4(key), view4(value), dtype_code(key.dtype), key.shape[2],
+                                     ctypes.byref(cache), int(position),
+                                     positions.data_ptr() if positions is not None else None,
+                                     positions_out.data_ptr() if positions_out is not None else None,
+                                     _stream_handle(pool.device)),
+        "ts_kv_append_int4")
+
+
+def kv_gather_int4(pool, page_table, length, *, page_size, dtype, starts=None, kv_lens=None):
+    """The cached values of ``length`` tokens of every row, from token ``starts[b]`` (default 0): dequantised
+    ``(keys, values)`` [B, Hkv, length, D] of ``dtype``; tokens at or past ``kv_lens[b]`` (optional) are zero."""
+    _require_cuda(pool)
+    if pool.dtype != torch.uint8 or pool.dim() != 3:
+        raise TypeError("a 4-bit pool must be uint8 [pages, kv heads, block]")
+    head_dim = pool.shape[2] * 8 // (9 * page_size) if page_size > 0 else 0
+    cache = _int4_cache(pool, page_table, page_size, head_dim)
+    code, length = dtype_code(dtype), int(length)
+    if length < 0:
+        raise ValueError("length must not be negative")
+    for name, t in (("starts", starts), ("kv_lens", kv_lens)):
+        if t is not None:
+            _int32_vector(t, name, cache.batch, pool.device)
+    both = torch.empty((2, cache.batch, cache.kv_heads, length, head_dim), dtype=dtype, device=pool.device)
+    key, value = both[0], both[1]
+    if length:
+        _lib.check(
+            _lib.lib().ts_kv_gather_int4(ctypes.byref(cache), starts.data_ptr() if starts is not None else None,
+                                         kv_lens.data_ptr() if kv_lens is not None else None, view4(key), view4(value),
+                                         code, length, _stream_handle(pool.device)),
+            "ts_kv_gather_int4")
+    return key, value
+
+
+def _int4_attn_params(q, out, lse, cache, kv_lens, max_len, is_causal, scale) -> _lib.AttnParams:
+    p = _lib.AttnParams()
+    p.q, p.o = view4(q), view4(out)
+    if lse is not None:
+        p.lse = lse.data_ptr()
+        p.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
+    p.dtype = dtype_code(q.dtype)
+    p.batch, p.q_heads, p.kv_heads = q.shape[0], q.shape[1], cache.kv_heads
+    p.q_len, p.kv_len, p.head_dim, p.value_dim = q.shape[2], max_len, cache.head_dim, cache.head_dim
+    p.scale = default_scale(cache.head_dim) if scale is None else float(scale)
+    p.is_causal = 1 if is_causal else 0
+    p.kv_lens = kv_lens.data_ptr()
+    return p
+
+
+def _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len):
+    _require_cuda(q, pool, page_table, kv_lens)
+    if q.dim() != 4:
+        raise ValueError("expected a [batch, heads, sequence, channels] view")
+    cache = _int4_cache(pool, page_table, page_size, q.shape[3])
+    if q.device != pool.device or q.shape[0] != cache.batch or q.shape[1] % cache.kv_heads or 0 in q.shape:
+        raise ValueError("query rows and heads must match the cache, on its device")
+    _int32_vector(kv_lens, "kv_lens", cache.batch, pool.device)
+    whole = cache.slots * page_size
+    max_len = whole if max_len is None else int(max_len)
+    if not 0 <= max_len <= whole:
+        raise ValueError("max_len must be between zero and the tokens the page table can hold")
+    return cache, max(1, max_len)
+
+
+def attention_int4_path(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_causal=True, scale=None) -> str:
+    """Name of the kernel family ``attention_int4`` selects: "decode" (straight over the pages) or "tcgen05"."""
+    cache, max_len = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len)
+    p = _int4_attn_params(q, q, None, cache, kv_lens, max_len, is_causal, scale)
+    code = _lib.lib().ts_attn_int4_path(ctypes.byref(p), ctypes.byref(cache))
+    if code < 0:
+        _lib.check(code, "ts_attn_int4_path")
+    return _lib.PATH_NAMES[code]
+
+
+def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_causal=True, scale=None,
+                   need_lse=False, out=None, lse=None, workspace=None):
+    """Attention of ``q`` [B, Hq, Tq, D] over a paged 4-bit cache: ``(out, lse or None)``.
+
+    Row b sees its first ``kv_lens[b]`` tokens; with ``is_causal`` its Tq queries are the last of them
+    (a row without a visible key gives zeros and an LSE of -inf).  ``max_len`` bounds ``kv_lens`` (default: what
+    the table can hold); the work is split for it, so pass the real bound where it is known."""
+    cache, max_len = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len)
+    dtype_code(q.dtype)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have the query's shape, dtype and device")
+    if need_lse:
+        if lse is None:
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
+            raise ValueError("lse must be fp32 [B, Hq, Tq] on the query's device")
+    p = _int4_attn_params(q, out, lse if need_lse else None, cache, kv_lens, max_len, is_causal, scale)
+    handle = _lib.lib()
+    need = int(handle.ts_attn_int4_workspace_size(ctypes.byref(p), ctypes.byref(cache)))
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _lib.check(handle.ts_attn_int4(ctypes.byref(p), ctypes.byref(cache), workspace.data_ptr() if need else None, need,
+                                   _stream_handle(q.device)), "ts_attn_int4")
+    return out, (lse if need_lse else None)
+
+
+# -- pages ---------------------------------------------------------------------
+
+
+PAGES_SHORT, PAGES_BAD_INDEX, PAGES_NO_SLOT = 1, 2, 4  # error bits of counters[2]
+
+
+def kv_pages_state(num_pages: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """``(refs, counters)`` of a pool without live pages: references to each page, and int32
+    {free pages, a page below which none is free, error bits, unused}."""
+    refs = torch.zeros(num_pages, dtype=torch.int32, device=device)
+    return refs, torch.tensor([num_pages, 0, 0, 0], dtype=torch.int32, device=device)
+
+
+def _page_pool(pool) -> _lib.PagePool:
+    """A pool [pages, ...] or [layers, pages, kv heads, block] as opaque pages."""
+    _require_cuda(pool)
+    if pool.dim() == 3:
+        pool = pool[None]
+    if pool.dim() != 4 or not pool[0, 0].is_contiguous():
+        raise ValueError("a page pool must be [layers, pages, kv heads, block] with contiguous pages")
+    size = pool.element_size()
+    return _lib.PagePool(pool.data_ptr(), pool.stride(0) * size, pool.stride(1) * size,
+                         pool.shape[2] * pool.shape[3] * size, pool.shape[0], pool.shape[1])
+
+
+def _page_counts(refs, counters, pages: int, device) -> None:
+    _int32_vector(refs, "refs", pages, device)
+    _int32_vector(counters, "counters", 4, device)
+
+
+def kv_pages_copy(src_pool, src, dst_pool, dst):
+    """Copy page ``src[i]`` of one pool to page ``dst[i]`` of another (or the same), in every layer; pairs with a
+    negative or out-of-range entry are skipped.  No page may be both read and written."""
+    a, b = _page_pool(src_pool), _page_pool(dst_pool)
+    _int32_vector(src, "src", src.shape[0], src_pool.device)
+    _int32_vector(dst, "dst", src.shape[0], src_pool.device)
+    if src_pool.device != dst_pool.device or a.page_bytes != b.page_bytes or a.layers != b.layers:
+        raise ValueError("pools must have the same layers and page size, on one device")
+    _lib.check(_lib.lib().ts_kv_pages_copy(ctypes.byref(a), ctypes.byref(b), src.data_ptr(), dst.data_ptr(),
+                                           src.shape[0], _stream_handle(src_pool.device)), "ts_kv_pages_copy")
+
+
+def kv_pages_fork(page_table, lens, index, refs, counters, *, page_size, table_out=None, lens_out=None):
+    """Rows that share the pages of the rows ``index`` names: fork, beam reorder, and free (an entry of -1 leaves
+    its row empty).  Returns ``(table, lens)`` with ``len(index)`` rows; ``refs`` and ``counters`` are updated."""
+    _require_cuda(page_table)
+    device = page_table.device
+    _page_table(page_table, device)
+    rows, slots = page_table.shape
+    _int32_vector(lens, "lens", rows, device)
+    _int32_vector(index, "index", index.shape[0], device)
+    _page_counts(refs, counters, refs.shape[0], device)
+    n = index.shape[0]
+    if n == 0 or page_size <= 0:
+        raise ValueError("fork needs at least one row and a positive page size")
+    table_out = torch.empty((n, slots), dtype=torch.int32, device=device) if table_out is None else table_out
+    lens_out = torch.empty(n, dtype=torch.int32, device=device) if lens_out is None else lens_out
+    if _page_table(table_out, device).shape != (n, slots):
+        raise ValueError("table_out must be [len(index), slots]")
+    _int32_vector(lens_out, "lens_out", n, device)
+    _lib.check(
+        _lib.lib().ts_kv_pages_fork(page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), rows,
+                                    index.data_ptr(), table_out.data_ptr(), table_out.stride(0), lens_out.data_ptr(),
+                                    n, slots, page_size, refs.data_ptr(), refs.shape[0], counters.data_ptr(),
+                                    _stream_handle(device)),
+        "ts_kv_pages_fork")
+    return table_out, lens_out
+
+
+def kv_pages_reserve(pool, page_table, lens, steps, refs, counters, *, page_size, workspace=None):
+    """Give every row pages of its own for the next ``steps`` tokens (an int, or int32 per row on the device):
+    free pages for empty slots, a copy of a partly filled page that other rows hold too.  Works in place; when the
+    pool or the table is too small it sets an error bit of ``counters[2]`` and changes nothing."""
+    p = _page_pool(pool)
+    device = pool.device
+    _page_table(page_table, device)
+    rows, slots = page_table.shape
+    _int32_vector(lens, "lens", rows, device)
+    _page_counts(refs, counters, p.pages, device)
+    row_steps = None
+    if isinstance(steps, torch.Tensor):
+        row_steps, steps = _int32_vector(steps, "steps", rows, device), 0
+    if steps < 0 or page_size <= 0:
+        raise ValueError("steps must not be negative and the page size must be positive")
+    handle = _lib.lib()
+    need = int(handle.ts_kv_pages_reserve_workspace_size(p.pages, rows))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.check(
+        handle.ts_kv_pages_reserve(ctypes.byref(p), page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), rows,
+                                   slots, page_size, steps, row_steps.data_ptr() if row_steps is not None else None,
+                                   refs.data_ptr(), counters.data_ptr(), workspace.data_ptr(), need,
+                                   _stream_handle(device)),
+        "ts_kv_pages_reserve")
+
+
+def kv_pages_compact(pool, page_table, refs, counters, *, table_out=None, refs_out=None, workspace=None):
+    """Move the live pages to the start of the pool (the highest page into the lowest hole, and so on) and rewrite
+    the tables and counts, in place unless ``table_out`` / ``refs_out`` are given.  Returns ``(table, refs)``."""
+    p = _page_pool(pool)
+    device = pool.device
+    _page_table(page_table, device)
+    _page_counts(refs, counters, p.pages, device)
+    rows, slots = page_table.shape
+    table_out = page_table if table_out is None else table_out
+    refs_out = refs if refs_out is None else refs_out
+    if _page_table(table_out, device).shape != (rows, slots):
+        raise ValueError("table_out must have the table's shape")
+    _int32_vector(refs_out, "refs_out", p.pages, device)
+    handle = _lib.lib()
+    need = int(handle.ts_kv_pages_compact_workspace_size(p.pages))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.check(
+        handle.ts_kv_pages_compact(ctypes.byref(p), page_table.data_ptr(), page_table.stride(0), table_out.data_ptr(),
+                                   table_out.stride(0), rows, slots, refs.data_ptr(), refs_out.data_ptr(),
+                                   counters.data_ptr(), workspace.data_ptr(), need, _stream_handle(device)),
+        "ts_kv_pages_compact")
+    return table_out, refs_out
+
+
 _INV_FREQ: dict = {}
 
 

@@ -51,7 +51,8 @@ typedef enum ts_status {
   TS_ERR_WORKSPACE = -3,        /* workspace missing or smaller than required */
   TS_ERR_LAUNCH = -4,           /* kernel launch or driver call failed */
   TS_ERR_DEVICE_TIMEOUT = -5,   /* a bounded wait inside a kernel gave up */
-  TS_ERR_CAPACITY = -6          /* KV-cache append would exceed the capacity */
+  TS_ERR_CAPACITY = -6,         /* KV-cache append would exceed the capacity */
+  TS_ERR_PAGE = -7              /* a kernel met a page table entry outside the pool */
 } ts_status;
 
 /* Which kernel family ts_attn_fwd would run (for tests and diagnostics). */
@@ -274,9 +275,124 @@ TS_ATTN_API int ts_attn_decode_int8(const ts_attn_params* params, const float* k
                                     const float* value_scales, int64_t scale_capacity, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* ---- A paged KV cache held in 4 bits (no counterpart in tensorsmith, whose
+ * smallest cache is int8, nn/cache.py:47-52) ----
+ *
+ * A page holds page_size tokens of every KV head, keys and values.  The block of
+ * one page and head is contiguous:
+ *   K nibbles [page_size, D/2] | K scales fp16 [page_size, D/32] | V nibbles | V scales
+ * A row's D/8 words are ordered so that word t * (D/32) + g holds the channels
+ * 32 g + 8 t + e in nibble e (bits 4e..4e+3).  One scale serves 32 channels of a
+ * token: scale = max|x| / 7 rounded up to 5 significant bits, held in
+ * [2^-20, 9216]; n = round_half_even(x / scale) in [-7, 7] is stored as n + 8.
+ * n * scale is exact in bf16 and fp16.  Inputs beyond +-64512 saturate, NaN is
+ * stored as 0.  4.5 bits a value. */
+typedef struct ts_kv4_cache {
+  void* pool;           /* uint8 [pages, kv_heads, block], 16-byte aligned */
+  int64_t page_stride;  /* bytes between pages: at least kv_heads * block, a multiple of 16 */
+  const int32_t* table; /* [batch, slots] (device): the page of each page_size tokens of a row, -1 none */
+  int64_t table_stride; /* entries between rows */
+  int32_t batch, slots, pages, kv_heads;
+  int32_t head_dim;  /* a multiple of 32, at most 256 */
+  int32_t page_size; /* 16, 32 or 64 */
+} ts_kv4_cache;
+
+/* Bytes of the block of one page and KV head, 0 for a head_dim or page_size the
+ * cache does not take. */
+TS_ATTN_API size_t ts_kv4_block_bytes(int32_t head_dim, int32_t page_size);
+
+/* Quantising append: tokens [pos_b, pos_b + steps) of every row receive the rows
+ * of key / value [batch, kv_heads, steps, D] (dtype F32, F16 or BF16), with
+ * pos_b = positions[b], or position for every row when positions is NULL.
+ * positions_out (optional, [batch]) receives pos_b + steps.  The table must
+ * already hold a page for every token written (ts_kv_pages_reserve); a token
+ * without one is not written and sets the fault word (TS_ERR_PAGE). */
+TS_ATTN_API int ts_kv_append_int4(ts_view4 key, ts_view4 value, int32_t dtype, int32_t steps,
+                                  const ts_kv4_cache* cache, int64_t position, const int32_t* positions,
+                                  int32_t* positions_out, void* stream);
+
+/* The values of `length` tokens of every row, from token starts[b] (0 when
+ * starts is NULL), into key / value [batch, kv_heads, length, D].  Tokens at or
+ * past lens[b] (optional) are written as zeros. */
+TS_ATTN_API int ts_kv_gather_int4(const ts_kv4_cache* cache, const int32_t* starts, const int32_t* lens,
+                                  ts_view4 key, ts_view4 value, int32_t dtype, int32_t length, void* stream);
+
+/* Kernel family ts_attn_int4 would run: TS_PATH_DECODE (straight over the pages)
+ * or TS_PATH_TCGEN05 (pages dequantised into the workspace, then the prefill
+ * kernel), or a negative ts_status.  The environment variable TS_INT4_KERNEL =
+ * "pages" or "prefill", read at every call, forces one where it supports the
+ * problem, for tests and measurements. */
+TS_ATTN_API int ts_attn_int4_path(const ts_attn_params* params, const ts_kv4_cache* cache);
+
+/* Workspace bytes ts_attn_int4 needs. */
+TS_ATTN_API size_t ts_attn_int4_workspace_size(const ts_attn_params* params, const ts_kv4_cache* cache);
+
+/* Attention of q [batch, Hq, Tq, D] over the cache: params as for ts_attn_decode,
+ * with k and v ignored, kv_lens required and kv_len an upper bound of them that
+ * the table can hold (kv_len <= slots * page_size); no explicit mask, no fp64.
+ * Any number of query tokens: one token a row, a few drafted ones, or a chunk of
+ * a prompt whose tokens are already in the cache. */
+TS_ATTN_API int ts_attn_int4(const ts_attn_params* params, const ts_kv4_cache* cache, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* ---- Pages of a paged cache (any storage: a page is opaque bytes) ----
+ * refs[p] counts the table entries that hold page p (and pins a caller adds); a
+ * page with refs 0 is free.  counters is int32 [4] on the device: {free pages, a
+ * page number below which none is free (0 is always right), error bits, unused};
+ * error bits, set and never cleared by the engine: 1 not enough free pages, 2 an
+ * index or page out of range was skipped, 4 a row would need more slots than the
+ * table has.  A reserve that sets 1 or 4 changes nothing. */
+typedef struct ts_page_pool {
+  void* data;                        /* 16-byte aligned */
+  int64_t layer_stride, page_stride; /* bytes, multiples of 16 */
+  int64_t page_bytes;                /* contiguous bytes of a page, a multiple of 16 */
+  int32_t layers, pages;             /* a page number means the same page of every layer */
+} ts_page_pool;
+
+/* Page from[i] of src is copied to page to[i] of dst, in every layer; a pair with
+ * a negative or out-of-range entry is skipped.  No page may be both read and
+ * written, and none written twice. */
+TS_ATTN_API int ts_kv_pages_copy(const ts_page_pool* src, const ts_page_pool* dst, const int32_t* from,
+                                 const int32_t* to, int32_t count, void* stream);
+
+/* Row r of the new table shares the pages that hold the lens[index[r]] tokens of
+ * old row index[r] (fork, beam reorder); index[r] < 0 leaves the row empty (free).
+ * Pages that no row holds any longer become free, pages reserved past a row's
+ * tokens too.  refs and counters are updated in place; table_out and lens_out
+ * must not alias table and lens. */
+TS_ATTN_API int ts_kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lens, int32_t rows,
+                                 const int32_t* index, int32_t* table_out, int64_t table_out_stride,
+                                 int32_t* lens_out, int32_t rows_out, int32_t slots, int32_t page_size,
+                                 int32_t* refs, int32_t pages, int32_t* counters, void* stream);
+
+/* Workspace bytes ts_kv_pages_reserve needs. */
+TS_ATTN_API size_t ts_kv_pages_reserve_workspace_size(int32_t pages, int32_t rows);
+
+/* Gives every row pages of its own for the tokens [lens[r], lens[r] + steps)
+ * (row_steps[r] in place of steps when given): empty slots get free pages, and a
+ * partly filled page that others hold too is replaced by a copy (in every layer of
+ * the pool); of its holders that write, the last keeps it if no other row has it.
+ * Pages are handed out lowest first, in the order of (row, slot).  lens stays. */
+TS_ATTN_API int ts_kv_pages_reserve(const ts_page_pool* pool, int32_t* table, int64_t table_stride,
+                                    const int32_t* lens, int32_t rows, int32_t slots, int32_t page_size,
+                                    int32_t steps, const int32_t* row_steps, int32_t* refs, int32_t* counters,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes ts_kv_pages_compact needs. */
+TS_ATTN_API size_t ts_kv_pages_compact_workspace_size(int32_t pages);
+
+/* Moves the pool's n live pages into its first n: the highest page into the lowest
+ * hole, and so on.  table_out / refs_out receive the tables and counts (they may
+ * be table / refs themselves). */
+TS_ATTN_API int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* table, int64_t table_stride,
+                                    int32_t* table_out, int64_t table_out_stride, int32_t rows, int32_t slots,
+                                    const int32_t* refs, int32_t* refs_out, int32_t* counters, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* Reads and clears the device fault word written by kernels whose bounded
- * waits gave up.  Synchronises `stream`.  Returns TS_OK or
- * TS_ERR_DEVICE_TIMEOUT; *info (optional) receives the recorded site code. */
+ * waits gave up, or that met a page outside the pool.  Synchronises `stream`.
+ * Returns TS_OK, TS_ERR_DEVICE_TIMEOUT or TS_ERR_PAGE; *info (optional) receives
+ * the recorded site code. */
 TS_ATTN_API int ts_attn_device_status(void* stream, uint32_t* info);
 
 #ifdef __cplusplus

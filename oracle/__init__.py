@@ -17,3 +17,12 @@ from .attention import (  # noqa: F401
     quantize_int8,
     rope,
 )
+from .int4 import (  # noqa: F401
+    PagesOracle,
+    attention_int4,
+    dequantize_int4,
+    int4_scale,
+    pack_block,
+    quantize_int4,
+    unpack_block,
+)
