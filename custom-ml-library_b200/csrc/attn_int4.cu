@@ -1,63 +1,101 @@
-// Host side of the attention over a 4-bit cache: what the kernels take, how the keys are split.
+// Host side of the attention over a 4-bit cache: what the kernels take, how the work is shared.
 #include "attn_int4.cuh"
 
 namespace tsa {
+
+namespace {
+constexpr int kMaxRows = 2048;  // rows of one launch: their prefix sums sit in shared memory
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      n <= 0)
+    n = 148;
+  return n;
+}
+
+bool rows_vec(const ts_view4& v, int size) {
+  return v.stride[3] == 1 && reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && v.stride[0] * size % 16 == 0 &&
+         v.stride[1] * size % 16 == 0 && v.stride[2] * size % 16 == 0;
+}
+
+// Fills what follows from the problem; returns the grid's blocks.
+int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
+  shape = int4_shape(p);
+  a.group = p.q_heads / p.kv_heads;
+  a.cols = a.group * p.q_len;
+  a.col_blocks = ceil_div(a.cols, shape.nt * 8);
+  a.slot_cols = a.cols < shape.nt * 8 ? a.cols : shape.nt * 8;
+  // One wave of blocks that fill the GPU, fewer where a warp would be left without a stage.
+  const int rows = p.batch < kMaxRows ? p.batch : kMaxRows;
+  const int64_t most = (int64_t)rows * p.kv_heads * a.col_blocks * ceil_div(p.kv_len, shape.keys);
+  const int blocks = (int)i64min(most, (int64_t)sm_count() * shape.blocks);
+  a.warps = blocks * shape.warps;
+  return blocks;
+}
+
+size_t partial_bytes(const Int4Attn& a, int head_dim) {
+  return (size_t)2 * a.warps * a.slot_cols * (head_dim + 2) * sizeof(float);
+}
+}  // namespace
 
 bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c) {
   if (p.dtype != TS_BF16 && p.dtype != TS_F16 && p.dtype != TS_F32) return false;
   return c.page_size == 16 || c.page_size == 32 || c.page_size == 64;
 }
 
-static int int4_tiles(const ts_attn_params& p) {
-  const int cols = p.q_heads / p.kv_heads * p.q_len;
-  return cols > 8 && p.dtype != TS_F32 && p.head_dim <= 128 ? 2 : 1;
-}
-
-// Keys of one split: enough blocks for two rounds of three a SM, and at least one stage for every
-// warp of a block.
-static int int4_split_keys(const ts_attn_params& p, int col_blocks) {
-  const int64_t work = (int64_t)p.batch * p.kv_heads * col_blocks * p.kv_len;
-  const int64_t target = 148 * 3 * 2;
-  const int64_t s = (work + target - 1) / target;
-  return (int)i64max(256, i64min((s + 255) / 256 * 256, 1 << 20));
-}
-
-static void int4_plan(const ts_attn_params& p, Int4Attn& a, int& nt) {
-  nt = int4_tiles(p);
-  a.group = p.q_heads / p.kv_heads;
-  a.cols = a.group * p.q_len;
-  a.col_blocks = ceil_div(a.cols, nt * 8);
-  a.split_keys = int4_split_keys(p, a.col_blocks);
-  a.max_splits = max(1, ceil_div(p.kv_len, a.split_keys));
+// Two column tiles share one pass over the nibbles where there are more than 8 columns (half types up to
+// D = 128; a second tile of wider rows or of fp32's two query parts does not fit the registers).
+Int4Shape int4_shape(const ts_attn_params& p) {
+  const int64_t cols = (int64_t)(p.q_heads / p.kv_heads) * p.q_len;
+  if (p.head_dim > 128) return {1, 32, 4, 2};
+  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2};
+  return {1, 64, 4, 3};
 }
 
 size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
   Int4Attn a;
-  int nt;
-  int4_plan(p, a, nt);
-  if (a.max_splits == 1) return 0;
-  return (size_t)p.batch * p.q_heads * p.q_len * a.max_splits * (p.head_dim + 2) * sizeof(float);
+  Int4Shape shape;
+  plan(p, a, shape);
+  const int rows = p.batch < kMaxRows ? p.batch : kMaxRows;
+  return partial_bytes(a, p.head_dim) + (size_t)(rows + 1) * sizeof(int32_t);
 }
 
 cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
                               uint32_t* fault, cudaStream_t st) {
   Int4Attn a;
-  int nt;
-  int4_plan(p, a, nt);
+  Int4Shape shape;
+  const int blocks = plan(p, a, shape);
+  if (ws_bytes < attn_int4_workspace(p, c)) return cudaErrorInvalidValue;
   a.p = p;
   a.c = c;
   a.page_log2 = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : 6;
   a.block_bytes = int4_block_bytes(p.head_dim, c.page_size);
   a.ws_acc = reinterpret_cast<float*>(ws);
-  a.ws_ml = a.ws_acc ? a.ws_acc + (size_t)p.batch * p.q_heads * p.q_len * a.max_splits * p.head_dim : nullptr;
+  a.ws_ml = a.ws_acc + (size_t)2 * a.warps * a.slot_cols * p.head_dim;
+  a.ws_first = reinterpret_cast<int32_t*>(a.ws_ml + (size_t)2 * a.warps * a.slot_cols * 2);
   a.fault = fault;
-  if (ws_bytes < attn_int4_workspace(p, c)) return cudaErrorInvalidValue;
-  switch (p.dtype) {
-    case TS_BF16: return attn_int4_launch<__nv_bfloat16>(a, nt, st);
-    case TS_F16: return attn_int4_launch<__half>(a, nt, st);
-    case TS_F32: return attn_int4_launch<float>(a, nt, st);
+  const int size = p.dtype == TS_F32 ? 4 : 2;
+  a.q_vec = rows_vec(p.q, size);
+  a.o_vec = rows_vec(p.o, size);
+  if ((int64_t)(p.batch < kMaxRows ? p.batch : kMaxRows) * p.q_heads * p.q_len > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  for (int row = 0; row < p.batch; row += kMaxRows) {  // launches follow one another on the stream
+    Int4Attn part = a;
+    part.p.batch = p.batch - row < kMaxRows ? p.batch - row : kMaxRows;
+    part.p.q.data = reinterpret_cast<unsigned char*>(p.q.data) + row * p.q.stride[0] * size;
+    part.p.o.data = reinterpret_cast<unsigned char*>(p.o.data) + row * p.o.stride[0] * size;
+    if (p.lse) part.p.lse = reinterpret_cast<float*>(p.lse) + row * p.lse_stride[0];
+    part.p.kv_lens = p.kv_lens + row;
+    part.c.table = c.table + row * c.table_stride;
+    cudaError_t e = cudaErrorInvalidValue;
+    switch (p.dtype) {
+      case TS_BF16: e = attn_int4_launch<__nv_bfloat16>(part, shape, blocks, st); break;
+      case TS_F16: e = attn_int4_launch<__half>(part, shape, blocks, st); break;
+      case TS_F32: e = attn_int4_launch<float>(part, shape, blocks, st); break;
+    }
+    if (e != cudaSuccess) return e;
   }
-  return cudaErrorInvalidValue;
+  return cudaSuccess;
 }
 
 }  // namespace tsa

@@ -13,12 +13,13 @@
 // (mma.sync: a fragment is built in registers straight from the nibbles, while tcgen05 would want
 // the dequantised tile written to shared memory first, four times the bytes.)  Everything is fp16 in
 // the products and fp32 in the sums and statistics:
-//   n       by the exponent trick, 0x6400 | nibble = 1024 + nibble: one logic op and one subtraction
-//           (or multiply-add) a pair; exact, and so is n * scale (8 significant bits)
-//   K scale on the fp32 sum of each 32-channel group; V scale on the fp16 operand
+//   n       by putting the nibble into the mantissa of a power of two, 0x6400 | nibble = 1024 + nibble
+//           or 0x5400 | nibble << 4 = 64 + nibble, and subtracting: a logic op and an addition a pair
+//   K scale on the fp32 sum of each 32-channel group
+//   V scale on the operand: n * scale = (64 + nibble) scale - 72 scale, exact in one multiply-add
 //   q       times a power of two that puts its largest element in [2^14, 2^15): exact for bf16 and
 //           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
-//   p       times 2^15, fp16; for fp16 and fp32 outputs hi + lo, since the 2^-12 of one fp16 part is
+//   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo, since the 2^-12 of one fp16 part is
 //           as large as the output's own rounding there
 // The rows of the K tile are permuted within 8 tokens so that the P^T fragment (one transposing
 // register move of S^T's) meets V rows whose shared-memory reads do not collide, see token_of_row.
@@ -37,33 +38,27 @@ struct Int4Attn {
   ts_kv4_cache c;
   int page_log2, block_bytes;
   int group;       // query heads of a KV head
-  int cols;        // query columns of a KV head: group * q_len
-  int col_blocks;  // grid slices of the columns
-  int split_keys, max_splits;
-  float* ws_acc;  // [rows, max_splits, D]
-  float* ws_ml;   // [rows, max_splits, 2]
+  int cols;        // query columns of a KV head: group * q_len, token-major (column = token * group + head)
+  int col_blocks;  // blocks of columns; one warp holds one at a time
+  int slot_cols;   // columns of a block that can be live
+  int warps;       // that share the work
+  bool q_vec, o_vec;  // rows of unit stride and 16-byte alignment
+  float* ws_acc;   // [2 * warps, slot_cols, D] partial results
+  float* ws_ml;    // [2 * warps, slot_cols, 2]
+  int32_t* ws_first;  // [batch + 1] first stage of each row
   uint32_t* fault;
 };
 
-// Columns of a KV head run token-major (column = token * group + head), so a block of columns
-// covers few tokens.  [0, end) are the keys that any of the block's columns sees.
-__device__ __forceinline__ void int4_range(const Int4Attn& a, int b, int col_end, int& len, int64_t& offset, int& end) {
-  len = min(a.p.kv_len, max(0, a.p.kv_lens[b]));
-  offset = (int64_t)len - a.p.q_len;
-  end = len;
-  if (a.p.is_causal) {
-    const int last = (min(col_end, a.cols) - 1) / a.group;
-    end = (int)i64max(0, i64min(len, offset + last + 1));
-  }
-}
+__device__ __forceinline__ int int4_len(const Int4Attn& a, int b) { return min(a.p.kv_len, max(0, a.p.kv_lens[b])); }
+// Stages of a warp's share: warp w takes [w * share, (w + 1) * share) of the line.
+__device__ __forceinline__ int int4_share(const Int4Attn& a, int total) { return max(1, ceil_div(total, a.warps)); }
 
 constexpr float kInt4Log2e = 1.4426950408889634f;
 constexpr float kInt4Ln2 = 0.6931471805599453f;
 
 template <typename T>
-__device__ __forceinline__ void int4_store_row(const Int4Attn& a, int b, int h, int i, int d, float value) {
-  T* o = reinterpret_cast<T*>(a.p.o.data) + b * a.p.o.stride[0] + h * a.p.o.stride[1] + i * a.p.o.stride[2];
-  o[d * a.p.o.stride[3]] = Elem<T>::from_acc(value);
+__device__ __forceinline__ T* int4_out_row(const Int4Attn& a, int b, int h, int i) {
+  return reinterpret_cast<T*>(a.p.o.data) + b * a.p.o.stride[0] + h * a.p.o.stride[1] + i * a.p.o.stride[2];
 }
 __device__ __forceinline__ void int4_store_lse(const Int4Attn& a, int b, int h, int i, float m, float l) {
   if (a.p.lse)
@@ -75,10 +70,16 @@ namespace {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = A B: a zero accumulator as an operand, where writing zeros to d first would cost four moves.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -88,18 +89,22 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 
-// (x & mask) | 1024's exponent in both halves, one three-input logic op.
-__device__ __forceinline__ uint32_t magic_or(uint32_t x, uint32_t mask) {
+// (x & mask) | magic, one three-input logic op.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(0x64006400u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(magic));
   return y;
 }
-// Nibbles 0 and 4 of a word as the pair (n, n'); nibbles 1 and 5 without shifting: 1024 + 16 n.
-__device__ __forceinline__ __half2 pair_low(uint32_t w) {
-  return __hsub2(bits_h2(magic_or(w, 0x000F000Fu)), __float2half2_rn(1032.f));
+// Nibbles 0 and 4 of a word as the fp16 pair 1024 + nibble (the nibble in the last four mantissa bits),
+// nibbles 1 and 5 as 64 + nibble (in the four bits above them, no shift).
+__device__ __forceinline__ uint32_t biased_low(uint32_t w) { return and_or(w, 0x000F000Fu, 0x64006400u); }
+__device__ __forceinline__ uint32_t biased_high(uint32_t w) { return and_or(w, 0x00F000F0u, 0x54005400u); }
+// The same pairs as the values n = nibble - 8.
+__device__ __forceinline__ uint32_t value_low(uint32_t w) {
+  return h2_bits(__hsub2(bits_h2(biased_low(w)), __float2half2_rn(1032.f)));
 }
-__device__ __forceinline__ __half2 pair_high(uint32_t w) {
-  return __hfma2(bits_h2(magic_or(w, 0x00F000F0u)), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+__device__ __forceinline__ uint32_t value_high(uint32_t w) {
+  return h2_bits(__hsub2(bits_h2(biased_high(w)), __float2half2_rn(72.f)));
 }
 
 // Token (of 8) that row r of a K tile holds.  V slots 2t and 2t + 1 of lane t are then the tokens t
@@ -109,74 +114,224 @@ __device__ __forceinline__ int token_of_row(int r) { return r & 1 ? 4 + ((r >> 1
 
 }  // namespace
 
-// T: type of q and o.  DG = D / 32.  NT: tiles of 8 query columns a block holds.  One warp streams
-// its own stages of KT tokens through a ring of kStages; the block's kWarps take the stages of a split
-// in turn and merge once at the end, so no barrier runs inside the loop.
-template <typename T, int DG, int NT, int KT, int kStages, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) attn_int4_kernel(const __grid_constant__ Int4Attn a) {
-  constexpr int D = DG * 32;
-  constexpr int QP = sizeof(T) == 4 ? 2 : 1;                                // fp16 parts of q
-  constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;         // fp16 parts of p
-  constexpr int NW = (DG + 1) / 2;                                          // V words a lane takes of a row
-  constexpr int kTiles = KT / 16;
-  constexpr int kStageBytes = 2 * KT * (D / 2 + D / 16);
-  constexpr int kRow = D / 2, kScaleRow = D / 16;
-
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  unsigned char* ring = smem + warp * (kStages * kStageBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes) + warp * kStages;
-
-  // Column blocks of one split are neighbours in the grid, so their reads of the cache meet in L2.
-  int64_t idx = blockIdx.x;
-  const int cb = (int)(idx % a.col_blocks);
-  idx /= a.col_blocks;
-  const int split = (int)(idx % a.max_splits);
-  idx /= a.max_splits;
-  const int hk = (int)(idx % a.p.kv_heads), b = (int)(idx / a.p.kv_heads);
-  const int col0 = cb * NT * 8;
-  int len, end;
-  int64_t offset;
-  int4_range(a, b, col0 + NT * 8, len, offset, end);
-  const int n_splits = max(1, ceil_div(end, a.split_keys));
-  if (split >= n_splits) return;
-  const int k_begin = split * a.split_keys, k_end = min(end, k_begin + a.split_keys);
-  const int stages = k_end > k_begin ? ceil_div(k_end - k_begin, KT) : 0;
-  const int mine = stages > warp ? ceil_div(stages - warp, kWarps) : 0;
-
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(&full[s], 1);
-    ptx::fence_mbar_init();
-  }
-  __syncwarp();
-
-  // Lane j fetches page j of a stage; its table entry is read one stage ahead.
-  const int page_size = 1 << a.page_log2;
-  const int stage_pages = KT >> a.page_log2 ? KT >> a.page_log2 : 1;
-  const int32_t* table = a.c.table + b * a.c.table_stride;
-  const unsigned char* pool = reinterpret_cast<const unsigned char*>(a.c.pool) + (int64_t)hk * a.block_bytes;
-  auto stage_key = [&](int n) { return k_begin + (warp + n * kWarps) * KT; };
-  auto entry = [&](int n) {
-    const int key = stage_key(n) + lane * page_size;
-    return n < mine && lane < stage_pages && key < k_end ? table[key >> a.page_log2] : -2;
-  };
-  auto issue = [&](int n, int page) {
-    unsigned char* dst = ring + (n % kStages) * kStageBytes;
-    uint64_t* bar = &full[n % kStages];
-    const bool wanted = page != -2;
-    const bool good = wanted && page >= 0 && page < a.c.pages;
-    if (wanted && !good) record_fault(a.fault, FAULT_PAGE);
-    if constexpr (KT >= 64) {  // whole pages (page_size <= 64)
-      const int n_good = __popc(__ballot_sync(0xffffffffu, good));
-      if (lane == 0) ptx::mbar_expect_tx(bar, (uint32_t)n_good * a.block_bytes);
-      __syncwarp();
-      if (good) ptx::bulk_g2s(dst + lane * a.block_bytes, pool + page * a.c.page_stride, a.block_bytes, bar);
-    }
-  };
-
-  // Queries: B fragments (channels 32 gr + 8 t + {0,4}, {1,5}, {2,6}, {3,7} of column g).
+// What a lane holds of its query columns and of their running softmax.
+template <typename T, int DG, int NT>
+struct Int4State {
+  static constexpr int QP = sizeof(T) == 4 ? 2 : 1;                          // fp16 parts of q
+  static constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;   // fp16 parts of p
+  static constexpr int NW = (DG + 1) / 2;                                    // V words a lane takes of a row
   uint32_t qf[QP][NT][DG][4];
-  float cs[NT][2];  // what turns a column's products into exponents of 2: columns 2t and 2t + 1
+  float cs[NT][2];       // turns a column's products into exponents of 2; columns 2t and 2t + 1
+  int limit[NT][2];      // last key a column sees
+  float acc[NT][4 * NW][4];
+  float m[NT][2], l[NT][2];
+};
+
+// N consecutive aligned 32-bit words from shared memory in the widest loads.
+template <int N>
+__device__ __forceinline__ void lds_words(const unsigned char* src, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(src)[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(src)[i];
+      w[2 * i] = v.x, w[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+  }
+}
+// N consecutive fp16 scales as pairs in words (an odd last one in the low half).
+template <int N>
+__device__ __forceinline__ void lds_scales(const unsigned char* src, uint32_t (&w)[(N + 1) / 2]) {
+  if constexpr (N % 2 == 0) {
+    lds_words<N / 2>(src, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) {
+      w[i] = reinterpret_cast<const uint16_t*>(src)[2 * i];
+      if (2 * i + 1 < N) w[i] |= (uint32_t) reinterpret_cast<const uint16_t*>(src)[2 * i + 1] << 16;
+    }
+  }
+}
+__device__ __forceinline__ float scale_float(uint32_t pair, int i) {
+  return i & 1 ? __high2float(bits_h2(pair)) : __low2float(bits_h2(pair));
+}
+
+// One stage: KT tokens at st, laid out like a page, the first of them key0.  kEdge: some column does not see
+// all of them, or the split ends among them.
+template <bool kEdge, typename T, int DG, int NT, int KT>
+__device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsigned char* st, int key0,
+                                           int k_end) {
+  using State = Int4State<T, DG, NT>;
+  constexpr int D = DG * 32, NW = State::NW, kTiles = KT / 16, kRow = D / 2, kScaleRow = D / 16;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int tok_a = token_of_row(g), tok_b = 8 + tok_a;
+
+  // S^T = K q^T, a 32-channel group at a time, the group's scale on its fp32 sum.
+  float s[NT][kTiles][4];
+#pragma unroll
+  for (int tile = 0; tile < kTiles; ++tile) {
+    const unsigned char* kb = st + tile * 16 * kRow + t * (DG * 4);
+    const unsigned char* ks = st + KT * kRow + tile * 16 * kScaleRow;
+    uint32_t wa[DG], wb[DG];
+    uint32_t ha[(DG + 1) / 2], hb[(DG + 1) / 2];
+    lds_words<DG>(kb + tok_a * kRow, wa);
+    lds_words<DG>(kb + tok_b * kRow, wb);
+    lds_scales<DG>(ks + tok_a * kScaleRow, ha);
+    lds_scales<DG>(ks + tok_b * kScaleRow, hb);
+#pragma unroll
+    for (int gr = 0; gr < DG; ++gr) {
+      const uint32_t va = wa[gr] >> 8, vb = wb[gr] >> 8;
+      const uint32_t k[8] = {value_low(wa[gr]), value_low(wb[gr]), value_high(wa[gr]), value_high(wb[gr]),
+                             value_low(va),     value_low(vb),     value_high(va),     value_high(vb)};
+      const float sa = scale_float(ha[gr / 2], gr), sb = scale_float(hb[gr / 2], gr);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float dot[4];
+        constexpr int kLast = State::QP - 1;  // the smaller part first
+        mma16816_first(dot, k[0], k[1], k[2], k[3], q.qf[kLast][nt][gr][0], q.qf[kLast][nt][gr][1]);
+        mma16816(dot, k[4], k[5], k[6], k[7], q.qf[kLast][nt][gr][2], q.qf[kLast][nt][gr][3]);
+        if constexpr (kLast > 0) {
+          mma16816(dot, k[0], k[1], k[2], k[3], q.qf[0][nt][gr][0], q.qf[0][nt][gr][1]);
+          mma16816(dot, k[4], k[5], k[6], k[7], q.qf[0][nt][gr][2], q.qf[0][nt][gr][3]);
+        }
+        float(&x)[4] = s[nt][tile];
+        x[0] = gr ? fmaf(sa, dot[0], x[0]) : sa * dot[0];
+        x[1] = gr ? fmaf(sa, dot[1], x[1]) : sa * dot[1];
+        x[2] = gr ? fmaf(sb, dot[2], x[2]) : sb * dot[2];
+        x[3] = gr ? fmaf(sb, dot[3], x[3]) : sb * dot[3];
+      }
+    }
+  }
+  // Softmax; a column's keys lie in the 8 lanes of equal t.
+  uint32_t pf[State::PP][NT][kTiles][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int tile = 0; tile < kTiles; ++tile) {
+      float(&x)[4] = s[nt][tile];
+      if constexpr (kEdge) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + tile * 16 + (e < 2 ? tok_a : tok_b);
+          if (key >= k_end || key > q.limit[nt][e & 1]) x[e] = -INFINITY;
+        }
+      }
+      top[0] = ptx::max3(top[0], x[0], x[2]);
+      top[1] = ptx::max3(top[1], x[1], x[3]);
+    }
+    // The reference m follows the maximum only when a score passes it by more than 2^8: p * 2^7 then
+    // stays below 2^15, and most stages need no reduction over the lanes.  (Products round up and sums
+    // down, so the fused x cs + base below cannot pass 15 however large the scores are.)
+    if (__any_sync(0xffffffffu, __fmul_ru(top[0], q.cs[nt][0]) > __fadd_rd(q.m[nt][0], 8.f) ||
+                                    __fmul_ru(top[1], q.cs[nt][1]) > __fadd_rd(q.m[nt][1], 8.f))) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float up = top[j];
+        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 4));
+        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 8));
+        up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 16));
+        up = fmaxf(q.m[nt][j], __fmul_ru(up, q.cs[nt][j]));
+        const float f = up > q.m[nt][j] ? ptx::ex2(q.m[nt][j] - up) : 1.f;
+        q.m[nt][j] = up;
+        q.l[nt][j] *= f;
+#pragma unroll
+        for (int k = 0; k < 4 * NW; ++k) {
+          q.acc[nt][k][j] *= f;
+          q.acc[nt][k][j + 2] *= f;
+        }
+      }
+    }
+    const uint64_t base2 = ptx::f2pack(__fadd_rd(7.f, q.m[nt][0] == -INFINITY ? 0.f : -q.m[nt][0]),
+                                       __fadd_rd(7.f, q.m[nt][1] == -INFINITY ? 0.f : -q.m[nt][1]));
+    const uint64_t cs2 = ptx::f2pack(q.cs[nt][0], q.cs[nt][1]);
+    uint64_t sum2 = ptx::f2pack(q.l[nt][0], q.l[nt][1]);
+#pragma unroll
+    for (int tile = 0; tile < kTiles; ++tile) {
+      const float(&x)[4] = s[nt][tile];
+      float p0, p1, p2, p3;
+      ptx::f2unpack(ptx::fma2(ptx::f2pack(x[0], x[1]), cs2, base2), p0, p1);
+      ptx::f2unpack(ptx::fma2(ptx::f2pack(x[2], x[3]), cs2, base2), p2, p3);
+      p0 = ptx::ex2(p0), p1 = ptx::ex2(p1), p2 = ptx::ex2(p2), p3 = ptx::ex2(p3);
+      sum2 = ptx::add2(sum2, ptx::add2(ptx::f2pack(p0, p1), ptx::f2pack(p2, p3)));
+      const __half2 ha = __floats2half2_rn(p0, p1), hb = __floats2half2_rn(p2, p3);
+      pf[0][nt][tile][0] = transpose8x8(h2_bits(ha));
+      pf[0][nt][tile][1] = transpose8x8(h2_bits(hb));
+      if constexpr (State::PP == 2) {
+        pf[1][nt][tile][0] = transpose8x8(h2_bits(__floats2half2_rn(p0 - __low2float(ha), p1 - __high2float(ha))));
+        pf[1][nt][tile][1] = transpose8x8(h2_bits(__floats2half2_rn(p2 - __low2float(hb), p3 - __high2float(hb))));
+      }
+    }
+    ptx::f2unpack(sum2, q.l[nt][0], q.l[nt][1]);
+  }
+  // O^T += V^T P^T.  Lane (g, t) supplies the words g * NW + j of the tokens in its four slots, as
+  // n * scale: exact, in one multiply-add where 72 scale (9 bits) is the bias's share.
+  const int slot[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};
+#pragma unroll
+  for (int tile = 0; tile < kTiles; ++tile) {
+    const unsigned char* vb = st + KT * (kRow + kScaleRow) + tile * 16 * kRow;
+    const unsigned char* vs = st + KT * (2 * kRow + kScaleRow) + tile * 16 * kScaleRow;
+    uint32_t w[4][NW], sc[4][(NW + 1) / 2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DG % 2 == 0) {
+        lds_words<NW>(vb + slot[k] * kRow + g * (NW * 4), w[k]);
+        lds_scales<NW>(vs + slot[k] * kScaleRow + (g * NW) % DG * 2, sc[k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < (NW + 1) / 2; ++j) sc[k][j] = 0;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+          const int word = g * NW + j;
+          const bool in = word < D / 8;
+          w[k][j] = in ? reinterpret_cast<const uint32_t*>(vb + slot[k] * kRow)[word] : 0;
+          if (in) sc[k][j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(vs + slot[k] * kScaleRow)[word % DG] << 16 * (j & 1);
+        }
+      }
+      if constexpr (kEdge) {  // past the end a page may hold anything: its nibbles are finite, its scale need not be
+        if (key0 + tile * 16 + slot[k] >= k_end)
+#pragma unroll
+          for (int j = 0; j < (NW + 1) / 2; ++j) sc[k][j] = 0;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      const __half2 sc0 = bits_h2(__byte_perm(sc[0][j / 2], sc[1][j / 2], j & 1 ? 0x7632 : 0x5410));
+      const __half2 sc1 = bits_h2(__byte_perm(sc[2][j / 2], sc[3][j / 2], j & 1 ? 0x7632 : 0x5410));
+      const __half2 off0 = __hmul2(sc0, __float2half2_rn(-72.f)), off1 = __hmul2(sc1, __float2half2_rn(-72.f));
+#pragma unroll
+      for (int byte = 0; byte < 4; ++byte) {
+        // byte `byte` of two tokens' words in the low bytes of the halves; the other bytes are masked off
+        const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x0400 + byte * 0x0101);
+        const uint32_t x1 = __byte_perm(w[2][j], w[3][j], 0x0400 + byte * 0x0101);
+        const uint32_t a0 = h2_bits(__hmul2(bits_h2(value_low(x0)), sc0));
+        const uint32_t a1 = h2_bits(__hfma2(bits_h2(biased_high(x0)), sc0, off0));
+        const uint32_t a2 = h2_bits(__hmul2(bits_h2(value_low(x1)), sc1));
+        const uint32_t a3 = h2_bits(__hfma2(bits_h2(biased_high(x1)), sc1, off1));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int part = State::PP - 1; part >= 0; --part)
+            mma16816(q.acc[nt][4 * j + byte], a0, a1, a2, a3, pf[part][nt][tile][0], pf[part][nt][tile][1]);
+      }
+    }
+  }
+}
+
+// Reads a block of query columns and clears their running softmax.
+template <typename T, int DG, int NT>
+__device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T, DG, NT>& q, int b, int hk, int col0,
+                                                  int len) {
+  using State = Int4State<T, DG, NT>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int col = col0 + nt * 8 + g;
@@ -187,327 +342,334 @@ __global__ void __launch_bounds__(kWarps * 32) attn_int4_kernel(const __grid_con
     float x[DG][8], amax = 0.f;
     bool odd = false;  // a NaN anywhere in the row
 #pragma unroll
-    for (int gr = 0; gr < DG; ++gr)
+    for (int gr = 0; gr < DG; ++gr) {
+      const T* src = qp + (int64_t)(32 * gr + 8 * t) * a.p.q.stride[3];
+      if (a.q_vec) {
+        alignas(16) T raw[8];
+#pragma unroll
+        for (int e = 0; e < (int)(8 * sizeof(T) / 16); ++e)
+          reinterpret_cast<uint4*>(raw)[e] = reinterpret_cast<const uint4*>(src)[e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[gr][e] = Elem<T>::to_acc(raw[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[gr][e] = Elem<T>::to_acc(src[e * a.p.q.stride[3]]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[gr][e] = live ? Elem<T>::to_acc(qp[(int64_t)(32 * gr + 8 * t + e) * a.p.q.stride[3]]) : 0.f;
+        x[gr][e] = live ? x[gr][e] : 0.f;
         amax = fmaxf(amax, fabsf(x[gr][e]));
         odd |= x[gr][e] != x[gr][e];
       }
+    }
     if (odd) amax = INFINITY;
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // up = 2^(14 - floor(log2 amax)); the exponent field stays within normal numbers
+    // up = 2^(14 - floor(log2 amax)); the exponent field stays within normal numbers.  The softmax scale's
+    // sign goes to q, so that the largest product is the largest score; where the scale leaves nothing of
+    // the products, q becomes zero (a zero factor would make NaN of a hidden key's -inf).
+    const float scale = (float)a.p.scale * kInt4Log2e;
     const int up_exp = min(253, max(1, 268 - (int)(__float_as_uint(amax) >> 23)));
-    const float up = __uint_as_float((uint32_t)up_exp << 23);
-    float unit = __uint_as_float((uint32_t)(254 - up_exp) << 23) * ((float)a.p.scale * kInt4Log2e);
+    float unit = __uint_as_float((uint32_t)(254 - up_exp) << 23) * fabsf(scale);
+    float up = __uint_as_float((uint32_t)up_exp << 23) * (scale < 0.f ? -1.f : 1.f);
+    if (unit == 0.f) up = 0.f, unit = 1.f;
     if (!(amax < INFINITY)) unit = __int_as_float(0x7fc00000);  // a non-finite query gives NaN, as its product would
 #pragma unroll
-    for (int j = 0; j < 2; ++j) cs[nt][j] = __shfl_sync(0xffffffffu, unit, (2 * t + j) * 4);
+    for (int j = 0; j < 2; ++j) q.cs[nt][j] = __shfl_sync(0xffffffffu, unit, (2 * t + j) * 4);
+    // B fragments: channels 32 gr + 8 t + {0,4}, {1,5}, {2,6}, {3,7} of column g
 #pragma unroll
     for (int gr = 0; gr < DG; ++gr)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float lo = x[gr][e] * up, hi = x[gr][e + 4] * up;
         const __half2 part = __floats2half2_rn(lo, hi);
-        qf[0][nt][gr][e] = h2_bits(part);
-        if constexpr (QP == 2)
-          qf[1][nt][gr][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
+        q.qf[0][nt][gr][e] = h2_bits(part);
+        if constexpr (State::QP == 2)
+          q.qf[1][nt][gr][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
       }
-  }
-  // Last key each of this lane's columns sees, and the last that all of them see.
-  int limit[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int col = min(col0 + nt * 8 + 2 * t + j, a.cols - 1);
-      limit[nt][j] = a.p.is_causal ? (int)i64max(-1, i64min(len, offset + col / a.group + 1) - 1) : len - 1;
+      const int tok = min(col0 + nt * 8 + 2 * t + j, a.cols - 1) / a.group;
+      q.limit[nt][j] = a.p.is_causal ? max(-1, len - a.p.q_len + tok) : len - 1;
+      q.m[nt][j] = -INFINITY;
+      q.l[nt][j] = 0.f;
     }
-  const int all_see = a.p.is_causal ? (int)i64max(-1, i64min(len, offset + col0 / a.group + 1) - 1) : len - 1;
-
-  float acc[NT][4 * NW][4];
-  float m[NT][2], l[NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+    for (int k = 0; k < 4 * State::NW; ++k)
 #pragma unroll
-    for (int k = 0; k < 4 * NW; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-
-  int ahead = entry(0);
-#pragma unroll
-  for (int n = 0; n < kStages - 1; ++n) {
-    if (n < mine) issue(n, ahead);
-    ahead = entry(n + 1);
-  }
-  const int tok_a = token_of_row(g), tok_b = 8 + tok_a;
-  bool ok = true;
-  int issued = min(mine, kStages - 1);
-  for (int n = 0; n < mine; ++n) {
-    if (issued < mine) {
-      issue(issued, ahead);
-      ++issued;
-      ahead = entry(issued);
-    }
-    ok = __all_sync(0xffffffffu, ptx::mbar_wait(&full[n % kStages], (n / kStages) & 1, a.fault, FAULT_DEC_FULL));
-    if (!ok) break;
-    const unsigned char* st = ring + (n % kStages) * kStageBytes;
-    const int key0 = stage_key(n);
-
-    float s[NT][kTiles][4];
-#pragma unroll
-    for (int tile = 0; tile < kTiles; ++tile) {
-      const int in_page = (tile * 16) & (page_size - 1);
-      const unsigned char* kb = st + ((tile * 16) >> a.page_log2) * a.block_bytes;
-      const unsigned char* ks = kb + page_size * kRow + in_page * kScaleRow;
-      kb += in_page * kRow + t * (DG * 4);
-      uint32_t wa[DG], wb[DG];
-      if constexpr (DG % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < DG / 4; ++i) {
-          *reinterpret_cast<uint4*>(&wa[4 * i]) = reinterpret_cast<const uint4*>(kb + tok_a * kRow)[i];
-          *reinterpret_cast<uint4*>(&wb[4 * i]) = reinterpret_cast<const uint4*>(kb + tok_b * kRow)[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < DG; ++i) {
-          wa[i] = reinterpret_cast<const uint32_t*>(kb + tok_a * kRow)[i];
-          wb[i] = reinterpret_cast<const uint32_t*>(kb + tok_b * kRow)[i];
-        }
-      }
-#pragma unroll
-      for (int gr = 0; gr < DG; ++gr) {
-        const float sa = __half2float(reinterpret_cast<const __half*>(ks + tok_a * kScaleRow)[gr]);
-        const float sb = __half2float(reinterpret_cast<const __half*>(ks + tok_b * kScaleRow)[gr]);
-        const uint32_t a0 = h2_bits(pair_low(wa[gr])), a2 = h2_bits(pair_high(wa[gr]));
-        const uint32_t a1 = h2_bits(pair_low(wb[gr])), a3 = h2_bits(pair_high(wb[gr]));
-        const uint32_t c0 = h2_bits(pair_low(wa[gr] >> 8)), c2 = h2_bits(pair_high(wa[gr] >> 8));
-        const uint32_t c1 = h2_bits(pair_low(wb[gr] >> 8)), c3 = h2_bits(pair_high(wb[gr] >> 8));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float dot[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int q = QP - 1; q >= 0; --q) {
-            mma16816(dot, a0, a1, a2, a3, qf[q][nt][gr][0], qf[q][nt][gr][1]);
-            mma16816(dot, c0, c1, c2, c3, qf[q][nt][gr][2], qf[q][nt][gr][3]);
-          }
-          float(&x)[4] = s[nt][tile];
-          x[0] = gr ? fmaf(sa, dot[0], x[0]) : sa * dot[0];
-          x[1] = gr ? fmaf(sa, dot[1], x[1]) : sa * dot[1];
-          x[2] = gr ? fmaf(sb, dot[2], x[2]) : sb * dot[2];
-          x[3] = gr ? fmaf(sb, dot[3], x[3]) : sb * dot[3];
-        }
-      }
-    }
-    // Softmax of the stage's KT keys, a column's keys spread over the 8 lanes of equal t.
-    const bool edge = key0 + KT > min(k_end, all_see + 1);
-    uint32_t pf[PP][NT][kTiles][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int tile = 0; tile < kTiles; ++tile)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float& x = s[nt][tile][e];
-          x *= cs[nt][e & 1];
-          if (edge) {
-            const int key = key0 + tile * 16 + (e < 2 ? tok_a : tok_b);
-            if (key >= k_end || key > limit[nt][e & 1]) x = -INFINITY;
-          }
-          top[e & 1] = fmaxf(top[e & 1], x);
-        }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 4));
-        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
-        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float up = fmaxf(m[nt][j], top[j]);
-          const float f = up > m[nt][j] ? ptx::ex2(m[nt][j] - up) : 1.f;
-          m[nt][j] = up;
-          l[nt][j] *= f;
-#pragma unroll
-          for (int k = 0; k < 4 * NW; ++k) {
-            acc[nt][k][j] *= f;
-            acc[nt][k][j + 2] *= f;
-          }
-        }
-      }
-      const float base0 = (m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 15.f;
-      const float base1 = (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 15.f;
-#pragma unroll
-      for (int tile = 0; tile < kTiles; ++tile) {
-        const float(&x)[4] = s[nt][tile];
-        const float p0 = ptx::ex2(x[0] - base0), p1 = ptx::ex2(x[1] - base1);
-        const float p2 = ptx::ex2(x[2] - base0), p3 = ptx::ex2(x[3] - base1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        const __half2 ha = __floats2half2_rn(p0, p1), hb = __floats2half2_rn(p2, p3);
-        pf[0][nt][tile][0] = transpose8x8(h2_bits(ha));
-        pf[0][nt][tile][1] = transpose8x8(h2_bits(hb));
-        if constexpr (PP == 2) {
-          pf[1][nt][tile][0] = transpose8x8(h2_bits(__floats2half2_rn(p0 - __low2float(ha), p1 - __high2float(ha))));
-          pf[1][nt][tile][1] = transpose8x8(h2_bits(__floats2half2_rn(p2 - __low2float(hb), p3 - __high2float(hb))));
-        }
-      }
-    }
-    // O^T += V^T P^T.  Lane (g, t) supplies the words g * NW + j of the tokens in its four slots.
-#pragma unroll
-    for (int tile = 0; tile < kTiles; ++tile) {
-      const int in_page = (tile * 16) & (page_size - 1);
-      const unsigned char* vb = st + ((tile * 16) >> a.page_log2) * a.block_bytes + (a.block_bytes >> 1);
-      const unsigned char* vs = vb + page_size * kRow + in_page * kScaleRow;
-      vb += in_page * kRow;
-      const int slot[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};
-      uint32_t w[4][NW];
-      __half sc[4][NW];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < NW; ++j) {
-          const int word = g * NW + j;
-          if (DG % 2 == 0 || word < D / 8) {
-            w[k][j] = reinterpret_cast<const uint32_t*>(vb + slot[k] * kRow)[word];
-            sc[k][j] = reinterpret_cast<const __half*>(vs + slot[k] * kScaleRow)[word % DG];
-          } else {
-            w[k][j] = 0;
-            sc[k][j] = __ushort_as_half(0);
-          }
-          // Past the end the page may hold anything; its nibbles are finite, its scale need not be.
-          if (edge && key0 + tile * 16 + slot[k] >= k_end) sc[k][j] = __ushort_as_half(0);
-        }
-#pragma unroll
-      for (int j = 0; j < NW; ++j) {
-        const __half2 sc0 = __halves2half2(sc[0][j], sc[1][j]), sc1 = __halves2half2(sc[2][j], sc[3][j]);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t x0 = __byte_perm(w[0][j], w[1][j], half ? 0x7632 : 0x5410);
-          const uint32_t x1 = __byte_perm(w[2][j], w[3][j], half ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int hi = 0; hi < 2; ++hi) {
-            const uint32_t a0 = h2_bits(__hmul2(pair_low(x0 >> (8 * hi)), sc0));
-            const uint32_t a1 = h2_bits(__hmul2(pair_high(x0 >> (8 * hi)), sc0));
-            const uint32_t a2 = h2_bits(__hmul2(pair_low(x1 >> (8 * hi)), sc1));
-            const uint32_t a3 = h2_bits(__hmul2(pair_high(x1 >> (8 * hi)), sc1));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int q = PP - 1; q >= 0; --q)
-                mma16816(acc[nt][4 * j + 2 * half + hi], a0, a1, a2, a3, pf[q][nt][tile][0], pf[q][nt][tile][1]);
-          }
-        }
-      }
-    }
-    __syncwarp();  // every lane is done with the stage before it is filled again
-  }
-  if (!ok) {  // let the copies that are still in flight land before the block ends
-    for (int n = 0; n < issued; ++n) {
-      if (n + kStages < issued) continue;
-      ptx::mbar_wait(&full[n % kStages], (n / kStages) & 1, a.fault, FAULT_DEC_FULL);
-    }
-  }
-  // Merge the warps' partial results through shared memory.
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
-      l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
-      l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
-    }
-  constexpr int kCols = NT * 8;
-  constexpr int kPad = D + 4;
-  float* red = reinterpret_cast<float*>(smem);
-  float* ml = red + kWarps * kCols * kPad;
-  const bool all_ok = __syncthreads_and(ok);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int j = 0; j < NW; ++j) {
-      const int word = g * NW + j;
-      if (DG % 2 == 0 || word < D / 8) {
-        const int ch = 32 * (word % DG) + 8 * (word / DG);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            red[(warp * kCols + nt * 8 + 2 * t + (e & 1)) * kPad + ch + 2 * k + (e >> 1)] = acc[nt][4 * j + k][e];
-      }
-    }
-    if (g == 0)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        ml[(warp * kCols + nt * 8 + 2 * t + j) * 2] = m[nt][j];
-        ml[(warp * kCols + nt * 8 + 2 * t + j) * 2 + 1] = l[nt][j];
-      }
-  }
-  __syncthreads();
-  if (!all_ok) return;
-  for (int i = threadIdx.x; i < kCols * D; i += kWarps * 32) {
-    const int col = i / D, d = i - col * D;
-    if (col0 + col >= a.cols) break;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[(w * kCols + col) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, out = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ptx::ex2(ml[(w * kCols + col) * 2] - base);
-      sum += ml[(w * kCols + col) * 2 + 1] * f;
-      out += red[(w * kCols + col) * kPad + d] * f;
-    }
-    const int tok = (col0 + col) / a.group, h = hk * a.group + (col0 + col) - tok * a.group;
-    if (n_splits == 1) {
-      int4_store_row<T>(a, b, h, tok, d, sum == 0.f ? 0.f : out / sum);
-      if (d == 0) int4_store_lse(a, b, h, tok, top - 15.f, sum);
-    } else {
-      const int64_t row = ((int64_t)b * a.p.q_heads + h) * a.p.q_len + tok;
-      a.ws_acc[(row * a.max_splits + split) * D + d] = out;
-      if (d == 0) {
-        a.ws_ml[(row * a.max_splits + split) * 2] = top;
-        a.ws_ml[(row * a.max_splits + split) * 2 + 1] = sum;
-      }
-    }
+      for (int e = 0; e < 4; ++e) q.acc[nt][k][e] = 0.f;
   }
 }
 
-// One block an output row: merges its splits.
-template <typename T>
-__global__ void attn_int4_combine(const __grid_constant__ Int4Attn a, int block_cols) {
+// Writes the columns' results: to the output when the warp saw all of their keys, else to a partial slot.
+template <typename T, int DG, int NT>
+__device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, NT>& q, int b, int hk, int col0,
+                                           int slot) {
+  constexpr int D = DG * 32, NW = Int4State<T, DG, NT>::NW;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum = q.l[nt][j];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      const int local = nt * 8 + 2 * t + j, col = col0 + local;
+      if (col >= a.cols) continue;
+      const int tok = col / a.group, h = hk * a.group + col - tok * a.group;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      float* part = slot < 0 ? nullptr : a.ws_acc + ((int64_t)slot * a.slot_cols + local) * D;
+      T* row = int4_out_row<T>(a, b, h, tok);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const int word = g * NW + w, ch = 32 * (word % DG) + 8 * (word / DG);
+        if (DG % 2 && word >= D / 8) continue;
+        float x[8];  // channels ch..ch + 7
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = q.acc[nt][4 * w + e / 2][j + 2 * (e & 1)];
+        if (slot >= 0) {
+          reinterpret_cast<float4*>(part + ch)[0] = make_float4(x[0], x[1], x[2], x[3]);
+          reinterpret_cast<float4*>(part + ch)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+          alignas(16) T y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = Elem<T>::from_acc(x[e] * inv);
+          if (a.o_vec) {
+#pragma unroll
+            for (int e = 0; e < (int)(8 * sizeof(T) / 16); ++e)
+              reinterpret_cast<uint4*>(row + ch)[e] = reinterpret_cast<const uint4*>(y)[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) row[(ch + e) * a.p.o.stride[3]] = y[e];
+          }
+        }
+      }
+      if (g == 0) {
+        if (slot >= 0)
+          reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * a.slot_cols + local] = make_float2(q.m[nt][j], sum);
+        else
+          int4_store_lse(a, b, h, tok, q.m[nt][j] - 7.f, sum);
+      }
+    }
+}
+
+// T: type of q and o.  DG = D / 32.  NT: tiles of 8 query columns a warp holds.
+//
+// The work is a line of stages of KT tokens, ordered by (row, KV head, column block, key); rows differ in
+// length, so every warp takes an equal share of the line instead of whole rows or splits of one size.  A
+// share may begin and end inside a row: what it holds of such a row goes to one of the warp's two partial
+// slots, and attn_int4_combine merges them.  Each warp runs its own ring of bulk copies through its whole
+// share, the next row's first stages in flight while it finishes the last one; no block barrier runs
+// after the start.
+template <typename T, int DG, int NT, int KT, int kStages, int kWarps, int kMinBlocks>
+__global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(const __grid_constant__ Int4Attn a) {
+  constexpr int D = DG * 32;
+  constexpr int kRowBytes = D / 2 + D / 16, kStageBytes = 2 * KT * kRowBytes;
+
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* ring = smem + warp * (kStages * kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes) + warp * kStages;
+  int* first = reinterpret_cast<int*>(smem + kWarps * kStages * (kStageBytes + (int)sizeof(uint64_t)));
+  const int pairs = a.p.kv_heads * a.col_blocks;
+
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(&full[s], 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0) {  // first[b]: the stages of the rows before b
+    int carry = 0;
+    for (int b0 = 0; b0 < a.p.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const int n = b < a.p.batch ? ceil_div(int4_len(a, b), KT) * pairs : 0;
+      int inc = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += below;
+      }
+      if (b < a.p.batch) first[b] = carry + inc - n;
+      carry += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) first[a.p.batch] = carry;
+    __syncwarp();
+    if (blockIdx.x == 0 && a.ws_first)
+      for (int b = lane; b <= a.p.batch; b += 32) a.ws_first[b] = first[b];
+  }
+  __syncthreads();
+  // Neighbouring shares go to different blocks, so a short line spreads over the SMs.
+  const int id = warp * gridDim.x + blockIdx.x;
+  const int total = first[a.p.batch], share = int4_share(a, total);
+  const int begin = (int)i64min((int64_t)id * share, total), mine = min(share, total - begin);
+  if (mine <= 0) return;
+
+  struct Place {  // of a stage: row, column block and KV head, stage of the row and their number
+    int b, pair, st, n_st;
+  };
+  auto place = [&](int i) {
+    int lo = 0, hi = a.p.batch - 1;  // the last row whose first stage is not past i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    Place p;
+    p.b = lo;
+    p.n_st = (first[lo + 1] - first[lo]) / pairs;
+    p.pair = (i - first[lo]) / p.n_st;
+    p.st = i - first[lo] - p.pair * p.n_st;
+    return p;
+  };
+
+  // A stage in shared memory is laid out like a page of KT tokens, whatever the page size.  Lane 4 j + k
+  // fetches part k (keys, key scales, values, value scales) of its j-th `unit` tokens; where a page is a
+  // stage, lane 0 fetches it in one copy.  The addresses of the next 32 units are worked out by one lane
+  // each, so a stage costs a few shuffles.
+  const int unit = min(1 << a.page_log2, KT), units = KT / unit;  // units of a stage: 1, 2 or 4
+  const bool whole = (1 << a.page_log2) == KT;
+  const int part = whole ? 0 : lane & 3, my_unit = whole ? 0 : lane >> 2;
+  const bool fetches = whole ? lane == 0 : my_unit < units;
+  const int row_bytes = part & 1 ? D / 16 : D / 2;
+  const uint32_t bytes = whole ? kStageBytes : unit * row_bytes;
+  const uint32_t to = (part >> 1) * (kStageBytes / 2) + (part & 1) * KT * (D / 2) + my_unit * bytes;
+  const int part_at = (part >> 1) * (a.block_bytes / 2) + (part & 1) * ((D / 2) << a.page_log2);
+  const unsigned char* ahead = nullptr;  // block of this lane's unit, nullptr: none
+  int ahead_tok = 0;                     // the unit's first token in its page
+  uint32_t ahead_mask = 0;               // lanes that have one
+  auto look = [&](int n) {               // from stage n of the share on
+    const int i = n + lane / units;
+    ahead = nullptr;
+    if (i < mine) {
+      const Place p = place(begin + i);
+      const int key = p.st * KT + lane % units * unit;
+      if (key < int4_len(a, p.b)) {
+        const int page = a.c.table[p.b * a.c.table_stride + (key >> a.page_log2)];
+        ahead_tok = key & ((1 << a.page_log2) - 1);
+        if (page >= 0 && page < a.c.pages)
+          ahead = reinterpret_cast<const unsigned char*>(a.c.pool) + page * a.c.page_stride +
+                  (int64_t)(p.pair / a.col_blocks) * a.block_bytes;
+        else
+          record_fault(a.fault, FAULT_PAGE);
+      }
+    }
+    __syncwarp();
+    ahead_mask = __ballot_sync(0xffffffffu, ahead != nullptr);
+  };
+  auto issue = [&](int n) {
+    const int at = n * units & 31;
+    if (at == 0) look(n);
+    unsigned char* dst = ring + (n % kStages) * kStageBytes;
+    uint64_t* bar = &full[n % kStages];
+    const int from = at + my_unit;
+    const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ahead), from & 31);
+    const int tok = whole ? 0 : __shfl_sync(0xffffffffu, ahead_tok, from & 31);
+    const uint32_t live = ahead_mask >> at & ((1u << units) - 1);
+    if (lane == 0) ptx::mbar_expect_tx(bar, __popc(live) * (kStageBytes / units));
+    __syncwarp();
+    if (fetches && src) ptx::bulk_g2s(dst + to, reinterpret_cast<const void*>(src + part_at + tok * row_bytes), bytes, bar);
+  };
+  int issued = 0;
+  while (issued < min(mine, kStages - 1)) issue(issued++);
+
+  Int4State<T, DG, NT> q;
+  int n = 0;
+  while (n < mine) {
+    const Place p = place(begin + n);
+    const int len = int4_len(a, p.b), hk = p.pair / a.col_blocks, col0 = (p.pair - hk * a.col_blocks) * NT * 8;
+    const int count = min(mine - n, p.n_st - p.st);
+    int4_load_queries(a, q, p.b, hk, col0, len);
+    // the first key that some column does not see
+    const int plain = a.p.is_causal ? min(len, max(0, len - a.p.q_len + col0 / a.group + 1)) : len;
+    int key0 = p.st * KT;
+    for (int k = 0; k < count; ++k, ++n, key0 += KT) {
+      if (issued < mine) issue(issued++);
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[n % kStages], (n / kStages) & 1, a.fault, FAULT_DEC_FULL))) {
+        // let the copies that are still in flight land before the block ends
+        for (int s = n + 1; s < issued; ++s)
+          ptx::mbar_wait(&full[s % kStages], (s / kStages) & 1, a.fault, FAULT_DEC_FULL);
+        return;
+      }
+      const unsigned char* st = ring + (n % kStages) * kStageBytes;
+      if (key0 + KT <= plain)
+        int4_stage<false, T, DG, NT, KT>(q, st, key0, len);
+      else
+        int4_stage<true, T, DG, NT, KT>(q, st, key0, len);
+      __syncwarp();  // every lane is done with the stage before it is filled again
+    }
+    int4_store(a, q, p.b, hk, col0, count == p.n_st ? -1 : 2 * id + (n == count ? 0 : 1));
+  }
+}
+
+constexpr int kInt4CombineThreads = 256;
+
+// One block an output row.  Rows without keys become zeros; a row that one warp saw whole is done; of the
+// others the block's warps take every eighth partial, a lane D / 32 of the channels.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kInt4CombineThreads) attn_int4_combine(const __grid_constant__ Int4Attn a) {
+  constexpr int kWarps = kInt4CombineThreads / 32;
+  __shared__ float part[kWarps][256];
+  __shared__ float sums[kWarps];
   const int64_t row = blockIdx.x;
   const int tok = (int)(row % a.p.q_len), h = (int)(row / a.p.q_len % a.p.q_heads);
   const int b = (int)(row / ((int64_t)a.p.q_len * a.p.q_heads));
-  const int col = tok * a.group + h % a.group;
-  int len, end;
-  int64_t offset;
-  int4_range(a, b, col / block_cols * block_cols + block_cols, len, offset, end);
-  const int n = max(1, ceil_div(end, a.split_keys));
-  if (n == 1) return;
-  const float* ml = a.ws_ml + row * a.max_splits * 2;
-  float top = -INFINITY;
-  for (int s = 0; s < n; ++s) top = fmaxf(top, ml[2 * s]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int s = 0; s < n; ++s) sum += ml[2 * s + 1] * ptx::ex2(ml[2 * s] - base);
-  for (int d = threadIdx.x; d < a.p.head_dim; d += blockDim.x) {
-    float out = 0.f;
-    for (int s = 0; s < n; ++s)
-      out += a.ws_acc[(row * a.max_splits + s) * a.p.head_dim + d] * ptx::ex2(ml[2 * s] - base);
-    int4_store_row<T>(a, b, h, tok, d, sum == 0.f ? 0.f : out / sum);
+  const int hk = h / a.group, col = tok * a.group + h - hk * a.group;
+  const int pairs = a.p.kv_heads * a.col_blocks, pair = hk * a.col_blocks + col / (NT * 8), local = col % (NT * 8);
+  const int total = a.ws_first[a.p.batch], row_first = a.ws_first[b];
+  const int n_st = (a.ws_first[b + 1] - row_first) / pairs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = a.p.head_dim / 32;
+  float o = 0.f, l = 0.f, top = -INFINITY;
+  if (n_st) {
+    const int begin = row_first + pair * n_st, last = begin + n_st - 1;
+    const int share = int4_share(a, total), w0 = begin / share, w1 = last / share;
+    if (w0 == w1) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + local;
+    auto slot = [&](int w) {  // where warp w left its part of the row
+      return (int64_t)(2 * w + ((int64_t)w * share < begin)) * a.slot_cols;
+    };
+    for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, ml[slot(w)].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float base = top == -INFINITY ? 0.f : top;
+    float out[8] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int w = w0 + warp; w <= w1; w += kWarps) {
+      const int64_t s = slot(w);
+      const float2 x = ml[s];
+      const float f = ptx::ex2(x.x - base);
+      sum += x.y * f;
+      const float* acc = a.ws_acc + (s + local) * a.p.head_dim + lane;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < groups) out[k] = fmaf(acc[k * 32], f, out[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = out[k];
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < a.p.head_dim) {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        o += part[w][threadIdx.x];
+        l += sums[w];
+      }
+    }
   }
-  if (threadIdx.x == 0) int4_store_lse(a, b, h, tok, top - 15.f, sum);
+  if (threadIdx.x >= a.p.head_dim) return;
+  int4_out_row<T>(a, b, h, tok)[threadIdx.x * a.p.o.stride[3]] = Elem<T>::from_acc(l == 0.f ? 0.f : o / l);
+  if (threadIdx.x == 0) int4_store_lse(a, b, h, tok, top - 7.f, l);
 }
 
+// Shape of the kernel that takes a problem.
+struct Int4Shape {
+  int nt;      // column tiles of a warp
+  int keys;    // tokens of a stage
+  int warps;   // of a block
+  int blocks;  // resident on an SM
+};
+Int4Shape int4_shape(const ts_attn_params& p);
+
 template <typename T>
-cudaError_t attn_int4_launch(const Int4Attn& a, int nt, cudaStream_t st);
+cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st);
 
 }  // namespace tsa

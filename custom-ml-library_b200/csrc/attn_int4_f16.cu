@@ -2,5 +2,5 @@
 #include "attn_int4_launch.cuh"
 
 namespace tsa {
-template cudaError_t attn_int4_launch<__half>(const Int4Attn& a, int nt, cudaStream_t st);
+template cudaError_t attn_int4_launch<__half>(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st);
 }  // namespace tsa

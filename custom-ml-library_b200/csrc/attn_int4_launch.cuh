@@ -4,51 +4,47 @@
 
 namespace tsa {
 
-constexpr int kInt4Keys = 64;   // tokens of a stage
-constexpr int kInt4Stages = 2;  // stages in flight for each warp
+constexpr int kInt4Stages = 2;  // stages in a warp's ring
 constexpr int kInt4Warps = 4;
 
-template <typename T, int DG, int NT>
-static cudaError_t int4_run(const Int4Attn& a, cudaStream_t st) {
-  constexpr int D = DG * 32;
-  constexpr size_t ring = (size_t)kInt4Warps * kInt4Stages * (2 * kInt4Keys * (D / 2 + D / 16) + sizeof(uint64_t));
-  constexpr size_t red = (size_t)kInt4Warps * NT * 8 * (D + 4 + 2) * sizeof(float);
-  constexpr size_t smem = ring > red ? ring : red;
-  auto kernel = attn_int4_kernel<T, DG, NT, kInt4Keys, kInt4Stages, kInt4Warps>;
+template <typename T, int DG, int NT, int KT, int kMinBlocks>
+static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
+  constexpr size_t ring =
+      (size_t)kInt4Warps * kInt4Stages * (2 * KT * (DG * 16 + DG * 2) + sizeof(uint64_t));
+  const size_t smem = ring + (size_t)(a.p.batch + 1) * sizeof(int);
+  auto kernel = attn_int4_kernel<T, DG, NT, KT, kInt4Stages, kInt4Warps, kMinBlocks>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = (int64_t)a.p.batch * a.p.kv_heads * a.max_splits * a.col_blocks;
-  const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
-  if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  kernel<<<(unsigned)blocks, kInt4Warps * 32, smem, st>>>(a);
+  kernel<<<blocks, kInt4Warps * 32, smem, st>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.max_splits == 1) return e;
-  attn_int4_combine<T><<<(unsigned)rows, 128, 0, st>>>(a, NT * 8);
+  if (e != cudaSuccess) return e;
+  attn_int4_combine<T, NT><<<(unsigned)((int64_t)a.p.batch * a.p.q_heads * a.p.q_len), kInt4CombineThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t attn_int4_launch(const Int4Attn& a, int nt, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2) {  // two column tiles: half types up to D = 128 (registers)
-    if (nt == 2) {
-      switch (a.p.head_dim) {
-        case 32: return int4_run<T, 1, 2>(a, st);
-        case 64: return int4_run<T, 2, 2>(a, st);
-        case 96: return int4_run<T, 3, 2>(a, st);
-        case 128: return int4_run<T, 4, 2>(a, st);
+cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st) {
+  const int groups = a.p.head_dim / 32;
+  if constexpr (sizeof(T) == 2) {
+    if (shape.nt == 2) {
+      switch (groups) {
+        case 1: return int4_run<T, 1, 2, 64, 2>(a, blocks, st);
+        case 2: return int4_run<T, 2, 2, 64, 2>(a, blocks, st);
+        case 3: return int4_run<T, 3, 2, 64, 2>(a, blocks, st);
+        case 4: return int4_run<T, 4, 2, 64, 2>(a, blocks, st);
       }
       return cudaErrorInvalidValue;
     }
   }
-  switch (a.p.head_dim) {
-    case 32: return int4_run<T, 1, 1>(a, st);
-    case 64: return int4_run<T, 2, 1>(a, st);
-    case 96: return int4_run<T, 3, 1>(a, st);
-    case 128: return int4_run<T, 4, 1>(a, st);
-    case 160: return int4_run<T, 5, 1>(a, st);
-    case 192: return int4_run<T, 6, 1>(a, st);
-    case 224: return int4_run<T, 7, 1>(a, st);
-    case 256: return int4_run<T, 8, 1>(a, st);
+  switch (groups) {
+    case 1: return int4_run<T, 1, 1, 64, 3>(a, blocks, st);
+    case 2: return int4_run<T, 2, 1, 64, 3>(a, blocks, st);
+    case 3: return int4_run<T, 3, 1, 64, 3>(a, blocks, st);
+    case 4: return int4_run<T, 4, 1, 64, 3>(a, blocks, st);
+    case 5: return int4_run<T, 5, 1, 32, 2>(a, blocks, st);
+    case 6: return int4_run<T, 6, 1, 32, 2>(a, blocks, st);
+    case 7: return int4_run<T, 7, 1, 32, 2>(a, blocks, st);
+    case 8: return int4_run<T, 8, 1, 32, 2>(a, blocks, st);
   }
   return cudaErrorInvalidValue;
 }
