@@ -31,6 +31,7 @@ int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
   const int64_t most = (int64_t)rows * p.kv_heads * a.col_blocks * ceil_div(p.kv_len, shape.keys);
   const int blocks = (int)i64min(most, (int64_t)sm_count() * shape.blocks);
   a.warps = blocks * shape.warps;
+  a.parts = (int)(blocks / i64max(1, (int64_t)rows * p.kv_heads * a.col_blocks));
   return blocks;
 }
 
@@ -58,7 +59,7 @@ size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
   Int4Shape shape;
   plan(p, a, shape);
   const int rows = p.batch < kMaxRows ? p.batch : kMaxRows;
-  return partial_bytes(a, p.head_dim) + (size_t)(rows + 1) * sizeof(int32_t);
+  return partial_bytes(a, p.head_dim) + (size_t)2 * (rows + 1) * sizeof(int32_t);
 }
 
 cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,

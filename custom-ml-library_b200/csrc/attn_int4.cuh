@@ -42,16 +42,19 @@ struct Int4Attn {
   int col_blocks;  // blocks of columns; one warp holds one at a time
   int slot_cols;   // columns of a block that can be live
   int warps;       // that share the work
+  int parts;       // about how many blocks share a row at the longest length
   bool q_vec, o_vec;  // rows of unit stride and 16-byte alignment
   float* ws_acc;   // [2 * warps, slot_cols, D] partial results
   float* ws_ml;    // [2 * warps, slot_cols, 2]
-  int32_t* ws_first;  // [batch + 1] first stage of each row
+  int32_t* ws_first;  // [2, batch + 1] stages and units before each row
   uint32_t* fault;
 };
 
 __device__ __forceinline__ int int4_len(const Int4Attn& a, int b) { return min(a.p.kv_len, max(0, a.p.kv_lens[b])); }
-// Stages of a warp's share: warp w takes [w * share, (w + 1) * share) of the line.
-__device__ __forceinline__ int int4_share(const Int4Attn& a, int total) { return max(1, ceil_div(total, a.warps)); }
+// The shares count n + 1 units for a pair (KV head and column block) of a row with n stages: entering it
+// (its queries read, its result written) takes a warp about as long as a stage.  Unit 0 of a pair is the
+// entry, unit i + 1 its stage i.  Warp w takes the units [w * share, (w + 1) * share).
+__device__ __forceinline__ int int4_share(const Int4Attn& a, int units) { return max(1, ceil_div(units, a.warps)); }
 
 constexpr float kInt4Log2e = 1.4426950408889634f;
 constexpr float kInt4Ln2 = 0.6931471805599453f;
@@ -164,11 +167,29 @@ __device__ __forceinline__ float scale_float(uint32_t pair, int i) {
   return i & 1 ? __high2float(bits_h2(pair)) : __low2float(bits_h2(pair));
 }
 
-// One stage: KT tokens at st, laid out like a page, the first of them key0.  kEdge: some column does not see
+// Where the 16-token tiles of a stage begin: a stage is `units` blocks of `unit` tokens, each laid out like
+// a page, so tile 2 i + j starts i * pair + j * one bytes after tile 0.
+struct Int4Tiles {
+  int row_one, row_pair;      // nibble rows
+  int scale_one, scale_pair;  // scales
+  int scales;                 // from a block's rows to its scales
+  int values;                 // from keys to values
+};
+__device__ __forceinline__ Int4Tiles int4_tiles(int unit, int row, int scale_row) {
+  const int block = 2 * unit * (row + scale_row);
+  return Int4Tiles{unit == 16 ? block : 16 * row,
+                   unit == 64 ? 32 * row : unit == 32 ? block : 2 * block,
+                   unit == 16 ? block : 16 * scale_row,
+                   unit == 64 ? 32 * scale_row : unit == 32 ? block : 2 * block,
+                   unit * row,
+                   block / 2};
+}
+
+// One stage: KT tokens at st, the first of them key0.  kEdge: some column does not see
 // all of them, or the split ends among them.
 template <bool kEdge, typename T, int DG, int NT, int KT>
-__device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsigned char* st, int key0,
-                                           int k_end) {
+__device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsigned char* st,
+                                           const Int4Tiles& at, int key0, int k_end) {
   using State = Int4State<T, DG, NT>;
   constexpr int D = DG * 32, NW = State::NW, kTiles = KT / 16, kRow = D / 2, kScaleRow = D / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -178,8 +199,15 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
   float s[NT][kTiles][4];
 #pragma unroll
   for (int tile = 0; tile < kTiles; ++tile) {
-    const unsigned char* kb = st + tile * 16 * kRow + t * (DG * 4);
-    const unsigned char* ks = st + KT * kRow + tile * 16 * kScaleRow;
+    if (kEdge && tile > 0 && key0 + tile * 16 >= k_end) {  // none of its keys exists
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][tile][e] = -INFINITY;
+      continue;
+    }
+    const unsigned char* kb = st + (tile >> 1) * at.row_pair + (tile & 1) * at.row_one + t * (DG * 4);
+    const unsigned char* ks = st + at.scales + (tile >> 1) * at.scale_pair + (tile & 1) * at.scale_one;
     uint32_t wa[DG], wb[DG];
     uint32_t ha[(DG + 1) / 2], hb[(DG + 1) / 2];
     lds_words<DG>(kb + tok_a * kRow, wa);
@@ -277,8 +305,9 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
   const int slot[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};
 #pragma unroll
   for (int tile = 0; tile < kTiles; ++tile) {
-    const unsigned char* vb = st + KT * (kRow + kScaleRow) + tile * 16 * kRow;
-    const unsigned char* vs = st + KT * (2 * kRow + kScaleRow) + tile * 16 * kScaleRow;
+    if (kEdge && tile > 0 && key0 + tile * 16 >= k_end) break;
+    const unsigned char* vb = st + at.values + (tile >> 1) * at.row_pair + (tile & 1) * at.row_one;
+    const unsigned char* vs = st + at.values + at.scales + (tile >> 1) * at.scale_pair + (tile & 1) * at.scale_one;
     uint32_t w[4][NW], sc[4][(NW + 1) / 2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -378,7 +407,7 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     for (int j = 0; j < 2; ++j) q.cs[nt][j] = __shfl_sync(0xffffffffu, unit, (2 * t + j) * 4);
     // B fragments: channels 32 gr + 8 t + {0,4}, {1,5}, {2,6}, {3,7} of column g
 #pragma unroll
-    for (int gr = 0; gr < DG; ++gr)
+    for (int gr = 0; gr < DG; ++gr) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float lo = x[gr][e] * up, hi = x[gr][e + 4] * up;
@@ -387,6 +416,7 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
         if constexpr (State::QP == 2)
           q.qf[1][nt][gr][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
       }
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int tok = min(col0 + nt * 8 + 2 * t + j, a.cols - 1) / a.group;
@@ -461,7 +491,7 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
 // share may begin and end inside a row: what it holds of such a row goes to one of the warp's two partial
 // slots, and attn_int4_combine merges them.  Each warp runs its own ring of bulk copies through its whole
 // share, the next row's first stages in flight while it finishes the last one; no block barrier runs
-// after the start.
+// between the start and the merge.
 template <typename T, int DG, int NT, int KT, int kStages, int kWarps, int kMinBlocks>
 __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(const __grid_constant__ Int4Attn a) {
   constexpr int D = DG * 32;
@@ -474,46 +504,60 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   int* first = reinterpret_cast<int*>(smem + kWarps * kStages * (kStageBytes + (int)sizeof(uint64_t)));
   const int pairs = a.p.kv_heads * a.col_blocks;
 
+  const int unit = min(1 << a.page_log2, KT), units = KT / unit;  // 1, 2 or 4
+  const Int4Tiles tiles = int4_tiles(unit, D / 2, D / 16);
   if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) ptx::mbar_init(&full[s], 1);
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(&full[s], units);
     ptx::fence_mbar_init();
   }
-  if (warp == 0) {  // first[b]: the stages of the rows before b
-    int carry = 0;
-    for (int b0 = 0; b0 < a.p.batch; b0 += 32) {
+  int* first_unit = first + a.p.batch + 1;
+  if (warp == 0) {  // stages and units of the rows before b
+    int stages = 0, rows = 0;
+    for (int b0 = 0; b0 <= a.p.batch; b0 += 32) {
       const int b = b0 + lane;
-      const int n = b < a.p.batch ? ceil_div(int4_len(a, b), KT) * pairs : 0;
-      int inc = n;
+      const int n = b < a.p.batch ? ceil_div(int4_len(a, b), KT) : 0;
+      int before = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int below = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += below;
+        const int below = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += below;
       }
-      if (b < a.p.batch) first[b] = carry + inc - n;
-      carry += __shfl_sync(0xffffffffu, inc, 31);
+      const uint32_t filled = __ballot_sync(0xffffffffu, n > 0);
+      const int at = (stages + before - n) * pairs, unit_at = at + (rows + __popc(filled & ((1u << lane) - 1))) * pairs;
+      if (b <= a.p.batch) {
+        first[b] = at;
+        first_unit[b] = unit_at;
+        if (blockIdx.x == 0) a.ws_first[b] = at, a.ws_first[a.p.batch + 1 + b] = unit_at;
+      }
+      stages += __shfl_sync(0xffffffffu, before, 31);
+      rows += __popc(filled);
     }
-    if (lane == 0) first[a.p.batch] = carry;
-    __syncwarp();
-    if (blockIdx.x == 0 && a.ws_first)
-      for (int b = lane; b <= a.p.batch; b += 32) a.ws_first[b] = first[b];
   }
   __syncthreads();
-  // Neighbouring shares go to different blocks, so a short line spreads over the SMs.
-  const int id = warp * gridDim.x + blockIdx.x;
-  const int total = first[a.p.batch], share = int4_share(a, total);
-  const int begin = (int)i64min((int64_t)id * share, total), mine = min(share, total - begin);
-  if (mine <= 0) return;
+  const int id = blockIdx.x * kWarps + warp;
+  const int total = first[a.p.batch], total_units = first_unit[a.p.batch], share = int4_share(a, total_units);
+  auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
+    int lo = 0, hi = a.p.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (starts[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  };
+  auto stages_before = [&](int64_t u) {  // of the units before u
+    if (u >= total_units) return total;
+    const int b = row_of(first_unit, (int)u);
+    const int n = (first_unit[b + 1] - first_unit[b]) / pairs, at = (int)u - first_unit[b], pair = at / n;
+    return first[b] + pair * (n - 1) + max(0, at - pair * n - 1);
+  };
+  const int begin = stages_before((int64_t)id * share), mine = stages_before((int64_t)(id + 1) * share) - begin;
 
   struct Place {  // of a stage: row, column block and KV head, stage of the row and their number
     int b, pair, st, n_st;
   };
   auto place = [&](int i) {
-    int lo = 0, hi = a.p.batch - 1;  // the last row whose first stage is not past i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
+    const int lo = row_of(first, i);
     Place p;
     p.b = lo;
     p.n_st = (first[lo + 1] - first[lo]) / pairs;
@@ -521,22 +565,18 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     p.st = i - first[lo] - p.pair * p.n_st;
     return p;
   };
+  // A block whose share lies within one row merges its warps' parts before they leave the SM.
+  const int block_begin = stages_before((int64_t)blockIdx.x * kWarps * share);
+  const int block_mine = stages_before((int64_t)(blockIdx.x + 1) * kWarps * share) - block_begin;
+  if (block_mine <= 0) return;
+  const Place home = place(block_begin);
+  const bool together = home.st + block_mine <= home.n_st;
 
-  // A stage in shared memory is laid out like a page of KT tokens, whatever the page size.  Lane 4 j + k
-  // fetches part k (keys, key scales, values, value scales) of its j-th `unit` tokens; where a page is a
-  // stage, lane 0 fetches it in one copy.  The addresses of the next 32 units are worked out by one lane
-  // each, so a stage costs a few shuffles.
-  const int unit = min(1 << a.page_log2, KT), units = KT / unit;  // units of a stage: 1, 2 or 4
-  const bool whole = (1 << a.page_log2) == KT;
-  const int part = whole ? 0 : lane & 3, my_unit = whole ? 0 : lane >> 2;
-  const bool fetches = whole ? lane == 0 : my_unit < units;
-  const int row_bytes = part & 1 ? D / 16 : D / 2;
-  const uint32_t bytes = whole ? kStageBytes : unit * row_bytes;
-  const uint32_t to = (part >> 1) * (kStageBytes / 2) + (part & 1) * KT * (D / 2) + my_unit * bytes;
-  const int part_at = (part >> 1) * (a.block_bytes / 2) + (part & 1) * ((D / 2) << a.page_log2);
-  const unsigned char* ahead = nullptr;  // block of this lane's unit, nullptr: none
-  int ahead_tok = 0;                     // the unit's first token in its page
-  uint32_t ahead_mask = 0;               // lanes that have one
+  // A stage is `units` whole pages, or part of one.  The sources of the next 32 units are worked out by one
+  // lane each; that lane then issues its copies: the page's block, or of a part the keys, key scales, values
+  // and value scales.
+  const unsigned char* ahead = nullptr;  // this lane's unit: its block in the pool, nullptr: none
+  int ahead_tok = 0;                     // its first token in the page
   auto look = [&](int n) {               // from stage n of the share on
     const int i = n + lane / units;
     ahead = nullptr;
@@ -554,27 +594,39 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
       }
     }
     __syncwarp();
-    ahead_mask = __ballot_sync(0xffffffffu, ahead != nullptr);
   };
   auto issue = [&](int n) {
     const int at = n * units & 31;
     if (at == 0) look(n);
-    unsigned char* dst = ring + (n % kStages) * kStageBytes;
-    uint64_t* bar = &full[n % kStages];
-    const int from = at + my_unit;
-    const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ahead), from & 31);
-    const int tok = whole ? 0 : __shfl_sync(0xffffffffu, ahead_tok, from & 31);
-    const uint32_t live = ahead_mask >> at & ((1u << units) - 1);
-    if (lane == 0) ptx::mbar_expect_tx(bar, __popc(live) * (kStageBytes / units));
-    __syncwarp();
-    if (fetches && src) ptx::bulk_g2s(dst + to, reinterpret_cast<const void*>(src + part_at + tok * row_bytes), bytes, bar);
+    const int u = lane - at;
+    if ((unsigned)u < (unsigned)units) {
+      unsigned char* dst = ring + (n % kStages) * kStageBytes;
+      uint64_t* bar = &full[n % kStages];
+      if (!ahead) {
+        ptx::mbar_arrive(bar);
+      } else if (unit == 1 << a.page_log2) {
+        ptx::mbar_expect_tx(bar, kStageBytes / units);
+        ptx::bulk_g2s(dst + u * (kStageBytes / units), ahead, kStageBytes / units, bar);
+      } else {
+        ptx::mbar_expect_tx(bar, kStageBytes);
+        const unsigned char* rows = ahead + ahead_tok * (D / 2);
+        const unsigned char* scales = ahead + ((D / 2) << a.page_log2) + ahead_tok * (D / 16);
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+          unsigned char* to = dst + kind * (kStageBytes / 2);
+          ptx::bulk_g2s(to, rows + kind * (a.block_bytes / 2), KT * (D / 2), bar);
+          ptx::bulk_g2s(to + KT * (D / 2), scales + kind * (a.block_bytes / 2), KT * (D / 16), bar);
+        }
+      }
+    }
   };
   int issued = 0;
   while (issued < min(mine, kStages - 1)) issue(issued++);
 
   Int4State<T, DG, NT> q;
+  bool ok = true;
   int n = 0;
-  while (n < mine) {
+  while (n < mine && ok) {
     const Place p = place(begin + n);
     const int len = int4_len(a, p.b), hk = p.pair / a.col_blocks, col0 = (p.pair - hk * a.col_blocks) * NT * 8;
     const int count = min(mine - n, p.n_st - p.st);
@@ -584,80 +636,158 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     int key0 = p.st * KT;
     for (int k = 0; k < count; ++k, ++n, key0 += KT) {
       if (issued < mine) issue(issued++);
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[n % kStages], (n / kStages) & 1, a.fault, FAULT_DEC_FULL))) {
-        // let the copies that are still in flight land before the block ends
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&full[n % kStages], (n / kStages) & 1, a.fault, FAULT_DEC_FULL));
+      if (!ok) {  // let the copies that are still in flight land before the block ends
         for (int s = n + 1; s < issued; ++s)
           ptx::mbar_wait(&full[s % kStages], (s / kStages) & 1, a.fault, FAULT_DEC_FULL);
-        return;
+        break;
       }
       const unsigned char* st = ring + (n % kStages) * kStageBytes;
       if (key0 + KT <= plain)
-        int4_stage<false, T, DG, NT, KT>(q, st, key0, len);
+        int4_stage<false, T, DG, NT, KT>(q, st, tiles, key0, len);
       else
-        int4_stage<true, T, DG, NT, KT>(q, st, key0, len);
+        int4_stage<true, T, DG, NT, KT>(q, st, tiles, key0, len);
       __syncwarp();  // every lane is done with the stage before it is filled again
     }
-    int4_store(a, q, p.b, hk, col0, count == p.n_st ? -1 : 2 * id + (n == count ? 0 : 1));
+    if (ok && !together)
+      int4_store(a, q, p.b, hk, col0, count == p.n_st ? -1 : 2 * id + (n == count ? 0 : 1));
+  }
+  if (!together) return;
+
+  // Merge through shared memory, over the rings: warp w's columns behind those of the warps before it.
+  constexpr int kCols = NT * 8, kPad = D + 4, NW = Int4State<T, DG, NT>::NW;
+  float* red = reinterpret_cast<float*>(smem);
+  float2* ml = reinterpret_cast<float2*>(red + kWarps * kCols * kPad);
+  const int g = lane >> 2, t = lane & 3;
+  if (!__syncthreads_and(ok)) return;
+  if (mine <= 0) {
+    for (int i = lane; i < kCols; i += 32) ml[warp * kCols + i] = make_float2(-INFINITY, 0.f);
+  } else {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = q.l[nt][j];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int col = warp * kCols + nt * 8 + 2 * t + j;
+        if (g == 0) ml[col] = make_float2(q.m[nt][j], sum);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const int word = g * NW + w, ch = 32 * (word % DG) + 8 * (word / DG);
+          if (DG % 2 && word >= D / 8) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) red[col * kPad + ch + e] = q.acc[nt][4 * w + e / 2][j + 2 * (e & 1)];
+        }
+      }
+  }
+  __syncthreads();
+  const int hk = home.pair / a.col_blocks, col0 = (home.pair - hk * a.col_blocks) * NT * 8;
+  const bool all = block_mine == home.n_st;
+  for (int i = threadIdx.x; i < min(kCols, a.cols - col0) * D; i += kWarps * 32) {
+    const int col = i / D, d = i - col * D;
+    float top = -INFINITY, sum = 0.f, out = 0.f;
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * kCols + col].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 x = ml[w * kCols + col];
+      if (x.x == -INFINITY && x.y == 0.f) continue;  // nothing there
+      const float f = ptx::ex2(x.x - base);
+      sum += x.y * f;
+      out += red[(w * kCols + col) * kPad + d] * f;
+    }
+    const int tok = (col0 + col) / a.group, h = hk * a.group + col0 + col - tok * a.group;
+    if (all) {
+      int4_out_row<T>(a, home.b, h, tok)[d * a.p.o.stride[3]] = Elem<T>::from_acc(sum == 0.f ? 0.f : out / sum);
+      if (d == 0) int4_store_lse(a, home.b, h, tok, top - 7.f, sum);
+    } else {
+      const int64_t slot = (int64_t)2 * blockIdx.x * kWarps * a.slot_cols + col;
+      a.ws_acc[slot * D + d] = out;
+      if (d == 0) reinterpret_cast<float2*>(a.ws_ml)[slot] = make_float2(top, sum);
+    }
   }
 }
 
-constexpr int kInt4CombineThreads = 256;
-
-// One block an output row.  Rows without keys become zeros; a row that one warp saw whole is done; of the
-// others the block's warps take every eighth partial, a lane D / 32 of the channels.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kInt4CombineThreads) attn_int4_combine(const __grid_constant__ Int4Attn a) {
-  constexpr int kWarps = kInt4CombineThreads / 32;
-  __shared__ float part[kWarps][256];
-  __shared__ float sums[kWarps];
-  const int64_t row = blockIdx.x;
+// A warp (or, with few rows and many parts of each, a block) merges an output row; rows without keys become
+// zeros, and a row that was written whole is left alone.
+template <typename T, int NT, int kWarps>
+__global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__ Int4Attn a, int row_warps) {
+  __shared__ float part[8][256];
+  __shared__ float2 part_ml[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
+  const int64_t row = (int64_t)blockIdx.x * (8 / row_warps) + warp / row_warps;
+  const int sub = warp % row_warps;
+  if (row >= rows) return;  // row_warps is 1 or 8: a whole block or single warps
   const int tok = (int)(row % a.p.q_len), h = (int)(row / a.p.q_len % a.p.q_heads);
   const int b = (int)(row / ((int64_t)a.p.q_len * a.p.q_heads));
   const int hk = h / a.group, col = tok * a.group + h - hk * a.group;
   const int pairs = a.p.kv_heads * a.col_blocks, pair = hk * a.col_blocks + col / (NT * 8), local = col % (NT * 8);
-  const int total = a.ws_first[a.p.batch], row_first = a.ws_first[b];
-  const int n_st = (a.ws_first[b + 1] - row_first) / pairs;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = a.p.head_dim / 32;
-  float o = 0.f, l = 0.f, top = -INFINITY;
-  if (n_st) {
-    const int begin = row_first + pair * n_st, last = begin + n_st - 1;
-    const int share = int4_share(a, total), w0 = begin / share, w1 = last / share;
-    if (w0 == w1) return;
-    const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + local;
-    auto slot = [&](int w) {  // where warp w left its part of the row
-      return (int64_t)(2 * w + ((int64_t)w * share < begin)) * a.slot_cols;
+  const int32_t* first_unit = a.ws_first + a.p.batch + 1;
+  const int total = first_unit[a.p.batch], row_first = first_unit[b];
+  const int n = (first_unit[b + 1] - row_first) / pairs;  // units of a pair: one more than its stages
+  const int groups = a.p.head_dim / 32;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  float out[8] = {};
+  if (n) {
+    const int enter = row_first + pair * n;  // the pair's stages are the units enter + 1 .. enter + n - 1
+    const int share = int4_share(a, total), w0 = (enter + 1) / share, w1 = (enter + n - 1) / share;
+    const int c0 = w0 / kWarps, c1 = w1 / kWarps;
+    auto merged = [&](int c) {  // no stage of the block's share is another pair's (the next one's entry may be)
+      return (int64_t)c * kWarps * share >= enter &&
+             i64min((int64_t)(c + 1) * kWarps * share, total) <= (int64_t)enter + n + 1;
     };
-    for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, ml[slot(w)].x);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float base = top == -INFINITY ? 0.f : top;
-    float out[8] = {}, sum = 0.f;
+    const bool m0 = merged(c0), m1 = merged(c1);
+    if (w0 == w1 || (c0 == c1 && m0)) return;
+    // The row's parts: of the first block's warps, of the blocks that merged theirs, of the last block's warps.
+    const int head = m0 ? 0 : min(w1, c0 * kWarps + kWarps - 1) - w0 + 1;
+    const int lo = m0 ? c0 : c0 + 1, mid = max(0, (m1 ? c1 : c1 - 1) - lo + 1);
+    const int tail = c1 != c0 && !m1 ? w1 - c1 * kWarps + 1 : 0;
+    auto slot = [&](int i) {
+      const int w = i < head ? w0 + i : i < head + mid ? (lo + i - head) * kWarps : c1 * kWarps + i - head - mid;
+      return (int64_t)(2 * w + ((int64_t)w * share < enter)) * a.slot_cols + local;
+    };
+    const float2* all_ml = reinterpret_cast<const float2*>(a.ws_ml);
 #pragma unroll 4
-    for (int w = w0 + warp; w <= w1; w += kWarps) {
-      const int64_t s = slot(w);
-      const float2 x = ml[s];
-      const float f = ptx::ex2(x.x - base);
-      sum += x.y * f;
-      const float* acc = a.ws_acc + (s + local) * a.p.head_dim + lane;
+    for (int i = sub; i < head + mid + tail; i += row_warps) {
+      const int64_t s = slot(i);
+      const float2 x = all_ml[s];
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < groups) out[k] = fmaf(acc[k * 32], f, out[k]);
-    }
+      for (int k = 0; k < 8; ++k) v[k] = k < groups ? a.ws_acc[s * a.p.head_dim + k * 32 + lane] : 0.f;
+      const float top = fmaxf(ml.x, x.x), base = top == -INFINITY ? 0.f : top;
+      const float f0 = ptx::ex2(ml.x - base), f1 = ptx::ex2(x.x - base);
+      ml = make_float2(top, ml.y * f0 + x.y * f1);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = out[k];
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x < a.p.head_dim) {
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        o += part[w][threadIdx.x];
-        l += sums[w];
-      }
+      for (int k = 0; k < 8; ++k) out[k] = out[k] * f0 + v[k] * f1;
     }
   }
-  if (threadIdx.x >= a.p.head_dim) return;
-  int4_out_row<T>(a, b, h, tok)[threadIdx.x * a.p.o.stride[3]] = Elem<T>::from_acc(l == 0.f ? 0.f : o / l);
-  if (threadIdx.x == 0) int4_store_lse(a, b, h, tok, top - 7.f, l);
+  if (row_warps > 1) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = out[k];
+    if (lane == 0) part_ml[warp] = ml;
+    __syncthreads();
+    if (warp > 0) return;
+    float top = -INFINITY;
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, part_ml[w].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    ml = make_float2(top, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) out[k] = 0.f;
+    for (int w = 0; w < 8; ++w) {
+      const float f = ptx::ex2(part_ml[w].x - base);
+      ml.y += part_ml[w].y * f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) out[k] += part[w][k * 32 + lane] * f;
+    }
+  }
+  T* o = int4_out_row<T>(a, b, h, tok);
+  const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < groups) o[(k * 32 + lane) * a.p.o.stride[3]] = Elem<T>::from_acc(out[k] * inv);
+  if (lane == 0) int4_store_lse(a, b, h, tok, ml.x - 7.f, ml.y);
 }
 
 // Shape of the kernel that takes a problem.

@@ -9,16 +9,20 @@ constexpr int kInt4Warps = 4;
 
 template <typename T, int DG, int NT, int KT, int kMinBlocks>
 static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
-  constexpr size_t ring =
-      (size_t)kInt4Warps * kInt4Stages * (2 * KT * (DG * 16 + DG * 2) + sizeof(uint64_t));
-  const size_t smem = ring + (size_t)(a.p.batch + 1) * sizeof(int);
+  constexpr int D = DG * 32;
+  const size_t ring = (size_t)kInt4Warps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t)) +
+                      (size_t)2 * (a.p.batch + 1) * sizeof(int);
+  constexpr size_t merge = (size_t)kInt4Warps * NT * 8 * (D + 4 + 2) * sizeof(float);
+  const size_t smem = ring > merge ? ring : merge;
   auto kernel = attn_int4_kernel<T, DG, NT, KT, kInt4Stages, kInt4Warps, kMinBlocks>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   kernel<<<blocks, kInt4Warps * 32, smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  attn_int4_combine<T, NT><<<(unsigned)((int64_t)a.p.batch * a.p.q_heads * a.p.q_len), kInt4CombineThreads, 0, st>>>(a);
+  const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
+  const int row_warps = a.parts > 8 ? 8 : 1;  // warps that merge one row
+  attn_int4_combine<T, NT, kInt4Warps><<<(unsigned)((rows * row_warps + 7) / 8), 256, 0, st>>>(a, row_warps);
   return cudaGetLastError();
 }
 
