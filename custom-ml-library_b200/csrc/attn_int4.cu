@@ -4,8 +4,6 @@
 namespace tsa {
 
 namespace {
-constexpr int kMaxRows = 2048;  // rows of one launch: their prefix sums sit in shared memory
-
 int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
@@ -26,12 +24,14 @@ int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
   a.cols = a.group * p.q_len;
   a.col_blocks = ceil_div(a.cols, shape.nt * 8);
   a.slot_cols = a.cols < shape.nt * 8 ? a.cols : shape.nt * 8;
+  const int rows = p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows;
+  const int64_t pairs = (int64_t)rows * p.kv_heads * a.col_blocks;
+  a.by_pair = shape.by_pair;
   // One wave of blocks that fill the GPU, fewer where a warp would be left without a stage.
-  const int rows = p.batch < kMaxRows ? p.batch : kMaxRows;
-  const int64_t most = (int64_t)rows * p.kv_heads * a.col_blocks * ceil_div(p.kv_len, shape.keys);
-  const int blocks = (int)i64min(most, (int64_t)sm_count() * shape.blocks);
+  const int blocks = a.by_pair ? (int)pairs
+                               : (int)i64min(pairs * ceil_div(p.kv_len, shape.keys), (int64_t)sm_count() * shape.blocks);
   a.warps = blocks * shape.warps;
-  a.parts = (int)(blocks / i64max(1, (int64_t)rows * p.kv_heads * a.col_blocks));
+  a.parts = (int)(blocks / pairs);
   return blocks;
 }
 
@@ -49,16 +49,21 @@ bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c) {
 // D = 128; a second tile of wider rows or of fp32's two query parts does not fit the registers).
 Int4Shape int4_shape(const ts_attn_params& p) {
   const int64_t cols = (int64_t)(p.q_heads / p.kv_heads) * p.q_len;
-  if (p.head_dim > 128) return {1, 32, 4, 2};
-  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2};
-  return {1, 64, 4, 3};
+  const bool by_pair64 = p.kv_len <= 4 * 64;
+  if (p.head_dim > 128) return {1, 32, 4, 2, p.kv_len <= 4 * 32};
+  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2, by_pair64};
+  // Stages of 16 tokens where those of 64 would leave most warps without one.
+  const int64_t stages = (int64_t)p.batch * p.kv_heads * ((cols + 7) / 8) * ceil_div(p.kv_len, 64);
+  if (p.kv_len <= 64 || stages <= 148 * 3) return {1, 16, 4, 3, p.kv_len <= 4 * 16};
+  return {1, 64, 4, 3, by_pair64};
 }
 
 size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
   Int4Attn a;
   Int4Shape shape;
   plan(p, a, shape);
-  const int rows = p.batch < kMaxRows ? p.batch : kMaxRows;
+  if (a.by_pair) return 0;
+  const int rows = p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows;
   return partial_bytes(a, p.head_dim) + (size_t)2 * (rows + 1) * sizeof(int32_t);
 }
 
@@ -66,29 +71,30 @@ cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, vo
                               uint32_t* fault, cudaStream_t st) {
   Int4Attn a;
   Int4Shape shape;
-  const int blocks = plan(p, a, shape);
+  int blocks = plan(p, a, shape);
   if (ws_bytes < attn_int4_workspace(p, c)) return cudaErrorInvalidValue;
   a.p = p;
   a.c = c;
   a.page_log2 = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : 6;
   a.block_bytes = int4_block_bytes(p.head_dim, c.page_size);
   a.ws_acc = reinterpret_cast<float*>(ws);
-  a.ws_ml = a.ws_acc + (size_t)2 * a.warps * a.slot_cols * p.head_dim;
-  a.ws_first = reinterpret_cast<int32_t*>(a.ws_ml + (size_t)2 * a.warps * a.slot_cols * 2);
+  a.ws_ml = a.by_pair ? nullptr : a.ws_acc + (size_t)2 * a.warps * a.slot_cols * p.head_dim;
+  a.ws_first = a.by_pair ? nullptr : reinterpret_cast<int32_t*>(a.ws_ml + (size_t)2 * a.warps * a.slot_cols * 2);
   a.fault = fault;
   const int size = p.dtype == TS_F32 ? 4 : 2;
   a.q_vec = rows_vec(p.q, size);
   a.o_vec = rows_vec(p.o, size);
-  if ((int64_t)(p.batch < kMaxRows ? p.batch : kMaxRows) * p.q_heads * p.q_len > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  for (int row = 0; row < p.batch; row += kMaxRows) {  // launches follow one another on the stream
+  if ((int64_t)(p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows) * p.q_heads * p.q_len > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  for (int row = 0; row < p.batch; row += kInt4MaxRows) {  // launches follow one another on the stream
     Int4Attn part = a;
-    part.p.batch = p.batch - row < kMaxRows ? p.batch - row : kMaxRows;
+    part.p.batch = p.batch - row < kInt4MaxRows ? p.batch - row : kInt4MaxRows;
     part.p.q.data = reinterpret_cast<unsigned char*>(p.q.data) + row * p.q.stride[0] * size;
     part.p.o.data = reinterpret_cast<unsigned char*>(p.o.data) + row * p.o.stride[0] * size;
     if (p.lse) part.p.lse = reinterpret_cast<float*>(p.lse) + row * p.lse_stride[0];
     part.p.kv_lens = p.kv_lens + row;
     part.c.table = c.table + row * c.table_stride;
     cudaError_t e = cudaErrorInvalidValue;
+    if (a.by_pair) blocks = part.p.batch * p.kv_heads * a.col_blocks;
     switch (p.dtype) {
       case TS_BF16: e = attn_int4_launch<__nv_bfloat16>(part, shape, blocks, st); break;
       case TS_F16: e = attn_int4_launch<__half>(part, shape, blocks, st); break;

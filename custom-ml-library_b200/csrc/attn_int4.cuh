@@ -28,10 +28,13 @@
 
 #include <type_traits>
 
+#include "dependent.cuh"
 #include "int4.cuh"
 #include "ptx.cuh"
 
 namespace tsa {
+
+constexpr int kInt4MaxRows = 2048;  // rows of one launch: their prefix sums sit in shared memory
 
 struct Int4Attn {
   ts_attn_params p;
@@ -42,6 +45,7 @@ struct Int4Attn {
   int col_blocks;  // blocks of columns; one warp holds one at a time
   int slot_cols;   // columns of a block that can be live
   int warps;       // that share the work
+  bool by_pair;    // one block a (row, KV head, column block) instead of equal shares
   int parts;       // about how many blocks share a row at the longest length
   bool q_vec, o_vec;  // rows of unit stride and 16-byte alignment
   float* ws_acc;   // [2 * warps, slot_cols, D] partial results
@@ -489,7 +493,8 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
 // The work is a line of stages of KT tokens, ordered by (row, KV head, column block, key); rows differ in
 // length, so every warp takes an equal share of the line instead of whole rows or splits of one size.  A
 // share may begin and end inside a row: what it holds of such a row goes to one of the warp's two partial
-// slots, and attn_int4_combine merges them.  Each warp runs its own ring of bulk copies through its whole
+// slots, and attn_int4_combine merges them.  (Where a pair has at most one stage for each warp of a block,
+// by_pair gives every pair a block of its own: nothing is left to merge, so the second launch falls away.)  Each warp runs its own ring of bulk copies through its whole
 // share, the next row's first stages in flight while it finishes the last one; no block barrier runs
 // between the start and the merge.
 template <typename T, int DG, int NT, int KT, int kStages, int kWarps, int kMinBlocks>
@@ -511,7 +516,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     ptx::fence_mbar_init();
   }
   int* first_unit = first + a.p.batch + 1;
-  if (warp == 0) {  // stages and units of the rows before b
+  let_next_start();
+  if (warp == 0 && !a.by_pair) {  // stages and units of the rows before b
     int stages = 0, rows = 0;
     for (int b0 = 0; b0 <= a.p.batch; b0 += 32) {
       const int b = b0 + lane;
@@ -535,7 +541,13 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   }
   __syncthreads();
   const int id = blockIdx.x * kWarps + warp;
-  const int total = first[a.p.batch], total_units = first_unit[a.p.batch], share = int4_share(a, total_units);
+  struct Place {  // of a stage: row, column block and KV head, stage of the pair and their number
+    int b, pair, st, n_st;
+  };
+  Place home;       // of the block's first stage
+  int begin, mine;  // this warp's first stage and their number
+  int block_mine;   // the block's
+  int share = 0, total = 0, total_units = 0;
   auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
     int lo = 0, hi = a.p.batch - 1;
     while (lo < hi) {
@@ -551,25 +563,39 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     const int n = (first_unit[b + 1] - first_unit[b]) / pairs, at = (int)u - first_unit[b], pair = at / n;
     return first[b] + pair * (n - 1) + max(0, at - pair * n - 1);
   };
-  const int begin = stages_before((int64_t)id * share), mine = stages_before((int64_t)(id + 1) * share) - begin;
-
-  struct Place {  // of a stage: row, column block and KV head, stage of the row and their number
-    int b, pair, st, n_st;
-  };
   auto place = [&](int i) {
-    const int lo = row_of(first, i);
     Place p;
-    p.b = lo;
-    p.n_st = (first[lo + 1] - first[lo]) / pairs;
-    p.pair = (i - first[lo]) / p.n_st;
-    p.st = i - first[lo] - p.pair * p.n_st;
+    if (a.by_pair) {
+      p = home;
+      p.st = i;
+      return p;
+    }
+    p.b = row_of(first, i);
+    p.n_st = (first[p.b + 1] - first[p.b]) / pairs;
+    p.pair = (i - first[p.b]) / p.n_st;
+    p.st = i - first[p.b] - p.pair * p.n_st;
     return p;
   };
-  // A block whose share lies within one row merges its warps' parts before they leave the SM.
-  const int block_begin = stages_before((int64_t)blockIdx.x * kWarps * share);
-  const int block_mine = stages_before((int64_t)(blockIdx.x + 1) * kWarps * share) - block_begin;
-  if (block_mine <= 0) return;
-  const Place home = place(block_begin);
+  if (a.by_pair) {
+    home.b = blockIdx.x / pairs;
+    home.pair = blockIdx.x - home.b * pairs;
+    home.st = 0;
+    home.n_st = block_mine = ceil_div(int4_len(a, home.b), KT);
+    share = ceil_div(block_mine, kWarps);
+    begin = min(warp * share, block_mine);
+    mine = min(share, block_mine - begin);
+  } else {
+    total = first[a.p.batch];
+    total_units = first_unit[a.p.batch];
+    share = int4_share(a, total_units);
+    begin = stages_before((int64_t)id * share);
+    mine = stages_before((int64_t)(id + 1) * share) - begin;
+    const int block_begin = stages_before((int64_t)blockIdx.x * kWarps * share);
+    block_mine = stages_before((int64_t)(blockIdx.x + 1) * kWarps * share) - block_begin;
+    if (block_mine <= 0) return;
+    home = place(block_begin);
+  }
+  // A block whose share lies within one pair merges its warps' parts before they leave the SM.
   const bool together = home.st + block_mine <= home.n_st;
 
   // A stage is `units` whole pages, or part of one.  The sources of the next 32 units are worked out by one
@@ -715,6 +741,7 @@ template <typename T, int NT, int kWarps>
 __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__ Int4Attn a, int row_warps) {
   __shared__ float part[8][256];
   __shared__ float2 part_ml[8];
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
   const int64_t row = (int64_t)blockIdx.x * (8 / row_warps) + warp / row_warps;
@@ -796,6 +823,7 @@ struct Int4Shape {
   int keys;    // tokens of a stage
   int warps;   // of a block
   int blocks;  // resident on an SM
+  bool by_pair;
 };
 Int4Shape int4_shape(const ts_attn_params& p);
 

@@ -1,6 +1,7 @@
 // Launch of the attention kernels over a 4-bit cache for one element type.
 #pragma once
 #include "attn_int4.cuh"
+#include "tc_util.cuh"
 
 namespace tsa {
 
@@ -10,20 +11,21 @@ constexpr int kInt4Warps = 4;
 template <typename T, int DG, int NT, int KT, int kMinBlocks>
 static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
   constexpr int D = DG * 32;
-  const size_t ring = (size_t)kInt4Warps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t)) +
-                      (size_t)2 * (a.p.batch + 1) * sizeof(int);
+  constexpr size_t ring = (size_t)kInt4Warps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t));
   constexpr size_t merge = (size_t)kInt4Warps * NT * 8 * (D + 4 + 2) * sizeof(float);
-  const size_t smem = ring > merge ? ring : merge;
+  constexpr size_t most = ring + (size_t)2 * (kInt4MaxRows + 1) * sizeof(int);
+  const size_t need = ring + (a.by_pair ? 0 : (size_t)2 * (a.p.batch + 1) * sizeof(int));
+  const size_t smem = need > merge ? need : merge;
   auto kernel = attn_int4_kernel<T, DG, NT, KT, kInt4Stages, kInt4Warps, kMinBlocks>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), (int)(most > merge ? most : merge));
   if (e != cudaSuccess) return e;
   kernel<<<blocks, kInt4Warps * 32, smem, st>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || a.by_pair) return e;
   const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
   const int row_warps = a.parts > 8 ? 8 : 1;  // warps that merge one row
-  attn_int4_combine<T, NT, kInt4Warps><<<(unsigned)((rows * row_warps + 7) / 8), 256, 0, st>>>(a, row_warps);
-  return cudaGetLastError();
+  return launch_dependent(attn_int4_combine<T, NT, kInt4Warps>, dim3((unsigned)((rows * row_warps + 7) / 8)), dim3(256),
+                          0, st, a, row_warps);
 }
 
 template <typename T>
@@ -39,6 +41,15 @@ cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int bloc
       }
       return cudaErrorInvalidValue;
     }
+  }
+  if (shape.keys == 16) {
+    switch (groups) {
+      case 1: return int4_run<T, 1, 1, 16, 3>(a, blocks, st);
+      case 2: return int4_run<T, 2, 1, 16, 3>(a, blocks, st);
+      case 3: return int4_run<T, 3, 1, 16, 3>(a, blocks, st);
+      case 4: return int4_run<T, 4, 1, 16, 3>(a, blocks, st);
+    }
+    return cudaErrorInvalidValue;
   }
   switch (groups) {
     case 1: return int4_run<T, 1, 1, 64, 3>(a, blocks, st);

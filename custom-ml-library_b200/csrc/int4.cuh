@@ -34,12 +34,6 @@ __device__ __forceinline__ float int4_scale(float amax) {
   return fminf(fmaxf(up, kInt4ScaleMin), kInt4ScaleMax);
 }
 
-// Nibble of x for a scale made by int4_scale; NaN -> 8 (the value 0).
-__device__ __forceinline__ uint32_t int4_nibble(float x, float scale) {
-  const int n = __float2int_rn(fminf(fmaxf(__fdiv_rn(x, scale), -7.f), 7.f));
-  return (uint32_t)((x == x ? n : 0) + 8);
-}
-
 // Page of row b's token, or -1 where the table has none (a bad entry is the caller's error: the
 // kernels record it in the fault word and leave the page alone).
 __device__ __forceinline__ int int4_page(const ts_kv4_cache& c, int b, int slot) {

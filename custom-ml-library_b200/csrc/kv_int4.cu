@@ -1,6 +1,10 @@
 // Quantising append into the pages of a 4-bit KV cache, and the read-back of its values.
 // Both move each value once: 16 bits in and 4.5 out (the append), 4.5 in and 16 out (the gather),
 // so HBM, or for a token of each row the launch, bounds them.
+//
+// One thread owns a stored word (8 channels of K or V of one head) and walks over a block's tokens, four of
+// them in flight: 64 bytes a thread for half types, which is what covers the memory latency.  The four
+// neighbouring threads of a scale group share its maximum by two shuffles.
 #include "int4.cuh"
 
 namespace tsa {
@@ -14,116 +18,184 @@ struct Int4Rows {
   int32_t* positions_out;
   const int32_t* lens;
   uint32_t* fault;
-  bool vec;  // unit channel stride, 16-byte aligned rows
+  bool vec;          // unit channel stride, 16-byte aligned rows
+  int page_log2;
+  int tokens;        // of a block
+  int token_blocks;  // blocks of a row
+};
+
+constexpr int kInFlight = 4;
+
+template <typename T>
+struct Raw8 {
+  alignas(16) T x[8];
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, int64_t stride, bool vec, float (&x)[8]) {
+__device__ __forceinline__ void load8(const T* src, int64_t stride, bool vec, Raw8<T>& r) {
   if (vec) {
-    alignas(16) T raw[8];
 #pragma unroll
     for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-      reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(src)[i];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_acc(raw[e]);
+      reinterpret_cast<uint4*>(r.x)[i] = reinterpret_cast<const uint4*>(src)[i];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_acc(src[e * stride]);
+    for (int e = 0; e < 8; ++e) r.x[e] = src[e * stride];
   }
 }
 
-// One block a (row, token); one thread 8 channels (a stored word) of a K or V row, so the four
-// neighbouring threads of a scale group share its maximum by two shuffles.
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, int64_t stride, bool vec, const Raw8<T>& r) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(r.x)[i];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dst[e * stride] = r.x[e];
+  }
+}
+
+// The larger, or NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The word of 8 channels whose group has the finite maximum amax <= 7 * kInt4ScaleMax, so that no quotient
+// passes 7.  fp32 inputs divide; half types multiply by the reciprocal and correct the quotient once with its
+// remainder (Markstein, IBM J. Res. Dev. 34, 1990), which yields the same correctly rounded quotient at a
+// third of the instructions.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float scale) {
+  const float inv = __frcp_rn(scale);
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float n;
+    if constexpr (sizeof(T) == 4) {
+      n = __fdiv_rn(x[e], scale);
+    } else {
+      n = x[e] * inv;
+      n = fmaf(fmaf(-n, scale, x[e]), inv, n);
+    }
+    // round half to even and add 8, by a sum whose last place is 1: 1.5 * 2^23 + 8
+    word |= (__float_as_uint(n + 12582920.f) & 15u) << (4 * e);
+  }
+  return word;
+}
+
 template <typename T>
 __global__ void kv_append_int4_kernel(Int4Rows a) {
   const ts_kv4_cache& c = a.c;
-  const int b = blockIdx.x / a.steps, t = blockIdx.x - b * a.steps;
-  const int64_t pos = (a.positions ? (int64_t)a.positions[b] : a.position) + t;
+  const int b = blockIdx.x / a.token_blocks, t0 = (blockIdx.x - b * a.token_blocks) * a.tokens;
+  const int t1 = min(a.steps, t0 + a.tokens);
   const int chunks = c.head_dim / 8, groups = c.head_dim / 32;
-  const int64_t slot = pos / c.page_size;
-  const int page = pos < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
-  if (t == 0 && threadIdx.x == 0 && a.positions_out) a.positions_out[b] = (int32_t)(pos + a.steps);
-  if (page < 0) {
-    if (threadIdx.x == 0) record_fault(a.fault, FAULT_PAGE);
-    return;
-  }
-  const int at = (int)(pos - slot * c.page_size);
-  const int block = int4_block_bytes(c.head_dim, c.page_size);
   const int items = c.kv_heads * 2 * chunks;  // a multiple of 4
-  for (int i = threadIdx.x; i < items; i += blockDim.x) {
-    const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
-    const ts_view4& v = kind ? a.value : a.key;
-    const T* src = reinterpret_cast<const T*>(v.data) + b * v.stride[0] + h * v.stride[1] + t * v.stride[2] +
-                   (int64_t)chunk * 8 * v.stride[3];
-    float x[8];
-    load8(src, v.stride[3], a.vec, x);
-    float amax = 0.f;
+  const int i = blockIdx.y * blockDim.x + threadIdx.x;
+  const int64_t pos = a.positions ? (int64_t)a.positions[b] : a.position;
+  if (t0 == 0 && i == 0 && a.positions_out) a.positions_out[b] = (int32_t)(pos + a.steps);
+  if (i >= items) return;
+  const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
+  const int g = chunk / 4, w = chunk % 4 * groups + g;
+  const int64_t block = int4_block_bytes(c.head_dim, c.page_size);
+  const ts_view4& v = kind ? a.value : a.key;
+  const T* src = reinterpret_cast<const T*>(v.data) + b * v.stride[0] + h * v.stride[1] +
+                 (int64_t)chunk * 8 * v.stride[3];
+  unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + h * block + kind * (block / 2);
+  const uint32_t quad = 0xFu << (threadIdx.x & 28);
+  for (int t = t0; t < t1; t += kInFlight) {
+    Raw8<T> raw[kInFlight];
+    int page[kInFlight];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    const uint32_t quad = 0xFu << (threadIdx.x & 28);
-    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-    const float scale = int4_scale(amax);
-    uint32_t word = 0;
+    for (int u = 0; u < kInFlight; ++u) {
+      if (t + u >= t1) break;
+      load8(src + (int64_t)(t + u) * v.stride[2], v.stride[3], a.vec, raw[u]);
+      const int64_t slot = (pos + t + u) >> a.page_log2;
+      page[u] = slot < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) word |= int4_nibble(x[e], scale) << (4 * e);
-    unsigned char* dst = reinterpret_cast<unsigned char*>(c.pool) + page * c.page_stride + (int64_t)h * block +
-                         kind * (block / 2);
-    const int g = chunk / 4, w = chunk % 4 * groups + g;
-    reinterpret_cast<uint32_t*>(dst + (int64_t)at * (c.head_dim / 2))[w] = word;
-    if (chunk % 4 == 0)
-      reinterpret_cast<__half*>(dst + c.page_size * (c.head_dim / 2))[at * groups + g] = __float2half_rn(scale);
+    for (int u = 0; u < kInFlight; ++u) {
+      if (t + u >= t1) break;
+      float x[8], amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = Elem<T>::to_acc(raw[u].x[e]);
+        amax = max_nan(amax, fabsf(x[e]));
+      }
+      amax = max_nan(amax, __shfl_xor_sync(quad, amax, 1));
+      amax = max_nan(amax, __shfl_xor_sync(quad, amax, 2));
+      if (!(amax <= 7.f * kInt4ScaleMax)) {  // saturate, NaN to 0
+        amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -7.f * kInt4ScaleMax), 7.f * kInt4ScaleMax) : 0.f;
+          amax = fmaxf(amax, fabsf(x[e]));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+      }
+      const float scale = int4_scale(amax);
+      const uint32_t word = quantise8<T>(x, scale);
+      if (page[u] < 0) {
+        record_fault(a.fault, FAULT_PAGE);
+        continue;
+      }
+      const int at = (int)((pos + t + u) & (c.page_size - 1));
+      unsigned char* dst = base + page[u] * c.page_stride;
+      reinterpret_cast<uint32_t*>(dst + (int64_t)at * (c.head_dim / 2))[w] = word;
+      if (chunk % 4 == 0)
+        reinterpret_cast<__half*>(dst + c.page_size * (c.head_dim / 2))[at * groups + g] = __float2half_rn(scale);
+    }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* dst, int64_t stride, bool vec, const float (&x)[8]) {
-  if (vec) {
-    alignas(16) T raw[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) raw[e] = Elem<T>::from_acc(x[e]);
-#pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(raw)[i];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dst[e * stride] = Elem<T>::from_acc(x[e]);
-  }
-}
-
-// The same split as the append: one block a (row, token), one thread a word.
 template <typename T>
 __global__ void kv_gather_int4_kernel(Int4Rows a) {
   const ts_kv4_cache& c = a.c;
-  const int b = blockIdx.x / a.steps, t = blockIdx.x - b * a.steps;
-  const int64_t pos = (a.positions ? (int64_t)a.positions[b] : 0) + t;
+  const int b = blockIdx.x / a.token_blocks, t0 = (blockIdx.x - b * a.token_blocks) * a.tokens;
+  const int t1 = min(a.steps, t0 + a.tokens);
   const int chunks = c.head_dim / 8, groups = c.head_dim / 32;
-  const int64_t slot = pos / c.page_size;
-  const bool past = a.lens && pos >= a.lens[b];
-  const int page = past || pos < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
-  if (page < 0 && !past && threadIdx.x == 0) record_fault(a.fault, FAULT_PAGE);
-  const int at = (int)(pos - slot * c.page_size);
-  const int block = int4_block_bytes(c.head_dim, c.page_size);
   const int items = c.kv_heads * 2 * chunks;
-  for (int i = threadIdx.x; i < items; i += blockDim.x) {
-    const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
-    float x[8];
+  const int i = blockIdx.y * blockDim.x + threadIdx.x;
+  if (i >= items) return;
+  const int64_t pos = a.positions ? (int64_t)a.positions[b] : 0;
+  const int64_t len = a.lens ? (int64_t)a.lens[b] : INT64_MAX;
+  const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
+  const int g = chunk / 4, w = chunk % 4 * groups + g;
+  const int64_t block = int4_block_bytes(c.head_dim, c.page_size);
+  const ts_view4& v = kind ? a.value : a.key;
+  T* dst = reinterpret_cast<T*>(v.data) + b * v.stride[0] + h * v.stride[1] + (int64_t)chunk * 8 * v.stride[3];
+  const unsigned char* base = reinterpret_cast<const unsigned char*>(c.pool) + h * block + kind * (block / 2);
+  for (int t = t0; t < t1; t += kInFlight) {
+    uint32_t word[kInFlight];
+    __half scale[kInFlight];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (page >= 0) {
-      const unsigned char* src = reinterpret_cast<const unsigned char*>(c.pool) + page * c.page_stride +
-                                 (int64_t)h * block + kind * (block / 2);
-      const int g = chunk / 4, w = chunk % 4 * groups + g;
-      const uint32_t word = reinterpret_cast<const uint32_t*>(src + (int64_t)at * (c.head_dim / 2))[w];
-      const float scale =
-          __half2float(reinterpret_cast<const __half*>(src + c.page_size * (c.head_dim / 2))[at * groups + g]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)((int)(word >> (4 * e) & 15u) - 8) * scale;
+    for (int u = 0; u < kInFlight; ++u) {
+      word[u] = 0x88888888u;
+      scale[u] = __ushort_as_half(0);
+      const int64_t at = pos + t + u, slot = at >> a.page_log2;
+      if (t + u >= t1 || at >= len) continue;
+      const int page = slot < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
+      if (page < 0) {
+        record_fault(a.fault, FAULT_PAGE);
+        continue;
+      }
+      const int in = (int)(at & (c.page_size - 1));
+      const unsigned char* src = base + page * c.page_stride;
+      word[u] = reinterpret_cast<const uint32_t*>(src + (int64_t)in * (c.head_dim / 2))[w];
+      scale[u] = reinterpret_cast<const __half*>(src + c.page_size * (c.head_dim / 2))[in * groups + g];
     }
-    const ts_view4& v = kind ? a.value : a.key;
-    T* dst = reinterpret_cast<T*>(v.data) + b * v.stride[0] + h * v.stride[1] + t * v.stride[2] +
-             (int64_t)chunk * 8 * v.stride[3];
-    store8(dst, v.stride[3], a.vec, x);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (t + u >= t1) break;
+      const float s = __half2float(scale[u]);
+      Raw8<T> raw;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // the nibble under 2^23's exponent: 2^23 + n + 8
+        raw.x[e] = Elem<T>::from_acc((__uint_as_float((word[u] >> (4 * e) & 15u) | 0x4B000000u) - 8388616.f) * s);
+      store8(dst + (int64_t)(t + u) * v.stride[2], v.stride[3], a.vec, raw);
+    }
   }
 }
 
@@ -132,24 +204,33 @@ static bool rows_vec(const ts_view4& v, int size) {
          v.stride[1] * size % 16 == 0 && v.stride[2] * size % 16 == 0;
 }
 
-static int row_threads(const ts_kv4_cache& c) {
-  const int items = c.kv_heads * 2 * (c.head_dim / 8);
-  return items >= 256 ? 256 : (items + 31) / 32 * 32;
+// Blocks of up to 256 words; as many tokens each as leaves about eight blocks a SM.
+static bool rows_grid(Int4Rows& a, dim3& grid, int& threads) {
+  const int items = a.c.kv_heads * 2 * (a.c.head_dim / 8);
+  threads = items >= 256 ? 256 : (items + 31) / 32 * 32;
+  grid.y = (items + threads - 1) / threads;
+  const int64_t each = (int64_t)a.c.batch * a.steps * grid.y / (148 * 8);
+  a.tokens = each >= 16 ? 16 : each >= 4 ? (int)(each / kInFlight * kInFlight) : each < 1 ? 1 : (int)each;
+  a.token_blocks = (a.steps + a.tokens - 1) / a.tokens;
+  const int64_t blocks = (int64_t)a.c.batch * a.token_blocks;
+  grid.x = (unsigned)blocks;
+  a.page_log2 = a.c.page_size == 16 ? 4 : a.c.page_size == 32 ? 5 : 6;
+  return blocks <= 0x7FFFFFFF && grid.y <= 65535;
 }
 
 cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype, int steps, const ts_kv4_cache& c,
                            int64_t position, const int32_t* positions, int32_t* positions_out, uint32_t* fault,
                            cudaStream_t st) {
   const int size = dtype == TS_F32 ? 4 : 2;
-  const Int4Rows a{c,   key,     value, steps, position, positions, positions_out, nullptr, fault,
-                   rows_vec(key, size) && rows_vec(value, size)};
-  const int64_t blocks = (int64_t)c.batch * steps;
-  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const int threads = row_threads(c);
+  Int4Rows a{c, key, value, steps, position, positions, positions_out, nullptr, fault,
+             rows_vec(key, size) && rows_vec(value, size)};
+  dim3 grid;
+  int threads;
+  if (!rows_grid(a, grid, threads)) return cudaErrorInvalidValue;
   switch (dtype) {
-    case TS_F32: kv_append_int4_kernel<float><<<(unsigned)blocks, threads, 0, st>>>(a); break;
-    case TS_F16: kv_append_int4_kernel<__half><<<(unsigned)blocks, threads, 0, st>>>(a); break;
-    case TS_BF16: kv_append_int4_kernel<__nv_bfloat16><<<(unsigned)blocks, threads, 0, st>>>(a); break;
+    case TS_F32: kv_append_int4_kernel<float><<<grid, threads, 0, st>>>(a); break;
+    case TS_F16: kv_append_int4_kernel<__half><<<grid, threads, 0, st>>>(a); break;
+    case TS_BF16: kv_append_int4_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(a); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -157,17 +238,16 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
 
 cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const int32_t* lens, const ts_view4& key,
                            const ts_view4& value, int dtype, int length, uint32_t* fault, cudaStream_t st) {
+  if (length == 0) return cudaSuccess;
   const int size = dtype == TS_F32 ? 4 : 2;
-  const Int4Rows a{c, key, value, length, 0, starts, nullptr, lens, fault,
-                   rows_vec(key, size) && rows_vec(value, size)};
-  const int64_t blocks = (int64_t)c.batch * length;
-  if (blocks == 0) return cudaSuccess;
-  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const int threads = row_threads(c);
+  Int4Rows a{c, key, value, length, 0, starts, nullptr, lens, fault, rows_vec(key, size) && rows_vec(value, size)};
+  dim3 grid;
+  int threads;
+  if (!rows_grid(a, grid, threads)) return cudaErrorInvalidValue;
   switch (dtype) {
-    case TS_F32: kv_gather_int4_kernel<float><<<(unsigned)blocks, threads, 0, st>>>(a); break;
-    case TS_F16: kv_gather_int4_kernel<__half><<<(unsigned)blocks, threads, 0, st>>>(a); break;
-    case TS_BF16: kv_gather_int4_kernel<__nv_bfloat16><<<(unsigned)blocks, threads, 0, st>>>(a); break;
+    case TS_F32: kv_gather_int4_kernel<float><<<grid, threads, 0, st>>>(a); break;
+    case TS_F16: kv_gather_int4_kernel<__half><<<grid, threads, 0, st>>>(a); break;
+    case TS_BF16: kv_gather_int4_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(a); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();

@@ -9,6 +9,7 @@
 //
 // The pages themselves are opaque bytes.  Copies and compaction are bound by HBM (each byte read
 // and written once); the table work is one launch of a few microseconds.
+#include "dependent.cuh"
 #include "int4.cuh"
 
 namespace tsa {
@@ -57,6 +58,7 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* warp_sums) {
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(ts_page_pool src, ts_page_pool dst,
                                                                  const int32_t* from, const int32_t* to, int stride,
                                                                  int n, const int32_t* n_dev) {
+  wait_for_previous();
   if (n_dev) n = min(n, *n_dev);
   const int chunks = (int)((src.page_bytes + kCopyChunk - 1) / kCopyChunk);
   const int64_t work = (int64_t)n * src.layers * chunks;
@@ -83,19 +85,22 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(ts_page_pool sr
   }
 }
 
+// dependent: the kernel before it on the stream is one of this file's that made the list.
 static cudaError_t launch_copy(const ts_page_pool& src, const ts_page_pool& dst, const int32_t* from,
-                               const int32_t* to, int stride, int n, const int32_t* n_dev, cudaStream_t st) {
+                               const int32_t* to, int stride, int n, const int32_t* n_dev, bool dependent,
+                               cudaStream_t st) {
   const int64_t work = (int64_t)n * src.layers * ((src.page_bytes + kCopyChunk - 1) / kCopyChunk);
   if (work == 0) return cudaSuccess;
   const int64_t most = 148 * 8;  // every block of a full GPU; they stride over the rest
-  page_copy_kernel<<<(unsigned)(work < most ? work : most), kCopyThreads, 0, st>>>(src, dst, from, to, stride, n,
-                                                                                  n_dev);
+  const dim3 grid((unsigned)(work < most ? work : most));
+  if (dependent) return launch_dependent(page_copy_kernel, grid, dim3(kCopyThreads), 0, st, src, dst, from, to, stride, n, n_dev);
+  page_copy_kernel<<<grid, kCopyThreads, 0, st>>>(src, dst, from, to, stride, n, n_dev);
   return cudaGetLastError();
 }
 
 cudaError_t kv_pages_copy(const ts_page_pool& src, const ts_page_pool& dst, const int32_t* from, const int32_t* to,
                           int count, cudaStream_t st) {
-  return launch_copy(src, dst, from, to, 1, count, nullptr, st);
+  return launch_copy(src, dst, from, to, 1, count, nullptr, false, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -187,6 +192,7 @@ __device__ __forceinline__ int reserve_partial(const ReserveArgs& a, int r) {
 __global__ void __launch_bounds__(kScanThreads) kv_reserve_kernel(ReserveArgs a) {
   __shared__ int warp_sums[32];
   __shared__ int too_long;
+  let_next_start();
   const int tid = threadIdx.x;
   if (tid == 0) too_long = 0;
   for (int r = tid; r < a.rows; r += kScanThreads) {
@@ -310,7 +316,7 @@ cudaError_t kv_pages_reserve(const ts_page_pool& pool, int32_t* table, int64_t t
   kv_reserve_kernel<<<1, kScanThreads, 0, st>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_copy(pool, pool, a.pairs, a.pairs + 1, 2, rows, nullptr, st);
+  return launch_copy(pool, pool, a.pairs, a.pairs + 1, 2, rows, nullptr, true, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -323,6 +329,7 @@ constexpr int kRankPages = kScanThreads * 4;
 
 __global__ void __launch_bounds__(kScanThreads) compact_count_kernel(const int32_t* refs, int pages, int32_t* counts) {
   __shared__ int warp_sums[32];
+  let_next_start();
   const int64_t p0 = (int64_t)blockIdx.x * kRankPages + threadIdx.x * 4;
   int n = 0, total;
 #pragma unroll
@@ -336,6 +343,8 @@ __global__ void __launch_bounds__(kScanThreads) compact_rank_kernel(const int32_
                                                                     const int32_t* counts, int32_t* from, int32_t* to,
                                                                     int32_t* rank, int32_t* moves, int32_t* counters) {
   __shared__ int warp_sums[32];
+  let_next_start();
+  wait_for_previous();
   int before = 0, live = 0;
   for (int i = threadIdx.x; i < (int)gridDim.x; i += kScanThreads) {
     const int n = counts[i];
@@ -375,6 +384,8 @@ __global__ void compact_tables_kernel(const int32_t* table, int32_t* table_out, 
                                       int64_t table_stride, int64_t table_out_stride, const int32_t* refs,
                                       int32_t* refs_out, int pages, const int32_t* from, const int32_t* to,
                                       const int32_t* rank, const int32_t* moves, const int32_t* counters) {
+  let_next_start();
+  wait_for_previous();
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int live = counters[1];
   if (i < *moves) {
@@ -401,14 +412,17 @@ cudaError_t kv_pages_compact(const ts_page_pool& pool, const int32_t* table, int
   int32_t* from = reinterpret_cast<int32_t*>(ws);
   int32_t *to = from + pages, *rank = to + pages, *counts = rank + pages, *moves = counts + blocks;
   compact_count_kernel<<<blocks, kScanThreads, 0, st>>>(refs, pages, counts);
-  compact_rank_kernel<<<blocks, kScanThreads, 0, st>>>(refs, refs_out, pages, counts, from, to, rank, moves, counters);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_dependent(compact_rank_kernel, dim3(blocks), dim3(kScanThreads), 0, st, refs, refs_out, pages, counts, from,
+                         to, rank, moves, counters);
   const int64_t most = (int64_t)rows * slots > pages ? (int64_t)rows * slots : pages;
-  compact_tables_kernel<<<(unsigned)((most + 255) / 256), 256, 0, st>>>(table, table_out, rows, slots, table_stride,
-                                                                        table_out_stride, refs, refs_out, pages, from,
-                                                                        to, rank, moves, counters);
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_dependent(compact_tables_kernel, dim3((unsigned)((most + 255) / 256)), dim3(256), 0, st, table, table_out,
+                         rows, slots, table_stride, table_out_stride, refs, refs_out, pages, from, to, rank, moves,
+                         counters);
   if (e != cudaSuccess) return e;
-  return launch_copy(pool, pool, from, to, 1, pages, moves, st);
+  return launch_copy(pool, pool, from, to, 1, pages, moves, true, st);
 }
 
 }  // namespace tsa

@@ -196,26 +196,27 @@ SIGNATURES = {
         [ctypes.POINTER(AttnParams), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
          ctypes.c_size_t, ctypes.c_void_p],
     ),
+    # The structs of the calls below are passed by address: packed bytes or a byref (engine.py packs them).
     "ts_kv4_block_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
     "ts_kv_append_int4": (
         ctypes.c_int,
-        [View4, View4, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(Kv4Cache), ctypes.c_int64, ctypes.c_void_p,
+        [View4, View4, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_void_p],
     ),
     "ts_kv_gather_int4": (
         ctypes.c_int,
-        [ctypes.POINTER(Kv4Cache), ctypes.c_void_p, ctypes.c_void_p, View4, View4, ctypes.c_int32, ctypes.c_int32,
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, View4, View4, ctypes.c_int32, ctypes.c_int32,
          ctypes.c_void_p],
     ),
-    "ts_attn_int4_path": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache)]),
-    "ts_attn_int4_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache)]),
+    "ts_attn_int4_path": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_attn_int4_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
     "ts_attn_int4": (
         ctypes.c_int,
-        [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ts_kv_pages_copy": (
         ctypes.c_int,
-        [ctypes.POINTER(PagePool), ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
          ctypes.c_void_p],
     ),
     "ts_kv_pages_fork": (
@@ -227,14 +228,14 @@ SIGNATURES = {
     "ts_kv_pages_reserve_workspace_size": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
     "ts_kv_pages_reserve": (
         ctypes.c_int,
-        [ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
          ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ts_kv_pages_compact_workspace_size": (ctypes.c_size_t, [ctypes.c_int32]),
     "ts_kv_pages_compact": (
         ctypes.c_int,
-        [ctypes.POINTER(PagePool), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
          ctypes.c_void_p],
     ),

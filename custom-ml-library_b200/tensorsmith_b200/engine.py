@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -420,13 +421,28 @@ def decode_int8(q, k8, v8, key_scales, value_scales, *, is_causal=True, scale=No
 # -- the paged 4-bit cache ----------------------------------------------------
 
 
+# The calls below cost a few microseconds on the device, so their structs are packed in one go (the layouts of
+# _lib.AttnParams, _lib.Kv4Cache and _lib.PagePool) instead of field by field.
+_ATTN_STRUCT = struct.Struct("@" + "P4q" * 4 + "P3q" + "8i" + "d" + "iq" + "P" + "iP4q")
+_VIEW_STRUCT = struct.Struct("@P4q")
+_KV4_STRUCT = struct.Struct("@PqPq6i")
+_POOL_STRUCT = struct.Struct("@Pqqqii")
+
+
+def _packed_view(t) -> _lib.View4:
+    return _lib.View4.from_buffer_copy(_VIEW_STRUCT.pack(t.data_ptr(), *t.stride()))
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def int4_block_bytes(head_dim: int, page_size: int) -> int:
     """Bytes of one page and KV head, keys and values: 4.5 bits a value (ts_kv4_block_bytes)."""
-    size = int(_lib.lib().ts_kv4_block_bytes(int(head_dim), int(page_size)))
-    if not size:
+    if head_dim <= 0 or head_dim > 256 or head_dim % 32 or page_size not in (16, 32, 64):
         raise ValueError("a 4-bit cache takes head dimensions that are multiples of 32 up to 256 and pages of "
                          "16, 32 or 64 tokens")
-    return size
+    return page_size * head_dim * 9 // 8
 
 
 def int4_pool(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64, layers: int | None = None,
@@ -438,121 +454,125 @@ def int4_pool(num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 
     return torch.empty(shape if layers is None else (layers,) + shape, dtype=torch.uint8, device=device)
 
 
-def _int32_vector(t, name: str, size: int, device) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] != size or t.device != device:
+def _int32_vector(t, name: str, size: int, index: int) -> int:
+    if t.dtype != torch.int32 or t.get_device() != index or t.shape != (size,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector of {size} on the pool's device")
-    return t
+    return t.data_ptr()
 
 
-def _page_table(t, device) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.device != device or min(t.shape) <= 0:
+def _page_table(t, index: int) -> tuple:
+    """(pointer, stride, rows, slots) of a page table."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.get_device() != index or t.stride(1) != 1 or 0 in t.shape:
         raise ValueError("a page table must be int32 [rows, slots] with contiguous rows on the pool's device")
-    return t
+    rows, slots = t.shape
+    return t.data_ptr(), t.stride(0), rows, slots
 
 
-def _int4_cache(pool, page_table, page_size: int, head_dim: int) -> _lib.Kv4Cache:
-    _require_cuda(pool)
-    if pool.dtype != torch.uint8 or pool.dim() != 3:
-        raise TypeError("a 4-bit pool must be uint8 [pages, kv heads, block]")
-    pages, heads, block = pool.shape
-    if block != int4_block_bytes(head_dim, page_size) or pool.stride(2) != 1 or pool.stride(1) != block:
-        raise ValueError("the pool's blocks do not match the head dimension and page size")
-    _page_table(page_table, pool.device)
-    rows, slots = page_table.shape
-    return _lib.Kv4Cache(pool.data_ptr(), pool.stride(0), page_table.data_ptr(), page_table.stride(0), rows, slots,
-                         pages, heads, head_dim, page_size)
+class _Int4Cache:
+    """A checked pool with its page table: the packed ts_kv4_cache and the sizes the callers need."""
 
+    __slots__ = ("index", "rows", "slots", "heads", "packed")
 
-def _int4_rows(t, cache, what: str) -> None:
-    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[1] != cache.kv_heads or t.shape[3] != cache.head_dim:
-        raise ValueError(f"{what} must be [rows, kv heads, tokens, head dimension] of the cache")
+    def __init__(self, pool, page_table, page_size: int, head_dim: int):
+        if pool.dtype != torch.uint8 or pool.dim() != 3:
+            raise TypeError("a 4-bit pool must be uint8 [pages, kv heads, block]")
+        self.index = pool.get_device()
+        if self.index < 0:
+            raise ValueError("the B200 attention engine needs CUDA device tensors")
+        pages, self.heads, block = pool.shape
+        stride = pool.stride()
+        if block != int4_block_bytes(head_dim, page_size) or stride[2] != 1 or stride[1] != block:
+            raise ValueError("the pool's blocks do not match the head dimension and page size")
+        table, table_stride, self.rows, self.slots = _page_table(page_table, self.index)
+        self.packed = _KV4_STRUCT.pack(pool.data_ptr(), stride[0], table, table_stride, self.rows, self.slots, pages,
+                                       self.heads, head_dim, page_size)
 
 
 def kv_append_int4(key, value, pool, page_table, *, page_size, position=0, positions=None, positions_out=None):
     """Quantise a [B, Hkv, steps, D] chunk into the pages of its rows, at token ``position`` (or per-row
     ``positions``).  The table must hold a page for every token written (``kv_pages_reserve``)."""
-    _require_cuda(key, value)
-    cache = _int4_cache(pool, page_table, page_size, key.shape[-1])
-    _int4_rows(key, cache, "key")
-    if value.shape != key.shape:
-        raise ValueError("key and value must have the same shape")
+    if key.dim() != 4:
+        raise ValueError("key must be [rows, kv heads, tokens, head dimension] of the cache")
+    rows, heads, steps, dim = key.shape
+    cache = _Int4Cache(pool, page_table, page_size, dim)
+    if rows != cache.rows or heads != cache.heads:
+        raise ValueError("key must be [rows, kv heads, tokens, head dimension] of the cache")
+    if value.shape != key.shape or key.get_device() != cache.index or value.get_device() != cache.index:
+        raise ValueError("key and value must have the same shape, on the pool's device")
     if value.dtype != key.dtype:
         raise TypeError("key/value must share a dtype")
-    for name, t in (("positions", positions), ("positions_out", positions_out)):
-        if t is not None:
-            _int32_vector(t, name, cache.batch, pool.device)
-    _lib.check(
-        _lib.lib().ts_kv_append_int4(view4(key), view4(value), dtype_code(key.dtype), key.shape[2],
-                                     ctypes.byref(cache), int(position),
-                                     positions.data_ptr() if positions is not None else None,
-                                     positions_out.data_ptr() if positions_out is not None else None,
-                                     _stream_handle(pool.device)),
-        "ts_kv_append_int4")
+    status = _lib.lib().ts_kv_append_int4(
+        _packed_view(key), _packed_view(value), dtype_code(key.dtype), steps, cache.packed, int(position),
+        None if positions is None else _int32_vector(positions, "positions", rows, cache.index),
+        None if positions_out is None else _int32_vector(positions_out, "positions_out", rows, cache.index),
+        _raw_stream(cache.index))
+    if status:
+        _lib.check(status, "ts_kv_append_int4")
 
 
 def kv_gather_int4(pool, page_table, length, *, page_size, dtype, starts=None, kv_lens=None):
     """The cached values of ``length`` tokens of every row, from token ``starts[b]`` (default 0): dequantised
     ``(keys, values)`` [B, Hkv, length, D] of ``dtype``; tokens at or past ``kv_lens[b]`` (optional) are zero."""
-    _require_cuda(pool)
-    if pool.dtype != torch.uint8 or pool.dim() != 3:
-        raise TypeError("a 4-bit pool must be uint8 [pages, kv heads, block]")
-    head_dim = pool.shape[2] * 8 // (9 * page_size) if page_size > 0 else 0
-    cache = _int4_cache(pool, page_table, page_size, head_dim)
+    head_dim = pool.shape[-1] * 8 // (9 * page_size) if page_size > 0 else 0
+    cache = _Int4Cache(pool, page_table, page_size, head_dim)
     code, length = dtype_code(dtype), int(length)
     if length < 0:
         raise ValueError("length must not be negative")
-    for name, t in (("starts", starts), ("kv_lens", kv_lens)):
-        if t is not None:
-            _int32_vector(t, name, cache.batch, pool.device)
-    both = torch.empty((2, cache.batch, cache.kv_heads, length, head_dim), dtype=dtype, device=pool.device)
-    key, value = both[0], both[1]
+    rows = cache.rows
+    starts = None if starts is None else _int32_vector(starts, "starts", rows, cache.index)
+    kv_lens = None if kv_lens is None else _int32_vector(kv_lens, "kv_lens", rows, cache.index)
+    both = pool.new_empty((2, rows, cache.heads, length, head_dim), dtype=dtype)
+    key, value = both.unbind(0)
     if length:
-        _lib.check(
-            _lib.lib().ts_kv_gather_int4(ctypes.byref(cache), starts.data_ptr() if starts is not None else None,
-                                         kv_lens.data_ptr() if kv_lens is not None else None, view4(key), view4(value),
-                                         code, length, _stream_handle(pool.device)),
-            "ts_kv_gather_int4")
+        status = _lib.lib().ts_kv_gather_int4(cache.packed, starts, kv_lens, _packed_view(key), _packed_view(value), code,
+                                              length, _raw_stream(cache.index))
+        if status:
+            _lib.check(status, "ts_kv_gather_int4")
     return key, value
 
 
-def _int4_attn_params(q, out, lse, cache, kv_lens, max_len, is_causal, scale) -> _lib.AttnParams:
-    p = _lib.AttnParams()
-    p.q, p.o = view4(q), view4(out)
-    if lse is not None:
-        p.lse = lse.data_ptr()
-        p.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
-    p.dtype = dtype_code(q.dtype)
-    p.batch, p.q_heads, p.kv_heads = q.shape[0], q.shape[1], cache.kv_heads
-    p.q_len, p.kv_len, p.head_dim, p.value_dim = q.shape[2], max_len, cache.head_dim, cache.head_dim
-    p.scale = default_scale(cache.head_dim) if scale is None else float(scale)
-    p.is_causal = 1 if is_causal else 0
-    p.kv_lens = kv_lens.data_ptr()
-    return p
-
-
-def _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len):
-    _require_cuda(q, pool, page_table, kv_lens)
+def _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len, is_causal, scale, out, lse):
+    """(cache, packed ts_attn_params) of an attention_int4 call after its checks."""
     if q.dim() != 4:
         raise ValueError("expected a [batch, heads, sequence, channels] view")
-    cache = _int4_cache(pool, page_table, page_size, q.shape[3])
-    if q.device != pool.device or q.shape[0] != cache.batch or q.shape[1] % cache.kv_heads or 0 in q.shape:
+    rows, heads, tokens, dim = q.shape
+    cache = _Int4Cache(pool, page_table, page_size, dim)
+    if q.get_device() != cache.index or rows != cache.rows or heads % cache.heads or heads * tokens == 0:
         raise ValueError("query rows and heads must match the cache, on its device")
-    _int32_vector(kv_lens, "kv_lens", cache.batch, pool.device)
+    lens = _int32_vector(kv_lens, "kv_lens", rows, cache.index)
     whole = cache.slots * page_size
     max_len = whole if max_len is None else int(max_len)
     if not 0 <= max_len <= whole:
         raise ValueError("max_len must be between zero and the tokens the page table can hold")
-    return cache, max(1, max_len)
+    if lse is None:
+        lse = (0, 0, 0, 0)
+    elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.get_device() != cache.index:
+        raise ValueError("lse must be fp32 [B, Hq, Tq] on the query's device")
+    else:
+        lse = (lse.data_ptr(), *lse.stride())
+    if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != cache.index:
+        raise ValueError("out must have the query's shape, dtype and device")
+    none = (0, 0, 0, 0, 0)
+    return cache, _ATTN_STRUCT.pack(q.data_ptr(), *q.stride(), *none, *none, out.data_ptr(), *out.stride(), *lse,
+                                    dtype_code(q.dtype), rows, heads, cache.heads, tokens, max(1, max_len), dim, dim,
+                                    default_scale(dim) if scale is None else float(scale), 1 if is_causal else 0, 0,
+                                    lens, 0, *none)
 
 
 def attention_int4_path(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_causal=True, scale=None) -> str:
     """Name of the kernel family ``attention_int4`` selects: "decode" (straight over the pages) or "tcgen05"."""
-    cache, max_len = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len)
-    p = _int4_attn_params(q, q, None, cache, kv_lens, max_len, is_causal, scale)
-    code = _lib.lib().ts_attn_int4_path(ctypes.byref(p), ctypes.byref(cache))
+    cache, params = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len, is_causal, scale, q, None)
+    code = _lib.lib().ts_attn_int4_path(params, cache.packed)
     if code < 0:
         _lib.check(code, "ts_attn_int4_path")
     return _lib.PATH_NAMES[code]
+
+
+def attention_int4_workspace_bytes(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_causal=True,
+                                   scale=None) -> int:
+    """Bytes of the ``workspace`` that ``attention_int4`` needs for these arguments."""
+    cache, params = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len, is_causal, scale, q, None)
+    return int(_lib.lib().ts_attn_int4_workspace_size(params, cache.packed))
 
 
 def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_causal=True, scale=None,
@@ -562,25 +582,22 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
     Row b sees its first ``kv_lens[b]`` tokens; with ``is_causal`` its Tq queries are the last of them
     (a row without a visible key gives zeros and an LSE of -inf).  ``max_len`` bounds ``kv_lens`` (default: what
     the table can hold); the work is split for it, so pass the real bound where it is known."""
-    cache, max_len = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len)
-    dtype_code(q.dtype)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError("out must have the query's shape, dtype and device")
-    if need_lse:
-        if lse is None:
-            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        elif lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
-            raise ValueError("lse must be fp32 [B, Hq, Tq] on the query's device")
-    p = _int4_attn_params(q, out, lse if need_lse else None, cache, kv_lens, max_len, is_causal, scale)
+        out = q.new_empty(q.shape)
+    if not need_lse:
+        lse = None
+    elif lse is None:
+        lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    cache, params = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len, is_causal, scale, out, lse)
     handle = _lib.lib()
-    need = int(handle.ts_attn_int4_workspace_size(ctypes.byref(p), ctypes.byref(cache)))
+    need = handle.ts_attn_int4_workspace_size(params, cache.packed)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _lib.check(handle.ts_attn_int4(ctypes.byref(p), ctypes.byref(cache), workspace.data_ptr() if need else None, need,
-                                   _stream_handle(q.device)), "ts_attn_int4")
-    return out, (lse if need_lse else None)
+        workspace = pool.new_empty((need,))
+    status = handle.ts_attn_int4(params, cache.packed, workspace.data_ptr() if need else None, need,
+                                 _raw_stream(cache.index))
+    if status:
+        _lib.check(status, "ts_attn_int4")
+    return out, lse
 
 
 # -- pages ---------------------------------------------------------------------
@@ -596,59 +613,60 @@ def kv_pages_state(num_pages: int, device="cuda") -> tuple[torch.Tensor, torch.T
     return refs, torch.tensor([num_pages, 0, 0, 0], dtype=torch.int32, device=device)
 
 
-def _page_pool(pool) -> _lib.PagePool:
-    """A pool [pages, ...] or [layers, pages, kv heads, block] as opaque pages."""
-    _require_cuda(pool)
-    if pool.dim() == 3:
-        pool = pool[None]
-    if pool.dim() != 4 or not pool[0, 0].is_contiguous():
+def _page_pool(pool) -> tuple:
+    """(packed ts_page_pool, pages, device index, page bytes, layers) of a pool of opaque pages, [pages, kv heads,
+    block] or [layers, pages, kv heads, block]."""
+    index, shape, stride = pool.get_device(), pool.shape, pool.stride()
+    if index < 0:
+        raise ValueError("the B200 attention engine needs CUDA device tensors")
+    if len(shape) == 3:
+        shape, stride = (1, *shape), (0, *stride)
+    if len(shape) != 4 or stride[3] != 1 or stride[2] != shape[3]:
         raise ValueError("a page pool must be [layers, pages, kv heads, block] with contiguous pages")
     size = pool.element_size()
-    return _lib.PagePool(pool.data_ptr(), pool.stride(0) * size, pool.stride(1) * size,
-                         pool.shape[2] * pool.shape[3] * size, pool.shape[0], pool.shape[1])
-
-
-def _page_counts(refs, counters, pages: int, device) -> None:
-    _int32_vector(refs, "refs", pages, device)
-    _int32_vector(counters, "counters", 4, device)
+    page = shape[2] * shape[3] * size
+    return (_POOL_STRUCT.pack(pool.data_ptr(), stride[0] * size, stride[1] * size, page, shape[0], shape[1]), shape[1],
+            index, page, shape[0])
 
 
 def kv_pages_copy(src_pool, src, dst_pool, dst):
     """Copy page ``src[i]`` of one pool to page ``dst[i]`` of another (or the same), in every layer; pairs with a
     negative or out-of-range entry are skipped.  No page may be both read and written."""
-    a, b = _page_pool(src_pool), _page_pool(dst_pool)
-    _int32_vector(src, "src", src.shape[0], src_pool.device)
-    _int32_vector(dst, "dst", src.shape[0], src_pool.device)
-    if src_pool.device != dst_pool.device or a.page_bytes != b.page_bytes or a.layers != b.layers:
+    a, _, index, page, layers = _page_pool(src_pool)
+    b, _, other, other_page, other_layers = _page_pool(dst_pool)
+    count = src.shape[0]
+    from_ptr, to_ptr = _int32_vector(src, "src", count, index), _int32_vector(dst, "dst", count, index)
+    if (index, page, layers) != (other, other_page, other_layers):
         raise ValueError("pools must have the same layers and page size, on one device")
-    _lib.check(_lib.lib().ts_kv_pages_copy(ctypes.byref(a), ctypes.byref(b), src.data_ptr(), dst.data_ptr(),
-                                           src.shape[0], _stream_handle(src_pool.device)), "ts_kv_pages_copy")
+    status = _lib.lib().ts_kv_pages_copy(a, b, from_ptr, to_ptr, count, _raw_stream(index))
+    if status:
+        _lib.check(status, "ts_kv_pages_copy")
 
 
 def kv_pages_fork(page_table, lens, index, refs, counters, *, page_size, table_out=None, lens_out=None):
     """Rows that share the pages of the rows ``index`` names: fork, beam reorder, and free (an entry of -1 leaves
     its row empty).  Returns ``(table, lens)`` with ``len(index)`` rows; ``refs`` and ``counters`` are updated."""
-    _require_cuda(page_table)
-    device = page_table.device
-    _page_table(page_table, device)
-    rows, slots = page_table.shape
-    _int32_vector(lens, "lens", rows, device)
-    _int32_vector(index, "index", index.shape[0], device)
-    _page_counts(refs, counters, refs.shape[0], device)
-    n = index.shape[0]
+    device = page_table.get_device()
+    if device < 0:
+        raise ValueError("the B200 attention engine needs CUDA device tensors")
+    table, stride, rows, slots = _page_table(page_table, device)
+    n, pages = index.shape[0], refs.shape[0]
     if n == 0 or page_size <= 0:
         raise ValueError("fork needs at least one row and a positive page size")
-    table_out = torch.empty((n, slots), dtype=torch.int32, device=device) if table_out is None else table_out
-    lens_out = torch.empty(n, dtype=torch.int32, device=device) if lens_out is None else lens_out
-    if _page_table(table_out, device).shape != (n, slots):
+    if table_out is None:
+        table_out = page_table.new_empty((n, slots))
+    if lens_out is None:
+        lens_out = lens.new_empty((n,))
+    out, out_stride, out_rows, out_slots = _page_table(table_out, device)
+    if (out_rows, out_slots) != (n, slots):
         raise ValueError("table_out must be [len(index), slots]")
-    _int32_vector(lens_out, "lens_out", n, device)
-    _lib.check(
-        _lib.lib().ts_kv_pages_fork(page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), rows,
-                                    index.data_ptr(), table_out.data_ptr(), table_out.stride(0), lens_out.data_ptr(),
-                                    n, slots, page_size, refs.data_ptr(), refs.shape[0], counters.data_ptr(),
-                                    _stream_handle(device)),
-        "ts_kv_pages_fork")
+    status = _lib.lib().ts_kv_pages_fork(
+        table, stride, _int32_vector(lens, "lens", rows, device), rows, _int32_vector(index, "index", n, device), out,
+        out_stride, _int32_vector(lens_out, "lens_out", n, device), n, slots, page_size,
+        _int32_vector(refs, "refs", pages, device), pages, _int32_vector(counters, "counters", 4, device),
+        _raw_stream(device))
+    if status:
+        _lib.check(status, "ts_kv_pages_fork")
     return table_out, lens_out
 
 
@@ -656,51 +674,45 @@ def kv_pages_reserve(pool, page_table, lens, steps, refs, counters, *, page_size
     """Give every row pages of its own for the next ``steps`` tokens (an int, or int32 per row on the device):
     free pages for empty slots, a copy of a partly filled page that other rows hold too.  Works in place; when the
     pool or the table is too small it sets an error bit of ``counters[2]`` and changes nothing."""
-    p = _page_pool(pool)
-    device = pool.device
-    _page_table(page_table, device)
-    rows, slots = page_table.shape
-    _int32_vector(lens, "lens", rows, device)
-    _page_counts(refs, counters, p.pages, device)
+    packed, pages, device, _, _ = _page_pool(pool)
+    table, stride, rows, slots = _page_table(page_table, device)
     row_steps = None
     if isinstance(steps, torch.Tensor):
         row_steps, steps = _int32_vector(steps, "steps", rows, device), 0
     if steps < 0 or page_size <= 0:
         raise ValueError("steps must not be negative and the page size must be positive")
     handle = _lib.lib()
-    need = int(handle.ts_kv_pages_reserve_workspace_size(p.pages, rows))
+    need = handle.ts_kv_pages_reserve_workspace_size(pages, rows)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _lib.check(
-        handle.ts_kv_pages_reserve(ctypes.byref(p), page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), rows,
-                                   slots, page_size, steps, row_steps.data_ptr() if row_steps is not None else None,
-                                   refs.data_ptr(), counters.data_ptr(), workspace.data_ptr(), need,
-                                   _stream_handle(device)),
-        "ts_kv_pages_reserve")
+        workspace = page_table.new_empty((need // 4,))
+    status = handle.ts_kv_pages_reserve(
+        packed, table, stride, _int32_vector(lens, "lens", rows, device), rows, slots, page_size, steps, row_steps,
+        _int32_vector(refs, "refs", pages, device), _int32_vector(counters, "counters", 4, device),
+        workspace.data_ptr(), need, _raw_stream(device))
+    if status:
+        _lib.check(status, "ts_kv_pages_reserve")
 
 
 def kv_pages_compact(pool, page_table, refs, counters, *, table_out=None, refs_out=None, workspace=None):
     """Move the live pages to the start of the pool (the highest page into the lowest hole, and so on) and rewrite
     the tables and counts, in place unless ``table_out`` / ``refs_out`` are given.  Returns ``(table, refs)``."""
-    p = _page_pool(pool)
-    device = pool.device
-    _page_table(page_table, device)
-    _page_counts(refs, counters, p.pages, device)
-    rows, slots = page_table.shape
+    packed, pages, device, _, _ = _page_pool(pool)
+    table, stride, rows, slots = _page_table(page_table, device)
     table_out = page_table if table_out is None else table_out
     refs_out = refs if refs_out is None else refs_out
-    if _page_table(table_out, device).shape != (rows, slots):
+    out, out_stride, out_rows, out_slots = _page_table(table_out, device)
+    if (out_rows, out_slots) != (rows, slots):
         raise ValueError("table_out must have the table's shape")
-    _int32_vector(refs_out, "refs_out", p.pages, device)
     handle = _lib.lib()
-    need = int(handle.ts_kv_pages_compact_workspace_size(p.pages))
+    need = handle.ts_kv_pages_compact_workspace_size(pages)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _lib.check(
-        handle.ts_kv_pages_compact(ctypes.byref(p), page_table.data_ptr(), page_table.stride(0), table_out.data_ptr(),
-                                   table_out.stride(0), rows, slots, refs.data_ptr(), refs_out.data_ptr(),
-                                   counters.data_ptr(), workspace.data_ptr(), need, _stream_handle(device)),
-        "ts_kv_pages_compact")
+        workspace = page_table.new_empty((need // 4,))
+    status = handle.ts_kv_pages_compact(
+        packed, table, stride, out, out_stride, rows, slots, _int32_vector(refs, "refs", pages, device),
+        _int32_vector(refs_out, "refs_out", pages, device), _int32_vector(counters, "counters", 4, device),
+        workspace.data_ptr(), need, _raw_stream(device))
+    if status:
+        _lib.check(status, "ts_kv_pages_compact")
     return table_out, refs_out
 
 

@@ -166,13 +166,8 @@ def test_attention_groups_and_tokens(dtype, page, causal, group, q_len, monkeypa
 @pytest.mark.parametrize("group, q_len", [(1, 1), (4, 1), (4, 5)])
 def test_attention_splits_long_rows(dtype, group, q_len):
     c = Cache([4097, 1, 9000, 0], 1, 128, 64, seed=7)
-    need = engine._lib.lib()  # several splits: the workspace is not empty
     q = torch.zeros(4, group, q_len, 128, device="cuda", dtype=torch_dtype(dtype))
-    cache, most = engine._int4_attn_args(q, c.pool, c.table, c.kv_lens, 64, 9000)
-    p = engine._int4_attn_params(q, q, None, cache, c.kv_lens, most, True, None)
-    import ctypes
-
-    assert need.ts_attn_int4_workspace_size(ctypes.byref(p), ctypes.byref(cache)) > 0
+    assert engine.attention_int4_workspace_bytes(q, c.pool, c.table, c.kv_lens, page_size=64, max_len=9000) > 0
     check_attention(c, dtype, group, q_len)
 
 

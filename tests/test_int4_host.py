@@ -68,6 +68,12 @@ def test_ctypes_layout(tmp_path):
     include = Path(__file__).resolve().parent.parent / "include"
     subprocess.run([gcc, "-I", str(include), str(src), "-o", str(exe)], check=True)
     got = dict(x.rsplit(" ", 1) for x in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split("\n") if x)
+    assert engine._ATTN_STRUCT.size == ctypes.sizeof(_lib.AttnParams)
+    assert engine._KV4_STRUCT.size == ctypes.sizeof(_lib.Kv4Cache)
+    assert engine._POOL_STRUCT.size == ctypes.sizeof(_lib.PagePool)
+    p = _lib.AttnParams.from_buffer_copy(engine._ATTN_STRUCT.pack(*range(1, 43)))
+    assert (p.q.data, p.o.stride[3], p.lse, p.dtype, p.value_dim, p.scale, p.is_causal, p.causal_offset, p.kv_lens,
+            p.mask_kind, p.mask_stride[3]) == (1, 20, 21, 25, 32, 33.0, 34, 35, 36, 37, 42)
     for s, c in fields.items():
         assert int(got[s]) == ctypes.sizeof(c)
         for f, _ in c._fields_:
