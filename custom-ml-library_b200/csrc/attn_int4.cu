@@ -30,13 +30,13 @@ int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
   // One wave of blocks that fill the GPU, fewer where a warp would be left without a stage.
   const int blocks = a.by_pair ? (int)pairs
                                : (int)i64min(pairs * ceil_div(p.kv_len, shape.keys), (int64_t)sm_count() * shape.blocks);
-  a.warps = blocks * shape.warps;
+  a.blocks = blocks;
   a.parts = (int)(blocks / pairs);
   return blocks;
 }
 
-size_t partial_bytes(const Int4Attn& a, int head_dim) {
-  return (size_t)2 * a.warps * a.slot_cols * (head_dim + 2) * sizeof(float);
+size_t partial_bytes(const Int4Attn& a, const Int4Shape& shape, int head_dim) {
+  return (size_t)2 * a.blocks * shape.warps * a.slot_cols * (head_dim + 2) * sizeof(float);
 }
 }  // namespace
 
@@ -49,13 +49,16 @@ bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c) {
 // D = 128; a second tile of wider rows or of fp32's two query parts does not fit the registers).
 Int4Shape int4_shape(const ts_attn_params& p) {
   const int64_t cols = (int64_t)(p.q_heads / p.kv_heads) * p.q_len;
-  const bool by_pair64 = p.kv_len <= 4 * 64;
-  if (p.head_dim > 128) return {1, 32, 4, 2, p.kv_len <= 4 * 32};
-  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2, by_pair64};
-  // Stages of 16 tokens where those of 64 would leave most warps without one.
+  if (p.head_dim > 128) return {1, 32, 4, 2, false};
+  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2, false};
+  // Stages of 16 tokens where those of 64 would leave most warps without one: 9.6 against 11.5 us for 18 heads
+  // of up to 701 keys (fp32), 12.0 against 14.0 for 16 of up to 1024.  With two stages and more for every warp,
+  // one block of 12 warps a SM against three of 4: its merged parts are fewer (64 x 32 heads of 1024-8192 keys:
+  // 283 against 294 us; 16 heads of 2048 keys, one stage a warp: 19 against 13.6).
   const int64_t stages = (int64_t)p.batch * p.kv_heads * ((cols + 7) / 8) * ceil_div(p.kv_len, 64);
   if (p.kv_len <= 64 || stages <= 148 * 3) return {1, 16, 4, 3, p.kv_len <= 4 * 16};
-  return {1, 64, 4, 3, by_pair64};
+  if (stages >= 148 * 12 * 2) return {1, 64, 12, 1, false};
+  return {1, 64, 4, 3, false};
 }
 
 size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
@@ -64,7 +67,7 @@ size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
   plan(p, a, shape);
   if (a.by_pair) return 0;
   const int rows = p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows;
-  return partial_bytes(a, p.head_dim) + (size_t)2 * (rows + 1) * sizeof(int32_t);
+  return partial_bytes(a, shape, p.head_dim) + (size_t)2 * (rows + 1) * sizeof(int32_t);
 }
 
 cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
@@ -78,8 +81,8 @@ cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, vo
   a.page_log2 = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : 6;
   a.block_bytes = int4_block_bytes(p.head_dim, c.page_size);
   a.ws_acc = reinterpret_cast<float*>(ws);
-  a.ws_ml = a.by_pair ? nullptr : a.ws_acc + (size_t)2 * a.warps * a.slot_cols * p.head_dim;
-  a.ws_first = a.by_pair ? nullptr : reinterpret_cast<int32_t*>(a.ws_ml + (size_t)2 * a.warps * a.slot_cols * 2);
+  a.ws_ml = a.by_pair ? nullptr : a.ws_acc + (size_t)2 * a.blocks * shape.warps * a.slot_cols * p.head_dim;
+  a.ws_first = a.by_pair ? nullptr : reinterpret_cast<int32_t*>(a.ws_ml + (size_t)2 * a.blocks * shape.warps * a.slot_cols * 2);
   a.fault = fault;
   const int size = p.dtype == TS_F32 ? 4 : 2;
   a.q_vec = rows_vec(p.q, size);

@@ -34,7 +34,7 @@
 
 namespace tsa {
 
-constexpr int kInt4MaxRows = 2048;  // rows of one launch: their prefix sums sit in shared memory
+constexpr int kInt4MaxRows = 1024;  // rows of one launch: their prefix sums sit in shared memory
 
 struct Int4Attn {
   ts_attn_params p;
@@ -44,12 +44,12 @@ struct Int4Attn {
   int cols;        // query columns of a KV head: group * q_len, token-major (column = token * group + head)
   int col_blocks;  // blocks of columns; one warp holds one at a time
   int slot_cols;   // columns of a block that can be live
-  int warps;       // that share the work
+  int blocks;      // that share the work
   bool by_pair;    // one block a (row, KV head, column block) instead of equal shares
   int parts;       // about how many blocks share a row at the longest length
   bool q_vec, o_vec;  // rows of unit stride and 16-byte alignment
-  float* ws_acc;   // [2 * warps, slot_cols, D] partial results
-  float* ws_ml;    // [2 * warps, slot_cols, 2]
+  float* ws_acc;   // [2 * warps of all blocks, slot_cols, D] partial results
+  float* ws_ml;    // [2 * warps of all blocks, slot_cols, 2]
   int32_t* ws_first;  // [2, batch + 1] stages and units before each row
   uint32_t* fault;
 };
@@ -57,8 +57,16 @@ struct Int4Attn {
 __device__ __forceinline__ int int4_len(const Int4Attn& a, int b) { return min(a.p.kv_len, max(0, a.p.kv_lens[b])); }
 // The shares count n + 1 units for a pair (KV head and column block) of a row with n stages: entering it
 // (its queries read, its result written) takes a warp about as long as a stage.  Unit 0 of a pair is the
-// entry, unit i + 1 its stage i.  Warp w takes the units [w * share, (w + 1) * share).
-__device__ __forceinline__ int int4_share(const Int4Attn& a, int units) { return max(1, ceil_div(units, a.warps)); }
+// entry, unit i + 1 its stage i.  Worker w takes the units [w * share, (w + 1) * share): the first `block_warps`
+// warps of each block, which are fewer than the block has where a short line would else leave SMs idle (but
+// no fewer than four, whose parts merge on the SM).
+struct Int4Shares {
+  int block_warps, share;
+};
+__device__ __forceinline__ Int4Shares int4_shares(const Int4Attn& a, int units, int most_warps) {
+  const int block_warps = min(most_warps, max(4, ceil_div(units, a.blocks)));  // at least one a scheduler
+  return Int4Shares{block_warps, max(1, ceil_div(units, a.blocks * block_warps))};
+}
 
 constexpr float kInt4Log2e = 1.4426950408889634f;
 constexpr float kInt4Ln2 = 0.6931471805599453f;
@@ -540,13 +548,13 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     }
   }
   __syncthreads();
-  const int id = blockIdx.x * kWarps + warp;
   struct Place {  // of a stage: row, column block and KV head, stage of the pair and their number
     int b, pair, st, n_st;
   };
   Place home;       // of the block's first stage
   int begin, mine;  // this warp's first stage and their number
   int block_mine;   // the block's
+  int block_id = 0, id = 0;  // the block's first worker, this warp's
   int share = 0, total = 0, total_units = 0;
   auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
     int lo = 0, hi = a.p.batch - 1;
@@ -587,11 +595,15 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   } else {
     total = first[a.p.batch];
     total_units = first_unit[a.p.batch];
-    share = int4_share(a, total_units);
+    const Int4Shares shares = int4_shares(a, total_units, kWarps);
+    share = shares.share;
+    block_id = blockIdx.x * shares.block_warps;
+    id = block_id + warp;
     begin = stages_before((int64_t)id * share);
-    mine = stages_before((int64_t)(id + 1) * share) - begin;
-    const int block_begin = stages_before((int64_t)blockIdx.x * kWarps * share);
-    block_mine = stages_before((int64_t)(blockIdx.x + 1) * kWarps * share) - block_begin;
+    mine = warp < shares.block_warps ? stages_before((int64_t)(id + 1) * share) - begin : 0;
+    const int64_t block_units = (int64_t)shares.block_warps * share;
+    const int block_begin = stages_before(blockIdx.x * block_units);
+    block_mine = stages_before((blockIdx.x + 1) * block_units) - block_begin;
     if (block_mine <= 0) return;
     home = place(block_begin);
   }
@@ -685,6 +697,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   float* red = reinterpret_cast<float*>(smem);
   float2* ml = reinterpret_cast<float2*>(red + kWarps * kCols * kPad);
   const int g = lane >> 2, t = lane & 3;
+  const int hk = home.pair / a.col_blocks, col0 = (home.pair - hk * a.col_blocks) * NT * 8;
+  const int n_cols = min(kCols, a.cols - col0);
   if (!__syncthreads_and(ok)) return;
   if (mine <= 0) {
     for (int i = lane; i < kCols; i += 32) ml[warp * kCols + i] = make_float2(-INFINITY, 0.f);
@@ -702,16 +716,18 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           const int word = g * NW + w, ch = 32 * (word % DG) + 8 * (word / DG);
-          if (DG % 2 && word >= D / 8) continue;
+          if ((DG % 2 && word >= D / 8) || nt * 8 + 2 * t + j >= n_cols) continue;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) red[col * kPad + ch + e] = q.acc[nt][4 * w + e / 2][j + 2 * (e & 1)];
+          for (int e = 0; e < 8; e += 4)
+            *reinterpret_cast<float4*>(&red[col * kPad + ch + e]) =
+                make_float4(q.acc[nt][4 * w + e / 2][j], q.acc[nt][4 * w + e / 2][j + 2],
+                            q.acc[nt][4 * w + e / 2 + 1][j], q.acc[nt][4 * w + e / 2 + 1][j + 2]);
         }
       }
   }
   __syncthreads();
-  const int hk = home.pair / a.col_blocks, col0 = (home.pair - hk * a.col_blocks) * NT * 8;
   const bool all = block_mine == home.n_st;
-  for (int i = threadIdx.x; i < min(kCols, a.cols - col0) * D; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < n_cols * D; i += kWarps * 32) {
     const int col = i / D, d = i - col * D;
     float top = -INFINITY, sum = 0.f, out = 0.f;
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * kCols + col].x);
@@ -728,7 +744,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
       int4_out_row<T>(a, home.b, h, tok)[d * a.p.o.stride[3]] = Elem<T>::from_acc(sum == 0.f ? 0.f : out / sum);
       if (d == 0) int4_store_lse(a, home.b, h, tok, top - 7.f, sum);
     } else {
-      const int64_t slot = (int64_t)2 * blockIdx.x * kWarps * a.slot_cols + col;
+      const int64_t slot = (int64_t)2 * block_id * a.slot_cols + col;
       a.ws_acc[slot * D + d] = out;
       if (d == 0) reinterpret_cast<float2*>(a.ws_ml)[slot] = make_float2(top, sum);
     }
@@ -759,20 +775,21 @@ __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__
   float out[8] = {};
   if (n) {
     const int enter = row_first + pair * n;  // the pair's stages are the units enter + 1 .. enter + n - 1
-    const int share = int4_share(a, total), w0 = (enter + 1) / share, w1 = (enter + n - 1) / share;
-    const int c0 = w0 / kWarps, c1 = w1 / kWarps;
+    const Int4Shares shares = int4_shares(a, total, kWarps);
+    const int share = shares.share, warps = shares.block_warps;
+    const int w0 = (enter + 1) / share, w1 = (enter + n - 1) / share, c0 = w0 / warps, c1 = w1 / warps;
     auto merged = [&](int c) {  // no stage of the block's share is another pair's (the next one's entry may be)
-      return (int64_t)c * kWarps * share >= enter &&
-             i64min((int64_t)(c + 1) * kWarps * share, total) <= (int64_t)enter + n + 1;
+      return (int64_t)c * warps * share >= enter &&
+             i64min((int64_t)(c + 1) * warps * share, total) <= (int64_t)enter + n + 1;
     };
     const bool m0 = merged(c0), m1 = merged(c1);
     if (w0 == w1 || (c0 == c1 && m0)) return;
     // The row's parts: of the first block's warps, of the blocks that merged theirs, of the last block's warps.
-    const int head = m0 ? 0 : min(w1, c0 * kWarps + kWarps - 1) - w0 + 1;
+    const int head = m0 ? 0 : min(w1, c0 * warps + warps - 1) - w0 + 1;
     const int lo = m0 ? c0 : c0 + 1, mid = max(0, (m1 ? c1 : c1 - 1) - lo + 1);
-    const int tail = c1 != c0 && !m1 ? w1 - c1 * kWarps + 1 : 0;
+    const int tail = c1 != c0 && !m1 ? w1 - c1 * warps + 1 : 0;
     auto slot = [&](int i) {
-      const int w = i < head ? w0 + i : i < head + mid ? (lo + i - head) * kWarps : c1 * kWarps + i - head - mid;
+      const int w = i < head ? w0 + i : i < head + mid ? (lo + i - head) * warps : c1 * warps + i - head - mid;
       return (int64_t)(2 * w + ((int64_t)w * share < enter)) * a.slot_cols + local;
     };
     const float2* all_ml = reinterpret_cast<const float2*>(a.ws_ml);

@@ -6,25 +6,24 @@
 namespace tsa {
 
 constexpr int kInt4Stages = 2;  // stages in a warp's ring
-constexpr int kInt4Warps = 4;
 
-template <typename T, int DG, int NT, int KT, int kMinBlocks>
+template <typename T, int DG, int NT, int KT, int kWarps, int kMinBlocks>
 static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
   constexpr int D = DG * 32;
-  constexpr size_t ring = (size_t)kInt4Warps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t));
-  constexpr size_t merge = (size_t)kInt4Warps * NT * 8 * (D + 4 + 2) * sizeof(float);
+  constexpr size_t ring = (size_t)kWarps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t));
+  constexpr size_t merge = (size_t)kWarps * NT * 8 * (D + 4 + 2) * sizeof(float);
   constexpr size_t most = ring + (size_t)2 * (kInt4MaxRows + 1) * sizeof(int);
   const size_t need = ring + (a.by_pair ? 0 : (size_t)2 * (a.p.batch + 1) * sizeof(int));
   const size_t smem = need > merge ? need : merge;
-  auto kernel = attn_int4_kernel<T, DG, NT, KT, kInt4Stages, kInt4Warps, kMinBlocks>;
+  auto kernel = attn_int4_kernel<T, DG, NT, KT, kInt4Stages, kWarps, kMinBlocks>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), (int)(most > merge ? most : merge));
   if (e != cudaSuccess) return e;
-  kernel<<<blocks, kInt4Warps * 32, smem, st>>>(a);
+  kernel<<<blocks, kWarps * 32, smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.by_pair) return e;
   const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
   const int row_warps = a.parts > 8 ? 8 : 1;  // warps that merge one row
-  return launch_dependent(attn_int4_combine<T, NT, kInt4Warps>, dim3((unsigned)((rows * row_warps + 7) / 8)), dim3(256),
+  return launch_dependent(attn_int4_combine<T, NT, kWarps>, dim3((unsigned)((rows * row_warps + 7) / 8)), dim3(256),
                           0, st, a, row_warps);
 }
 
@@ -34,32 +33,41 @@ cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int bloc
   if constexpr (sizeof(T) == 2) {
     if (shape.nt == 2) {
       switch (groups) {
-        case 1: return int4_run<T, 1, 2, 64, 2>(a, blocks, st);
-        case 2: return int4_run<T, 2, 2, 64, 2>(a, blocks, st);
-        case 3: return int4_run<T, 3, 2, 64, 2>(a, blocks, st);
-        case 4: return int4_run<T, 4, 2, 64, 2>(a, blocks, st);
+        case 1: return int4_run<T, 1, 2, 64, 4, 2>(a, blocks, st);
+        case 2: return int4_run<T, 2, 2, 64, 4, 2>(a, blocks, st);
+        case 3: return int4_run<T, 3, 2, 64, 4, 2>(a, blocks, st);
+        case 4: return int4_run<T, 4, 2, 64, 4, 2>(a, blocks, st);
       }
       return cudaErrorInvalidValue;
     }
   }
   if (shape.keys == 16) {
     switch (groups) {
-      case 1: return int4_run<T, 1, 1, 16, 3>(a, blocks, st);
-      case 2: return int4_run<T, 2, 1, 16, 3>(a, blocks, st);
-      case 3: return int4_run<T, 3, 1, 16, 3>(a, blocks, st);
-      case 4: return int4_run<T, 4, 1, 16, 3>(a, blocks, st);
+      case 1: return int4_run<T, 1, 1, 16, 4, 3>(a, blocks, st);
+      case 2: return int4_run<T, 2, 1, 16, 4, 3>(a, blocks, st);
+      case 3: return int4_run<T, 3, 1, 16, 4, 3>(a, blocks, st);
+      case 4: return int4_run<T, 4, 1, 16, 4, 3>(a, blocks, st);
+    }
+    return cudaErrorInvalidValue;
+  }
+  if (shape.warps == 12) {
+    switch (groups) {
+      case 1: return int4_run<T, 1, 1, 64, 12, 1>(a, blocks, st);
+      case 2: return int4_run<T, 2, 1, 64, 12, 1>(a, blocks, st);
+      case 3: return int4_run<T, 3, 1, 64, 12, 1>(a, blocks, st);
+      case 4: return int4_run<T, 4, 1, 64, 12, 1>(a, blocks, st);
     }
     return cudaErrorInvalidValue;
   }
   switch (groups) {
-    case 1: return int4_run<T, 1, 1, 64, 3>(a, blocks, st);
-    case 2: return int4_run<T, 2, 1, 64, 3>(a, blocks, st);
-    case 3: return int4_run<T, 3, 1, 64, 3>(a, blocks, st);
-    case 4: return int4_run<T, 4, 1, 64, 3>(a, blocks, st);
-    case 5: return int4_run<T, 5, 1, 32, 2>(a, blocks, st);
-    case 6: return int4_run<T, 6, 1, 32, 2>(a, blocks, st);
-    case 7: return int4_run<T, 7, 1, 32, 2>(a, blocks, st);
-    case 8: return int4_run<T, 8, 1, 32, 2>(a, blocks, st);
+    case 1: return int4_run<T, 1, 1, 64, 4, 3>(a, blocks, st);
+    case 2: return int4_run<T, 2, 1, 64, 4, 3>(a, blocks, st);
+    case 3: return int4_run<T, 3, 1, 64, 4, 3>(a, blocks, st);
+    case 4: return int4_run<T, 4, 1, 64, 4, 3>(a, blocks, st);
+    case 5: return int4_run<T, 5, 1, 32, 4, 2>(a, blocks, st);
+    case 6: return int4_run<T, 6, 1, 32, 4, 2>(a, blocks, st);
+    case 7: return int4_run<T, 7, 1, 32, 4, 2>(a, blocks, st);
+    case 8: return int4_run<T, 8, 1, 32, 4, 2>(a, blocks, st);
   }
   return cudaErrorInvalidValue;
 }

@@ -2,6 +2,7 @@
 
 from .attention import rotary_embedding, scaled_dot_product_attention  # noqa: F401
 from .cache import KVCache  # noqa: F401
+from .paged import PagedKVCache  # noqa: F401
 from .transformer import (  # noqa: F401
     MultiHeadAttention,
     RMSNorm,

@@ -36,6 +36,7 @@ from .. import engine
 from ..tensor import Tensor, is_grad_enabled, no_grad
 from .attention import BACKENDS, scaled_dot_product_attention
 from .cache import KVCache
+from .paged import PagedKVCache, PagedLayer
 
 
 def _grad_mode() -> bool:
@@ -248,6 +249,14 @@ class MultiHeadAttention(_Module):
         else:
             if recording:
                 raise NotImplementedError("training with an explicit attention mask is not routed to the engine")
+            if isinstance(cache, PagedLayer):
+                # 4-bit pages: the chunk is quantised into them and attention reads them directly.
+                if attn_mask is not None:
+                    raise ValueError("a paged cache takes no attention mask")
+                (cache.append_rotary if self.rotary else cache.append)(_mirror(k), _mirror(v))
+                q_t = _mirror(engine.rope(q, positions=cache.cache.positions) if self.rotary else q)
+                attended = cache.attend(q_t)._data
+                return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
             q_t = _mirror(engine.rope(q, offset=offset) if self.rotary else q)
             if cache is not None:
                 # RoPE of the keys at their cache positions fused into the append (nn/transformer.py:139-142).
@@ -388,10 +397,20 @@ class TransformerLM(_Module):
         return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1), ignore_index=ignore_index,
                                label_smoothing=label_smoothing)
 
-    def new_cache(self, batch_size: int, max_seq_len: int | None = None, *, quantized=False) -> list[KVCache]:
+    def new_cache(self, batch_size: int, max_seq_len: int | None = None, *, quantized=False,
+                  num_pages: int | None = None) -> list[KVCache]:
+        """One cache a block: plain, int8 (``quantized=True``), or the layers of a ``PagedKVCache`` in 4 bits
+        (``quantized="int4"``, of ``num_pages`` pages: by default what ``batch_size`` full rows need)."""
         capacity = self.config.max_seq_len if max_seq_len is None else max_seq_len
         if capacity <= 0 or capacity > self.config.max_seq_len:
             raise ValueError("cache capacity must fit the model context")
+        if quantized == "int4":
+            attention = self.blocks[0].attention
+            return PagedKVCache(batch_size, len(self.blocks), attention.num_kv_heads, attention.head_dim, capacity,
+                                num_pages=num_pages, device=f"cuda:{self._device_index}",
+                                dtype=self.token_embedding_weight.dtype).layers
+        if not isinstance(quantized, bool) or num_pages is not None:
+            raise ValueError('quantized must be a bool or "int4", and only "int4" has pages')
         return [
             KVCache(batch_size, block.attention.num_kv_heads, block.attention.head_dim, capacity,
                     device=f"cuda:{self._device_index}", dtype=self.token_embedding_weight.dtype, quantized=quantized)
@@ -399,9 +418,12 @@ class TransformerLM(_Module):
         ]
 
     def generate(self, prompt, max_new_tokens: int, *, temperature=1.0, top_k: int | None = None, top_p: float = 1.0,
-                 eos_token_id: int | None = None, use_cache: bool = True, quantized_cache: bool = False,
-                 generator: torch.Generator | None = None) -> torch.Tensor:
-        """Batched greedy / top-k / nucleus sampling; returns prompt plus generated tokens."""
+                 eos_token_id: int | None = None, use_cache: bool = True, quantized_cache: bool | str = False,
+                 num_samples: int = 1, generator: torch.Generator | None = None) -> torch.Tensor:
+        """Batched greedy / top-k / nucleus sampling; returns prompt plus generated tokens.
+
+        ``num_samples`` continues every prompt that often, a prompt's rows one after the other.  With
+        ``quantized_cache="int4"`` the prompt runs once and its samples share the pages that hold it."""
         prompt = _as_tokens(prompt, self.device)
         if prompt.ndim != 2 or prompt.shape[1] == 0 or max_new_tokens < 0 or prompt.dtype not in (torch.int32,
                                                                                                    torch.int64):
@@ -414,16 +436,32 @@ class TransformerLM(_Module):
             raise ValueError("top_k must be within the vocabulary")
         if eos_token_id is not None and not 0 <= eos_token_id < self.config.vocab_size:
             raise ValueError("eos_token_id out of range")
+        if not isinstance(num_samples, int) or num_samples < 1:
+            raise ValueError("num_samples must be a positive integer")
+        shared = num_samples > 1 and use_cache and max_new_tokens > 0 and quantized_cache == "int4"
+        if num_samples > 1 and not shared:
+            prompt = prompt.repeat_interleave(num_samples, dim=0)
         modes = [(module, module.training) for module in self.modules()]
         try:
             self.eval()
             with no_grad(), torch.no_grad():
-                caches = (self.new_cache(prompt.shape[0], prompt.shape[1] + max_new_tokens, quantized=quantized_cache)
-                          if use_cache and max_new_tokens else None)
+                caches = None
+                if use_cache and max_new_tokens:
+                    rows, length, pages = prompt.shape[0], prompt.shape[1], None
+                    if shared:  # every prompt's pages once, and what each sample writes of its own
+                        size = PagedKVCache.PAGE_SIZE
+                        own = -(-(length + max_new_tokens) // size) - length // size
+                        pages = rows * (-(-length // size) + num_samples * own)
+                    caches = self.new_cache(rows, length + max_new_tokens, quantized=quantized_cache, num_pages=pages)
                 result, current = prompt.long(), prompt.long()
                 finished = torch.zeros(prompt.shape[0], dtype=torch.bool, device=self.device)
-                for _ in range(max_new_tokens):
+                for step in range(max_new_tokens):
                     logits = self(current, caches=caches, logits_to_keep=1)[:, -1, :]
+                    if shared and step == 0:
+                        rows = torch.arange(prompt.shape[0]).repeat_interleave(num_samples)
+                        caches[0].cache.fork(rows)
+                        rows = rows.to(self.device)
+                        logits, result, finished = logits[rows], result[rows], finished[rows]
                     next_token = sample_logits(logits, temperature, top_k, top_p, generator=generator)
                     if eos_token_id is not None:
                         next_token = torch.where(finished, torch.full_like(next_token, eos_token_id), next_token)

@@ -372,7 +372,9 @@ TS_ATTN_API size_t ts_kv_pages_reserve_workspace_size(int32_t pages, int32_t row
  * (row_steps[r] in place of steps when given): empty slots get free pages, and a
  * partly filled page that others hold too is replaced by a copy (in every layer of
  * the pool); of its holders that write, the last keeps it if no other row has it.
- * Pages are handed out lowest first, in the order of (row, slot).  lens stays. */
+ * Pages are handed out lowest first, in the order of (row, slot).  lens stays.
+ * Slots past a row's tokens must be -1 or pages of its own: after shortening a
+ * row, ts_kv_pages_fork onto itself drops the ones it no longer needs. */
 TS_ATTN_API int ts_kv_pages_reserve(const ts_page_pool* pool, int32_t* table, int64_t table_stride,
                                     const int32_t* lens, int32_t rows, int32_t slots, int32_t page_size,
                                     int32_t steps, const int32_t* row_steps, int32_t* refs, int32_t* counters,
