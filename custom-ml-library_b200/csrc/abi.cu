@@ -376,9 +376,20 @@ ts_attn_params int4_prefill_params(const ts_attn_params& p, void* ws) {
   return d;
 }
 
-// Query columns of a KV head (group x tokens) from which dequantising the pages and running the
-// prefill kernel is faster than attending over the pages.
-constexpr int kInt4PrefillColumns = 64;
+// Whether dequantising the pages and running the prefill kernel is the faster way, by what each costs a cached
+// key in nanoseconds (measured at D = 128, bf16, 2 and 16 rows of 8 KV heads, groups of 1, 4 and 8 query heads,
+// 64, 128 and 256 query columns a KV head).  Over the pages the time grows with the columns (group x tokens):
+// 1.95e-3 a KV head and column.  The other way writes and reads the dequantised rows, 0.133 a KV head, and then
+// runs one query tile a block: 6.1 a wave of 128-row tiles, 13.4 of 256-row ones (more than 128 tokens), however
+// few of a tile's rows are filled.  16 rows, 64 columns: 148 against 204 to 532 us by group; 256 columns: 521
+// against 250, 345 and 542; 2 rows, 256 columns: 53 against 79, 50 and 51.
+bool int4_prefill_faster(const ts_attn_params& p) {
+  const double heads = (double)p.batch * p.kv_heads, columns = (double)(p.q_heads / p.kv_heads) * p.q_len;
+  const int rows = p.q_len > 128 ? 256 : 128;
+  const int64_t tiles = (int64_t)p.batch * p.q_heads * ((p.q_len + rows - 1) / rows);
+  const double waves = (double)((tiles + 147) / 148);
+  return 1.95e-3 * heads * columns > 0.133 * heads + waves * (rows == 256 ? 13.4 : 6.1);
+}
 
 bool int4_prefill(const ts_attn_params& p) {
   if (!int4_dtype_ok(p.dtype) || p.dtype == TS_F32) return false;
@@ -387,7 +398,7 @@ bool int4_prefill(const ts_attn_params& p) {
   const char* force = std::getenv("TS_INT4_KERNEL");
   if (force && !std::strcmp(force, "pages")) return false;
   if (force && !std::strcmp(force, "prefill")) return true;
-  return (int64_t)p.q_heads / p.kv_heads * p.q_len >= kInt4PrefillColumns;
+  return int4_prefill_faster(p);
 }
 
 int check_page_pool(const ts_page_pool* p) {

@@ -45,12 +45,13 @@ bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c) {
   return c.page_size == 16 || c.page_size == 32 || c.page_size == 64;
 }
 
-// Two column tiles share one pass over the nibbles where there are more than 8 columns (half types up to
-// D = 128; a second tile of wider rows or of fp32's two query parts does not fit the registers).
 Int4Shape int4_shape(const ts_attn_params& p) {
-  const int64_t cols = (int64_t)(p.q_heads / p.kv_heads) * p.q_len;
+  const int cols = p.q_heads / p.kv_heads * p.q_len;
   if (p.head_dim > 128) return {1, 32, 4, 2, false};
-  if (cols > 8 && p.dtype != TS_F32) return {2, 64, 4, 2, false};
+  // Several column tiles share the operands made from the nibbles, with their queries in shared memory.  Three
+  // where that saves a second pass (16 rows x 8 KV heads, up to 8192 keys, 20 columns: 59 against 66 us with two;
+  // 12 columns: 55 against 46).  Four spill: 32 columns took 78 us against 71 with two passes of two.
+  if (cols > 8) return {cols > 16 && cols <= 24 && p.dtype != TS_F32 ? 3 : 2, 64, 4, 2, false};
   // Stages of 16 tokens where those of 64 would leave most warps without one: 9.6 against 11.5 us for 18 heads
   // of up to 701 keys (fp32), 12.0 against 14.0 for 16 of up to 1024.  With two stages and more for every warp,
   // one block of 12 warps a SM against three of 4: its merged parts are fewer (64 x 32 heads of 1024-8192 keys:

@@ -135,7 +135,22 @@ struct Int4State {
   static constexpr int QP = sizeof(T) == 4 ? 2 : 1;                          // fp16 parts of q
   static constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;   // fp16 parts of p
   static constexpr int NW = (DG + 1) / 2;                                    // V words a lane takes of a row
-  uint32_t qf[QP][NT][DG][4];
+  static constexpr bool kQueriesShared = NT > 1;  // several tiles' query fragments wait in shared memory
+  // Tiles of 16 keys whose scores and probabilities are held at a time: what the registers leave room for.
+  static constexpr int kChunk = NT == 1 ? 4 : NT == 2 ? 2 : 1;
+  uint32_t qf[kQueriesShared ? 1 : QP][kQueriesShared ? 1 : DG][4];
+  uint32_t qs;  // shared address of [QP, NT, DG, 32 lanes] x 16 bytes, this lane's first
+  __device__ __forceinline__ uint4 fragment(int part, int nt, int gr) const {
+    if constexpr (kQueriesShared) {
+      uint4 v;  // volatile: loaded where it is used, or the compiler keeps all of them in registers
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(qs + ((part * NT + nt) * DG + gr) * 512));
+      return v;
+    } else {
+      return make_uint4(qf[part][gr][0], qf[part][gr][1], qf[part][gr][2], qf[part][gr][3]);
+    }
+  }
   float cs[NT][2];       // turns a column's products into exponents of 2; columns 2t and 2t + 1
   int limit[NT][2];      // last key a column sees
   float acc[NT][4 * NW][4];
@@ -203,23 +218,28 @@ template <bool kEdge, typename T, int DG, int NT, int KT>
 __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsigned char* st,
                                            const Int4Tiles& at, int key0, int k_end) {
   using State = Int4State<T, DG, NT>;
-  constexpr int D = DG * 32, NW = State::NW, kTiles = KT / 16, kRow = D / 2, kScaleRow = D / 16;
+  constexpr int D = DG * 32, NW = State::NW, kRow = D / 2, kScaleRow = D / 16;
+  constexpr int kTiles = KT / 16 < State::kChunk ? KT / 16 : State::kChunk;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int tok_a = token_of_row(g), tok_b = 8 + tok_a;
 
+#pragma unroll 1
+  for (int tile0 = 0; tile0 < KT / 16; tile0 += kTiles) {
+  if (kEdge && tile0 > 0 && key0 + tile0 * 16 >= k_end) break;
   // S^T = K q^T, a 32-channel group at a time, the group's scale on its fp32 sum.
   float s[NT][kTiles][4];
 #pragma unroll
   for (int tile = 0; tile < kTiles; ++tile) {
-    if (kEdge && tile > 0 && key0 + tile * 16 >= k_end) {  // none of its keys exists
+    if (kEdge && tile > 0 && key0 + (tile0 + tile) * 16 >= k_end) {  // none of its keys exists
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nt][tile][e] = -INFINITY;
       continue;
     }
-    const unsigned char* kb = st + (tile >> 1) * at.row_pair + (tile & 1) * at.row_one + t * (DG * 4);
-    const unsigned char* ks = st + at.scales + (tile >> 1) * at.scale_pair + (tile & 1) * at.scale_one;
+    const int in = tile0 + tile;
+    const unsigned char* kb = st + (in >> 1) * at.row_pair + (in & 1) * at.row_one + t * (DG * 4);
+    const unsigned char* ks = st + at.scales + (in >> 1) * at.scale_pair + (in & 1) * at.scale_one;
     uint32_t wa[DG], wb[DG];
     uint32_t ha[(DG + 1) / 2], hb[(DG + 1) / 2];
     lds_words<DG>(kb + tok_a * kRow, wa);
@@ -236,11 +256,13 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
       for (int nt = 0; nt < NT; ++nt) {
         float dot[4];
         constexpr int kLast = State::QP - 1;  // the smaller part first
-        mma16816_first(dot, k[0], k[1], k[2], k[3], q.qf[kLast][nt][gr][0], q.qf[kLast][nt][gr][1]);
-        mma16816(dot, k[4], k[5], k[6], k[7], q.qf[kLast][nt][gr][2], q.qf[kLast][nt][gr][3]);
+        uint4 b = q.fragment(kLast, nt, gr);
+        mma16816_first(dot, k[0], k[1], k[2], k[3], b.x, b.y);
+        mma16816(dot, k[4], k[5], k[6], k[7], b.z, b.w);
         if constexpr (kLast > 0) {
-          mma16816(dot, k[0], k[1], k[2], k[3], q.qf[0][nt][gr][0], q.qf[0][nt][gr][1]);
-          mma16816(dot, k[4], k[5], k[6], k[7], q.qf[0][nt][gr][2], q.qf[0][nt][gr][3]);
+          b = q.fragment(0, nt, gr);
+          mma16816(dot, k[0], k[1], k[2], k[3], b.x, b.y);
+          mma16816(dot, k[4], k[5], k[6], k[7], b.z, b.w);
         }
         float(&x)[4] = s[nt][tile];
         x[0] = gr ? fmaf(sa, dot[0], x[0]) : sa * dot[0];
@@ -261,7 +283,7 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
       if constexpr (kEdge) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + tile * 16 + (e < 2 ? tok_a : tok_b);
+          const int key = key0 + (tile0 + tile) * 16 + (e < 2 ? tok_a : tok_b);
           if (key >= k_end || key > q.limit[nt][e & 1]) x[e] = -INFINITY;
         }
       }
@@ -317,9 +339,10 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
   const int slot[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};
 #pragma unroll
   for (int tile = 0; tile < kTiles; ++tile) {
-    if (kEdge && tile > 0 && key0 + tile * 16 >= k_end) break;
-    const unsigned char* vb = st + at.values + (tile >> 1) * at.row_pair + (tile & 1) * at.row_one;
-    const unsigned char* vs = st + at.values + at.scales + (tile >> 1) * at.scale_pair + (tile & 1) * at.scale_one;
+    if (kEdge && tile > 0 && key0 + (tile0 + tile) * 16 >= k_end) break;
+    const int in = tile0 + tile;
+    const unsigned char* vb = st + at.values + (in >> 1) * at.row_pair + (in & 1) * at.row_one;
+    const unsigned char* vs = st + at.values + at.scales + (in >> 1) * at.scale_pair + (in & 1) * at.scale_one;
     uint32_t w[4][NW], sc[4][(NW + 1) / 2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -338,7 +361,7 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
         }
       }
       if constexpr (kEdge) {  // past the end a page may hold anything: its nibbles are finite, its scale need not be
-        if (key0 + tile * 16 + slot[k] >= k_end)
+        if (key0 + (tile0 + tile) * 16 + slot[k] >= k_end)
 #pragma unroll
           for (int j = 0; j < (NW + 1) / 2; ++j) sc[k][j] = 0;
       }
@@ -364,6 +387,7 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
             mma16816(q.acc[nt][4 * j + byte], a0, a1, a2, a3, pf[part][nt][tile][0], pf[part][nt][tile][1]);
       }
     }
+  }
   }
 }
 
@@ -420,13 +444,24 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     // B fragments: channels 32 gr + 8 t + {0,4}, {1,5}, {2,6}, {3,7} of column g
 #pragma unroll
     for (int gr = 0; gr < DG; ++gr) {
+      uint32_t f[State::QP][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float lo = x[gr][e] * up, hi = x[gr][e + 4] * up;
         const __half2 part = __floats2half2_rn(lo, hi);
-        q.qf[0][nt][gr][e] = h2_bits(part);
+        f[0][e] = h2_bits(part);
         if constexpr (State::QP == 2)
-          q.qf[1][nt][gr][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
+          f[1][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
+      }
+#pragma unroll
+      for (int part = 0; part < State::QP; ++part) {
+        if constexpr (State::kQueriesShared) {  // read back by this lane alone
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(q.qs + ((part * NT + nt) * DG + gr) * 512),
+                       "r"(f[part][0]), "r"(f[part][1]), "r"(f[part][2]), "r"(f[part][3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q.qf[part][gr][e] = f[part][e];
+        }
       }
     }
 #pragma unroll
@@ -496,7 +531,7 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
     }
 }
 
-// T: type of q and o.  DG = D / 32.  NT: tiles of 8 query columns a warp holds.
+// T: type of q and o.  DG = D / 32.  NT: tiles of 8 query columns a warp holds, 1 to 3.
 //
 // The work is a line of stages of KT tokens, ordered by (row, KV head, column block, key); rows differ in
 // length, so every warp takes an equal share of the line instead of whole rows or splits of one size.  A
@@ -514,7 +549,11 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* ring = smem + warp * (kStages * kStageBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes) + warp * kStages;
-  int* first = reinterpret_cast<int*>(smem + kWarps * kStages * (kStageBytes + (int)sizeof(uint64_t)));
+  static_assert(kStages * sizeof(uint64_t) == 16, "");
+  using State = Int4State<T, DG, NT>;
+  constexpr int kQueryBytes = State::kQueriesShared ? State::QP * NT * DG * 512 : 0;
+  unsigned char* queries = smem + kWarps * kStages * kStageBytes + kWarps * 16;
+  int* first = reinterpret_cast<int*>(queries + kWarps * kQueryBytes);
   const int pairs = a.p.kv_heads * a.col_blocks;
 
   const int unit = min(1 << a.page_log2, KT), units = KT / unit;  // 1, 2 or 4
@@ -661,7 +700,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   int issued = 0;
   while (issued < min(mine, kStages - 1)) issue(issued++);
 
-  Int4State<T, DG, NT> q;
+  State q;
+  q.qs = ptx::smem_u32(queries + warp * kQueryBytes) + lane * 16;
   bool ok = true;
   int n = 0;
   while (n < mine && ok) {
@@ -693,7 +733,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   if (!together) return;
 
   // Merge through shared memory, over the rings: warp w's columns behind those of the warps before it.
-  constexpr int kCols = NT * 8, kPad = D + 4, NW = Int4State<T, DG, NT>::NW;
+  constexpr int kCols = NT * 8, kPad = D + 4, NW = State::NW;
   float* red = reinterpret_cast<float*>(smem);
   float2* ml = reinterpret_cast<float2*>(red + kWarps * kCols * kPad);
   const int g = lane >> 2, t = lane & 3;
@@ -846,5 +886,7 @@ Int4Shape int4_shape(const ts_attn_params& p);
 
 template <typename T>
 cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st);
+template <typename T>
+cudaError_t attn_int4_launch_wide(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st);
 
 }  // namespace tsa

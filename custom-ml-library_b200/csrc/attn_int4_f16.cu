@@ -1,4 +1,4 @@
-// f16 instances of the attention over a 4-bit cache (attn_int4.cuh).
+// f16 instances of the attention over a 4-bit cache (attn_int4.cuh): one column tile.
 #include "attn_int4_launch.cuh"
 
 namespace tsa {

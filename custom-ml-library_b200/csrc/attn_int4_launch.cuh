@@ -10,7 +10,8 @@ constexpr int kInt4Stages = 2;  // stages in a warp's ring
 template <typename T, int DG, int NT, int KT, int kWarps, int kMinBlocks>
 static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
   constexpr int D = DG * 32;
-  constexpr size_t ring = (size_t)kWarps * kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t));
+  constexpr size_t queries = NT > 1 ? (sizeof(T) == 4 ? 2 : 1) * NT * DG * 512 : 0;
+  constexpr size_t ring = (size_t)kWarps * (kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t)) + queries);
   constexpr size_t merge = (size_t)kWarps * NT * 8 * (D + 4 + 2) * sizeof(float);
   constexpr size_t most = ring + (size_t)2 * (kInt4MaxRows + 1) * sizeof(int);
   const size_t need = ring + (a.by_pair ? 0 : (size_t)2 * (a.p.batch + 1) * sizeof(int));
@@ -27,49 +28,39 @@ static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
                           0, st, a, row_warps);
 }
 
+template <typename T, int NT, int KT, int kWarps, int kMinBlocks>
+static cudaError_t int4_run_dims(const Int4Attn& a, int blocks, cudaStream_t st) {
+  switch (a.p.head_dim / 32) {
+    case 1: return int4_run<T, 1, NT, KT, kWarps, kMinBlocks>(a, blocks, st);
+    case 2: return int4_run<T, 2, NT, KT, kWarps, kMinBlocks>(a, blocks, st);
+    case 3: return int4_run<T, 3, NT, KT, kWarps, kMinBlocks>(a, blocks, st);
+    case 4: return int4_run<T, 4, NT, KT, kWarps, kMinBlocks>(a, blocks, st);
+  }
+  return cudaErrorInvalidValue;
+}
+
+// One column tile.
 template <typename T>
 cudaError_t attn_int4_launch(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st) {
-  const int groups = a.p.head_dim / 32;
-  if constexpr (sizeof(T) == 2) {
-    if (shape.nt == 2) {
-      switch (groups) {
-        case 1: return int4_run<T, 1, 2, 64, 4, 2>(a, blocks, st);
-        case 2: return int4_run<T, 2, 2, 64, 4, 2>(a, blocks, st);
-        case 3: return int4_run<T, 3, 2, 64, 4, 2>(a, blocks, st);
-        case 4: return int4_run<T, 4, 2, 64, 4, 2>(a, blocks, st);
-      }
-      return cudaErrorInvalidValue;
-    }
-  }
-  if (shape.keys == 16) {
-    switch (groups) {
-      case 1: return int4_run<T, 1, 1, 16, 4, 3>(a, blocks, st);
-      case 2: return int4_run<T, 2, 1, 16, 4, 3>(a, blocks, st);
-      case 3: return int4_run<T, 3, 1, 16, 4, 3>(a, blocks, st);
-      case 4: return int4_run<T, 4, 1, 16, 4, 3>(a, blocks, st);
-    }
-    return cudaErrorInvalidValue;
-  }
-  if (shape.warps == 12) {
-    switch (groups) {
-      case 1: return int4_run<T, 1, 1, 64, 12, 1>(a, blocks, st);
-      case 2: return int4_run<T, 2, 1, 64, 12, 1>(a, blocks, st);
-      case 3: return int4_run<T, 3, 1, 64, 12, 1>(a, blocks, st);
-      case 4: return int4_run<T, 4, 1, 64, 12, 1>(a, blocks, st);
-    }
-    return cudaErrorInvalidValue;
-  }
-  switch (groups) {
-    case 1: return int4_run<T, 1, 1, 64, 4, 3>(a, blocks, st);
-    case 2: return int4_run<T, 2, 1, 64, 4, 3>(a, blocks, st);
-    case 3: return int4_run<T, 3, 1, 64, 4, 3>(a, blocks, st);
-    case 4: return int4_run<T, 4, 1, 64, 4, 3>(a, blocks, st);
+  if (shape.nt > 1) return attn_int4_launch_wide<T>(a, shape, blocks, st);
+  if (shape.keys == 16) return int4_run_dims<T, 1, 16, 4, 3>(a, blocks, st);
+  if (shape.warps == 12) return int4_run_dims<T, 1, 64, 12, 1>(a, blocks, st);
+  switch (a.p.head_dim / 32) {
     case 5: return int4_run<T, 5, 1, 32, 4, 2>(a, blocks, st);
     case 6: return int4_run<T, 6, 1, 32, 4, 2>(a, blocks, st);
     case 7: return int4_run<T, 7, 1, 32, 4, 2>(a, blocks, st);
     case 8: return int4_run<T, 8, 1, 32, 4, 2>(a, blocks, st);
   }
-  return cudaErrorInvalidValue;
+  return int4_run_dims<T, 1, 64, 4, 3>(a, blocks, st);
+}
+
+// Two or (half types) three column tiles, D up to 128.
+template <typename T>
+cudaError_t attn_int4_launch_wide(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (shape.nt == 3) return int4_run_dims<T, 3, 64, 4, 2>(a, blocks, st);
+  }
+  return int4_run_dims<T, 2, 64, 4, 2>(a, blocks, st);
 }
 
 }  // namespace tsa

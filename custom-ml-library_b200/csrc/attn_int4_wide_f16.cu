@@ -1,0 +1,6 @@
+// f16 instances of the attention over a 4-bit cache (attn_int4.cuh): several column tiles.
+#include "attn_int4_launch.cuh"
+
+namespace tsa {
+template cudaError_t attn_int4_launch_wide<__half>(const Int4Attn& a, const Int4Shape& shape, int blocks, cudaStream_t st);
+}  // namespace tsa

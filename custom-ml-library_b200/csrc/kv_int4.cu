@@ -6,6 +6,7 @@
 // them in flight: 64 bytes a thread for half types, which is what covers the memory latency.  The four
 // neighbouring threads of a scale group share its maximum by two shuffles.
 #include "int4.cuh"
+#include "ptx.cuh"
 
 namespace tsa {
 
@@ -62,27 +63,53 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// The largest |x| of 8 values, NaN if one is NaN: as pairs where the type allows it.
+__device__ __forceinline__ float amax8(const Raw8<float>& r) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(r.x[e]));
+  return m;
+}
+__device__ __forceinline__ float amax8(const Raw8<__half>& r) {
+  const __half2* p = reinterpret_cast<const __half2*>(r.x);
+  const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float amax8(const Raw8<__nv_bfloat16>& r) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(r.x);
+  const __nv_bfloat162 m =
+      __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+
 // The word of 8 channels whose group has the finite maximum amax <= 7 * kInt4ScaleMax, so that no quotient
 // passes 7.  fp32 inputs divide; half types multiply by the reciprocal and correct the quotient once with its
 // remainder (Markstein, IBM J. Res. Dev. 34, 1990), which yields the same correctly rounded quotient at a
-// third of the instructions.
+// third of the instructions, two values at a time.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float scale) {
   const float inv = __frcp_rn(scale);
+  const uint64_t inv2 = ptx::f2pack(inv, inv), minus2 = ptx::f2pack(-scale, -scale);
+  // Rounding half to even and adding 8 by a sum whose last place is 1: 1.5 * 2^23 + 8.  The eight sums' bits are
+  // added up at their nibbles' places; what their common upper bits add is one constant.
+  constexpr uint32_t kBits = 0x4B400000u;
+  const uint64_t magic2 = ptx::f2pack(12582920.f, 12582920.f);
   uint32_t word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float n;
+  for (int e = 6; e >= 0; e -= 2) {
+    float lo, hi;
     if constexpr (sizeof(T) == 4) {
-      n = __fdiv_rn(x[e], scale);
+      lo = __fdiv_rn(x[e], scale) + 12582920.f;
+      hi = __fdiv_rn(x[e + 1], scale) + 12582920.f;
     } else {
-      n = x[e] * inv;
-      n = fmaf(fmaf(-n, scale, x[e]), inv, n);
+      const uint64_t v = ptx::f2pack(x[e], x[e + 1]);
+      uint64_t n = ptx::fma2(v, inv2, 0ull);
+      n = ptx::fma2(ptx::fma2(n, minus2, v), inv2, n);
+      ptx::f2unpack(ptx::add2(n, magic2), lo, hi);
     }
-    // round half to even and add 8, by a sum whose last place is 1: 1.5 * 2^23 + 8
-    word |= (__float_as_uint(n + 12582920.f) & 15u) << (4 * e);
+    word = (word * 16u + __float_as_uint(hi)) * 16u + __float_as_uint(lo);
   }
-  return word;
+  return word - kBits * 0x11111111u;
 }
 
 template <typename T>
@@ -117,12 +144,9 @@ __global__ void kv_append_int4_kernel(Int4Rows a) {
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (t + u >= t1) break;
-      float x[8], amax = 0.f;
+      float x[8], amax = amax8(raw[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = Elem<T>::to_acc(raw[u].x[e]);
-        amax = max_nan(amax, fabsf(x[e]));
-      }
+      for (int e = 0; e < 8; ++e) x[e] = Elem<T>::to_acc(raw[u].x[e]);
       amax = max_nan(amax, __shfl_xor_sync(quad, amax, 1));
       amax = max_nan(amax, __shfl_xor_sync(quad, amax, 2));
       if (!(amax <= 7.f * kInt4ScaleMax)) {  // saturate, NaN to 0
