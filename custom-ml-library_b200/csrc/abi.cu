@@ -337,6 +337,7 @@ int check_int4_cache(const ts_kv4_cache* c) {
   if (!c || !c->pool || !c->table || reinterpret_cast<uintptr_t>(c->pool) % 16) return TS_ERR_INVALID_ARGUMENT;
   if (c->batch <= 0 || c->slots <= 0 || c->pages <= 0 || c->kv_heads <= 0) return TS_ERR_INVALID_ARGUMENT;
   if (!int4_shape_ok(c->head_dim, c->page_size)) return TS_ERR_UNSUPPORTED;
+  if ((int64_t)c->slots * c->page_size > 0x7FFFFF00) return TS_ERR_INVALID_ARGUMENT;  // token numbers are int32
   if (c->page_stride % 16 ||
       c->page_stride < (int64_t)c->kv_heads * tsa::int4_block_bytes(c->head_dim, c->page_size))
     return TS_ERR_INVALID_ARGUMENT;

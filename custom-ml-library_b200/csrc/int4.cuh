@@ -29,7 +29,11 @@ __host__ __device__ __forceinline__ int int4_block_bytes(int head_dim, int page_
 }
 
 __device__ __forceinline__ float int4_scale(float amax) {
-  const float s = fminf(__fdiv_rn(amax, 7.f), kInt4ScaleMax);
+  // amax / 7, correctly rounded: the quotient by 1/7's nearest float, corrected once with its remainder
+  // (Markstein, IBM J. Res. Dev. 34, 1990)
+  constexpr float seventh = 1.f / 7.f;
+  float s = amax * seventh;
+  s = fminf(fmaf(fmaf(-7.f, s, amax), seventh, s), kInt4ScaleMax);
   const float up = __uint_as_float((__float_as_uint(s) + 0x7FFFFu) & ~0x7FFFFu);
   return fminf(fmaxf(up, kInt4ScaleMin), kInt4ScaleMax);
 }
@@ -37,7 +41,7 @@ __device__ __forceinline__ float int4_scale(float amax) {
 // Page of row b's token, or -1 where the table has none (a bad entry is the caller's error: the
 // kernels record it in the fault word and leave the page alone).
 __device__ __forceinline__ int int4_page(const ts_kv4_cache& c, int b, int slot) {
-  if (slot < 0 || slot >= c.slots) return -1;
+  if ((unsigned)slot >= (unsigned)c.slots) return -1;
   const int page = c.table[(int64_t)b * c.table_stride + slot];
   return page >= 0 && page < c.pages ? page : -1;
 }

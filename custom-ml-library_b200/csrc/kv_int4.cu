@@ -84,11 +84,13 @@ __device__ __forceinline__ float amax8(const Raw8<__nv_bfloat16>& r) {
 
 // The word of 8 channels whose group has the finite maximum amax <= 7 * kInt4ScaleMax, so that no quotient
 // passes 7.  fp32 inputs divide; half types multiply by the reciprocal and correct the quotient once with its
-// remainder (Markstein, IBM J. Res. Dev. 34, 1990), which yields the same correctly rounded quotient at a
-// third of the instructions, two values at a time.
+// remainder (Markstein, IBM J. Res. Dev. 34, 1990), which yields the same correctly rounded quotient (checked
+// for every scale and every 11-bit value) at a third of the instructions, two values at a time.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float scale) {
-  const float inv = __frcp_rn(scale);
+  float inv;  // 1 / scale, correctly rounded: one Newton step from the approximation (checked for every scale)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+  inv = fmaf(fmaf(-scale, inv, 1.f), inv, inv);
   const uint64_t inv2 = ptx::f2pack(inv, inv), minus2 = ptx::f2pack(-scale, -scale);
   // Rounding half to even and adding 8 by a sum whose last place is 1: 1.5 * 2^23 + 8.  The eight sums' bits are
   // added up at their nibbles' places; what their common upper bits add is one constant.
@@ -112,6 +114,21 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float scale) 
   return word - kBits * 0x11111111u;
 }
 
+// The blocks of one head and kind that kInFlight tokens from p0 on fall into: two at most, as a page holds more.
+struct Span {
+  unsigned char *first, *second;  // nullptr: no page
+};
+__device__ __forceinline__ unsigned char* page_block(const ts_kv4_cache& c, int b, int slot, unsigned char* base) {
+  const int page = int4_page(c, b, slot);
+  return page < 0 ? nullptr : base + page * c.page_stride;
+}
+__device__ __forceinline__ Span token_span(const ts_kv4_cache& c, int b, int p0, int log2, unsigned char* base) {
+  Span s;
+  s.first = page_block(c, b, p0 >> log2, base);
+  s.second = (p0 + kInFlight - 1) >> log2 != p0 >> log2 ? page_block(c, b, (p0 >> log2) + 1, base) : s.first;
+  return s;
+}
+
 template <typename T>
 __global__ void kv_append_int4_kernel(Int4Rows a) {
   const ts_kv4_cache& c = a.c;
@@ -120,26 +137,25 @@ __global__ void kv_append_int4_kernel(Int4Rows a) {
   const int chunks = c.head_dim / 8, groups = c.head_dim / 32;
   const int items = c.kv_heads * 2 * chunks;  // a multiple of 4
   const int i = blockIdx.y * blockDim.x + threadIdx.x;
-  const int64_t pos = a.positions ? (int64_t)a.positions[b] : a.position;
-  if (t0 == 0 && i == 0 && a.positions_out) a.positions_out[b] = (int32_t)(pos + a.steps);
+  const int pos = a.positions ? a.positions[b] : (int)a.position;
+  if (t0 == 0 && i == 0 && a.positions_out) a.positions_out[b] = pos + a.steps;
   if (i >= items) return;
   const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
   const int g = chunk / 4, w = chunk % 4 * groups + g;
-  const int64_t block = int4_block_bytes(c.head_dim, c.page_size);
+  const int block = int4_block_bytes(c.head_dim, c.page_size), row = c.head_dim / 2;
   const ts_view4& v = kind ? a.value : a.key;
-  const T* src = reinterpret_cast<const T*>(v.data) + b * v.stride[0] + h * v.stride[1] +
+  const T* src = reinterpret_cast<const T*>(v.data) + b * v.stride[0] + h * v.stride[1] + t0 * v.stride[2] +
                  (int64_t)chunk * 8 * v.stride[3];
-  unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + h * block + kind * (block / 2);
+  unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + (int64_t)h * block + kind * (block / 2);
+  const int scales = c.page_size * row + g * 2, mask = c.page_size - 1;
   const uint32_t quad = 0xFu << (threadIdx.x & 28);
   for (int t = t0; t < t1; t += kInFlight) {
     Raw8<T> raw[kInFlight];
-    int page[kInFlight];
+    const Span span = token_span(c, b, pos + t, a.page_log2, base);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      if (t + u >= t1) break;
-      load8(src + (int64_t)(t + u) * v.stride[2], v.stride[3], a.vec, raw[u]);
-      const int64_t slot = (pos + t + u) >> a.page_log2;
-      page[u] = slot < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
+      if (t + u < t1) load8(src, v.stride[3], a.vec, raw[u]);
+      src += v.stride[2];
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
@@ -161,15 +177,14 @@ __global__ void kv_append_int4_kernel(Int4Rows a) {
       }
       const float scale = int4_scale(amax);
       const uint32_t word = quantise8<T>(x, scale);
-      if (page[u] < 0) {
+      const int p = pos + t + u, at = p & mask;
+      unsigned char* dst = (p ^ (pos + t)) >> a.page_log2 ? span.second : span.first;
+      if (!dst) {
         record_fault(a.fault, FAULT_PAGE);
         continue;
       }
-      const int at = (int)((pos + t + u) & (c.page_size - 1));
-      unsigned char* dst = base + page[u] * c.page_stride;
-      reinterpret_cast<uint32_t*>(dst + (int64_t)at * (c.head_dim / 2))[w] = word;
-      if (chunk % 4 == 0)
-        reinterpret_cast<__half*>(dst + c.page_size * (c.head_dim / 2))[at * groups + g] = __float2half_rn(scale);
+      reinterpret_cast<uint32_t*>(dst + at * row)[w] = word;
+      if (chunk % 4 == 0) *reinterpret_cast<__half*>(dst + scales + at * (row / 8)) = __float2half_rn(scale);
     }
   }
 }
@@ -183,42 +198,51 @@ __global__ void kv_gather_int4_kernel(Int4Rows a) {
   const int items = c.kv_heads * 2 * chunks;
   const int i = blockIdx.y * blockDim.x + threadIdx.x;
   if (i >= items) return;
-  const int64_t pos = a.positions ? (int64_t)a.positions[b] : 0;
-  const int64_t len = a.lens ? (int64_t)a.lens[b] : INT64_MAX;
+  const int pos = a.positions ? a.positions[b] : 0, len = a.lens ? a.lens[b] : INT32_MAX;
   const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
   const int g = chunk / 4, w = chunk % 4 * groups + g;
-  const int64_t block = int4_block_bytes(c.head_dim, c.page_size);
+  const int block = int4_block_bytes(c.head_dim, c.page_size), row = c.head_dim / 2;
   const ts_view4& v = kind ? a.value : a.key;
-  T* dst = reinterpret_cast<T*>(v.data) + b * v.stride[0] + h * v.stride[1] + (int64_t)chunk * 8 * v.stride[3];
-  const unsigned char* base = reinterpret_cast<const unsigned char*>(c.pool) + h * block + kind * (block / 2);
+  T* dst = reinterpret_cast<T*>(v.data) + b * v.stride[0] + h * v.stride[1] + t0 * v.stride[2] +
+           (int64_t)chunk * 8 * v.stride[3];
+  unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + (int64_t)h * block + kind * (block / 2);
+  const int scales = c.page_size * row + g * 2, mask = c.page_size - 1;
+  const int live = min(t1, max(t0, len - pos));  // tokens from here on are zeros
   for (int t = t0; t < t1; t += kInFlight) {
     uint32_t word[kInFlight];
-    __half scale[kInFlight];
+    float scale[kInFlight];
+    Span span{nullptr, nullptr};
+    if (t < live) span = token_span(c, b, pos + t, a.page_log2, base);
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       word[u] = 0x88888888u;
-      scale[u] = __ushort_as_half(0);
-      const int64_t at = pos + t + u, slot = at >> a.page_log2;
-      if (t + u >= t1 || at >= len) continue;
-      const int page = slot < 0 || slot >= c.slots ? -1 : int4_page(c, b, (int)slot);
-      if (page < 0) {
+      scale[u] = 0.f;
+      if (t + u >= live) continue;
+      const int p = pos + t + u, at = p & mask;
+      const unsigned char* src = (p ^ (pos + t)) >> a.page_log2 ? span.second : span.first;
+      if (!src) {
         record_fault(a.fault, FAULT_PAGE);
         continue;
       }
-      const int in = (int)(at & (c.page_size - 1));
-      const unsigned char* src = base + page * c.page_stride;
-      word[u] = reinterpret_cast<const uint32_t*>(src + (int64_t)in * (c.head_dim / 2))[w];
-      scale[u] = reinterpret_cast<const __half*>(src + c.page_size * (c.head_dim / 2))[in * groups + g];
+      word[u] = reinterpret_cast<const uint32_t*>(src + at * row)[w];
+      scale[u] = __half2float(*reinterpret_cast<const __half*>(src + scales + at * (row / 8)));
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       if (t + u >= t1) break;
-      const float s = __half2float(scale[u]);
+      const uint64_t scale2 = ptx::f2pack(scale[u], scale[u]);
       Raw8<T> raw;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // the nibble under 2^23's exponent: 2^23 + n + 8
-        raw.x[e] = Elem<T>::from_acc((__uint_as_float((word[u] >> (4 * e) & 15u) | 0x4B000000u) - 8388616.f) * s);
-      store8(dst + (int64_t)(t + u) * v.stride[2], v.stride[3], a.vec, raw);
+      for (int e = 0; e < 8; e += 2) {  // the nibbles under 2^23's exponent: 2^23 + n + 8
+        const uint64_t n = ptx::f2pack(__uint_as_float((word[u] >> (4 * e) & 15u) | 0x4B000000u),
+                                       __uint_as_float((word[u] >> (4 * e + 4) & 15u) | 0x4B000000u));
+        float lo, hi;
+        ptx::f2unpack(ptx::fma2(ptx::add2(n, ptx::f2pack(-8388616.f, -8388616.f)), scale2, 0ull), lo, hi);
+        raw.x[e] = Elem<T>::from_acc(lo);
+        raw.x[e + 1] = Elem<T>::from_acc(hi);
+      }
+      store8(dst, v.stride[3], a.vec, raw);
+      dst += v.stride[2];
     }
   }
 }

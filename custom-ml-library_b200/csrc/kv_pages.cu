@@ -112,6 +112,7 @@ cudaError_t kv_pages_copy(const ts_page_pool& src, const ts_page_pool& dst, cons
 __global__ void kv_fork_kernel(const int32_t* table, int64_t table_stride, const int32_t* lens, int rows,
                                const int32_t* index, int32_t* table_out, int64_t table_out_stride, int32_t* lens_out,
                                int rows_out, int slots, int page_size, int32_t* refs, int pages, int32_t* counters) {
+  let_next_start();
   const int r = blockIdx.x;
   int freed = 0, lowest = pages;
   if (r < rows_out) {
@@ -188,20 +189,25 @@ __device__ __forceinline__ int reserve_partial(const ReserveArgs& a, int r) {
   return page >= 0 && page < a.pages ? page : -1;
 }
 
-// One block: the tables are small and the order of the hand-out runs through all rows.
+// One block: the tables are small and the order of the hand-out runs through all rows.  What bounds it is the
+// chain of dependent loads, so a thread keeps what it knows of its first row.
 __global__ void __launch_bounds__(kScanThreads) kv_reserve_kernel(ReserveArgs a) {
   __shared__ int warp_sums[32];
   __shared__ int too_long;
   let_next_start();
+  wait_for_previous();
   const int tid = threadIdx.x;
   if (tid == 0) too_long = 0;
+  const int own_page = tid < a.rows ? reserve_partial(a, tid) : -1;
+  auto partial = [&](int r) { return r == tid ? own_page : reserve_partial(a, r); };
+  const int first_free = a.counters[1], n_free = a.counters[0];
   for (int r = tid; r < a.rows; r += kScanThreads) {
-    const int page = reserve_partial(a, r);
+    const int page = partial(r);
     if (page >= 0) a.writers[page] = a.last[page] = 0;
   }
   __syncthreads();
   for (int r = tid; r < a.rows; r += kScanThreads) {
-    const int page = reserve_partial(a, r);
+    const int page = partial(r);
     if (page >= 0) {
       atomicAdd(&a.writers[page], 1);
       atomicMax(&a.last[page], r + 1);
@@ -215,7 +221,7 @@ __global__ void __launch_bounds__(kScanThreads) kv_reserve_kernel(ReserveArgs a)
     int need = 0;
     bool copy = false;
     if (r < a.rows) {
-      const int page = reserve_partial(a, r);
+      const int page = partial(r);
       copy = page >= 0 && (a.refs[page] > a.writers[page] || r + 1 < a.last[page]);
       need = copy ? 1 : 0;
       const int64_t len = max(0, a.lens[r]), stop = len + reserve_steps(a, r);
@@ -236,14 +242,14 @@ __global__ void __launch_bounds__(kScanThreads) kv_reserve_kernel(ReserveArgs a)
     total += sum;
   }
   __syncthreads();
-  const bool short_of_pages = total > a.counters[0];
+  const bool short_of_pages = total > n_free;
   if (too_long || short_of_pages) {
     if (tid == 0) atomicOr(&a.counters[2], too_long ? kErrSlots : kErrPages);
     return;  // pairs[][1] is -1 everywhere, so nothing is copied either
   }
   // The lowest free pages.
-  int found = 0, next = a.counters[1];
-  for (int64_t base = next; found < total && base < a.pages; base += kScanThreads * 4) {
+  int found = 0;
+  for (int64_t base = first_free; found < total && base < a.pages; base += kScanThreads * 4) {
     int free4 = 0, ex;
     const int64_t p0 = base + tid * 4;
 #pragma unroll
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kScanThreads) kv_reserve_kernel(ReserveArgs a)
       }
   }
   if (tid == 0 && total > 0) {
-    a.counters[0] -= total;
+    a.counters[0] = n_free - total;
     a.counters[1] = a.list[total - 1] + 1;
   }
 }
@@ -313,8 +319,8 @@ cudaError_t kv_pages_reserve(const ts_page_pool& pool, int32_t* table, int64_t t
   a.pages = pool.pages;
   a.page_size = page_size;
   a.steps = steps;
-  kv_reserve_kernel<<<1, kScanThreads, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  // usually right behind a fork, whose end it may await on the SM
+  const cudaError_t e = launch_dependent(kv_reserve_kernel, dim3(1), dim3(kScanThreads), 0, st, a);
   if (e != cudaSuccess) return e;
   return launch_copy(pool, pool, a.pairs, a.pairs + 1, 2, rows, nullptr, true, st);
 }
