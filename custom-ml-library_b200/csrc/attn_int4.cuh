@@ -19,8 +19,8 @@
 //   V scale on the operand: n * scale = (64 + nibble) scale - 72 scale, exact in one multiply-add
 //   q       times a power of two that puts its largest element in [2^14, 2^15): exact for bf16 and
 //           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
-//   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo, since the 2^-12 of one fp16 part is
-//           as large as the output's own rounding there
+//   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo,
+//           since the 2^-12 of one fp16 part is as large as the output's own rounding there
 // The rows of the K tile are permuted within 8 tokens so that the P^T fragment (one transposing
 // register move of S^T's) meets V rows whose shared-memory reads do not collide, see token_of_row.
 #pragma once
@@ -130,10 +130,13 @@ __device__ __forceinline__ int token_of_row(int r) { return r & 1 ? 4 + ((r >> 1
 }  // namespace
 
 // What a lane holds of its query columns and of their running softmax.
-template <typename T, int DG, int NT>
+// kTwin: at most 4 columns, each held twice; the second of a column takes the other fp16 part of p, so that
+// one product serves both parts.
+template <typename T, int DG, int NT, bool kTwin>
 struct Int4State {
   static constexpr int QP = sizeof(T) == 4 ? 2 : 1;                          // fp16 parts of q
-  static constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;   // fp16 parts of p
+  static constexpr int PP = std::is_same<T, __nv_bfloat16>::value || kTwin ? 1 : 2;  // products with p's fp16 parts
+  static constexpr int kColumns = kTwin ? 4 : 8 * NT;
   static constexpr int NW = (DG + 1) / 2;                                    // V words a lane takes of a row
   static constexpr bool kQueriesShared = NT > 1;  // several tiles' query fragments wait in shared memory
   // Tiles of 16 keys whose scores and probabilities are held at a time: what the registers leave room for.
@@ -214,10 +217,10 @@ __device__ __forceinline__ Int4Tiles int4_tiles(int unit, int row, int scale_row
 
 // One stage: KT tokens at st, the first of them key0.  kEdge: some column does not see
 // all of them, or the split ends among them.
-template <bool kEdge, typename T, int DG, int NT, int KT>
-__device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsigned char* st,
+template <bool kEdge, typename T, int DG, int NT, bool kTwin, int KT>
+__device__ __forceinline__ void int4_stage(Int4State<T, DG, NT, kTwin>& q, const unsigned char* st,
                                            const Int4Tiles& at, int key0, int k_end) {
-  using State = Int4State<T, DG, NT>;
+  using State = Int4State<T, DG, NT, kTwin>;
   constexpr int D = DG * 32, NW = State::NW, kRow = D / 2, kScaleRow = D / 16;
   constexpr int kTiles = KT / 16 < State::kChunk ? KT / 16 : State::kChunk;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -324,7 +327,12 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
       ptx::f2unpack(ptx::fma2(ptx::f2pack(x[2], x[3]), cs2, base2), p2, p3);
       p0 = ptx::ex2(p0), p1 = ptx::ex2(p1), p2 = ptx::ex2(p2), p3 = ptx::ex2(p3);
       sum2 = ptx::add2(sum2, ptx::add2(ptx::f2pack(p0, p1), ptx::f2pack(p2, p3)));
-      const __half2 ha = __floats2half2_rn(p0, p1), hb = __floats2half2_rn(p2, p3);
+      __half2 ha = __floats2half2_rn(p0, p1), hb = __floats2half2_rn(p2, p3);
+      if constexpr (kTwin) {  // the second columns (t >= 2) keep what the first ones' rounding leaves
+        const float rest = t >= 2 ? -1.f : 0.f;
+        ha = __floats2half2_rn(fmaf(rest, __low2float(ha), p0), fmaf(rest, __high2float(ha), p1));
+        hb = __floats2half2_rn(fmaf(rest, __low2float(hb), p2), fmaf(rest, __high2float(hb), p3));
+      }
       pf[0][nt][tile][0] = transpose8x8(h2_bits(ha));
       pf[0][nt][tile][1] = transpose8x8(h2_bits(hb));
       if constexpr (State::PP == 2) {
@@ -392,14 +400,14 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT>& q, const unsign
 }
 
 // Reads a block of query columns and clears their running softmax.
-template <typename T, int DG, int NT>
-__device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T, DG, NT>& q, int b, int hk, int col0,
+template <typename T, int DG, int NT, bool kTwin>
+__device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T, DG, NT, kTwin>& q, int b, int hk, int col0,
                                                   int len) {
-  using State = Int4State<T, DG, NT>;
+  using State = Int4State<T, DG, NT, kTwin>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int col = col0 + nt * 8 + g;
+    const int col = kTwin ? g & 3 : col0 + nt * 8 + g;
     const bool live = col < a.cols;
     const int i = live ? col / a.group : 0, h = hk * a.group + (live ? col - i * a.group : 0);
     const T* qp = reinterpret_cast<const T*>(a.p.q.data) + b * a.p.q.stride[0] + h * a.p.q.stride[1] +
@@ -466,7 +474,8 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int tok = min(col0 + nt * 8 + 2 * t + j, a.cols - 1) / a.group;
+      const int mine = kTwin ? (2 * t + j) & 3 : col0 + nt * 8 + 2 * t + j;
+      const int tok = min(mine, a.cols - 1) / a.group;
       q.limit[nt][j] = a.p.is_causal ? max(-1, len - a.p.q_len + tok) : len - 1;
       q.m[nt][j] = -INFINITY;
       q.l[nt][j] = 0.f;
@@ -479,10 +488,10 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
 }
 
 // Writes the columns' results: to the output when the warp saw all of their keys, else to a partial slot.
-template <typename T, int DG, int NT>
-__device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, NT>& q, int b, int hk, int col0,
+template <typename T, int DG, int NT, bool kTwin>
+__device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, NT, kTwin>& q, int b, int hk, int col0,
                                            int slot) {
-  constexpr int D = DG * 32, NW = Int4State<T, DG, NT>::NW;
+  constexpr int D = DG * 32, NW = Int4State<T, DG, NT, kTwin>::NW;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -493,7 +502,14 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       const int local = nt * 8 + 2 * t + j, col = col0 + local;
-      if (col >= a.cols) continue;
+      if constexpr (kTwin) {
+#pragma unroll
+        for (int k = 0; k < 4 * NW; ++k) {
+          q.acc[nt][k][j] += __shfl_xor_sync(0xffffffffu, q.acc[nt][k][j], 2);
+          q.acc[nt][k][j + 2] += __shfl_xor_sync(0xffffffffu, q.acc[nt][k][j + 2], 2);
+        }
+      }
+      if (col >= a.cols || local >= Int4State<T, DG, NT, kTwin>::kColumns) continue;
       const int tok = col / a.group, h = hk * a.group + col - tok * a.group;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       float* part = slot < 0 ? nullptr : a.ws_acc + ((int64_t)slot * a.slot_cols + local) * D;
@@ -540,7 +556,7 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
 // by_pair gives every pair a block of its own: nothing is left to merge, so the second launch falls away.)  Each warp runs its own ring of bulk copies through its whole
 // share, the next row's first stages in flight while it finishes the last one; no block barrier runs
 // between the start and the merge.
-template <typename T, int DG, int NT, int KT, int kStages, int kWarps, int kMinBlocks>
+template <typename T, int DG, int NT, bool kTwin, int KT, int kStages, int kWarps, int kMinBlocks>
 __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(const __grid_constant__ Int4Attn a) {
   constexpr int D = DG * 32;
   constexpr int kRowBytes = D / 2 + D / 16, kStageBytes = 2 * KT * kRowBytes;
@@ -550,7 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   unsigned char* ring = smem + warp * (kStages * kStageBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes) + warp * kStages;
   static_assert(kStages * sizeof(uint64_t) == 16, "");
-  using State = Int4State<T, DG, NT>;
+  using State = Int4State<T, DG, NT, kTwin>;
   constexpr int kQueryBytes = State::kQueriesShared ? State::QP * NT * DG * 512 : 0;
   unsigned char* queries = smem + kWarps * kStages * kStageBytes + kWarps * 16;
   int* first = reinterpret_cast<int*>(queries + kWarps * kQueryBytes);
@@ -722,9 +738,9 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
       }
       const unsigned char* st = ring + (n % kStages) * kStageBytes;
       if (key0 + KT <= plain)
-        int4_stage<false, T, DG, NT, KT>(q, st, tiles, key0, len);
+        int4_stage<false, T, DG, NT, kTwin, KT>(q, st, tiles, key0, len);
       else
-        int4_stage<true, T, DG, NT, KT>(q, st, tiles, key0, len);
+        int4_stage<true, T, DG, NT, kTwin, KT>(q, st, tiles, key0, len);
       __syncwarp();  // every lane is done with the stage before it is filled again
     }
     if (ok && !together)
@@ -738,7 +754,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   float2* ml = reinterpret_cast<float2*>(red + kWarps * kCols * kPad);
   const int g = lane >> 2, t = lane & 3;
   const int hk = home.pair / a.col_blocks, col0 = (home.pair - hk * a.col_blocks) * NT * 8;
-  const int n_cols = min(kCols, a.cols - col0);
+  const int n_cols = min(State::kColumns, a.cols - col0);
   if (!__syncthreads_and(ok)) return;
   if (mine <= 0) {
     for (int i = lane; i < kCols; i += 32) ml[warp * kCols + i] = make_float2(-INFINITY, 0.f);
@@ -756,7 +772,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           const int word = g * NW + w, ch = 32 * (word % DG) + 8 * (word / DG);
-          if ((DG % 2 && word >= D / 8) || nt * 8 + 2 * t + j >= n_cols) continue;
+          if ((DG % 2 && word >= D / 8) || (kTwin ? (2 * t + j) & 3 : nt * 8 + 2 * t + j) >= n_cols) continue;
 #pragma unroll
           for (int e = 0; e < 8; e += 4)
             *reinterpret_cast<float4*>(&red[col * kPad + ch + e]) =
@@ -778,6 +794,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
       const float f = ptx::ex2(x.x - base);
       sum += x.y * f;
       out += red[(w * kCols + col) * kPad + d] * f;
+      if (kTwin) out += red[(w * kCols + col + 4) * kPad + d] * f;
     }
     const int tok = (col0 + col) / a.group, h = hk * a.group + col0 + col - tok * a.group;
     if (all) {
@@ -881,6 +898,7 @@ struct Int4Shape {
   int warps;   // of a block
   int blocks;  // resident on an SM
   bool by_pair;
+  bool twin;   // columns held twice
 };
 Int4Shape int4_shape(const ts_attn_params& p);
 
