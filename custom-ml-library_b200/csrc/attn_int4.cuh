@@ -13,10 +13,14 @@
 // (mma.sync: a fragment is built in registers straight from the nibbles, while tcgen05 would want
 // the dequantised tile written to shared memory first, four times the bytes.)  Everything is fp16 in
 // the products and fp32 in the sums and statistics:
-//   n       by putting the nibble into the mantissa of a power of two, 0x6400 | nibble = 1024 + nibble
-//           or 0x5400 | nibble << 4 = 64 + nibble, and subtracting: a logic op and an addition a pair
-//   K scale on the fp32 sum of each 32-channel group
-//   V scale on the operand: n * scale = (64 + nibble) scale - 72 scale, exact in one multiply-add
+//   K       (one column tile) the masked nibbles themselves: a nibble in the low bits of a half is the subnormal nibble * 2^-24, in
+//           the next four bits nibble * 2^-20, so the queries of the odd ones are a sixteenth; one logic op a
+//           pair.  What the nibbles' offset of 8 adds to a 32-channel group's product is a constant of the
+//           column, the accumulator's start.  The group's scale goes on its fp32 sum.  (Two and three tiles
+//           subtract instead, as V does: 59 against 63 us for 20 columns)
+//   V       needs its scale on the operand: the nibble in the mantissa of a power of two, 0x6400 | nibble = 1024 +
+//           nibble or 0x5400 | nibble << 4 = 64 + nibble, then n * scale = (64 + nibble) scale - 72 scale, exact
+//           in one multiply-add (for the other a subtraction and a product)
 //   q       times a power of two that puts its largest element in [2^14, 2^15): exact for bf16 and
 //           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
 //   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo,
@@ -58,8 +62,10 @@ __device__ __forceinline__ int int4_len(const Int4Attn& a, int b) { return min(a
 // The shares count n + 1 units for a pair (KV head and column block) of a row with n stages: entering it
 // (its queries read, its result written) takes a warp about as long as a stage.  Unit 0 of a pair is the
 // entry, unit i + 1 its stage i.  Worker w takes the units [w * share, (w + 1) * share): the first `block_warps`
-// warps of each block, which are fewer than the block has where a short line would else leave SMs idle (but
-// no fewer than four, whose parts merge on the SM).
+// warps of each block, which are fewer than the block has where a short line would else leave SMs idle (but no
+// fewer than four, whose parts merge on the SM).  Shares of one size leave some workers idle; shares that differ
+// by a unit kept all of them busy and lost more to the extra parts (two rows of up to 131072 keys: 34.7 against
+// 31.4 us).
 struct Int4Shares {
   int block_warps, share;
 };
@@ -89,12 +95,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// d = A B: a zero accumulator as an operand, where writing zeros to d first would cost four moves.
+// d = A B + c, one c a column: an operand of its own, where writing it to d first would cost four moves.
 __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                                               uint32_t b0, uint32_t b1, float2 c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -104,6 +110,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 
+constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;  // nibbles 0 and 4 of a word, 1 and 5
+
 // (x & mask) | magic, one three-input logic op.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t y;
@@ -112,8 +120,8 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t m
 }
 // Nibbles 0 and 4 of a word as the fp16 pair 1024 + nibble (the nibble in the last four mantissa bits),
 // nibbles 1 and 5 as 64 + nibble (in the four bits above them, no shift).
-__device__ __forceinline__ uint32_t biased_low(uint32_t w) { return and_or(w, 0x000F000Fu, 0x64006400u); }
-__device__ __forceinline__ uint32_t biased_high(uint32_t w) { return and_or(w, 0x00F000F0u, 0x54005400u); }
+__device__ __forceinline__ uint32_t biased_low(uint32_t w) { return and_or(w, kLow, 0x64006400u); }
+__device__ __forceinline__ uint32_t biased_high(uint32_t w) { return and_or(w, kHigh, 0x54005400u); }
 // The same pairs as the values n = nibble - 8.
 __device__ __forceinline__ uint32_t value_low(uint32_t w) {
   return h2_bits(__hsub2(bits_h2(biased_low(w)), __float2half2_rn(1032.f)));
@@ -142,6 +150,9 @@ struct Int4State {
   // Tiles of 16 keys whose scores and probabilities are held at a time: what the registers leave room for.
   static constexpr int kChunk = NT == 1 ? 4 : NT == 2 ? 2 : 1;
   uint32_t qf[kQueriesShared ? 1 : QP][kQueriesShared ? 1 : DG][4];
+  // One tile multiplies the masked nibbles (of several, the offsets below would cost more than they save).
+  static constexpr bool kMaskedK = NT == 1;
+  float qb[kMaskedK ? DG : 1][2];  // what the nibbles' 8 takes from a group's products, columns 2t and 2t + 1
   uint32_t qs;  // shared address of [QP, NT, DG, 32 lanes] x 16 bytes, this lane's first
   __device__ __forceinline__ uint4 fragment(int part, int nt, int gr) const {
     if constexpr (kQueriesShared) {
@@ -252,15 +263,23 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT, kTwin>& q, const
 #pragma unroll
     for (int gr = 0; gr < DG; ++gr) {
       const uint32_t va = wa[gr] >> 8, vb = wb[gr] >> 8;
-      const uint32_t k[8] = {value_low(wa[gr]), value_low(wb[gr]), value_high(wa[gr]), value_high(wb[gr]),
-                             value_low(va),     value_low(vb),     value_high(va),     value_high(vb)};
+      uint32_t k[8];
+      float2 offset = make_float2(0.f, 0.f);
+      if constexpr (State::kMaskedK) {
+        k[0] = wa[gr] & kLow, k[1] = wb[gr] & kLow, k[2] = wa[gr] & kHigh, k[3] = wb[gr] & kHigh;
+        k[4] = va & kLow, k[5] = vb & kLow, k[6] = va & kHigh, k[7] = vb & kHigh;
+        offset = make_float2(q.qb[gr][0], q.qb[gr][1]);
+      } else {
+        k[0] = value_low(wa[gr]), k[1] = value_low(wb[gr]), k[2] = value_high(wa[gr]), k[3] = value_high(wb[gr]);
+        k[4] = value_low(va), k[5] = value_low(vb), k[6] = value_high(va), k[7] = value_high(vb);
+      }
       const float sa = scale_float(ha[gr / 2], gr), sb = scale_float(hb[gr / 2], gr);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float dot[4];
         constexpr int kLast = State::QP - 1;  // the smaller part first
         uint4 b = q.fragment(kLast, nt, gr);
-        mma16816_first(dot, k[0], k[1], k[2], k[3], b.x, b.y);
+        mma16816_first(dot, k[0], k[1], k[2], k[3], b.x, b.y, offset);
         mma16816(dot, k[4], k[5], k[6], k[7], b.z, b.w);
         if constexpr (kLast > 0) {
           b = q.fragment(0, nt, gr);
@@ -443,7 +462,9 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     // the products, q becomes zero (a zero factor would make NaN of a hidden key's -inf).
     const float scale = (float)a.p.scale * kInt4Log2e;
     const int up_exp = min(253, max(1, 268 - (int)(__float_as_uint(amax) >> 23)));
-    float unit = __uint_as_float((uint32_t)(254 - up_exp) << 23) * fabsf(scale);
+    // Products of masked nibbles come out times 2^-24.  (A query beyond 8e34 would take their factor past fp32; held at its end
+    // it is still the largest score that stands alone.)
+    float unit = fminf(__uint_as_float((uint32_t)(254 - up_exp) << 23) * fabsf(scale) * (State::kMaskedK ? 0x1p24f : 1.f), 3.4e38f);
     float up = __uint_as_float((uint32_t)up_exp << 23) * (scale < 0.f ? -1.f : 1.f);
     if (unit == 0.f) up = 0.f, unit = 1.f;
     if (!(amax < INFINITY)) unit = __int_as_float(0x7fc00000);  // a non-finite query gives NaN, as its product would
@@ -453,23 +474,37 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
 #pragma unroll
     for (int gr = 0; gr < DG; ++gr) {
       uint32_t f[State::QP][4];
+      float sum = 0.f;  // of the parts as they are multiplied, the odd ones times 16
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float lo = x[gr][e] * up, hi = x[gr][e + 4] * up;
+        const float sixteenth = State::kMaskedK && e & 1 ? 0.0625f : 1.f, lo = x[gr][e] * up * sixteenth, hi = x[gr][e + 4] * up * sixteenth;
         const __half2 part = __floats2half2_rn(lo, hi);
         f[0][e] = h2_bits(part);
-        if constexpr (State::QP == 2)
-          f[1][e] = h2_bits(__floats2half2_rn(lo - __low2float(part), hi - __high2float(part)));
+        float both = __low2float(part) + __high2float(part);
+        if constexpr (State::QP == 2) {
+          const __half2 rest = __floats2half2_rn(lo - __low2float(part), hi - __high2float(part));
+          f[1][e] = h2_bits(rest);
+          both += __low2float(rest) + __high2float(rest);
+        }
+        sum = fmaf(both, e & 1 ? 16.f : 1.f, sum);
       }
+      if constexpr (State::kMaskedK) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -8.f * 0x1p-24f;
 #pragma unroll
-      for (int part = 0; part < State::QP; ++part) {
-        if constexpr (State::kQueriesShared) {  // read back by this lane alone
+        for (int j = 0; j < 2; ++j) q.qb[gr][j] = __shfl_sync(0xffffffffu, sum, (2 * t + j) * 4);
+      }
+      if constexpr (State::kQueriesShared) {  // read back by this lane alone
+#pragma unroll
+        for (int part = 0; part < State::QP; ++part)
           asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(q.qs + ((part * NT + nt) * DG + gr) * 512),
                        "r"(f[part][0]), "r"(f[part][1]), "r"(f[part][2]), "r"(f[part][3]));
-        } else {
+      } else {
+#pragma unroll
+        for (int part = 0; part < State::QP; ++part)
 #pragma unroll
           for (int e = 0; e < 4; ++e) q.qf[part][gr][e] = f[part][e];
-        }
       }
     }
 #pragma unroll
@@ -610,7 +645,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   int begin, mine;  // this warp's first stage and their number
   int block_mine;   // the block's
   int block_id = 0, id = 0;  // the block's first worker, this warp's
-  int share = 0, total = 0, total_units = 0;
+  int total = 0, total_units = 0;
   auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
     int lo = 0, hi = a.p.batch - 1;
     while (lo < hi) {
@@ -644,21 +679,20 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     home.pair = blockIdx.x - home.b * pairs;
     home.st = 0;
     home.n_st = block_mine = ceil_div(int4_len(a, home.b), KT);
-    share = ceil_div(block_mine, kWarps);
+    const int share = ceil_div(block_mine, kWarps);
     begin = min(warp * share, block_mine);
     mine = min(share, block_mine - begin);
   } else {
     total = first[a.p.batch];
     total_units = first_unit[a.p.batch];
     const Int4Shares shares = int4_shares(a, total_units, kWarps);
-    share = shares.share;
+    const int share = shares.share;
     block_id = blockIdx.x * shares.block_warps;
     id = block_id + warp;
     begin = stages_before((int64_t)id * share);
     mine = warp < shares.block_warps ? stages_before((int64_t)(id + 1) * share) - begin : 0;
-    const int64_t block_units = (int64_t)shares.block_warps * share;
-    const int block_begin = stages_before(blockIdx.x * block_units);
-    block_mine = stages_before((blockIdx.x + 1) * block_units) - block_begin;
+    const int block_begin = stages_before((int64_t)block_id * share);
+    block_mine = stages_before((int64_t)(block_id + shares.block_warps) * share) - block_begin;
     if (block_mine <= 0) return;
     home = place(block_begin);
   }
@@ -845,9 +879,10 @@ __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__
     const int head = m0 ? 0 : min(w1, c0 * warps + warps - 1) - w0 + 1;
     const int lo = m0 ? c0 : c0 + 1, mid = max(0, (m1 ? c1 : c1 - 1) - lo + 1);
     const int tail = c1 != c0 && !m1 ? w1 - c1 * warps + 1 : 0;
+    const bool late = (int64_t)w0 * share < enter;  // the row is not the first thing of its first worker
     auto slot = [&](int i) {
       const int w = i < head ? w0 + i : i < head + mid ? (lo + i - head) * warps : c1 * warps + i - head - mid;
-      return (int64_t)(2 * w + ((int64_t)w * share < enter)) * a.slot_cols + local;
+      return (int64_t)(2 * w + (late && w == w0)) * a.slot_cols + local;
     };
     const float2* all_ml = reinterpret_cast<const float2*>(a.ws_ml);
 #pragma unroll 4
