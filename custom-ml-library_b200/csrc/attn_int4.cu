@@ -31,7 +31,7 @@ int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
   const int blocks = a.by_pair ? (int)pairs
                                : (int)i64min(pairs * ceil_div(p.kv_len, shape.keys), (int64_t)sm_count() * shape.blocks);
   a.blocks = blocks;
-  a.parts = (int)(blocks / pairs);
+  a.parts = (int)i64min((int64_t)blocks * shape.warps / pairs, 1 << 20);
   return blocks;
 }
 
@@ -39,11 +39,6 @@ size_t partial_bytes(const Int4Attn& a, const Int4Shape& shape, int head_dim) {
   return (size_t)2 * a.blocks * shape.warps * a.slot_cols * (head_dim + 2) * sizeof(float);
 }
 }  // namespace
-
-bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c) {
-  if (p.dtype != TS_BF16 && p.dtype != TS_F16 && p.dtype != TS_F32) return false;
-  return c.page_size == 16 || c.page_size == 32 || c.page_size == 64;
-}
 
 Int4Shape int4_shape(const ts_attn_params& p) {
   const int cols = p.q_heads / p.kv_heads * p.q_len;

@@ -50,7 +50,7 @@ struct Int4Attn {
   int slot_cols;   // columns of a block that can be live
   int blocks;      // that share the work
   bool by_pair;    // one block a (row, KV head, column block) instead of equal shares
-  int parts;       // about how many blocks share a row at the longest length
+  int parts;       // about how many warps share a row where rows are of one length
   bool q_vec, o_vec;  // rows of unit stride and 16-byte alignment
   float* ws_acc;   // [2 * warps of all blocks, slot_cols, D] partial results
   float* ws_ml;    // [2 * warps of all blocks, slot_cols, 2]
@@ -418,11 +418,14 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT, kTwin>& q, const
   }
 }
 
-// Reads a block of query columns and clears their running softmax.
+// A lane's elements of a block of query columns, as they are in memory.
+template <typename T, int DG, int NT>
+struct Int4Queries {
+  alignas(16) T x[NT][DG][8];
+};
+
 template <typename T, int DG, int NT, bool kTwin>
-__device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T, DG, NT, kTwin>& q, int b, int hk, int col0,
-                                                  int len) {
-  using State = Int4State<T, DG, NT, kTwin>;
+__device__ __forceinline__ void int4_fetch_queries(const Int4Attn& a, Int4Queries<T, DG, NT>& raw, int b, int hk, int col0) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -431,25 +434,37 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     const int i = live ? col / a.group : 0, h = hk * a.group + (live ? col - i * a.group : 0);
     const T* qp = reinterpret_cast<const T*>(a.p.q.data) + b * a.p.q.stride[0] + h * a.p.q.stride[1] +
                   i * a.p.q.stride[2];
-    float x[DG][8], amax = 0.f;
-    bool odd = false;  // a NaN anywhere in the row
 #pragma unroll
     for (int gr = 0; gr < DG; ++gr) {
       const T* src = qp + (int64_t)(32 * gr + 8 * t) * a.p.q.stride[3];
       if (a.q_vec) {
-        alignas(16) T raw[8];
 #pragma unroll
         for (int e = 0; e < (int)(8 * sizeof(T) / 16); ++e)
-          reinterpret_cast<uint4*>(raw)[e] = reinterpret_cast<const uint4*>(src)[e];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[gr][e] = Elem<T>::to_acc(raw[e]);
+          reinterpret_cast<uint4*>(raw.x[nt][gr])[e] = reinterpret_cast<const uint4*>(src)[e];
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[gr][e] = Elem<T>::to_acc(src[e * a.p.q.stride[3]]);
+        for (int e = 0; e < 8; ++e) raw.x[nt][gr][e] = src[e * a.p.q.stride[3]];
       }
+    }
+  }
+}
+
+// Turns a block of query columns into operands and clears their running softmax.
+template <typename T, int DG, int NT, bool kTwin>
+__device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T, DG, NT, kTwin>& q,
+                                                  const Int4Queries<T, DG, NT>& raw, int col0, int len) {
+  using State = Int4State<T, DG, NT, kTwin>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const bool live = (kTwin ? g & 3 : col0 + nt * 8 + g) < a.cols;
+    float x[DG][8], amax = 0.f;
+    bool odd = false;  // a NaN anywhere in the row
+#pragma unroll
+    for (int gr = 0; gr < DG; ++gr) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[gr][e] = live ? x[gr][e] : 0.f;
+        x[gr][e] = live ? Elem<T>::to_acc(raw.x[nt][gr][e]) : 0.f;
         amax = fmaxf(amax, fabsf(x[gr][e]));
         odd |= x[gr][e] != x[gr][e];
       }
@@ -615,6 +630,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   }
   int* first_unit = first + a.p.batch + 1;
   let_next_start();
+  wait_for_previous();
   if (warp == 0 && !a.by_pair) {  // stages and units of the rows before b
     int stages = 0, rows = 0;
     for (int b0 = 0; b0 <= a.p.batch; b0 += 32) {
@@ -643,7 +659,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   };
   Place home;       // of the block's first stage
   int begin, mine;  // this warp's first stage and their number
-  int block_mine;   // the block's
+  int block_begin = 0, block_mine;  // the block's
   int block_id = 0, id = 0;  // the block's first worker, this warp's
   int total = 0, total_units = 0;
   auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
@@ -689,26 +705,25 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     const int share = shares.share;
     block_id = blockIdx.x * shares.block_warps;
     id = block_id + warp;
-    begin = stages_before((int64_t)id * share);
-    mine = warp < shares.block_warps ? stages_before((int64_t)(id + 1) * share) - begin : 0;
-    const int block_begin = stages_before((int64_t)block_id * share);
-    block_mine = stages_before((int64_t)(block_id + shares.block_warps) * share) - block_begin;
+    // The four bounds on four lanes at once: one after the other these searches took 2 us of the start.
+    const int worker = lane == 0 ? id : lane == 1 ? id + 1 : lane == 2 ? block_id : block_id + shares.block_warps;
+    const int bound = stages_before((int64_t)worker * share);
+    begin = __shfl_sync(0xffffffffu, bound, 0);
+    mine = warp < shares.block_warps ? __shfl_sync(0xffffffffu, bound, 1) - begin : 0;
+    block_begin = __shfl_sync(0xffffffffu, bound, 2);
+    block_mine = __shfl_sync(0xffffffffu, bound, 3) - block_begin;
     if (block_mine <= 0) return;
-    home = place(block_begin);
   }
-  // A block whose share lies within one pair merges its warps' parts before they leave the SM.
-  const bool together = home.st + block_mine <= home.n_st;
 
   // A stage is `units` whole pages, or part of one.  The sources of the next 32 units are worked out by one
   // lane each; that lane then issues its copies: the page's block, or of a part the keys, key scales, values
   // and value scales.
   const unsigned char* ahead = nullptr;  // this lane's unit: its block in the pool, nullptr: none
   int ahead_tok = 0;                     // its first token in the page
-  auto look = [&](int n) {               // from stage n of the share on
-    const int i = n + lane / units;
+  auto ahead_place = [&](int n) { return place(begin + min(n + lane / units, mine - 1)); };
+  auto look = [&](int n, const Place& p) {  // from stage n of the share on
     ahead = nullptr;
-    if (i < mine) {
-      const Place p = place(begin + i);
+    if (n + lane / units < mine) {
       const int key = p.st * KT + lane % units * unit;
       if (key < int4_len(a, p.b)) {
         const int page = a.c.table[p.b * a.c.table_stride + (key >> a.page_log2)];
@@ -724,7 +739,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   };
   auto issue = [&](int n) {
     const int at = n * units & 31;
-    if (at == 0) look(n);
+    if (at == 0 && n > 0) look(n, ahead_place(n));
     const int u = lane - at;
     if ((unsigned)u < (unsigned)units) {
       unsigned char* dst = ring + (n % kStages) * kStageBytes;
@@ -747,18 +762,37 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
       }
     }
   };
+  // The first queries are asked for before the first stages: behind them they took 3 us to come.  (The registers
+  // that hold them cost several column tiles more than that: 65 against 59 us for 20 columns.)
+  constexpr bool kEarly = NT == 1;
   int issued = 0;
-  while (issued < min(mine, kStages - 1)) issue(issued++);
+  Place p = home;
+  Int4Queries<T, DG, NT> raw;
+  if (mine > 0) {
+    const Place at = ahead_place(0);
+    p.b = __shfl_sync(0xffffffffu, at.b, 0);
+    p.pair = __shfl_sync(0xffffffffu, at.pair, 0);
+    p.st = __shfl_sync(0xffffffffu, at.st, 0);
+    p.n_st = __shfl_sync(0xffffffffu, at.n_st, 0);
+    const int hk = p.pair / a.col_blocks;
+    if constexpr (kEarly) int4_fetch_queries<T, DG, NT, kTwin>(a, raw, p.b, hk, (p.pair - hk * a.col_blocks) * NT * 8);
+    look(0, at);
+    while (issued < min(mine, kStages - 1)) issue(issued++);
+  }
+  // A block whose share lies within one pair merges its warps' parts before they leave the SM.
+  if (!a.by_pair) home = place(block_begin);
+  const bool together = home.st + block_mine <= home.n_st;
 
   State q;
   q.qs = ptx::smem_u32(queries + warp * kQueryBytes) + lane * 16;
   bool ok = true;
   int n = 0;
   while (n < mine && ok) {
-    const Place p = place(begin + n);
+    if (n > 0) p = place(begin + n);
     const int len = int4_len(a, p.b), hk = p.pair / a.col_blocks, col0 = (p.pair - hk * a.col_blocks) * NT * 8;
     const int count = min(mine - n, p.n_st - p.st);
-    int4_load_queries(a, q, p.b, hk, col0, len);
+    if (!kEarly || n > 0) int4_fetch_queries<T, DG, NT, kTwin>(a, raw, p.b, hk, col0);
+    int4_load_queries<T, DG, NT, kTwin>(a, q, raw, col0, len);
     // the first key that some column does not see
     const int plain = a.p.is_causal ? min(len, max(0, len - a.p.q_len + col0 / a.group + 1)) : len;
     int key0 = p.st * KT;
@@ -842,22 +876,23 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   }
 }
 
-// A warp (or, with few rows and many parts of each, a block) merges an output row; rows without keys become
-// zeros, and a row that was written whole is left alone.
+// row_warps warps (1, 2, 4 or 8) merge an output row; rows without keys become zeros, and a row that was
+// written whole is left alone.
 template <typename T, int NT, int kWarps>
 __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__ Int4Attn a, int row_warps) {
   __shared__ float part[8][256];
   __shared__ float2 part_ml[8];
-  wait_for_previous();
+  let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
-  const int64_t row = (int64_t)blockIdx.x * (8 / row_warps) + warp / row_warps;
+  const int rows = a.p.batch * a.p.q_heads * a.p.q_len;  // the host has checked that it fits
+  const int64_t row64 = (int64_t)blockIdx.x * (8 / row_warps) + warp / row_warps;
   const int sub = warp % row_warps;
-  if (row >= rows) return;  // row_warps is 1 or 8: a whole block or single warps
-  const int tok = (int)(row % a.p.q_len), h = (int)(row / a.p.q_len % a.p.q_heads);
-  const int b = (int)(row / ((int64_t)a.p.q_len * a.p.q_heads));
+  if (row64 >= rows) return;  // all warps of a row, like every return below
+  const int row = (int)row64, of_head = row / a.p.q_len, tok = row - of_head * a.p.q_len;
+  const int b = of_head / a.p.q_heads, h = of_head - b * a.p.q_heads;
   const int hk = h / a.group, col = tok * a.group + h - hk * a.group;
   const int pairs = a.p.kv_heads * a.col_blocks, pair = hk * a.col_blocks + col / (NT * 8), local = col % (NT * 8);
+  wait_for_previous();
   const int32_t* first_unit = a.ws_first + a.p.batch + 1;
   const int total = first_unit[a.p.batch], row_first = first_unit[b];
   const int n = (first_unit[b + 1] - row_first) / pairs;  // units of a pair: one more than its stages
@@ -903,15 +938,15 @@ __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__
 #pragma unroll
     for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = out[k];
     if (lane == 0) part_ml[warp] = ml;
-    __syncthreads();
-    if (warp > 0) return;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / row_warps), "r"(32 * row_warps) : "memory");
+    if (sub > 0) return;
     float top = -INFINITY;
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, part_ml[w].x);
+    for (int w = warp; w < warp + row_warps; ++w) top = fmaxf(top, part_ml[w].x);
     const float base = top == -INFINITY ? 0.f : top;
     ml = make_float2(top, 0.f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) out[k] = 0.f;
-    for (int w = 0; w < 8; ++w) {
+    for (int w = warp; w < warp + row_warps; ++w) {
       const float f = ptx::ex2(part_ml[w].x - base);
       ml.y += part_ml[w].y * f;
 #pragma unroll

@@ -19,11 +19,11 @@ static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
   auto kernel = attn_int4_kernel<T, DG, NT, kTwin, KT, kInt4Stages, kWarps, kMinBlocks>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), (int)(most > merge ? most : merge));
   if (e != cudaSuccess) return e;
-  kernel<<<blocks, kWarps * 32, smem, st>>>(a);
-  e = cudaGetLastError();
+  e = launch_dependent(kernel, dim3((unsigned)blocks), dim3(kWarps * 32), smem, st, a);
   if (e != cudaSuccess || a.by_pair) return e;
   const int64_t rows = (int64_t)a.p.batch * a.p.q_heads * a.p.q_len;
-  const int row_warps = a.parts > 8 ? 8 : 1;  // warps that merge one row
+  // Warps that merge one row: about four parts each, which they have in flight at once.
+  const int row_warps = a.parts > 16 ? 8 : a.parts > 8 ? 4 : a.parts > 4 ? 2 : 1;
   return launch_dependent(attn_int4_combine<T, NT, kWarps>, dim3((unsigned)((rows * row_warps + 7) / 8)), dim3(256),
                           0, st, a, row_warps);
 }
@@ -70,5 +70,10 @@ cudaError_t attn_int4_launch_wide(const Int4Attn& a, const Int4Shape& shape, int
   }
   return int4_run_dims<T, 2, false, 64, 4, 2>(a, blocks, st);
 }
+
+// Instantiated once, in the sources of the wide kernels.
+extern template cudaError_t attn_int4_launch_wide<__nv_bfloat16>(const Int4Attn&, const Int4Shape&, int, cudaStream_t);
+extern template cudaError_t attn_int4_launch_wide<__half>(const Int4Attn&, const Int4Shape&, int, cudaStream_t);
+extern template cudaError_t attn_int4_launch_wide<float>(const Int4Attn&, const Int4Shape&, int, cudaStream_t);
 
 }  // namespace tsa

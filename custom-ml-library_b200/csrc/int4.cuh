@@ -55,7 +55,6 @@ cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const i
                            const ts_view4& value, int dtype, int length, uint32_t* fault, cudaStream_t st);
 
 // The kernel that attends straight over the pages.
-bool attn_int4_supported(const ts_attn_params& p, const ts_kv4_cache& c);
 size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache& c);
 cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
                               uint32_t* fault, cudaStream_t st);

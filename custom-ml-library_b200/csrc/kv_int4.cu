@@ -5,6 +5,7 @@
 // One thread owns a stored word (8 channels of K or V of one head) and walks over a block's tokens, four of
 // them in flight: 64 bytes a thread for half types, which is what covers the memory latency.  The four
 // neighbouring threads of a scale group share its maximum by two shuffles.
+#include "dependent.cuh"
 #include "int4.cuh"
 #include "ptx.cuh"
 
@@ -130,7 +131,9 @@ __device__ __forceinline__ Span token_span(const ts_kv4_cache& c, int b, int p0,
 }
 
 template <typename T>
-__global__ void kv_append_int4_kernel(Int4Rows a) {
+__global__ void kv_append_int4_kernel(const __grid_constant__ Int4Rows a) {
+  let_next_start();
+  wait_for_previous();
   const ts_kv4_cache& c = a.c;
   const int b = blockIdx.x / a.token_blocks, t0 = (blockIdx.x - b * a.token_blocks) * a.tokens;
   const int t1 = min(a.steps, t0 + a.tokens);
@@ -190,7 +193,9 @@ __global__ void kv_append_int4_kernel(Int4Rows a) {
 }
 
 template <typename T>
-__global__ void kv_gather_int4_kernel(Int4Rows a) {
+__global__ void kv_gather_int4_kernel(const __grid_constant__ Int4Rows a) {
+  let_next_start();
+  wait_for_previous();
   const ts_kv4_cache& c = a.c;
   const int b = blockIdx.x / a.token_blocks, t0 = (blockIdx.x - b * a.token_blocks) * a.tokens;
   const int t1 = min(a.steps, t0 + a.tokens);
@@ -276,12 +281,11 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
   int threads;
   if (!rows_grid(a, grid, threads)) return cudaErrorInvalidValue;
   switch (dtype) {
-    case TS_F32: kv_append_int4_kernel<float><<<grid, threads, 0, st>>>(a); break;
-    case TS_F16: kv_append_int4_kernel<__half><<<grid, threads, 0, st>>>(a); break;
-    case TS_BF16: kv_append_int4_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(a); break;
-    default: return cudaErrorInvalidValue;
+    case TS_F32: return launch_dependent(kv_append_int4_kernel<float>, grid, dim3(threads), 0, st, a);
+    case TS_F16: return launch_dependent(kv_append_int4_kernel<__half>, grid, dim3(threads), 0, st, a);
+    case TS_BF16: return launch_dependent(kv_append_int4_kernel<__nv_bfloat16>, grid, dim3(threads), 0, st, a);
   }
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
 cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const int32_t* lens, const ts_view4& key,
@@ -293,12 +297,11 @@ cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const i
   int threads;
   if (!rows_grid(a, grid, threads)) return cudaErrorInvalidValue;
   switch (dtype) {
-    case TS_F32: kv_gather_int4_kernel<float><<<grid, threads, 0, st>>>(a); break;
-    case TS_F16: kv_gather_int4_kernel<__half><<<grid, threads, 0, st>>>(a); break;
-    case TS_BF16: kv_gather_int4_kernel<__nv_bfloat16><<<grid, threads, 0, st>>>(a); break;
-    default: return cudaErrorInvalidValue;
+    case TS_F32: return launch_dependent(kv_gather_int4_kernel<float>, grid, dim3(threads), 0, st, a);
+    case TS_F16: return launch_dependent(kv_gather_int4_kernel<__half>, grid, dim3(threads), 0, st, a);
+    case TS_BF16: return launch_dependent(kv_gather_int4_kernel<__nv_bfloat16>, grid, dim3(threads), 0, st, a);
   }
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace tsa

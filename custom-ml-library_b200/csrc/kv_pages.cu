@@ -58,6 +58,7 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* warp_sums) {
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(ts_page_pool src, ts_page_pool dst,
                                                                  const int32_t* from, const int32_t* to, int stride,
                                                                  int n, const int32_t* n_dev) {
+  let_next_start();
   wait_for_previous();
   if (n_dev) n = min(n, *n_dev);
   const int chunks = (int)((src.page_bytes + kCopyChunk - 1) / kCopyChunk);
