@@ -657,9 +657,9 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   struct Place {  // of a stage: row, column block and KV head, stage of the pair and their number
     int b, pair, st, n_st;
   };
-  Place home;       // of the block's first stage
+  Place home, p;    // of the block's first stage, of this warp's next pair
   int begin, mine;  // this warp's first stage and their number
-  int block_begin = 0, block_mine;  // the block's
+  int block_mine;   // the block's
   int block_id = 0, id = 0;  // the block's first worker, this warp's
   int total = 0, total_units = 0;
   auto row_of = [&](const int* starts, int i) {  // the last row that starts at or before i
@@ -671,11 +671,19 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     }
     return lo;
   };
-  auto stages_before = [&](int64_t u) {  // of the units before u
+  auto stages_before = [&](int64_t u, Place& p) {  // of the units before u; p: where they end
+    p = Place{0, 0, 0, 0};
     if (u >= total_units) return total;
-    const int b = row_of(first_unit, (int)u);
-    const int n = (first_unit[b + 1] - first_unit[b]) / pairs, at = (int)u - first_unit[b], pair = at / n;
-    return first[b] + pair * (n - 1) + max(0, at - pair * n - 1);
+    p.b = row_of(first_unit, (int)u);
+    const int n = (first_unit[p.b + 1] - first_unit[p.b]) / pairs, at = (int)u - first_unit[p.b];
+    p.pair = at / n;
+    p.n_st = n - 1;
+    p.st = max(0, at - p.pair * n - 1);
+    return first[p.b] + p.pair * p.n_st + p.st;
+  };
+  auto from_lane = [](const Place& p, int l) {
+    return Place{__shfl_sync(0xffffffffu, p.b, l), __shfl_sync(0xffffffffu, p.pair, l), __shfl_sync(0xffffffffu, p.st, l),
+                 __shfl_sync(0xffffffffu, p.n_st, l)};
   };
   auto place = [&](int i) {
     Place p;
@@ -698,6 +706,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     const int share = ceil_div(block_mine, kWarps);
     begin = min(warp * share, block_mine);
     mine = min(share, block_mine - begin);
+    p = home;
+    p.st = begin;
   } else {
     total = first[a.p.batch];
     total_units = first_unit[a.p.batch];
@@ -707,12 +717,14 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     id = block_id + warp;
     // The four bounds on four lanes at once: one after the other these searches took 2 us of the start.
     const int worker = lane == 0 ? id : lane == 1 ? id + 1 : lane == 2 ? block_id : block_id + shares.block_warps;
-    const int bound = stages_before((int64_t)worker * share);
+    Place at;
+    const int bound = stages_before((int64_t)worker * share, at);
     begin = __shfl_sync(0xffffffffu, bound, 0);
     mine = warp < shares.block_warps ? __shfl_sync(0xffffffffu, bound, 1) - begin : 0;
-    block_begin = __shfl_sync(0xffffffffu, bound, 2);
-    block_mine = __shfl_sync(0xffffffffu, bound, 3) - block_begin;
+    block_mine = __shfl_sync(0xffffffffu, bound, 3) - __shfl_sync(0xffffffffu, bound, 2);
     if (block_mine <= 0) return;
+    p = from_lane(at, 0);
+    home = from_lane(at, 2);
   }
 
   // A stage is `units` whole pages, or part of one.  The sources of the next 32 units are worked out by one
@@ -720,7 +732,6 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   // and value scales.
   const unsigned char* ahead = nullptr;  // this lane's unit: its block in the pool, nullptr: none
   int ahead_tok = 0;                     // its first token in the page
-  auto ahead_place = [&](int n) { return place(begin + min(n + lane / units, mine - 1)); };
   auto look = [&](int n, const Place& p) {  // from stage n of the share on
     ahead = nullptr;
     if (n + lane / units < mine) {
@@ -739,7 +750,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   };
   auto issue = [&](int n) {
     const int at = n * units & 31;
-    if (at == 0 && n > 0) look(n, ahead_place(n));
+    if (at == 0 && n > 0) look(n, place(begin + min(n + lane / units, mine - 1)));
     const int u = lane - at;
     if ((unsigned)u < (unsigned)units) {
       unsigned char* dst = ring + (n % kStages) * kStageBytes;
@@ -766,21 +777,18 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   // that hold them cost several column tiles more than that: 65 against 59 us for 20 columns.)
   constexpr bool kEarly = NT == 1;
   int issued = 0;
-  Place p = home;
   Int4Queries<T, DG, NT> raw;
   if (mine > 0) {
-    const Place at = ahead_place(0);
-    p.b = __shfl_sync(0xffffffffu, at.b, 0);
-    p.pair = __shfl_sync(0xffffffffu, at.pair, 0);
-    p.st = __shfl_sync(0xffffffffu, at.st, 0);
-    p.n_st = __shfl_sync(0xffffffffu, at.n_st, 0);
+    Place at = p;
+    const int i = min(lane / units, mine - 1);
+    if (p.st + i < p.n_st) at.st += i;
+    else at = place(begin + i);
     const int hk = p.pair / a.col_blocks;
     if constexpr (kEarly) int4_fetch_queries<T, DG, NT, kTwin>(a, raw, p.b, hk, (p.pair - hk * a.col_blocks) * NT * 8);
     look(0, at);
     while (issued < min(mine, kStages - 1)) issue(issued++);
   }
   // A block whose share lies within one pair merges its warps' parts before they leave the SM.
-  if (!a.by_pair) home = place(block_begin);
   const bool together = home.st + block_mine <= home.n_st;
 
   State q;
@@ -788,7 +796,15 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   bool ok = true;
   int n = 0;
   while (n < mine && ok) {
-    if (n > 0) p = place(begin + n);
+    if (n > 0) {  // the next pair with keys
+      p.st = 0;
+      if (++p.pair == pairs) {
+        p.pair = 0;
+        do ++p.b;
+        while (first[p.b + 1] == first[p.b]);
+        p.n_st = (first[p.b + 1] - first[p.b]) / pairs;
+      }
+    }
     const int len = int4_len(a, p.b), hk = p.pair / a.col_blocks, col0 = (p.pair - hk * a.col_blocks) * NT * 8;
     const int count = min(mine - n, p.n_st - p.st);
     if (!kEarly || n > 0) int4_fetch_queries<T, DG, NT, kTwin>(a, raw, p.b, hk, col0);
