@@ -382,8 +382,8 @@ ts_attn_params int4_prefill_params(const ts_attn_params& p, void* ws) {
 // 64, 128 and 256 query columns a KV head).  Over the pages the time grows with the columns (group x tokens):
 // 1.95e-3 a KV head and column.  The other way writes and reads the dequantised rows, 0.133 a KV head, and then
 // runs one query tile a block: 6.1 a wave of 128-row tiles, 13.4 of 256-row ones (more than 128 tokens), however
-// few of a tile's rows are filled.  16 rows, 64 columns: 148 against 204 to 532 us by group; 256 columns: 521
-// against 250, 345 and 542; 2 rows, 256 columns: 53 against 79, 50 and 51.
+// few of a tile's rows are filled.  16 rows, 64 columns: 147 against 199 to 524 us by group; 256 columns: 525
+// against 246, 343 and 549; 2 rows, 256 columns: 51 against 80, 49 and 50.
 bool int4_prefill_faster(const ts_attn_params& p) {
   const double heads = (double)p.batch * p.kv_heads, columns = (double)(p.q_heads / p.kv_heads) * p.q_len;
   const int rows = p.q_len > 128 ? 256 : 128;
