@@ -13,11 +13,11 @@
 // (mma.sync: a fragment is built in registers straight from the nibbles, while tcgen05 would want
 // the dequantised tile written to shared memory first, four times the bytes.)  Everything is fp16 in
 // the products and fp32 in the sums and statistics:
-//   K       (one column tile) the masked nibbles themselves: a nibble in the low bits of a half is the subnormal nibble * 2^-24, in
+//   K       (one column tile, half types) the masked nibbles themselves: a nibble in the low bits of a half is the subnormal nibble * 2^-24, in
 //           the next four bits nibble * 2^-20, so the queries of the odd ones are a sixteenth; one logic op a
 //           pair.  What the nibbles' offset of 8 adds to a 32-channel group's product is a constant of the
 //           column, the accumulator's start.  The group's scale goes on its fp32 sum.  (Two and three tiles
-//           subtract instead, as V does: 59 against 63 us for 20 columns)
+//           and fp32 subtract instead, as V does: 59 against 63 us for 20 columns)
 //   V       needs its scale on the operand: the nibble in the mantissa of a power of two, 0x6400 | nibble = 1024 +
 //           nibble or 0x5400 | nibble << 4 = 64 + nibble, then n * scale = (64 + nibble) scale - 72 scale, exact
 //           in one multiply-add (for the other a subtraction and a product)
@@ -154,8 +154,9 @@ struct Int4State {
   // Tiles of 16 keys whose scores and probabilities are held at a time: what the registers leave room for.
   static constexpr int kChunk = NT == 1 ? 4 : NT == 2 ? 2 : 1;
   uint32_t qf[kQueriesShared ? 1 : QP][kQueriesShared ? 1 : DG][4];
-  // One tile multiplies the masked nibbles (of several, the offsets below would cost more than they save).
-  static constexpr bool kMaskedK = NT == 1;
+  // One tile multiplies the masked nibbles (of several, the offsets below would cost more than they save).  fp32
+  // rows keep subtracting: the offset cancels most of the fp32 sums' upper bits, 1.1e-6 of the output against 2e-7.
+  static constexpr bool kMaskedK = NT == 1 && sizeof(T) == 2;
   float qb[kMaskedK ? DG : 1][2];  // what the nibbles' 8 takes from a group's products, columns 2t and 2t + 1
   uint32_t qs;  // shared address of [QP, NT, DG, 32 lanes] x 16 bytes, this lane's first
   __device__ __forceinline__ uint4 fragment(int part, int nt, int gr) const {

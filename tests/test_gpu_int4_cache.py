@@ -94,6 +94,22 @@ def check_attention(cache, dtype, q_heads, q_len, *, causal=True, seed=1, scale=
     return out
 
 
+@pytest.mark.parametrize("group, q_len", [(1, 1), (5, 1), (2, 5)])
+@pytest.mark.parametrize("dim, page", [(32, 16), (64, 32), (96, 16), (128, 64), (256, 32)])
+def test_fp32_attention_keeps_fp32_precision(dim, page, group, q_len):
+    """The error's norm against the output's: q in two fp16 parts, the scores' sums, the exponential and p in two
+    parts each move a probability by at most 2^-22 of itself (scores of size one); independent, they add up to
+    2^-21.  The n additions' truncation is the 2^-27 each of the other bounds here."""
+    c = Cache([40, 33, 37], 2, dim, page, seed=dim)
+    c.v = np.random.default_rng(dim + 1).standard_normal(c.v.shape)
+    keys, values = c.fill("float32")
+    q = torch.from_numpy(np.random.default_rng(3).standard_normal((3, 2 * group, q_len, dim))).cuda().float()
+    out, _ = engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=page)
+    engine.check_device_status()
+    ref, _, _ = oracle.attention_int4(to_np(q).astype(np.float64), keys, values, c.lens, is_causal=True, scale=None)
+    assert np.linalg.norm(to_np(out) - ref) <= (2.0**-21 + 40 * 2.0**-27) * np.linalg.norm(ref)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 @pytest.mark.parametrize("dim, page, heads", [(32, 16, 1), (64, 32, 3), (96, 16, 2), (128, 64, 8), (256, 32, 2)])
 def test_append_and_gather_match_the_oracle(dtype, dim, page, heads):
