@@ -266,6 +266,70 @@ def test_out_tensors_streams_and_graphs():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("rows, heads, start", [(3, 2, 11), (16, 8, 700)])
+def test_calls_in_a_row_see_one_anothers_writes(rows, heads, start):
+    """The kernels of one call start while those of the call before it end: a chain in which every call reads what
+    the one before it wrote gives the same bits as with a synchronisation after each, and from a graph."""
+    dim, page, steps = 64, 16, 12
+    slots = (start + steps) // page + 2
+    pages = rows * slots + rows
+
+    def chain(after):
+        gen = torch.Generator(device="cuda").manual_seed(5)
+        pool = torch.zeros_like(engine.int4_pool(pages, heads, dim, page_size=page, layers=1))
+        refs, counters = engine.kv_pages_state(pages)
+        table = torch.full((rows, slots), -1, dtype=torch.int32, device="cuda")
+        lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        prompt = torch.randn(2, rows, heads, start, dim, generator=gen, device="cuda").half()
+        x = torch.randn(rows, heads, 1, dim, generator=gen, device="cuda").half()
+        parents = torch.arange(rows, device="cuda", dtype=torch.int32) // 2
+        engine.kv_pages_reserve(pool, table, lens, start, refs, counters, page_size=page)
+        engine.kv_append_int4(prompt[0], prompt[1], pool[0], table, page_size=page, positions=lens)
+        lens = lens + start
+        torch.cuda.synchronize()
+
+        def run():
+            t, n, token, outs = table, lens, x, []
+            for step in range(steps):
+                engine.kv_pages_reserve(pool, t, n, 1, refs, counters, page_size=page)
+                after()
+                engine.kv_append_int4(token, token * 0.5, pool[0], t, page_size=page, positions=n)
+                after()
+                n = n + 1
+                token, _ = engine.attention_int4(token, pool[0], t, n, page_size=page, max_len=start + steps)
+                after()
+                again, _ = engine.attention_int4(token * 2, pool[0], t, n, page_size=page, max_len=start + steps)
+                after()
+                outs.append(again)
+                token = token + again
+                if step % 4 == 3:
+                    t, n = engine.kv_pages_fork(t, n, parents, refs, counters, page_size=page)
+                    after()
+                    engine.kv_pages_compact(pool, t, refs, counters)
+                    after()
+                    key, value = engine.kv_gather_int4(pool[0], t, start, page_size=page, dtype=torch.float16, kv_lens=n)
+                    after()
+                    outs.append(key + value)
+            return [o.clone() for o in outs] + [t, n, refs, counters]
+
+        return run
+
+    expect = chain(torch.cuda.synchronize)()
+    torch.cuda.synchronize()
+    assert expect[-1][2].item() == 0 and torch.isfinite(expect[0]).all()
+    for _ in range(3):
+        got = chain(lambda: None)()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(expect, got))
+    graph, run = torch.cuda.CUDAGraph(), chain(lambda: None)
+    with torch.cuda.graph(graph):
+        got = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    engine.check_device_status()
+    assert all(torch.equal(a, b) for a, b in zip(expect, got))
+
+
 def test_refusals_on_device_tensors():
     c = Cache([10, 20], 2, 64, 16)
     q = torch.zeros(2, 4, 1, 64, device="cuda", dtype=torch.bfloat16)
