@@ -612,7 +612,7 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
 // share, the next row's first stages in flight while it finishes the last one; no block barrier runs
 // between the start and the merge.
 // Beside its stages a call of 16 rows x 8 heads takes 1 us until the rows' lengths are summed up, 2.5 until its
-// first copies are under way, 2 until they are there, 2 to write the parts and about 5 to merge them: 31 us in all,
+// first copies are under way, 2 until they are there, 2 to write the parts and about 4 to merge them: 27 us in all,
 // where the bytes alone would take 12.
 template <typename T, int DG, int NT, bool kTwin, int KT, int kStages, int kWarps, int kMinBlocks>
 __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(const __grid_constant__ Int4Attn a) {
@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     ptx::fence_mbar_init();
   }
   int* first_unit = first + a.p.batch + 1;
-  let_next_start();
   wait_for_previous();
+  let_next_start();  // the merge reads the lengths without waiting for this kernel's end
   if (warp == 0 && !a.by_pair) {  // stages and units of the rows before b
     int stages = 0, rows = 0;
     for (int b0 = 0; b0 <= a.p.batch; b0 += 32) {
@@ -901,10 +901,14 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
 }
 
 // row_warps warps (1, 2, 4 or 8) merge an output row; rows without keys become zeros, and a row that was
-// written whole is left alone.
+// written whole is left alone.  What bounds it is one chain of dependent loads behind the first kernel's end, so up
+// to 32 rows' places are worked out before it (from the lengths, for stages of `keys` tokens; of more rows the first
+// kernel leaves the sums), and a warp has eight parts in flight.  Two rows of up to 131072 keys: 24.4 us a call against
+// 29.6 with the places found behind the wait and four parts in flight, 18 heads of up to 701 keys 7.6 against 9.0.
 template <typename T, int NT, int kWarps>
-__global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__ Int4Attn a, int row_warps) {
-  __shared__ float part[8][256];
+__global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__ Int4Attn a, int row_warps, int keys) {
+  constexpr int kFlight = 8, kChannels = 128;
+  __shared__ float part[8][kChannels];
   __shared__ float2 part_ml[8];
   let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -916,73 +920,120 @@ __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__
   const int b = of_head / a.p.q_heads, h = of_head - b * a.p.q_heads;
   const int hk = h / a.group, col = tok * a.group + h - hk * a.group;
   const int pairs = a.p.kv_heads * a.col_blocks, pair = hk * a.col_blocks + col / (NT * 8), local = col % (NT * 8);
-  wait_for_previous();
-  const int32_t* first_unit = a.ws_first + a.p.batch + 1;
-  const int total = first_unit[a.p.batch], row_first = first_unit[b];
-  const int n = (first_unit[b + 1] - row_first) / pairs;  // units of a pair: one more than its stages
-  const int groups = a.p.head_dim / 32;
-  float2 ml = make_float2(-INFINITY, 0.f);
-  float out[8] = {};
-  if (n) {
+  int n = 0;  // units of a pair: one more than its stages
+  int head = 0, mid = 0, tail = 0, lo = 0, c0 = 0, c1 = 0, w0 = 0, w1 = 0;
+  int warps = 0;  // of a block
+  bool whole = false, late = false;
+  // Finds the row's parts: of the first block's warps, of the blocks that merged theirs, of the last block's warps.
+  auto locate = [&](int total, int row_first) {
     const int enter = row_first + pair * n;  // the pair's stages are the units enter + 1 .. enter + n - 1
     const Int4Shares shares = int4_shares(a, total, kWarps);
-    const int share = shares.share, warps = shares.block_warps;
-    const int w0 = (enter + 1) / share, w1 = (enter + n - 1) / share, c0 = w0 / warps, c1 = w1 / warps;
+    const int share = shares.share;
+    warps = shares.block_warps;
+    w0 = (enter + 1) / share, w1 = (enter + n - 1) / share, c0 = w0 / warps, c1 = w1 / warps;
     auto merged = [&](int c) {  // no stage of the block's share is another pair's (the next one's entry may be)
       return (int64_t)c * warps * share >= enter &&
              i64min((int64_t)(c + 1) * warps * share, total) <= (int64_t)enter + n + 1;
     };
     const bool m0 = merged(c0), m1 = merged(c1);
-    if (w0 == w1 || (c0 == c1 && m0)) return;
-    // The row's parts: of the first block's warps, of the blocks that merged theirs, of the last block's warps.
-    const int head = m0 ? 0 : min(w1, c0 * warps + warps - 1) - w0 + 1;
-    const int lo = m0 ? c0 : c0 + 1, mid = max(0, (m1 ? c1 : c1 - 1) - lo + 1);
-    const int tail = c1 != c0 && !m1 ? w1 - c1 * warps + 1 : 0;
-    const bool late = (int64_t)w0 * share < enter;  // the row is not the first thing of its first worker
-    auto slot = [&](int i) {
-      const int w = i < head ? w0 + i : i < head + mid ? (lo + i - head) * warps : c1 * warps + i - head - mid;
-      return (int64_t)(2 * w + (late && w == w0)) * a.slot_cols + local;
-    };
-    const float2* all_ml = reinterpret_cast<const float2*>(a.ws_ml);
-#pragma unroll 4
-    for (int i = sub; i < head + mid + tail; i += row_warps) {
-      const int64_t s = slot(i);
-      const float2 x = all_ml[s];
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k < groups ? a.ws_acc[s * a.p.head_dim + k * 32 + lane] : 0.f;
-      const float top = fmaxf(ml.x, x.x), base = top == -INFINITY ? 0.f : top;
-      const float f0 = ptx::ex2(ml.x - base), f1 = ptx::ex2(x.x - base);
-      ml = make_float2(top, ml.y * f0 + x.y * f1);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) out[k] = out[k] * f0 + v[k] * f1;
-    }
+    whole = w0 == w1 || (c0 == c1 && m0);
+    head = m0 ? 0 : min(w1, c0 * warps + warps - 1) - w0 + 1;
+    lo = m0 ? c0 : c0 + 1, mid = max(0, (m1 ? c1 : c1 - 1) - lo + 1);
+    tail = c1 != c0 && !m1 ? w1 - c1 * warps + 1 : 0;
+    late = (int64_t)w0 * share < enter;  // the row is not the first thing of its first worker
+    lo *= warps, c1 *= warps;
+  };
+  const bool few = a.p.batch <= 32;
+  if (few) {
+    const int stages = lane < a.p.batch ? ceil_div(int4_len(a, lane), keys) : 0, units = stages ? stages + 1 : 0;
+    n = __shfl_sync(0xffffffffu, units, b);
+    const int total = __reduce_add_sync(0xffffffffu, units), before = __reduce_add_sync(0xffffffffu, lane < b ? units : 0);
+    if (n) locate(total * pairs, before * pairs);
   }
-  if (row_warps > 1) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = out[k];
-    if (lane == 0) part_ml[warp] = ml;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / row_warps), "r"(32 * row_warps) : "memory");
-    if (sub > 0) return;
-    float top = -INFINITY;
-    for (int w = warp; w < warp + row_warps; ++w) top = fmaxf(top, part_ml[w].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    ml = make_float2(top, 0.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) out[k] = 0.f;
-    for (int w = warp; w < warp + row_warps; ++w) {
-      const float f = ptx::ex2(part_ml[w].x - base);
-      ml.y += part_ml[w].y * f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) out[k] += part[w][k * 32 + lane] * f;
-    }
+  wait_for_previous();
+  if (!few) {
+    const int32_t* first_unit = a.ws_first + a.p.batch + 1;
+    const int total = first_unit[a.p.batch], row_first = first_unit[b];
+    n = (first_unit[b + 1] - row_first) / pairs;
+    if (n) locate(total, row_first);
   }
+  if (whole) return;
+  auto slot = [&](int i) {
+    const int w = i < head ? w0 + i : i < head + mid ? lo + (i - head) * warps : c1 + i - head - mid;
+    return (int64_t)(2 * w + (late && w == w0)) * a.slot_cols + local;
+  };
+  const int parts = head + mid + tail;
+  const float2* all_ml = reinterpret_cast<const float2*>(a.ws_ml);
   T* o = int4_out_row<T>(a, b, h, tok);
-  const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+#pragma unroll 1
+  for (int d0 = 0; d0 < a.p.head_dim; d0 += kChannels) {
+    const int channels = min(kChannels, a.p.head_dim - d0);  // four of them a lane
+    float m = -INFINITY, l = 0.f;
+    float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = sub; i0 < parts; i0 += row_warps * kFlight) {
+      float2 x[kFlight];
+      float4 v[kFlight];
+      float top = m;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < groups) o[(k * 32 + lane) * a.p.o.stride[3]] = Elem<T>::from_acc(out[k] * inv);
-  if (lane == 0) int4_store_lse(a, b, h, tok, ml.x - 7.f, ml.y);
+      for (int u = 0; u < kFlight; ++u) {
+        const int i = i0 + u * row_warps;
+        x[u] = make_float2(-INFINITY, 0.f);
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < parts) {
+          const int64_t s = slot(i);
+          x[u] = all_ml[s];
+          if (lane * 4 < channels) v[u] = *reinterpret_cast<const float4*>(a.ws_acc + s * a.p.head_dim + d0 + lane * 4);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) top = fmaxf(top, x[u].x);
+      const float base = top == -INFINITY ? 0.f : top, f0 = ptx::ex2(m - base);
+      m = top;
+      l *= f0;
+      out = make_float4(out.x * f0, out.y * f0, out.z * f0, out.w * f0);
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        const float f = ptx::ex2(x[u].x - base);
+        l += x[u].y * f;
+        out.x += v[u].x * f, out.y += v[u].y * f, out.z += v[u].z * f, out.w += v[u].w * f;
+      }
+    }
+    if (row_warps == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float y[4] = {out.x, out.y, out.z, out.w};
+      if (lane * 4 < channels)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[(d0 + lane * 4 + e) * a.p.o.stride[3]] = Elem<T>::from_acc(y[e] * inv);
+    } else {  // every warp joins some of the channels
+      const int w_row = warp - sub;
+      auto row_sync = [&] {
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / row_warps), "r"(32 * row_warps) : "memory");
+      };
+      if (d0 > 0) row_sync();  // the part before has been read
+      reinterpret_cast<float4*>(part[warp])[lane] = out;
+      if (lane == 0) part_ml[warp] = make_float2(m, l);
+      row_sync();
+      m = -INFINITY, l = 0.f;
+      for (int w = 0; w < row_warps; ++w) m = fmaxf(m, part_ml[w_row + w].x);
+      const float base = m == -INFINITY ? 0.f : m;
+      float f[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float2 x = w < row_warps ? part_ml[w_row + w] : make_float2(-INFINITY, 0.f);
+        f[w] = ptx::ex2(x.x - base);
+        l += x.y * f[w];
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int d = sub * 32 + lane; d < channels; d += row_warps * 32) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          if (w < row_warps) y += part[w_row + w][d] * f[w];
+        o[(d0 + d) * a.p.o.stride[3]] = Elem<T>::from_acc(y * inv);
+      }
+    }
+    if (d0 == 0 && sub == 0 && lane == 0) int4_store_lse(a, b, h, tok, m - 7.f, l);
+  }
 }
 
 // Shape of the kernel that takes a problem.
