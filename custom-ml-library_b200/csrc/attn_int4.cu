@@ -45,15 +45,16 @@ Int4Shape int4_shape(const ts_attn_params& p) {
   const bool twin = cols <= 4 && p.dtype != TS_BF16;
   if (p.head_dim > 128) return {1, 32, 4, 2, false, twin};
   // Several column tiles share the operands made from the nibbles, with their queries in shared memory.  Three
-  // where that saves a second pass (16 rows x 8 KV heads, up to 8192 keys, 20 columns: 56 against 63 us with two,
-  // 64 rows 143 against 191; 12 columns: 51 against 42).  Four spill: 32 columns took 78 us against 71 with two
-  // passes of two.  Stages of 32 tokens keep too little in flight: 69 against 56 us for 20 columns.
+  // where that saves a second pass (16 rows x 8 KV heads, up to 8192 keys, 20 columns: 51 against 60 us with two,
+  // 64 rows 144 against 193; 12 columns: 47 against 39).  Four spill: 32 columns took 78 us against 71 with two
+  // passes of two.  Stages of 32 tokens keep too little in flight: 173 against 143 us for 64 rows
+  // of 20 columns.
   if (cols > 8) return {cols > 16 && cols <= 24 && p.dtype != TS_F32 ? 3 : 2, 64, 4, 2, false, false};
-  // Stages of 16 tokens where those of 64 would leave most warps without one: 9.6 against 11.1 us for 18 heads
-  // of up to 701 keys (fp32); with more the two meet (16 heads of 2048 keys: 11.3 against 10.6).  With two stages
+  // Stages of 16 tokens where those of 64 would leave most warps without one: 7.5 against 9.6 us for 18 heads
+  // of up to 701 keys (fp32); with more the two meet (16 heads of 2048 keys: 8.8 against 9.2).  With two stages
   // and more for every warp, one block of 12 warps a SM against three of 4: its merged parts are fewer (64 x 32
-  // heads of 1024-8192 keys: 253 against 258 us, 4 heads of up to 131072: 31 against 33; 16 heads of 2048 keys, one
-  // stage a warp: 12.2 against 10.6).
+  // heads of 1024-8192 keys: 251 against 258 us, 4 heads of up to 131072: 26 against 29; 16 heads of 2048 keys, one
+  // stage a warp: 9.6 against 9.2).
   const int64_t stages = (int64_t)p.batch * p.kv_heads * ((cols + 7) / 8) * ceil_div(p.kv_len, 64);
   if (p.kv_len <= 64 || stages <= 148 * 3) return {1, 16, 4, 3, p.kv_len <= 4 * 16, twin};
   if (stages >= 148 * 12 * 2) return {1, 64, 12, 1, false, twin};

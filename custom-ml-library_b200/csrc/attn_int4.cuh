@@ -25,7 +25,7 @@
 //           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
 //   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo,
 //           since the 2^-12 of one fp16 part is as large as the output's own rounding there
-// Measured, 64 rows x 32 heads of 1024-8192 keys, D = 128 (1.36 GB): 253 us in fp16, 248 in bf16, 83 % and 85 % of
+// Measured, 64 rows x 32 heads of 1024-8192 keys, D = 128 (1.36 GB): 251 us in fp16, 244 in bf16, 84 % and 86 % of
 // the copy rate.  Issue bounds it: 288 warp instructions a tile of 16 keys at 60 % of the issue slots, no pipe above
 // 51 %; the copies alone take 212 us, the arithmetic alone about 228.  Twelve warps an SM fit (168 registers); 16 of
 // 128 spill, and lost what they hid (308 against 253 us).
