@@ -19,8 +19,8 @@
 //           column, the accumulator's start.  The group's scale goes on its fp32 sum.  (Two and three tiles
 //           and fp32 subtract instead, as V does: 59 against 63 us for 20 columns)
 //   V       needs its scale on the operand: the nibble in the mantissa of a power of two, 0x6400 | nibble = 1024 +
-//           nibble or 0x5400 | nibble << 4 = 64 + nibble, then n * scale = (64 + nibble) scale - 72 scale, exact
-//           in one multiply-add (for the other a subtraction and a product)
+//           nibble or 0x5400 | nibble << 4 = 64 + nibble, then a subtraction and a product, both exact.  (As one
+//           multiply-add, (64 + nibble) scale - 72 scale, the last term would leave fp16 from a scale of 910 on)
 //   q       times a power of two that puts its largest element in [2^14, 2^15): exact for bf16 and
 //           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
 //   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo,
@@ -367,7 +367,7 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT, kTwin>& q, const
     ptx::f2unpack(sum2, q.l[nt][0], q.l[nt][1]);
   }
   // O^T += V^T P^T.  Lane (g, t) supplies the words g * NW + j of the tokens in its four slots, as
-  // n * scale: exact, in one multiply-add where 72 scale (9 bits) is the bias's share.
+  // n * scale, exact over the whole range of scales: at most 8 bits, between 2^-20 and 64512.
   const int slot[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};
 #pragma unroll
   for (int tile = 0; tile < kTiles; ++tile) {
@@ -402,16 +402,15 @@ __device__ __forceinline__ void int4_stage(Int4State<T, DG, NT, kTwin>& q, const
     for (int j = 0; j < NW; ++j) {
       const __half2 sc0 = bits_h2(__byte_perm(sc[0][j / 2], sc[1][j / 2], j & 1 ? 0x7632 : 0x5410));
       const __half2 sc1 = bits_h2(__byte_perm(sc[2][j / 2], sc[3][j / 2], j & 1 ? 0x7632 : 0x5410));
-      const __half2 off0 = __hmul2(sc0, __float2half2_rn(-72.f)), off1 = __hmul2(sc1, __float2half2_rn(-72.f));
 #pragma unroll
       for (int byte = 0; byte < 4; ++byte) {
         // byte `byte` of two tokens' words in the low bytes of the halves; the other bytes are masked off
         const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x0400 + byte * 0x0101);
         const uint32_t x1 = __byte_perm(w[2][j], w[3][j], 0x0400 + byte * 0x0101);
         const uint32_t a0 = h2_bits(__hmul2(bits_h2(value_low(x0)), sc0));
-        const uint32_t a1 = h2_bits(__hfma2(bits_h2(biased_high(x0)), sc0, off0));
+        const uint32_t a1 = h2_bits(__hmul2(bits_h2(value_high(x0)), sc0));
         const uint32_t a2 = h2_bits(__hmul2(bits_h2(value_low(x1)), sc1));
-        const uint32_t a3 = h2_bits(__hfma2(bits_h2(biased_high(x1)), sc1, off1));
+        const uint32_t a3 = h2_bits(__hmul2(bits_h2(value_high(x1)), sc1));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
