@@ -54,6 +54,7 @@ class PagedKVCache:
         self._lens = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self._before = self._lens  # the lengths before the last append
         self._host_lens = np.zeros(batch_size, dtype=np.int64)
+        self._host_before = self._host_lens  # host copy of _before
         self._reserved = np.zeros(batch_size, dtype=np.int64)  # tokens the rows' own pages can hold
         self._free = self.num_pages  # a lower bound
         self.layers = [PagedLayer(self, i) for i in range(num_layers)]
@@ -115,7 +116,7 @@ class PagedKVCache:
         self._table, self._lens = engine.kv_pages_fork(self._table, self._lens, dev_index, self._refs, self._counters,
                                                        page_size=self.page_size)
         self._before = self._lens
-        self._host_lens = np.where(index < 0, 0, self._host_lens[index])
+        self._host_lens = self._host_before = np.where(index < 0, 0, self._host_lens[index])
         # full pages stay; the partly filled one may be shared now, reserved ones behind it went back
         self._reserved = self._host_lens // self.page_size * self.page_size
         for layer in self.layers:
@@ -150,11 +151,19 @@ class PagedKVCache:
             layer.length = self.length
         self.fork(np.full(self.batch_size, -1))
 
-    def truncate(self, length: int) -> None:
-        """Forget the tokens past ``length``."""
-        if not 0 <= length <= self.length:
+    def truncate(self, length) -> None:
+        """Forget the tokens past ``length``, one number for all rows or one a row.  A step that only some layers
+        have appended is forgotten in every row."""
+        if np.ndim(length):
+            host = self._rows(length)
+            if host.shape != self._host_lens.shape or (host < 0).any() or (host > self._host_lens).any():
+                raise ValueError("truncate lengths must be between zero and every row's length")
+        elif not 0 <= length <= self.length:
             raise ValueError("truncate length must be between zero and the current length")
-        self._host_lens = np.minimum(self._host_lens, length)
+        else:
+            host = length
+        whole = self._host_before if self._unfinished() else self._host_lens
+        self._host_lens = self._host_before = np.minimum(whole, host)
         dev = self._table.device
         lens = torch.as_tensor(self._host_lens.astype(np.int32), device=dev)
         # a fork onto themselves lets the rows drop the pages past their tokens, which others may share
@@ -164,10 +173,14 @@ class PagedKVCache:
         self._before = self._lens
         self._reserved = self._host_lens // self.page_size * self.page_size
         for layer in self.layers:
-            layer.length = min(layer.length, length)
+            layer.length = self.length
+
+    def _unfinished(self) -> bool:
+        """Whether some layer has not yet appended the tokens of the last step."""
+        return any(layer.length != self.length for layer in self.layers)
 
     def _settled(self) -> None:
-        if any(layer.length != self.length for layer in self.layers):
+        if self._unfinished():
             raise RuntimeError("every layer must append a step's tokens before the rows change")
 
     # -- appends ---------------------------------------------------------------
@@ -187,7 +200,7 @@ class PagedKVCache:
             self._free -= need
             self._reserved = -(-stop // size) * size
         self._before, self._lens = self._lens, self._lens + steps
-        self._host_lens = stop
+        self._host_before, self._host_lens = self._host_lens, stop
 
     def _fits(self, steps: int) -> bool:
         """The exact need against the free pages, read from the device: copies of pages that several writers share
@@ -286,11 +299,9 @@ class PagedLayer:
                                              dtype=cache.dtype, kv_lens=cache._lens)
         return Tensor(keys, device=cache.device), Tensor(values, device=cache.device)
 
-    def truncate(self, length: int) -> None:
-        """Forget the tokens past ``length``, in every layer (they share the rows)."""
-        if not 0 <= length <= max(self.length, self.cache.length):
-            raise ValueError("truncate length must be between zero and the current length")
-        if length < self.cache.length:
+    def truncate(self, length) -> None:
+        """``PagedKVCache.truncate``: in every layer, as they share the rows."""
+        if np.ndim(length) or length != self.cache.length:
             self.cache.truncate(length)
 
     def __len__(self):

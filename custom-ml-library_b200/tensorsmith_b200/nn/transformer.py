@@ -364,6 +364,8 @@ class TransformerLM(_Module):
             if self.training or _grad_mode():
                 raise RuntimeError("cached decoding requires eval() and no_grad()")
             offset = caches[0].length
+            # a paged cache's rows may differ in length
+            starts = [cache.cache.lengths if isinstance(cache, PagedLayer) else offset for cache in caches]
             for block, cache in zip(self.blocks, caches):
                 if cache.batch_size != tokens.shape[0] or cache.device.index != self._device_index:
                     raise ValueError("cache batch/device does not match tokens")
@@ -387,8 +389,8 @@ class TransformerLM(_Module):
         except Exception:
             if caches is not None:
                 # Roll every cache back to where this call started (nn/transformer.py:308-312).
-                for cache in caches:
-                    cache.truncate(offset)
+                for cache, start in zip(caches, starts):
+                    cache.truncate(start)
             raise
 
     def loss(self, tokens, targets, *, ignore_index=-100, label_smoothing=0.0):

@@ -1,0 +1,69 @@
+"""Rows of different lengths in a ``PagedKVCache``: failed steps, truncation, refused calls."""
+
+import numpy as np
+import pytest
+
+from test_gpu_paged_cache import Mirror, model, tensor
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+import tensorsmith_b200 as ts  # noqa: E402
+
+
+class Failure(Exception):
+    pass
+
+
+def fail(*_, **__):
+    raise Failure
+
+
+@pytest.mark.parametrize("where", ["before the first append", "between two layers", "after the last append"])
+def test_a_failed_step_restores_every_row(where):
+    lm = model()
+    part = {"before the first append": lm.blocks[0].attention.q_proj, "between two layers": lm.blocks[1].attention_norm,
+            "after the last append": lm.final_norm}[where]
+    gen = torch.Generator().manual_seed(4)
+    prompt, chunk, step, wrong = (torch.randint(0, 97, (2, n), generator=gen) for n in (70, 5, 1, 3))
+    with ts.no_grad(), torch.no_grad():
+        both = [lm.new_cache(2, 160, quantized="int4") for _ in range(2)]
+        for caches in both:
+            lm(prompt, caches=caches)
+            caches[0].cache.fork([0, -1])
+            lm(chunk, caches=caches)
+        caches, twin = both
+        good, part.forward = part.forward, fail
+        with pytest.raises(Failure):
+            lm(wrong, caches=caches)
+        part.forward = good
+        cache = caches[0].cache
+        assert cache.lengths.tolist() == cache.seq_lens.tolist() == [75, 5]
+        assert [layer.length for layer in caches] == [75, 75] and cache.free_pages() == twin[0].cache.free_pages()
+        for _ in range(2):
+            assert torch.equal(lm(step, caches=caches), lm(step, caches=twin))
+
+
+def test_truncation_of_ragged_rows():
+    m = Mirror(2, page_size=16)
+    m.append(20)
+    m.fork([0, -1, 1])
+    m.append(7)
+    m.cache.truncate([25, 3, 27])
+    m.tokens = [[layer[:n] for layer in row] for row, n in zip(m.tokens, (25, 3, 27))]
+    m.check()
+    m.append(2)
+    m.check()
+    # a step that one layer has appended goes whole, whatever it is truncated to
+    with ts.no_grad():
+        m.cache.layers[0].append(*(tensor(torch.ones(3, 2, 4, 64, device="cuda")),) * 2)
+    assert m.cache.lengths.tolist() == [31, 9, 33]
+    m.cache.layers[1].truncate(29)
+    assert m.cache.lengths.tolist() == [27, 5, 29] and [c.length for c in m.cache.layers] == [29, 29]
+    m.check()
+    m.truncate(6)
+    m.check()
+    for bad in ([6, 6, 6], [1, 2], [-1, 0, 0], [0.5, 0, 0], -1, 7):
+        with pytest.raises(ValueError):
+            m.cache.truncate(bad)
+    m.check()
