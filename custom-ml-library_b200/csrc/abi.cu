@@ -359,6 +359,7 @@ int check_int4_attn(const ts_attn_params* p, const ts_kv4_cache* c) {
   if (!p->q.data || !p->o.data || !p->kv_lens) return TS_ERR_INVALID_ARGUMENT;
   if (!(p->scale == p->scale) || p->scale > 1.0e300 || p->scale < -1.0e300) return TS_ERR_INVALID_ARGUMENT;
   if ((int64_t)p->q_heads / p->kv_heads * p->q_len > 0x40000000) return TS_ERR_UNSUPPORTED;
+  if (!tsa::attn_int4_supported(*p)) return TS_ERR_UNSUPPORTED;
   return TS_OK;
 }
 

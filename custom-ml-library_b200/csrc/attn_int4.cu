@@ -1,4 +1,6 @@
 // Host side of the attention over a 4-bit cache: what the kernels take, how the work is shared.
+#include <cstdlib>
+
 #include "attn_int4.cuh"
 
 namespace tsa {
@@ -17,15 +19,38 @@ bool rows_vec(const ts_view4& v, int size) {
          v.stride[1] * size % 16 == 0 && v.stride[2] * size % 16 == 0;
 }
 
-// Fills what follows from the problem; returns the grid's blocks.
-int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape) {
-  shape = int4_shape(p);
-  a.group = p.q_heads / p.kv_heads;
-  a.cols = a.group * p.q_len;
+int64_t max_units() {
+  const char* lower = std::getenv("TS_INT4_LINE");
+  const int64_t n = lower ? std::atoll(lower) : 0;
+  return n > 0 && n < kInt4MaxUnits ? n : kInt4MaxUnits;
+}
+
+struct Part {  // rows and query tokens of a launch; no tokens: one token of one row is too much already
+  int rows, tokens;
+};
+Part part_of(const ts_attn_params& p, const Int4Shape& shape) {
+  const int64_t limit = max_units(), columns = shape.nt * 8, group = p.q_heads / p.kv_heads;
+  const int64_t pair = (int64_t)ceil_div(p.kv_len, shape.keys) + 1, blocks = limit / (pair * p.kv_heads);
+  const int64_t tokens = i64min(p.q_len, i64min(blocks * columns / group, kInt4MaxUnits / p.q_heads));
+  if (tokens <= 0) return Part{0, 0};
+  const int64_t row = pair * p.kv_heads * ((tokens * group + columns - 1) / columns);
+  const int64_t rows = i64min(limit / row, kInt4MaxUnits / (p.q_heads * tokens));  // its output rows are counted too
+  return Part{(int)i64min(i64min(p.batch, kInt4MaxRows), rows), (int)tokens};
+}
+
+void set_tokens(const Int4Shape& shape, int tokens, Int4Attn& a) {
+  a.cols = a.group * tokens;
   a.col_blocks = ceil_div(a.cols, shape.nt * 8);
+}
+
+// Fills what follows from the problem and its parts; returns the grid's blocks.
+int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape, Part& part) {
+  shape = int4_shape(p);
+  part = part_of(p, shape);
+  a.group = p.q_heads / p.kv_heads;
+  set_tokens(shape, part.tokens, a);
   a.slot_cols = a.cols < shape.nt * 8 ? a.cols : shape.nt * 8;
-  const int rows = p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows;
-  const int64_t pairs = (int64_t)rows * p.kv_heads * a.col_blocks;
+  const int64_t pairs = (int64_t)part.rows * p.kv_heads * a.col_blocks;
   a.by_pair = shape.by_pair;
   // One wave of blocks that fill the GPU, fewer where a warp would be left without a stage.
   const int blocks = a.by_pair ? (int)pairs
@@ -61,20 +86,23 @@ Int4Shape int4_shape(const ts_attn_params& p) {
   return {1, 64, 4, 3, false, twin};
 }
 
+bool attn_int4_supported(const ts_attn_params& p) { return part_of(p, int4_shape(p)).tokens > 0; }
+
 size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
   Int4Attn a;
   Int4Shape shape;
-  plan(p, a, shape);
+  Part part;
+  plan(p, a, shape, part);
   if (a.by_pair) return 0;
-  const int rows = p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows;
-  return partial_bytes(a, shape, p.head_dim) + (size_t)2 * (rows + 1) * sizeof(int32_t);
+  return partial_bytes(a, shape, p.head_dim) + (size_t)2 * (part.rows + 1) * sizeof(int32_t);
 }
 
 cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
                               uint32_t* fault, cudaStream_t st) {
   Int4Attn a;
   Int4Shape shape;
-  int blocks = plan(p, a, shape);
+  Part each;
+  int blocks = plan(p, a, shape, each);
   if (ws_bytes < attn_int4_workspace(p, c)) return cudaErrorInvalidValue;
   a.p = p;
   a.c = c;
@@ -87,24 +115,27 @@ cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, vo
   const int size = p.dtype == TS_F32 ? 4 : 2;
   a.q_vec = rows_vec(p.q, size);
   a.o_vec = rows_vec(p.o, size);
-  if ((int64_t)(p.batch < kInt4MaxRows ? p.batch : kInt4MaxRows) * p.q_heads * p.q_len > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  for (int row = 0; row < p.batch; row += kInt4MaxRows) {  // launches follow one another on the stream
-    Int4Attn part = a;
-    part.p.batch = p.batch - row < kInt4MaxRows ? p.batch - row : kInt4MaxRows;
-    part.p.q.data = reinterpret_cast<unsigned char*>(p.q.data) + row * p.q.stride[0] * size;
-    part.p.o.data = reinterpret_cast<unsigned char*>(p.o.data) + row * p.o.stride[0] * size;
-    if (p.lse) part.p.lse = reinterpret_cast<float*>(p.lse) + row * p.lse_stride[0];
-    part.p.kv_lens = p.kv_lens + row;
-    part.c.table = c.table + row * c.table_stride;
-    cudaError_t e = cudaErrorInvalidValue;
-    if (a.by_pair) blocks = part.p.batch * p.kv_heads * a.col_blocks;
-    switch (p.dtype) {
-      case TS_BF16: e = attn_int4_launch<__nv_bfloat16>(part, shape, blocks, st); break;
-      case TS_F16: e = attn_int4_launch<__half>(part, shape, blocks, st); break;
-      case TS_F32: e = attn_int4_launch<float>(part, shape, blocks, st); break;
+  for (int token = 0; token < p.q_len; token += each.tokens)  // launches follow one another on the stream
+    for (int row = 0; row < p.batch; row += each.rows) {
+      Int4Attn part = a;
+      part.p.batch = (int)i64min(p.batch - row, each.rows);
+      part.p.q_len = (int)i64min(p.q_len - token, each.tokens);
+      part.tokens_left = p.q_len - token;
+      set_tokens(shape, part.p.q_len, part);
+      part.p.q.data = reinterpret_cast<unsigned char*>(p.q.data) + (row * p.q.stride[0] + token * p.q.stride[2]) * size;
+      part.p.o.data = reinterpret_cast<unsigned char*>(p.o.data) + (row * p.o.stride[0] + token * p.o.stride[2]) * size;
+      if (p.lse) part.p.lse = reinterpret_cast<float*>(p.lse) + row * p.lse_stride[0] + token * p.lse_stride[2];
+      part.p.kv_lens = p.kv_lens + row;
+      part.c.table = c.table + row * c.table_stride;
+      cudaError_t e = cudaErrorInvalidValue;
+      if (a.by_pair) blocks = part.p.batch * p.kv_heads * part.col_blocks;
+      switch (p.dtype) {
+        case TS_BF16: e = attn_int4_launch<__nv_bfloat16>(part, shape, blocks, st); break;
+        case TS_F16: e = attn_int4_launch<__half>(part, shape, blocks, st); break;
+        case TS_F32: e = attn_int4_launch<float>(part, shape, blocks, st); break;
+      }
+      if (e != cudaSuccess) return e;
     }
-    if (e != cudaSuccess) return e;
-  }
   return cudaSuccess;
 }
 

@@ -43,6 +43,9 @@
 namespace tsa {
 
 constexpr int kInt4MaxRows = 1024;  // rows of one launch: their prefix sums sit in shared memory
+// Units of one launch's line of work (see Int4Shares), which the kernels count in 32 bits with room for a share
+// more: a call with a longer line takes several launches.
+constexpr int64_t kInt4MaxUnits = 1 << 30;
 
 struct Int4Attn {
   ts_attn_params p;
@@ -52,6 +55,7 @@ struct Int4Attn {
   int cols;        // query columns of a KV head: group * q_len, token-major (column = token * group + head)
   int col_blocks;  // blocks of columns; one warp holds one at a time
   int slot_cols;   // columns of a block that can be live
+  int tokens_left; // query tokens of a row from this launch's first on
   int blocks;      // that share the work
   bool by_pair;    // one block a (row, KV head, column block) instead of equal shares
   int parts;       // about how many warps share a row where rows are of one length
@@ -530,7 +534,7 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
     for (int j = 0; j < 2; ++j) {
       const int mine = kTwin ? (2 * t + j) & 3 : col0 + nt * 8 + 2 * t + j;
       const int tok = min(mine, a.cols - 1) / a.group;
-      q.limit[nt][j] = a.p.is_causal ? max(-1, len - a.p.q_len + tok) : len - 1;
+      q.limit[nt][j] = a.p.is_causal ? max(-1, len - a.tokens_left + tok) : len - 1;
       q.m[nt][j] = -INFINITY;
       q.l[nt][j] = 0.f;
     }
@@ -817,7 +821,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
     if (!kEarly || n > 0) int4_fetch_queries<T, DG, NT, kTwin>(a, raw, p.b, hk, col0);
     int4_load_queries<T, DG, NT, kTwin>(a, q, raw, col0, len);
     // the first key that some column does not see
-    const int plain = a.p.is_causal ? min(len, max(0, len - a.p.q_len + col0 / a.group + 1)) : len;
+    const int plain = a.p.is_causal ? min(len, max(0, len - a.tokens_left + col0 / a.group + 1)) : len;
     int key0 = p.st * KT;
     for (int k = 0; k < count; ++k, ++n, key0 += KT) {
       if (issued < mine) issue(issued++);

@@ -324,7 +324,9 @@ TS_ATTN_API int ts_kv_gather_int4(const ts_kv4_cache* cache, const int32_t* star
  * problem, for tests and measurements. */
 TS_ATTN_API int ts_attn_int4_path(const ts_attn_params* params, const ts_kv4_cache* cache);
 
-/* Workspace bytes ts_attn_int4 needs. */
+/* Workspace bytes ts_attn_int4 needs.  (A problem over the pages whose line of
+ * work passes 2^30 stages runs in several launches; the environment variable
+ * TS_INT4_LINE lowers that limit, for tests.) */
 TS_ATTN_API size_t ts_attn_int4_workspace_size(const ts_attn_params* params, const ts_kv4_cache* cache);
 
 /* Attention of q [batch, Hq, Tq, D] over the cache: params as for ts_attn_decode,

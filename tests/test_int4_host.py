@@ -194,3 +194,18 @@ def test_page_oracle_shares_copies_and_closes_up():
     o.compact()
     assert o.table.tolist() == [[3, 0, -1], [3, 4, -1], [2, 1, -1]] and o.refs.tolist() == [1, 1, 1, 2, 1, 0, 0, 0]
     assert not o.reserve([100, 0, 0])
+
+
+def test_attention_refuses_a_line_of_work_past_32_bits():
+    """64 heads of 2^25 stages for one token; half as many heads, or many tokens of a shorter row, run in parts."""
+    def cache(heads, tokens):
+        return _cache(slots=tokens // 64, table_stride=tokens // 64, kv_heads=heads, page_stride=heads * 9216)
+
+    most = 0x7FFFFF00
+    for heads, kv_len, q_len, ok in ((64, most, 1, False), (8, most, 1, True), (8, most // 2, 4096, True)):
+        c = cache(heads, kv_len)
+        p = _params(dtype=_lib.F32, q_heads=heads, kv_heads=heads, kv_len=kv_len, q_len=q_len)
+        need = _lib.lib().ts_attn_int4_workspace_size(ctypes.byref(p), ctypes.byref(c))
+        assert (need > 0) == ok
+        assert _lib.lib().ts_attn_int4(ctypes.byref(p), ctypes.byref(c), None, 0, None) == (
+            _lib.ERR_WORKSPACE if ok else _lib.ERR_UNSUPPORTED)
