@@ -425,6 +425,9 @@ int ts_kv_append_int4(ts_view4 key, ts_view4 value, int32_t dtype, int32_t steps
   if (st != TS_OK) return st;
   if (!int4_dtype_ok(dtype)) return TS_ERR_UNSUPPORTED;
   if (!key.data || !value.data) return TS_ERR_INVALID_ARGUMENT;
+  // a row's blocks read its position while one of them writes the next one
+  if (positions && positions_out && positions < positions_out + cache->batch && positions_out < positions + cache->batch)
+    return TS_ERR_INVALID_ARGUMENT;
   if (steps <= 0) return TS_ERR_CAPACITY;
   if (!positions && (position < 0 || position + steps > (int64_t)cache->slots * cache->page_size))
     return TS_ERR_CAPACITY;

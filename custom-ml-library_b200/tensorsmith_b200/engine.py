@@ -490,7 +490,8 @@ class _Int4Cache:
 
 def kv_append_int4(key, value, pool, page_table, *, page_size, position=0, positions=None, positions_out=None):
     """Quantise a [B, Hkv, steps, D] chunk into the pages of its rows, at token ``position`` (or per-row
-    ``positions``).  The table must hold a page for every token written (``kv_pages_reserve``)."""
+    ``positions``).  ``positions_out``, another vector, receives where the rows then end.  The table must hold a page
+    for every token written (``kv_pages_reserve``)."""
     if key.dim() != 4:
         raise ValueError("key must be [rows, kv heads, tokens, head dimension] of the cache")
     rows, heads, steps, dim = key.shape

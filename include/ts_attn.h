@@ -304,9 +304,10 @@ TS_ATTN_API size_t ts_kv4_block_bytes(int32_t head_dim, int32_t page_size);
 /* Quantising append: tokens [pos_b, pos_b + steps) of every row receive the rows
  * of key / value [batch, kv_heads, steps, D] (dtype F32, F16 or BF16), with
  * pos_b = positions[b], or position for every row when positions is NULL.
- * positions_out (optional, [batch]) receives pos_b + steps.  The table must
- * already hold a page for every token written (ts_kv_pages_reserve); a token
- * without one is not written and sets the fault word (TS_ERR_PAGE). */
+ * positions_out (optional, [batch]) receives pos_b + steps; it must not overlap
+ * positions.  The table must already hold a page for every token written
+ * (ts_kv_pages_reserve); a token without one is not written and sets the fault
+ * word (TS_ERR_PAGE). */
 TS_ATTN_API int ts_kv_append_int4(ts_view4 key, ts_view4 value, int32_t dtype, int32_t steps,
                                   const ts_kv4_cache* cache, int64_t position, const int32_t* positions,
                                   int32_t* positions_out, void* stream);

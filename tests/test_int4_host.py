@@ -209,3 +209,13 @@ def test_attention_refuses_a_line_of_work_past_32_bits():
         assert (need > 0) == ok
         assert _lib.lib().ts_attn_int4(ctypes.byref(p), ctypes.byref(c), None, 0, None) == (
             _lib.ERR_WORKSPACE if ok else _lib.ERR_UNSUPPORTED)
+
+
+def test_append_refuses_to_advance_positions_in_place():
+    h, ok = _lib.lib(), ctypes.byref(_cache())
+    view = _lib.View4(4096, (ctypes.c_int64 * 4)(1, 1, 1, 1))
+    # no steps: refused as such once the positions have passed
+    for positions, out, status in ((4096, 4096, _lib.ERR_INVALID_ARGUMENT), (4096, 4100, _lib.ERR_INVALID_ARGUMENT),
+                                   (4100, 4096, _lib.ERR_INVALID_ARGUMENT), (4096, 4104, _lib.ERR_CAPACITY),
+                                   (None, 4096, _lib.ERR_CAPACITY), (4096, None, _lib.ERR_CAPACITY)):
+        assert h.ts_kv_append_int4(view, view, _lib.BF16, 0, ok, 0, positions, out, None) == status
