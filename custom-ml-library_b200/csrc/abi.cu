@@ -505,7 +505,9 @@ int ts_kv_pages_reserve(const ts_page_pool* pool, int32_t* table, int64_t table_
   if (st != TS_OK) return st;
   if (!table || !lens || !refs || !counters || rows <= 0 || slots <= 0 || page_size <= 0 || steps < 0)
     return TS_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < tsa::kv_pages_reserve_workspace(pool->pages, rows)) return TS_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < tsa::kv_pages_reserve_workspace(pool->pages, rows) ||
+      reinterpret_cast<uintptr_t>(workspace) % sizeof(int32_t))
+    return TS_ERR_WORKSPACE;
   return from_cuda(tsa::kv_pages_reserve(*pool, table, table_stride, lens, rows, slots, page_size, steps, row_steps,
                                          refs, counters, workspace, as_stream(stream)));
 }
@@ -522,7 +524,9 @@ int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* table, int64_t 
   if (st != TS_OK) return st;
   if (!table || !table_out || !refs || !refs_out || !counters || rows <= 0 || slots <= 0)
     return TS_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < tsa::kv_pages_compact_workspace(pool->pages)) return TS_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < tsa::kv_pages_compact_workspace(pool->pages) ||
+      reinterpret_cast<uintptr_t>(workspace) % sizeof(int32_t))
+    return TS_ERR_WORKSPACE;
   return from_cuda(tsa::kv_pages_compact(*pool, table, table_out, rows, slots, table_stride, table_out_stride, refs,
                                          refs_out, counters, workspace, as_stream(stream)));
 }

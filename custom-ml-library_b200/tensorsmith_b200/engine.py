@@ -468,6 +468,15 @@ def _page_table(t, index: int) -> tuple:
     return t.data_ptr(), t.stride(0), rows, slots
 
 
+def _workspace(given, need: int, like):
+    """``given`` where it holds ``need`` bytes, else as many new ones on the device of ``like``."""
+    if given is None or given.numel() * given.element_size() < need:
+        return like.new_empty((need,), dtype=torch.uint8)
+    if given.get_device() != like.get_device() or not given.is_contiguous():
+        raise ValueError("a workspace must be contiguous, on the pool's device")
+    return given
+
+
 class _Int4Cache:
     """A checked pool with its page table: the packed ts_kv4_cache and the sizes the callers need."""
 
@@ -592,8 +601,8 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
     cache, params = _int4_attn_args(q, pool, page_table, kv_lens, page_size, max_len, is_causal, scale, out, lse)
     handle = _lib.lib()
     need = handle.ts_attn_int4_workspace_size(params, cache.packed)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = pool.new_empty((need,))
+    if need:
+        workspace = _workspace(workspace, need, pool)
     status = handle.ts_attn_int4(params, cache.packed, workspace.data_ptr() if need else None, need,
                                  _raw_stream(cache.index))
     if status:
@@ -684,8 +693,7 @@ def kv_pages_reserve(pool, page_table, lens, steps, refs, counters, *, page_size
         raise ValueError("steps must not be negative and the page size must be positive")
     handle = _lib.lib()
     need = handle.ts_kv_pages_reserve_workspace_size(pages, rows)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = page_table.new_empty((need // 4,))
+    workspace = _workspace(workspace, need, page_table)
     status = handle.ts_kv_pages_reserve(
         packed, table, stride, _int32_vector(lens, "lens", rows, device), rows, slots, page_size, steps, row_steps,
         _int32_vector(refs, "refs", pages, device), _int32_vector(counters, "counters", 4, device),
@@ -706,8 +714,7 @@ def kv_pages_compact(pool, page_table, refs, counters, *, table_out=None, refs_o
         raise ValueError("table_out must have the table's shape")
     handle = _lib.lib()
     need = handle.ts_kv_pages_compact_workspace_size(pages)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = page_table.new_empty((need // 4,))
+    workspace = _workspace(workspace, need, page_table)
     status = handle.ts_kv_pages_compact(
         packed, table, stride, out, out_stride, rows, slots, _int32_vector(refs, "refs", pages, device),
         _int32_vector(refs_out, "refs_out", pages, device), _int32_vector(counters, "counters", 4, device),

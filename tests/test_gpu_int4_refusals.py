@@ -1,0 +1,31 @@
+"""Arguments of the 4-bit cache's calls that are refused before anything is launched."""
+
+import pytest
+
+from test_gpu_int4_cache import Cache
+from test_gpu_kv_pages import Pages
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from tensorsmith_b200 import engine  # noqa: E402
+
+
+def test_workspaces_elsewhere_or_scattered():
+    c = Cache([300, 200], 2, 64, 16)
+    c.fill("bfloat16")
+    q = torch.randn(2, 4, 1, 64, device="cuda", dtype=torch.bfloat16)
+    p = Pages([20, 5], 12, 16)
+    args = dict(page_size=16)
+    calls = [lambda ws: engine.attention_int4(q, c.pool, c.table, c.kv_lens, workspace=ws, **args),
+             lambda ws: engine.kv_pages_reserve(p.pool, p.table, p.lens, 1, p.refs, p.counters, workspace=ws, **args),
+             lambda ws: engine.kv_pages_compact(p.pool, p.table, p.refs, p.counters, workspace=ws)]
+    for call in calls:
+        for bad in (torch.empty(1 << 22, dtype=torch.uint8), torch.empty(1, device="cuda").expand(1 << 22),
+                    torch.empty(1 << 22, 2, dtype=torch.uint8, device="cuda")[:, 0]):
+            with pytest.raises(ValueError, match="workspace"):
+                call(bad)
+        call(torch.empty(1 << 22, dtype=torch.uint8, device="cuda"))
+        call(torch.empty(1, dtype=torch.uint8))  # too small to be used: a new one takes its place
+    torch.cuda.synchronize()
+    engine.check_device_status()

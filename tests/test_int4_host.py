@@ -219,3 +219,10 @@ def test_append_refuses_to_advance_positions_in_place():
                                    (4100, 4096, _lib.ERR_INVALID_ARGUMENT), (4096, 4104, _lib.ERR_CAPACITY),
                                    (None, 4096, _lib.ERR_CAPACITY), (4096, None, _lib.ERR_CAPACITY)):
         assert h.ts_kv_append_int4(view, view, _lib.BF16, 0, ok, 0, positions, out, None) == status
+
+
+def test_page_calls_refuse_an_unaligned_workspace():
+    h, a = _lib.lib(), 4096
+    pool = ctypes.byref(_lib.PagePool(4096, 1 << 20, 1024, 1024, 2, 8))
+    assert h.ts_kv_pages_reserve(pool, a, 4, a, 2, 4, 16, 1, None, a, a, a + 2, 1 << 20, None) == _lib.ERR_WORKSPACE
+    assert h.ts_kv_pages_compact(pool, a, 4, a, 4, 2, 4, a, a, a, a + 1, 1 << 20, None) == _lib.ERR_WORKSPACE
