@@ -411,6 +411,9 @@ int check_page_pool(const ts_page_pool* p) {
   return TS_OK;
 }
 
+// A table that is written to: its rows share no entry.
+bool table_rows_apart(int64_t stride, int rows, int slots) { return rows == 1 || stride >= slots; }
+
 }  // namespace
 
 extern "C" {
@@ -490,6 +493,7 @@ int ts_kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* 
       lens == lens_out)
     return TS_ERR_INVALID_ARGUMENT;
   if (rows <= 0 || rows_out <= 0 || slots <= 0 || page_size <= 0 || pages <= 0) return TS_ERR_INVALID_ARGUMENT;
+  if (!table_rows_apart(table_out_stride, rows_out, slots)) return TS_ERR_INVALID_ARGUMENT;
   return from_cuda(tsa::kv_pages_fork(table, table_stride, lens, rows, index, table_out, table_out_stride, lens_out,
                                       rows_out, slots, page_size, refs, pages, counters, as_stream(stream)));
 }
@@ -505,6 +509,7 @@ int ts_kv_pages_reserve(const ts_page_pool* pool, int32_t* table, int64_t table_
   if (st != TS_OK) return st;
   if (!table || !lens || !refs || !counters || rows <= 0 || slots <= 0 || page_size <= 0 || steps < 0)
     return TS_ERR_INVALID_ARGUMENT;
+  if (!table_rows_apart(table_stride, rows, slots)) return TS_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < tsa::kv_pages_reserve_workspace(pool->pages, rows) ||
       reinterpret_cast<uintptr_t>(workspace) % sizeof(int32_t))
     return TS_ERR_WORKSPACE;
@@ -524,6 +529,7 @@ int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* table, int64_t 
   if (st != TS_OK) return st;
   if (!table || !table_out || !refs || !refs_out || !counters || rows <= 0 || slots <= 0)
     return TS_ERR_INVALID_ARGUMENT;
+  if (!table_rows_apart(table_out_stride, rows, slots)) return TS_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < tsa::kv_pages_compact_workspace(pool->pages) ||
       reinterpret_cast<uintptr_t>(workspace) % sizeof(int32_t))
     return TS_ERR_WORKSPACE;

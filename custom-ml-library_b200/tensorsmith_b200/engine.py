@@ -460,11 +460,13 @@ def _int32_vector(t, name: str, size: int, index: int) -> int:
     return t.data_ptr()
 
 
-def _page_table(t, index: int) -> tuple:
-    """(pointer, stride, rows, slots) of a page table."""
+def _page_table(t, index: int, *, written: bool = False) -> tuple:
+    """(pointer, stride, rows, slots) of a page table; rows that are ``written`` must not share entries."""
     if t.dtype != torch.int32 or t.dim() != 2 or t.get_device() != index or t.stride(1) != 1 or 0 in t.shape:
         raise ValueError("a page table must be int32 [rows, slots] with contiguous rows on the pool's device")
     rows, slots = t.shape
+    if written and rows > 1 and t.stride(0) < slots:
+        raise ValueError("the rows of a page table that is written to must not overlap")
     return t.data_ptr(), t.stride(0), rows, slots
 
 
@@ -667,7 +669,7 @@ def kv_pages_fork(page_table, lens, index, refs, counters, *, page_size, table_o
         table_out = page_table.new_empty((n, slots))
     if lens_out is None:
         lens_out = lens.new_empty((n,))
-    out, out_stride, out_rows, out_slots = _page_table(table_out, device)
+    out, out_stride, out_rows, out_slots = _page_table(table_out, device, written=True)
     if (out_rows, out_slots) != (n, slots):
         raise ValueError("table_out must be [len(index), slots]")
     status = _lib.lib().ts_kv_pages_fork(
@@ -685,7 +687,7 @@ def kv_pages_reserve(pool, page_table, lens, steps, refs, counters, *, page_size
     free pages for empty slots, a copy of a partly filled page that other rows hold too.  Works in place; when the
     pool or the table is too small it sets an error bit of ``counters[2]`` and changes nothing."""
     packed, pages, device, _, _ = _page_pool(pool)
-    table, stride, rows, slots = _page_table(page_table, device)
+    table, stride, rows, slots = _page_table(page_table, device, written=True)
     row_steps = None
     if isinstance(steps, torch.Tensor):
         row_steps, steps = _int32_vector(steps, "steps", rows, device), 0
@@ -709,7 +711,7 @@ def kv_pages_compact(pool, page_table, refs, counters, *, table_out=None, refs_o
     table, stride, rows, slots = _page_table(page_table, device)
     table_out = page_table if table_out is None else table_out
     refs_out = refs if refs_out is None else refs_out
-    out, out_stride, out_rows, out_slots = _page_table(table_out, device)
+    out, out_stride, out_rows, out_slots = _page_table(table_out, device, written=True)
     if (out_rows, out_slots) != (rows, slots):
         raise ValueError("table_out must have the table's shape")
     handle = _lib.lib()

@@ -344,7 +344,8 @@ TS_ATTN_API int ts_attn_int4(const ts_attn_params* params, const ts_kv4_cache* c
  * page number below which none is free (0 is always right), error bits, unused};
  * error bits, set and never cleared by the engine: 1 not enough free pages, 2 an
  * index or page out of range was skipped, 4 a row would need more slots than the
- * table has.  A reserve that sets 1 or 4 changes nothing. */
+ * table has.  A reserve that sets 1 or 4 changes nothing.  The rows of a table
+ * that a call writes to must not overlap. */
 typedef struct ts_page_pool {
   void* data;                        /* 16-byte aligned */
   int64_t layer_stride, page_stride; /* bytes, multiples of 16 */

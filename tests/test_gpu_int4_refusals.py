@@ -29,3 +29,23 @@ def test_workspaces_elsewhere_or_scattered():
         call(torch.empty(1, dtype=torch.uint8))  # too small to be used: a new one takes its place
     torch.cuda.synchronize()
     engine.check_device_status()
+
+
+def test_tables_whose_rows_overlap():
+    p = Pages([20, 5], 12, 16)
+    shared = p.table[:1].expand(2, -1)
+    index = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        engine.kv_pages_reserve(p.pool, shared, p.lens, 1, p.refs, p.counters, page_size=16)
+    with pytest.raises(ValueError, match="overlap"):
+        engine.kv_pages_fork(p.table, p.lens, index, p.refs, p.counters, page_size=16, table_out=shared)
+    with pytest.raises(ValueError, match="overlap"):
+        engine.kv_pages_compact(p.pool, shared, p.refs, p.counters)
+    p.check()
+    # rows that only read the same pages may share a table row
+    c = Cache([40], 1, 64, 16)
+    c.fill("bfloat16")
+    q = torch.randn(1, 1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    one, _ = engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=16)
+    two, _ = engine.attention_int4(q.expand(2, -1, -1, -1), c.pool, c.table.expand(2, -1), c.kv_lens.repeat(2), page_size=16)
+    assert torch.equal(two[0], one[0]) and torch.equal(two[1], one[0])

@@ -226,3 +226,14 @@ def test_page_calls_refuse_an_unaligned_workspace():
     pool = ctypes.byref(_lib.PagePool(4096, 1 << 20, 1024, 1024, 2, 8))
     assert h.ts_kv_pages_reserve(pool, a, 4, a, 2, 4, 16, 1, None, a, a, a + 2, 1 << 20, None) == _lib.ERR_WORKSPACE
     assert h.ts_kv_pages_compact(pool, a, 4, a, 4, 2, 4, a, a, a, a + 1, 1 << 20, None) == _lib.ERR_WORKSPACE
+
+
+def test_page_calls_refuse_tables_whose_rows_overlap():
+    h, a, bad = _lib.lib(), 4096, _lib.ERR_INVALID_ARGUMENT
+    pool = ctypes.byref(_lib.PagePool(4096, 1 << 20, 1024, 1024, 2, 8))
+    for stride in (0, 3):  # of two rows with four slots
+        assert h.ts_kv_pages_fork(a, 4, a, 2, a, 8192, stride, 8192, 2, 4, 16, a, 8, a, None) == bad
+        # refused for the table, before the workspace that is missing
+        assert h.ts_kv_pages_reserve(pool, a, stride, a, 2, 4, 16, 1, None, a, a, None, 0, None) == bad
+        assert h.ts_kv_pages_compact(pool, a, stride, a, stride, 2, 4, a, a, a, None, 0, None) == bad
+    assert h.ts_kv_pages_reserve(pool, a, 0, a, 1, 4, 16, 1, None, a, a, None, 0, None) == _lib.ERR_WORKSPACE
