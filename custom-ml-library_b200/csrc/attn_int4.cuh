@@ -465,7 +465,9 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const bool live = (kTwin ? g & 3 : col0 + nt * 8 + g) < a.cols;
+    const int col = kTwin ? g & 3 : col0 + nt * 8 + g;
+    // A query that sees no key counts as zeros, whatever it holds: its hidden scores stay -inf and its row empty.
+    const bool live = col < a.cols && (!a.p.is_causal || len >= a.tokens_left || col / a.group >= a.tokens_left - len);
     float x[DG][8], amax = 0.f;
     bool odd = false;  // a NaN anywhere in the row
 #pragma unroll

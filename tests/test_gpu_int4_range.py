@@ -90,3 +90,29 @@ def test_keys_over_the_whole_range(dtype, group, q_len):
     assert (np.abs(to_np(out).astype(np.float64) - ref) <= bound).all()
     finite = np.isfinite(ref_lse)
     assert (np.abs(to_np(lse).astype(np.float64)[finite] - ref_lse[finite]) <= 2.0**-19 * (1 + top)).all()
+
+
+@pytest.mark.parametrize("path", ["pages", "prefill"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("group, q_len", [(1, 3), (3, 7), (1, 40)])
+def test_queries_that_see_no_key_may_hold_anything(path, dtype, group, q_len, monkeypatch):
+    """The first tokens of a chunk longer than its row: zeros and -inf, like a row without tokens, beside queries
+    that are as before."""
+    if path == "prefill" and dtype == "float32":
+        pytest.skip("the prefill kernel takes half types")
+    c = Cache([0, 2, 1, 90], 2, 64, 16, seed=2)
+    c.fill(dtype)
+    monkeypatch.setenv("TS_INT4_KERNEL", path)
+    kw = dict(page_size=16, max_len=90, need_lse=True)
+    q = torch.randn(4, 2 * group, q_len, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    q = q.to(torch_dtype(dtype))
+    want, want_lse = engine.attention_int4(q, c.pool, c.table, c.kv_lens, **kw)
+    odd = q.clone()
+    for r, n in enumerate(c.lens):
+        blind = max(0, q_len - int(n))
+        odd[r, :, :blind, ::3] = float("nan")
+        odd[r, :, :blind, 1::3] = float("inf")
+    got, got_lse = engine.attention_int4(odd, c.pool, c.table, c.kv_lens, **kw)
+    engine.check_device_status()
+    assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+    assert not got[0].any() and not got[2, :, :-1].any() and torch.isneginf(got_lse[1, :, : q_len - 2]).all()
