@@ -411,8 +411,8 @@ class TransformerLM(_Module):
             return PagedKVCache(batch_size, len(self.blocks), attention.num_kv_heads, attention.head_dim, capacity,
                                 num_pages=num_pages, device=f"cuda:{self._device_index}",
                                 dtype=self.token_embedding_weight.dtype).layers
-        if not isinstance(quantized, bool) or num_pages is not None:
-            raise ValueError('quantized must be a bool or "int4", and only "int4" has pages')
+        if isinstance(quantized, str) or num_pages is not None:
+            raise ValueError('quantized must be a truth value or "int4", and only "int4" has pages')
         return [
             KVCache(batch_size, block.attention.num_kv_heads, block.attention.head_dim, capacity,
                     device=f"cuda:{self._device_index}", dtype=self.token_embedding_weight.dtype, quantized=quantized)

@@ -67,3 +67,15 @@ def test_truncation_of_ragged_rows():
         with pytest.raises(ValueError):
             m.cache.truncate(bad)
     m.check()
+
+
+def test_quantized_takes_any_truth_value():
+    lm = model()
+    for value in (1, True, np.True_):
+        assert all(cache.quantized for cache in lm.new_cache(1, 32, quantized=value))
+    for value in (0, None, False, np.False_):
+        assert not any(cache.quantized for cache in lm.new_cache(1, 32, quantized=value))
+    prompt = torch.zeros(1, 4, dtype=torch.int64)
+    for value, same in ((1, True), (None, False)):
+        assert torch.equal(lm.generate(prompt, 3, temperature=0, quantized_cache=value),
+                           lm.generate(prompt, 3, temperature=0, quantized_cache=same))
