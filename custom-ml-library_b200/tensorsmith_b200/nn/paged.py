@@ -277,8 +277,8 @@ class PagedLayer:
         engine.kv_append_int4(raw, val, self.pool, cache._table, page_size=cache.page_size, positions=cache._before)
         self.length += steps
 
-    def attend(self, query: Tensor, *, scale: float | None = None) -> Tensor:
-        """Causal attention of ``query`` [B, Hq, Tq, D], the newest Tq tokens of every row, over the row's pages."""
+    def attend(self, query: Tensor, *, scale: float | None = None, is_causal: bool = True) -> Tensor:
+        """Attention of ``query`` [B, Hq, Tq, D], the newest Tq tokens of every row, over the row's pages."""
         cache = self.cache
         if query.ndim != 4 or query.shape[0] != cache.batch_size or query.shape[-1] != cache.head_dim:
             raise ValueError("query shape does not match cache configuration")
@@ -289,7 +289,7 @@ class PagedLayer:
         if self.length != cache.length or self.length == 0 or query.shape[2] > self.length:
             raise ValueError("the cache must already hold the query tokens")
         out, _ = engine.attention_int4(query._data, self.pool, cache._table, cache._lens, page_size=cache.page_size,
-                                       max_len=self.length, scale=scale)
+                                       max_len=self.length, is_causal=is_causal, scale=scale)
         return Tensor(out, device=cache.device)
 
     def get(self) -> tuple[Tensor, Tensor]:

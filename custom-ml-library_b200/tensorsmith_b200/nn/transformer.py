@@ -255,7 +255,7 @@ class MultiHeadAttention(_Module):
                     raise ValueError("a paged cache takes no attention mask")
                 (cache.append_rotary if self.rotary else cache.append)(_mirror(k), _mirror(v))
                 q_t = _mirror(engine.rope(q, positions=cache.cache.positions) if self.rotary else q)
-                attended = cache.attend(q_t)._data
+                attended = cache.attend(q_t, is_causal=is_causal)._data
                 return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
             q_t = _mirror(engine.rope(q, offset=offset) if self.rotary else q)
             if cache is not None:

@@ -3,12 +3,15 @@
 import numpy as np
 import pytest
 
+import oracle
+from helpers import to_np
 from test_gpu_paged_cache import Mirror, model, tensor
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 import tensorsmith_b200 as ts  # noqa: E402
+from tensorsmith_b200 import engine, nn  # noqa: E402
 
 
 class Failure(Exception):
@@ -79,3 +82,23 @@ def test_quantized_takes_any_truth_value():
     for value, same in ((1, True), (None, False)):
         assert torch.equal(lm.generate(prompt, 3, temperature=0, quantized_cache=value),
                            lm.generate(prompt, 3, temperature=0, quantized_cache=same))
+
+
+@pytest.mark.parametrize("is_causal", [True, False])
+def test_the_attention_module_passes_the_mask_on(is_causal):
+    """A chunk of five tokens over pages that hold them and seven before, against fp64 attention over the pages."""
+    attention = model(layers=1).blocks[0].attention
+    cache = nn.PagedKVCache(2, 1, 2, 32, 64, device="cuda:0", page_size=16)
+    layer = cache.layers[0]
+    gen = torch.Generator("cuda").manual_seed(0)
+    first, x = (torch.randn(2, n, 128, generator=gen, device="cuda") for n in (7, 5))
+    with ts.no_grad(), torch.no_grad():
+        attention(first, cache=layer)
+        got = attention(x, cache=layer, is_causal=is_causal)
+        q = engine.rope(attention.q_proj(x).reshape(2, 5, 4, 32).permute(0, 2, 1, 3), offset=7)
+        keys, values = (to_np(t._data).astype(np.float64) for t in layer.get())
+        ref, _, _ = oracle.attention_int4(to_np(q).astype(np.float64), list(keys), list(values), [12, 12],
+                                          is_causal=is_causal)
+        want = attention.out_proj(torch.from_numpy(ref).float().cuda().permute(0, 2, 1, 3).reshape(2, 5, 128))
+    # fp32 attention and one projection of 128 terms, at tf32 at worst
+    assert (got - want).abs().max() <= 1e-3 * want.abs().max()
