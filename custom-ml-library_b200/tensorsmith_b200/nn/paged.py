@@ -286,6 +286,8 @@ class PagedLayer:
             raise ValueError("query heads must be a multiple of the cache heads, on the cache device")
         if query.dtype != cache.dtype:
             raise TypeError("query dtype must be the cache compute dtype")
+        if is_grad_enabled() and query.requires_grad:
+            raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
         if self.length != cache.length or self.length == 0 or query.shape[2] > self.length:
             raise ValueError("the cache must already hold the query tokens")
         out, _ = engine.attention_int4(query._data, self.pool, cache._table, cache._lens, page_size=cache.page_size,

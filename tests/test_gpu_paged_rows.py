@@ -102,3 +102,14 @@ def test_the_attention_module_passes_the_mask_on(is_causal):
         want = attention.out_proj(torch.from_numpy(ref).float().cuda().permute(0, 2, 1, 3).reshape(2, 5, 128))
     # fp32 attention and one projection of 128 terms, at tf32 at worst
     assert (got - want).abs().max() <= 1e-3 * want.abs().max()
+
+
+def test_attend_refuses_a_query_that_wants_gradients():
+    m = Mirror(2, layers=1)
+    m.append(3)
+    layer = m.cache.layers[0]
+    query = ts.tensor(np.ones((2, 2, 1, 64), np.float32), device="cuda:0", requires_grad=True)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        layer.attend(query)
+    with ts.no_grad():
+        assert layer.attend(query).shape == (2, 2, 1, 64)
