@@ -262,6 +262,8 @@ class PagedLayer:
             raise ValueError("key shape does not match cache configuration")
         if value.shape != key.shape:
             raise ValueError("value shape does not match cache configuration")
+        if rotary is not None:
+            engine.dtype_code(key.dtype)  # raises on a type that cannot be rotated, before the step begins
         steps = key.shape[2]
         if self.length == cache.length:
             if steps == 0 or cache.length + steps > cache.max_seq_len:

@@ -113,3 +113,15 @@ def test_attend_refuses_a_query_that_wants_gradients():
         layer.attend(query)
     with ts.no_grad():
         assert layer.attend(query).shape == (2, 2, 1, 64)
+
+
+def test_a_refused_append_changes_nothing():
+    m = Mirror(2, page_size=16)
+    m.append(16)
+    free = m.cache.free_pages()
+    whole = tensor(torch.ones(2, 2, 1, 64, dtype=torch.int64, device="cuda"))
+    with ts.no_grad(), pytest.raises(TypeError):
+        m.cache.layers[0].append_rotary(whole, whole)
+    assert m.cache.length == 16 and m.cache.free_pages() == free
+    m.append(1)
+    m.check()
