@@ -67,6 +67,14 @@ struct Int4Attn {
 };
 
 __device__ __forceinline__ int int4_len(const Int4Attn& a, int b) { return min(a.p.kv_len, max(0, a.p.kv_lens[b])); }
+// The same for the merge ahead of its wait.  What wrote the lengths has ended by then, though the attention kernel has
+// not: that one's blocks let the merge start only after they have themselves waited for the kernels before them, whose
+// writes are at device scope with that.  The load asks there, past this SM's L1, which promises nothing before the wait.
+__device__ __forceinline__ int int4_len_early(const Int4Attn& a, int b) {
+  int n;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(n) : "l"(a.p.kv_lens + b) : "memory");
+  return min(a.p.kv_len, max(0, n));
+}
 // The shares count n + 1 units for a pair (KV head and column block) of a row with n stages: entering it
 // (its queries read, its result written) takes a warp about as long as a stage.  Unit 0 of a pair is the
 // entry, unit i + 1 its stage i.  Worker w takes the units [w * share, (w + 1) * share): the first `block_warps`
@@ -643,7 +651,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
   }
   int* first_unit = first + a.p.batch + 1;
   wait_for_previous();
-  let_next_start();  // the merge reads the lengths without waiting for this kernel's end
+  let_next_start();  // the merge reads the lengths without waiting for this kernel's end: not before the wait above
   if (warp == 0 && !a.by_pair) {  // stages and units of the rows before b
     int stages = 0, rows = 0;
     for (int b0 = 0; b0 <= a.p.batch; b0 += 32) {
@@ -950,7 +958,7 @@ __global__ void __launch_bounds__(256) attn_int4_combine(const __grid_constant__
   };
   const bool few = a.p.batch <= 32;
   if (few) {
-    const int stages = lane < a.p.batch ? ceil_div(int4_len(a, lane), keys) : 0, units = stages ? stages + 1 : 0;
+    const int stages = lane < a.p.batch ? ceil_div(int4_len_early(a, lane), keys) : 0, units = stages ? stages + 1 : 0;
     n = __shfl_sync(0xffffffffu, units, b);
     const int total = __reduce_add_sync(0xffffffffu, units), before = __reduce_add_sync(0xffffffffu, lane < b ? units : 0);
     if (n) locate(total * pairs, before * pairs);
