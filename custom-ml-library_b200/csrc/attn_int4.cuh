@@ -473,9 +473,7 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int col = kTwin ? g & 3 : col0 + nt * 8 + g;
-    // A query that sees no key counts as zeros, whatever it holds: its hidden scores stay -inf and its row empty.
-    const bool live = col < a.cols && (!a.p.is_causal || len >= a.tokens_left || col / a.group >= a.tokens_left - len);
+    const bool live = (kTwin ? g & 3 : col0 + nt * 8 + g) < a.cols;
     float x[DG][8], amax = 0.f;
     bool odd = false;  // a NaN anywhere in the row
 #pragma unroll
@@ -545,6 +543,7 @@ __device__ __forceinline__ void int4_load_queries(const Int4Attn& a, Int4State<T
       const int mine = kTwin ? (2 * t + j) & 3 : col0 + nt * 8 + 2 * t + j;
       const int tok = min(mine, a.cols - 1) / a.group;
       q.limit[nt][j] = a.p.is_causal ? max(-1, len - a.tokens_left + tok) : len - 1;
+      if (q.limit[nt][j] < 0) q.cs[nt][j] = 1.f;  // sees no key: its hidden scores stay -inf whatever the query holds
       q.m[nt][j] = -INFINITY;
       q.l[nt][j] = 0.f;
     }
