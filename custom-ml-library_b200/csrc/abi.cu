@@ -363,44 +363,75 @@ int check_int4_attn(const ts_attn_params* p, const ts_kv4_cache* c) {
   return TS_OK;
 }
 
-// Bytes of the dequantised keys (and of the values after them) the prefill route works on.
-size_t int4_prefill_half(const ts_attn_params& p) {
-  return (size_t)p.batch * p.kv_heads * p.kv_len * p.head_dim * 2;
+// The prefill route dequantises the keys and values of this many rows and KV heads at a time: as many as fit the
+// bytes of the pool, or 1 GiB where that is more, and one head of one row at the least.  (A row takes its room up
+// to kv_len, so a batch with one long row would otherwise ask for many times what its pages hold.)
+struct Int4Chunk {
+  int rows, heads;
+};
+int64_t int4_head_bytes(const ts_attn_params& p) { return (int64_t)4 * p.kv_len * p.head_dim; }  // keys and values
+Int4Chunk int4_chunk(const ts_attn_params& p, const ts_kv4_cache& c) {
+  const int64_t limit = tsa::i64max((int64_t)1 << 30, c.pages * c.page_stride);
+  const int64_t fit = tsa::i64max(1, limit / int4_head_bytes(p));
+  if (fit < p.kv_heads) return Int4Chunk{1, (int)fit};
+  return Int4Chunk{(int)tsa::i64min(tsa::i64min(p.batch, 32768), fit / p.kv_heads), p.kv_heads};
+}
+size_t int4_prefill_bytes(const ts_attn_params& p, const ts_kv4_cache& c) {
+  const Int4Chunk chunk = int4_chunk(p, c);
+  return (size_t)int4_head_bytes(p) * chunk.rows * chunk.heads;
 }
 
-// The same problem over contiguous keys and values of q's type at `ws`.
-ts_attn_params int4_prefill_params(const ts_attn_params& p, void* ws) {
+// Rows [row, row + chunk.rows) and KV heads [head, head + chunk.heads) of the problem over contiguous keys and
+// values of q's type at `ws`.
+ts_attn_params int4_prefill_params(const ts_attn_params& p, Int4Chunk chunk, int row, int head, void* ws) {
   ts_attn_params d = p;
-  const int64_t row = p.head_dim, head = row * p.kv_len;
-  d.k = ts_view4{ws, {head * p.kv_heads, head, row, 1}};
-  d.v = ts_view4{reinterpret_cast<unsigned char*>(ws) + int4_prefill_half(p), {head * p.kv_heads, head, row, 1}};
+  const int group = p.q_heads / p.kv_heads;
+  d.batch = (int)tsa::i64min(chunk.rows, p.batch - row);
+  d.kv_heads = (int)tsa::i64min(chunk.heads, p.kv_heads - head);
+  d.q_heads = d.kv_heads * group;
+  auto from = [&](const ts_view4& v) {
+    return reinterpret_cast<unsigned char*>(v.data) + (row * v.stride[0] + (int64_t)head * group * v.stride[1]) * 2;
+  };
+  d.q.data = from(p.q);
+  d.o.data = from(p.o);
+  if (p.lse)
+    d.lse = reinterpret_cast<float*>(p.lse) + row * p.lse_stride[0] + (int64_t)head * group * p.lse_stride[1];
+  d.kv_lens = p.kv_lens ? p.kv_lens + row : nullptr;
+  const int64_t stride = p.head_dim, keys = stride * p.kv_len, all = keys * d.kv_heads * d.batch;
+  d.k = ts_view4{ws, {keys * d.kv_heads, keys, stride, 1}};
+  d.v = ts_view4{reinterpret_cast<unsigned char*>(ws) + 2 * all, {keys * d.kv_heads, keys, stride, 1}};
   d.causal_offset = 0;
   return d;
 }
 
 // Whether dequantising the pages and running the prefill kernel is the faster way, by what each costs a cached
-// key in nanoseconds (measured at D = 128, bf16, 2 and 16 rows of 8 KV heads, groups of 1, 4 and 8 query heads,
+// key in nanoseconds (fitted at D = 128, bf16, 2 and 16 rows of 8 KV heads, groups of 1, 4 and 8 query heads,
 // 64, 128 and 256 query columns a KV head).  Over the pages the time grows with the columns (group x tokens):
 // 1.95e-3 a KV head and column.  The other way writes and reads the dequantised rows, 0.133 a KV head, and then
 // runs one query tile a block: 6.1 a wave of 128-row tiles, 13.4 of 256-row ones (more than 128 tokens), however
-// few of a tile's rows are filled.  16 rows, 64 columns: 147 against 199 to 524 us by group; 256 columns: 525
-// against 246, 343 and 549; 2 rows, 256 columns: 51 against 80, 49 and 50.
-bool int4_prefill_faster(const ts_attn_params& p) {
+// few of a tile's rows are filled; a chunk of the batch starts a wave of its own.  Rows of 8000 keys: 16 rows, 64
+// columns 186 against 225 to 625 us by group; 256 columns 686 against 261, 414 and 626; 2 rows, 256 columns 102
+// against 145, 93 and 94.  The same numbers serve f16 (its pages cost 1.16 times as much) and D = 64 (pages 0.65,
+// tiles 0.86): over these sizes and 1024 columns the way taken is the faster one or within 1.08 (bf16, D = 128),
+// 1.23 (f16, D = 128) and 1.20 (D = 64) of it.
+bool int4_prefill_faster(const ts_attn_params& p, const ts_kv4_cache& c) {
   const double heads = (double)p.batch * p.kv_heads, columns = (double)(p.q_heads / p.kv_heads) * p.q_len;
   const int rows = p.q_len > 128 ? 256 : 128;
-  const int64_t tiles = (int64_t)p.batch * p.q_heads * ((p.q_len + rows - 1) / rows);
-  const double waves = (double)((tiles + 147) / 148);
+  const Int4Chunk chunk = int4_chunk(p, c);
+  const int64_t tiles = (int64_t)chunk.rows * chunk.heads * (p.q_heads / p.kv_heads) * ((p.q_len + rows - 1) / rows);
+  const int64_t chunks = (int64_t)((p.batch + chunk.rows - 1) / chunk.rows) * ((p.kv_heads + chunk.heads - 1) / chunk.heads);
+  const double waves = (double)(chunks * ((tiles + 147) / 148));
   return 1.95e-3 * heads * columns > 0.133 * heads + waves * (rows == 256 ? 13.4 : 6.1);
 }
 
-bool int4_prefill(const ts_attn_params& p) {
+bool int4_prefill(const ts_attn_params& p, const ts_kv4_cache& c) {
   if (!int4_dtype_ok(p.dtype) || p.dtype == TS_F32) return false;
   alignas(16) static unsigned char aligned[16];  // stands for the workspace, which must be 16-byte aligned
-  if (!tsa::tc_fwd_supported(int4_prefill_params(p, aligned))) return false;
+  if (!tsa::tc_fwd_supported(int4_prefill_params(p, int4_chunk(p, c), 0, 0, aligned))) return false;
   const char* force = std::getenv("TS_INT4_KERNEL");
   if (force && !std::strcmp(force, "pages")) return false;
   if (force && !std::strcmp(force, "prefill")) return true;
-  return int4_prefill_faster(p);
+  return int4_prefill_faster(p, c);
 }
 
 int check_page_pool(const ts_page_pool* p) {
@@ -445,36 +476,46 @@ int ts_kv_gather_int4(const ts_kv4_cache* cache, const int32_t* starts, const in
   if (!int4_dtype_ok(dtype)) return TS_ERR_UNSUPPORTED;
   if (!key.data || !value.data || length < 0) return TS_ERR_INVALID_ARGUMENT;
   if (!starts && length > (int64_t)cache->slots * cache->page_size) return TS_ERR_INVALID_ARGUMENT;
-  return from_cuda(tsa::kv_gather_int4(*cache, starts, lens, key, value, dtype, length, fault_ptr(),
+  return from_cuda(tsa::kv_gather_int4(*cache, starts, lens, key, value, dtype, length, 0, fault_ptr(),
                                        as_stream(stream)));
 }
 
 int ts_attn_int4_path(const ts_attn_params* p, const ts_kv4_cache* cache) {
   const int st = check_int4_attn(p, cache);
   if (st != TS_OK) return st;
-  return int4_prefill(*p) ? TS_PATH_TCGEN05 : TS_PATH_DECODE;
+  return int4_prefill(*p, *cache) ? TS_PATH_TCGEN05 : TS_PATH_DECODE;
 }
 
 size_t ts_attn_int4_workspace_size(const ts_attn_params* p, const ts_kv4_cache* cache) {
   if (check_int4_attn(p, cache) != TS_OK) return 0;
-  return int4_prefill(*p) ? 2 * int4_prefill_half(*p) : tsa::attn_int4_workspace(*p, *cache);
+  return int4_prefill(*p, *cache) ? int4_prefill_bytes(*p, *cache) : tsa::attn_int4_workspace(*p, *cache);
 }
 
 int ts_attn_int4(const ts_attn_params* p, const ts_kv4_cache* cache, void* workspace, size_t workspace_bytes,
                  void* stream) {
   const int st = check_int4_attn(p, cache);
   if (st != TS_OK) return st;
-  const bool prefill = int4_prefill(*p);
-  const size_t need = prefill ? 2 * int4_prefill_half(*p) : tsa::attn_int4_workspace(*p, *cache);
+  const bool prefill = int4_prefill(*p, *cache);
+  const size_t need = prefill ? int4_prefill_bytes(*p, *cache) : tsa::attn_int4_workspace(*p, *cache);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return TS_ERR_WORKSPACE;
   if (!prefill)
     return from_cuda(tsa::attn_int4_forward(*p, *cache, workspace, workspace_bytes, fault_ptr(), as_stream(stream)));
-  const ts_attn_params d = int4_prefill_params(*p, workspace);
-  const cudaError_t e = tsa::kv_gather_int4(*cache, nullptr, p->kv_lens, d.k, d.v, p->dtype, p->kv_len, fault_ptr(),
-                                            as_stream(stream));
-  if (e != cudaSuccess) return from_cuda(e);
-  return from_cuda(tsa::tc_forward(d, fault_ptr(), as_stream(stream)));
+  const Int4Chunk chunk = int4_chunk(*p, *cache);
+  for (int row = 0; row < p->batch; row += chunk.rows)  // one after the other on the stream, in the same workspace
+    for (int head = 0; head < p->kv_heads; head += chunk.heads) {
+      const ts_attn_params d = int4_prefill_params(*p, chunk, row, head, workspace);
+      ts_kv4_cache c = *cache;
+      c.pool = reinterpret_cast<unsigned char*>(c.pool) + (int64_t)head * tsa::int4_block_bytes(c.head_dim, c.page_size);
+      c.kv_heads = d.kv_heads;
+      c.table += row * c.table_stride;
+      c.batch = d.batch;
+      cudaError_t e = tsa::kv_gather_int4(c, nullptr, d.kv_lens, d.k, d.v, d.dtype, d.kv_len, tsa::kTcKeyTile,
+                                          fault_ptr(), as_stream(stream));
+      if (e == cudaSuccess) e = tsa::tc_forward(d, fault_ptr(), as_stream(stream));
+      if (e != cudaSuccess) return from_cuda(e);
+    }
+  return TS_OK;
 }
 
 int ts_kv_pages_copy(const ts_page_pool* src, const ts_page_pool* dst, const int32_t* from, const int32_t* to,

@@ -46,7 +46,7 @@ namespace tsa {
 
 namespace {
 
-constexpr int kBM = 128, kBN = 128;
+constexpr int kBM = 128, kBN = kTcKeyTile;
 constexpr int kSlabBytes = 128 * 128;  // 128 rows x 128 bytes
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

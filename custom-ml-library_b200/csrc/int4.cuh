@@ -50,9 +50,10 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
                            int64_t position, const int32_t* positions, int32_t* positions_out, uint32_t* fault,
                            cudaStream_t st);
 // Dequantises tokens [starts[b] (or 0), + length) of every row; tokens at or past lens[b] (when
-// given) are written as zeros.
+// given) are written as zeros, with `tile` > 0 (and no starts) only up to the end of the tile of that many tokens that
+// the row ends in.
 cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const int32_t* lens, const ts_view4& key,
-                           const ts_view4& value, int dtype, int length, uint32_t* fault, cudaStream_t st);
+                           const ts_view4& value, int dtype, int length, int tile, uint32_t* fault, cudaStream_t st);
 
 // The kernel that attends straight over the pages.  Not supported: a token of a row whose line of work passes
 // what one launch counts (2^30 stages of 16 to 64 keys, over all KV heads).

@@ -21,6 +21,7 @@ struct Int4Rows {
   const int32_t* positions;
   int32_t* positions_out;
   const int32_t* lens;
+  int tile;  // of the read-back: tokens past the tile that a row ends in are left alone, 0: none are
   uint32_t* fault;
   bool vec;          // unit channel stride, 16-byte aligned rows
   int page_log2;
@@ -200,12 +201,13 @@ __global__ void kv_gather_int4_kernel(const __grid_constant__ Int4Rows a) {
   wait_for_previous();
   const ts_kv4_cache& c = a.c;
   const int b = blockIdx.x / a.token_blocks, t0 = (blockIdx.x - b * a.token_blocks) * a.tokens;
-  const int t1 = min(a.steps, t0 + a.tokens);
+  int t1 = min(a.steps, t0 + a.tokens);
   const int chunks = c.head_dim / 8, groups = c.head_dim / 32;
   const int items = c.kv_heads * 2 * chunks;
   const int i = blockIdx.y * blockDim.x + threadIdx.x;
   if (i >= items) return;
   const int pos = a.positions ? a.positions[b] : 0, len = a.lens ? a.lens[b] : INT32_MAX;
+  if (a.tile > 0) t1 = min(t1, ceil_div(min(max(len, 0), a.steps), a.tile) * a.tile);
   const int chunk = i % chunks, kind = i / chunks & 1, h = i / (2 * chunks);
   const int g = chunk / 4, w = chunk % 4 * groups + g;
   const int block = int4_block_bytes(c.head_dim, c.page_size), row = c.head_dim / 2;
@@ -277,7 +279,7 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
                            int64_t position, const int32_t* positions, int32_t* positions_out, uint32_t* fault,
                            cudaStream_t st) {
   const int size = dtype == TS_F32 ? 4 : 2;
-  Int4Rows a{c, key, value, steps, position, positions, positions_out, nullptr, fault,
+  Int4Rows a{c, key, value, steps, position, positions, positions_out, nullptr, 0, fault,
              rows_vec(key, size) && rows_vec(value, size)};
   dim3 grid;
   int threads;
@@ -291,10 +293,10 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
 }
 
 cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const int32_t* lens, const ts_view4& key,
-                           const ts_view4& value, int dtype, int length, uint32_t* fault, cudaStream_t st) {
+                           const ts_view4& value, int dtype, int length, int tile, uint32_t* fault, cudaStream_t st) {
   if (length == 0) return cudaSuccess;
   const int size = dtype == TS_F32 ? 4 : 2;
-  Int4Rows a{c, key, value, length, 0, starts, nullptr, lens, fault, rows_vec(key, size) && rows_vec(value, size)};
+  Int4Rows a{c, key, value, length, 0, starts, nullptr, lens, tile, fault, rows_vec(key, size) && rows_vec(value, size)};
   dim3 grid;
   int threads;
   if (!rows_grid(a, grid, threads)) return cudaErrorInvalidValue;

@@ -6,6 +6,8 @@
 #include "dropout.cuh"
 
 namespace tsa {
+// Keys of a tile: of a row that ends inside one (kv_lens) the rest of its keys and values is read, and must be finite.
+constexpr int kTcKeyTile = 128;
 // True when the tensor-core kernel takes this problem.
 bool tc_fwd_supported(const ts_attn_params& p);
 // `drop` set: attention dropout on P before P.V (the generic kernels' mask).

@@ -40,3 +40,47 @@ def test_a_line_too_long_for_one_token_is_refused(monkeypatch):
     with pytest.raises(_lib.EngineError) as error:
         engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=32)
     assert error.value.status == _lib.ERR_UNSUPPORTED
+
+
+def test_the_prefill_route_asks_for_no_more_than_the_pool(monkeypatch):
+    """64 rows, one of which may hold 131072 tokens: dequantised whole, the batch would take 34 GB."""
+    pool = engine.int4_pool(600, 8, 128, page_size=64)
+    table = torch.full((64, 2048), -1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(64, 32, 64, 128, device="cuda", dtype=torch.bfloat16)
+    args = (q, pool, table, torch.full((64,), 500, dtype=torch.int32, device="cuda"))
+    kw = dict(page_size=64, max_len=131072)
+    assert engine.attention_int4_path(*args, **kw) == "decode"  # the padding would cost more than it saves
+    assert engine.attention_int4_workspace_bytes(*args, **kw) < 1 << 28
+    monkeypatch.setenv("TS_INT4_KERNEL", "prefill")
+    assert engine.attention_int4_path(*args, **kw) == "tcgen05"
+    assert engine.attention_int4_workspace_bytes(*args, **kw) <= max(1 << 30, pool.numel())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("q_len", [40, 200])
+@pytest.mark.parametrize("dim, bound, parts", [(128, 1 << 20, "rows"), (64, 1 << 22, "heads")])
+def test_the_prefill_route_in_parts(dtype, q_len, dim, bound, parts, monkeypatch):
+    """Rows or KV heads one after the other in a workspace that holds NaN where nothing of a row is due."""
+    lens = [300, 40, 0, 129]
+    c = Cache(lens, 2, dim, 64, seed=q_len)
+    keys, values = c.fill(dtype)
+    table = torch.full((4, bound // 64), -1, dtype=torch.int32, device="cuda")
+    table[:, : c.table.shape[1]] = c.table
+    q = torch.from_numpy(np.random.default_rng(0).standard_normal((4, q_len, 6, dim))).to("cuda", torch_dtype(dtype))
+    q = q.permute(0, 2, 1, 3)
+    monkeypatch.setenv("TS_INT4_KERNEL", "prefill")
+    args, kw = (q, c.pool, table, c.kv_lens), dict(page_size=64, max_len=bound)
+    need = engine.attention_int4_workspace_bytes(*args, **kw)
+    assert need == {"rows": 2, "heads": 1}[parts] * 4 * bound * dim
+    workspace = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    out, lse = engine.attention_int4(*args, **kw, need_lse=True, workspace=workspace)
+    engine.check_device_status()
+    short = dict(page_size=64, max_len=300)
+    whole, whole_lse = engine.attention_int4(q, c.pool, c.table, c.kv_lens, **short, need_lse=True)
+    assert torch.equal(out, whole) and torch.equal(lse, whole_lse)
+    ref, ref_lse, spread = oracle.attention_int4(to_np(q).astype(np.float64), keys, values, lens)
+    unit = {"bfloat16": 2.0**-8, "float16": 2.0**-11}[dtype]
+    # the bounds of test_gpu_int4_cache for the prefill kernel
+    top = float(np.abs(ref_lse[np.isfinite(ref_lse)]).max()) + 10
+    bound = unit * np.abs(ref) + (unit + 2.0**-13 + 2.0**-19 * (1 + top) + 300 * 2.0**-27) * spread + 1e-7
+    assert (np.abs(to_np(out).astype(np.float64) - ref) <= bound).all()
