@@ -614,6 +614,11 @@ __device__ __forceinline__ void int4_store(const Int4Attn& a, Int4State<T, DG, N
     }
 }
 
+// Shared memory of the warps' barriers.
+__host__ __device__ constexpr int int4_barrier_bytes(int warps, int stages) {
+  return (warps * stages * (int)sizeof(uint64_t) + 127) / 128 * 128;
+}
+
 // T: type of q and o.  DG = D / 32.  NT: tiles of 8 query columns a warp holds, 1 to 3.
 //
 // The work is a line of stages of KT tokens, ordered by (row, KV head, column block, key); rows differ in
@@ -633,12 +638,14 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
 
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* ring = smem + warp * (kStages * kStageBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes) + warp * kStages;
-  static_assert(kStages * sizeof(uint64_t) == 16, "");
+  // The barriers lie ahead of what the merge overlays: their words may hold nothing else while the block runs.
+  constexpr int kBarriers = int4_barrier_bytes(kWarps, kStages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem) + warp * kStages;
+  unsigned char* rings = smem + kBarriers;
+  unsigned char* ring = rings + warp * (kStages * kStageBytes);
   using State = Int4State<T, DG, NT, kTwin>;
   constexpr int kQueryBytes = State::kQueriesShared ? State::QP * NT * DG * 512 : 0;
-  unsigned char* queries = smem + kWarps * kStages * kStageBytes + kWarps * 16;
+  unsigned char* queries = rings + kWarps * kStages * kStageBytes;
   int* first = reinterpret_cast<int*>(queries + kWarps * kQueryBytes);
   const int pairs = a.p.kv_heads * a.col_blocks;
 
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMinBlocks) attn_int4_kernel(cons
 
   // Merge through shared memory, over the rings: warp w's columns behind those of the warps before it.
   constexpr int kCols = NT * 8, kPad = D + 4, NW = State::NW;
-  float* red = reinterpret_cast<float*>(smem);
+  float* red = reinterpret_cast<float*>(rings);
   float2* ml = reinterpret_cast<float2*>(red + kWarps * kCols * kPad);
   const int g = lane >> 2, t = lane & 3;
   const int hk = home.pair / a.col_blocks, col0 = (home.pair - hk * a.col_blocks) * NT * 8;

@@ -11,8 +11,9 @@ template <typename T, int DG, int NT, bool kTwin, int KT, int kWarps, int kMinBl
 static cudaError_t int4_run(const Int4Attn& a, int blocks, cudaStream_t st) {
   constexpr int D = DG * 32;
   constexpr size_t queries = NT > 1 ? (sizeof(T) == 4 ? 2 : 1) * NT * DG * 512 : 0;
-  constexpr size_t ring = (size_t)kWarps * (kInt4Stages * (2 * KT * (D / 2 + D / 16) + sizeof(uint64_t)) + queries);
-  constexpr size_t merge = (size_t)kWarps * NT * 8 * (D + 4 + 2) * sizeof(float);
+  constexpr size_t barriers = int4_barrier_bytes(kWarps, kInt4Stages);
+  constexpr size_t ring = barriers + (size_t)kWarps * (kInt4Stages * 2 * KT * (D / 2 + D / 16) + queries);
+  constexpr size_t merge = barriers + (size_t)kWarps * NT * 8 * (D + 4 + 2) * sizeof(float);
   constexpr size_t most = ring + (size_t)2 * (kInt4MaxRows + 1) * sizeof(int);
   const size_t need = ring + (a.by_pair ? 0 : (size_t)2 * (a.p.batch + 1) * sizeof(int));
   const size_t smem = need > merge ? need : merge;

@@ -84,3 +84,19 @@ def test_the_prefill_route_in_parts(dtype, q_len, dim, bound, parts, monkeypatch
     top = float(np.abs(ref_lse[np.isfinite(ref_lse)]).max()) + 10
     bound = unit * np.abs(ref) + (unit + 2.0**-13 + 2.0**-19 * (1 + top) + 300 * 2.0**-27) * spread + 1e-7
     assert (np.abs(to_np(out).astype(np.float64) - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("dim, page", [(32, 16), (64, 16), (96, 32), (128, 64)])
+@pytest.mark.parametrize("group", [1, 2, 7])
+def test_several_waves_of_short_rows(dtype, dim, page, group):
+    """A block a pair, many blocks an SM one after the other; every call gives the same bits."""
+    lens = np.random.default_rng(group).integers(0, 60, 300)
+    lens[:4] = [0, 60, 17, 1]
+    c = Cache(lens, 4, dim, page, seed=dim)
+    out = check_attention(c, dtype, 4 * group, 1)
+    q = np.random.default_rng(1).standard_normal((300, 1, 4 * group, dim))  # as check_attention draws it
+    q = torch.from_numpy(q).to("cuda", torch_dtype(dtype)).permute(0, 2, 1, 3)
+    for _ in range(20):
+        again, _ = engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=page, max_len=60)
+        assert torch.equal(out, again)
