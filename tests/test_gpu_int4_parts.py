@@ -100,3 +100,36 @@ def test_several_waves_of_short_rows(dtype, dim, page, group):
     for _ in range(20):
         again, _ = engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=page, max_len=60)
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("most, group, q_len", [(40, 2, 1), (90, 2, 1), (90, 3, 4)])
+def test_more_rows_than_a_launch_takes(dtype, most, group, q_len):
+    """1100 rows: the second launch starts at its own lengths, table rows, outputs and LSE (most <= 64: a block a
+    pair, else a shared line)."""
+    lens = np.random.default_rng(most).integers(0, most + 1, 1100)
+    lens[[0, 1023, 1024, 1099]] = [most, 1, most, 2]
+    check_attention(Cache(lens, 1, 32, 16, seed=1), dtype, group, q_len)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("dim", [64, 96, 256])
+@pytest.mark.parametrize("lens, group, q_len", [([37, 5], 1, 1), ([700, 2000, 0], 3, 1), ([700, 90], 3, 7)])
+def test_rows_that_no_wide_access_takes(dtype, dim, lens, group, q_len):
+    """Queries and outputs with a channel stride of two from an odd element on, a strided LSE: the same bits."""
+    c = Cache(lens, 2, dim, 32, seed=dim)
+    c.fill(dtype)
+    rows, heads = len(lens), 2 * group
+    kw = dict(page_size=32, max_len=max(lens), need_lse=True)
+    args = (c.pool, c.table, c.kv_lens)
+    q = torch.randn(rows, heads, q_len, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    q = q.to(torch_dtype(dtype))
+    want, want_lse = engine.attention_int4(q, *args, **kw)
+    wide = torch.zeros(rows, q_len, heads, 2 * dim + 1, device="cuda", dtype=q.dtype)
+    odd = wide[..., 1::2].permute(0, 2, 1, 3)
+    odd.copy_(q)
+    into = torch.full((rows, heads, q_len, 2 * dim + 1), 7.0, device="cuda", dtype=q.dtype)
+    lse = torch.zeros(heads, rows, q_len, 3, device="cuda")[..., 1].permute(1, 0, 2)
+    got, got_lse = engine.attention_int4(odd, *args, out=into[..., 1::2], lse=lse, **kw)
+    engine.check_device_status()
+    assert torch.equal(got, want) and torch.equal(got_lse, want_lse) and (into[..., ::2] == 7).all()
