@@ -216,7 +216,7 @@ __global__ void kv_gather_int4_kernel(const __grid_constant__ Int4Rows a) {
            (int64_t)chunk * 8 * v.stride[3];
   unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + (int64_t)h * block + kind * (block / 2);
   const int scales = c.page_size * row + g * 2, mask = c.page_size - 1;
-  const int live = min(t1, max(t0, len - pos));  // tokens from here on are zeros
+  const int live = (int)i64min(t1, i64max(t0, (int64_t)len - pos));  // tokens from here on are zeros
   for (int t = t0; t < t1; t += kInFlight) {
     uint32_t word[kInFlight];
     float scale[kInFlight];

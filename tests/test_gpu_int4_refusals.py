@@ -8,7 +8,7 @@ from test_gpu_kv_pages import Pages
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from tensorsmith_b200 import engine  # noqa: E402
+from tensorsmith_b200 import _lib, engine  # noqa: E402
 
 
 def test_workspaces_elsewhere_or_scattered():
@@ -49,3 +49,14 @@ def test_tables_whose_rows_overlap():
     one, _ = engine.attention_int4(q, c.pool, c.table, c.kv_lens, page_size=16)
     two, _ = engine.attention_int4(q.expand(2, -1, -1, -1), c.pool, c.table.expand(2, -1), c.kv_lens.repeat(2), page_size=16)
     assert torch.equal(two[0], one[0]) and torch.equal(two[1], one[0])
+
+
+def test_tokens_before_the_first_are_reported():
+    """A read-back from a negative start has no page for its first tokens, with lengths given or without."""
+    c = Cache([20], 1, 64, 16)
+    keys, _ = c.fill("float32")
+    for lens in (None, c.kv_lens):
+        k, _ = engine.kv_gather_int4(c.pool, c.table, 8, page_size=16, dtype=torch.float32, kv_lens=lens,
+                                     starts=torch.tensor([-3], dtype=torch.int32, device="cuda"))
+        assert engine.device_status() == (_lib.ERR_PAGE, 0x301)
+        assert not k[0, :, :3].any() and (k[0, :, 3:].cpu().double().numpy() == keys[0][:, :5]).all()
