@@ -359,7 +359,6 @@ int check_int4_attn(const ts_attn_params* p, const ts_kv4_cache* c) {
   if (!p->q.data || !p->o.data || !p->kv_lens) return TS_ERR_INVALID_ARGUMENT;
   if (!(p->scale == p->scale) || p->scale > 1.0e300 || p->scale < -1.0e300) return TS_ERR_INVALID_ARGUMENT;
   if ((int64_t)p->q_heads / p->kv_heads * p->q_len > 0x40000000) return TS_ERR_UNSUPPORTED;
-  if (!tsa::attn_int4_supported(*p)) return TS_ERR_UNSUPPORTED;
   return TS_OK;
 }
 
@@ -434,6 +433,16 @@ bool int4_prefill(const ts_attn_params& p, const ts_kv4_cache& c) {
   return int4_prefill_faster(p, c);
 }
 
+// The checked problem's route and the workspace it needs.
+int int4_plan(const ts_attn_params* p, const ts_kv4_cache* c, bool* prefill, size_t* bytes) {
+  const int st = check_int4_attn(p, c);
+  if (st != TS_OK) return st;
+  *prefill = int4_prefill(*p, *c);
+  if (*prefill) *bytes = int4_prefill_bytes(*p, *c);
+  else if (!tsa::attn_int4_workspace(*p, bytes)) return TS_ERR_UNSUPPORTED;
+  return TS_OK;
+}
+
 int check_page_pool(const ts_page_pool* p) {
   if (!p || !p->data || p->layers <= 0 || p->pages <= 0 || p->page_bytes <= 0) return TS_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(p->data) % 16 || p->page_bytes % 16 || p->page_stride % 16 ||
@@ -481,26 +490,27 @@ int ts_kv_gather_int4(const ts_kv4_cache* cache, const int32_t* starts, const in
 }
 
 int ts_attn_int4_path(const ts_attn_params* p, const ts_kv4_cache* cache) {
-  const int st = check_int4_attn(p, cache);
-  if (st != TS_OK) return st;
-  return int4_prefill(*p, *cache) ? TS_PATH_TCGEN05 : TS_PATH_DECODE;
+  bool prefill = false;
+  size_t bytes = 0;
+  const int st = int4_plan(p, cache, &prefill, &bytes);
+  return st != TS_OK ? st : prefill ? TS_PATH_TCGEN05 : TS_PATH_DECODE;
 }
 
 size_t ts_attn_int4_workspace_size(const ts_attn_params* p, const ts_kv4_cache* cache) {
-  if (check_int4_attn(p, cache) != TS_OK) return 0;
-  return int4_prefill(*p, *cache) ? int4_prefill_bytes(*p, *cache) : tsa::attn_int4_workspace(*p, *cache);
+  bool prefill = false;
+  size_t bytes = 0;
+  return int4_plan(p, cache, &prefill, &bytes) == TS_OK ? bytes : 0;
 }
 
 int ts_attn_int4(const ts_attn_params* p, const ts_kv4_cache* cache, void* workspace, size_t workspace_bytes,
                  void* stream) {
-  const int st = check_int4_attn(p, cache);
+  bool prefill = false;
+  size_t need = 0;
+  const int st = int4_plan(p, cache, &prefill, &need);
   if (st != TS_OK) return st;
-  const bool prefill = int4_prefill(*p, *cache);
-  const size_t need = prefill ? int4_prefill_bytes(*p, *cache) : tsa::attn_int4_workspace(*p, *cache);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return TS_ERR_WORKSPACE;
-  if (!prefill)
-    return from_cuda(tsa::attn_int4_forward(*p, *cache, workspace, workspace_bytes, fault_ptr(), as_stream(stream)));
+  if (!prefill) return from_cuda(tsa::attn_int4_forward(*p, *cache, workspace, fault_ptr(), as_stream(stream)));
   const Int4Chunk chunk = int4_chunk(*p, *cache);
   for (int row = 0; row < p->batch; row += chunk.rows)  // one after the other on the stream, in the same workspace
     for (int head = 0; head < p->kv_heads; head += chunk.heads) {

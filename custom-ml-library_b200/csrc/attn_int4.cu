@@ -47,6 +47,7 @@ void set_tokens(const Int4Shape& shape, int tokens, Int4Attn& a) {
 int plan(const ts_attn_params& p, Int4Attn& a, Int4Shape& shape, Part& part) {
   shape = int4_shape(p);
   part = part_of(p, shape);
+  if (part.tokens <= 0) return 0;
   a.group = p.q_heads / p.kv_heads;
   set_tokens(shape, part.tokens, a);
   a.slot_cols = a.cols < shape.nt * 8 ? a.cols : shape.nt * 8;
@@ -86,24 +87,23 @@ Int4Shape int4_shape(const ts_attn_params& p) {
   return {1, 64, 4, 3, false, twin};
 }
 
-bool attn_int4_supported(const ts_attn_params& p) { return part_of(p, int4_shape(p)).tokens > 0; }
-
-size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache&) {
+bool attn_int4_workspace(const ts_attn_params& p, size_t* bytes) {
   Int4Attn a;
   Int4Shape shape;
   Part part;
   plan(p, a, shape, part);
-  if (a.by_pair) return 0;
-  return partial_bytes(a, shape, p.head_dim) + (size_t)2 * (part.rows + 1) * sizeof(int32_t);
+  if (part.tokens <= 0) return false;
+  *bytes = a.by_pair ? 0 : partial_bytes(a, shape, p.head_dim) + (size_t)2 * (part.rows + 1) * sizeof(int32_t);
+  return true;
 }
 
-cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
-                              uint32_t* fault, cudaStream_t st) {
+cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, uint32_t* fault,
+                              cudaStream_t st) {
   Int4Attn a;
   Int4Shape shape;
   Part each;
   int blocks = plan(p, a, shape, each);
-  if (ws_bytes < attn_int4_workspace(p, c)) return cudaErrorInvalidValue;
+  if (each.tokens <= 0) return cudaErrorInvalidValue;
   a.p = p;
   a.c = c;
   a.page_log2 = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : 6;

@@ -55,12 +55,11 @@ cudaError_t kv_append_int4(const ts_view4& key, const ts_view4& value, int dtype
 cudaError_t kv_gather_int4(const ts_kv4_cache& c, const int32_t* starts, const int32_t* lens, const ts_view4& key,
                            const ts_view4& value, int dtype, int length, int tile, uint32_t* fault, cudaStream_t st);
 
-// The kernel that attends straight over the pages.  Not supported: a token of a row whose line of work passes
-// what one launch counts (2^30 stages of 16 to 64 keys, over all KV heads).
-bool attn_int4_supported(const ts_attn_params& p);
-size_t attn_int4_workspace(const ts_attn_params& p, const ts_kv4_cache& c);
-cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, size_t ws_bytes,
-                              uint32_t* fault, cudaStream_t st);
+// The kernel that attends straight over the pages.  Its workspace; false where it takes not even one token of one
+// row, whose line of work would pass what a launch counts (2^30 stages of 16 to 64 keys, over all KV heads).
+bool attn_int4_workspace(const ts_attn_params& p, size_t* bytes);
+cudaError_t attn_int4_forward(const ts_attn_params& p, const ts_kv4_cache& c, void* ws, uint32_t* fault,
+                              cudaStream_t st);
 
 cudaError_t kv_pages_copy(const ts_page_pool& src, const ts_page_pool& dst, const int32_t* from, const int32_t* to,
                           int count, cudaStream_t st);
