@@ -60,6 +60,12 @@ __device__ __forceinline__ void store8(T* dst, int64_t stride, bool vec, const R
   }
 }
 
+__device__ __forceinline__ int sub_sat(int a, int b) {
+  int r;
+  asm("sub.sat.s32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // The larger, or NaN if either is one.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -216,7 +222,7 @@ __global__ void kv_gather_int4_kernel(const __grid_constant__ Int4Rows a) {
            (int64_t)chunk * 8 * v.stride[3];
   unsigned char* base = reinterpret_cast<unsigned char*>(c.pool) + (int64_t)h * block + kind * (block / 2);
   const int scales = c.page_size * row + g * 2, mask = c.page_size - 1;
-  const int live = (int)i64min(t1, i64max(t0, (int64_t)len - pos));  // tokens from here on are zeros
+  const int live = min(t1, max(t0, sub_sat(len, pos)));  // tokens from here on are zeros
   for (int t = t0; t < t1; t += kInFlight) {
     uint32_t word[kInFlight];
     float scale[kInFlight];
