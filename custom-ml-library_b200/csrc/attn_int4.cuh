@@ -21,14 +21,16 @@
 //   V       needs its scale on the operand: the nibble in the mantissa of a power of two, 0x6400 | nibble = 1024 +
 //           nibble or 0x5400 | nibble << 4 = 64 + nibble, then a subtraction and a product, both exact.  (As one
 //           multiply-add, (64 + nibble) scale - 72 scale, the last term would leave fp16 from a scale of 910 on)
-//   q       times a power of two that puts its largest element in [2^14, 2^15): exact for bf16 and
-//           fp16 rows except elements 2^-38 below the largest; fp32 rows as hi + lo (22 bits)
+//   q       times a power of two that puts its largest element in [2^14, 2^15), rounded to fp16: by at most 2^-39
+//           of that element, 2^-35 in the odd channels of the masked form.  So half types keep all their bits down
+//           to 2^-31 (bf16) and 2^-28 (fp16) of the largest, odd channels to 2^-27 and 2^-24; fp32 rows as hi + lo
+//           (22 bits)
 //   p       times 2^7 of a reference within 2^8 of the maximum, fp16; for fp16 and fp32 outputs hi + lo,
 //           since the 2^-12 of one fp16 part is as large as the output's own rounding there
-// Measured, 64 rows x 32 heads of 1024-8192 keys, D = 128 (1.36 GB): 251 us in fp16, 244 in bf16, 84 % and 86 % of
-// the copy rate.  Issue bounds it: 288 warp instructions a tile of 16 keys at 60 % of the issue slots, no pipe above
-// 51 %; the copies alone take 212 us, the arithmetic alone about 228.  Twelve warps an SM fit (168 registers); 16 of
-// 128 spill, and lost what they hid (308 against 253 us).
+// Measured, 64 rows x 32 heads of 1024-8192 keys, D = 128 (1.36 GB): 252 us in fp16, 246 in bf16, 313 in fp32: 84, 86
+// and 67 % of the copy rate.  Issue bounds it: 299 warp instructions a tile of 16 keys at 62 % of the issue slots, no
+// pipe above 51 %; the copies alone take 212 us, the arithmetic alone took about 228 with 11 instructions fewer.
+// Twelve warps an SM fit (168 registers); 16 of 128 spill, and lost what they hid (308 against 253 us).
 // The rows of the K tile are permuted within 8 tokens so that the P^T fragment (one transposing
 // register move of S^T's) meets V rows whose shared-memory reads do not collide, see token_of_row.
 #pragma once

@@ -1,8 +1,8 @@
 // Quantising append into the pages of a 4-bit KV cache, and the read-back of its values.
 // Both move each value once: 16 bits in and 4.5 out (the append), 4.5 in and 16 out (the gather),
-// so HBM should bound them: 8 rows x 2047 tokens, 8 heads, D = 128, bf16, move 86 MB each, 13 us.  Issue does: the
-// append takes 28 us there (131 instructions a stored word, 64 % of the issue slots), the read-back 21 (100, 68 %).
-// One token of 64 rows takes the launch, 2 us.
+// so HBM should bound them: 8 rows x 2047 tokens, 8 heads, D = 128, bf16, move 86 MB each, 13 us.  Instructions do: the
+// append takes 27 us there (131 a stored word, 63 % of the issue slots; fp16 26, fp32 with its divisions 44 for 153 MB),
+// the read-back 19.5 (100 and 68 %; fp32 40).  One token of 64 rows takes the launch, 2.4 us.
 //
 // One thread owns a stored word (8 channels of K or V of one head) and walks over a block's tokens, four of
 // them in flight: 64 bytes a thread for half types, which is what covers the memory latency.  The four

@@ -6,6 +6,8 @@
 // counters = {free pages, a page number below which no page is free, error bits, unused}.
 // Every result is a function of the inputs alone: integer sums commute, pages are handed out
 // lowest first in the order of (row, slot), and of the writers that share a page the last keeps it.
+// The one exception is counters[1] after a fork: a page that passes from row to row may be counted as
+// free for a moment, so how far the bound lies below the lowest free page depends on the order of blocks.
 //
 // The pages themselves are opaque bytes.  Copies are bound by HBM (each byte read and written once): 2.65 GB of a
 // compaction's pages move in 442 us, 93 % of the measured copy rate.  The table work is a chain of small launches,

@@ -593,7 +593,9 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
 
     Row b sees its first ``kv_lens[b]`` tokens; with ``is_causal`` its Tq queries are the last of them
     (a row without a visible key gives zeros and an LSE of -inf).  ``max_len`` bounds ``kv_lens`` (default: what
-    the table can hold); the work is split for it, so pass the real bound where it is known."""
+    the table can hold); the work is split for it, so pass the real bound where it is known.  Chunks of a prompt may
+    run on the prefill kernel (``attention_int4_path``), whose probabilities are rounded to q's type, where the
+    kernel over the pages keeps 11 bits of them for bf16 and 22 for fp16 and fp32."""
     if out is None:
         out = q.new_empty(q.shape)
     if not need_lse:

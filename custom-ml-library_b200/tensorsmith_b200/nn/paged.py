@@ -4,7 +4,8 @@ tensorsmith's cache owns a preallocated block a batch row (src/tensorsmith/nn/ca
 smallest.  Here every layer has a pool of pages in 4 bits, and one page table serves all layers: rows take
 pages as they grow, forked rows (parallel samples, beams) share them until one writes, and freed pages return
 to the pool.  ``layers`` are the per-layer views that ``TransformerLM`` takes in the place of ``KVCache``
-objects; like those they are for inference only.
+objects; like those they are for inference only.  A step appends the same number of tokens to every row, an
+emptied one included; ``engine.kv_pages_reserve`` and ``kv_append_int4`` take rows that step by numbers of their own.
 
 The tables, lengths, reference counts and free-page counters live on the device and are changed by the
 engine's page operations without a host round trip.  The host keeps the row lengths, which decide when a

@@ -334,14 +334,19 @@ TS_ATTN_API size_t ts_attn_int4_workspace_size(const ts_attn_params* params, con
  * with k and v ignored, kv_lens required and kv_len an upper bound of them that
  * the table can hold (kv_len <= slots * page_size); no explicit mask, no fp64.
  * Any number of query tokens: one token a row, a few drafted ones, or a chunk of
- * a prompt whose tokens are already in the cache. */
+ * a prompt whose tokens are already in the cache.  The route decides how the
+ * probabilities enter the product with V: over the pages in fp16 relative to the
+ * row's maximum (two parts, 22 bits, for F16 and F32 outputs), on the prefill route
+ * in q's type, as ts_attn_fwd has them (BF16: 8 bits; F16: 11 bits, and 2^-25 of the
+ * largest at the least). */
 TS_ATTN_API int ts_attn_int4(const ts_attn_params* params, const ts_kv4_cache* cache, void* workspace,
                              size_t workspace_bytes, void* stream);
 
 /* ---- Pages of a paged cache (any storage: a page is opaque bytes) ----
  * refs[p] counts the table entries that hold page p (and pins a caller adds); a
  * page with refs 0 is free.  counters is int32 [4] on the device: {free pages, a
- * page number below which none is free (0 is always right), error bits, unused};
+ * page number below which none is free (0 is always right; after a fork the engine's
+ * may vary from run to run), error bits, unused};
  * error bits, set and never cleared by the engine: 1 not enough free pages, 2 an
  * index or page out of range was skipped, 4 a row would need more slots than the
  * table has.  A reserve that sets 1 or 4 changes nothing.  The rows of a table
