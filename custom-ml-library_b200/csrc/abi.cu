@@ -12,10 +12,12 @@
 #include "int8.cuh"
 #include "kv_cache.cuh"
 #include "rope.cuh"
+#include "rows.cuh"
 #include "simt.cuh"
 #include "symbols.cuh"
 #include "tc_bwd.cuh"
 #include "tc_fwd.cuh"
+#include "token_logprobs.cuh"
 
 namespace {
 
@@ -586,6 +588,240 @@ int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* table, int64_t 
     return TS_ERR_WORKSPACE;
   return from_cuda(tsa::kv_pages_compact(*pool, table, table_out, rows, slots, table_stride, table_out_stride, refs,
                                          refs_out, counters, workspace, as_stream(stream)));
+}
+
+}  // extern "C"
+
+namespace {
+
+// One of the four instantiations of a family of kernels.
+template <typename F32, typename F64, typename F16, typename BF16, typename... A>
+cudaError_t by_dtype(int dtype, F32 f32, F64 f64, F16 f16, BF16 bf16, A&&... a) {
+  switch (dtype) {
+    case TS_F32: return f32(a...);
+    case TS_F64: return f64(a...);
+    case TS_F16: return f16(a...);
+    case TS_BF16: return bf16(a...);
+  }
+  return cudaErrorInvalidValue;
+}
+
+constexpr int kGridMax = 65535;  // of a grid's second and third dimension
+
+int check_window(const ts_attn_params* p, const ts_window* w) {
+  const int st = check_params(p);
+  if (st != TS_OK) return st;
+  if (!w || w->window < 1 || w->sinks < 0 || !p->is_causal) return TS_ERR_INVALID_ARGUMENT;
+  if (p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
+  if (p->q_heads > kGridMax || p->batch > kGridMax || (int64_t)p->kv_heads * p->batch > 0x7fffffff ||
+      p->kv_len > 16 * kGridMax)
+    return TS_ERR_UNSUPPORTED;
+  return TS_OK;
+}
+tsa::WindowArgs window_args(const ts_window* w) {
+  tsa::WindowArgs a;
+  a.window = w->window;
+  a.sinks = w->sinks;
+  return a;
+}
+
+int check_window_bwd(const ts_attn_bwd_params* bp, const ts_window* w) {
+  if (!bp) return TS_ERR_INVALID_ARGUMENT;
+  const int st = check_window(&bp->fwd, w);
+  if (st != TS_OK) return st;
+  if (!bp->fwd.lse || !bp->dout.data || !bp->dq.data || !bp->dk.data || !bp->dv.data) return TS_ERR_INVALID_ARGUMENT;
+  if ((int64_t)bp->fwd.batch * bp->fwd.q_heads > 0x7fffffff ||
+      (int64_t)bp->fwd.batch * bp->fwd.q_heads * bp->fwd.q_len > (int64_t)1 << 33)
+    return TS_ERR_UNSUPPORTED;
+  return TS_OK;
+}
+size_t window_bwd_workspace(const ts_attn_bwd_params& bp) {
+  return tsa::tc_bwd_window_supported(bp) ? tsa::tc_bwd_workspace(bp) : tsa::simt_backward_workspace(bp);
+}
+
+int check_tree(const ts_attn_params* p, const ts_tree* t) {
+  if (!t || !p || !p->kv_lens) return TS_ERR_INVALID_ARGUMENT;
+  ts_attn_params q = *p;  // the rule is the tree's, whatever the causal fields hold
+  q.causal_offset = 0;
+  const int st = check_params(&q);
+  if (st != TS_OK) return st;
+  if (t->window < 0 || t->sinks < 0) return TS_ERR_INVALID_ARGUMENT;
+  if (p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
+  if (t->parents && p->q_len > TS_TREE_MAX_NODES) return TS_ERR_UNSUPPORTED;
+  if ((int64_t)p->q_heads / p->kv_heads * p->q_len > 0x40000000 ||
+      (int64_t)p->batch * p->q_heads * p->q_len > 0x40000000)
+    return TS_ERR_UNSUPPORTED;
+  return TS_OK;
+}
+cudaError_t rows_tree(const ts_attn_params& p, tsa::TreeArgs* a, size_t* bytes, void* ws, cudaStream_t st) {
+  return by_dtype(p.dtype, tsa::rows_tree_f32, tsa::rows_tree_f64, tsa::rows_tree_f16, tsa::rows_tree_bf16, p, a,
+                  bytes, ws, st);
+}
+size_t tree_workspace(const ts_attn_params& p) {
+  if (tsa::tc_tree_supported(p)) return tsa::tc_tree_workspace(p);
+  size_t bytes = 0;
+  if (p.dtype != TS_F64) (void)rows_tree(p, nullptr, &bytes, nullptr, nullptr);
+  return bytes;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ts_attn_window_path(const ts_attn_params* p, const ts_window* w) {
+  const int st = check_window(p, w);
+  if (st != TS_OK) return st;
+  return tsa::tc_window_supported(*p) ? TS_PATH_TCGEN05 : TS_PATH_SIMT;
+}
+
+int ts_attn_fwd_window(const ts_attn_params* p, const ts_window* w, void* stream) {
+  const int st = check_window(p, w);
+  if (st != TS_OK) return st;
+  const tsa::WindowArgs win = window_args(w);
+  if (tsa::tc_window_supported(*p)) return from_cuda(tsa::tc_forward_window(*p, win, fault_ptr(), as_stream(stream)));
+  const tsa::RowsWindow a = {*p, win};
+  return from_cuda(by_dtype(p->dtype, tsa::rows_window_fwd_f32, tsa::rows_window_fwd_f64, tsa::rows_window_fwd_f16,
+                            tsa::rows_window_fwd_bf16, a, as_stream(stream)));
+}
+
+size_t ts_attn_bwd_window_workspace_size(const ts_attn_bwd_params* bp, const ts_window* w) {
+  return check_window_bwd(bp, w) == TS_OK ? window_bwd_workspace(*bp) : 0;
+}
+
+int ts_attn_bwd_window(const ts_attn_bwd_params* bp, const ts_window* w, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  const int st = check_window_bwd(bp, w);
+  if (st != TS_OK) return st;
+  if (!workspace || workspace_bytes < window_bwd_workspace(*bp) || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return TS_ERR_WORKSPACE;
+  const tsa::WindowArgs win = window_args(w);
+  if (tsa::tc_bwd_window_supported(*bp))
+    return from_cuda(
+        tsa::tc_backward(*bp, workspace, workspace_bytes, fault_ptr(), as_stream(stream), nullptr, &win));
+  return from_cuda(by_dtype(bp->fwd.dtype, tsa::rows_window_bwd_f32, tsa::rows_window_bwd_f64,
+                            tsa::rows_window_bwd_f16, tsa::rows_window_bwd_bf16, *bp, win, workspace,
+                            as_stream(stream)));
+}
+
+int ts_attn_tree_path(const ts_attn_params* p, const ts_tree* t) {
+  const int st = check_tree(p, t);
+  if (st != TS_OK) return st;
+  return tsa::tc_tree_supported(*p) ? TS_PATH_TCGEN05 : TS_PATH_SIMT;
+}
+
+size_t ts_attn_tree_workspace_size(const ts_attn_params* p, const ts_tree* t) {
+  return check_tree(p, t) == TS_OK ? tree_workspace(*p) : 0;
+}
+
+int ts_attn_tree(const ts_attn_params* p, const ts_tree* t, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_tree(p, t);
+  if (st != TS_OK) return st;
+  const size_t need = tree_workspace(*p);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return TS_ERR_WORKSPACE;
+  tsa::WindowArgs win;
+  win.window = t->window;
+  win.sinks = t->sinks;
+  if (tsa::tc_tree_supported(*p))
+    return from_cuda(
+        tsa::tc_tree(*p, t->parents, t->parents_stride, win, workspace, fault_ptr(), as_stream(stream)));
+  tsa::TreeArgs a = {};
+  a.parents = t->parents;
+  a.parents_stride = t->parents_stride;
+  a.win = win;
+  size_t bytes;
+  return from_cuda(rows_tree(*p, &a, &bytes, workspace, as_stream(stream)));
+}
+
+int ts_tree_positions(const int32_t* parents, int64_t parents_stride, const int32_t* lens, int32_t batch,
+                      int32_t nodes, int32_t* positions, void* stream) {
+  if (!parents || !lens || !positions || batch <= 0 || nodes <= 0) return TS_ERR_INVALID_ARGUMENT;
+  return from_cuda(tsa::tree_positions(parents, parents_stride, lens, batch, nodes, positions, as_stream(stream)));
+}
+
+int ts_rope_at(ts_view4 x, ts_view4 y, int32_t dtype, int32_t batch, int32_t heads, int32_t seq, int32_t channels,
+               int32_t rotary_dim, const int32_t* positions, const float* inv_freq, int32_t inverse, void* stream) {
+  if (!dtype_ok(dtype)) return TS_ERR_UNSUPPORTED;
+  if (!x.data || !y.data || !inv_freq || !positions || batch <= 0 || heads <= 0 || seq <= 0 || channels <= 0)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > channels) return TS_ERR_INVALID_ARGUMENT;
+  if (batch > kGridMax) return TS_ERR_UNSUPPORTED;
+  return from_cuda(tsa::rope_apply(x, y, dtype, batch, heads, seq, channels, rotary_dim, 0, positions, inv_freq,
+                                   inverse, as_stream(stream), true));
+}
+
+int ts_kv_keep(const ts_kv_keep_params* p, void* stream) {
+  if (!p || !p->keys || !p->values || !p->base || !p->path || !p->counts) return TS_ERR_INVALID_ARGUMENT;
+  if (!dtype_ok(p->dtype) && p->dtype != TS_I8) return TS_ERR_UNSUPPORTED;
+  if (p->layers <= 0 || p->batch <= 0 || p->heads <= 0 || p->head_dim <= 0 || p->value_dim <= 0 || p->capacity <= 0 ||
+      p->nodes <= 0 || p->key_stride[3] != 1 || p->value_stride[3] != 1)
+    return TS_ERR_INVALID_ARGUMENT;
+  if (p->batch > kGridMax) return TS_ERR_UNSUPPORTED;
+  const int size = p->dtype == TS_F64 ? 8 : p->dtype == TS_F32 ? 4 : p->dtype == TS_I8 ? 1 : 2;
+  tsa::KvKeep a = {};
+  for (int i = 0; i < 3; ++i) {
+    a.stride[0][i] = p->key_stride[i] * size;
+    a.stride[1][i] = p->value_stride[i] * size;
+  }
+  a.row_bytes[0] = p->head_dim * size;
+  a.row_bytes[1] = p->value_dim * size;
+  a.batch = p->batch;
+  a.heads = p->heads;
+  a.nodes = p->nodes;
+  a.capacity = p->capacity;
+  a.base = p->base;
+  a.path = p->path;
+  a.counts = p->counts;
+  a.path_stride = p->path_stride;
+  for (int l = 0; l < p->layers; ++l)
+    if (!p->keys[l] || !p->values[l]) return TS_ERR_INVALID_ARGUMENT;
+  for (int l0 = 0; l0 < p->layers; l0 += tsa::kKeepTensors / 2) {
+    a.tensors = 0;
+    for (int l = l0; l < p->layers && a.tensors < tsa::kKeepTensors; ++l) {
+      a.data[a.tensors++] = p->keys[l];
+      a.data[a.tensors++] = p->values[l];
+    }
+    const cudaError_t e = tsa::kv_keep(a, as_stream(stream));
+    if (e != cudaSuccess) return from_cuda(e);
+  }
+  return TS_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_logprobs(const ts_token_logprobs* p) {
+  if (!p || !p->logits || p->rows <= 0 || p->vocab <= 0 || p->top < 0 || p->top > p->vocab)
+    return TS_ERR_INVALID_ARGUMENT;
+  if ((p->dtype != TS_F32 && p->dtype != TS_F16 && p->dtype != TS_BF16) || p->top > TS_TOP_TOKENS_MAX)
+    return TS_ERR_UNSUPPORTED;
+  const int size = p->dtype == TS_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(p->logits) % size || (p->rows > 1 && p->stride < 0)) return TS_ERR_INVALID_ARGUMENT;
+  return TS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ts_token_logprobs_fwd(const ts_token_logprobs* p, void* stream) {
+  const int st = check_logprobs(p);
+  if (st != TS_OK) return st;
+  if ((p->logprob && !p->targets) || (p->top && (!p->top_logprobs || !p->top_indices))) return TS_ERR_INVALID_ARGUMENT;
+  return from_cuda(tsa::token_logprobs(*p, as_stream(stream)));
+}
+
+int ts_token_logprobs_bwd(const ts_token_logprobs* p, const float* grad_logprob, const float* grad_entropy,
+                          const float* grad_top, void* grad_logits, int64_t grad_stride, void* stream) {
+  const int st = check_logprobs(p);
+  if (st != TS_OK) return st;
+  if (!p->targets || !p->norm || !p->entropy || !grad_logits || grad_logits == p->logits ||
+      (grad_top && p->top && !p->top_indices) || (p->rows > 1 && grad_stride < p->vocab))
+    return TS_ERR_INVALID_ARGUMENT;
+  if ((int64_t)p->rows * (p->vocab / 4096 + 1) > 0x7fffffff) return TS_ERR_UNSUPPORTED;
+  return from_cuda(tsa::token_logprobs_bwd(*p, grad_logprob, grad_entropy, grad_top, grad_logits, grad_stride,
+                                           as_stream(stream)));
 }
 
 int ts_attn_device_status(void* stream, uint32_t* info) {

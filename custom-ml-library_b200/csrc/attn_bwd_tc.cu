@@ -43,7 +43,9 @@
 #include "ptx.cuh"
 #include "simt.cuh"
 #include "tc_bwd.cuh"
+#include "tc_fwd.cuh"
 #include "tc_util.cuh"
+#include "window.cuh"
 
 namespace tsa {
 
@@ -92,11 +94,12 @@ struct TcBwdArgs {
   int n_k_tiles;
   uint32_t* fault;
   DropoutArgs drop;  // used by the kDrop instantiation only
+  WindowArgs win;    // used by the kWin instantiation only
 };
 
 }  // namespace
 
-template <int D, bool kBF16, bool kDrop>
+template <int D, bool kBF16, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(512, 1)
     tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -116,7 +119,10 @@ __global__ void __launch_bounds__(512, 1)
   float* sStat = reinterpret_cast<float*>(smem + C::kOffStat);  // [buf][lse2 | delta][64]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kt = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  // kWin: every (head, row) of key tile 0 first, as a tile with sinks is seen by all the queries behind it.
+  const int kt = kWin ? blockIdx.y : blockIdx.x;
+  const int hk = kWin ? (int)blockIdx.x % p.kv_heads : (int)blockIdx.y;
+  const int b = kWin ? (int)blockIdx.x / p.kv_heads : (int)blockIdx.z;
   const int rep = p.q_heads / p.kv_heads;
   const int k0 = kt * kBN;
 
@@ -129,7 +135,13 @@ __global__ void __launch_bounds__(512, 1)
   const int n_qt_all = ceil_div(p.q_len, kBM);
   int qt_start = 0;
   if (p.is_causal) qt_start = (int)(i64max(0, (int64_t)k0 - offset) / kBM);
-  const int n_qt = k0 < kv_end ? max(0, n_qt_all - qt_start) : 0;
+  int qt_end = n_qt_all;
+  if (kWin && k0 >= args.win.sinks) {
+    // The last query that sees the tile's last key.
+    const int64_t last = (int64_t)k0 + kBN - 1 + args.win.window - 1 - offset;
+    qt_end = last < 0 ? 0 : (int)i64min(n_qt_all, last / kBM + 1);
+  }
+  const int n_qt = k0 < kv_end ? max(0, qt_end - qt_start) : 0;
   const int n_it = rep * n_qt;
   const bool dead = fault_set(args.fault);
 
@@ -278,6 +290,8 @@ __global__ void __launch_bounds__(512, 1)
         // i + offset >= key), none when the key is past the row's end.
         const int64_t cm = p.is_causal ? (int64_t)key - offset - q0 : 0;
         const int c_min = key_ok ? (int)i64max(0, i64min(kBM, cm)) : kBM;
+        // kWin: and col < c_max, where the window has left the key behind.
+        const int c_max = !kWin || key < args.win.sinks ? kBM : (int)i64max(0, i64min(kBM, cm + args.win.window));
         {
           uint32_t rs[32], rd[32];
           ptx::tmem_ld32(t_row + C::kColS + 32 * half, rs);
@@ -310,7 +324,7 @@ __global__ void __launch_bounds__(512, 1)
           }
           const float dinv = kDrop ? args.drop.inv_keep_f : 1.f;
           // Columns below c_min are masked; warp-uniform fast path when none of this half is.
-          const bool all_vis = __all_sync(0xffffffffu, c_min <= 32 * half);
+          const bool all_vis = __all_sync(0xffffffffu, c_min <= 32 * half && (!kWin || c_max >= 32 * half + 32));
           const uint64_t sl2x2 = ptx::f2pack(sl2, sl2), scx2 = ptx::f2pack(scale, scale);
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
@@ -322,8 +336,8 @@ __global__ void __launch_bounds__(512, 1)
             float p0 = ptx::ex2(x0), p1 = ptx::ex2(x1);
             if (!all_vis) {
               const int col = 32 * half + c;
-              p0 = col >= c_min ? p0 : 0.f;
-              p1 = col + 1 >= c_min ? p1 : 0.f;
+              p0 = col >= c_min && (!kWin || col < c_max) ? p0 : 0.f;
+              p1 = col + 1 >= c_min && (!kWin || col + 1 < c_max) ? p1 : 0.f;
             }
             const uint64_t p2 = ptx::f2pack(p0, p1);
             uint64_t t2;
@@ -402,7 +416,7 @@ __global__ void __launch_bounds__(512, 1)
             else
               v = make_uint4(ptx::pack_f16(f[0], f[1]), ptx::pack_f16(f[2], f[3]), ptx::pack_f16(f[4], f[5]),
                              ptx::pack_f16(f[6], f[7]));
-            *reinterpret_cast<uint4*>(out + 32 * c + e) = v;
+            if (!kWin || 32 * c + e < p.head_dim) *reinterpret_cast<uint4*>(out + 32 * c + e) = v;
           }
         }
       }
@@ -473,7 +487,7 @@ __global__ void __launch_bounds__(512, 1)
 // shared memory so both the read and the write are coalesced.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dq_convert_kernel(const float* __restrict__ acc, ts_view4 dq, int heads,
-                                                         int len, int n_tiles) {
+                                                         int len, int n_tiles, int dim = D) {
   __shared__ float tile[kBM][D + 1];
   const int bh = blockIdx.x, t = blockIdx.y;
   const float4* src = reinterpret_cast<const float4*>(acc + ((int64_t)bh * n_tiles + t) * (D * kBM));
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(256) dq_convert_kernel(const float* __restrict
   T* out = reinterpret_cast<T*>(dq.data) + (int64_t)b * dq.stride[0] + (int64_t)h * dq.stride[1];
   for (int idx = threadIdx.x; idx < kBM * D; idx += blockDim.x) {
     const int r = idx / D, d = idx % D, i = t * kBM + r;
-    if (i < len) out[(int64_t)i * dq.stride[2] + (int64_t)d * dq.stride[3]] = Elem<T>::from_acc(tile[r][d]);
+    if (i < len && d < dim) out[(int64_t)i * dq.stride[2] + (int64_t)d * dq.stride[3]] = Elem<T>::from_acc(tile[r][d]);
   }
 }
 
@@ -512,15 +526,21 @@ bool tc_bwd_supported(const ts_attn_bwd_params& bp) {
   return encode_fn() != nullptr;
 }
 
+bool tc_bwd_window_supported(const ts_attn_bwd_params& bp) {
+  return tc_window_supported(bp.fwd) && bp.fwd.lse && view_tma_ok(bp.dout) && out_rows_ok(bp.dk) && out_rows_ok(bp.dv);
+}
+
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 static int t_padded(int q_len) { return ceil_div(q_len, kBM) * kBM; }
+
+static int padded_dim(int dim) { return dim <= 64 ? 64 : 128; }
 
 size_t tc_bwd_workspace(const ts_attn_bwd_params& bp) {
   const ts_attn_params& p = bp.fwd;
   const size_t rows = (size_t)p.batch * p.q_heads * t_padded(p.q_len);
   const size_t stats = (size_t)p.batch * p.q_heads * 2 * t_padded(p.q_len);
-  return align256(stats * sizeof(float)) + align256(rows * p.head_dim * sizeof(float));
+  return align256(stats * sizeof(float)) + align256(rows * padded_dim(p.head_dim) * sizeof(float));
 }
 
 // stats[bh][0][i] = -LSE*log2e (-inf for a fully masked row or i >= Tq) and
@@ -561,16 +581,19 @@ __global__ void bwd_stats_kernel(ts_attn_bwd_params bp, float* stats, int t_pad)
 template <int D, bool BF16>
 static cudaError_t launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                               const CUtensorMap& mdo, const TcBwdArgs& a, cudaStream_t st) {
-  auto kern = a.drop.p > 0.f ? tc_bwd_kernel<D, BF16, true> : tc_bwd_kernel<D, BF16, false>;
+  const bool win = a.win.window > 0;
+  auto kern = win              ? tc_bwd_kernel<D, BF16, false, true>
+              : a.drop.p > 0.f ? tc_bwd_kernel<D, BF16, true, false>
+                               : tc_bwd_kernel<D, BF16, false, false>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kern), BwdCfg<D>::kSmem);
   if (e != cudaSuccess) return e;
-  dim3 grid(a.n_k_tiles, a.p.kv_heads, a.p.batch);
+  const dim3 grid = win ? dim3((unsigned)(a.p.kv_heads * a.p.batch), a.n_k_tiles) : dim3(a.n_k_tiles, a.p.kv_heads, a.p.batch);
   kern<<<grid, 512, BwdCfg<D>::kSmem, st>>>(mq, mk, mv, mdo, a);
   return cudaGetLastError();
 }
 
 cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes, uint32_t* fault,
-                        cudaStream_t st, const DropoutArgs* drop) {
+                        cudaStream_t st, const DropoutArgs* drop, const WindowArgs* win) {
   const ts_attn_params& p = bp.fwd;
   if (ws_bytes < tc_bwd_workspace(bp)) return cudaErrorInvalidValue;
   const int t_pad = t_padded(p.q_len);
@@ -594,7 +617,7 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = cudaMemsetAsync(dq_acc, 0, rows * p.head_dim * sizeof(float), st);
+  e = cudaMemsetAsync(dq_acc, 0, rows * padded_dim(p.head_dim) * sizeof(float), st);
   if (e != cudaSuccess) return e;
   TcBwdArgs a;
   a.p = p;
@@ -606,24 +629,25 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
   a.n_k_tiles = ceil_div(p.kv_len, kBN);
   a.fault = fault;
   a.drop = drop ? *drop : DropoutArgs{};
+  a.win = win ? *win : WindowArgs{};
   const bool bf = p.dtype == TS_BF16;
-  if (p.head_dim == 64)
+  if (p.head_dim <= 64)
     e = bf ? launch_bwd<64, true>(mq, mk, mv, mdo, a, st) : launch_bwd<64, false>(mq, mk, mv, mdo, a, st);
   else
     e = bf ? launch_bwd<128, true>(mq, mk, mv, mdo, a, st) : launch_bwd<128, false>(mq, mk, mv, mdo, a, st);
   if (e != cudaSuccess) return e;
   const dim3 cgrid((unsigned)(p.batch * p.q_heads), (unsigned)(t_pad / kBM));
   const int n_tiles = t_pad / kBM;
-  if (p.head_dim == 64) {
+  if (p.head_dim <= 64) {
     if (bf)
-      dq_convert_kernel<__nv_bfloat16, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles);
+      dq_convert_kernel<__nv_bfloat16, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
     else
-      dq_convert_kernel<__half, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles);
+      dq_convert_kernel<__half, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
   } else {
     if (bf)
-      dq_convert_kernel<__nv_bfloat16, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles);
+      dq_convert_kernel<__nv_bfloat16, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
     else
-      dq_convert_kernel<__half, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles);
+      dq_convert_kernel<__half, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
   }
   return cudaGetLastError();
 }

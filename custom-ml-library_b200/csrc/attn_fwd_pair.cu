@@ -26,11 +26,19 @@
 // allocator) runs on 56 registers a thread so that the softmax warpgroups
 // hold a 128-key row of scores, its 64 packed probabilities and the running
 // state in 216 without spilling.  No TMA load uses cluster multicast.
+//
+// kWin: the sliding window with sinks (window.cuh).  The CTA's list of key
+// tiles leaves out those between the sinks and the window of its first row;
+// a tile is masked by the bits of its 128 keys, from the row's two visible
+// ranges, and only where some row of the query tile does not see all of it.
+// Head dimensions that are multiples of 8 below D run on D columns: the
+// tensor maps fill the missing channels with zeros and they are not stored.
 #include <type_traits>
 
 #include "ptx.cuh"
 #include "tc_fwd.cuh"
 #include "tc_util.cuh"
+#include "window.cuh"
 
 namespace tsa {
 
@@ -77,6 +85,7 @@ struct PairArgs {
   int n_units;  // ceil(q_len / 256) per (batch, head)
   uint32_t* fault;
   DropoutArgs drop;  // kDrop instantiation only
+  WindowArgs win;    // kWin instantiation only
 };
 
 // Key tiles visible to query rows [r0, r0 + 128) (0 when the tile is empty).
@@ -92,7 +101,7 @@ __device__ __forceinline__ int visible_tiles(const ts_attn_params& p, int r0, in
 
 }  // namespace
 
-template <int D, bool kBF16, bool kDrop>
+template <int D, bool kBF16, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(384, 1)
     tc_fwd_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, PairArgs args) {
@@ -122,7 +131,13 @@ __global__ void __launch_bounds__(384, 1)
     kv_end = min(kv_end, max(0, p.kv_lens[b]));
     offset = (int64_t)kv_end - p.q_len;
   }
-  const int n_t[2] = {visible_tiles(p, q0, kv_end, offset), visible_tiles(p, q0 + kBM, kv_end, offset)};
+  const WindowTiles wt(args.win, (int64_t)q0 + offset, kv_end, kBN);
+  auto key_tile = [&](int j) { return kWin ? wt.tile(j) : j; };
+  auto tiles_of = [&](int r0) {
+    const int n = visible_tiles(p, r0, kv_end, offset);
+    return kWin ? wt.count(n) : n;
+  };
+  const int n_t[2] = {tiles_of(q0), tiles_of(q0 + kBM)};
   const int n_max = max(n_t[0], n_t[1]);
   const bool dead = fault_set(args.fault);
 
@@ -177,7 +192,7 @@ __global__ void __launch_bounds__(384, 1)
           ptx::mbar_expect_tx(&bars->kv_full[s], C::kTileBytes);
           const CUtensorMap* map = (f & 1) ? &tm_v : &tm_k;
           for (int sl = 0; sl < C::kSlabs; ++sl)
-            ptx::tma_load_4d(slot_addr(f) + sl * kSlabBytes, map, 64 * sl, (f >> 1) * kBN, hk, b,
+            ptx::tma_load_4d(slot_addr(f) + sl * kSlabBytes, map, 64 * sl, key_tile(f >> 1) * kBN, hk, b,
                              &bars->kv_full[s]);
           issued = f + 1;
         }
@@ -274,11 +289,24 @@ __global__ void __launch_bounds__(384, 1)
       for (int c = 0; c < kBN / 32; ++c)
         ptx::tmem_ld32(t_row + col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
       ptx::tmem_wait_ld();
-      const int k0 = j * kBN;
+      const int k0 = key_tile(j) * kBN;
       // Tiles away from the diagonal and the sequence end take the unmasked
       // branch (uniform for the warpgroup).
-      const bool need_mask = (k0 + kBN > kv_end) || (p.is_causal && (int64_t)k0 + kBN - 1 > (int64_t)r0 + offset);
+      const bool need_mask = (k0 + kBN > kv_end) || (p.is_causal && (int64_t)k0 + kBN - 1 > (int64_t)r0 + offset) ||
+                             (kWin && k0 + kBN > args.win.sinks &&
+                              (int64_t)k0 <= (int64_t)r0 + kBM - 1 + offset - args.win.window);
       const int64_t lim = p.is_causal ? (int64_t)qi + offset : (int64_t)kv_end - 1;
+      uint32_t seen[4];  // kWin: bit c of the 128 tells whether the row sees key k0 + c
+      if constexpr (kWin) {
+        const int64_t end = i64min(kv_end, lim + 1), near = lim + 1 - args.win.window;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          seen[w] = range_bits(near, end, k0 + 32 * w) | range_bits(0, i64min(end, args.win.sinks), k0 + 32 * w);
+      }
+      auto visible = [&](int c) -> bool {
+        if constexpr (kWin) return (seen[c >> 5] >> (c & 31)) & 1u;
+        return k0 + c < kv_end && (int64_t)(k0 + c) <= lim;
+      };
       // Row max of the (masked) raw scores, scaled once (scale > 0).
       float mx = -INFINITY;
       if (!need_mask) {
@@ -294,8 +322,7 @@ __global__ void __launch_bounds__(384, 1)
       } else {
 #pragma unroll
         for (int c = 0; c < kBN; ++c) {
-          const int key = k0 + c;
-          if (key < kv_end && (int64_t)key <= lim) mx = fmaxf(mx, __uint_as_float(r[c]));
+          if (visible(c)) mx = fmaxf(mx, __uint_as_float(r[c]));
         }
       }
       mx = mx == -INFINITY ? mx : mx * qk_scale;
@@ -353,11 +380,10 @@ __global__ void __launch_bounds__(384, 1)
       } else {
 #pragma unroll
         for (int c = 0; c < kBN; c += 2) {
-          const int key = k0 + c;
           float p0 = ptx::ex2(fmaf(__uint_as_float(r[c]), qk_scale, -safe));
           float p1 = ptx::ex2(fmaf(__uint_as_float(r[c + 1]), qk_scale, -safe));
-          p0 = (key < kv_end && (int64_t)key <= lim) ? p0 : 0.f;
-          p1 = (key + 1 < kv_end && (int64_t)key + 1 <= lim) ? p1 : 0.f;
+          p0 = visible(c) ? p0 : 0.f;
+          p1 = visible(c + 1) ? p1 : 0.f;
           sum2[0] = ptx::add2(sum2[0], ptx::f2pack(p0, p1));
           p0 = dropped(p0, c);
           p1 = dropped(p1, c + 1);
@@ -427,7 +453,7 @@ __global__ void __launch_bounds__(384, 1)
             v = make_uint4(ptx::pack_f16(f[0], f[1]), ptx::pack_f16(f[2], f[3]), ptx::pack_f16(f[4], f[5]),
                            ptx::pack_f16(f[6], f[7]));
           }
-          *reinterpret_cast<uint4*>(orow + 32 * c + e) = v;
+          if (!kWin || 32 * c + e < p.head_dim) *reinterpret_cast<uint4*>(orow + 32 * c + e) = v;
         }
       }
     }
@@ -451,7 +477,9 @@ __global__ void __launch_bounds__(384, 1)
 template <int D, bool BF16>
 static cudaError_t launch_pair(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                                const PairArgs& a, cudaStream_t st) {
-  auto kern = a.drop.p > 0.f ? tc_fwd_pair_kernel<D, BF16, true> : tc_fwd_pair_kernel<D, BF16, false>;
+  auto kern = a.win.window > 0 ? tc_fwd_pair_kernel<D, BF16, false, true>
+              : a.drop.p > 0.f ? tc_fwd_pair_kernel<D, BF16, true, false>
+                               : tc_fwd_pair_kernel<D, BF16, false, false>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kern), PairCfg<D>::kSmem);
   if (e != cudaSuccess) return e;
   dim3 grid(a.n_units, a.p.q_heads, a.p.batch);
@@ -460,15 +488,36 @@ static cudaError_t launch_pair(const CUtensorMap& mq, const CUtensorMap& mk, con
 }
 
 cudaError_t tc_forward_pair(const ts_attn_params& p, const CUtensorMap& mq, const CUtensorMap& mk,
-                            const CUtensorMap& mv, uint32_t* fault, cudaStream_t st, const DropoutArgs* drop) {
+                            const CUtensorMap& mv, uint32_t* fault, cudaStream_t st, const DropoutArgs* drop,
+                            const WindowArgs* win) {
   PairArgs a;
   a.p = p;
   a.n_units = ceil_div(p.q_len, 2 * kBM);
   a.fault = fault;
   a.drop = drop ? *drop : DropoutArgs{};
+  a.win = win ? *win : WindowArgs{};
   const bool bf = p.dtype == TS_BF16;
-  if (p.head_dim == 64) return bf ? launch_pair<64, true>(mq, mk, mv, a, st) : launch_pair<64, false>(mq, mk, mv, a, st);
+  if (p.head_dim <= 64) return bf ? launch_pair<64, true>(mq, mk, mv, a, st) : launch_pair<64, false>(mq, mk, mv, a, st);
   return bf ? launch_pair<128, true>(mq, mk, mv, a, st) : launch_pair<128, false>(mq, mk, mv, a, st);
+}
+
+// Half types, equal head dimensions that are multiples of 8 up to 128, rows TMA can address, a positive scale.
+bool tc_window_supported(const ts_attn_params& p) {
+  if (p.dtype != TS_BF16 && p.dtype != TS_F16) return false;
+  if (p.head_dim != p.value_dim || p.head_dim % 8 || p.head_dim > 128) return false;
+  if (p.mask_kind != TS_MASK_NONE || !(p.scale > 0.0)) return false;
+  if (!view_tma_ok(p.q) || !view_tma_ok(p.k) || !view_tma_ok(p.v) || !view_tma_ok(p.o)) return false;
+  return encode_fn() != nullptr;
+}
+
+// The two-tile kernel takes a single query tile too: its second tile is then empty.
+cudaError_t tc_forward_window(const ts_attn_params& p, const WindowArgs& win, uint32_t* fault, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, p.q, p.dtype, p.batch, p.q_heads, p.q_len, p.head_dim, kBM) ||
+      !make_map(&mk, p.k, p.dtype, p.batch, p.kv_heads, p.kv_len, p.head_dim, kBN) ||
+      !make_map(&mv, p.v, p.dtype, p.batch, p.kv_heads, p.kv_len, p.value_dim, kBN))
+    return cudaErrorInvalidValue;
+  return tc_forward_pair(p, mq, mk, mv, fault, st, nullptr, &win);
 }
 
 }  // namespace tsa

@@ -28,6 +28,7 @@ struct RopeLaunch {
   int batch, heads, seq, channels, rotary_dim;
   int64_t offset;       // position of t = 0 when positions == NULL
   const int32_t* positions;
+  bool per_token;       // positions is [B, T]: every token's own
   const float* inv_freq;  // [rotary_dim / 2]
   float sign;           // +1 forward, -1 inverse (VJP)
   // KV-append fusion: when cache.data != NULL, y is ignored and rows go to
@@ -43,7 +44,7 @@ __global__ void rope_kernel(RopeLaunch L) {
   using A = typename Elem<T>::acc;
   const int t = blockIdx.x, b = blockIdx.y;
   const int64_t base = L.positions ? (int64_t)L.positions[b] : L.offset;
-  const int64_t pos = base + t;
+  const int64_t pos = L.per_token ? (int64_t)L.positions[(int64_t)b * L.seq + t] : base + t;
   const bool to_cache = L.cache.data != nullptr;
   const int pairs = L.rotary_dim / 2;
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
@@ -127,8 +128,9 @@ static cudaError_t launch(const RopeLaunch& L, int dtype, int cache_dtype, cudaS
 
 cudaError_t rope_apply(const ts_view4& x, const ts_view4& y, int dtype, int batch, int heads, int seq,
                        int channels, int rotary_dim, int64_t offset, const int32_t* positions,
-                       const float* inv_freq, int inverse, cudaStream_t st) {
+                       const float* inv_freq, int inverse, cudaStream_t st, bool per_token) {
   RopeLaunch L = {};
+  L.per_token = per_token;
   L.x = x;
   L.y = y;
   L.batch = batch;

@@ -2,6 +2,7 @@
 #pragma once
 #include "common.cuh"
 #include "dropout.cuh"
+#include "window.cuh"
 
 namespace tsa {
 // True when the tensor-core backward takes this problem.
@@ -10,5 +11,7 @@ bool tc_bwd_supported(const ts_attn_bwd_params& bp);
 size_t tc_bwd_workspace(const ts_attn_bwd_params& bp);
 // `drop` set: the VJP of a forward that applied this dropout (mask regenerated).
 cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* workspace, size_t workspace_bytes, uint32_t* fault,
-                        cudaStream_t stream, const DropoutArgs* drop = nullptr);
+                        cudaStream_t stream, const DropoutArgs* drop = nullptr, const WindowArgs* win = nullptr);
+// True when it takes a forward that had a sliding window (tc_window_supported).
+bool tc_bwd_window_supported(const ts_attn_bwd_params& bp);
 }  // namespace tsa

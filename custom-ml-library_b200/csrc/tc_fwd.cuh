@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "dropout.cuh"
+#include "window.cuh"
 
 namespace tsa {
 // Keys of a tile: of a row that ends inside one (kv_lens) the rest of its keys and values is read, and must be finite.
@@ -17,7 +18,12 @@ cudaError_t tc_forward(const ts_attn_params& p, uint32_t* fault, cudaStream_t st
 // The two-query-tile kernel (attn_fwd_pair.cu) on the maps tc_forward built
 // (128-row boxes of Q, K and V).
 cudaError_t tc_forward_pair(const ts_attn_params& p, const CUtensorMap& mq, const CUtensorMap& mk,
-                            const CUtensorMap& mv, uint32_t* fault, cudaStream_t stream, const DropoutArgs* drop);
+                            const CUtensorMap& mv, uint32_t* fault, cudaStream_t stream, const DropoutArgs* drop,
+                            const WindowArgs* win = nullptr);
+
+// The same kernel for a sliding window with sinks (causal problems).
+bool tc_window_supported(const ts_attn_params& p);
+cudaError_t tc_forward_window(const ts_attn_params& p, const WindowArgs& win, uint32_t* fault, cudaStream_t stream);
 
 // Fewest (batch, KV head) pairs for which a grouped-query decode step runs on
 // the prefill kernel (one CTA per pair, no split along the keys): with fewer,

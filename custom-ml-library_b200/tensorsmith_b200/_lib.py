@@ -139,6 +139,62 @@ class PagePool(ctypes.Structure):
     ]
 
 
+class Window(ctypes.Structure):
+    _fields_ = [("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class Tree(ctypes.Structure):
+    _fields_ = [
+        ("parents", ctypes.c_void_p),
+        ("parents_stride", ctypes.c_int64),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+    ]
+
+
+class KvKeepParams(ctypes.Structure):
+    _fields_ = [
+        ("keys", ctypes.POINTER(ctypes.c_void_p)),
+        ("values", ctypes.POINTER(ctypes.c_void_p)),
+        ("key_stride", ctypes.c_int64 * 4),
+        ("value_stride", ctypes.c_int64 * 4),
+        ("dtype", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("value_dim", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("nodes", ctypes.c_int32),
+        ("base", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("path_stride", ctypes.c_int64),
+    ]
+
+
+class TokenLogprobs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("top", ctypes.c_int32),
+        ("targets", ctypes.c_void_p),
+        ("ignore_index", ctypes.c_int64),
+        ("logprob", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p),
+        ("top_indices", ctypes.c_void_p),
+    ]
+
+
+# Limits of ts_attn_tree (TS_TREE_MAX_NODES) and ts_token_logprobs_fwd (TS_TOP_TOKENS_MAX).
+TREE_MAX_NODES = 64
+TOP_TOKENS_MAX = 32
+
 # Every symbol include/ts_attn.h declares, with its ctypes signature.
 SIGNATURES = {
     "ts_attn_abi_version": (ctypes.c_int, []),
@@ -238,6 +294,39 @@ SIGNATURES = {
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
          ctypes.c_void_p],
+    ),
+    "ts_attn_fwd_window": (
+        ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), ctypes.c_void_p]
+    ),
+    "ts_attn_window_path": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
+    "ts_attn_bwd_window_workspace_size": (
+        ctypes.c_size_t, [ctypes.POINTER(AttnBwdParams), ctypes.POINTER(Window)]
+    ),
+    "ts_attn_bwd_window": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnBwdParams), ctypes.POINTER(Window), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ts_attn_tree": (
+        ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    ),
+    "ts_attn_tree_path": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_attn_tree_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_tree_positions": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+         ctypes.c_void_p],
+    ),
+    "ts_rope_at": (
+        ctypes.c_int,
+        [View4, View4, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+         ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p],
+    ),
+    "ts_kv_keep": (ctypes.c_int, [ctypes.POINTER(KvKeepParams), ctypes.c_void_p]),
+    "ts_token_logprobs_fwd": (ctypes.c_int, [ctypes.POINTER(TokenLogprobs), ctypes.c_void_p]),
+    "ts_token_logprobs_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(TokenLogprobs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_int64, ctypes.c_void_p],
     ),
     "ts_attn_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "ts_attn_source_digest": (ctypes.c_char_p, []),

@@ -9,9 +9,11 @@ C contract requires, and never compute anything on the host.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -54,6 +56,14 @@ def view4(t: torch.Tensor) -> _lib.View4:
 
 def _stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(index: int):
+    """A context in which ``index`` is the current device, as the C ABI wants it."""
+    return _SAME_DEVICE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def default_scale(head_dim: int) -> float:
@@ -136,9 +146,39 @@ def _dropout_struct(dropout) -> _lib.Dropout:
     return _lib.Dropout(float(p), int(seed) & (2**64 - 1), int(offset) & (2**64 - 1))
 
 
+def _window_struct(window, sinks, is_causal, mask, dropout) -> _lib.Window:
+    """The checked window of a call, or raises."""
+    if window < 1 or sinks < 0 or max(window, sinks) >= 2**31:
+        raise ValueError("a window must be positive and the number of sinks must not be negative")
+    if not is_causal:
+        raise ValueError("a sliding window needs is_causal")
+    if mask is not None or dropout is not None:
+        raise ValueError("a sliding window takes neither an explicit mask nor dropout")
+    return _lib.Window(int(window), int(sinks))
+
+
+def _no_window(sinks) -> None:
+    if sinks:
+        raise ValueError("sinks need a window")
+
+
+def window_path(q, k, v, *, window, sinks=0, causal_offset=0, scale=None, kv_lens=None) -> str:
+    """Name of the kernel family that ``forward`` and ``backward`` select under a window."""
+    w = _window_struct(window, sinks, True, None, None)
+    o = torch.empty((q.shape[0], q.shape[1], q.shape[2], v.shape[3]), dtype=q.dtype, device=q.device)
+    p, keep = make_params(q, k, v, o, None, is_causal=True, scale=scale, causal_offset=causal_offset, kv_lens=kv_lens)
+    code = _lib.lib().ts_attn_window_path(ctypes.byref(p), ctypes.byref(w))
+    if code < 0:
+        _lib.check(code, "ts_attn_window_path")
+    return _lib.PATH_NAMES[code]
+
+
 def forward(q, k, v, *, is_causal=False, scale=None, causal_offset=0, kv_lens=None, mask=None,
-            need_lse=True, out=None, lse=None, dropout=None):
+            need_lse=True, out=None, lse=None, dropout=None, window=None, sinks=0):
     """Attention forward: returns ``(out [B,Hq,Tq,Dv], lse [B,Hq,Tq] or None)``.
+
+    ``window`` (with ``is_causal``): a query at position i sees the keys j <= i with i - j < window or j < ``sinks``.
+    Pass both to ``backward``.
 
     ``lse`` is fp32 (fp64 for fp64 inputs), natural-log units, -inf on fully masked rows.
     ``dropout = (p, seed, offset)`` applies attention dropout (ts_attn_fwd_dropout); pass
@@ -151,6 +191,14 @@ def forward(q, k, v, *, is_causal=False, scale=None, causal_offset=0, kv_lens=No
         lse = torch.empty((b, hq, tq), dtype=lse_dtype(q.dtype), device=q.device)
     p, keep = make_params(q, k, v, out, lse if need_lse else None, is_causal=is_causal, scale=scale,
                           causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
+    if window is not None:
+        w = _window_struct(window, sinks, is_causal, mask, dropout)
+        with _on(q.get_device()):
+            _lib.check(_lib.lib().ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), _stream_handle(q.device)),
+                       "ts_attn_fwd_window")
+        del keep
+        return out, (lse if need_lse else None)
+    _no_window(sinks)
     if dropout is not None:
         d = _dropout_struct(dropout)
         _lib.check(_lib.lib().ts_attn_fwd_dropout(ctypes.byref(p), ctypes.byref(d), _stream_handle(q.device)),
@@ -235,8 +283,8 @@ def bwd_path(q, k, v, out, lse, dout, **kw) -> str:
 
 
 def backward(q, k, v, out, lse, dout, *, is_causal=False, scale=None, causal_offset=0, kv_lens=None,
-             mask=None, dq=None, dk=None, dv=None, dropout=None):
-    """dQ, dK, dV of attention from the forward output and its LSE (``dropout`` as given
+             mask=None, dq=None, dk=None, dv=None, dropout=None, window=None, sinks=0):
+    """dQ, dK, dV of attention from the forward output and its LSE (``dropout``, ``window`` and ``sinks`` as given
     to the forward)."""
     _check_inputs(q, k, v)
     _require_cuda(out, lse, dout)
@@ -248,6 +296,16 @@ def backward(q, k, v, out, lse, dout, *, is_causal=False, scale=None, causal_off
     bp, keep = _bwd_params(q, k, v, out, lse, dout, dq, dk, dv, is_causal=is_causal, scale=scale,
                            causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
     handle = _lib.lib()
+    if window is not None:
+        w = _window_struct(window, sinks, is_causal, mask, dropout)
+        need = int(handle.ts_attn_bwd_window_workspace_size(ctypes.byref(bp), ctypes.byref(w)))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        with _on(q.get_device()):
+            _lib.check(handle.ts_attn_bwd_window(ctypes.byref(bp), ctypes.byref(w), ws.data_ptr(), ws.numel(),
+                                                 _stream_handle(q.device)), "ts_attn_bwd_window")
+        del keep
+        return dq, dk, dv
+    _no_window(sinks)
     if dropout is not None:
         d = _dropout_struct(dropout)
         need = int(handle.ts_attn_bwd_dropout_workspace_size(ctypes.byref(bp)))
@@ -614,6 +672,275 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
     return out, lse
 
 
+# -- drafted tokens over a cache -----------------------------------------------
+
+
+_TREE_STRUCT = struct.Struct("@Pqii")
+
+
+def _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse):
+    """(packed ts_attn_params, packed ts_tree, device index) of an attention_tree call after its checks."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("expected [batch, heads, sequence, channels] views")
+    index = q.get_device()
+    if index < 0 or k.get_device() != index or v.get_device() != index:
+        raise ValueError("the B200 attention engine needs CUDA device tensors, all on one device")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise TypeError("attention inputs must have the same floating-point dtype")
+    code = dtype_code(q.dtype)
+    rows, heads, nodes, dim = q.shape
+    kv_heads, capacity, value_dim = v.shape[1:]
+    if k.shape != (rows, kv_heads, capacity, dim) or v.shape[0] != rows:
+        raise ValueError("query, key and value shapes do not match")
+    if 0 in q.shape or 0 in v.shape or heads % kv_heads:
+        raise ValueError("query heads must be a multiple of the cache heads, and nothing may be empty")
+    lens = _int32_vector(kv_lens, "kv_lens", rows, index)
+    tree, stride = 0, 0
+    if parents is not None:
+        if parents.dtype != torch.int32 or parents.shape != (rows, nodes) or parents.get_device() != index or (
+                parents.stride(1) != 1 and nodes > 1):
+            raise ValueError("parents must be int32 [batch, nodes] with contiguous rows on the query's device")
+        if nodes > _lib.TREE_MAX_NODES:
+            raise ValueError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes")
+        tree, stride = parents.data_ptr(), parents.stride(0)
+    if window is None:
+        _no_window(sinks)
+        window = 0
+    elif window < 1 or sinks < 0 or max(window, sinks) >= 2**31:
+        raise ValueError("a window must be positive and the number of sinks must not be negative")
+    if lse is None:
+        lse = (0, 0, 0, 0)
+    elif lse.shape != q.shape[:3] or lse.dtype != lse_dtype(q.dtype) or lse.get_device() != index:
+        raise ValueError("lse must be [B, Hq, T] on the query's device, fp32 (fp64 for fp64 inputs)")
+    else:
+        lse = (lse.data_ptr(), *lse.stride())
+    if out.shape != (rows, heads, nodes, value_dim) or out.dtype != q.dtype or out.get_device() != index:
+        raise ValueError("out must be [B, Hq, T, Dv] of the query's dtype and device")
+    scale = default_scale(dim) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("attention scale must be finite")
+    return (_ATTN_STRUCT.pack(q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(),
+                              out.data_ptr(), *out.stride(), *lse, code, rows, heads, kv_heads, nodes, capacity, dim,
+                              value_dim, scale, 1, 0, lens, 0, 0, 0, 0, 0, 0),
+            _TREE_STRUCT.pack(tree, stride, int(window), int(sinks)), index)
+
+
+def _tree_out(q, v):
+    return q.new_empty((*q.shape[:3], v.shape[-1]))
+
+
+def attention_tree_path(q, k, v, kv_lens, parents=None, *, window=None, sinks=0, scale=None) -> str:
+    """Name of the kernel family ``attention_tree`` selects: "tcgen05" or "simt"."""
+    params, tree, _ = _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, _tree_out(q, v), None)
+    code = _lib.lib().ts_attn_tree_path(params, tree)
+    if code < 0:
+        _lib.check(code, "ts_attn_tree_path")
+    return _lib.PATH_NAMES[code]
+
+
+def attention_tree_workspace_bytes(q, k, v, kv_lens, parents=None, *, window=None, sinks=0, scale=None) -> int:
+    """Bytes of the ``workspace`` that ``attention_tree`` needs for these arguments."""
+    params, tree, _ = _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, _tree_out(q, v), None)
+    return int(_lib.lib().ts_attn_tree_workspace_size(params, tree))
+
+
+def attention_tree(q, k, v, kv_lens, parents=None, *, window=None, sinks=0, scale=None, need_lse=False, out=None,
+                   lse=None, workspace=None):
+    """Attention of T drafted tokens a row, ``q`` [B, Hq, T, D], over a KV cache: ``(out, lse or None)``.
+
+    The last T of row b's ``kv_lens[b]`` keys in ``k``, ``v`` [B, Hkv, capacity, D] are the drafted tokens (T = 1: a
+    plain decode step).  ``parents`` (int32 [B, T]) makes them a tree of at most 64 nodes: node i's parent is an
+    earlier node, or -1 for the committed tokens; it sees every committed token, its ancestors and itself.  Any other
+    entry marks a padded node: its output is zero (LSE -inf), and neither it nor its children are seen by others.
+    Without ``parents`` the tokens are a chain.  ``window`` and ``sinks`` as in ``forward``, by the nodes' positions
+    (``tree_positions``)."""
+    if out is None:
+        out = _tree_out(q, v)
+    if not need_lse:
+        lse = None
+    elif lse is None:
+        lse = q.new_empty(q.shape[:3], dtype=lse_dtype(q.dtype))
+    params, tree, index = _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse)
+    handle = _lib.lib()
+    need = handle.ts_attn_tree_workspace_size(params, tree)
+    if need:
+        workspace = _workspace(workspace, need, q)
+    with _on(index):
+        status = handle.ts_attn_tree(params, tree, workspace.data_ptr() if need else None, need, _raw_stream(index))
+    if status:
+        _lib.check(status, "ts_attn_tree")
+    return out, lse
+
+
+def tree_positions(parents, lens):
+    """Positions int32 [B, T] of drafted nodes: ``lens[b]`` committed tokens plus the node's depth, -1 for padded
+    nodes.  ``rope`` takes them for the nodes' queries and keys."""
+    index = parents.get_device()
+    if parents.dtype != torch.int32 or parents.dim() != 2 or index < 0 or 0 in parents.shape or (
+            parents.stride(1) != 1 and parents.shape[1] > 1):
+        raise ValueError("parents must be int32 [batch, nodes] with contiguous rows on a CUDA device")
+    rows, nodes = parents.shape
+    positions = parents.new_empty((rows, nodes))
+    with _on(index):
+        status = _lib.lib().ts_tree_positions(parents.data_ptr(), parents.stride(0),
+                                              _int32_vector(lens, "lens", rows, index), rows, nodes,
+                                              positions.data_ptr(), _raw_stream(index))
+    if status:
+        _lib.check(status, "ts_tree_positions")
+    return positions
+
+
+def kv_keep(caches, base, path, counts):
+    """Close caches behind the accepted path: of every ``(keys, values)`` pair [B, H, capacity, C] in ``caches``, slot
+    ``base[b] + path[b, k]`` moves to slot ``base[b] + k`` for k < ``counts[b]``.
+
+    ``path`` (int32 [B, N]) holds the accepted nodes in ascending order, ``base`` and ``counts`` int32 vectors.  All
+    layers share their shapes, strides and dtype (int8 storage too; the scales of an int8 cache are caches of one
+    channel)."""
+    caches = [tuple(pair) for pair in caches]
+    if not caches or any(len(pair) != 2 for pair in caches):
+        raise ValueError("caches must be (keys, values) pairs")
+    key, value = caches[0]
+    index = key.get_device()
+    if index < 0 or key.dim() != 4 or value.dim() != 4 or value.shape[:3] != key.shape[:3]:
+        raise ValueError("caches must be [batch, heads, capacity, channels] on a CUDA device")
+    if 0 in key.shape or 0 in value.shape or key.dtype != value.dtype:
+        raise ValueError("caches must not be empty, keys and values of one dtype")
+    for pair in caches:
+        for t, like in zip(pair, (key, value)):
+            if t.shape != like.shape or t.stride() != like.stride() or t.dtype != like.dtype or t.get_device() != index:
+                raise ValueError("the caches of all layers must have the same shape, strides, dtype and device")
+    for t in (key, value):
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            raise ValueError("a cache's channels must be contiguous")
+    rows = key.shape[0]
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != rows or path.get_device() != index or (
+            path.stride(1) != 1 and path.shape[1] > 1):
+        raise ValueError("path must be int32 [batch, nodes] with contiguous rows on the caches' device")
+    base, counts = _int32_vector(base, "base", rows, index), _int32_vector(counts, "counts", rows, index)
+    if path.shape[1] == 0:
+        return
+    n = len(caches)
+    p = _lib.KvKeepParams()
+    p.keys = (ctypes.c_void_p * n)(*(pair[0].data_ptr() for pair in caches))
+    p.values = (ctypes.c_void_p * n)(*(pair[1].data_ptr() for pair in caches))
+    p.key_stride = (ctypes.c_int64 * 4)(*key.stride()[:3], 1)
+    p.value_stride = (ctypes.c_int64 * 4)(*value.stride()[:3], 1)
+    p.dtype = _storage_code(key.dtype)
+    p.layers, p.batch, p.heads, p.capacity, p.head_dim = n, *key.shape
+    p.value_dim, p.nodes = value.shape[3], path.shape[1]
+    p.base, p.path, p.counts, p.path_stride = base, path.data_ptr(), counts, path.stride(0)
+    with _on(index):
+        _lib.check(_lib.lib().ts_kv_keep(ctypes.byref(p), ctypes.c_void_p(_raw_stream(index))), "ts_kv_keep")
+
+
+# -- log probabilities of tokens -------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` gives for [..., V] logits: fp32 ``logprob`` and ``entropy`` [...], ``top_logprobs``
+    [..., top] and int64 ``top_indices`` [..., top]; ``norm`` [..., 2] is the backward's."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_indices: torch.Tensor
+    norm: torch.Tensor
+
+    @property
+    def lse(self) -> torch.Tensor:
+        """log sum exp of the logits."""
+        return self.norm[..., 0] + self.norm[..., 1]
+
+
+_LOGPROB_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _logit_rows(logits):
+    """Logits [..., V] as [rows, V] with contiguous rows, without a copy where their strides allow it."""
+    if logits.dtype not in _LOGPROB_DTYPES:
+        raise TypeError("logits must be float32, float16 or bfloat16")
+    if logits.get_device() < 0:
+        raise ValueError("the B200 attention engine needs CUDA device tensors")
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError("logits must be [..., vocabulary]")
+    flat = logits.reshape(-1, logits.shape[-1])
+    if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < 0):
+        flat = flat.contiguous()
+    return flat
+
+
+def _logprob_params(flat, targets, top, ignore_index):
+    p = _lib.TokenLogprobs()
+    p.logits, p.stride, p.dtype = flat.data_ptr(), flat.stride(0), dtype_code(flat.dtype)
+    p.rows, p.vocab, p.top = flat.shape[0], flat.shape[1], top
+    p.targets, p.ignore_index = targets.data_ptr(), ignore_index
+    return p
+
+
+def _target_rows(targets, logits):
+    if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1] or targets.get_device() != logits.get_device():
+        raise ValueError("targets must be int64 and have the shape of the logits without the vocabulary, on their device")
+    return targets.reshape(-1).contiguous()
+
+
+def token_logprobs(logits, targets, *, top=0, ignore_index=-100) -> TokenLogprobs:
+    """Log probabilities of ``targets`` [...] under softmax of ``logits`` [..., V], entropies (nats) and the ``top``
+    most likely alternatives (at most 32; equal logits by index), in one pass.
+
+    A target equal to ``ignore_index`` has log probability 0; one outside the vocabulary NaN.  A row of -inf has log
+    probabilities of -inf and entropy 0."""
+    flat = _logit_rows(logits)
+    goal = _target_rows(targets, logits)
+    shape, (rows, vocab) = targets.shape, flat.shape
+    if not 0 <= top <= min(vocab, _lib.TOP_TOKENS_MAX):
+        raise ValueError(f"top must be between zero and {_lib.TOP_TOKENS_MAX}, and within the vocabulary")
+    sums = flat.new_empty((4 + top, rows), dtype=torch.float32)
+    logprob, entropy, norm = sums[0], sums[1], sums[2:4].view(rows, 2)
+    values, indices = sums[4:].view(rows, top), targets.new_empty((rows, top))
+    if rows:
+        p = _logprob_params(flat, goal, top, int(ignore_index))
+        p.logprob, p.entropy, p.norm = logprob.data_ptr(), entropy.data_ptr(), norm.data_ptr()
+        p.top_logprobs, p.top_indices = (values.data_ptr(), indices.data_ptr()) if top else (None, None)
+        index = flat.get_device()
+        with _on(index):
+            status = _lib.lib().ts_token_logprobs_fwd(ctypes.byref(p), ctypes.c_void_p(_raw_stream(index)))
+        if status:
+            _lib.check(status, "ts_token_logprobs_fwd")
+    return TokenLogprobs(logprob.view(shape), entropy.view(shape), values.view(*shape, top), indices.view(*shape, top),
+                         norm.view(*shape, 2))
+
+
+def token_logprobs_backward(logits, targets, result, grad_logprob=None, grad_entropy=None, grad_top=None, *,
+                            ignore_index=-100):
+    """Gradient of the logits from those of ``result = token_logprobs(logits, targets)``: of its ``logprob``,
+    ``entropy`` and ``top_logprobs`` (each fp32, optional)."""
+    flat = _logit_rows(logits)
+    goal = _target_rows(targets, logits)
+    top, index = result.top_indices.shape[-1], flat.get_device()
+    given = []
+    for g, like in ((grad_logprob, result.logprob), (grad_entropy, result.entropy), (grad_top, result.top_logprobs)):
+        if g is not None:
+            if g.shape != like.shape or g.dtype != torch.float32 or g.get_device() != index:
+                raise ValueError("gradients must be fp32 of the shapes of what they belong to, on the logits' device")
+            g = g.contiguous()
+        given.append(g)
+    if result.logprob.shape != targets.shape or result.logprob.get_device() != index:
+        raise ValueError("the result belongs to other logits")
+    grad = torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
+    if flat.shape[0]:
+        keep = [t.contiguous() for t in (result.entropy, result.norm, result.top_indices)]
+        p = _logprob_params(flat, goal, top, int(ignore_index))
+        p.entropy, p.norm, p.top_indices = keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr() if top else None
+        with _on(index):
+            status = _lib.lib().ts_token_logprobs_bwd(
+                ctypes.byref(p), *(None if g is None else ctypes.c_void_p(g.data_ptr()) for g in given),
+                ctypes.c_void_p(grad.data_ptr()), grad.stride(0), ctypes.c_void_p(_raw_stream(index)))
+        if status:
+            _lib.check(status, "ts_token_logprobs_bwd")
+    return grad.view(logits.shape)
+
+
 # -- pages ---------------------------------------------------------------------
 
 
@@ -745,7 +1072,8 @@ def rope_inv_freq(rotary_dim: int, base: float, device) -> torch.Tensor:
 
 def rope(x, *, offset=0, base=10000.0, rotary_dim=None, positions=None, inverse=False, out=None):
     """Interleaved-pair rotary embedding of a [B, H, T, C] view at positions offset + t
-    (or positions[b] + t); ``inverse`` applies the inverse rotation (the VJP)."""
+    (or positions[b] + t; or positions[b, t], as ``tree_positions`` gives them); ``inverse`` applies the inverse
+    rotation (the VJP)."""
     _require_cuda(x)
     dim = x.shape[3] if rotary_dim is None else int(rotary_dim)
     out = torch.empty_like(x) if out is None else out
@@ -753,6 +1081,16 @@ def rope(x, *, offset=0, base=10000.0, rotary_dim=None, positions=None, inverse=
     pos = None
     if positions is not None:
         pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
+        if pos.dim() == 2:
+            if pos.shape != (x.shape[0], x.shape[2]) or pos.device != x.device:
+                raise ValueError("positions of every token must be [B, T] on the input's device")
+            pos = pos.contiguous()
+            with _on(x.get_device()):
+                _lib.check(
+                    _lib.lib().ts_rope_at(view4(x), view4(out), dtype_code(x.dtype), x.shape[0], x.shape[1],
+                                          x.shape[2], x.shape[3], dim, pos.data_ptr(), inv.data_ptr(),
+                                          1 if inverse else 0, _stream_handle(x.device)), "ts_rope_at")
+            return out
     _lib.check(
         _lib.lib().ts_rope(view4(x), view4(out), dtype_code(x.dtype), x.shape[0], x.shape[1], x.shape[2],
                            x.shape[3], dim, int(offset), pos.data_ptr() if pos is not None else None,

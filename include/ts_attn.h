@@ -400,6 +400,100 @@ TS_ATTN_API int ts_kv_pages_compact(const ts_page_pool* pool, const int32_t* tab
                                     const int32_t* refs, int32_t* refs_out, int32_t* counters, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* ---- Attention under a sliding window with sinks (no counterpart in tensorsmith, whose causal rule is
+ * nn/attention.py:108-111) ----
+ * A query at position i (causal_offset + its index; kv_lens[b] - q_len + its index where kv_lens is set) sees the
+ * keys j <= i with i - j < window or j < sinks. */
+typedef struct ts_window {
+  int32_t window; /* at least 1; 0 where a call takes it as "no window" */
+  int32_t sinks;  /* first keys that stay visible, at least 0 */
+} ts_window;
+
+/* ts_attn_fwd under a window: is_causal must be set, no explicit mask, no dropout.  Keys between the sinks and the
+ * window of a block of queries are not read.  Half types with equal head dimensions that are multiples of 8 up to 128
+ * run on the tcgen05 kernel (P in q's type, as ts_attn_fwd), everything else on CUDA cores. */
+TS_ATTN_API int ts_attn_fwd_window(const ts_attn_params* params, const ts_window* window, void* stream);
+/* Kernel family of both directions: TS_PATH_TCGEN05 or TS_PATH_SIMT, or a negative ts_status. */
+TS_ATTN_API int ts_attn_window_path(const ts_attn_params* params, const ts_window* window);
+TS_ATTN_API size_t ts_attn_bwd_window_workspace_size(const ts_attn_bwd_params* params, const ts_window* window);
+/* ts_attn_bwd for a forward made by ts_attn_fwd_window with the same window. */
+TS_ATTN_API int ts_attn_bwd_window(const ts_attn_bwd_params* params, const ts_window* window, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ---- Drafted tokens over a KV cache: a tree of them, or a chain (no counterpart in tensorsmith) ----
+ * The last q_len of row b's kv_lens[b] keys are drafted tokens: node i sits in slot kv_lens[b] - q_len + i.  A node
+ * sees every committed key (before them), its ancestors and itself; under a window, those of them that the rule of
+ * ts_window lets it see, its position being the number of committed keys plus its depth.  Nodes whose slot would lie
+ * before the cache do not exist. */
+typedef struct ts_tree {
+  const int32_t* parents; /* [batch, q_len] (device): node i's parent, a node before it, or -1: the committed tokens.
+                             Any other value marks a padded node: it and its children give zeros (LSE -inf) and are
+                             seen by nobody.  NULL: a chain, node i's parent is node i - 1. */
+  int64_t parents_stride; /* entries between rows */
+  int32_t window, sinks;  /* ts_window; window 0: none */
+} ts_tree;
+#define TS_TREE_MAX_NODES 64 /* q_len with parents; chains may be longer */
+
+/* Attention of q [batch, Hq, q_len, D] over the cache k, v: params as for ts_attn_decode with kv_lens required;
+ * is_causal and causal_offset are ignored, no explicit mask.  Slots at and behind kv_lens[b] are not used, whatever
+ * they hold.  Half types with equal head dimensions that are multiples of 8 up to 128 run on the tcgen05 kernel. */
+TS_ATTN_API int ts_attn_tree(const ts_attn_params* params, const ts_tree* tree, void* workspace,
+                             size_t workspace_bytes, void* stream);
+TS_ATTN_API int ts_attn_tree_path(const ts_attn_params* params, const ts_tree* tree);
+TS_ATTN_API size_t ts_attn_tree_workspace_size(const ts_attn_params* params, const ts_tree* tree);
+
+/* positions[b, i] = lens[b] + depth of node i (int32 [batch, nodes], contiguous), -1 for padded nodes: what ts_rope_at
+ * rotates the queries and keys of drafted tokens by.  lens: committed tokens. */
+TS_ATTN_API int ts_tree_positions(const int32_t* parents, int64_t parents_stride, const int32_t* lens, int32_t batch,
+                                  int32_t nodes, int32_t* positions, void* stream);
+/* ts_rope with a position of its own for every token: positions int32 [batch, seq], contiguous. */
+TS_ATTN_API int ts_rope_at(ts_view4 x, ts_view4 y, int32_t dtype, int32_t batch, int32_t heads, int32_t seq,
+                           int32_t channels, int32_t rotary_dim, const int32_t* positions, const float* inv_freq,
+                           int32_t inverse, void* stream);
+
+/* Closes caches behind the accepted path: slot base[b] + path[b, k] moves to slot base[b] + k for k < counts[b], in
+ * the key and value caches of every layer.  path ascends (nodes of one root-to-leaf path do); entries that would read
+ * past the capacity are skipped. */
+typedef struct ts_kv_keep_params {
+  void* const* keys; /* host arrays of `layers` device pointers, all with the strides below */
+  void* const* values;
+  int64_t key_stride[4], value_stride[4]; /* elements between rows, heads, slots, channels (1) */
+  int32_t dtype;                          /* any ts_dtype, TS_I8 included */
+  int32_t layers, batch, heads, head_dim, value_dim, capacity, nodes;
+  const int32_t* base;   /* [batch] committed tokens */
+  const int32_t* path;   /* [batch, nodes] */
+  const int32_t* counts; /* [batch], at most nodes are used */
+  int64_t path_stride;
+} ts_kv_keep_params;
+TS_ATTN_API int ts_kv_keep(const ts_kv_keep_params* params, void* stream);
+
+/* ---- Log probabilities of given tokens (a language model's loss is their mean, negated) ----
+ * logprob[r] = x[r, targets[r]] - lse(x[r]); 0 where targets[r] == ignore_index, NaN where it lies outside the
+ * vocabulary.  entropy[r] = -sum p log p, in nats.  The `top` largest logits, in descending order, equal ones by
+ * index (NaN is the largest): their log probabilities and indices.  A row of -inf has log probabilities of -inf,
+ * entropy 0 and no gradient; NaN and +inf give NaN. */
+typedef struct ts_token_logprobs {
+  const void* logits; /* [rows, vocab], contiguous rows */
+  int64_t stride;     /* elements between rows */
+  int32_t dtype;      /* F32, F16 or BF16; sums in fp32 */
+  int32_t rows, vocab;
+  int32_t top; /* 0 to TS_TOP_TOKENS_MAX, at most vocab */
+  const int64_t* targets;
+  int64_t ignore_index;
+  float* logprob;       /* [rows] */
+  float* entropy;       /* [rows] */
+  float* norm;          /* [rows, 2]: the largest logit m and log sum e^(x - m) (-inf: a row of -inf); optional */
+  float* top_logprobs;  /* [rows, top] */
+  int64_t* top_indices; /* [rows, top] */
+} ts_token_logprobs;
+#define TS_TOP_TOKENS_MAX 32
+TS_ATTN_API int ts_token_logprobs_fwd(const ts_token_logprobs* params, void* stream);
+/* grad_logits [rows, vocab] (dtype of the logits, another buffer) from the gradients of logprob, entropy and
+ * top_logprobs (each optional, fp32, contiguous), given the forward's norm, entropy and top_indices. */
+TS_ATTN_API int ts_token_logprobs_bwd(const ts_token_logprobs* params, const float* grad_logprob,
+                                      const float* grad_entropy, const float* grad_top, void* grad_logits,
+                                      int64_t grad_stride, void* stream);
+
 /* Reads and clears the device fault word written by kernels whose bounded
  * waits gave up, or that met a page outside the pool.  Synchronises `stream`.
  * Returns TS_OK, TS_ERR_DEVICE_TIMEOUT or TS_ERR_PAGE; *info (optional) receives
