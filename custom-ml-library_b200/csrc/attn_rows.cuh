@@ -79,6 +79,49 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
   }
 }
 
+// Rows [r0, r0 + rows) of the packed rows (head h0 + r / tokens, token r % tokens), r < end.
+template <typename T, typename A>
+__device__ __forceinline__ void stage_packed(A* dst, int stride, const ts_view4& src, int b, int h0, int r0, int rows,
+                                             int end, int tokens, int C) {
+  constexpr int kVec = 16 / sizeof(T), kBatch = 4;
+  const T* base = reinterpret_cast<const T*>(src.data) + (int64_t)b * src.stride[0];
+  auto row_at = [&](int r) { return base + (int64_t)(h0 + r / tokens) * src.stride[1] + (int64_t)(r % tokens) * src.stride[2]; };
+  const bool vec = src.stride[3] == 1 && C % kVec == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
+                   (src.stride[1] * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0;
+  const int wide = ceil_div(C, 4) * 4, per = vec ? C / kVec : wide, n = rows * per;
+  for (int x0 = threadIdx.x; x0 < n; x0 += kRowsThreads * kBatch) {
+    if (vec) {
+      uint4 raw[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int x = x0 + u * kRowsThreads, r = x / per, c = x % per;
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (x < n && r0 + r < end) raw[u] = *reinterpret_cast<const uint4*>(row_at(r0 + r) + c * kVec);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int x = x0 + u * kRowsThreads, r = x / per, c = x % per;
+        if (x >= n) break;
+        const T* e = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) dst[r * stride + c * kVec + i] = Elem<T>::to_acc(e[i]);
+      }
+    } else {
+      T raw[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int x = x0 + u * kRowsThreads, r = x / per, c = x % per;
+        raw[u] = x < n && r0 + r < end && c < C ? row_at(r0 + r)[c * src.stride[3]] : Elem<T>::from_acc(A(0));
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int x = x0 + u * kRowsThreads;
+        if (x < n) dst[x / per * stride + x % per] = Elem<T>::to_acc(raw[u]);
+      }
+    }
+  }
+}
+
 // acc[r][k] = sum_c rows[ty + 16 r][c] cols[tx + 8 k][c].
 template <int RT, typename A>
 __device__ __forceinline__ void dots(A (&acc)[RT][4], const A* rows, const A* cols, int stride, int C, int ty, int tx) {
@@ -281,32 +324,24 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
   using A = typename F::A;
   constexpr bool kSplit = sizeof(A) == 4;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ int64_t s_rest, s_tiles;
-  __shared__ int s_row;
+  __shared__ LinePlace s_ends[2];
+  __shared__ int s_parents[kTreeNodes];
   const ts_attn_params& p = a.p;
   wait_for_previous();
   let_next_start();
   F f(reinterpret_cast<A*>(smem_raw));
-  const TreeLine line(a, kRowsCols);
+  const TreeLine line(a, kRowsCols, 0);
   const int group = p.q_heads / p.kv_heads;
   const A scale2 = (A)(p.scale * kLog2eD);
   LineWalk walk;
   if constexpr (kSplit) {
     if (threadIdx.x < 32) {
-      int64_t before;
-      const int64_t total = line_total(line, threadIdx.x, 0, &before);
-      const int ctas = (int)i64min(a.ctas, total);
-      int row = 0;
-      int64_t rest = 0, tiles = 0;
-      if ((int)blockIdx.x < ctas) {
-        const int64_t at = line_bound(blockIdx.x, total, ctas);
-        tiles = line_bound(blockIdx.x + 1, total, ctas) - at;
-        line_find(line, threadIdx.x, at, &row, &rest);
-      }
-      if (threadIdx.x == 0) s_row = row, s_rest = rest, s_tiles = tiles;
+      LinePlace ends[2];
+      line_share(line, threadIdx.x, blockIdx.x, a.ctas, ends);
+      if (threadIdx.x == 0) s_ends[0] = ends[0], s_ends[1] = ends[1];
     }
     __syncthreads();
-    walk.start(s_row, s_rest, s_tiles, line);
+    walk.start(s_ends[0], s_ends[1].tiles - s_ends[0].tiles, line);
   } else {
     walk.b = blockIdx.x / line.units;
     walk.unit = blockIdx.x % line.units;
@@ -318,20 +353,15 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
     const int len = tree_len(p, b);
     const int64_t base = (int64_t)len - p.q_len;
     const WindowTiles wt(a.win, base, len, kRowsCols);
-    const int32_t* parents = a.parents + b * a.parents_stride;
     __syncthreads();  // the unit before is used up
-    for (int x = threadIdx.x; x < F::C::kRows * p.head_dim; x += kRowsThreads) {
-      const int r = x / p.head_dim, c = x % p.head_dim, i = r0 + r;
-      f.q[r * F::C::kStride + c] =
-          i < a.rows ? Elem<T>::to_acc(*at4<T>(p.q, b, hk * group + i / p.q_len, i % p.q_len, c)) : A(0);
-    }
-    for (int x = threadIdx.x; x < F::C::kRows * 4; x += kRowsThreads)  // to a whole quad
-      if (p.head_dim + x % 4 < ceil_div(p.head_dim, 4) * 4) f.q[x / 4 * F::C::kStride + p.head_dim + x % 4] = A(0);
+    if (a.parents && (int)threadIdx.x < p.q_len) s_parents[threadIdx.x] = a.parents[b * a.parents_stride + threadIdx.x];
+    stage_packed<T, A>(f.q, F::C::kStride, p.q, b, hk * group, r0, F::C::kRows, a.rows, p.q_len, p.head_dim);
+    __syncthreads();
     NodeView view[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int i = r0 + f.ty + 16 * r;
-      view[r] = tree_node(i % p.q_len, base, !a.parents, a.win, [&](int node) { return parents[node]; });
+      view[r] = tree_node(i % p.q_len, base, !a.parents, a.win, [&](int node) { return s_parents[node]; });
       if (i >= a.rows) view[r].end = 0, view[r].drafted = 0;
     }
     f.start();
@@ -604,7 +634,7 @@ cudaError_t rows_tree_t(TreeArgs& a, cudaStream_t st) {
   const unsigned grid = sizeof(A) == 4 ? (unsigned)a.ctas : (unsigned)(a.p.batch * a.p.kv_heads * a.row_tiles);
   const cudaError_t e = launch_rows(rows_tree_kernel<T, RT, DC>, dim3(grid), C::kFwdSmem, st, a);
   if (e != cudaSuccess || sizeof(A) == 8) return e;
-  return tree_merge(a, kRowsCols, 1, st);
+  return tree_merge(a, kRowsCols, 0, st);
 }
 
 template <typename T, int DC>
@@ -645,12 +675,12 @@ inline int rows_tree_dc(const ts_attn_params& p) {
 template <typename T, int DC>
 cudaError_t rows_tree_d(const ts_attn_params& p, TreeArgs* a, size_t* bytes, void* workspace, cudaStream_t st) {
   const int rt = rows_tree_rt<T, DC>(p);
-  TreeArgs made = tree_args(p, 16 * rt, 2 * device_sms(), 1, bytes);
+  TreeArgs made = tree_args(p, 16 * rt, 2 * device_sms(), bytes);
   if (!a) return cudaSuccess;  // the workspace's size alone
   made.parents = a->parents;
   made.parents_stride = a->parents_stride;
   made.win = a->win;
-  tree_place(&made, 1, workspace);
+  tree_place(&made, workspace);
   if constexpr (sizeof(typename Elem<T>::acc) == 4) {
     if constexpr (DC <= 4)
       if (rt == 4) return rows_tree_t<T, 4, DC>(made, st);

@@ -6,12 +6,14 @@
 // which every SM takes an equal share; a unit that several CTAs share is joined by tree_merge_kernel.
 // Per CTA, one pipeline over its whole share, across units:
 //   warp 0      TMA producer, K and V tiles through one ring, in the order in which they are multiplied
-//   warp 1      MMA issuer: S_t = Q K^T and O_t += P_t V for tile i, t = i mod 2
+//   warp 1      MMA issuer: S(i + 1) = Q K(i + 1)^T, then O_t += P_t(i) V(i) for the two halves t of the keys
 //   warps 2, 3  the rows of Q, packed by plain loads (any T, any strides), one unit ahead
-//   warps 4-7   softmax of the even tiles, warps 8-11 of the odd ones: the same rows, a running maximum,
-//               sum and accumulator of their own, thread r on row r
-// The two softmax groups halve the time of a tile's exponentials, which one group alone would spend longer
-// on (about 1850 clocks) than the tile's bytes take from memory per SM (about 1500 at two tiles in flight).
+//   warps 4-7   softmax of the lower 64 keys of every tile, warps 8-11 of the upper ones: the same rows, a
+//               running maximum, sum and accumulator of their own, thread r on row r; joined at a unit's end
+// S is a tile ahead, so a V tile waits in the ring for its own P alone and the rest of the ring is in flight.
+// (Groups on alternate whole tiles hold two V tiles back, and the ring then keeps too little in flight: 198
+// against 150 us for 32 rows of 500 to 8192 keys, 16 nodes; with six slots instead of five, the queries of up to 64 rows
+// in half the room, 122.)
 // P is rounded to the type of V, as in the prefill kernels; scores, sums and accumulators are fp32.
 #include <type_traits>
 
@@ -24,7 +26,8 @@ namespace tsa {
 
 namespace {
 
-constexpr int kBM = 128, kBN = 128;
+constexpr int kBM = 128, kBN = 128, kHalf = kBN / 2;
+constexpr int kUnitPlaces = 2;  // what a unit's start and end cost, in tiles (about 2.5 us; a tile takes 1.65)
 constexpr int kSlabBytes = 128 * 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -33,23 +36,26 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 template <int D> struct TreeCfg {
   static constexpr int kSlabs = D / 64;
   static constexpr int kTileBytes = kSlabs * kSlabBytes;
-  static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kOffKV = 2 * kTileBytes;  // behind the two buffers of Q
-  static constexpr int kOffBar = kOffKV + kStages * kTileBytes;
-  static constexpr int kSmem = kOffBar + 512 + 1024;  // barriers; alignment
+  // Two buffers of Q and a ring of K and V tiles share kTiles tiles' room.  Up to 64 rows the buffers of Q take half
+  // of it each (the products then read other bytes for the rows behind, whose results are not used).
+  static constexpr int kTiles = D == 128 ? 7 : 12;
+  static constexpr int kOffBar = kTiles * kTileBytes;
+  static constexpr int kSmem = kOffBar + 1536 + 1024;  // barriers; alignment
   static constexpr uint32_t kColS = 0, kColO = 256;
 };
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 11;
 
 struct TreeBars {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t s_full[2], p_full[2], o_done[2], drain;
-  int64_t rest, tiles;  // the share: its place within its first row, its length
-  int row;
+  uint64_t halves, joined, o_read;  // at a segment's end: the upper half's sums, the factors, O read by both groups
+  LinePlace from;  // the share's beginning
+  int64_t tiles;   // and its tiles
   uint32_t tmem_base;
+  float2 red[kBM];
 };
-static_assert(sizeof(TreeBars) <= 512, "barriers");
+static_assert(sizeof(TreeBars) <= 1536, "barriers");
 
 }  // namespace
 
@@ -58,13 +64,15 @@ __global__ void __launch_bounds__(384, 1)
     attn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ TreeArgs args) {
   using C = TreeCfg<D>;
-  constexpr int S = C::kStages;
   const ts_attn_params& p = args.p;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
   TreeBars* bars = reinterpret_cast<TreeBars*>(smem + C::kOffBar);
-  unsigned char* sQ = smem;
-  unsigned char* sKV = smem + C::kOffKV;
+  const bool low = args.part_rows <= kBM / 2;
+  const int S = C::kTiles - (low ? 1 : 2);                        // slots of the ring
+  const int q_slab = low ? kSlabBytes / 2 : kSlabBytes;           // 64 channels of a buffer's rows
+  unsigned char* sQ = smem;                                       // buffer i at i * kSlabs * q_slab
+  unsigned char* sKV = smem + (low ? 1 : 2) * C::kTileBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -80,6 +88,9 @@ __global__ void __launch_bounds__(384, 1)
       ptx::mbar_init(&bars->kv_empty[s], 1);
     }
     ptx::mbar_init(&bars->drain, 1);
+    ptx::mbar_init(&bars->halves, 4);
+    ptx::mbar_init(&bars->joined, 4);
+    ptx::mbar_init(&bars->o_read, 8);
     ptx::fence_mbar_init();
   }
   if (warp == 2) {
@@ -88,22 +99,13 @@ __global__ void __launch_bounds__(384, 1)
   }
   wait_for_previous();
   let_next_start();
-  const TreeLine line(args, kBN);
+  const TreeLine line(args, kBN, kUnitPlaces);
   if (warp == 0) {
-    int64_t before;
-    const int64_t total = line_total(line, lane, 0, &before);
-    const int ctas = (int)i64min(args.ctas, total);
-    int row = 0;
-    int64_t rest = 0, tiles = 0;
-    if ((int)blockIdx.x < ctas) {
-      const int64_t at = line_bound(blockIdx.x, total, ctas);
-      tiles = line_bound(blockIdx.x + 1, total, ctas) - at;
-      line_find(line, lane, at, &row, &rest);
-    }
+    LinePlace ends[2];
+    line_share(line, lane, blockIdx.x, args.ctas, ends);
     if (lane == 0) {
-      bars->row = row;
-      bars->rest = rest;
-      bars->tiles = fault_set(args.fault) ? 0 : tiles;
+      bars->from = ends[0];
+      bars->tiles = fault_set(args.fault) ? 0 : ends[1].tiles - ends[0].tiles;
     }
   }
   ptx::tc_fence_before();
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t tmem = bars->tmem_base;
   const int64_t n_tiles = bars->tiles;
   LineWalk walk;
-  walk.start(bars->row, bars->rest, n_tiles, line);
+  walk.start(bars->from, n_tiles, line);
 
   if (warp < 4) {
     // 4 x 32 x 80 + 8 x 32 x 208 = 63488 of the 64512 registers of the launch
@@ -122,34 +124,42 @@ __global__ void __launch_bounds__(384, 1)
       if (lane == 0 && n_tiles > 0) {
         ptx::prefetch_tensormap(&tm_k);
         ptx::prefetch_tensormap(&tm_v);
-        LineWalk of[2] = {walk, walk};  // K is two tiles ahead of V
-        int j[2] = {0, 0};
-        int64_t f = 0;
-        auto load = [&](int which) -> bool {
-          LineWalk& w = of[which];
-          if (j[which] == w.count) {
-            if (!w.next(line)) return true;  // no tile left
-            j[which] = 0;
+        // K is a tile ahead of V: they walk along the share by themselves.
+        struct Stream {
+          LineWalk walk;
+          int j, sink_tiles, skip, hk;
+        } of[2] = {{walk, 0, 0, 0, 0}, {walk, 0, 0, 0, 0}};
+        int slot = 0, fills = 0;
+        uint32_t phase = 1;  // of kv_empty: the ring's first round finds every slot free
+        auto load = [&](Stream& w, const CUtensorMap* map) -> bool {
+          if (w.j == w.walk.count) {
+            if (!w.walk.next(line)) return true;  // no tile left
+            const int len = tree_len(p, w.walk.b);
+            const WindowTiles wt(args.win, (int64_t)len - p.q_len, len, kBN);
+            w.j = 0;
+            w.sink_tiles = wt.sink_tiles;
+            w.skip = wt.skip;
+            w.hk = w.walk.unit / args.row_tiles;
           }
-          const int s = (int)(f % S);
-          if (f >= S && !wait_bar(&bars->kv_empty[s], (uint32_t)((f / S) - 1) & 1, args.fault, FAULT_FWD_EMPTY))
-            return false;
-          const int len = tree_len(p, w.b);
-          const WindowTiles wt(args.win, (int64_t)len - p.q_len, len, kBN);
-          const int key = wt.tile(w.first + j[which]) * kBN, hk = w.unit / args.row_tiles;
-          ptx::mbar_expect_tx(&bars->kv_full[s], C::kTileBytes);
+          if (fills >= S && !wait_bar(&bars->kv_empty[slot], phase, args.fault, FAULT_FWD_EMPTY)) return false;
+          const int t = w.walk.first + w.j, key = (t < w.sink_tiles ? t : t + w.skip) * kBN;
+          ptx::mbar_expect_tx(&bars->kv_full[slot], C::kTileBytes);
           for (int sl = 0; sl < C::kSlabs; ++sl)
-            ptx::tma_load_4d(sKV + s * C::kTileBytes + sl * kSlabBytes, which ? &tm_v : &tm_k, 64 * sl, key, hk, w.b,
-                             &bars->kv_full[s]);
-          ++j[which];
-          ++f;
+            ptx::tma_load_4d(sKV + slot * C::kTileBytes + sl * kSlabBytes, map, 64 * sl, key, w.hk, w.walk.b,
+                             &bars->kv_full[slot]);
+          ++w.j;
+          fills = min(fills + 1, S);
+          if (++slot == S) slot = 0, phase ^= 1;
           return true;
         };
-        bool ok = load(0) && load(0);
-        for (int64_t i = 0; i < n_tiles && ok; ++i) ok = load(1) && load(0);
-        // Every issued copy must have landed before shared memory is released.
-        for (int64_t g = i64max(0, f - S); g < f; ++g)
-          (void)wait_bar(&bars->kv_full[g % S], (uint32_t)(g / S) & 1, nullptr, FAULT_FWD_DRAIN);
+        bool ok = load(of[0], &tm_k);
+        for (int64_t i = 0; i < n_tiles && ok; ++i) ok = load(of[0], &tm_k) && load(of[1], &tm_v);
+        // Every issued copy must have landed before shared memory is released.  kv_full's phase of a round is the
+        // opposite of kv_empty's for the round before; slots before `slot` were filled in the present round.
+        for (int s = 0; s < S; ++s) {
+          const uint32_t round = s < slot ? phase ^ 1 : phase;
+          if (s < slot || fills == S) (void)wait_bar(&bars->kv_full[s], round, nullptr, FAULT_FWD_DRAIN);
+        }
       }
     } else if (warp == 1) {
       // ---------------------------- MMA issuer ----------------------------
@@ -159,7 +169,12 @@ __global__ void __launch_bounds__(384, 1)
         const uint32_t aQ = ptx::smem_u32(sQ), aKV = ptx::smem_u32(sKV);
         LineWalk ws = walk, wp = walk;  // of the next S and the next P.V
         int js = 0, jp = 0, seg = -1;   // tiles of their segments done; the S segment's number
-        int64_t f = 0, is = 0, ip = 0;  // ring fills used, tiles done
+        uint32_t is = 0, ip = 0;        // tiles done (their lowest bits count)
+        int s = 0;                      // the ring's next slot
+        uint32_t round = 0;
+        auto used = [&] {
+          if (++s == S) s = 0, round ^= 1;
+        };
         auto issue_s = [&]() -> bool {
           if (js == ws.count) {
             if (!ws.next(line)) return true;
@@ -167,47 +182,48 @@ __global__ void __launch_bounds__(384, 1)
             ++seg;
             if (!wait_bar(&bars->q_full[seg & 1], (uint32_t)(seg >> 1) & 1, args.fault, FAULT_FWD_Q)) return false;
           }
-          const int s = (int)(f % S);
-          if (!wait_bar(&bars->kv_full[s], (uint32_t)(f / S) & 1, args.fault, FAULT_FWD_KV)) return false;
+          if (!wait_bar(&bars->kv_full[s], round, args.fault, FAULT_FWD_KV)) return false;
           ptx::tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kSlabBytes + (kk & 3) * 32;
-            ptx::mma_f16_ss(tmem + C::kColS + (uint32_t)(is & 1) * kBN,
-                            ptx::sw128_desc(aQ + (seg & 1) * C::kTileBytes + off, 16, 1024),
-                            ptx::sw128_desc(aKV + s * C::kTileBytes + off, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            ptx::mma_f16_ss(
+                tmem + C::kColS + (is & 1) * kBN,
+                ptx::sw128_desc(aQ + ((seg & 1) * C::kSlabs + (kk >> 2)) * q_slab + (kk & 3) * 32, 16, 1024),
+                ptx::sw128_desc(aKV + s * C::kTileBytes + (kk >> 2) * kSlabBytes + (kk & 3) * 32, 16, 1024), idesc_qk,
+                kk > 0 ? 1u : 0u);
           ptx::mma_commit(&bars->s_full[is & 1]);
           ptx::mma_commit(&bars->kv_empty[s]);
           if (++js == ws.count) ptx::mma_commit(&bars->q_empty[seg & 1]);
-          ++f;
+          used();
           ++is;
           return true;
         };
+        // P(i) V(i), the two halves of the tile's keys into their own accumulators.
         auto issue_pv = [&]() -> bool {
           if (jp == wp.count) {
             wp.next(line);
             jp = 0;
           }
-          const int t = (int)(ip & 1), s = (int)(f % S);
-          if (!wait_bar(&bars->kv_full[s], (uint32_t)(f / S) & 1, args.fault, FAULT_FWD_KV) ||
-              !wait_bar(&bars->p_full[t], (uint32_t)(ip >> 1) & 1, args.fault, FAULT_FWD_P))
-            return false;
-          ptx::tc_fence_after();
+          if (!wait_bar(&bars->kv_full[s], round, args.fault, FAULT_FWD_KV)) return false;
+          for (int t = 0; t < 2; ++t) {
+            if (!wait_bar(&bars->p_full[t], ip & 1, args.fault, FAULT_FWD_P)) return false;
+            ptx::tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < kBN / 16; ++kk)
-            ptx::mma_f16_ts(tmem + C::kColO + (uint32_t)t * D, tmem + C::kColS + (uint32_t)t * kBN + 8 * kk,
-                            ptx::sw128_desc(aKV + s * C::kTileBytes + kk * 16 * 128, kSlabBytes, 1024), idesc_pv,
-                            (jp >= 2 || kk > 0) ? 1u : 0u);  // a segment's first tile of each group starts O_t
+            for (int kk = 0; kk < kHalf / 16; ++kk)
+              ptx::mma_f16_ts(tmem + C::kColO + (uint32_t)t * D,
+                              tmem + C::kColS + (ip & 1) * kBN + t * kHalf + 8 * kk,
+                              ptx::sw128_desc(aKV + s * C::kTileBytes + (t * kHalf + kk * 16) * 128, kSlabBytes, 1024),
+                              idesc_pv, (jp > 0 || kk > 0) ? 1u : 0u);  // a segment's first tile starts O_t
+            ptx::mma_commit(&bars->o_done[t]);
+          }
           ptx::mma_commit(&bars->kv_empty[s]);
-          if (jp + 2 >= wp.count) ptx::mma_commit(&bars->o_done[t]);
           ++jp;
-          ++f;
+          used();
           ++ip;
           return true;
         };
-        bool ok = issue_s() && issue_s();
-        for (int64_t i = 0; i < n_tiles && ok; ++i) ok = issue_pv() && issue_s();
+        bool ok = issue_s();
+        for (int64_t i = 0; i < n_tiles && ok; ++i) ok = issue_s() && issue_pv();
         ptx::mma_commit(&bars->drain);
         (void)wait_bar(&bars->drain, 0, nullptr, FAULT_FWD_DRAIN);
         if (!ok) record_fault(args.fault, FAULT_FWD_P);
@@ -223,27 +239,19 @@ __global__ void __launch_bounds__(384, 1)
                                                           args.fault, FAULT_FWD_EMPTY)))
           break;
         const int hk = walk.unit / args.row_tiles, r0 = walk.unit % args.row_tiles * kBM;
-        unsigned char* dst = sQ + (seg & 1) * C::kTileBytes;
-        constexpr int kBatch = 8;  // loads in flight a thread
-        for (int i0 = threadIdx.x - 64; i0 < kBM * kChunks; i0 += 64 * kBatch) {
-          uint4 v[kBatch];
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + 64 * u, r = i / kChunks, c = i % kChunks;
-            v[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r0 + r < args.rows && 8 * c < p.head_dim) {
-              const int h = hk * group + (r0 + r) / p.q_len, node = (r0 + r) % p.q_len;
-              v[u] = *reinterpret_cast<const uint4*>(q + (int64_t)walk.b * p.q.stride[0] +
-                                                     (int64_t)h * p.q.stride[1] + (int64_t)node * p.q.stride[2] +
-                                                     8 * c);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + 64 * u, r = i / kChunks, c = i % kChunks;
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * kSlabBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[u];
-          }
+        unsigned char* dst = sQ + (seg & 1) * C::kSlabs * q_slab;
+        const int rows = min(kBM, args.rows - r0);  // what the rows behind them give is not used
+        const int c = (threadIdx.x - 64) % kChunks;
+        const T* from = q + (int64_t)walk.b * p.q.stride[0] + (int64_t)(hk * group) * p.q.stride[1] + 8 * c;
+        for (int r = (threadIdx.x - 64) / kChunks; r < rows; r += 64 / kChunks) {
+          unsigned char* to = dst + (c >> 3) * q_slab + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          const int h = (r0 + r) / p.q_len, node = r0 + r - h * p.q_len;
+          if (8 * c < p.head_dim)
+            ptx::copy16_async(to, from + (int64_t)h * p.q.stride[1] + (int64_t)node * p.q.stride[2]);
+          else
+            *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
         }
+        ptx::copies_done();
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars->q_full[seg & 1]);
@@ -252,83 +260,82 @@ __global__ void __launch_bounds__(384, 1)
   } else {
     // ------------------------- softmax warpgroups --------------------------
     ptx::setmaxnreg_inc<208>();
-    const int t = (warp - 4) >> 2;
+    const int t = (warp - 4) >> 2;  // half of a tile's keys
     const int row = (warp & 3) * 32 + lane;
     const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t col_s = C::kColS + (uint32_t)t * kBN;
     const uint32_t col_o = C::kColO + (uint32_t)t * D;
     const float qk_scale = (float)p.scale * kLog2e;
-    int64_t i0 = 0;      // tiles of the share before this segment
-    uint32_t done = 0;   // segments in which this group had a tile
+    int64_t i = 0;  // tile of the share
+    NodeView view;
+    int view_b = -1, view_r0 = -1;
     bool ok = true;
-    while (ok && walk.next(line)) {
+    for (int seg = 0; ok && walk.next(line); ++seg) {
       const int r0 = walk.unit % args.row_tiles * kBM, b = walk.b;
       const int len = tree_len(p, b);
       const int64_t base = (int64_t)len - p.q_len;
       const WindowTiles wt(args.win, base, len, kBN);
       const bool live_warp = r0 + (warp & 3) * 32 < args.rows;  // some row of the warp is a query's
       const bool live = r0 + row < args.rows;
-      const int32_t* parents = args.parents + b * args.parents_stride;
-      NodeView view = tree_node((r0 + row) % p.q_len, base, !args.parents, args.win,
-                                [&](int i) { return parents[i]; });
-      if (!live) {
-        view.end = 0;
-        view.drafted = 0;
+      if (b != view_b || r0 != view_r0) {  // the heads of a row share it
+        view = tree_node_of_warp((r0 + row) % p.q_len, p.q_len, base, args, b, lane);
+        if (!live) {
+          view.end = 0;
+          view.drafted = 0;
+        }
+        view_b = b;
+        view_r0 = r0;
       }
       float m_run = -INFINITY, l_run = 0.f;
-      const int j0 = (int)((t - i0) & 1);  // this group's first tile of the segment
-      for (int j = j0; j < walk.count; j += 2) {
-        const int64_t i = i0 + j;
-        if (!__all_sync(0xffffffffu, wait_bar(&bars->s_full[t], (uint32_t)(i >> 1) & 1, args.fault, FAULT_FWD_S))) {
+      for (int j = 0; j < walk.count; ++j, ++i) {
+        const uint32_t t_s = t_row + C::kColS + (uint32_t)(i & 1) * kBN + t * kHalf;
+        if (!__all_sync(0xffffffffu, wait_bar(&bars->s_full[i & 1], (uint32_t)(i >> 1) & 1, args.fault, FAULT_FWD_S))) {
           ok = false;
           break;
         }
         ptx::tc_fence_after();
-        const int k0 = wt.tile(walk.first + j) * kBN;
+        const int k0 = wt.tile(walk.first + j) * kBN, kh = k0 + t * kHalf;
+        bool rescale = false;
+        float factor = 1.f;
         if (live_warp) {
-          uint32_t r[kBN];
+          uint32_t r[kHalf];
 #pragma unroll
-          for (int c = 0; c < kBN / 32; ++c)
-            ptx::tmem_ld32(t_row + col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
+          for (int c = 0; c < kHalf / 32; ++c)
+            ptx::tmem_ld32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
           ptx::tmem_wait_ld();
-          // Only tiles with drafted tokens, the cache's end, or an edge of some node's window are masked.
-          const bool need_mask = k0 + kBN > base || (args.win.window > 0 && k0 + kBN > args.win.sinks &&
-                                                     (int64_t)k0 <= (int64_t)len - 1 - args.win.window);
-          uint32_t seen[4];
+          // Only halves with drafted tokens, the cache's end, or an edge of some node's window are masked.
+          const bool need_mask = kh + kHalf > base || (args.win.window > 0 && kh + kHalf > args.win.sinks &&
+                                                       (int64_t)kh <= (int64_t)len - 1 - args.win.window);
+          uint32_t seen[2];
           float mx = -INFINITY;
           if (!need_mask) {
-            float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+            float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kBN; c += 8) {
+            for (int c = 0; c < kHalf; c += 4) {
               m0 = ptx::max3(m0, __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
               m1 = ptx::max3(m1, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
-              m2 = ptx::max3(m2, __uint_as_float(r[c + 4]), __uint_as_float(r[c + 5]));
-              m3 = ptx::max3(m3, __uint_as_float(r[c + 6]), __uint_as_float(r[c + 7]));
             }
-            mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+            mx = fmaxf(m0, m1);
           } else {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) seen[w] = view_bits(view, base, args.win.sinks, k0 + 32 * w);
+            for (int w = 0; w < 2; ++w) seen[w] = view_bits(view, base, args.win.sinks, kh + 32 * w);
 #pragma unroll
-            for (int c = 0; c < kBN; ++c)
+            for (int c = 0; c < kHalf; ++c)
               if ((seen[c >> 5] >> (c & 31)) & 1u) mx = fmaxf(mx, __uint_as_float(r[c]));
           }
           mx = mx == -INFINITY ? mx : mx * qk_scale;
           const float m_new = fmaxf(m_run, mx);
-          const bool rescale =
-              m_new > m_run + kRescaleThreshold || (m_run == -INFINITY && m_new != -INFINITY);
-          float factor = 1.f;
+          rescale = m_new > m_run + kRescaleThreshold || (m_run == -INFINITY && m_new != -INFINITY);
           if (rescale) {
             factor = m_run == -INFINITY ? 0.f : ptx::ex2(m_run - m_new);
             m_run = m_new;
             l_run *= factor;
           }
           const float safe = m_run == -INFINITY ? 0.f : m_run;
-          uint32_t pk[kBN / 2];
+          uint32_t pk[kHalf / 2];
           uint64_t sum2[2] = {ptx::f2pack(0.f, 0.f), ptx::f2pack(0.f, 0.f)};
           const uint64_t sc2 = ptx::f2pack(qk_scale, qk_scale), ng2 = ptx::f2pack(-safe, -safe);
 #pragma unroll
-          for (int c = 0; c < kBN; c += 2) {
+          for (int c = 0; c < kHalf; c += 2) {
             float x0, x1;
             ptx::f2unpack(ptx::fma2(ptx::f2pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sc2, ng2), x0, x1);
             float p0 = ptx::ex2(x0), p1 = ptx::ex2(x1);
@@ -343,10 +350,19 @@ __global__ void __launch_bounds__(384, 1)
           ptx::f2unpack(sum2[0], a0, a1);
           ptx::f2unpack(sum2[1], b0, b1);
           l_run += (a0 + a1) + (b0 + b1);
-          ptx::tmem_st32(t_row + col_s, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-          ptx::tmem_st32(t_row + col_s + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
-          // S_t(i) was issued behind the group's last P.V, so O_t holds all of them: rescale it in place.
-          if (j > j0 && __any_sync(0xffffffffu, rescale)) {
+          // P over the first half of the scores that this thread has read.
+          ptx::tmem_st32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+        }
+        // O_t holds the products up to the tile before once those have completed.  Warps without a live row wait as
+        // well: S is a tile ahead, and what they say of one tile must not count for the tile before.
+        if (j > 0 && !__all_sync(0xffffffffu,
+                                 wait_bar(&bars->o_done[t], (uint32_t)(i - 1) & 1, args.fault, FAULT_FWD_O))) {
+          ok = false;
+          break;
+        }
+        if (live_warp) {
+          if (j > 0 && __any_sync(0xffffffffu, rescale)) {
+            ptx::tc_fence_after();
             if (!rescale) factor = 1.f;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -360,7 +376,7 @@ __global__ void __launch_bounds__(384, 1)
           }
           ptx::tmem_wait_st();
         }
-        if (k0 + kBN > len) {
+        if (kh + kHalf > len) {
           // The cache may hold anything behind its last key: its values there become zeros, as 0 * NaN is NaN.
           const int64_t f = i64min(2 + 2 * i, 2 * n_tiles - 1);  // the fill that brought this tile's V
           unsigned char* v = sKV + (int)(f % S) * C::kTileBytes;
@@ -369,9 +385,9 @@ __global__ void __launch_bounds__(384, 1)
             ok = false;
             break;
           }
-          const int gone = len - k0;  // first row to clear
-          for (int x = row; x < (kBN - gone) * (D / 8); x += 128) {
-            const int vr = gone + x / (D / 8), c = x % (D / 8);
+          const int gone = max(len - kh, 0);  // first row of the half to clear
+          for (int x = row; x < (kHalf - gone) * (D / 8); x += 128) {
+            const int vr = t * kHalf + gone + x / (D / 8), c = x % (D / 8);
             *reinterpret_cast<uint4*>(v + (c >> 3) * kSlabBytes + vr * 128 + ((c & 7) << 4)) =
                 make_uint4(0u, 0u, 0u, 0u);
           }
@@ -381,34 +397,62 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars->p_full[t]);
       }
-      // The segment's partial result: channel quads of all rows, rows side by side.
-      const bool any = j0 < walk.count;
-      if (ok && any) {
-        ok = __all_sync(0xffffffffu, wait_bar(&bars->o_done[t], done & 1, args.fault, FAULT_FWD_O));
-        ++done;
-      }
-      ptx::tc_fence_after();
-      const int64_t part = 2 * ((int64_t)b * line.units + walk.unit + blockIdx.x) + t;
       // A padded node has taken part in the tiles that need no mask: it has seen nothing.
-      if (live) args.ml[part * args.part_rows + row] = view.depth < 0 ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
-      if (ok && any && live_warp) {
+      if (view.depth < 0) m_run = -INFINITY, l_run = 0.f;
+      // Join the halves: both groups learn the row's reference and sum and their accumulators' factors.
+      if (ok && t == 1) bars->red[row] = make_float2(m_run, l_run);
+      __syncwarp();
+      if (t == 1 && lane == 0) ptx::mbar_arrive(&bars->halves);
+      float own = 0.f, other = 0.f;  // factors of this group's accumulator and of the other one
+      if (t == 0) {
+        ok = __all_sync(0xffffffffu, wait_bar(&bars->halves, (uint32_t)seg & 1, args.fault, FAULT_FWD_O) && ok);
+        const float2 high = bars->red[row];
+        const float m = fmaxf(m_run, high.x), safe = m == -INFINITY ? 0.f : m;
+        own = m_run == -INFINITY ? 0.f : ptx::ex2(m_run - safe);
+        other = high.x == -INFINITY ? 0.f : ptx::ex2(high.x - safe);
+        const int64_t part = (int64_t)b * line.units + walk.unit + blockIdx.x;
+        if (live) args.ml[part * args.part_rows + row] = make_float2(m, own * l_run + other * high.y);
+        bars->red[row] = make_float2(other, own);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars->joined);
+      } else {
+        ok = __all_sync(0xffffffffu, wait_bar(&bars->joined, (uint32_t)seg & 1, args.fault, FAULT_FWD_O) && ok);
+        const float2 factors = bars->red[row];
+        own = factors.x;
+        other = factors.y;
+      }
+      // The segment's partial result: channel quads of all rows, rows side by side; each group half of the channels.
+      if (ok)
+        ok = __all_sync(0xffffffffu,
+                        wait_bar(&bars->o_done[0], (uint32_t)(i - 1) & 1, args.fault, FAULT_FWD_O) &&
+                            wait_bar(&bars->o_done[1], (uint32_t)(i - 1) & 1, args.fault, FAULT_FWD_O));
+      ptx::tc_fence_after();
+      if (ok && live_warp) {
+        const int64_t part = (int64_t)b * line.units + walk.unit + blockIdx.x;
         float4* out = reinterpret_cast<float4*>(args.part + part * args.part_rows * p.head_dim);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld32(t_row + col_o + 32 * c, o);
+        for (int c = 0; c < D / 64; ++c) {
+          const int ch = t * (D / 2) + 32 * c;
+          uint32_t o[32], x[32];
+          ptx::tmem_ld32(t_row + col_o + ch, o);
+          ptx::tmem_ld32(t_row + C::kColO + (uint32_t)(1 - t) * D + ch, x);
           ptx::tmem_wait_ld();
+          auto joined = [&](int e) {  // an accumulator without a key may hold anything
+            const float a = own == 0.f ? 0.f : own * __uint_as_float(o[e]);
+            return other == 0.f ? a : fmaf(other, __uint_as_float(x[e]), a);
+          };
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            if (live && 32 * c + e < p.head_dim)
-              out[(8 * c + e / 4) * args.part_rows + row] =
-                  make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
-                              __uint_as_float(o[e + 3]));
+            if (live && ch + e < p.head_dim)
+              out[((ch + e) / 4) * args.part_rows + row] =
+                  make_float4(joined(e), joined(e + 1), joined(e + 2), joined(e + 3));
         }
       }
-      // The next segment's first P_t must not start O_t over before it is read.
+      // Both groups have read both accumulators before the next segment's first product starts them over.
       ptx::tc_fence_before();
-      i0 += walk.count;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&bars->o_read);
+      ok = __all_sync(0xffffffffu, wait_bar(&bars->o_read, (uint32_t)seg & 1, args.fault, FAULT_FWD_O) && ok);
     }
   }
 
@@ -422,98 +466,170 @@ __global__ void __launch_bounds__(384, 1)
 
 // ---------------------------------------------------------------------------
 // Joining: out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p over the partial
-// results p of a row.  One block a (unit, 8 rows); a thread holds one channel
-// quad of a row over every kSplit-th part.
+// results p of a row.  blockIdx.y takes a share of a unit's (channel quad, row)
+// items, rows fastest; where a share has fewer items than the block threads,
+// several threads take every split-th partial result of an item.
 // ---------------------------------------------------------------------------
 namespace {
-constexpr int kMergeRows = 8, kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kFewParts = 4, kMergeParts = 8;  // partial results in flight a thread
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const __grid_constant__ TreeArgs a, int tile_keys,
-                                                                   int parts_of) {
+__global__ void __launch_bounds__(kMergeThreads)
+    tree_merge_kernel(const __grid_constant__ TreeArgs a, int tile_keys, int start_places, int share) {
   const ts_attn_params& p = a.p;
   __shared__ int64_t s_first, s_total;
+  __shared__ float2 s_row[kBM];  // the reference and 1 / sum of every row
   __shared__ float4 s_sum[kMergeThreads];
-  wait_for_previous();
-  let_next_start();
-  const TreeLine line(a, tile_keys);
+  const TreeLine line(a, tile_keys, start_places, true);
   const int unit = blockIdx.x % line.units, b = blockIdx.x / line.units;
-  const int r0 = unit % a.row_tiles * a.tile_rows, row0 = blockIdx.y * kMergeRows;
-  if (r0 + row0 >= a.rows) return;  // the last row tile is shorter
-  if (threadIdx.x < 32) {
+  const int r0 = unit % a.row_tiles * a.tile_rows, rows = min(a.tile_rows, a.rows - r0);
+  const int quads = part_quads(p), items = rows * quads, first = blockIdx.y * share;
+  if (first >= items) {  // the last row tile is shorter
+    wait_for_previous();
+    return;
+  }
+  const int mine = min(share, items - first);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (warp == 0) {
     int64_t before;
-    const int64_t total = line_total(line, threadIdx.x, b, &before);
-    if (threadIdx.x == 0) {
+    const int64_t total = line_total(line, lane, b, &before);
+    if (lane == 0) {
       s_first = before;
       s_total = total;
     }
   }
   __syncthreads();
   const int n = line.tiles(b);
-  const int64_t total = s_total, at = s_first + (int64_t)unit * n;
+  const int64_t total = s_total, at = s_first + unit * line.places(n) + start_places;  // its first tile's place
   const int ctas = (int)i64min(a.ctas, total);
   int64_t part0 = 0;
   int parts = 0;
   if (n > 0) {
     const int c0 = line_owner(at, total, ctas), c1 = line_owner(at + n - 1, total, ctas);
-    part0 = parts_of * ((int64_t)blockIdx.x + c0);
-    parts = parts_of * (c1 - c0 + 1);
+    part0 = (int64_t)blockIdx.x + c0;
+    parts = c1 - c0 + 1;
   }
-  const int quads = part_quads(p);
-  const int items = min(kMergeRows, a.rows - r0 - row0) * quads;  // (quad, row), rows fastest
-  const int rows = items / quads;
-  const int split = max(1, min(parts, kMergeThreads / max(1, items)));
+  wait_for_previous();
+  let_next_start();
+  const float2* ml = a.ml + part0 * a.part_rows;
   const int hk = unit / a.row_tiles, group = p.q_heads / p.kv_heads;
-  for (int x0 = 0; x0 < items; x0 += kMergeThreads / split) {
-    const int x = x0 + threadIdx.x % (kMergeThreads / split), s = threadIdx.x / (kMergeThreads / split);
-    const bool mine = x < items && s < split;
-    const int row = row0 + (mine ? x % rows : 0), quad = mine ? x / rows : 0;
-    float m = -INFINITY, l = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) {
-      const float2* ml = a.ml + part0 * a.part_rows + row;
-      for (int i = 0; i < parts; ++i) m = fmaxf(m, ml[(int64_t)i * a.part_rows].x);
-      if (m != -INFINITY) {
-        for (int i = 0; i < parts; ++i) {
-          const float2 v = ml[(int64_t)i * a.part_rows];
-          if (v.x == -INFINITY) continue;
-          const float w = ptx::ex2(v.x - m);
-          l += w * v.y;
-          if (i % split != s) continue;
-          const float4 o = reinterpret_cast<const float4*>(
-              a.part)[(part0 + i) * a.part_rows * quads + (int64_t)quad * a.part_rows + row];
-          sum.x += w * o.x;
-          sum.y += w * o.y;
-          sum.z += w * o.z;
-          sum.w += w * o.w;
-        }
-      }
-    }
-    s_sum[threadIdx.x] = sum;
-    __syncthreads();
-    if (mine && s == 0) {
-      for (int i = 1; i < split; ++i) {
-        const float4 o = s_sum[i * (kMergeThreads / split) + threadIdx.x];
-        sum.x += o.x;
-        sum.y += o.y;
-        sum.z += o.z;
-        sum.w += o.w;
-      }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int h = hk * group + (r0 + row) / p.q_len, node = (r0 + row) % p.q_len;
-      T* out = reinterpret_cast<T*>(p.o.data) + (int64_t)b * p.o.stride[0] + (int64_t)h * p.o.stride[1] +
-               (int64_t)node * p.o.stride[2] + (int64_t)(4 * quad) * p.o.stride[3];
-      const float value[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+  const float4* from = reinterpret_cast<const float4*>(a.part) + part0 * a.part_rows * quads;
+  auto write_lse = [&](int row, float m, float l) {
+    const int h = hk * group + (r0 + row) / p.q_len, node = (r0 + row) % p.q_len;
+    reinterpret_cast<float*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
+                                    (int64_t)node * p.lse_stride[2]] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  };
+  // A quad of the output in one store, where its rows lie on such boundaries.
+  const bool whole = p.o.stride[3] == 1 && p.value_dim % 4 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.o.data) / sizeof(T)) | p.o.stride[0] | p.o.stride[1] | p.o.stride[2]) % 4 == 0;
+  auto write = [&](int row, int quad, float4 sum, float inv) {
+    const int h = hk * group + (r0 + row) / p.q_len, node = (r0 + row) % p.q_len;
+    T* out = reinterpret_cast<T*>(p.o.data) + (int64_t)b * p.o.stride[0] + (int64_t)h * p.o.stride[1] +
+             (int64_t)node * p.o.stride[2] + (int64_t)(4 * quad) * p.o.stride[3];
+    alignas(4 * sizeof(T)) const T value[4] = {Elem<T>::from_acc(sum.x * inv), Elem<T>::from_acc(sum.y * inv),
+                                               Elem<T>::from_acc(sum.z * inv), Elem<T>::from_acc(sum.w * inv)};
+    if (whole) {
+      struct alignas(4 * sizeof(T)) Four {
+        T v[4];
+      };
+      *reinterpret_cast<Four*>(out) = *reinterpret_cast<const Four*>(value);
+    } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (4 * quad + e < p.value_dim) out[e * p.o.stride[3]] = Elem<T>::from_acc(value[e]);
-      if (quad == 0 && p.lse)
-        reinterpret_cast<float*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
-                                        (int64_t)node * p.lse_stride[2]] =
-            l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (4 * quad + e < p.value_dim) out[e * p.o.stride[3]] = value[e];
     }
-    __syncthreads();
+  };
+  auto add = [](float4& sum, float w, const float4& o) {
+    if (w == 0.f) return;  // a part that has seen nothing may hold anything
+    sum.x = fmaf(w, o.x, sum.x);
+    sum.y = fmaf(w, o.y, sum.y);
+    sum.z = fmaf(w, o.z, sum.z);
+    sum.w = fmaf(w, o.w, sum.w);
+  };
+  if (parts <= kFewParts) {
+    // Few results: a thread reads all that its item needs at once.
+    for (int x = threadIdx.x; x < mine; x += kMergeThreads) {
+      const int row = (first + x) % rows, quad = (first + x) / rows;
+      float2 v[kFewParts];
+      float4 o[kFewParts], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kFewParts; ++i) {
+        v[i] = make_float2(-INFINITY, 0.f);
+        if (i < parts) {
+          v[i] = ml[i * a.part_rows + row];
+          o[i] = from[(int64_t)i * a.part_rows * quads + (int64_t)quad * a.part_rows + row];
+        }
+      }
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kFewParts; ++i) m = fmaxf(m, v[i].x);
+#pragma unroll
+      for (int i = 0; i < kFewParts; ++i) {
+        const float w = v[i].x == -INFINITY ? 0.f : ptx::ex2(v[i].x - m);
+        l = fmaf(w, v[i].y, l);
+        add(sum, w, o[i]);
+      }
+      write(row, quad, sum, l > 0.f ? 1.f / l : l);  // a sum that is NaN stays one
+      if (quad == 0 && p.lse) write_lse(row, m, l);
+    }
+    return;
+  }
+  // A warp a row, lanes over its results.
+  for (int row = warp; row < rows; row += kMergeThreads / 32) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml[(int64_t)i * a.part_rows + row].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    for (int i = lane; i < parts; i += 32) {
+      const float2 v = ml[(int64_t)i * a.part_rows + row];
+      if (v.x != -INFINITY) l = fmaf(ptx::ex2(v.x - m), v.y, l);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane != 0) continue;
+    s_row[row] = make_float2(m, l > 0.f ? 1.f / l : l);
+    if (blockIdx.y == 0 && p.lse) write_lse(row, m, l);
+  }
+  __syncthreads();
+  const int split = max(1, min(parts, kMergeThreads / mine)), lanes = kMergeThreads / split;
+  for (int x0 = 0; x0 < mine; x0 += lanes) {
+    const int x = x0 + threadIdx.x % lanes, s = threadIdx.x / lanes;
+    const bool live = x < mine && s < split;
+    const int row = live ? (first + x) % rows : 0, quad = live ? (first + x) / rows : 0;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float m = s_row[row].x;
+    if (live && m != -INFINITY) {
+      for (int i0 = s; i0 < parts; i0 += split * kMergeParts) {
+        float4 o[kMergeParts];
+        float w[kMergeParts];
+#pragma unroll
+        for (int u = 0; u < kMergeParts; ++u) {
+          const int i = i0 + u * split;
+          w[u] = 0.f;
+          if (i < parts) {
+            w[u] = ptx::ex2(ml[(int64_t)i * a.part_rows + row].x - m);  // 0 where the part has seen nothing
+            o[u] = from[(int64_t)i * a.part_rows * quads + (int64_t)quad * a.part_rows + row];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kMergeParts; ++u) add(sum, w[u], o[u]);
+      }
+    }
+    if (split > 1) {
+      s_sum[threadIdx.x] = sum;
+      __syncthreads();
+      if (live && s == 0)
+        for (int i = 1; i < split; ++i) {
+          const float4 o = s_sum[i * lanes + threadIdx.x];
+          sum.x += o.x;
+          sum.y += o.y;
+          sum.z += o.z;
+          sum.w += o.w;
+        }
+      __syncthreads();
+    }
+    if (live && s == 0) write(row, quad, sum, s_row[row].y);
   }
 }
 
@@ -546,7 +662,12 @@ bool tc_tree_supported(const ts_attn_params& p) {
   return encode_fn() != nullptr;
 }
 
-TreeArgs tree_args(const ts_attn_params& p, int tile_rows, int ctas, int parts_of, size_t* bytes) {
+// Partial results: segments of the line, one a unit and one more for every border between CTAs.
+static size_t tree_parts(const TreeArgs& a) {
+  return (size_t)a.p.batch * a.p.kv_heads * a.row_tiles + a.ctas;
+}
+
+TreeArgs tree_args(const ts_attn_params& p, int tile_rows, int ctas, size_t* bytes) {
   TreeArgs a = {};
   a.p = p;
   a.rows = p.q_heads / p.kv_heads * p.q_len;
@@ -554,31 +675,30 @@ TreeArgs tree_args(const ts_attn_params& p, int tile_rows, int ctas, int parts_o
   a.row_tiles = ceil_div(a.rows, tile_rows);
   a.part_rows = min(a.rows, tile_rows);
   a.ctas = ctas;
-  // Segments: one a unit, one more for every border between CTAs.
-  const size_t parts = parts_of * ((size_t)p.batch * p.kv_heads * a.row_tiles + ctas);
-  *bytes = parts * a.part_rows * (part_quads(p) * sizeof(float4) + sizeof(float2));
+  *bytes = tree_parts(a) * a.part_rows * (part_quads(p) * sizeof(float4) + sizeof(float2));
   return a;
 }
 
-void tree_place(TreeArgs* a, int parts_of, void* workspace) {
-  const size_t parts = parts_of * ((size_t)a->p.batch * a->p.kv_heads * a->row_tiles + a->ctas);
+void tree_place(TreeArgs* a, void* workspace) {
   a->part = reinterpret_cast<float*>(workspace);
-  a->ml = reinterpret_cast<float2*>(a->part + parts * a->part_rows * part_quads(a->p) * 4);
+  a->ml = reinterpret_cast<float2*>(a->part + tree_parts(*a) * a->part_rows * part_quads(a->p) * 4);
 }
 
 size_t tc_tree_workspace(const ts_attn_params& p) {
   size_t bytes;
-  tree_args(p, kBM, device_sms(), 2, &bytes);
+  tree_args(p, kBM, device_sms(), &bytes);
   return bytes;
 }
 
-cudaError_t tree_merge(const TreeArgs& a, int tile_keys, int parts_of, cudaStream_t st) {
-  const dim3 grid((unsigned)(a.p.batch * a.p.kv_heads * a.row_tiles), (unsigned)ceil_div(a.part_rows, kMergeRows));
+cudaError_t tree_merge(const TreeArgs& a, int tile_keys, int start_places, cudaStream_t st) {
+  // Shares of 64 items at least, and blocks for the SMs two or three times over where there are that many.
+  const int units = a.p.batch * a.p.kv_heads * a.row_tiles, items = a.part_rows * part_quads(a.p);
+  const int share = max(64, ceil_div(items, max(1, 600 / units)));
+  const dim3 grid((unsigned)units, (unsigned)ceil_div(items, share)), block(kMergeThreads);
   switch (a.p.dtype) {
-    case TS_F32: return launch_dependent(tree_merge_kernel<float>, grid, kMergeThreads, 0, st, a, tile_keys, parts_of);
-    case TS_F16: return launch_dependent(tree_merge_kernel<__half>, grid, kMergeThreads, 0, st, a, tile_keys, parts_of);
-    case TS_BF16:
-      return launch_dependent(tree_merge_kernel<__nv_bfloat16>, grid, kMergeThreads, 0, st, a, tile_keys, parts_of);
+    case TS_F32: return launch_dependent(tree_merge_kernel<float>, grid, block, 0, st, a, tile_keys, start_places, share);
+    case TS_F16: return launch_dependent(tree_merge_kernel<__half>, grid, block, 0, st, a, tile_keys, start_places, share);
+    case TS_BF16: return launch_dependent(tree_merge_kernel<__nv_bfloat16>, grid, block, 0, st, a, tile_keys, start_places, share);
   }
   return cudaErrorInvalidValue;
 }
@@ -594,8 +714,8 @@ static cudaError_t launch_tree(const CUtensorMap& mk, const CUtensorMap& mv, con
 cudaError_t tc_tree(const ts_attn_params& p, const int32_t* parents, int64_t parents_stride, const WindowArgs& win,
                     void* workspace, uint32_t* fault, cudaStream_t st) {
   size_t bytes;
-  TreeArgs a = tree_args(p, kBM, device_sms(), 2, &bytes);
-  tree_place(&a, 2, workspace);
+  TreeArgs a = tree_args(p, kBM, device_sms(), &bytes);
+  tree_place(&a, workspace);
   a.parents = parents;
   a.parents_stride = parents_stride;
   a.win = win;
@@ -611,7 +731,7 @@ cudaError_t tc_tree(const ts_attn_params& p, const int32_t* parents, int64_t par
   else
     e = bf ? launch_tree<128, true>(mk, mv, a, st) : launch_tree<128, false>(mk, mv, a, st);
   if (e != cudaSuccess) return e;
-  return tree_merge(a, kBN, 2, st);
+  return tree_merge(a, kBN, kUnitPlaces, st);
 }
 
 }  // namespace tsa

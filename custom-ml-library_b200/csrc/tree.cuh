@@ -33,6 +33,11 @@ __host__ __device__ __forceinline__ int part_quads(const ts_attn_params& p) { re
 __device__ __forceinline__ int tree_len(const ts_attn_params& p, int b) {
   return min(p.kv_len, max(0, p.kv_lens[b]));
 }
+// The same from L2: for a kernel that asks before it has waited for the one in front of it (which has waited for what
+// wrote the lengths).
+__device__ __forceinline__ int tree_len_early(const ts_attn_params& p, int b) {
+  return min(p.kv_len, max(0, __ldcg(p.kv_lens + b)));
+}
 
 // What a node sees: the slots [near, end), those below min(end, sinks), and `drafted`'s bits from slot `base` on.
 struct NodeView {
@@ -83,6 +88,57 @@ __device__ __forceinline__ NodeView tree_node(int node, int64_t base, bool chain
   return v;
 }
 
+// The same for 32 nodes of a row at once, parents by shuffles: lane l holds those of nodes l and l + 32.
+__device__ __forceinline__ NodeView tree_node_of_warp(int node, int nodes, int64_t base, const TreeArgs& a, int b,
+                                                      int lane) {
+  const bool chain = a.parents == nullptr;
+  if (chain) return tree_node(node, base, true, a.win, [](int) { return -1; });
+  const int32_t* parents = a.parents + b * a.parents_stride;
+  const int low = lane < nodes ? parents[lane] : -2, high = lane + 32 < nodes ? parents[lane + 32] : -2;
+  auto up = [&](int i) {  // all lanes
+    const int x = __shfl_sync(0xffffffffu, low, i & 31), y = __shfl_sync(0xffffffffu, high, i & 31);
+    return i < 32 ? x : y;
+  };
+  NodeView v;
+  v.near = v.end = 0;
+  v.drafted = 0;
+  v.depth = -1;
+  uint64_t drafted = 0;
+  int i = node, depth = 0;
+  bool going = base + i >= 0, live = going;
+  while (__any_sync(0xffffffffu, going)) {  // parents come before their children, so this ends
+    const int above = up(i);
+    if (going) {
+      drafted |= 1ull << i;
+      if (above < 0 || above >= i || base + above < 0) {
+        live = above == -1;
+        going = false;
+      } else {
+        i = above;
+        ++depth;
+      }
+    }
+  }
+  if (a.win.window > 0 && __any_sync(0xffffffffu, live)) {
+    const int64_t at = base + depth;
+    drafted = 0;
+    i = node;
+    going = live;
+    for (int d = 0; __any_sync(0xffffffffu, going); ++d) {
+      if (going && (d < a.win.window || at - d < a.win.sinks)) drafted |= 1ull << i;
+      going = going && d < depth;
+      const int above = up(i);
+      if (going) i = max(0, above);
+    }
+    v.near = i64max(0, at + 1 - a.win.window);
+  }
+  if (!live) return v;
+  v.depth = depth;
+  v.end = i64max(0, base);
+  v.drafted = drafted;
+  return v;
+}
+
 // Bits k of [0, 32): the node sees slot `slot` + k.
 __device__ __forceinline__ uint32_t view_bits(const NodeView& v, int64_t base, int sinks, int64_t slot) {
   uint32_t bits = range_bits(v.near, v.end, slot) | range_bits(0, i64min(v.end, sinks), slot);
@@ -92,79 +148,107 @@ __device__ __forceinline__ uint32_t view_bits(const NodeView& v, int64_t base, i
 }
 
 // Units of work, (row b, KV head, row tile), stand in line one behind the other, each with the key tiles that it
-// reads; CTA c takes [c L / G, (c + 1) L / G) of the L tiles.
+// reads and, in front of them, `start` places for what a unit costs by itself (its queries, its epilogue); CTA c takes
+// the places [c L / G, (c + 1) L / G) of L.
 struct TreeLine {
   int batch, units;  // units of a row b
-  int tile;          // keys of a tile
+  int tile, start;   // keys of a tile; places in front of a unit's tiles
+  bool early;
   const ts_attn_params* p;
   WindowArgs win;
-  __device__ __forceinline__ TreeLine(const TreeArgs& a, int tile_keys)
-      : batch(a.p.batch), units(a.p.kv_heads * a.row_tiles), tile(tile_keys), p(&a.p), win(a.win) {}
+  __device__ __forceinline__ TreeLine(const TreeArgs& a, int tile_keys, int start_places, bool asks_early = false)
+      : batch(a.p.batch), units(a.p.kv_heads * a.row_tiles), tile(tile_keys), start(start_places), early(asks_early),
+        p(&a.p), win(a.win) {}
   __device__ __forceinline__ int tiles(int b) const {
-    const int len = tree_len(*p, b);
+    const int len = early ? tree_len_early(*p, b) : tree_len(*p, b);
     return WindowTiles(win, (int64_t)len - p->q_len, len, tile).count(ceil_div(len, tile));
   }
+  // Places of a unit with n tiles: none for rows without a key.
+  __device__ __forceinline__ int64_t places(int n) const { return n > 0 ? n + start : 0; }
 };
 __device__ __forceinline__ int64_t line_bound(int c, int64_t total, int ctas) { return c * total / ctas; }
 __device__ __forceinline__ int line_owner(int64_t at, int64_t total, int ctas) {
   return (int)(((at + 1) * ctas - 1) / total);
 }
 
-// One warp: tiles of all rows' units, and of those before row `b`.
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
+// One warp: the line's places, and those before the units of row `b`.
 __device__ __forceinline__ int64_t line_total(const TreeLine& line, int lane, int b, int64_t* before) {
   int64_t sum = 0, first = 0;
   for (int i = lane; i < line.batch; i += 32) {
-    const int n = line.tiles(i);
+    const int64_t n = line.places(line.tiles(i));
     sum += n;
     if (i < b) first += n;
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    first += __shfl_xor_sync(0xffffffffu, first, off);
-  }
-  *before = first * line.units;
-  return sum * line.units;
+  *before = warp_sum(first) * line.units;
+  return warp_sum(sum) * line.units;
 }
 
-// One warp: the row b, and the place within its tiles, of the line's position `at`.
-__device__ __forceinline__ void line_find(const TreeLine& line, int lane, int64_t at, int* row, int64_t* rest) {
-  int64_t before = 0;
-  for (int b0 = 0; b0 < line.batch; b0 += 32) {
-    const int64_t n = b0 + lane < line.batch ? (int64_t)line.tiles(b0 + lane) * line.units : 0;
-    int64_t up_to = n;
+// A place of the line: the row it belongs to, its place within the row's units, and the tiles in front of it.
+struct LinePlace {
+  int row;
+  int64_t rest, tiles;
+};
+
+// One warp: the two ends of CTA `c`'s share of the line (both at its beginning for a CTA without one).
+__device__ __forceinline__ void line_share(const TreeLine& line, int lane, int c, int max_ctas, LinePlace (&ends)[2]) {
+  const int own = lane < line.batch ? line.tiles(lane) : 0;  // kept for batches of up to 32 rows
+  int64_t total = line.places(own);
+  for (int i = lane + 32; i < line.batch; i += 32) total += line.places(line.tiles(i));
+  total = warp_sum(total) * line.units;
+  const int ctas = (int)i64min(max_ctas, total);
+  ends[0] = ends[1] = LinePlace{0, 0, 0};
+  if (c >= ctas) return;
+  const int64_t at[2] = {line_bound(c, total, ctas), line_bound(c + 1, total, ctas)};
+  int64_t places = 0, tiles = 0;  // in front of this step's rows
+  bool found[2] = {false, false};
+  for (int b0 = 0; b0 < line.batch && !(found[0] && found[1]); b0 += 32) {
+    const int n = b0 == 0 ? own : b0 + lane < line.batch ? line.tiles(b0 + lane) : 0;
+    const int64_t mine = line.places(n) * line.units, mine_tiles = (int64_t)n * line.units;
+    int64_t up_to = mine, up_tiles = mine_tiles;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, up_to, off);
-      if (lane >= off) up_to += other;
+      const int64_t x = __shfl_up_sync(0xffffffffu, up_to, off), y = __shfl_up_sync(0xffffffffu, up_tiles, off);
+      if (lane >= off) up_to += x, up_tiles += y;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + up_to > at);
-    if (past) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      // the row that holds the first place, and the last one
+      const uint32_t past = __ballot_sync(0xffffffffu, places + up_to > at[e] - e);
+      if (found[e] || !past) continue;
       const int l = __ffs(past) - 1;
-      *row = b0 + l;
-      *rest = at - before - __shfl_sync(0xffffffffu, up_to - n, l);
-      return;
+      found[e] = true;
+      const int64_t rest = at[e] - places - __shfl_sync(0xffffffffu, up_to - mine, l);
+      const int of = __shfl_sync(0xffffffffu, n, l);
+      const int64_t unit = rest / line.places(of), in_unit = rest % line.places(of);
+      ends[e] = LinePlace{b0 + l, rest,
+                          tiles + __shfl_sync(0xffffffffu, up_tiles - mine_tiles, l) + unit * of +
+                              i64max(0, in_unit - line.start)};
     }
-    before += __shfl_sync(0xffffffffu, up_to, 31);
+    places += __shfl_sync(0xffffffffu, up_to, 31);
+    tiles += __shfl_sync(0xffffffffu, up_tiles, 31);
   }
-  *row = line.batch;
-  *rest = 0;
 }
 
-// A CTA's walk along its part of the line, segment by segment (one unit each).
+// A CTA's walk along its tiles, segment by segment (one unit each).
 struct LineWalk {
   int b, unit, first;  // of the present segment: row, unit of the row, first tile of the unit's list
   int count;           // its tiles; 0 before the first segment
   int64_t left;        // tiles behind it
-  __device__ __forceinline__ void start(int row, int64_t rest, int64_t tiles, const TreeLine& line) {
-    b = row;
+  __device__ __forceinline__ void start(const LinePlace& from, int64_t tiles, const TreeLine& line) {
+    b = from.row;
     count = 0;
     left = tiles;
     unit = first = 0;
     if (tiles > 0) {
-      const int n = line.tiles(row);
-      unit = (int)(rest / n);
-      first = (int)(rest % n);
+      const int64_t size = line.places(line.tiles(b));
+      unit = (int)(from.rest / size);
+      first = (int)i64max(0, from.rest % size - line.start);
     }
   }
   __device__ __forceinline__ bool next(const TreeLine& line) {
@@ -185,12 +269,12 @@ struct LineWalk {
   }
 };
 
-// Row tiles of `tile_rows` rows, partial results for `parts_of` a segment in a workspace of *bytes.
-TreeArgs tree_args(const ts_attn_params& p, int tile_rows, int ctas, int parts_of, size_t* bytes);
+// Row tiles of `tile_rows` rows, with partial results in a workspace of *bytes.
+TreeArgs tree_args(const ts_attn_params& p, int tile_rows, int ctas, size_t* bytes);
 // Where a workspace holds them.
-void tree_place(TreeArgs* a, int parts_of, void* workspace);
+void tree_place(TreeArgs* a, void* workspace);
 // Joins the partial results of a line of work over tiles of `tile_keys` keys.
-cudaError_t tree_merge(const TreeArgs& a, int tile_keys, int parts_of, cudaStream_t st);
+cudaError_t tree_merge(const TreeArgs& a, int tile_keys, int start_places, cudaStream_t st);
 
 // attn_tree.cu: half types on the tensor cores.
 bool tc_tree_supported(const ts_attn_params& p);
