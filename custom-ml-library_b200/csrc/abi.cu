@@ -635,8 +635,16 @@ int check_window_bwd(const ts_attn_bwd_params* bp, const ts_window* w) {
     return TS_ERR_UNSUPPORTED;
   return TS_OK;
 }
-size_t window_bwd_workspace(const ts_attn_bwd_params& bp) {
-  return tsa::tc_bwd_window_supported(bp) ? tsa::tc_bwd_workspace(bp) : tsa::simt_backward_workspace(bp);
+cudaError_t rows_window_bwd(const ts_attn_bwd_params& bp, const tsa::WindowArgs& win, size_t* bytes, void* ws,
+                            cudaStream_t st) {
+  return by_dtype(bp.fwd.dtype, tsa::rows_window_bwd_f32, tsa::rows_window_bwd_f64, tsa::rows_window_bwd_f16,
+                  tsa::rows_window_bwd_bf16, bp, win, bytes, ws, st);
+}
+size_t window_bwd_workspace(const ts_attn_bwd_params& bp, const tsa::WindowArgs& win) {
+  if (tsa::tc_bwd_window_supported(bp)) return tsa::tc_bwd_workspace(bp);
+  size_t bytes = 0;
+  (void)rows_window_bwd(bp, win, &bytes, nullptr, nullptr);
+  return bytes;
 }
 
 int check_tree(const ts_attn_params* p, const ts_tree* t) {
@@ -685,22 +693,21 @@ int ts_attn_fwd_window(const ts_attn_params* p, const ts_window* w, void* stream
 }
 
 size_t ts_attn_bwd_window_workspace_size(const ts_attn_bwd_params* bp, const ts_window* w) {
-  return check_window_bwd(bp, w) == TS_OK ? window_bwd_workspace(*bp) : 0;
+  return check_window_bwd(bp, w) == TS_OK ? window_bwd_workspace(*bp, window_args(w)) : 0;
 }
 
 int ts_attn_bwd_window(const ts_attn_bwd_params* bp, const ts_window* w, void* workspace, size_t workspace_bytes,
                        void* stream) {
   const int st = check_window_bwd(bp, w);
   if (st != TS_OK) return st;
-  if (!workspace || workspace_bytes < window_bwd_workspace(*bp) || reinterpret_cast<uintptr_t>(workspace) % 16)
-    return TS_ERR_WORKSPACE;
   const tsa::WindowArgs win = window_args(w);
+  if (!workspace || workspace_bytes < window_bwd_workspace(*bp, win) || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return TS_ERR_WORKSPACE;
   if (tsa::tc_bwd_window_supported(*bp))
     return from_cuda(
         tsa::tc_backward(*bp, workspace, workspace_bytes, fault_ptr(), as_stream(stream), nullptr, &win));
-  return from_cuda(by_dtype(bp->fwd.dtype, tsa::rows_window_bwd_f32, tsa::rows_window_bwd_f64,
-                            tsa::rows_window_bwd_f16, tsa::rows_window_bwd_bf16, *bp, win, workspace,
-                            as_stream(stream)));
+  size_t bytes;
+  return from_cuda(rows_window_bwd(*bp, win, &bytes, workspace, as_stream(stream)));
 }
 
 int ts_attn_tree_path(const ts_attn_params* p, const ts_tree* t) {

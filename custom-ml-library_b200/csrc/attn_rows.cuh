@@ -2,11 +2,12 @@
 // cache: fp32 and fp64, and the half-type problems that the tensor-core kernels leave (head dimensions above 128 or
 // not a multiple of 8, Dv != D, strides that TMA cannot address, a scale that is not positive).
 //
-// A block of 128 threads holds R = 16 RT rows and walks over tiles of 32 columns, both in shared memory.  Thread
+// A block of 128 threads holds R = 16 RT rows and walks over tiles of 8 NC columns, both in shared memory.  Thread
 // (ty, tx) owns rows ty + 16 r and columns tx + 8 k of the products, and channels 4 (tx + 8 c) of the accumulators, so
-// that RT + 4 (products) and RT + DC (accumulators) 16-byte reads feed 16 RT and 4 RT DC multiply-adds.  The arithmetic
-// is exact in the accumulation type (fp32, or fp64 for fp64), exponentials in base 2.
-// Which columns a row sees is one 32-bit word a row and tile (tree.cuh, window.cuh).
+// that RT + NC (products) and RT + 4 DC (accumulators, four columns) 16-byte reads feed 4 RT NC and 16 RT DC
+// multiply-adds.  In fp32 the next operand is on its way (cp.async) while this one is multiplied.  The arithmetic is
+// exact in the accumulation type (fp32, or fp64 for fp64), exponentials in base 2.
+// Which columns a row sees is a 32-bit word a row and 32 columns (tree.cuh, window.cuh).
 #pragma once
 #include "dependent.cuh"
 #include "simt_kernels.cuh"
@@ -15,7 +16,7 @@
 
 namespace tsa {
 
-constexpr int kRowsThreads = 128, kRowsCols = 32, kRowsPad = 4;
+constexpr int kRowsThreads = 128, kRowsPad = 4;
 constexpr double kLog2eD = 1.4426950408889634, kLn2D = 0.6931471805599453;
 
 __device__ __forceinline__ float acc_exp2(float x) { return exp2f(x); }
@@ -39,8 +40,13 @@ __device__ __forceinline__ Quad<A> quad(const A* p) {
   return q;
 }
 
+__device__ __forceinline__ void copy_row16(void* dst, const void* src, bool live) {  // zeros where it is not live
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(live ? 16 : 0)
+               : "memory");
+}
+
 // Rows [t0, t0 + rows) of (b, h) into shared memory, a row every `stride` elements; zeros at and behind row `end` and
-// channel C (to a whole quad).
+// channel C (to a whole quad).  fp32 rows on 16-byte boundaries are under way when it returns (ptx::copies_done).
 template <typename T, typename A>
 __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& src, int b, int h, int64_t t0, int rows,
                                            int64_t end, int C) {
@@ -50,6 +56,14 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
                    reinterpret_cast<uintptr_t>(base) % 16 == 0;
   if (vec) {
     const int per = C / kVec, n = rows * per;
+    if constexpr (sizeof(T) == 4) {
+      for (int x = threadIdx.x; x < n; x += kRowsThreads) {
+        const int r = x / per, c = x - r * per;
+        const bool live = t0 + r < end;
+        copy_row16(dst + r * stride + c * kVec, live ? base + (t0 + r) * src.stride[2] + c * kVec : base, live);
+      }
+      return;
+    }
     constexpr int kBatch = 4;
     for (int x0 = threadIdx.x; x0 < n; x0 += kRowsThreads * kBatch) {
       uint4 raw[kBatch];
@@ -71,11 +85,20 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
     }
     return;
   }
-  const int wide = ceil_div(C, 4) * 4;
-  for (int x = threadIdx.x; x < rows * wide; x += kRowsThreads) {
-    const int r = x / wide, c = x % wide;
-    dst[r * stride + c] = c < C && t0 + r < end ? Elem<T>::to_acc(base[(t0 + r) * src.stride[2] + c * src.stride[3]])
-                                                : A(0);
+  const int wide = ceil_div(C, 4) * 4, n = rows * wide;
+  constexpr int kBatch = 8;
+  for (int x0 = threadIdx.x; x0 < n; x0 += kRowsThreads * kBatch) {
+    T raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int x = x0 + u * kRowsThreads, r = x / wide, c = x % wide;
+      raw[u] = x < n && c < C && t0 + r < end ? base[(t0 + r) * src.stride[2] + c * src.stride[3]] : Elem<T>::from_acc(A(0));
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int x = x0 + u * kRowsThreads;
+      if (x < n) dst[x / wide * stride + x % wide] = Elem<T>::to_acc(raw[u]);
+    }
   }
 }
 
@@ -123,36 +146,36 @@ __device__ __forceinline__ void stage_packed(A* dst, int stride, const ts_view4&
 }
 
 // acc[r][k] = sum_c rows[ty + 16 r][c] cols[tx + 8 k][c].
-template <int RT, typename A>
-__device__ __forceinline__ void dots(A (&acc)[RT][4], const A* rows, const A* cols, int stride, int C, int ty, int tx) {
+template <int RT, int NC, typename A>
+__device__ __forceinline__ void dots(A (&acc)[RT][NC], const A* rows, const A* cols, int stride, int C, int ty, int tx) {
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[r][k] = A(0);
+    for (int k = 0; k < NC; ++k) acc[r][k] = A(0);
 #pragma unroll 2
   for (int c = 0; c < C; c += 4) {
-    Quad<A> a[RT], b[4];
+    Quad<A> a[RT], b[NC];
 #pragma unroll
     for (int r = 0; r < RT; ++r) a[r] = quad(rows + (ty + 16 * r) * stride + c);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) b[k] = quad(cols + (tx + 8 * k) * stride + c);
+    for (int k = 0; k < NC; ++k) b[k] = quad(cols + (tx + 8 * k) * stride + c);
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[r][k] += a[r].v[e] * b[k].v[e];
+        for (int k = 0; k < NC; ++k) acc[r][k] += a[r].v[e] * b[k].v[e];
   }
 }
 
-// acc[r][c] += sum_j w[ty + 16 r][j] cols[j][4 (tx + 8 c) ..]; w has kRowsCols + kRowsPad elements a row.
-template <int RT, int DC, typename A>
+// acc[r][c] += sum_j w[ty + 16 r][j] cols[j][4 (tx + 8 c) ..]; w has 8 NC + kRowsPad elements a row.
+template <int RT, int NC, int DC, typename A>
 __device__ __forceinline__ void accumulate(A (&acc)[RT][DC][4], const A* w, const A* cols, int stride, int ty, int tx) {
 #pragma unroll 2
-  for (int j = 0; j < kRowsCols; j += 4) {
+  for (int j = 0; j < 8 * NC; j += 4) {
     Quad<A> p[RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) p[r] = quad(w + (ty + 16 * r) * (kRowsCols + kRowsPad) + j);
+    for (int r = 0; r < RT; ++r) p[r] = quad(w + (ty + 16 * r) * (8 * NC + kRowsPad) + j);
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
@@ -195,16 +218,21 @@ __device__ __forceinline__ A lanes8_max(A x) {
 template <typename A, int RT, int DC> struct RowsCfg {
   static constexpr int kRows = 16 * RT;
   static constexpr int kStride = 32 * DC + kRowsPad;
-  static constexpr size_t kFwdSmem = sizeof(A) * ((kRows + 2 * kRowsCols) * kStride + kRows * (kRowsCols + kRowsPad));
-  // rows' two operands, the tile's two, P and dS
-  static constexpr size_t kBwdSmem =
-      sizeof(A) * ((2 * kRows + 2 * kRowsCols) * kStride + 2 * kRows * (kRowsCols + kRowsPad));
+  // Columns of a thread: 8 feed more multiply-adds a read, 4 leave room for a second block where rows are long.
+  static constexpr int kFwdNC = sizeof(A) == 4 && DC == 2 ? 8 : 4, kBwdNC = 4;
+  static constexpr int kFwdCols = 8 * kFwdNC, kBwdCols = 8 * kBwdNC;
+  static constexpr size_t kFwdSmem = sizeof(A) * ((kRows + 2 * kFwdCols) * kStride + kRows * (kFwdCols + kRowsPad));
+  // rows' two operands, the tile's two (twice in fp32, where the next ones are under way), P and dS
+  static constexpr int kBufs = sizeof(A) == 4 ? 2 : 1;
+  static constexpr size_t kBwdSmem = sizeof(A) * ((2 * kRows + 2 * kBufs * kBwdCols) * kStride +
+                                                  2 * kRows * (kBwdCols + kRowsPad));
 };
 
 // The running softmax of R rows over tiles of keys.
 template <typename T, int RT, int DC> struct RowsForward {
   using A = typename Elem<T>::acc;
   using C = RowsCfg<A, RT, DC>;
+  static constexpr int kNC = C::kFwdNC, kCols = C::kFwdCols;
   A acc[RT][DC][4], m[RT], l[RT];
   A *q, *k, *v, *w;
   int ty, tx;
@@ -212,8 +240,8 @@ template <typename T, int RT, int DC> struct RowsForward {
   __device__ __forceinline__ RowsForward(A* smem) {
     q = smem;
     k = q + C::kRows * C::kStride;
-    v = k + kRowsCols * C::kStride;
-    w = v + kRowsCols * C::kStride;
+    v = k + kCols * C::kStride;
+    w = v + kCols * C::kStride;
     ty = threadIdx.x / 8;
     tx = threadIdx.x % 8;
   }
@@ -222,44 +250,53 @@ template <typename T, int RT, int DC> struct RowsForward {
 #pragma unroll
     for (int r = 0; r < RT; ++r) m[r] = neg_inf<A>(), l[r] = A(0);
   }
-  // Keys [k0, k0 + 32) of head hk; bits[r]: what row ty + 16 r sees of them.  Keys at and behind `end` are not read.
-  template <typename Bits>
-  __device__ __forceinline__ void tile(const ts_attn_params& p, int b, int hk, int k0, int end, A scale2, Bits bits) {
-    __syncthreads();  // the tile before is used up
-    stage_tile<T, A>(k, C::kStride, p.k, b, hk, k0, kRowsCols, end, p.head_dim);
-    stage_tile<T, A>(v, C::kStride, p.v, b, hk, k0, kRowsCols, end, p.value_dim);
-    __syncthreads();
-    A s[RT][4];
-    dots<RT>(s, q, k, C::kStride, p.head_dim, ty, tx);
+  // n tiles, tile j at key key_of(j), of head hk; bits(r, slot): what row ty + 16 r sees of the 32 keys from `slot` on.
+  // Keys at and behind `end` are not read.  K of the next tile is under way during P.V, V during Q.K.
+  template <typename Key, typename Bits>
+  __device__ __forceinline__ void run(const ts_attn_params& p, int b, int hk, int n, int end, A scale2, Key key_of,
+                                      Bits bits) {
+    if (n > 0) stage_tile<T, A>(k, C::kStride, p.k, b, hk, key_of(0), kCols, end, p.head_dim);
+    for (int j = 0; j < n; ++j) {
+      const int k0 = key_of(j);
+      ptx::copies_done();
+      __syncthreads();  // K(j) is there, V(j - 1) is used up
+      stage_tile<T, A>(v, C::kStride, p.v, b, hk, k0, kCols, end, p.value_dim);
+      A s[RT][kNC];
+      dots<RT, kNC>(s, q, k, C::kStride, p.head_dim, ty, tx);
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const uint32_t see = bits(r);
-      A top = neg_inf<A>();
+      for (int r = 0; r < RT; ++r) {
+        uint32_t see[kNC / 4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[r][c] = (see >> (tx + 8 * c)) & 1u ? s[r][c] * scale2 : neg_inf<A>();
-        top = s[r][c] > top ? s[r][c] : top;
+        for (int x = 0; x < kNC / 4; ++x) see[x] = bits(r, k0 + 32 * x);
+        A top = neg_inf<A>();
+#pragma unroll
+        for (int c = 0; c < kNC; ++c) {
+          s[r][c] = (see[c / 4] >> (tx + 8 * (c % 4))) & 1u ? s[r][c] * scale2 : neg_inf<A>();
+          top = s[r][c] > top ? s[r][c] : top;
+        }
+        top = lanes8_max(top);
+        const A next = top > m[r] ? top : m[r];
+        const A safe = next == neg_inf<A>() ? A(0) : next;
+        const A factor = acc_exp2(m[r] - safe);
+        A sum = A(0);
+#pragma unroll
+        for (int c = 0; c < kNC; ++c) {
+          const A e = acc_exp2(s[r][c] - safe);
+          w[(ty + 16 * r) * (kCols + kRowsPad) + tx + 8 * c] = e;
+          sum += e;
+        }
+        l[r] = l[r] * factor + lanes8_sum(sum);
+        m[r] = next;
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][c][e] *= factor;
       }
-      top = lanes8_max(top);
-      const A next = top > m[r] ? top : m[r];
-      const A safe = next == neg_inf<A>() ? A(0) : next;
-      const A factor = acc_exp2(m[r] - safe);
-      A sum = A(0);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const A e = acc_exp2(s[r][c] - safe);
-        w[(ty + 16 * r) * (kRowsCols + kRowsPad) + tx + 8 * c] = e;
-        sum += e;
-      }
-      l[r] = l[r] * factor + lanes8_sum(sum);
-      m[r] = next;
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[r][c][e] *= factor;
+      ptx::copies_done();
+      __syncthreads();  // V(j) is there, K(j) is used up
+      if (j + 1 < n) stage_tile<T, A>(k, C::kStride, p.k, b, hk, key_of(j + 1), kCols, end, p.head_dim);
+      accumulate<RT, kNC, DC>(acc, w, v, C::kStride, ty, tx);
     }
-    __syncwarp();  // a row's weights are written and read by one warp
-    accumulate<RT, DC>(acc, w, v, C::kStride, ty, tx);
   }
 };
 
@@ -276,25 +313,23 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_fwd_kernel(const __g
   let_next_start();
   F f(reinterpret_cast<A*>(smem_raw));
   const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.q_heads / p.kv_heads);
-  const int i0 = blockIdx.x * F::C::kRows;
+  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * F::C::kRows;  // the longest rows first
   const int kv_end = a.kv_end(b);
   const int64_t offset = a.offset(b);
   stage_tile<T, A>(f.q, F::C::kStride, p.q, b, h, i0, F::C::kRows, p.q_len, p.head_dim);
   f.start();
   const int64_t last = (int64_t)min(i0 + F::C::kRows, p.q_len) - 1 + offset;
   const int end = (int)i64max(0, i64min(kv_end, last + 1));
-  const WindowTiles wt(a.win, i0 + offset, kv_end, kRowsCols);
-  const int n = wt.count(ceil_div(end, kRowsCols));
+  const WindowTiles wt(a.win, i0 + offset, kv_end, F::kCols);
   const A scale2 = (A)(p.scale * kLog2eD);
-  for (int j = 0; j < n; ++j) {
-    const int k0 = wt.tile(j) * kRowsCols;
-    f.tile(p, b, hk, k0, kv_end, scale2, [&](int r) {
-      const int i = i0 + f.ty + 16 * r;
-      if (i >= p.q_len) return 0u;
-      const int64_t stop = i64min(kv_end, i + offset + 1);
-      return range_bits(i + offset + 1 - a.win.window, stop, k0) | range_bits(0, i64min(stop, a.win.sinks), k0);
-    });
-  }
+  f.run(p, b, hk, wt.count(ceil_div(end, F::kCols)), kv_end, scale2, [&](int j) { return wt.tile(j) * F::kCols; },
+        [&](int r, int slot) {
+          const int i = i0 + f.ty + 16 * r;
+          if (i >= p.q_len) return 0u;
+          const int64_t stop = i64min(kv_end, i + offset + 1);
+          return range_bits(i + offset + 1 - a.win.window, stop, slot) |
+                 range_bits(0, i64min(stop, a.win.sinks), slot);
+        });
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int i = i0 + f.ty + 16 * r;
@@ -330,7 +365,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
   wait_for_previous();
   let_next_start();
   F f(reinterpret_cast<A*>(smem_raw));
-  const TreeLine line(a, kRowsCols, 0);
+  const TreeLine line(a, F::kCols, 0);
   const int group = p.q_heads / p.kv_heads;
   const A scale2 = (A)(p.scale * kLog2eD);
   LineWalk walk;
@@ -352,7 +387,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
     const int b = walk.b, hk = walk.unit / a.row_tiles, r0 = walk.unit % a.row_tiles * F::C::kRows;
     const int len = tree_len(p, b);
     const int64_t base = (int64_t)len - p.q_len;
-    const WindowTiles wt(a.win, base, len, kRowsCols);
+    const WindowTiles wt(a.win, base, len, F::kCols);
     __syncthreads();  // the unit before is used up
     if (a.parents && (int)threadIdx.x < p.q_len) s_parents[threadIdx.x] = a.parents[b * a.parents_stride + threadIdx.x];
     stage_packed<T, A>(f.q, F::C::kStride, p.q, b, hk * group, r0, F::C::kRows, a.rows, p.q_len, p.head_dim);
@@ -365,10 +400,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
       if (i >= a.rows) view[r].end = 0, view[r].drafted = 0;
     }
     f.start();
-    for (int j = 0; j < walk.count; ++j) {
-      const int k0 = wt.tile(walk.first + j) * kRowsCols;
-      f.tile(p, b, hk, k0, len, scale2, [&](int r) { return view_bits(view[r], base, a.win.sinks, k0); });
-    }
+    f.run(p, b, hk, walk.count, len, scale2, [&](int j) { return wt.tile(walk.first + j) * F::kCols; },
+          [&](int r, int slot) { return view_bits(view[r], base, a.win.sinks, slot); });
     const int64_t part = (int64_t)b * line.units + walk.unit + blockIdx.x;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -432,6 +465,12 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) delta[row] = sum;
 }
 
+// Key blocks [first, first + count) whose queries are divided into parts of `queries`, a multiple of a tile.
+struct RowsKeyBlocks {
+  int first, count, parts, queries;
+  void* part;
+};
+
 template <typename A>
 __device__ __forceinline__ A row_lse2(const ts_attn_params& p, int b, int h, int i) {
   const A v = reinterpret_cast<const A*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
@@ -443,19 +482,19 @@ template <typename T, int RT, int DC>
 __global__ void __launch_bounds__(kRowsThreads) rows_window_dq_kernel(const __grid_constant__ RowsWindowBwd a) {
   using A = typename Elem<T>::acc;
   using C = RowsCfg<A, RT, DC>;
+  constexpr int kNC = C::kBwdNC, kCols = C::kBwdCols, kBufs = C::kBufs;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const ts_attn_params& p = a.bp.fwd;
   A* q = reinterpret_cast<A*>(smem_raw);
   A* g = q + C::kRows * C::kStride;
-  A* k = g + C::kRows * C::kStride;
-  A* v = k + kRowsCols * C::kStride;
-  A* w = v + kRowsCols * C::kStride;
+  A* tiles = g + C::kRows * C::kStride;  // K and V, kBufs times
+  A* w = tiles + 2 * kBufs * kCols * C::kStride;
   wait_for_previous();
   let_next_start();
   const RowsWindow rule{p, a.win};
   const int ty = threadIdx.x / 8, tx = threadIdx.x % 8;
   const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.q_heads / p.kv_heads);
-  const int i0 = blockIdx.x * C::kRows;
+  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * C::kRows;  // the longest rows first
   const int kv_end = rule.kv_end(b);
   const int64_t offset = rule.offset(b);
   stage_tile<T, A>(q, C::kStride, p.q, b, h, i0, C::kRows, p.q_len, p.head_dim);
@@ -470,31 +509,41 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_dq_kernel(const __gr
   }
   const int64_t last = (int64_t)min(i0 + C::kRows, p.q_len) - 1 + offset;
   const int end = (int)i64max(0, i64min(kv_end, last + 1));
-  const WindowTiles wt(a.win, i0 + offset, kv_end, kRowsCols);
-  const int n = wt.count(ceil_div(end, kRowsCols));
+  const WindowTiles wt(a.win, i0 + offset, kv_end, kCols);
+  const int n = wt.count(ceil_div(end, kCols));
   const A scale = (A)p.scale, scale2 = (A)(p.scale * kLog2eD);
+  auto stage = [&](int j) {
+    A* k = tiles + j % kBufs * 2 * kCols * C::kStride;
+    stage_tile<T, A>(k, C::kStride, p.k, b, hk, wt.tile(j) * kCols, kCols, kv_end, p.head_dim);
+    stage_tile<T, A>(k + kCols * C::kStride, C::kStride, p.v, b, hk, wt.tile(j) * kCols, kCols, kv_end, p.value_dim);
+  };
+  if (n > 0) stage(0);
   for (int j = 0; j < n; ++j) {
-    const int k0 = wt.tile(j) * kRowsCols;
-    __syncthreads();
-    stage_tile<T, A>(k, C::kStride, p.k, b, hk, k0, kRowsCols, kv_end, p.head_dim);
-    stage_tile<T, A>(v, C::kStride, p.v, b, hk, k0, kRowsCols, kv_end, p.value_dim);
-    __syncthreads();
-    A s[RT][4], d[RT][4];
-    dots<RT>(s, q, k, C::kStride, p.head_dim, ty, tx);
-    dots<RT>(d, g, v, C::kStride, p.value_dim, ty, tx);
+    const int k0 = wt.tile(j) * kCols;
+    const A* k = tiles + j % kBufs * 2 * kCols * C::kStride;
+    ptx::copies_done();
+    __syncthreads();  // this tile is there, the one before is used up
+    if (kBufs > 1 && j + 1 < n) stage(j + 1);
+    A s[RT][kNC], d[RT][kNC];
+    dots<RT, kNC>(s, q, k, C::kStride, p.head_dim, ty, tx);
+    dots<RT, kNC>(d, g, k + kCols * C::kStride, C::kStride, p.value_dim, ty, tx);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int64_t stop = i64min(kv_end, i0 + ty + 16 * r + offset + 1);
       const uint32_t see = range_bits(i0 + ty + 16 * r + offset + 1 - a.win.window, stop, k0) |
                            range_bits(0, i64min(stop, a.win.sinks), k0);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kNC; ++c) {
         const A pr = (see >> (tx + 8 * c)) & 1u ? acc_exp2(s[r][c] * scale2 - lse2[r]) : A(0);
-        w[(ty + 16 * r) * (kRowsCols + kRowsPad) + tx + 8 * c] = pr * (d[r][c] - delta[r]) * scale;
+        w[(ty + 16 * r) * (kCols + kRowsPad) + tx + 8 * c] = pr * (d[r][c] - delta[r]) * scale;
       }
     }
-    __syncwarp();
-    accumulate<RT, DC>(acc, w, k, C::kStride, ty, tx);
+    __syncwarp();  // a row's weights are written and read by one warp
+    accumulate<RT, kNC, DC>(acc, w, k, C::kStride, ty, tx);
+    if (kBufs == 1 && j + 1 < n) {
+      __syncthreads();
+      stage(j + 1);
+    }
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -510,25 +559,28 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_dq_kernel(const __gr
   }
 }
 
+// Blocks (KV head and row, key block, part of the queries).  With one part dK and dV are written at once; with more,
+// each part leaves its sums in `part` and rows_dkv_sum_kernel adds them in order.
 template <typename T, int RT, int DC>
-__global__ void __launch_bounds__(kRowsThreads) rows_window_dkv_kernel(const __grid_constant__ RowsWindowBwd a) {
+__global__ void __launch_bounds__(kRowsThreads)
+    rows_window_dkv_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks) {
   using A = typename Elem<T>::acc;
   using C = RowsCfg<A, RT, DC>;
+  constexpr int kNC = C::kBwdNC, kCols = C::kBwdCols, kBufs = C::kBufs;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ A s_lse2[kRowsCols], s_delta[kRowsCols];
+  __shared__ A s_lse2[kBufs][kCols], s_delta[kBufs][kCols];
   const ts_attn_params& p = a.bp.fwd;
   A* k = reinterpret_cast<A*>(smem_raw);
   A* v = k + C::kRows * C::kStride;
-  A* q = v + C::kRows * C::kStride;
-  A* g = q + kRowsCols * C::kStride;
-  A* wp = g + kRowsCols * C::kStride;
-  A* ws = wp + C::kRows * (kRowsCols + kRowsPad);
+  A* tiles = v + C::kRows * C::kStride;  // Q and dO, kBufs times
+  A* wp = tiles + 2 * kBufs * kCols * C::kStride;
+  A* ws = wp + C::kRows * (kCols + kRowsPad);
   wait_for_previous();
   let_next_start();
   const RowsWindow rule{p, a.win};
   const int ty = threadIdx.x / 8, tx = threadIdx.x % 8;
-  // Blocks of the first keys first: all the queries see the sinks.
-  const int hk = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, j0 = blockIdx.y * C::kRows;
+  const int hk = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads;
+  const int block = blocks.first + blockIdx.y, j0 = block * C::kRows;
   const int kv_end = rule.kv_end(b), rep = p.q_heads / p.kv_heads;
   const int64_t offset = rule.offset(b);
   stage_tile<T, A>(k, C::kStride, p.k, b, hk, j0, C::kRows, kv_end, p.head_dim);
@@ -537,49 +589,81 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_dkv_kernel(const __g
   clear(dk);
   clear(dv);
   const A scale = (A)p.scale, scale2 = (A)(p.scale * kLog2eD);
-  // Queries that see some of the block's keys.
-  const int first = (int)i64min(p.q_len, i64max(0, j0 - offset) / kRowsCols * kRowsCols);
-  int64_t stop = p.q_len;
+  // Queries that see some of the block's keys, and this part's of them.
+  int64_t first = i64min(p.q_len, i64max(0, j0 - offset) / kCols * kCols), stop = p.q_len;
   if (j0 >= a.win.sinks) stop = i64min(stop, (int64_t)min(j0 + C::kRows, kv_end) - 1 - offset + a.win.window);
   if (j0 >= kv_end) stop = 0;
-  for (int h = hk * rep; h < (hk + 1) * rep; ++h)
-    for (int i0 = first; i0 < stop; i0 += kRowsCols) {
-      __syncthreads();
-      stage_tile<T, A>(q, C::kStride, p.q, b, h, i0, kRowsCols, p.q_len, p.head_dim);
-      stage_tile<T, A>(g, C::kStride, a.bp.dout, b, h, i0, kRowsCols, p.q_len, p.value_dim);
-      if (threadIdx.x < kRowsCols) {
-        const int i = i0 + threadIdx.x;
-        s_lse2[threadIdx.x] = i < p.q_len ? row_lse2<A>(p, b, h, i) : -neg_inf<A>();
-        s_delta[threadIdx.x] =
-            i < p.q_len ? reinterpret_cast<const A*>(a.delta)[((int64_t)b * p.q_heads + h) * p.q_len + i] : A(0);
-      }
-      __syncthreads();
-      A s[RT][4], d[RT][4];
-      dots<RT>(s, k, q, C::kStride, p.head_dim, ty, tx);
-      dots<RT>(d, v, g, C::kStride, p.value_dim, ty, tx);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int key = j0 + ty + 16 * r;
-        const int64_t from = key - offset;  // the first query that sees it
-        const uint32_t see = key >= kv_end ? 0u
-                                           : range_bits(from, key < a.win.sinks ? p.q_len
-                                                                                : i64min(p.q_len, from + a.win.window), i0);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = tx + 8 * c;
-          const A pr = (see >> col) & 1u ? acc_exp2(s[r][c] * scale2 - s_lse2[col]) : A(0);
-          wp[(ty + 16 * r) * (kRowsCols + kRowsPad) + col] = pr;
-          ws[(ty + 16 * r) * (kRowsCols + kRowsPad) + col] = pr * (d[r][c] - s_delta[col]) * scale;
-        }
-      }
-      __syncwarp();
-      accumulate<RT, DC>(dv, wp, g, C::kStride, ty, tx);
-      accumulate<RT, DC>(dk, ws, q, C::kStride, ty, tx);
+  if (blocks.parts > 1) {
+    const int64_t from = first + (int64_t)blockIdx.z * blocks.queries;
+    stop = i64min(stop, from + blocks.queries);
+    first = from;
+  }
+  const int tiles_a_head = first < stop ? (int)((stop - first + kCols - 1) / kCols) : 0, n = rep * tiles_a_head;
+  auto stage = [&](int it) {
+    const int h = hk * rep + it / tiles_a_head, i0 = (int)first + it % tiles_a_head * kCols;
+    A* q = tiles + it % kBufs * 2 * kCols * C::kStride;
+    stage_tile<T, A>(q, C::kStride, p.q, b, h, i0, kCols, p.q_len, p.head_dim);
+    stage_tile<T, A>(q + kCols * C::kStride, C::kStride, a.bp.dout, b, h, i0, kCols, p.q_len, p.value_dim);
+    if (threadIdx.x < kCols) {
+      const int i = i0 + threadIdx.x;
+      s_lse2[it % kBufs][threadIdx.x] = i < p.q_len ? row_lse2<A>(p, b, h, i) : -neg_inf<A>();
+      s_delta[it % kBufs][threadIdx.x] =
+          i < p.q_len ? reinterpret_cast<const A*>(a.delta)[((int64_t)b * p.q_heads + h) * p.q_len + i] : A(0);
     }
+  };
+  if (n > 0) stage(0);
+  for (int it = 0; it < n; ++it) {
+    const int i0 = (int)first + it % tiles_a_head * kCols;
+    const A *q = tiles + it % kBufs * 2 * kCols * C::kStride, *g = q + kCols * C::kStride;
+    const A *lse2 = s_lse2[it % kBufs], *delta = s_delta[it % kBufs];
+    ptx::copies_done();
+    __syncthreads();  // this tile is there, the one before is used up
+    if (kBufs > 1 && it + 1 < n) stage(it + 1);
+    A s[RT][kNC], d[RT][kNC];
+    dots<RT, kNC>(s, k, q, C::kStride, p.head_dim, ty, tx);
+    dots<RT, kNC>(d, v, g, C::kStride, p.value_dim, ty, tx);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int key = j0 + ty + 16 * r;
+      const int64_t from = key - offset;  // the first query that sees it
+      const uint32_t see =
+          key >= kv_end ? 0u
+                        : range_bits(from, key < a.win.sinks ? p.q_len : i64min(p.q_len, from + a.win.window), i0);
+#pragma unroll
+      for (int c = 0; c < kNC; ++c) {
+        const int col = tx + 8 * c;
+        const A pr = (see >> col) & 1u ? acc_exp2(s[r][c] * scale2 - lse2[col]) : A(0);
+        wp[(ty + 16 * r) * (kCols + kRowsPad) + col] = pr;
+        ws[(ty + 16 * r) * (kCols + kRowsPad) + col] = pr * (d[r][c] - delta[col]) * scale;
+      }
+    }
+    __syncwarp();  // a row's weights are written and read by one warp
+    accumulate<RT, kNC, DC>(dv, wp, g, C::kStride, ty, tx);
+    accumulate<RT, kNC, DC>(dk, ws, q, C::kStride, ty, tx);
+    if (kBufs == 1 && it + 1 < n) {
+      __syncthreads();
+      stage(it + 1);
+    }
+  }
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int key = j0 + ty + 16 * r;
     if (key >= p.kv_len) continue;
+    if (blocks.parts > 1) {
+      // [part][row and head][row of the blocks][channels of K, of V]
+      A* out = reinterpret_cast<A*>(blocks.part) +
+               (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * blocks.count * C::kRows + blockIdx.y * C::kRows + ty + 16 * r) *
+                   (p.head_dim + p.value_dim);
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int ch = 4 * (tx + 8 * c) + e;
+          if (ch < p.head_dim) out[ch] = dk[r][c][e];
+          if (ch < p.value_dim) out[p.head_dim + ch] = dv[r][c][e];
+        }
+      continue;
+    }
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
@@ -591,14 +675,36 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_dkv_kernel(const __g
   }
 }
 
+// dK and dV of the blocks' keys from their parts, one thread a channel of a key.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    rows_dkv_sum_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks, int rows) {
+  using A = typename Elem<T>::acc;
+  const ts_attn_params& p = a.bp.fwd;
+  wait_for_previous();
+  let_next_start();
+  const int wide = p.head_dim + p.value_dim, keys = blocks.count * rows;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x, heads = (int64_t)p.kv_heads * p.batch;
+  if (x >= heads * keys * wide) return;
+  const int ch = (int)(x % wide), local = (int)(x / wide % keys), bh = (int)(x / wide / keys);
+  const int key = blocks.first * rows + local;
+  if (key >= p.kv_len) return;
+  const A* part = reinterpret_cast<const A*>(blocks.part) + x;
+  A sum = A(0);
+#pragma unroll 8
+  for (int z = 0; z < blocks.parts; ++z) sum += part[z * heads * keys * wide];
+  const ts_view4& out = ch < p.head_dim ? a.bp.dk : a.bp.dv;
+  *at4w<T>(out, bh / p.kv_heads, bh % p.kv_heads, key, ch < p.head_dim ? ch : ch - p.head_dim) = Elem<T>::from_acc(sum);
+}
+
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-template <typename K, typename Args>
-cudaError_t launch_rows(K kernel, dim3 grid, size_t smem, cudaStream_t st, const Args& a) {
+template <typename K, typename... Args>
+cudaError_t launch_rows(K kernel, dim3 grid, size_t smem, cudaStream_t st, const Args&... a) {
   const cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), (int)smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, grid, dim3(kRowsThreads), smem, st, a);
+  return launch_dependent(kernel, grid, dim3(kRowsThreads), smem, st, a...);
 }
 
 // Row tiles of a block: the widest that the registers and shared memory hold, narrower while `rows` rows in `slices`
@@ -617,14 +723,60 @@ cudaError_t rows_window_fwd_t(const RowsWindow& a, cudaStream_t st) {
   return launch_rows(rows_window_fwd_kernel<T, RT, DC>, grid, C::kFwdSmem, st, a);
 }
 
+// The key blocks with sinks, which all the queries behind them see, and the others, each divided until the SMs have
+// work for several blocks (at most 64 parts: a part's sums are written and read once more).
+template <typename A>
+void rows_key_blocks(const ts_attn_params& p, const WindowArgs& win, int rows, int cols, RowsKeyBlocks (&sets)[2],
+                     size_t* bytes) {
+  const int blocks = ceil_div(p.kv_len, rows), with_sinks = min(blocks, ceil_div(win.sinks, rows));
+  const int64_t heads = (int64_t)p.kv_heads * p.batch, want = 6 * (int64_t)device_sms();
+  size_t used = 0;
+  for (int i = 0; i < 2; ++i) {
+    RowsKeyBlocks& s = sets[i];
+    s.first = i == 0 ? 0 : with_sinks;
+    s.count = i == 0 ? with_sinks : blocks - with_sinks;
+    if (s.count == 0) continue;
+    const int64_t seen = i == 0 ? p.q_len : i64min(p.q_len, (int64_t)win.window + rows + cols);
+    const int64_t tiles = (seen + cols - 1) / cols;
+    const int64_t parts = i64max(1, i64min(i64min(64, tiles), want / i64max(1, heads * s.count)));
+    s.queries = (int)((tiles + parts - 1) / parts) * cols;
+    s.parts = (int)((seen + s.queries - 1) / s.queries);
+    s.part = reinterpret_cast<void*>(used);  // an offset until it is placed
+    if (s.parts > 1) used += sizeof(A) * (size_t)s.parts * heads * s.count * rows * (p.head_dim + p.value_dim);
+  }
+  *bytes = used;
+}
+
 template <typename T, int RT, int DC>
-cudaError_t rows_window_bwd_t(const RowsWindowBwd& a, cudaStream_t st) {
+cudaError_t rows_window_dq_t(const RowsWindowBwd& a, cudaStream_t st) {
   using C = RowsCfg<typename Elem<T>::acc, RT, DC>;
   const ts_attn_params& p = a.bp.fwd;
-  const dim3 dq(ceil_div(p.q_len, C::kRows), p.q_heads, p.batch), dkv(p.kv_heads * p.batch, ceil_div(p.kv_len, C::kRows));
-  const cudaError_t e = launch_rows(rows_window_dq_kernel<T, RT, DC>, dq, C::kBwdSmem, st, a);
-  if (e != cudaSuccess) return e;
-  return launch_rows(rows_window_dkv_kernel<T, RT, DC>, dkv, C::kBwdSmem, st, a);
+  return launch_rows(rows_window_dq_kernel<T, RT, DC>, dim3(ceil_div(p.q_len, C::kRows), p.q_heads, p.batch), C::kBwdSmem,
+                     st, a);
+}
+
+// Into a workspace behind the deltas; ws null: its bytes alone.
+template <typename T, int RT, int DC>
+cudaError_t rows_window_dkv_t(const RowsWindowBwd& a, size_t* bytes, unsigned char* ws, cudaStream_t st) {
+  using A = typename Elem<T>::acc;
+  using C = RowsCfg<A, RT, DC>;
+  const ts_attn_params& p = a.bp.fwd;
+  RowsKeyBlocks sets[2];
+  rows_key_blocks<A>(p, a.win, C::kRows, C::kBwdCols, sets, bytes);
+  if (!ws) return cudaSuccess;
+  const int64_t heads = (int64_t)p.kv_heads * p.batch;
+  for (RowsKeyBlocks& s : sets) {
+    if (s.count == 0) continue;
+    s.part = ws + reinterpret_cast<size_t>(s.part);
+    cudaError_t e = launch_rows(rows_window_dkv_kernel<T, RT, DC>, dim3((unsigned)heads, s.count, s.parts), C::kBwdSmem,
+                                st, a, s);
+    if (e == cudaSuccess && s.parts > 1)
+      e = launch_dependent(rows_dkv_sum_kernel<T>,
+                           dim3((unsigned)((heads * s.count * C::kRows * (p.head_dim + p.value_dim) + 255) / 256)),
+                           dim3(256), 0, st, a, s, C::kRows);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 template <typename T, int RT, int DC>
@@ -634,7 +786,7 @@ cudaError_t rows_tree_t(TreeArgs& a, cudaStream_t st) {
   const unsigned grid = sizeof(A) == 4 ? (unsigned)a.ctas : (unsigned)(a.p.batch * a.p.kv_heads * a.row_tiles);
   const cudaError_t e = launch_rows(rows_tree_kernel<T, RT, DC>, dim3(grid), C::kFwdSmem, st, a);
   if (e != cudaSuccess || sizeof(A) == 8) return e;
-  return tree_merge(a, kRowsCols, 0, st);
+  return tree_merge(a, C::kFwdCols, 0, st);
 }
 
 template <typename T, int DC>
@@ -648,14 +800,33 @@ cudaError_t rows_window_fwd_d(const RowsWindow& a, cudaStream_t st) {
   return rows_window_fwd_t<T, 1, DC>(a, st);
 }
 
+// ws null: the workspace's bytes alone.
 template <typename T, int DC>
-cudaError_t rows_window_bwd_d(const RowsWindowBwd& a, cudaStream_t st) {
+cudaError_t rows_window_bwd_d(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes, void* ws, cudaStream_t st) {
   using A = typename Elem<T>::acc;
-  const ts_attn_params& p = a.bp.fwd;
-  const int rt = rows_rt<A, DC>(min(p.q_len, p.kv_len), (int64_t)p.kv_heads * p.batch, DC <= 4 && sizeof(A) == 4 ? 2 : 1);
-  if constexpr (sizeof(A) == 4 && DC <= 4)
-    if (rt == 2) return rows_window_bwd_t<T, 2, DC>(a, st);
-  return rows_window_bwd_t<T, 1, DC>(a, st);
+  const ts_attn_params& p = bp.fwd;
+  constexpr int kMost = sizeof(A) == 8 ? 1 : DC == 2 ? 4 : DC == 4 ? 2 : 1;  // row tiles that the registers hold
+  const size_t delta = (sizeof(A) * (size_t)p.batch * p.q_heads * p.q_len + 255) / 256 * 256;
+  const RowsWindowBwd a{bp, win, ws};
+  unsigned char* parts = ws ? reinterpret_cast<unsigned char*>(ws) + delta : nullptr;
+  if (ws) {
+    const int64_t rows = (int64_t)p.batch * p.q_heads * p.q_len;
+    cudaError_t e = launch_dependent(rows_delta_kernel<T>, dim3((unsigned)((rows * 32 + 255) / 256)), dim3(256), 0, st, bp,
+                                     reinterpret_cast<A*>(ws));
+    if (e != cudaSuccess) return e;
+    const int rt = rows_rt<A, DC>(p.q_len, (int64_t)p.q_heads * p.batch, kMost);
+    if (rt == 1) e = rows_window_dq_t<T, 1, DC>(a, st);
+    if constexpr (kMost >= 2)
+      if (rt == 2) e = rows_window_dq_t<T, 2, DC>(a, st);
+    if constexpr (kMost >= 4)
+      if (rt == 4) e = rows_window_dq_t<T, 4, DC>(a, st);
+    if (e != cudaSuccess) return e;
+  }
+  // Key blocks are divided along the queries, so they may be wide whatever their number.
+  const cudaError_t e = p.kv_len > 16 ? rows_window_dkv_t<T, kMost, DC>(a, bytes, parts, st)
+                                      : rows_window_dkv_t<T, 1, DC>(a, bytes, parts, st);
+  *bytes += delta;
+  return e;
 }
 
 template <typename T, int DC>
@@ -699,19 +870,13 @@ cudaError_t rows_window_fwd_dispatch(const RowsWindow& a, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t rows_window_bwd_dispatch(const ts_attn_bwd_params& bp, const WindowArgs& win, void* ws, cudaStream_t st) {
-  using A = typename Elem<T>::acc;
-  const ts_attn_params& p = bp.fwd;
-  const int64_t rows = (int64_t)p.batch * p.q_heads * p.q_len;
-  const cudaError_t e = launch_dependent(rows_delta_kernel<T>, dim3((unsigned)((rows * 32 + 255) / 256)), dim3(256), 0,
-                                         st, bp, reinterpret_cast<A*>(ws));
-  if (e != cudaSuccess) return e;
-  const RowsWindowBwd a{bp, win, ws};
-  switch (rows_tree_dc(p)) {
-    case 2: return rows_window_bwd_d<T, 2>(a, st);
-    case 4: return rows_window_bwd_d<T, 4>(a, st);
+cudaError_t rows_window_bwd_dispatch(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes, void* ws,
+                                     cudaStream_t st) {
+  switch (rows_tree_dc(bp.fwd)) {
+    case 2: return rows_window_bwd_d<T, 2>(bp, win, bytes, ws, st);
+    case 4: return rows_window_bwd_d<T, 4>(bp, win, bytes, ws, st);
   }
-  return rows_window_bwd_d<T, 8>(a, st);
+  return rows_window_bwd_d<T, 8>(bp, win, bytes, ws, st);
 }
 
 template <typename T>
@@ -727,9 +892,9 @@ cudaError_t rows_tree_dispatch(const ts_attn_params& p, TreeArgs* a, size_t* byt
   cudaError_t rows_window_fwd_##suffix(const RowsWindow& a, cudaStream_t st) {                                   \
     return rows_window_fwd_dispatch<T>(a, st);                                                                   \
   }                                                                                                              \
-  cudaError_t rows_window_bwd_##suffix(const ts_attn_bwd_params& bp, const WindowArgs& win, void* ws,            \
-                                       cudaStream_t st) {                                                        \
-    return rows_window_bwd_dispatch<T>(bp, win, ws, st);                                                         \
+  cudaError_t rows_window_bwd_##suffix(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes,       \
+                                       void* ws, cudaStream_t st) {                                              \
+    return rows_window_bwd_dispatch<T>(bp, win, bytes, ws, st);                                                  \
   }                                                                                                              \
   cudaError_t rows_tree_##suffix(const ts_attn_params& p, TreeArgs* a, size_t* bytes, void* ws, cudaStream_t st) { \
     return rows_tree_dispatch<T>(p, a, bytes, ws, st);                                                           \

@@ -17,11 +17,11 @@ struct RowsWindow {
   }
 };
 
-// Without arguments (a null) rows_tree only gives the workspace's bytes.
+// Without arguments or a workspace (a null) rows_tree and rows_window_bwd only give the workspace's bytes.
 #define TS_ROWS_DECLARE(suffix)                                                                                    \
   cudaError_t rows_window_fwd_##suffix(const RowsWindow& a, cudaStream_t st);                                      \
-  cudaError_t rows_window_bwd_##suffix(const ts_attn_bwd_params& bp, const WindowArgs& win, void* ws,              \
-                                       cudaStream_t st);                                                           \
+  cudaError_t rows_window_bwd_##suffix(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes,         \
+                                       void* ws, cudaStream_t st);                                                 \
   cudaError_t rows_tree_##suffix(const ts_attn_params& p, TreeArgs* a, size_t* bytes, void* ws, cudaStream_t st);
 TS_ROWS_DECLARE(f32)
 TS_ROWS_DECLARE(f64)
