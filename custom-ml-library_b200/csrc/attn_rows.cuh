@@ -148,6 +148,38 @@ __device__ __forceinline__ void stage_packed(A* dst, int stride, const ts_view4&
 // acc[r][k] = sum_c rows[ty + 16 r][c] cols[tx + 8 k][c].
 template <int RT, int NC, typename A>
 __device__ __forceinline__ void dots(A (&acc)[RT][NC], const A* rows, const A* cols, int stride, int C, int ty, int tx) {
+  if constexpr (sizeof(A) == 4) {  // sums of even and of odd channels, two products an instruction
+    uint64_t two[RT][NC];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int k = 0; k < NC; ++k) two[r][k] = 0;
+#pragma unroll 2
+    for (int c = 0; c < C; c += 4) {
+      ulonglong2 a[RT], b[NC];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) a[r] = *reinterpret_cast<const ulonglong2*>(rows + (ty + 16 * r) * stride + c);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) b[k] = *reinterpret_cast<const ulonglong2*>(cols + (tx + 8 * k) * stride + c);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int k = 0; k < NC; ++k) two[r][k] = ptx::fma2(a[r].x, b[k].x, two[r][k]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int k = 0; k < NC; ++k) two[r][k] = ptx::fma2(a[r].y, b[k].y, two[r][k]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        float x, y;
+        ptx::f2unpack(two[r][k], x, y);
+        acc[r][k] = x + y;
+      }
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -171,6 +203,45 @@ __device__ __forceinline__ void dots(A (&acc)[RT][NC], const A* rows, const A* c
 // acc[r][c] += sum_j w[ty + 16 r][j] cols[j][4 (tx + 8 c) ..]; w has 8 NC + kRowsPad elements a row.
 template <int RT, int NC, int DC, typename A>
 __device__ __forceinline__ void accumulate(A (&acc)[RT][DC][4], const A* w, const A* cols, int stride, int ty, int tx) {
+  if constexpr (sizeof(A) == 4) {
+    uint64_t two[RT][DC][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        two[r][c][0] = ptx::f2pack(acc[r][c][0], acc[r][c][1]);
+        two[r][c][1] = ptx::f2pack(acc[r][c][2], acc[r][c][3]);
+      }
+#pragma unroll 2
+    for (int j = 0; j < 8 * NC; j += 4) {
+      Quad<A> p[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) p[r] = quad(w + (ty + 16 * r) * (8 * NC + kRowsPad) + j);
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        uint64_t both[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) both[r] = ptx::f2pack(p[r].v[jj], p[r].v[jj]);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols + (j + jj) * stride + 4 * (tx + 8 * c));
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            two[r][c][0] = ptx::fma2(both[r], v.x, two[r][c][0]);
+            two[r][c][1] = ptx::fma2(both[r], v.y, two[r][c][1]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        ptx::f2unpack(two[r][c][0], acc[r][c][0], acc[r][c][1]);
+        ptx::f2unpack(two[r][c][1], acc[r][c][2], acc[r][c][3]);
+      }
+    return;
+  }
 #pragma unroll 2
   for (int j = 0; j < 8 * NC; j += 4) {
     Quad<A> p[RT];
