@@ -671,6 +671,53 @@ size_t tree_workspace(const ts_attn_params& p) {
   if (p.dtype != TS_F64) (void)rows_tree(p, nullptr, &bytes, nullptr, nullptr);
   return bytes;
 }
+cudaError_t tree_run(const ts_attn_params& p, const int32_t* parents, int64_t parents_stride, const tsa::WindowArgs& win,
+                     void* workspace, cudaStream_t st) {
+  if (tsa::tc_tree_supported(p)) return tsa::tc_tree(p, parents, parents_stride, win, workspace, fault_ptr(), st);
+  tsa::TreeArgs a = {};
+  a.parents = parents;
+  a.parents_stride = parents_stride;
+  a.win = win;
+  size_t bytes;
+  return rows_tree(p, &a, &bytes, workspace, st);
+}
+
+// Whether a windowed forward is shared along its keys (ts_attn_tree's kernels over a chain) rather than given to one
+// block a query tile, by what both take in microseconds.  On the tensor cores a tile of 128 keys takes a query tile's
+// CTA 1.45 and an SM's share of the line 2.5, which also starts, waits and merges for 14 and 0.16 a row (one token of
+// 32 / 8 heads of 128 over a window of 4096: 19 against 51; 16 tokens 30 against 51, 128 tokens 67 against 52; one
+// token, a window of 100: 12 against 9).  On CUDA cores a block's tile takes 4.5 while its SM has no other, the line's
+// 25 (64 keys, up to 64 channels) or 16 (32 keys) behind 15 (one token of 8 heads of 64, a window of 500: 23 against
+// 45, 500 tokens 75 against 59; 300 tokens of 8 / 2 heads of 128, a window of 2000: 156 against 311).
+bool window_split_faster(const ts_attn_params& p, const tsa::WindowArgs& win, bool tc) {
+  const int dim = p.head_dim > p.value_dim ? p.head_dim : p.value_dim, sms = tsa::device_sms();
+  const int group = p.q_heads / p.kv_heads, keys = tc ? 128 : dim <= 64 ? 64 : 32, line_rows = tc ? 128 : 64;
+  const int64_t heads = (int64_t)p.q_heads * p.batch;
+  const int widest = dim <= 128 ? 4 : 2, rt = tc ? 8 : tsa::rows_rt(p.q_len, heads, widest);
+  const int64_t rows = (int64_t)group * p.q_len, units = (rows + line_rows - 1) / line_rows * p.kv_heads * p.batch;
+  // Key tiles of a block of `queries` tokens.
+  auto tiles = [&](int64_t queries) {
+    const int64_t all = (p.kv_len + keys - 1) / keys;
+    const int64_t near = (win.window + tsa::i64min(queries, p.q_len) + keys - 2) / keys + 1;
+    return (double)tsa::i64min(all, near + (win.sinks + keys - 1) / keys);
+  };
+  const int64_t blocks = (p.q_len + 16 * rt - 1) / (16 * rt) * heads, waves = (blocks + sms - 1) / sms;
+  const double line = (double)units * (tiles(line_rows) + (tc ? 2 : 0)) / (tc ? sms : 2 * sms);
+  if (tc) return 14 + 2.5 * line + 0.16 * (rows < 128 ? rows : 128) < 0.9 * (5 + 1.45 * waves * tiles(128));
+  const double share = waves * (8.0 + rt) / 13;
+  return 15 + (keys == 64 ? 25 : 16) * (line > 1 ? line : 1) < 0.9 * (5 + 4.5 * tiles(16 * rt) * (share > 1 ? share : 1));
+}
+
+bool window_split(const ts_attn_params& p, const tsa::WindowArgs& win) {
+  if (p.dtype == TS_F64) return false;
+  if (!p.kv_lens && p.causal_offset + p.q_len > p.kv_len) return false;  // a chain's tokens are the last of the keys
+  const bool tc = tsa::tc_window_supported(p);
+  if (tc != tsa::tc_tree_supported(p) || (int64_t)p.q_heads * p.q_len * p.batch > 0x40000000) return false;
+  const char* force = std::getenv("TS_WINDOW_KERNEL");
+  if (force && !std::strcmp(force, "split")) return true;
+  if (force && (!std::strcmp(force, "tile") || !std::strcmp(force, "pair"))) return false;
+  return window_split_faster(p, win, tc);
+}
 
 }  // namespace
 
@@ -682,10 +729,20 @@ int ts_attn_window_path(const ts_attn_params* p, const ts_window* w) {
   return tsa::tc_window_supported(*p) ? TS_PATH_TCGEN05 : TS_PATH_SIMT;
 }
 
-int ts_attn_fwd_window(const ts_attn_params* p, const ts_window* w, void* stream) {
+size_t ts_attn_fwd_window_workspace_size(const ts_attn_params* p, const ts_window* w) {
+  return check_window(p, w) == TS_OK && window_split(*p, window_args(w)) ? tree_workspace(*p) : 0;
+}
+
+int ts_attn_fwd_window(const ts_attn_params* p, const ts_window* w, void* workspace, size_t workspace_bytes,
+                       void* stream) {
   const int st = check_window(p, w);
   if (st != TS_OK) return st;
   const tsa::WindowArgs win = window_args(w);
+  if (window_split(*p, win)) {  // a chain of tokens over the keys
+    if (!workspace || workspace_bytes < tree_workspace(*p) || reinterpret_cast<uintptr_t>(workspace) % 16)
+      return TS_ERR_WORKSPACE;
+    return from_cuda(tree_run(*p, nullptr, 0, win, workspace, as_stream(stream)));
+  }
   if (tsa::tc_window_supported(*p)) return from_cuda(tsa::tc_forward_window(*p, win, fault_ptr(), as_stream(stream)));
   const tsa::RowsWindow a = {*p, win};
   return from_cuda(by_dtype(p->dtype, tsa::rows_window_fwd_f32, tsa::rows_window_fwd_f64, tsa::rows_window_fwd_f16,
@@ -729,15 +786,7 @@ int ts_attn_tree(const ts_attn_params* p, const ts_tree* t, void* workspace, siz
   tsa::WindowArgs win;
   win.window = t->window;
   win.sinks = t->sinks;
-  if (tsa::tc_tree_supported(*p))
-    return from_cuda(
-        tsa::tc_tree(*p, t->parents, t->parents_stride, win, workspace, fault_ptr(), as_stream(stream)));
-  tsa::TreeArgs a = {};
-  a.parents = t->parents;
-  a.parents_stride = t->parents_stride;
-  a.win = win;
-  size_t bytes;
-  return from_cuda(rows_tree(*p, &a, &bytes, workspace, as_stream(stream)));
+  return from_cuda(tree_run(*p, t->parents, t->parents_stride, win, workspace, as_stream(stream)));
 }
 
 int ts_tree_positions(const int32_t* parents, int64_t parents_stride, const int32_t* lens, int32_t batch,

@@ -501,23 +501,4 @@ cudaError_t tc_forward_pair(const ts_attn_params& p, const CUtensorMap& mq, cons
   return bf ? launch_pair<128, true>(mq, mk, mv, a, st) : launch_pair<128, false>(mq, mk, mv, a, st);
 }
 
-// Half types, equal head dimensions that are multiples of 8 up to 128, rows TMA can address, a positive scale.
-bool tc_window_supported(const ts_attn_params& p) {
-  if (p.dtype != TS_BF16 && p.dtype != TS_F16) return false;
-  if (p.head_dim != p.value_dim || p.head_dim % 8 || p.head_dim > 128) return false;
-  if (p.mask_kind != TS_MASK_NONE || !(p.scale > 0.0)) return false;
-  if (!view_tma_ok(p.q) || !view_tma_ok(p.k) || !view_tma_ok(p.v) || !view_tma_ok(p.o)) return false;
-  return encode_fn() != nullptr;
-}
-
-// The two-tile kernel takes a single query tile too: its second tile is then empty.
-cudaError_t tc_forward_window(const ts_attn_params& p, const WindowArgs& win, uint32_t* fault, cudaStream_t st) {
-  CUtensorMap mq, mk, mv;
-  if (!make_map(&mq, p.q, p.dtype, p.batch, p.q_heads, p.q_len, p.head_dim, kBM) ||
-      !make_map(&mk, p.k, p.dtype, p.batch, p.kv_heads, p.kv_len, p.head_dim, kBN) ||
-      !make_map(&mv, p.v, p.dtype, p.batch, p.kv_heads, p.kv_len, p.value_dim, kBN))
-    return cudaErrorInvalidValue;
-  return tc_forward_pair(p, mq, mk, mv, fault, st, nullptr, &win);
-}
-
 }  // namespace tsa

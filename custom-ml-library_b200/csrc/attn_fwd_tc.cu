@@ -110,11 +110,13 @@ struct TcFwdArgs {
   int n_units;  // batch * heads * half_x
   uint32_t* fault;
   DropoutArgs drop;  // used by the kDrop instantiation only
+  WindowArgs win;    // used by the kWin instantiation only
 };
 
 }  // namespace
 
-template <int D, bool kBF16, bool kDrop>
+// kWin: the sliding window with sinks and head dimensions below D, as in tc_fwd_pair_kernel.
+template <int D, bool kBF16, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(384, 1)
     tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, TcFwdArgs args) {
@@ -148,7 +150,9 @@ __global__ void __launch_bounds__(384, 1)
   const int q_last = min(q0 + kBM - 1, p.q_len - 1);
   int kv_lim = kv_end;
   if (p.is_causal) kv_lim = (int)i64max(0, i64min(kv_end, (int64_t)q_last + offset + 1));
-  const int n_tiles = ceil_div(kv_lim, kBN);
+  const WindowTiles wt(args.win, (int64_t)q0 + offset, kv_end, kBN);
+  const int n_tiles = kWin ? wt.count(ceil_div(kv_lim, kBN)) : ceil_div(kv_lim, kBN);
+  auto key_tile = [&](int j) { return kWin ? wt.tile(j) : j; };
   const bool dead = fault_set(args.fault);
 
   if (threadIdx.x == 0) {
@@ -195,13 +199,13 @@ __global__ void __launch_bounds__(384, 1)
         if (j >= C::kStages && !wait_bar(&bars->k_empty[s], ph, args.fault, FAULT_FWD_EMPTY)) break;
         ptx::mbar_expect_tx(&bars->k_full[s], C::kTileBytes);
         for (int sl = 0; sl < C::kSlabs; ++sl)
-          ptx::tma_load_4d(sK + (s * C::kSlabs + sl) * kSlabBytes, &tm_k, 64 * sl, j * kBN, hk, b,
+          ptx::tma_load_4d(sK + (s * C::kSlabs + sl) * kSlabBytes, &tm_k, 64 * sl, key_tile(j) * kBN, hk, b,
                            &bars->k_full[s]);
         k_issued = j + 1;
         if (j >= C::kStages && !wait_bar(&bars->v_empty[s], ph, args.fault, FAULT_FWD_EMPTY)) break;
         ptx::mbar_expect_tx(&bars->v_full[s], C::kTileBytes);
         for (int sl = 0; sl < C::kSlabs; ++sl)
-          ptx::tma_load_4d(sV + (s * C::kSlabs + sl) * kSlabBytes, &tm_v, 64 * sl, j * kBN, hk, b,
+          ptx::tma_load_4d(sV + (s * C::kSlabs + sl) * kSlabBytes, &tm_v, 64 * sl, key_tile(j) * kBN, hk, b,
                            &bars->v_full[s]);
         v_issued = j + 1;
       }
@@ -291,9 +295,22 @@ __global__ void __launch_bounds__(384, 1)
         ptx::tmem_ld32(t_row + C::kColS + (uint32_t)(j & 1) * kBN + half * kHN + 32 * c,
                        *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
       ptx::tmem_wait_ld();
-      const int k0 = j * kBN + half * kHN;
-      const bool need_mask = (k0 + kHN > kv_end) || (p.is_causal && (int64_t)k0 + kHN - 1 > (int64_t)q0 + offset);
+      const int k0 = key_tile(j) * kBN + half * kHN;
+      const bool need_mask = (k0 + kHN > kv_end) || (p.is_causal && (int64_t)k0 + kHN - 1 > (int64_t)q0 + offset) ||
+                             (kWin && k0 + kHN > args.win.sinks &&
+                              (int64_t)k0 <= (int64_t)q0 + kBM - 1 + offset - args.win.window);
       const int64_t lim = p.is_causal ? (int64_t)qi + offset : (int64_t)kv_end - 1;
+      uint32_t seen[2];  // kWin: bit c of the 64 tells whether the row sees key k0 + c
+      if constexpr (kWin) {
+        const int64_t end = i64min(kv_end, lim + 1), near = lim + 1 - args.win.window;
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          seen[w] = range_bits(near, end, k0 + 32 * w) | range_bits(0, i64min(end, args.win.sinks), k0 + 32 * w);
+      }
+      auto visible = [&](int c) -> bool {
+        if constexpr (kWin) return (seen[c >> 5] >> (c & 31)) & 1u;
+        return k0 + c < kv_end && (int64_t)(k0 + c) <= lim;
+      };
       // Row max of the (masked) raw scores, scaled once (scale > 0).  Halves
       // away from the diagonal and the sequence end take the unmasked branch
       // (warp-uniform).
@@ -309,8 +326,7 @@ __global__ void __launch_bounds__(384, 1)
       } else {
 #pragma unroll
         for (int c = 0; c < kHN; ++c) {
-          const int key = k0 + c;
-          if (key < kv_end && (int64_t)key <= lim) mx = fmaxf(mx, __uint_as_float(r[c]));
+          if (visible(c)) mx = fmaxf(mx, __uint_as_float(r[c]));
         }
       }
       mx = mx == -INFINITY ? mx : mx * qk_scale;
@@ -370,11 +386,10 @@ __global__ void __launch_bounds__(384, 1)
       } else {
 #pragma unroll
         for (int c = 0; c < kHN; c += 2) {
-          const int key = k0 + c;
           float p0 = ptx::ex2(fmaf(__uint_as_float(r[c]), qk_scale, -safe));
           float p1 = ptx::ex2(fmaf(__uint_as_float(r[c + 1]), qk_scale, -safe));
-          p0 = (key < kv_end && (int64_t)key <= lim) ? p0 : 0.f;
-          p1 = (key + 1 < kv_end && (int64_t)key + 1 <= lim) ? p1 : 0.f;
+          p0 = visible(c) ? p0 : 0.f;
+          p1 = visible(c + 1) ? p1 : 0.f;
           sum2[0] = ptx::add2(sum2[0], ptx::f2pack(p0, p1));
           p0 = dropped(p0, c);
           p1 = dropped(p1, c + 1);
@@ -475,7 +490,7 @@ __global__ void __launch_bounds__(384, 1)
             v = make_uint4(ptx::pack_f16(f[e], f[e + 1]), ptx::pack_f16(f[e + 2], f[e + 3]),
                            ptx::pack_f16(f[e + 4], f[e + 5]), ptx::pack_f16(f[e + 6], f[e + 7]));
           }
-          *reinterpret_cast<uint4*>(orow + col + e) = v;
+          if (!kWin || (int)col + e < p.head_dim) *reinterpret_cast<uint4*>(orow + col + e) = v;
         }
       }
     }
@@ -1043,6 +1058,14 @@ static FwdKernel fwd_kernel_env() {
   return FwdKernel::kDefault;
 }
 
+// The same for windows: TS_WINDOW_KERNEL = "tile" or "pair".
+static FwdKernel window_kernel_env() {
+  const char* e = getenv("TS_WINDOW_KERNEL");
+  if (e && !strcmp(e, "pair")) return FwdKernel::kPair;
+  if (e && !strcmp(e, "tile")) return FwdKernel::kTile;
+  return FwdKernel::kDefault;
+}
+
 template <int D, bool BF16>
 static cudaError_t launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                              const TcFwdArgs& a, cudaStream_t st, bool persistent) {
@@ -1054,7 +1077,9 @@ static cudaError_t launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const
     pk<<<dim3((unsigned)sms), 384, Cfg<D>::kSmem, st>>>(mq, mk, mv, a);
     return cudaGetLastError();
   }
-  auto kern = a.drop.p > 0.f ? tc_fwd_kernel<D, BF16, true> : tc_fwd_kernel<D, BF16, false>;
+  auto kern = a.win.window > 0 ? tc_fwd_kernel<D, BF16, false, true>
+              : a.drop.p > 0.f ? tc_fwd_kernel<D, BF16, true, false>
+                               : tc_fwd_kernel<D, BF16, false, false>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kern), Cfg<D>::kSmem);
   if (e != cudaSuccess) return e;
   dim3 grid(a.n_q_tiles, a.p.q_heads, a.p.batch);
@@ -1093,6 +1118,44 @@ cudaError_t tc_forward(const ts_attn_params& p, uint32_t* fault, cudaStream_t st
   if (p.head_dim == 64)
     return bf ? launch_tc<64, true>(mq, mk, mv, a, st, persistent) : launch_tc<64, false>(mq, mk, mv, a, st, persistent);
   return bf ? launch_tc<128, true>(mq, mk, mv, a, st, persistent) : launch_tc<128, false>(mq, mk, mv, a, st, persistent);
+}
+
+// Half types, equal head dimensions that are multiples of 8 up to 128, rows TMA can address, a positive scale.
+bool tc_window_supported(const ts_attn_params& p) {
+  if (p.dtype != TS_BF16 && p.dtype != TS_F16) return false;
+  if (p.head_dim != p.value_dim || p.head_dim % 8 || p.head_dim > 128) return false;
+  if (p.mask_kind != TS_MASK_NONE || !(p.scale > 0.0)) return false;
+  if (!view_tma_ok(p.q) || !view_tma_ok(p.k) || !view_tma_ok(p.v) || !view_tma_ok(p.o)) return false;
+  return encode_fn() != nullptr;
+}
+
+// A key tile takes a CTA of the two-tile kernel about 1.75 times as long as one of the one-tile kernel: the former for
+// grids of several waves, the latter where its CTAs take fewer of them (2 rows of 1001 queries, 8 heads of 64, a
+// window of 2048: 32 against 52 us; one row of 1024 queries, 32 / 8 heads of 128, a window of 4096: 106 against 93).
+static bool window_on_pairs(const ts_attn_params& p) {
+  const FwdKernel env = window_kernel_env();
+  if (env != FwdKernel::kDefault) return env == FwdKernel::kPair;
+  const int64_t heads = (int64_t)p.q_heads * p.batch, sms = sm_count();
+  const int64_t pairs = ceil_div(p.q_len, 2 * kBM) * heads, tiles = ceil_div(p.q_len, kBM) * heads;
+  return (pairs + sms - 1) / sms * 7 <= (tiles + sms - 1) / sms * 4;
+}
+
+cudaError_t tc_forward_window(const ts_attn_params& p, const WindowArgs& win, uint32_t* fault, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, p.q, p.dtype, p.batch, p.q_heads, p.q_len, p.head_dim, kBM) ||
+      !make_map(&mk, p.k, p.dtype, p.batch, p.kv_heads, p.kv_len, p.head_dim, kBN) ||
+      !make_map(&mv, p.v, p.dtype, p.batch, p.kv_heads, p.kv_len, p.value_dim, kBN))
+    return cudaErrorInvalidValue;
+  if (window_on_pairs(p)) return tc_forward_pair(p, mq, mk, mv, fault, st, nullptr, &win);
+  TcFwdArgs a = {};
+  a.p = p;
+  a.n_q_tiles = ceil_div(p.q_len, kBM);
+  a.fault = fault;
+  a.win = win;
+  const bool bf = p.dtype == TS_BF16;
+  if (p.head_dim <= 64)
+    return bf ? launch_tc<64, true>(mq, mk, mv, a, st, false) : launch_tc<64, false>(mq, mk, mv, a, st, false);
+  return bf ? launch_tc<128, true>(mq, mk, mv, a, st, false) : launch_tc<128, false>(mq, mk, mv, a, st, false);
 }
 
 }  // namespace tsa

@@ -452,13 +452,14 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
     walk.b = blockIdx.x / line.units;
     walk.unit = blockIdx.x % line.units;
     walk.first = 0;
-    walk.count = line.tiles(walk.b);
+    walk.list = line.list(walk.b, walk.unit % line.row_tiles);
+    walk.count = walk.list.count;
   }
   while (!kSplit || walk.next(line)) {
     const int b = walk.b, hk = walk.unit / a.row_tiles, r0 = walk.unit % a.row_tiles * F::C::kRows;
     const int len = tree_len(p, b);
     const int64_t base = (int64_t)len - p.q_len;
-    const WindowTiles wt(a.win, base, len, F::kCols);
+    const WindowTiles& wt = walk.list.tiles;
     __syncthreads();  // the unit before is used up
     if (a.parents && (int)threadIdx.x < p.q_len) s_parents[threadIdx.x] = a.parents[b * a.parents_stride + threadIdx.x];
     stage_packed<T, A>(f.q, F::C::kStride, p.q, b, hk * group, r0, F::C::kRows, a.rows, p.q_len, p.head_dim);
@@ -778,15 +779,6 @@ cudaError_t launch_rows(K kernel, dim3 grid, size_t smem, cudaStream_t st, const
   return launch_dependent(kernel, grid, dim3(kRowsThreads), smem, st, a...);
 }
 
-// Row tiles of a block: the widest that the registers and shared memory hold, narrower while `rows` rows in `slices`
-// grids leave SMs without two blocks.
-template <typename A, int DC> int rows_rt(int rows, int64_t slices, int widest) {
-  int rt = sizeof(A) == 8 ? (DC <= 4 ? 2 : 1) : (DC <= 4 ? 4 : 2);
-  rt = min(rt, widest);
-  while (rt > 1 && (rows <= 8 * rt || ceil_div(rows, 16 * rt) * slices < 2 * device_sms())) rt >>= 1;
-  return rt;
-}
-
 template <typename T, int RT, int DC>
 cudaError_t rows_window_fwd_t(const RowsWindow& a, cudaStream_t st) {
   using C = RowsCfg<typename Elem<T>::acc, RT, DC>;
@@ -863,7 +855,7 @@ cudaError_t rows_tree_t(TreeArgs& a, cudaStream_t st) {
 template <typename T, int DC>
 cudaError_t rows_window_fwd_d(const RowsWindow& a, cudaStream_t st) {
   using A = typename Elem<T>::acc;
-  const int rt = rows_rt<A, DC>(a.p.q_len, (int64_t)a.p.q_heads * a.p.batch, 4);
+  const int rt = rows_rt(a.p.q_len, (int64_t)a.p.q_heads * a.p.batch, sizeof(A) == 8 ? (DC <= 4 ? 2 : 1) : DC <= 4 ? 4 : 2);
   if constexpr (sizeof(A) == 4 && DC <= 4)
     if (rt == 4) return rows_window_fwd_t<T, 4, DC>(a, st);
   if constexpr (sizeof(A) == 4 || DC <= 4)
@@ -885,7 +877,7 @@ cudaError_t rows_window_bwd_d(const ts_attn_bwd_params& bp, const WindowArgs& wi
     cudaError_t e = launch_dependent(rows_delta_kernel<T>, dim3((unsigned)((rows * 32 + 255) / 256)), dim3(256), 0, st, bp,
                                      reinterpret_cast<A*>(ws));
     if (e != cudaSuccess) return e;
-    const int rt = rows_rt<A, DC>(p.q_len, (int64_t)p.q_heads * p.batch, kMost);
+    const int rt = rows_rt(p.q_len, (int64_t)p.q_heads * p.batch, kMost);
     if (rt == 1) e = rows_window_dq_t<T, 1, DC>(a, st);
     if constexpr (kMost >= 2)
       if (rt == 2) e = rows_window_dq_t<T, 2, DC>(a, st);

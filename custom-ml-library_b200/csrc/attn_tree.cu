@@ -127,22 +127,18 @@ __global__ void __launch_bounds__(384, 1)
         // K is a tile ahead of V: they walk along the share by themselves.
         struct Stream {
           LineWalk walk;
-          int j, sink_tiles, skip, hk;
-        } of[2] = {{walk, 0, 0, 0, 0}, {walk, 0, 0, 0, 0}};
+          int j, hk;
+        } of[2] = {{walk, 0, 0}, {walk, 0, 0}};
         int slot = 0, fills = 0;
         uint32_t phase = 1;  // of kv_empty: the ring's first round finds every slot free
         auto load = [&](Stream& w, const CUtensorMap* map) -> bool {
           if (w.j == w.walk.count) {
             if (!w.walk.next(line)) return true;  // no tile left
-            const int len = tree_len(p, w.walk.b);
-            const WindowTiles wt(args.win, (int64_t)len - p.q_len, len, kBN);
             w.j = 0;
-            w.sink_tiles = wt.sink_tiles;
-            w.skip = wt.skip;
             w.hk = w.walk.unit / args.row_tiles;
           }
           if (fills >= S && !wait_bar(&bars->kv_empty[slot], phase, args.fault, FAULT_FWD_EMPTY)) return false;
-          const int t = w.walk.first + w.j, key = (t < w.sink_tiles ? t : t + w.skip) * kBN;
+          const int key = w.walk.list.tiles.tile(w.walk.first + w.j) * kBN;
           ptx::mbar_expect_tx(&bars->kv_full[slot], C::kTileBytes);
           for (int sl = 0; sl < C::kSlabs; ++sl)
             ptx::tma_load_4d(sKV + slot * C::kTileBytes + sl * kSlabBytes, map, 64 * sl, key, w.hk, w.walk.b,
@@ -273,7 +269,9 @@ __global__ void __launch_bounds__(384, 1)
       const int r0 = walk.unit % args.row_tiles * kBM, b = walk.b;
       const int len = tree_len(p, b);
       const int64_t base = (int64_t)len - p.q_len;
-      const WindowTiles wt(args.win, base, len, kBN);
+      const WindowTiles& wt = walk.list.tiles;
+      // Keys that all the tile's queries see: those before the first of a chain's tokens and it, a tree's committed ones.
+      const int64_t common = args.parents ? base : walk.list.first + 1;
       const bool live_warp = r0 + (warp & 3) * 32 < args.rows;  // some row of the warp is a query's
       const bool live = r0 + row < args.rows;
       if (b != view_b || r0 != view_r0) {  // the heads of a row share it
@@ -303,8 +301,8 @@ __global__ void __launch_bounds__(384, 1)
             ptx::tmem_ld32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * c));
           ptx::tmem_wait_ld();
           // Only halves with drafted tokens, the cache's end, or an edge of some node's window are masked.
-          const bool need_mask = kh + kHalf > base || (args.win.window > 0 && kh + kHalf > args.win.sinks &&
-                                                       (int64_t)kh <= (int64_t)len - 1 - args.win.window);
+          const bool need_mask = kh + kHalf > common || (args.win.window > 0 && kh + kHalf > args.win.sinks &&
+                                                         (int64_t)kh <= walk.list.last - args.win.window);
           uint32_t seen[2];
           float mx = -INFINITY;
           if (!need_mask) {
@@ -479,6 +477,7 @@ __global__ void __launch_bounds__(kMergeThreads)
     tree_merge_kernel(const __grid_constant__ TreeArgs a, int tile_keys, int start_places, int share) {
   const ts_attn_params& p = a.p;
   __shared__ int64_t s_first, s_total;
+  __shared__ int s_tiles;
   __shared__ float2 s_row[kBM];  // the reference and 1 / sum of every row
   __shared__ float4 s_sum[kMergeThreads];
   const TreeLine line(a, tile_keys, start_places, true);
@@ -495,13 +494,21 @@ __global__ void __launch_bounds__(kMergeThreads)
     int64_t before;
     const int64_t total = line_total(line, lane, b, &before);
     if (lane == 0) {
+      const int h = unit / line.row_tiles, t = unit % line.row_tiles;
+      if (h > 0) {
+        int64_t places, tiles;
+        line.head(b, &places, &tiles);
+        before += h * places;
+      }
+      for (int x = 0; x < t; ++x) before += line.places(line.list(b, x).count);
+      s_tiles = line.list(b, t).count;
       s_first = before;
       s_total = total;
     }
   }
   __syncthreads();
-  const int n = line.tiles(b);
-  const int64_t total = s_total, at = s_first + unit * line.places(n) + start_places;  // its first tile's place
+  const int n = s_tiles;
+  const int64_t total = s_total, at = s_first + start_places;  // its first tile's place
   const int ctas = (int)i64min(a.ctas, total);
   int64_t part0 = 0;
   int parts = 0;

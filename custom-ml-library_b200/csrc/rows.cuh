@@ -17,6 +17,19 @@ struct RowsWindow {
   }
 };
 
+// Row tiles of a block, at most `widest`.  A tile costs the reads of its columns, the same for any number of row tiles,
+// and those of its rows (about 8 to 1), and the blocks of an SM share what it can read.
+inline int rows_rt(int rows, int64_t slices, int widest) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int rt = 1; rt <= widest; rt *= 2) {
+    const int64_t blocks = ceil_div(rows, 16 * rt) * slices, sms = device_sms();
+    const int64_t cost = (blocks + sms - 1) / sms * (8 + rt);
+    if (cost < least) least = cost, best = rt;
+  }
+  return best;
+}
+
 // Without arguments or a workspace (a null) rows_tree and rows_window_bwd only give the workspace's bytes.
 #define TS_ROWS_DECLARE(suffix)                                                                                    \
   cudaError_t rows_window_fwd_##suffix(const RowsWindow& a, cudaStream_t st);                                      \

@@ -30,13 +30,14 @@ struct TreeArgs {
 // Channel quads of a partial result's row.
 __host__ __device__ __forceinline__ int part_quads(const ts_attn_params& p) { return ceil_div(p.value_dim, 4); }
 
+// Keys of a row, without kv_lens those that the last of the q_len tokens behind causal_offset sees (a windowed chunk).
 __device__ __forceinline__ int tree_len(const ts_attn_params& p, int b) {
-  return min(p.kv_len, max(0, p.kv_lens[b]));
+  return min(p.kv_len, p.kv_lens ? max(0, p.kv_lens[b]) : (int)(p.causal_offset + p.q_len));
 }
 // The same from L2: for a kernel that asks before it has waited for the one in front of it (which has waited for what
 // wrote the lengths).
 __device__ __forceinline__ int tree_len_early(const ts_attn_params& p, int b) {
-  return min(p.kv_len, max(0, __ldcg(p.kv_lens + b)));
+  return min(p.kv_len, p.kv_lens ? max(0, __ldcg(p.kv_lens + b)) : (int)(p.causal_offset + p.q_len));
 }
 
 // What a node sees: the slots [near, end), those below min(end, sinks), and `drafted`'s bits from slot `base` on.
@@ -147,24 +148,49 @@ __device__ __forceinline__ uint32_t view_bits(const NodeView& v, int64_t base, i
   return bits;
 }
 
+// What a row tile of row b reads: the tiles of its list, for queries at positions [first, last].
+struct TileList {
+  WindowTiles tiles;
+  int count;
+  int64_t first, last;
+};
+
 // Units of work, (row b, KV head, row tile), stand in line one behind the other, each with the key tiles that it
 // reads and, in front of them, `start` places for what a unit costs by itself (its queries, its epilogue); CTA c takes
 // the places [c L / G, (c + 1) L / G) of L.
 struct TreeLine {
-  int batch, units;  // units of a row b
-  int tile, start;   // keys of a tile; places in front of a unit's tiles
+  int batch, heads, row_tiles, units;  // units of a row b: unit h row_tiles + t is row tile t of KV head h
+  int tile, start;                     // keys of a tile; places in front of a unit's tiles
   bool early;
-  const ts_attn_params* p;
-  WindowArgs win;
-  __device__ __forceinline__ TreeLine(const TreeArgs& a, int tile_keys, int start_places, bool asks_early = false)
-      : batch(a.p.batch), units(a.p.kv_heads * a.row_tiles), tile(tile_keys), start(start_places), early(asks_early),
-        p(&a.p), win(a.win) {}
-  __device__ __forceinline__ int tiles(int b) const {
-    const int len = early ? tree_len_early(*p, b) : tree_len(*p, b);
-    return WindowTiles(win, (int64_t)len - p->q_len, len, tile).count(ceil_div(len, tile));
+  const TreeArgs* a;
+  __device__ __forceinline__ TreeLine(const TreeArgs& args, int tile_keys, int start_places, bool asks_early = false)
+      : batch(args.p.batch), heads(args.p.kv_heads), row_tiles(args.row_tiles), units(heads * row_tiles),
+        tile(tile_keys), start(start_places), early(asks_early), a(&args) {}
+  __device__ __forceinline__ TileList list(int b, int row_tile) const {
+    const ts_attn_params& p = a->p;
+    const int len = early ? tree_len_early(p, b) : tree_len(p, b);
+    const int64_t base = (int64_t)len - p.q_len;
+    // The tokens of a chain that lie within one head are consecutive positions; a tree's may be anywhere.
+    int n0 = 0, n1 = p.q_len - 1;
+    if (!a->parents && p.q_len > 1) {
+      const int r0 = row_tile * a->tile_rows, r1 = min(r0 + a->tile_rows, a->rows) - 1, h = r0 / p.q_len;
+      if (r1 / p.q_len == h) n0 = r0 - h * p.q_len, n1 = r1 - h * p.q_len;
+    }
+    const WindowTiles tiles(a->win, base + n0, len, tile);
+    const int end = (int)i64max(0, i64min(len, base + n1 + 1));
+    return TileList{tiles, tiles.count(ceil_div(end, tile)), base + n0, base + n1};
   }
-  // Places of a unit with n tiles: none for rows without a key.
+  // Places of a unit with n tiles: none for one without a key.
   __device__ __forceinline__ int64_t places(int n) const { return n > 0 ? n + start : 0; }
+  // Places and tiles of one KV head of row b.
+  __device__ __forceinline__ void head(int b, int64_t* all_places, int64_t* all_tiles) const {
+    *all_places = *all_tiles = 0;
+    for (int t = 0; t < row_tiles; ++t) {
+      const int n = list(b, t).count;
+      *all_places += places(n);
+      *all_tiles += n;
+    }
+  }
 };
 __device__ __forceinline__ int64_t line_bound(int c, int64_t total, int ctas) { return c * total / ctas; }
 __device__ __forceinline__ int line_owner(int64_t at, int64_t total, int ctas) {
@@ -181,35 +207,44 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 __device__ __forceinline__ int64_t line_total(const TreeLine& line, int lane, int b, int64_t* before) {
   int64_t sum = 0, first = 0;
   for (int i = lane; i < line.batch; i += 32) {
-    const int64_t n = line.places(line.tiles(i));
+    int64_t n, tiles;
+    line.head(i, &n, &tiles);
     sum += n;
     if (i < b) first += n;
   }
-  *before = warp_sum(first) * line.units;
-  return warp_sum(sum) * line.units;
+  *before = warp_sum(first) * line.heads;
+  return warp_sum(sum) * line.heads;
 }
 
-// A place of the line: the row it belongs to, its place within the row's units, and the tiles in front of it.
+// A place of the line: the unit it belongs to, its place within the unit, and the tiles in front of it.
 struct LinePlace {
-  int row;
+  int row, unit;
   int64_t rest, tiles;
 };
 
 // One warp: the two ends of CTA `c`'s share of the line (both at its beginning for a CTA without one).
 __device__ __forceinline__ void line_share(const TreeLine& line, int lane, int c, int max_ctas, LinePlace (&ends)[2]) {
-  const int own = lane < line.batch ? line.tiles(lane) : 0;  // kept for batches of up to 32 rows
-  int64_t total = line.places(own);
-  for (int i = lane + 32; i < line.batch; i += 32) total += line.places(line.tiles(i));
-  total = warp_sum(total) * line.units;
+  int64_t own = 0, own_tiles = 0;  // of one KV head of row `lane`: kept for batches of up to 32 rows
+  if (lane < line.batch) line.head(lane, &own, &own_tiles);
+  int64_t total = own;
+  for (int i = lane + 32; i < line.batch; i += 32) {
+    int64_t n, tiles;
+    line.head(i, &n, &tiles);
+    total += n;
+  }
+  total = warp_sum(total) * line.heads;
   const int ctas = (int)i64min(max_ctas, total);
-  ends[0] = ends[1] = LinePlace{0, 0, 0};
+  ends[0] = ends[1] = LinePlace{0, 0, 0, 0};
   if (c >= ctas) return;
   const int64_t at[2] = {line_bound(c, total, ctas), line_bound(c + 1, total, ctas)};
   int64_t places = 0, tiles = 0;  // in front of this step's rows
   bool found[2] = {false, false};
   for (int b0 = 0; b0 < line.batch && !(found[0] && found[1]); b0 += 32) {
-    const int n = b0 == 0 ? own : b0 + lane < line.batch ? line.tiles(b0 + lane) : 0;
-    const int64_t mine = line.places(n) * line.units, mine_tiles = (int64_t)n * line.units;
+    if (b0 > 0) {
+      own = own_tiles = 0;
+      if (b0 + lane < line.batch) line.head(b0 + lane, &own, &own_tiles);
+    }
+    const int64_t mine = own * line.heads, mine_tiles = own_tiles * line.heads;
     int64_t up_to = mine, up_tiles = mine_tiles;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -223,12 +258,23 @@ __device__ __forceinline__ void line_share(const TreeLine& line, int lane, int c
       if (found[e] || !past) continue;
       const int l = __ffs(past) - 1;
       found[e] = true;
-      const int64_t rest = at[e] - places - __shfl_sync(0xffffffffu, up_to - mine, l);
-      const int of = __shfl_sync(0xffffffffu, n, l);
-      const int64_t unit = rest / line.places(of), in_unit = rest % line.places(of);
-      ends[e] = LinePlace{b0 + l, rest,
-                          tiles + __shfl_sync(0xffffffffu, up_tiles - mine_tiles, l) + unit * of +
-                              i64max(0, in_unit - line.start)};
+      int64_t rest = at[e] - places - __shfl_sync(0xffffffffu, up_to - mine, l);
+      const int64_t size = __shfl_sync(0xffffffffu, own, l), size_tiles = __shfl_sync(0xffffffffu, own_tiles, l);
+      LinePlace at_e = {b0 + l, 0, 0, tiles + __shfl_sync(0xffffffffu, up_tiles - mine_tiles, l)};
+      const int64_t h = rest / size;
+      rest -= h * size;
+      at_e.tiles += h * size_tiles;
+      int t = 0;
+      for (; t < line.row_tiles; ++t) {
+        const int n = line.list(b0 + l, t).count;
+        if (rest < line.places(n)) break;
+        rest -= line.places(n);
+        at_e.tiles += n;
+      }
+      at_e.unit = (int)h * line.row_tiles + t;
+      at_e.rest = rest;
+      at_e.tiles += i64max(0, rest - line.start);
+      ends[e] = at_e;
     }
     places += __shfl_sync(0xffffffffu, up_to, 31);
     tiles += __shfl_sync(0xffffffffu, up_tiles, 31);
@@ -240,30 +286,32 @@ struct LineWalk {
   int b, unit, first;  // of the present segment: row, unit of the row, first tile of the unit's list
   int count;           // its tiles; 0 before the first segment
   int64_t left;        // tiles behind it
+  TileList list;
   __device__ __forceinline__ void start(const LinePlace& from, int64_t tiles, const TreeLine& line) {
     b = from.row;
+    unit = from.unit;
+    first = (int)i64max(0, from.rest - line.start);
     count = 0;
     left = tiles;
-    unit = first = 0;
-    if (tiles > 0) {
-      const int64_t size = line.places(line.tiles(b));
-      unit = (int)(from.rest / size);
-      first = (int)i64max(0, from.rest % size - line.start);
-    }
   }
   __device__ __forceinline__ bool next(const TreeLine& line) {
     if (left == 0) return false;
     if (count) {
       first = 0;
-      if (++unit == line.units) {
+      ++unit;
+    }
+    for (;;) {  // units without a key take no place in the line
+      if (unit >= line.units) {
         unit = 0;
         ++b;
       }
+      if (b >= line.batch) return false;  // not reached while the lengths stay as they are
+      list = line.list(b, unit % line.row_tiles);
+      if (list.count > first) break;
+      first = 0;
+      ++unit;
     }
-    int n = 0;
-    while (b < line.batch && (n = line.tiles(b)) == 0) ++b;  // rows without a key take no place in the line
-    if (n <= first) return false;                              // not reached while the lengths stay as they are
-    count = (int)i64min(left, n - first);
+    count = (int)i64min(left, list.count - first);
     left -= count;
     return true;
   }

@@ -21,6 +21,7 @@ __device__ __forceinline__ uint32_t range_bits(int64_t lo, int64_t hi, int64_t b
 // Tile j of the list is key tile j below `sink_tiles`, j + skip behind.
 struct WindowTiles {
   int sink_tiles, skip;
+  WindowTiles() = default;
   // Queries from position `first` (may be negative), keys [0, kv_end) in tiles of `tile` keys.
   __device__ __forceinline__ WindowTiles(const WindowArgs& w, int64_t first, int kv_end, int tile) {
     sink_tiles = ceil_div(min(max(w.sinks, 0), kv_end), tile);

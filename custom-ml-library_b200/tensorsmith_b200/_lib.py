@@ -296,8 +296,10 @@ SIGNATURES = {
          ctypes.c_void_p],
     ),
     "ts_attn_fwd_window": (
-        ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), ctypes.c_void_p]
+        ctypes.c_int,
+        [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
     ),
+    "ts_attn_fwd_window_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
     "ts_attn_window_path": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
     "ts_attn_bwd_window_workspace_size": (
         ctypes.c_size_t, [ctypes.POINTER(AttnBwdParams), ctypes.POINTER(Window)]

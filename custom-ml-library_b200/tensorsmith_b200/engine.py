@@ -193,9 +193,12 @@ def forward(q, k, v, *, is_causal=False, scale=None, causal_offset=0, kv_lens=No
                           causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
     if window is not None:
         w = _window_struct(window, sinks, is_causal, mask, dropout)
+        handle = _lib.lib()
         with _on(q.get_device()):
-            _lib.check(_lib.lib().ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), _stream_handle(q.device)),
-                       "ts_attn_fwd_window")
+            need = handle.ts_attn_fwd_window_workspace_size(ctypes.byref(p), ctypes.byref(w))
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            _lib.check(handle.ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), ws.data_ptr() if need else None, need,
+                                                 _stream_handle(q.device)), "ts_attn_fwd_window")
         del keep
         return out, (lse if need_lse else None)
     _no_window(sinks)
@@ -298,9 +301,9 @@ def backward(q, k, v, out, lse, dout, *, is_causal=False, scale=None, causal_off
     handle = _lib.lib()
     if window is not None:
         w = _window_struct(window, sinks, is_causal, mask, dropout)
-        need = int(handle.ts_attn_bwd_window_workspace_size(ctypes.byref(bp), ctypes.byref(w)))
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
         with _on(q.get_device()):
+            need = int(handle.ts_attn_bwd_window_workspace_size(ctypes.byref(bp), ctypes.byref(w)))
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
             _lib.check(handle.ts_attn_bwd_window(ctypes.byref(bp), ctypes.byref(w), ws.data_ptr(), ws.numel(),
                                                  _stream_handle(q.device)), "ts_attn_bwd_window")
         del keep
@@ -762,10 +765,10 @@ def attention_tree(q, k, v, kv_lens, parents=None, *, window=None, sinks=0, scal
         lse = q.new_empty(q.shape[:3], dtype=lse_dtype(q.dtype))
     params, tree, index = _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse)
     handle = _lib.lib()
-    need = handle.ts_attn_tree_workspace_size(params, tree)
-    if need:
-        workspace = _workspace(workspace, need, q)
     with _on(index):
+        need = handle.ts_attn_tree_workspace_size(params, tree)
+        if need:
+            workspace = _workspace(workspace, need, q)
         status = handle.ts_attn_tree(params, tree, workspace.data_ptr() if need else None, need, _raw_stream(index))
     if status:
         _lib.check(status, "ts_attn_tree")

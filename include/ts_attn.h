@@ -411,8 +411,13 @@ typedef struct ts_window {
 
 /* ts_attn_fwd under a window: is_causal must be set, no explicit mask, no dropout.  Keys between the sinks and the
  * window of a block of queries are not read.  Half types with equal head dimensions that are multiples of 8 up to 128
- * run on the tcgen05 kernel (P in q's type, as ts_attn_fwd), everything else on CUDA cores. */
-TS_ATTN_API int ts_attn_fwd_window(const ts_attn_params* params, const ts_window* window, void* stream);
+ * run on the tcgen05 kernels (P in q's type, as ts_attn_fwd), everything else on CUDA cores.  Chunks too short to give
+ * every SM a block are shared along their keys as in ts_attn_tree and then need the workspace; the environment variable
+ * TS_WINDOW_KERNEL = "split", "tile" or "pair" (a block for 128 or 256 queries), read at every call, forces one way where
+ * it supports the problem, for tests and measurements. */
+TS_ATTN_API int ts_attn_fwd_window(const ts_attn_params* params, const ts_window* window, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+TS_ATTN_API size_t ts_attn_fwd_window_workspace_size(const ts_attn_params* params, const ts_window* window);
 /* Kernel family of both directions: TS_PATH_TCGEN05 or TS_PATH_SIMT, or a negative ts_status. */
 TS_ATTN_API int ts_attn_window_path(const ts_attn_params* params, const ts_window* window);
 TS_ATTN_API size_t ts_attn_bwd_window_workspace_size(const ts_attn_bwd_params* params, const ts_window* window);

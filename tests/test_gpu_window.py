@@ -10,6 +10,13 @@ torch = pytest.importorskip("torch")
 from tensorsmith_b200 import engine  # noqa: E402
 
 
+@pytest.fixture(autouse=True, params=["chosen", "split", "tile", "pair"])
+def route(request, monkeypatch):
+    """The way the engine chooses, the one along the keys, and a block for one or two query tiles."""
+    if request.param != "chosen":
+        monkeypatch.setenv("TS_WINDOW_KERNEL", request.param)
+
+
 def heads(gen, rows, tokens, n, dim, dtype):
     """[B, H, T, D] as the projections give it: a view of [B, T, H, D]."""
     return torch.randn(rows, tokens, n, dim, generator=gen, device="cuda").to(DTYPES[dtype]).permute(0, 2, 1, 3)
@@ -86,8 +93,9 @@ def test_value_dimension_and_scale():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_wide_window_is_the_causal_rule(dtype):
+def test_wide_window_is_the_causal_rule(dtype, monkeypatch):
     """A window over everything gives what the call without one gives (same kernels for half types)."""
+    monkeypatch.setenv("TS_WINDOW_KERNEL", "pair")
     q, k, v, g, out, lse = run(dtype, 2, 4, 2, 300, 64, 2**31 - 1, 0)
     plain, plain_lse = engine.forward(q, k, v, is_causal=True)
     if dtype == "bf16":

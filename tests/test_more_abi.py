@@ -61,7 +61,8 @@ def test_window_refusals():
              (problem(head_dim=257), good, UNSUPPORTED), (problem(mask_kind=1, mask=FAKE), good, UNSUPPORTED),
              (problem(batch=70000), good, UNSUPPORTED)]
     for p, w, status in cases:
-        assert lib.ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), None) == status
+        assert lib.ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), FAKE, 1 << 40, None) == status
+        assert lib.ts_attn_fwd_window_workspace_size(ctypes.byref(p), ctypes.byref(w)) == 0
         assert lib.ts_attn_window_path(ctypes.byref(p), ctypes.byref(w)) == status
         b = _lib.AttnBwdParams()
         b.fwd = p
@@ -69,8 +70,8 @@ def test_window_refusals():
             getattr(b, name).data = FAKE
         assert lib.ts_attn_bwd_window(ctypes.byref(b), ctypes.byref(w), FAKE, 1 << 40, None) == status
         assert lib.ts_attn_bwd_window_workspace_size(ctypes.byref(b), ctypes.byref(w)) == 0
-    assert lib.ts_attn_fwd_window(None, ctypes.byref(good), None) == BAD
-    assert lib.ts_attn_fwd_window(ctypes.byref(problem()), None, None) == BAD
+    assert lib.ts_attn_fwd_window(None, ctypes.byref(good), FAKE, 1 << 40, None) == BAD
+    assert lib.ts_attn_fwd_window(ctypes.byref(problem()), None, FAKE, 1 << 40, None) == BAD
     b = _lib.AttnBwdParams()
     b.fwd = problem()
     assert lib.ts_attn_bwd_window(ctypes.byref(b), ctypes.byref(good), FAKE, 1 << 40, None) == BAD  # no gradients' views
