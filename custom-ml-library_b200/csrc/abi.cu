@@ -699,7 +699,7 @@ bool window_split_faster(const ts_attn_params& p, const tsa::WindowArgs& win, bo
   auto tiles = [&](int64_t queries) {
     const int64_t all = (p.kv_len + keys - 1) / keys;
     const int64_t near = (win.window + tsa::i64min(queries, p.q_len) + keys - 2) / keys + 1;
-    return (double)tsa::i64min(all, near + (win.sinks + keys - 1) / keys);
+    return (double)tsa::i64min(all, near + ((int64_t)win.sinks + keys - 1) / keys);
   };
   const int64_t blocks = (p.q_len + 16 * rt - 1) / (16 * rt) * heads, waves = (blocks + sms - 1) / sms;
   const double line = (double)units * (tiles(line_rows) + (tc ? 2 : 0)) / (tc ? sms : 2 * sms);

@@ -791,7 +791,7 @@ cudaError_t rows_window_fwd_t(const RowsWindow& a, cudaStream_t st) {
 template <typename A>
 void rows_key_blocks(const ts_attn_params& p, const WindowArgs& win, int rows, int cols, RowsKeyBlocks (&sets)[2],
                      size_t* bytes) {
-  const int blocks = ceil_div(p.kv_len, rows), with_sinks = min(blocks, ceil_div(win.sinks, rows));
+  const int blocks = ceil_div(p.kv_len, rows), with_sinks = ceil_div(min(win.sinks, p.kv_len), rows);
   const int64_t heads = (int64_t)p.kv_heads * p.batch, want = 6 * (int64_t)device_sms();
   size_t used = 0;
   for (int i = 0; i < 2; ++i) {

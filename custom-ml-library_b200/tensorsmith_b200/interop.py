@@ -42,12 +42,13 @@ def from_torch(t: torch.Tensor, like):
 
 def attention_node(query, key, value, *, mask=None, is_causal=False, scale=None, causal_offset=0,
                    kv_lens=None, dropout=None, op="sdpa_native", recording=True, compute=engine,
-                   decode_rows=None):
+                   decode_rows=None, window=None, sinks=0):
     """Attention output of ``query``/``key``/``value`` (Tensors of one tape implementation) as a
     Tensor of the same class: one ``_from_op`` node whose backward returns ``(dq, dk, dv)`` in the
     parents' array type and dtypes, or a plain Tensor when nothing is recorded.
 
-    ``dropout = (p, seed, offset)`` (the forward's draw, replayed by the backward).
+    ``dropout = (p, seed, offset)`` (the forward's draw, replayed by the backward); ``window`` and ``sinks`` as in
+    ``engine.forward``.
     ``decode_rows`` (query rows per KV head) lets a short, unmasked, unrecorded call take the
     split-K decode path."""
     cls = type(query)
@@ -57,8 +58,10 @@ def attention_node(query, key, value, *, mask=None, is_causal=False, scale=None,
     kwargs = dict(is_causal=is_causal, scale=scale, causal_offset=causal_offset, kv_lens=to_torch(kv_lens), mask=m)
     if dropout is not None:
         kwargs["dropout"] = dropout
+    if window is not None:
+        kwargs.update(window=window, sinks=sinks)
     if not recording:
-        if dropout is None and m is None and decode_rows is not None and decode_rows <= engine.DECODE_MAX_ROWS:
+        if window is None and dropout is None and m is None and decode_rows is not None and decode_rows <= engine.DECODE_MAX_ROWS:
             out, _ = compute.decode(q, k, v, **kwargs)
         else:
             out, _ = compute.forward(q, k, v, need_lse=False, **kwargs)

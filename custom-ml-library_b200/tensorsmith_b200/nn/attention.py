@@ -19,6 +19,15 @@ from ..tensor import Tensor, is_grad_enabled
 BACKENDS = {"auto", "dense", "streaming", "native"}
 
 
+def check_window(window, sinks) -> None:
+    """Raises unless ``window`` is None (and there are no sinks) or a positive size with sinks of zero or more."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+    elif not (isinstance(window, int) and isinstance(sinks, int) and 0 < window < 2**31 and 0 <= sinks < 2**31):
+        raise ValueError("a window must be a positive integer and the sinks an integer of zero or more")
+
+
 def scaled_dot_product_attention(
     query: Tensor,
     key: Tensor,
@@ -33,6 +42,8 @@ def scaled_dot_product_attention(
     block_size: int = 64,
     enable_gqa: bool = False,
     kv_lens=None,
+    window: int | None = None,
+    sinks: int = 0,
 ) -> Tensor:
     """Attention for [batch, heads, sequence, channels] tensors.
 
@@ -43,6 +54,10 @@ def scaled_dot_product_attention(
     Engine extension: ``kv_lens`` (int32 [B] on the device) gives each batch
     row its own number of valid keys, with its queries at the end of them;
     it is what ``KVCache`` passes for ragged rows.
+
+    Engine extension: ``window`` (with ``is_causal``, without mask and dropout)
+    lets the query at position i see the keys j <= i with i - j < window, and
+    the first ``sinks`` keys.
     """
     if any(t.ndim != 4 for t in (query, key, value)):
         raise ValueError("attention expects [batch, heads, sequence, channels]")
@@ -63,6 +78,9 @@ def scaled_dot_product_attention(
         raise ValueError("query/key head dimensions must match and sequences must be nonempty")
     if not 0 <= dropout_p < 1 or block_size <= 0 or causal_offset < 0:
         raise ValueError("invalid dropout probability, block size, or causal offset")
+    check_window(window, sinks)
+    if window is not None and (not is_causal or attn_mask is not None or dropout_p):
+        raise ValueError("a sliding window needs is_causal and takes neither an attention mask nor dropout")
     if backend not in BACKENDS:
         raise ValueError("attention backend must be auto, dense, streaming, or native")
     if query.device.type != "cuda":
@@ -92,7 +110,8 @@ def scaled_dot_product_attention(
     dropout = engine.DROPOUT_GENERATOR.draw(dropout_p) if dropout_p else None  # one draw per call
     return interop.attention_node(query, key, value, mask=mask, is_causal=is_causal, scale=multiplier,
                                   causal_offset=causal_offset, kv_lens=kv_lens, dropout=dropout,
-                                  op="sdpa_" + selected, recording=recording, decode_rows=repetitions * qlen)
+                                  op="sdpa_" + selected, recording=recording, decode_rows=repetitions * qlen,
+                                  window=window, sinks=sinks)
 
 
 def rotary_embedding(input: Tensor, offset: int = 0, base: float = 10000.0, rotary_dim: int | None = None) -> Tensor:

@@ -46,6 +46,51 @@ def _torch_dtype(dtype) -> torch.dtype:
         raise TypeError("cache compute dtype must be floating point") from None
 
 
+def keep_drafts(caches, drafted: int, path, counts=None) -> None:
+    """Close the caches of all layers behind the accepted paths of a tree of drafted tokens (engine extension).
+
+    The last ``drafted`` tokens of every row are the tree's nodes.  Row b keeps the nodes ``path[b, :counts[b]]``
+    (ascending, as on a path from the root; all of them where ``counts`` is None), which move behind its committed
+    tokens, and has its own length from then on."""
+    caches = list(caches)
+    if not caches:
+        raise ValueError("no cache to keep tokens of")
+    first = caches[0]
+    lengths = first.lengths
+    if any(type(c) is not KVCache or not np.array_equal(c.lengths, lengths) or c.device != first.device
+           or c.quantized != first.quantized for c in caches):
+        raise ValueError("the caches of all layers must be KVCaches of one kind at the same position")
+    host = _host_ints(path)
+    if host.ndim != 2 or host.shape[0] != first.batch_size:
+        raise ValueError("path must be integers [batch, nodes]")
+    taken = np.full(host.shape[0], host.shape[1]) if counts is None else _host_ints(counts)
+    if taken.shape != (host.shape[0],) or (taken < 0).any() or (taken > host.shape[1]).any():
+        raise ValueError("counts must be one number of path entries a row")
+    if drafted < 0 or (lengths < drafted).any():
+        raise ValueError("the caches hold fewer tokens than were drafted")
+    used = np.arange(host.shape[1]) < taken[:, None]
+    steps = np.diff(host, axis=1) > 0
+    if ((host < 0) | (host >= drafted))[used].any() or not steps[used[:, 1:]].all():
+        raise ValueError("a path must be ascending nodes of the tree")
+    base = lengths - drafted
+    if taken.any():
+        dev = first._keys.device
+        ints = [torch.as_tensor(x.astype(np.int32), device=dev) for x in (base, np.where(used, host, 0), taken)]
+        engine.kv_keep([(c._keys, c._values) for c in caches], *ints)
+        if first.quantized:
+            engine.kv_keep([(c._key_scales, c._value_scales) for c in caches], *ints)
+    for c in caches:
+        c.set_lengths(base + taken)
+
+
+def _host_ints(x) -> np.ndarray:
+    raw = x._data if isinstance(x, Tensor) else x
+    host = raw.detach().cpu().numpy() if isinstance(raw, torch.Tensor) else np.asarray(raw)
+    if host.dtype.kind not in "iu":
+        raise ValueError("expected integers")
+    return host.astype(np.int64)
+
+
 class KVCache:
     """Preallocated [B,H,capacity,D] keys/values for autoregressive inference."""
 
@@ -235,6 +280,11 @@ class KVCache:
             self._key_scales, self._value_scales = ks, vs
         if self._host_lens is not None:
             self.set_lengths(self._host_lens[host])
+
+    def keep(self, drafted: int, path, counts=None) -> None:
+        """Forget the last ``drafted`` tokens of every row but those of its accepted path (engine extension):
+        ``keep_drafts`` for this cache alone."""
+        keep_drafts([self], drafted, path, counts)
 
     @property
     def storage(self) -> tuple:

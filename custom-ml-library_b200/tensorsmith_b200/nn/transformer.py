@@ -34,7 +34,7 @@ import torch.nn.functional as F
 
 from .. import engine
 from ..tensor import Tensor, is_grad_enabled, no_grad
-from .attention import BACKENDS, scaled_dot_product_attention
+from .attention import BACKENDS, check_window, scaled_dot_product_attention
 from .cache import KVCache
 from .paged import PagedKVCache, PagedLayer
 
@@ -61,18 +61,47 @@ class _AttentionFn(torch.autograd.Function):
     """Attention forward / recomputing backward on the engine (nn/attention.py:132-252)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, is_causal, causal_offset, scale, dropout):
-        out, lse = engine.forward(q, k, v, is_causal=is_causal, causal_offset=causal_offset, scale=scale,
-                                  need_lse=True, dropout=dropout)
+    def forward(ctx, q, k, v, is_causal, causal_offset, scale, dropout, window, sinks):
+        kw = dict(is_causal=is_causal, causal_offset=causal_offset, scale=scale, dropout=dropout, window=window,
+                  sinks=sinks)
+        out, lse = engine.forward(q, k, v, need_lse=True, **kw)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.kw = dict(is_causal=is_causal, causal_offset=causal_offset, scale=scale, dropout=dropout)
+        ctx.kw = kw
         return out
 
     @staticmethod
     def backward(ctx, g):
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv = engine.backward(q, k, v, out, lse, g.contiguous(), **ctx.kw)
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    """Log probabilities, entropies and alternatives of logits; their joint gradient in one pass."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, top, ignore_index):
+        result = engine.token_logprobs(logits, targets, top=top, ignore_index=ignore_index)
+        ctx.save_for_backward(logits, targets, *result)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(result.top_indices, result.norm)
+        ctx.set_materialize_grads(False)
+        return tuple(result)
+
+    @staticmethod
+    def backward(ctx, g_logprob, g_entropy, g_top, *_):
+        logits, targets, *result = ctx.saved_tensors
+        grads = [None if g is None else g.float() for g in (g_logprob, g_entropy, g_top)]
+        if all(g is None for g in grads):
+            return None, None, None, None
+        return engine.token_logprobs_backward(logits, targets, engine.TokenLogprobs(*result), *grads,
+                                              ignore_index=ctx.ignore_index), None, None, None
+
+
+def token_logprobs(logits, targets, *, top: int = 0, ignore_index: int = -100) -> engine.TokenLogprobs:
+    """Log probabilities of ``targets`` [...] under ``logits`` [..., V], entropies and the ``top`` most likely
+    alternatives (``engine.token_logprobs``), differentiable in ``logits``."""
+    return engine.TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, top, ignore_index))
 
 
 def _param(shape, bound=None, *, std=None, device=None, ones=False):
@@ -195,7 +224,7 @@ class MultiHeadAttention(_Module):
     """Self attention with grouped-query heads and rotary positions (nn/transformer.py:49-155)."""
 
     def __init__(self, embed_dim, num_heads, *, num_kv_heads=None, dropout=0.0, bias=False, rotary=True,
-                 backend="auto", device=None):
+                 backend="auto", window=None, sinks=0, device=None):
         kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if min(embed_dim, num_heads, kv_heads) <= 0 or embed_dim % num_heads or num_heads % kv_heads:
             raise ValueError("embed_dim must divide into heads and query heads must divide into KV groups")
@@ -205,13 +234,20 @@ class MultiHeadAttention(_Module):
             raise ValueError("rotary attention requires an even head dimension")
         if not 0 <= dropout < 1 or backend not in BACKENDS:
             raise ValueError("invalid attention dropout/backend")
+        check_window(window, sinks)
+        if window is not None and dropout:
+            raise ValueError("a sliding window takes no attention dropout")
+        self.window, self.sinks = window, sinks
         self.rotary, self.backend, self.dropout_p = rotary, backend, dropout
         self.q_proj = Linear(embed_dim, embed_dim, bias=bias, device=device)
         self.k_proj = Linear(embed_dim, kv_heads * self.head_dim, bias=bias, device=device)
         self.v_proj = Linear(embed_dim, kv_heads * self.head_dim, bias=bias, device=device)
         self.out_proj = Linear(embed_dim, embed_dim, bias=bias, device=device)
 
-    def forward(self, input, context=None, *, attn_mask=None, is_causal=True, cache: KVCache | None = None):
+    def forward(self, input, context=None, *, attn_mask=None, is_causal=True, cache: KVCache | None = None,
+                parents=None):
+        """``parents`` (int32 [B, T], with a cache): the input tokens are a tree of drafted ones, as in
+        ``engine.attention_tree``.  A ``KVCache`` whose rows have their own lengths is continued row by row."""
         if input.ndim != 3 or input.shape[-1] != self.embed_dim:
             raise ValueError("attention input must be [batch, sequence, embed_dim]")
         source = input if context is None else context
@@ -222,6 +258,12 @@ class MultiHeadAttention(_Module):
             raise RuntimeError(
                 "cached self-attention requires eval() and no_grad(); cross-attention caching is not supported"
             )
+        if self.window is not None and (not is_causal or attn_mask is not None or context is not None
+                                        or isinstance(cache, PagedLayer)):
+            raise ValueError("a sliding window needs causal self-attention without a mask, over a plain cache")
+        if parents is not None and (cache is None or not is_causal or attn_mask is not None
+                                    or isinstance(cache, PagedLayer)):
+            raise ValueError("drafted trees need causal attention over a KVCache, without a mask")
         batch, steps, _ = input.shape
         offset = 0 if cache is None else cache.length
         if attn_mask is not None:
@@ -245,7 +287,8 @@ class MultiHeadAttention(_Module):
                 q = _RopeFn.apply(q, offset)
                 k = _RopeFn.apply(k, offset if context is None else 0)
             draw = engine.DROPOUT_GENERATOR.draw(dropout) if dropout else None
-            attended = _AttentionFn.apply(q, k, v, is_causal, offset, 1 / math.sqrt(self.head_dim), draw)
+            attended = _AttentionFn.apply(q, k, v, is_causal, offset, 1 / math.sqrt(self.head_dim), draw, self.window,
+                                          self.sinks)
         else:
             if recording:
                 raise NotImplementedError("training with an explicit attention mask is not routed to the engine")
@@ -256,6 +299,10 @@ class MultiHeadAttention(_Module):
                 (cache.append_rotary if self.rotary else cache.append)(_mirror(k), _mirror(v))
                 q_t = _mirror(engine.rope(q, positions=cache.cache.positions) if self.rotary else q)
                 attended = cache.attend(q_t, is_causal=is_causal)._data
+                return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
+            if parents is not None or (type(cache) is KVCache and cache.seq_lens is not None and is_causal
+                                       and attn_mask is None):
+                attended = self._attend_rows(q, k, v, cache, parents)
                 return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
             q_t = _mirror(engine.rope(q, offset=offset) if self.rotary else q)
             if cache is not None:
@@ -269,24 +316,40 @@ class MultiHeadAttention(_Module):
                 v_t = _mirror(v)
             mask = None if attn_mask is None else _mirror(attn_mask)
             attended = scaled_dot_product_attention(q_t, k_t, v_t, mask, dropout, is_causal, causal_offset=offset,
-                                                    backend=self.backend, enable_gqa=gqa)._data
+                                                    backend=self.backend, enable_gqa=gqa, window=self.window,
+                                                    sinks=self.sinks)._data
         return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
+
+
+    def _attend_rows(self, q, k, v, cache, parents):
+        """A step over a cache whose rows stand at their own lengths, or of drafted trees: every row's tokens take the
+        slots behind its keys, and positions by their depth in the tree."""
+        lens = cache.seq_lens
+        if lens is None:
+            lens = torch.full((q.shape[0],), cache.length, dtype=torch.int32, device=q.device)
+        if self.rotary:
+            positions = lens if parents is None else engine.tree_positions(parents, lens)
+            q, k = engine.rope(q, positions=positions), engine.rope(k, positions=positions)
+        after = lens + q.shape[2]
+        keys, values = cache.append(_mirror(k), _mirror(v))
+        return engine.attention_tree(q, keys._data, values._data, after, parents, window=self.window,
+                                     sinks=self.sinks)[0]
 
 
 class TransformerDecoderBlock(_Module):
     """Pre-RMSNorm block: GQA/RoPE attention and a SwiGLU MLP (nn/transformer.py:158-194)."""
 
     def __init__(self, dim, num_heads, hidden_dim=None, *, num_kv_heads=None, dropout=0.0,
-                 attention_backend="auto", device=None):
+                 attention_backend="auto", window=None, sinks=0, device=None):
         self.attention_norm = RMSNorm(dim, device=device)
         self.attention = MultiHeadAttention(dim, num_heads, num_kv_heads=num_kv_heads, dropout=dropout,
-                                            backend=attention_backend, device=device)
+                                            backend=attention_backend, window=window, sinks=sinks, device=device)
         self.residual_dropout = dropout
         self.ffn_norm = RMSNorm(dim, device=device)
         self.ffn = SwiGLU(dim, hidden_dim or 4 * dim, dropout, device)
 
-    def forward(self, input, *, cache=None, attn_mask=None):
-        a = self.attention(self.attention_norm(input), cache=cache, attn_mask=attn_mask)
+    def forward(self, input, *, cache=None, attn_mask=None, parents=None):
+        a = self.attention(self.attention_norm(input), cache=cache, attn_mask=attn_mask, parents=parents)
         if self.residual_dropout and self.training:
             a = F.dropout(a, self.residual_dropout, True)
         hidden = input + a
@@ -305,6 +368,8 @@ class TransformerConfig:
     dropout: float = 0.0
     tie_weights: bool = True
     attention_backend: str = "auto"
+    window: int | None = None  # tokens that a token sees, itself included (None: all before it)
+    sinks: int = 0             # first tokens that every token sees under a window
 
     def __post_init__(self):
         if min(self.vocab_size, self.dim, self.num_heads, self.num_layers, self.max_seq_len) <= 0:
@@ -318,6 +383,9 @@ class TransformerConfig:
             raise ValueError("dropout must be in [0, 1)")
         if self.attention_backend not in BACKENDS:
             raise ValueError("invalid attention backend")
+        check_window(self.window, self.sinks)
+        if self.window is not None and self.dropout:
+            raise ValueError("a sliding window takes no attention dropout")
 
 
 def _as_tokens(tokens, device) -> torch.Tensor:
@@ -339,7 +407,7 @@ class TransformerLM(_Module):
         self.blocks = [
             TransformerDecoderBlock(config.dim, config.num_heads, config.hidden_dim, num_kv_heads=config.num_kv_heads,
                                     dropout=config.dropout, attention_backend=config.attention_backend,
-                                    device=device)
+                                    window=config.window, sinks=config.sinks, device=device)
             for _ in range(config.num_layers)
         ]
         self.final_norm = RMSNorm(config.dim, device=device)
@@ -351,12 +419,22 @@ class TransformerLM(_Module):
         for name, value in super().named_parameters(prefix):
             yield name.replace("token_embedding_weight", "token_embedding.weight"), value
 
-    def forward(self, tokens, *, caches: list[KVCache] | None = None, attn_mask=None, logits_to_keep: int = 0):
+    def forward(self, tokens, *, caches: list[KVCache] | None = None, attn_mask=None, logits_to_keep: int = 0,
+                parents=None):
+        """``parents`` (integers [B, T], with caches): the tokens are trees of drafted ones; node i's parent is an
+        earlier node, -1 the last token in the cache, anything else marks padding (``engine.attention_tree``).
+        ``keep_drafts`` then closes the caches behind the accepted nodes."""
         tokens = _as_tokens(tokens, self.device)
         if tokens.ndim != 2 or tokens.dtype not in (torch.int32, torch.int64) or tokens.shape[1] == 0:
             raise ValueError("tokens must be a nonempty integer [batch, time] tensor")
         if not isinstance(logits_to_keep, int) or not 0 <= logits_to_keep <= tokens.shape[1]:
             raise ValueError("logits_to_keep must be between zero (all) and the input length")
+        if parents is not None:
+            if caches is None:
+                raise ValueError("drafted trees need caches")
+            parents = torch.as_tensor(parents).to(self.device, torch.int32).contiguous()
+            if parents.shape != tokens.shape:
+                raise ValueError("parents must be one integer a token")
         offset = 0
         if caches is not None:
             if len(caches) != len(self.blocks) or len({cache.length for cache in caches}) != 1:
@@ -366,6 +444,7 @@ class TransformerLM(_Module):
             offset = caches[0].length
             # a paged cache's rows may differ in length
             starts = [cache.cache.lengths if isinstance(cache, PagedLayer) else offset for cache in caches]
+            rows = [cache.lengths if type(cache) is KVCache and cache.seq_lens is not None else None for cache in caches]
             for block, cache in zip(self.blocks, caches):
                 if cache.batch_size != tokens.shape[0] or cache.device.index != self._device_index:
                     raise ValueError("cache batch/device does not match tokens")
@@ -382,15 +461,18 @@ class TransformerLM(_Module):
             hidden = F.dropout(hidden, self.config.dropout, True)
         try:
             for i, block in enumerate(self.blocks):
-                hidden = block(hidden, cache=None if caches is None else caches[i], attn_mask=attn_mask)
+                hidden = block(hidden, cache=None if caches is None else caches[i], attn_mask=attn_mask, parents=parents)
             if logits_to_keep:
                 hidden = hidden[:, -logits_to_keep:, :]
             return F.linear(self.final_norm(hidden), self.output_weight).float()
         except Exception:
             if caches is not None:
                 # Roll every cache back to where this call started (nn/transformer.py:308-312).
-                for cache, start in zip(caches, starts):
-                    cache.truncate(start)
+                for cache, start, own in zip(caches, starts, rows):
+                    if own is None:
+                        cache.truncate(start)
+                    else:
+                        cache.set_lengths(own)
             raise
 
     def loss(self, tokens, targets, *, ignore_index=-100, label_smoothing=0.0):
@@ -399,6 +481,12 @@ class TransformerLM(_Module):
         return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1), ignore_index=ignore_index,
                                label_smoothing=label_smoothing)
 
+    def token_logprobs(self, tokens, targets, *, top: int = 0, ignore_index: int = -100) -> engine.TokenLogprobs:
+        """Log probabilities that the model gives ``targets`` [B, T] after ``tokens`` [B, T], with entropies and the
+        ``top`` most likely alternatives (``nn.token_logprobs``)."""
+        targets = _as_tokens(targets, self.device).long()
+        return token_logprobs(self(tokens), targets, top=top, ignore_index=ignore_index)
+
     def new_cache(self, batch_size: int, max_seq_len: int | None = None, *, quantized=False,
                   num_pages: int | None = None) -> list[KVCache]:
         """One cache a block: plain, int8 (``quantized=True``), or the layers of a ``PagedKVCache`` in 4 bits
@@ -406,6 +494,8 @@ class TransformerLM(_Module):
         capacity = self.config.max_seq_len if max_seq_len is None else max_seq_len
         if capacity <= 0 or capacity > self.config.max_seq_len:
             raise ValueError("cache capacity must fit the model context")
+        if quantized == "int4" and self.config.window is not None:
+            raise ValueError("a paged cache takes no sliding window")
         if quantized == "int4":
             attention = self.blocks[0].attention
             return PagedKVCache(batch_size, len(self.blocks), attention.num_kv_heads, attention.head_dim, capacity,

@@ -59,7 +59,7 @@ def test_head_dimensions(dtype, dim):
 # Windows around the tiles of 128 keys and 64 queries, sinks within and over a tile, one token to several tiles.
 @pytest.mark.parametrize("tokens,window,sinks", [
     (1, 1, 0), (2, 1, 1), (127, 5, 0), (129, 128, 1), (256, 129, 130), (257, 1, 0), (385, 127, 127), (513, 300, 0),
-    (700, 64, 260), (640, 700, 5), (1000, 999, 1000), (900, 256, 128)])
+    (700, 64, 260), (640, 700, 5), (1000, 999, 1000), (900, 256, 128), (300, 40, 2**31 - 1)])
 def test_window_edges(tokens, window, sinks):
     run("bf16", 1, 2, 1, tokens, 64, window, sinks, path="tcgen05")
 
