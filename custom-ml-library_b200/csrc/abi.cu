@@ -641,7 +641,7 @@ cudaError_t rows_window_bwd(const ts_attn_bwd_params& bp, const tsa::WindowArgs&
                   tsa::rows_window_bwd_bf16, bp, win, bytes, ws, st);
 }
 size_t window_bwd_workspace(const ts_attn_bwd_params& bp, const tsa::WindowArgs& win) {
-  if (tsa::tc_bwd_window_supported(bp)) return tsa::tc_bwd_workspace(bp);
+  if (tsa::tc_bwd_window_supported(bp)) return tsa::tc_bwd_window_workspace(bp, win);
   size_t bytes = 0;
   (void)rows_window_bwd(bp, win, &bytes, nullptr, nullptr);
   return bytes;

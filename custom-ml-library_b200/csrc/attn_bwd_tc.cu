@@ -45,6 +45,7 @@
 #include "tc_bwd.cuh"
 #include "tc_fwd.cuh"
 #include "tc_util.cuh"
+#include "tree.cuh"
 #include "window.cuh"
 
 namespace tsa {
@@ -94,7 +95,11 @@ struct TcBwdArgs {
   int n_k_tiles;
   uint32_t* fault;
   DropoutArgs drop;  // used by the kDrop instantiation only
-  WindowArgs win;    // used by the kWin instantiation only
+  // Used by the kWin instantiation only: the window; key tiles with sinks, the parts that each one's queries are
+  // divided into, and where the parts leave dK and dV: [part][batch x KV heads][tile][128 keys][dK | dV][D] fp32.
+  WindowArgs win;
+  int sink_tiles, sink_parts;
+  float* sink_sums;
 };
 
 }  // namespace
@@ -119,8 +124,13 @@ __global__ void __launch_bounds__(512, 1)
   float* sStat = reinterpret_cast<float*>(smem + C::kOffStat);  // [buf][lse2 | delta][64]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // kWin: every (head, row) of key tile 0 first, as a tile with sinks is seen by all the queries behind it.
-  const int kt = kWin ? blockIdx.y : blockIdx.x;
+  // kWin: the key tiles with sinks, which all the queries behind them see, first, and each in parts where they would
+  // outlast everything else.
+  const int divided = kWin ? args.sink_tiles * args.sink_parts : 0;
+  const bool in_parts = kWin && args.sink_parts > 1 && (int)blockIdx.y < divided;
+  const int kt = !kWin                      ? (int)blockIdx.x
+                 : (int)blockIdx.y < divided ? (int)blockIdx.y / args.sink_parts
+                                             : (int)blockIdx.y - divided + args.sink_tiles;
   const int hk = kWin ? (int)blockIdx.x % p.kv_heads : (int)blockIdx.y;
   const int b = kWin ? (int)blockIdx.x / p.kv_heads : (int)blockIdx.z;
   const int rep = p.q_heads / p.kv_heads;
@@ -142,7 +152,12 @@ __global__ void __launch_bounds__(512, 1)
     qt_end = last < 0 ? 0 : (int)i64min(n_qt_all, last / kBM + 1);
   }
   const int n_qt = k0 < kv_end ? max(0, qt_end - qt_start) : 0;
-  const int n_it = rep * n_qt;
+  int it0 = 0, n_it = rep * n_qt;
+  if (in_parts) {
+    const int64_t part = blockIdx.y % args.sink_parts;
+    it0 = (int)(part * n_it / args.sink_parts);
+    n_it = (int)((part + 1) * n_it / args.sink_parts) - it0;
+  }
   const bool dead = fault_set(args.fault);
 
   if (threadIdx.x == 0) {
@@ -168,8 +183,8 @@ __global__ void __launch_bounds__(512, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
-  auto it_head = [&](int it) { return hk * rep + it / n_qt; };
-  auto it_q0 = [&](int it) { return (qt_start + it % n_qt) * kBM; };
+  auto it_head = [&](int it) { return hk * rep + (kWin ? it + it0 : it) / n_qt; };
+  auto it_q0 = [&](int it) { return (qt_start + (kWin ? it + it0 : it) % n_qt) * kBM; };
 
   if (warp == 0) {
     // ------------------------------ producer ------------------------------
@@ -405,7 +420,14 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
         }
-        if (store_row) {
+        if (kWin && in_parts) {
+          const int64_t tile = ((int64_t)(blockIdx.y % args.sink_parts) * gridDim.x + blockIdx.x) * args.sink_tiles + kt;
+          float* sums = args.sink_sums + ((tile * kBN + row) * 2 + which) * D + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(sums + e) = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]),
+                                                               __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+        } else if (store_row) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             const float* f = reinterpret_cast<const float*>(r + e);
@@ -543,6 +565,61 @@ size_t tc_bwd_workspace(const ts_attn_bwd_params& bp) {
   return align256(stats * sizeof(float)) + align256(rows * padded_dim(p.head_dim) * sizeof(float));
 }
 
+// How the key tiles with sinks are divided.  A CTA's time is its number of (query tile, head) pairs; undivided, a tile
+// with sinks takes those of all queries.  Parts of half an SM's even share of all pairs (16 at least) end no later
+// than the rest (16000 queries, 4 heads on one KV head of 128, a window of 500, 4 sinks: 131 us, 1668 undivided).
+struct SinkParts {
+  int tiles, parts;
+};
+static SinkParts sink_parts(const ts_attn_params& p, const WindowArgs& win) {
+  const int64_t rep = p.q_heads / p.kv_heads, heads = (int64_t)p.kv_heads * p.batch;
+  const int64_t tiles = ceil_div(p.kv_len, kBN), with_sinks = ceil_div(min(win.sinks, p.kv_len), kBN);
+  if (with_sinks == 0) return SinkParts{0, 1};
+  const int64_t all = rep * ceil_div(p.q_len, kBM);
+  const int64_t near = rep * i64min(ceil_div(p.q_len, kBM), ((int64_t)win.window + kBN) / kBM + 1);
+  const int64_t share = heads * (with_sinks * all + (tiles - with_sinks) * near) / device_sms();
+  const int64_t parts = (all + i64max(16, share / 2) - 1) / i64max(16, share / 2);
+  return SinkParts{(int)with_sinks, (int)i64max(1, i64min(64, parts))};
+}
+
+size_t tc_bwd_window_workspace(const ts_attn_bwd_params& bp, const WindowArgs& win) {
+  const SinkParts sinks = sink_parts(bp.fwd, win);
+  const size_t floats = sinks.parts > 1 ? (size_t)sinks.parts * bp.fwd.batch * bp.fwd.kv_heads * sinks.tiles * kBN * 2 *
+                                              padded_dim(bp.fwd.head_dim)
+                                        : 0;
+  return tc_bwd_workspace(bp) + floats * sizeof(float);
+}
+
+// dK and dV of the tiles with sinks from their parts, added in order; a thread four channels of a key.
+template <typename T>
+__global__ void __launch_bounds__(256) sink_sum_kernel(const __grid_constant__ TcBwdArgs a, int dim) {
+  const ts_attn_params& p = a.p;
+  const int quads = dim / 4;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t all = (int64_t)p.batch * p.kv_heads * a.sink_tiles * kBN * 2 * quads;  // of a part
+  if (x >= all) return;
+  const int ch = (int)(x % quads) * 4, which = (int)(x / quads % 2), key = (int)(x / (2 * quads) % (a.sink_tiles * kBN));
+  const int bh = (int)(x / (2 * quads) / (a.sink_tiles * kBN));
+  if (key >= p.kv_len || ch >= p.head_dim) return;
+  const float4* from = reinterpret_cast<const float4*>(a.sink_sums) + x;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < a.sink_parts; ++i) {
+    const float4 f = from[i * all];
+    sum.x += f.x;
+    sum.y += f.y;
+    sum.z += f.z;
+    sum.w += f.w;
+  }
+  const ts_view4& to = which ? a.dv : a.dk;
+  T* out = reinterpret_cast<T*>(to.data) + (int64_t)(bh / p.kv_heads) * to.stride[0] +
+           (int64_t)(bh % p.kv_heads) * to.stride[1] + (int64_t)key * to.stride[2] + ch;
+  out[0] = Elem<T>::from_acc(sum.x);
+  out[1] = Elem<T>::from_acc(sum.y);
+  out[2] = Elem<T>::from_acc(sum.z);
+  out[3] = Elem<T>::from_acc(sum.w);
+}
+
 // stats[bh][0][i] = -LSE*log2e (-inf for a fully masked row or i >= Tq) and
 // stats[bh][1][i] = -sum_c dO*O (0 for i >= Tq): the backward's row statistics
 // (nn/attention.py:231), one warp per padded row.
@@ -578,6 +655,54 @@ __global__ void bwd_stats_kernel(ts_attn_bwd_params bp, float* stats, int t_pad)
   }
 }
 
+// The same under a window: 8 or 16 lanes a row with 16-byte loads, four rows of each in flight (16 heads of 16384
+// rows of 128: 42 us, where a warp a row with loads of one element takes 95).
+template <typename T>
+__global__ void __launch_bounds__(256)
+    window_stats_kernel(const __grid_constant__ ts_attn_bwd_params bp, float* stats, int t_pad, int lanes) {
+  constexpr int kRows = 4;
+  const ts_attn_params& p = bp.fwd;
+  const int64_t total = (int64_t)p.batch * p.q_heads * t_pad;
+  const int c = threadIdx.x % lanes;
+  const int64_t row0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes * kRows;
+  // t_pad is a multiple of 64, so the rows of a thread belong to one head.
+  const int64_t bh = row0 / t_pad;
+  const int i0 = (int)(row0 - bh * t_pad), b = (int)(bh / p.q_heads), h = (int)(bh - (int64_t)b * p.q_heads);
+  uint4 g[kRows], o[kRows];
+  float lse[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t i = i0 + u;
+    g[u] = o[u] = make_uint4(0u, 0u, 0u, 0u);
+    lse[u] = -INFINITY;
+    if (row0 < total && i < p.q_len) {
+      if (8 * c < p.value_dim) {
+        g[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(bp.dout.data) + b * bp.dout.stride[0] +
+                                               h * bp.dout.stride[1] + i * bp.dout.stride[2] + 8 * c);
+        o[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.o.data) + b * p.o.stride[0] +
+                                               h * p.o.stride[1] + i * p.o.stride[2] + 8 * c);
+      }
+      if (c == 0)
+        lse[u] = reinterpret_cast<const float*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
+                                                       (int64_t)i * p.lse_stride[2]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const T *x = reinterpret_cast<const T*>(&g[u]), *y = reinterpret_cast<const T*>(&o[u]);
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf(Elem<T>::to_acc(x[e]), Elem<T>::to_acc(y[e]), acc);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1)
+      if (off < lanes) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (c == 0 && row0 < total) {
+      stats[bh * 2 * t_pad + i0 + u] = lse[u] == -INFINITY ? -INFINITY : -lse[u] * kLog2e;
+      stats[bh * 2 * t_pad + t_pad + i0 + u] = -acc;
+    }
+  }
+}
+
 template <int D, bool BF16>
 static cudaError_t launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                               const CUtensorMap& mdo, const TcBwdArgs& a, cudaStream_t st) {
@@ -587,7 +712,8 @@ static cudaError_t launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, cons
                                : tc_bwd_kernel<D, BF16, false, false>;
   cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kern), BwdCfg<D>::kSmem);
   if (e != cudaSuccess) return e;
-  const dim3 grid = win ? dim3((unsigned)(a.p.kv_heads * a.p.batch), a.n_k_tiles) : dim3(a.n_k_tiles, a.p.kv_heads, a.p.batch);
+  const dim3 grid = win ? dim3((unsigned)(a.p.kv_heads * a.p.batch), a.n_k_tiles + a.sink_tiles * (a.sink_parts - 1))
+                        : dim3(a.n_k_tiles, a.p.kv_heads, a.p.batch);
   kern<<<grid, 512, BwdCfg<D>::kSmem, st>>>(mq, mk, mv, mdo, a);
   return cudaGetLastError();
 }
@@ -607,7 +733,14 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
       !make_map(&mv, p.v, p.dtype, p.batch, p.kv_heads, p.kv_len, p.value_dim, kBN) ||
       !make_map(&mdo, bp.dout, p.dtype, p.batch, p.q_heads, p.q_len, p.value_dim, kBM))
     return cudaErrorInvalidValue;
-  {
+  if (win) {
+    const int lanes = p.value_dim <= 64 ? 8 : 16;
+    const unsigned blocks = (unsigned)(((int64_t)p.batch * p.q_heads * t_pad * lanes / 4 + 255) / 256);
+    if (p.dtype == TS_BF16)
+      window_stats_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(bp, stats, t_pad, lanes);
+    else
+      window_stats_kernel<__half><<<blocks, 256, 0, st>>>(bp, stats, t_pad, lanes);
+  } else {
     const int64_t warps = (int64_t)p.batch * p.q_heads * t_pad;
     const unsigned blocks = (unsigned)((warps * 32 + 255) / 256);
     if (p.dtype == TS_BF16)
@@ -619,7 +752,7 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
   if (e != cudaSuccess) return e;
   e = cudaMemsetAsync(dq_acc, 0, rows * padded_dim(p.head_dim) * sizeof(float), st);
   if (e != cudaSuccess) return e;
-  TcBwdArgs a;
+  TcBwdArgs a = {};
   a.p = p;
   a.dk = bp.dk;
   a.dv = bp.dv;
@@ -630,12 +763,29 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
   a.fault = fault;
   a.drop = drop ? *drop : DropoutArgs{};
   a.win = win ? *win : WindowArgs{};
+  if (win) {
+    const SinkParts sinks = sink_parts(p, *win);
+    a.sink_tiles = sinks.tiles;
+    a.sink_parts = sinks.parts;
+    a.sink_sums = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(ws) + tc_bwd_workspace(bp));
+  }
   const bool bf = p.dtype == TS_BF16;
   if (p.head_dim <= 64)
     e = bf ? launch_bwd<64, true>(mq, mk, mv, mdo, a, st) : launch_bwd<64, false>(mq, mk, mv, mdo, a, st);
   else
     e = bf ? launch_bwd<128, true>(mq, mk, mv, mdo, a, st) : launch_bwd<128, false>(mq, mk, mv, mdo, a, st);
   if (e != cudaSuccess) return e;
+  if (win && a.sink_parts > 1) {
+    const int dim = padded_dim(p.head_dim);
+    const int64_t quads = (int64_t)p.batch * p.kv_heads * a.sink_tiles * kBN * 2 * (dim / 4);
+    const unsigned blocks = (unsigned)((quads + 255) / 256);
+    if (bf)
+      sink_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, dim);
+    else
+      sink_sum_kernel<__half><<<blocks, 256, 0, st>>>(a, dim);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
   const dim3 cgrid((unsigned)(p.batch * p.q_heads), (unsigned)(t_pad / kBM));
   const int n_tiles = t_pad / kBM;
   if (p.head_dim <= 64) {

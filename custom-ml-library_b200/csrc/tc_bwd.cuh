@@ -14,4 +14,5 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* workspace, size_t wo
                         cudaStream_t stream, const DropoutArgs* drop = nullptr, const WindowArgs* win = nullptr);
 // True when it takes a forward that had a sliding window (tc_window_supported).
 bool tc_bwd_window_supported(const ts_attn_bwd_params& bp);
+size_t tc_bwd_window_workspace(const ts_attn_bwd_params& bp, const WindowArgs& win);
 }  // namespace tsa

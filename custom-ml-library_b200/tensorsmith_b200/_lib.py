@@ -296,17 +296,13 @@ SIGNATURES = {
          ctypes.c_void_p],
     ),
     "ts_attn_fwd_window": (
-        ctypes.c_int,
-        [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+        ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     ),
-    "ts_attn_fwd_window_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
-    "ts_attn_window_path": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
-    "ts_attn_bwd_window_workspace_size": (
-        ctypes.c_size_t, [ctypes.POINTER(AttnBwdParams), ctypes.POINTER(Window)]
-    ),
+    "ts_attn_fwd_window_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_attn_window_path": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_attn_bwd_window_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
     "ts_attn_bwd_window": (
-        ctypes.c_int,
-        [ctypes.POINTER(AttnBwdParams), ctypes.POINTER(Window), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+        ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     ),
     "ts_attn_tree": (
         ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
@@ -323,11 +319,11 @@ SIGNATURES = {
         [View4, View4, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p],
     ),
-    "ts_kv_keep": (ctypes.c_int, [ctypes.POINTER(KvKeepParams), ctypes.c_void_p]),
-    "ts_token_logprobs_fwd": (ctypes.c_int, [ctypes.POINTER(TokenLogprobs), ctypes.c_void_p]),
+    "ts_kv_keep": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "ts_token_logprobs_fwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "ts_token_logprobs_bwd": (
         ctypes.c_int,
-        [ctypes.POINTER(TokenLogprobs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+        [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_int64, ctypes.c_void_p],
     ),
     "ts_attn_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),

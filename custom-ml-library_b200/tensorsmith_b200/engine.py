@@ -58,12 +58,40 @@ def _stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# Calls that cost a few microseconds on the device pack their structs in one go (the layouts of _lib.AttnParams,
+# _lib.Kv4Cache, _lib.PagePool and so on) instead of field by field.
+_ATTN_STRUCT = struct.Struct("@" + "P4q" * 4 + "P3q" + "8i" + "d" + "iq" + "P" + "iP4q")
+_VIEW_STRUCT = struct.Struct("@P4q")
+_KV4_STRUCT = struct.Struct("@PqPq6i")
+_POOL_STRUCT = struct.Struct("@Pqqqii")
+_WINDOW_STRUCT = struct.Struct("@ii")
+_TREE_STRUCT = struct.Struct("@Pqii")
+_KEEP_STRUCT = struct.Struct("@PP4q4q8iPPPq")
+_LOGPROB_STRUCT = struct.Struct("@Pq4iPqPPPPP")
+
+
+def _packed_view(t) -> _lib.View4:
+    return _lib.View4.from_buffer_copy(_VIEW_STRUCT.pack(t.data_ptr(), *t.stride()))
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 _SAME_DEVICE = contextlib.nullcontext()
 
 
 def _on(index: int):
     """A context in which ``index`` is the current device, as the C ABI wants it."""
     return _SAME_DEVICE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _one_device(first, *others) -> int:
+    """The CUDA device that all the given tensors live on."""
+    index = first.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in others):
+        raise ValueError("the B200 attention engine needs CUDA device tensors, all on one device")
+    return index
 
 
 def default_scale(head_dim: int) -> float:
@@ -146,15 +174,36 @@ def _dropout_struct(dropout) -> _lib.Dropout:
     return _lib.Dropout(float(p), int(seed) & (2**64 - 1), int(offset) & (2**64 - 1))
 
 
-def _window_struct(window, sinks, is_causal, mask, dropout) -> _lib.Window:
-    """The checked window of a call, or raises."""
+def _window_struct(window, sinks, is_causal, mask, dropout) -> bytes:
+    """The checked window of a call as a packed ts_window, or raises."""
     if window < 1 or sinks < 0 or max(window, sinks) >= 2**31:
         raise ValueError("a window must be positive and the number of sinks must not be negative")
     if not is_causal:
         raise ValueError("a sliding window needs is_causal")
     if mask is not None or dropout is not None:
         raise ValueError("a sliding window takes neither an explicit mask nor dropout")
-    return _lib.Window(int(window), int(sinks))
+    return _WINDOW_STRUCT.pack(window, sinks)
+
+
+def _window_params(q, k, v, o, lse, scale, causal_offset, kv_lens) -> tuple:
+    """(packed ts_attn_params of a causal problem, what must outlive the call)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or o.dim() != 4:
+        raise ValueError("expected a [batch, heads, sequence, channels] view")
+    b, hq, tq, d = q.shape
+    hkv, tk = k.shape[1], k.shape[2]
+    if k.shape != (b, hkv, tk, d) or v.shape[:3] != (b, hkv, tk) or o.shape != (b, hq, tq, v.shape[3]):
+        raise ValueError("query, key, value and output shapes do not match")
+    if kv_lens is not None and kv_lens.dtype != torch.int32:
+        kv_lens = kv_lens.to(torch.int32)
+    if kv_lens is not None and (kv_lens.shape != (b,) or not kv_lens.is_contiguous() or not kv_lens.is_cuda):
+        raise ValueError("kv_lens must be one length a row, on the device")
+    if lse is not None and (lse.shape != (b, hq, tq) or lse.dtype != lse_dtype(q.dtype)):
+        raise ValueError("lse must be [B, Hq, T], fp32 (fp64 for fp64 inputs)")
+    return _ATTN_STRUCT.pack(
+        q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), o.data_ptr(), *o.stride(),
+        *((0, 0, 0, 0) if lse is None else (lse.data_ptr(), *lse.stride())), dtype_code(q.dtype), b, hq, hkv, tq, tk, d,
+        v.shape[3], default_scale(d) if scale is None else float(scale), 1, int(causal_offset),
+        0 if kv_lens is None else kv_lens.data_ptr(), _lib.MASK_NONE, 0, 0, 0, 0, 0), kv_lens
 
 
 def _no_window(sinks) -> None:
@@ -166,8 +215,8 @@ def window_path(q, k, v, *, window, sinks=0, causal_offset=0, scale=None, kv_len
     """Name of the kernel family that ``forward`` and ``backward`` select under a window."""
     w = _window_struct(window, sinks, True, None, None)
     o = torch.empty((q.shape[0], q.shape[1], q.shape[2], v.shape[3]), dtype=q.dtype, device=q.device)
-    p, keep = make_params(q, k, v, o, None, is_causal=True, scale=scale, causal_offset=causal_offset, kv_lens=kv_lens)
-    code = _lib.lib().ts_attn_window_path(ctypes.byref(p), ctypes.byref(w))
+    p, keep = _window_params(q, k, v, o, None, scale, causal_offset, kv_lens)
+    code = _lib.lib().ts_attn_window_path(p, w)
     if code < 0:
         _lib.check(code, "ts_attn_window_path")
     return _lib.PATH_NAMES[code]
@@ -189,18 +238,20 @@ def forward(q, k, v, *, is_causal=False, scale=None, causal_offset=0, kv_lens=No
         out = torch.empty((b, hq, tq, v.shape[3]), dtype=q.dtype, device=q.device)
     if need_lse and lse is None:
         lse = torch.empty((b, hq, tq), dtype=lse_dtype(q.dtype), device=q.device)
-    p, keep = make_params(q, k, v, out, lse if need_lse else None, is_causal=is_causal, scale=scale,
-                          causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
     if window is not None:
         w = _window_struct(window, sinks, is_causal, mask, dropout)
+        index = _one_device(q, k, v, out, lse if need_lse else None, kv_lens)
+        p, keep = _window_params(q, k, v, out, lse if need_lse else None, scale, causal_offset, kv_lens)
         handle = _lib.lib()
-        with _on(q.get_device()):
-            need = handle.ts_attn_fwd_window_workspace_size(ctypes.byref(p), ctypes.byref(w))
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            _lib.check(handle.ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), ws.data_ptr() if need else None, need,
-                                                 _stream_handle(q.device)), "ts_attn_fwd_window")
-        del keep
+        with _on(index):
+            need = handle.ts_attn_fwd_window_workspace_size(p, w)
+            ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+            status = handle.ts_attn_fwd_window(p, w, ws.data_ptr() if need else None, need, _raw_stream(index))
+        if status:
+            _lib.check(status, "ts_attn_fwd_window")
         return out, (lse if need_lse else None)
+    p, keep = make_params(q, k, v, out, lse if need_lse else None, is_causal=is_causal, scale=scale,
+                          causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
     _no_window(sinks)
     if dropout is not None:
         d = _dropout_struct(dropout)
@@ -296,18 +347,26 @@ def backward(q, k, v, out, lse, dout, *, is_causal=False, scale=None, causal_off
     dv = torch.empty_like(v) if dv is None else dv
     if dout.dtype != q.dtype:
         dout = dout.to(q.dtype)
+    if window is not None:
+        w = _window_struct(window, sinks, is_causal, mask, dropout)
+        index = _one_device(q, k, v, out, lse, dout, dq, dk, dv, kv_lens)
+        p, keep = _window_params(q, k, v, out, lse, scale, causal_offset, kv_lens)
+        if dout.shape != out.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != v.shape:
+            raise ValueError("gradients must have the shapes of what they belong to")
+        if dq.dtype != q.dtype or dk.dtype != q.dtype or dv.dtype != q.dtype:
+            raise TypeError("gradients must have the dtype of the inputs")
+        p += b"".join(_VIEW_STRUCT.pack(t.data_ptr(), *t.stride()) for t in (dout, dq, dk, dv))
+        handle = _lib.lib()
+        with _on(index):
+            need = handle.ts_attn_bwd_window_workspace_size(p, w)
+            ws = q.new_empty((max(need, 16),), dtype=torch.uint8)
+            status = handle.ts_attn_bwd_window(p, w, ws.data_ptr(), ws.numel(), _raw_stream(index))
+        if status:
+            _lib.check(status, "ts_attn_bwd_window")
+        return dq, dk, dv
     bp, keep = _bwd_params(q, k, v, out, lse, dout, dq, dk, dv, is_causal=is_causal, scale=scale,
                            causal_offset=causal_offset, kv_lens=kv_lens, mask=mask)
     handle = _lib.lib()
-    if window is not None:
-        w = _window_struct(window, sinks, is_causal, mask, dropout)
-        with _on(q.get_device()):
-            need = int(handle.ts_attn_bwd_window_workspace_size(ctypes.byref(bp), ctypes.byref(w)))
-            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-            _lib.check(handle.ts_attn_bwd_window(ctypes.byref(bp), ctypes.byref(w), ws.data_ptr(), ws.numel(),
-                                                 _stream_handle(q.device)), "ts_attn_bwd_window")
-        del keep
-        return dq, dk, dv
     _no_window(sinks)
     if dropout is not None:
         d = _dropout_struct(dropout)
@@ -480,22 +539,6 @@ def decode_int8(q, k8, v8, key_scales, value_scales, *, is_causal=True, scale=No
 
 
 # -- the paged 4-bit cache ----------------------------------------------------
-
-
-# The calls below cost a few microseconds on the device, so their structs are packed in one go (the layouts of
-# _lib.AttnParams, _lib.Kv4Cache and _lib.PagePool) instead of field by field.
-_ATTN_STRUCT = struct.Struct("@" + "P4q" * 4 + "P3q" + "8i" + "d" + "iq" + "P" + "iP4q")
-_VIEW_STRUCT = struct.Struct("@P4q")
-_KV4_STRUCT = struct.Struct("@PqPq6i")
-_POOL_STRUCT = struct.Struct("@Pqqqii")
-
-
-def _packed_view(t) -> _lib.View4:
-    return _lib.View4.from_buffer_copy(_VIEW_STRUCT.pack(t.data_ptr(), *t.stride()))
-
-
-def _raw_stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def int4_block_bytes(head_dim: int, page_size: int) -> int:
@@ -678,9 +721,6 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
 # -- drafted tokens over a cache -----------------------------------------------
 
 
-_TREE_STRUCT = struct.Struct("@Pqii")
-
-
 def _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse):
     """(packed ts_attn_params, packed ts_tree, device index) of an attention_tree call after its checks."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -800,41 +840,43 @@ def kv_keep(caches, base, path, counts):
     ``path`` (int32 [B, N]) holds the accepted nodes in ascending order, ``base`` and ``counts`` int32 vectors.  All
     layers share their shapes, strides and dtype (int8 storage too; the scales of an int8 cache are caches of one
     channel)."""
-    caches = [tuple(pair) for pair in caches]
-    if not caches or any(len(pair) != 2 for pair in caches):
+    keys, values = [], []
+    for key, value in caches:
+        keys.append(key)
+        values.append(value)
+    if not keys:
         raise ValueError("caches must be (keys, values) pairs")
-    key, value = caches[0]
+    key, value = keys[0], values[0]
     index = key.get_device()
     if index < 0 or key.dim() != 4 or value.dim() != 4 or value.shape[:3] != key.shape[:3]:
         raise ValueError("caches must be [batch, heads, capacity, channels] on a CUDA device")
     if 0 in key.shape or 0 in value.shape or key.dtype != value.dtype:
         raise ValueError("caches must not be empty, keys and values of one dtype")
-    for pair in caches:
-        for t, like in zip(pair, (key, value)):
-            if t.shape != like.shape or t.stride() != like.stride() or t.dtype != like.dtype or t.get_device() != index:
-                raise ValueError("the caches of all layers must have the same shape, strides, dtype and device")
-    for t in (key, value):
-        if t.shape[3] > 1 and t.stride(3) != 1:
-            raise ValueError("a cache's channels must be contiguous")
-    rows = key.shape[0]
+    for tensors in (keys, values):
+        if len({(t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors}) > 1:
+            raise ValueError("the caches of all layers must have the same shape, strides, dtype and device")
+    key_stride, value_stride = key.stride(), value.stride()
+    if value.get_device() != index or (key.shape[3] > 1 and key_stride[3] != 1) or (
+            value.shape[3] > 1 and value_stride[3] != 1):
+        raise ValueError("a cache's channels must be contiguous, keys and values on one device")
+    rows, heads, capacity, dim = key.shape
     if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != rows or path.get_device() != index or (
             path.stride(1) != 1 and path.shape[1] > 1):
         raise ValueError("path must be int32 [batch, nodes] with contiguous rows on the caches' device")
     base, counts = _int32_vector(base, "base", rows, index), _int32_vector(counts, "counts", rows, index)
-    if path.shape[1] == 0:
+    nodes = path.shape[1]
+    if nodes == 0:
         return
-    n = len(caches)
-    p = _lib.KvKeepParams()
-    p.keys = (ctypes.c_void_p * n)(*(pair[0].data_ptr() for pair in caches))
-    p.values = (ctypes.c_void_p * n)(*(pair[1].data_ptr() for pair in caches))
-    p.key_stride = (ctypes.c_int64 * 4)(*key.stride()[:3], 1)
-    p.value_stride = (ctypes.c_int64 * 4)(*value.stride()[:3], 1)
-    p.dtype = _storage_code(key.dtype)
-    p.layers, p.batch, p.heads, p.capacity, p.head_dim = n, *key.shape
-    p.value_dim, p.nodes = value.shape[3], path.shape[1]
-    p.base, p.path, p.counts, p.path_stride = base, path.data_ptr(), counts, path.stride(0)
+    n = len(keys)
+    pointers = (ctypes.c_void_p * (2 * n))(*[t.data_ptr() for t in keys], *[t.data_ptr() for t in values])
+    at = ctypes.addressof(pointers)
+    params = _KEEP_STRUCT.pack(at, at + n * ctypes.sizeof(ctypes.c_void_p), *key_stride[:3], 1, *value_stride[:3], 1,
+                               _storage_code(key.dtype), n, rows, heads, dim, value.shape[3], capacity, nodes, base,
+                               path.data_ptr(), counts, path.stride(0))
     with _on(index):
-        _lib.check(_lib.lib().ts_kv_keep(ctypes.byref(p), ctypes.c_void_p(_raw_stream(index))), "ts_kv_keep")
+        status = _lib.lib().ts_kv_keep(params, _raw_stream(index))
+    if status:
+        _lib.check(status, "ts_kv_keep")
 
 
 # -- log probabilities of tokens -------------------------------------------------
@@ -867,24 +909,16 @@ def _logit_rows(logits):
         raise ValueError("the B200 attention engine needs CUDA device tensors")
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError("logits must be [..., vocabulary]")
-    flat = logits.reshape(-1, logits.shape[-1])
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < 0):
         flat = flat.contiguous()
     return flat
 
 
-def _logprob_params(flat, targets, top, ignore_index):
-    p = _lib.TokenLogprobs()
-    p.logits, p.stride, p.dtype = flat.data_ptr(), flat.stride(0), dtype_code(flat.dtype)
-    p.rows, p.vocab, p.top = flat.shape[0], flat.shape[1], top
-    p.targets, p.ignore_index = targets.data_ptr(), ignore_index
-    return p
-
-
 def _target_rows(targets, logits):
     if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1] or targets.get_device() != logits.get_device():
         raise ValueError("targets must be int64 and have the shape of the logits without the vocabulary, on their device")
-    return targets.reshape(-1).contiguous()
+    return targets if targets.dim() == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
 
 
 def token_logprobs(logits, targets, *, top=0, ignore_index=-100) -> TokenLogprobs:
@@ -895,23 +929,26 @@ def token_logprobs(logits, targets, *, top=0, ignore_index=-100) -> TokenLogprob
     probabilities of -inf and entropy 0."""
     flat = _logit_rows(logits)
     goal = _target_rows(targets, logits)
-    shape, (rows, vocab) = targets.shape, flat.shape
+    rows, vocab = flat.shape
     if not 0 <= top <= min(vocab, _lib.TOP_TOKENS_MAX):
         raise ValueError(f"top must be between zero and {_lib.TOP_TOKENS_MAX}, and within the vocabulary")
-    sums = flat.new_empty((4 + top, rows), dtype=torch.float32)
-    logprob, entropy, norm = sums[0], sums[1], sums[2:4].view(rows, 2)
-    values, indices = sums[4:].view(rows, top), targets.new_empty((rows, top))
+    fp32 = dict(dtype=torch.float32, device=flat.device)
+    logprob, entropy, norm = torch.empty((rows,), **fp32), torch.empty((rows,), **fp32), torch.empty((rows, 2), **fp32)
+    values, indices = torch.empty((rows, top), **fp32), targets.new_empty((rows, top))
     if rows:
-        p = _logprob_params(flat, goal, top, int(ignore_index))
-        p.logprob, p.entropy, p.norm = logprob.data_ptr(), entropy.data_ptr(), norm.data_ptr()
-        p.top_logprobs, p.top_indices = (values.data_ptr(), indices.data_ptr()) if top else (None, None)
         index = flat.get_device()
+        params = _LOGPROB_STRUCT.pack(flat.data_ptr(), flat.stride(0), dtype_code(flat.dtype), rows, vocab, top,
+                                      goal.data_ptr(), ignore_index, logprob.data_ptr(), entropy.data_ptr(),
+                                      norm.data_ptr(), values.data_ptr(), indices.data_ptr())
         with _on(index):
-            status = _lib.lib().ts_token_logprobs_fwd(ctypes.byref(p), ctypes.c_void_p(_raw_stream(index)))
+            status = _lib.lib().ts_token_logprobs_fwd(params, _raw_stream(index))
         if status:
             _lib.check(status, "ts_token_logprobs_fwd")
-    return TokenLogprobs(logprob.view(shape), entropy.view(shape), values.view(*shape, top), indices.view(*shape, top),
-                         norm.view(*shape, 2))
+    shape = targets.shape
+    if len(shape) != 1:
+        logprob, entropy, norm = logprob.view(shape), entropy.view(shape), norm.view(*shape, 2)
+        values, indices = values.view(*shape, top), indices.view(*shape, top)
+    return TokenLogprobs(logprob, entropy, values, indices, norm)
 
 
 def token_logprobs_backward(logits, targets, result, grad_logprob=None, grad_entropy=None, grad_top=None, *,
@@ -930,18 +967,19 @@ def token_logprobs_backward(logits, targets, result, grad_logprob=None, grad_ent
         given.append(g)
     if result.logprob.shape != targets.shape or result.logprob.get_device() != index:
         raise ValueError("the result belongs to other logits")
-    grad = torch.empty(flat.shape, dtype=flat.dtype, device=flat.device)
-    if flat.shape[0]:
-        keep = [t.contiguous() for t in (result.entropy, result.norm, result.top_indices)]
-        p = _logprob_params(flat, goal, top, int(ignore_index))
-        p.entropy, p.norm, p.top_indices = keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr() if top else None
+    rows, vocab = flat.shape
+    grad = torch.empty((rows, vocab), dtype=flat.dtype, device=flat.device)
+    if rows:
+        entropy, norm, indices = (t.contiguous() for t in (result.entropy, result.norm, result.top_indices))
+        params = _LOGPROB_STRUCT.pack(flat.data_ptr(), flat.stride(0), dtype_code(flat.dtype), rows, vocab, top,
+                                      goal.data_ptr(), ignore_index, 0, entropy.data_ptr(), norm.data_ptr(), 0,
+                                      indices.data_ptr())
         with _on(index):
-            status = _lib.lib().ts_token_logprobs_bwd(
-                ctypes.byref(p), *(None if g is None else ctypes.c_void_p(g.data_ptr()) for g in given),
-                ctypes.c_void_p(grad.data_ptr()), grad.stride(0), ctypes.c_void_p(_raw_stream(index)))
+            status = _lib.lib().ts_token_logprobs_bwd(params, *(None if g is None else g.data_ptr() for g in given),
+                                                      grad.data_ptr(), grad.stride(0), _raw_stream(index))
         if status:
             _lib.check(status, "ts_token_logprobs_bwd")
-    return grad.view(logits.shape)
+    return grad if logits.dim() == 2 else grad.view(logits.shape)
 
 
 # -- pages ---------------------------------------------------------------------
