@@ -8,6 +8,11 @@
 // multiply-adds.  In fp32 the next operand is on its way (cp.async) while this one is multiplied.  The arithmetic is
 // exact in the accumulation type (fp32, or fp64 for fp64), exponentials in base 2.
 // Which columns a row sees is a 32-bit word a row and 32 columns (tree.cuh, window.cuh).
+//
+// Bound by the shared memory's reads of large problems, by the latency of a block's tiles of small ones.  Measured in
+// fp32, D 64 (the products that the mask needs, not the tiles'): 2 x 2000 queries, 8 heads, forward 428 us (19 TFLOP/s of
+// 74), with a window of 500 195 us; forward and backward 1402 and 749 us; 2 x 511 queries, 4 heads on 2, a window of
+// 128 and 3 sinks, forward and backward 107 us.
 #pragma once
 #include "dependent.cuh"
 #include "simt_kernels.cuh"
@@ -538,9 +543,12 @@ __global__ void __launch_bounds__(256)
 }
 
 // Key blocks [first, first + count) whose queries are divided into parts of `queries`, a multiple of a tile.
-struct RowsKeyBlocks {
+struct RowsKeySet {
   int first, count, parts, queries;
   void* part;
+};
+struct RowsKeyBlocks {
+  RowsKeySet with_sinks, others;  // the former have the longest parts and come first
 };
 
 template <typename A>
@@ -550,23 +558,22 @@ __device__ __forceinline__ A row_lse2(const ts_attn_params& p, int b, int h, int
   return v == neg_inf<A>() ? -neg_inf<A>() : v * (A)kLog2eD;  // a row that sees nothing: every p is 0
 }
 
+// dQ of a query block of a row and head.
 template <typename T, int RT, int DC>
-__global__ void __launch_bounds__(kRowsThreads) rows_window_dq_kernel(const __grid_constant__ RowsWindowBwd a) {
+__device__ __forceinline__ void rows_window_dq(const RowsWindowBwd& a, unsigned char* smem_raw, int index) {
   using A = typename Elem<T>::acc;
   using C = RowsCfg<A, RT, DC>;
   constexpr int kNC = C::kBwdNC, kCols = C::kBwdCols, kBufs = C::kBufs;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
   const ts_attn_params& p = a.bp.fwd;
   A* q = reinterpret_cast<A*>(smem_raw);
   A* g = q + C::kRows * C::kStride;
   A* tiles = g + C::kRows * C::kStride;  // K and V, kBufs times
   A* w = tiles + 2 * kBufs * kCols * C::kStride;
-  wait_for_previous();
-  let_next_start();
   const RowsWindow rule{p, a.win};
   const int ty = threadIdx.x / 8, tx = threadIdx.x % 8;
-  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.q_heads / p.kv_heads);
-  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * C::kRows;  // the longest rows first
+  const int heads = p.q_heads * p.batch, bh = index % heads;
+  const int h = bh % p.q_heads, b = bh / p.q_heads, hk = h / (p.q_heads / p.kv_heads);
+  const int i0 = (ceil_div(p.q_len, C::kRows) - 1 - index / heads) * C::kRows;  // the longest rows first
   const int kv_end = rule.kv_end(b);
   const int64_t offset = rule.offset(b);
   stage_tile<T, A>(q, C::kStride, p.q, b, h, i0, C::kRows, p.q_len, p.head_dim);
@@ -631,15 +638,14 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_dq_kernel(const __gr
   }
 }
 
-// Blocks (KV head and row, key block, part of the queries).  With one part dK and dV are written at once; with more,
+// dK and dV of (KV head and row, key block, part of the queries).  With one part they are written at once; with more,
 // each part leaves its sums in `part` and rows_dkv_sum_kernel adds them in order.
 template <typename T, int RT, int DC>
-__global__ void __launch_bounds__(kRowsThreads)
-    rows_window_dkv_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks) {
+__device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const RowsKeyBlocks& blocks, unsigned char* smem_raw,
+                                                int index) {
   using A = typename Elem<T>::acc;
   using C = RowsCfg<A, RT, DC>;
   constexpr int kNC = C::kBwdNC, kCols = C::kBwdCols, kBufs = C::kBufs;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ A s_lse2[kBufs][kCols], s_delta[kBufs][kCols];
   const ts_attn_params& p = a.bp.fwd;
   A* k = reinterpret_cast<A*>(smem_raw);
@@ -647,12 +653,14 @@ __global__ void __launch_bounds__(kRowsThreads)
   A* tiles = v + C::kRows * C::kStride;  // Q and dO, kBufs times
   A* wp = tiles + 2 * kBufs * kCols * C::kStride;
   A* ws = wp + C::kRows * (kCols + kRowsPad);
-  wait_for_previous();
-  let_next_start();
   const RowsWindow rule{p, a.win};
   const int ty = threadIdx.x / 8, tx = threadIdx.x % 8;
-  const int hk = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads;
-  const int block = blocks.first + blockIdx.y, j0 = block * C::kRows;
+  const int heads = p.kv_heads * p.batch, bh = index % heads, hk = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int first_others = blocks.with_sinks.count * blocks.with_sinks.parts;
+  int local = index / heads;
+  const RowsKeySet& set = local < first_others ? blocks.with_sinks : blocks.others;
+  if (local >= first_others) local -= first_others;
+  const int part = local / set.count, block = local % set.count, j0 = (set.first + block) * C::kRows;
   const int kv_end = rule.kv_end(b), rep = p.q_heads / p.kv_heads;
   const int64_t offset = rule.offset(b);
   stage_tile<T, A>(k, C::kStride, p.k, b, hk, j0, C::kRows, kv_end, p.head_dim);
@@ -665,9 +673,9 @@ __global__ void __launch_bounds__(kRowsThreads)
   int64_t first = i64min(p.q_len, i64max(0, j0 - offset) / kCols * kCols), stop = p.q_len;
   if (j0 >= a.win.sinks) stop = i64min(stop, (int64_t)min(j0 + C::kRows, kv_end) - 1 - offset + a.win.window);
   if (j0 >= kv_end) stop = 0;
-  if (blocks.parts > 1) {
-    const int64_t from = first + (int64_t)blockIdx.z * blocks.queries;
-    stop = i64min(stop, from + blocks.queries);
+  if (set.parts > 1) {
+    const int64_t from = first + (int64_t)part * set.queries;
+    stop = i64min(stop, from + set.queries);
     first = from;
   }
   const int tiles_a_head = first < stop ? (int)((stop - first + kCols - 1) / kCols) : 0, n = rep * tiles_a_head;
@@ -721,10 +729,10 @@ __global__ void __launch_bounds__(kRowsThreads)
   for (int r = 0; r < RT; ++r) {
     const int key = j0 + ty + 16 * r;
     if (key >= p.kv_len) continue;
-    if (blocks.parts > 1) {
+    if (set.parts > 1) {
       // [part][row and head][row of the blocks][channels of K, of V]
-      A* out = reinterpret_cast<A*>(blocks.part) +
-               (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * blocks.count * C::kRows + blockIdx.y * C::kRows + ty + 16 * r) *
+      A* out = reinterpret_cast<A*>(set.part) +
+               (((int64_t)part * heads + bh) * set.count * C::kRows + block * C::kRows + ty + 16 * r) *
                    (p.head_dim + p.value_dim);
 #pragma unroll
       for (int c = 0; c < DC; ++c)
@@ -747,7 +755,22 @@ __global__ void __launch_bounds__(kRowsThreads)
   }
 }
 
-// dK and dV of the blocks' keys from their parts, one thread a channel of a key.
+// Both in one launch, dK and dV first (a pair costs them four products, dQ three): small calls keep the SMs busy with
+// either, and larger ones have one tail.  In launches one behind the other (dQ, blocks with sinks, other blocks) the
+// gradients of the last example above took 105 us, now 70; of 2 x 2000 queries 1400, now 970.
+template <typename T, int RTQ, int RTK, int DC>
+__global__ void __launch_bounds__(kRowsThreads)
+    rows_window_bwd_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks, int dkv_blocks) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  wait_for_previous();
+  let_next_start();
+  if ((int)blockIdx.x < dkv_blocks)
+    rows_window_dkv<T, RTK, DC>(a, blocks, smem_raw, blockIdx.x);
+  else
+    rows_window_dq<T, RTQ, DC>(a, smem_raw, blockIdx.x - dkv_blocks);
+}
+
+// dK and dV of the divided blocks' keys from their parts, one thread a channel of a key.
 template <typename T>
 __global__ void __launch_bounds__(256)
     rows_dkv_sum_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks, int rows) {
@@ -755,16 +778,21 @@ __global__ void __launch_bounds__(256)
   const ts_attn_params& p = a.bp.fwd;
   wait_for_previous();
   let_next_start();
-  const int wide = p.head_dim + p.value_dim, keys = blocks.count * rows;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x, heads = (int64_t)p.kv_heads * p.batch;
-  if (x >= heads * keys * wide) return;
+  const int wide = p.head_dim + p.value_dim;
+  const int64_t heads = (int64_t)p.kv_heads * p.batch;
+  const int64_t first_others = blocks.with_sinks.parts > 1 ? heads * blocks.with_sinks.count * rows * wide : 0;
+  int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const RowsKeySet& set = x < first_others ? blocks.with_sinks : blocks.others;
+  if (x >= first_others) x -= first_others;
+  const int keys = set.count * rows;
+  if (set.parts <= 1 || x >= heads * keys * wide) return;
   const int ch = (int)(x % wide), local = (int)(x / wide % keys), bh = (int)(x / wide / keys);
-  const int key = blocks.first * rows + local;
+  const int key = set.first * rows + local;
   if (key >= p.kv_len) return;
-  const A* part = reinterpret_cast<const A*>(blocks.part) + x;
+  const A* part = reinterpret_cast<const A*>(set.part) + x;
   A sum = A(0);
 #pragma unroll 8
-  for (int z = 0; z < blocks.parts; ++z) sum += part[z * heads * keys * wide];
+  for (int z = 0; z < set.parts; ++z) sum += part[z * heads * keys * wide];
   const ts_view4& out = ch < p.head_dim ? a.bp.dk : a.bp.dv;
   *at4w<T>(out, bh / p.kv_heads, bh % p.kv_heads, key, ch < p.head_dim ? ch : ch - p.head_dim) = Elem<T>::from_acc(sum);
 }
@@ -789,57 +817,56 @@ cudaError_t rows_window_fwd_t(const RowsWindow& a, cudaStream_t st) {
 // The key blocks with sinks, which all the queries behind them see, and the others, each divided until the SMs have
 // work for several blocks (at most 64 parts: a part's sums are written and read once more).
 template <typename A>
-void rows_key_blocks(const ts_attn_params& p, const WindowArgs& win, int rows, int cols, RowsKeyBlocks (&sets)[2],
-                     size_t* bytes) {
+RowsKeyBlocks rows_key_blocks(const ts_attn_params& p, const WindowArgs& win, int rows, int cols, unsigned char* ws,
+                              size_t* bytes) {
   const int blocks = ceil_div(p.kv_len, rows), with_sinks = ceil_div(min(win.sinks, p.kv_len), rows);
   const int64_t heads = (int64_t)p.kv_heads * p.batch, want = 6 * (int64_t)device_sms();
-  size_t used = 0;
-  for (int i = 0; i < 2; ++i) {
-    RowsKeyBlocks& s = sets[i];
-    s.first = i == 0 ? 0 : with_sinks;
-    s.count = i == 0 ? with_sinks : blocks - with_sinks;
-    if (s.count == 0) continue;
-    const int64_t seen = i == 0 ? p.q_len : i64min(p.q_len, (int64_t)win.window + rows + cols);
+  *bytes = 0;
+  auto divide = [&](int first, int count, int64_t seen) {
+    RowsKeySet s{first, count, 0, 0, nullptr};
+    if (count == 0) return s;
     const int64_t tiles = (seen + cols - 1) / cols;
-    const int64_t parts = i64max(1, i64min(i64min(64, tiles), want / i64max(1, heads * s.count)));
+    const int64_t parts = i64max(1, i64min(i64min(64, tiles), want / i64max(1, heads * count)));
     s.queries = (int)((tiles + parts - 1) / parts) * cols;
     s.parts = (int)((seen + s.queries - 1) / s.queries);
-    s.part = reinterpret_cast<void*>(used);  // an offset until it is placed
-    if (s.parts > 1) used += sizeof(A) * (size_t)s.parts * heads * s.count * rows * (p.head_dim + p.value_dim);
-  }
-  *bytes = used;
+    s.part = ws ? ws + *bytes : nullptr;
+    if (s.parts > 1) *bytes += sizeof(A) * (size_t)s.parts * heads * count * rows * (p.head_dim + p.value_dim);
+    return s;
+  };
+  RowsKeyBlocks made;
+  made.with_sinks = divide(0, with_sinks, p.q_len);
+  made.others = divide(with_sinks, blocks - with_sinks, i64min(p.q_len, (int64_t)win.window + rows + cols));
+  return made;
 }
 
-template <typename T, int RT, int DC>
-cudaError_t rows_window_dq_t(const RowsWindowBwd& a, cudaStream_t st) {
-  using C = RowsCfg<typename Elem<T>::acc, RT, DC>;
-  const ts_attn_params& p = a.bp.fwd;
-  return launch_rows(rows_window_dq_kernel<T, RT, DC>, dim3(ceil_div(p.q_len, C::kRows), p.q_heads, p.batch), C::kBwdSmem,
-                     st, a);
-}
-
-// Into a workspace behind the deltas; ws null: its bytes alone.
-template <typename T, int RT, int DC>
-cudaError_t rows_window_dkv_t(const RowsWindowBwd& a, size_t* bytes, unsigned char* ws, cudaStream_t st) {
+// ws null: the workspace's bytes alone.  It holds the deltas, then the parts of dK and dV.
+template <typename T, int RTQ, int RTK, int DC>
+cudaError_t rows_window_bwd_t(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes, void* ws, cudaStream_t st) {
   using A = typename Elem<T>::acc;
-  using C = RowsCfg<A, RT, DC>;
-  const ts_attn_params& p = a.bp.fwd;
-  RowsKeyBlocks sets[2];
-  rows_key_blocks<A>(p, a.win, C::kRows, C::kBwdCols, sets, bytes);
+  using CQ = RowsCfg<A, RTQ, DC>;
+  using CK = RowsCfg<A, RTK, DC>;
+  const ts_attn_params& p = bp.fwd;
+  const int64_t heads = (int64_t)p.kv_heads * p.batch, q_rows = (int64_t)p.batch * p.q_heads * p.q_len;
+  const size_t delta = (sizeof(A) * (size_t)q_rows + 255) / 256 * 256;
+  const RowsKeyBlocks blocks =
+      rows_key_blocks<A>(p, win, CK::kRows, CK::kBwdCols, ws ? reinterpret_cast<unsigned char*>(ws) + delta : nullptr, bytes);
+  *bytes += delta;
   if (!ws) return cudaSuccess;
-  const int64_t heads = (int64_t)p.kv_heads * p.batch;
-  for (RowsKeyBlocks& s : sets) {
-    if (s.count == 0) continue;
-    s.part = ws + reinterpret_cast<size_t>(s.part);
-    cudaError_t e = launch_rows(rows_window_dkv_kernel<T, RT, DC>, dim3((unsigned)heads, s.count, s.parts), C::kBwdSmem,
-                                st, a, s);
-    if (e == cudaSuccess && s.parts > 1)
-      e = launch_dependent(rows_dkv_sum_kernel<T>,
-                           dim3((unsigned)((heads * s.count * C::kRows * (p.head_dim + p.value_dim) + 255) / 256)),
-                           dim3(256), 0, st, a, s, C::kRows);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  const RowsWindowBwd a{bp, win, ws};
+  cudaError_t e = launch_dependent(rows_delta_kernel<T>, dim3((unsigned)((q_rows * 32 + 255) / 256)), dim3(256), 0, st, bp,
+                                   reinterpret_cast<A*>(ws));
+  if (e != cudaSuccess) return e;
+  const RowsKeySet &s = blocks.with_sinks, &o = blocks.others;
+  const int64_t dkv = heads * ((int64_t)s.count * s.parts + (int64_t)o.count * o.parts);
+  const int64_t dq = (int64_t)p.batch * p.q_heads * ceil_div(p.q_len, CQ::kRows);
+  if (dkv + dq > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  e = launch_rows(rows_window_bwd_kernel<T, RTQ, RTK, DC>, dim3((unsigned)(dkv + dq)), std::max(CQ::kBwdSmem, CK::kBwdSmem),
+                  st, a, blocks, (int)dkv);
+  const int64_t divided = (s.parts > 1 ? s.count : 0) + (o.parts > 1 ? o.count : 0);
+  if (e != cudaSuccess || divided == 0) return e;
+  return launch_dependent(rows_dkv_sum_kernel<T>,
+                          dim3((unsigned)((heads * divided * CK::kRows * (p.head_dim + p.value_dim) + 255) / 256)),
+                          dim3(256), 0, st, a, blocks, (int)CK::kRows);
 }
 
 template <typename T, int RT, int DC>
@@ -863,33 +890,20 @@ cudaError_t rows_window_fwd_d(const RowsWindow& a, cudaStream_t st) {
   return rows_window_fwd_t<T, 1, DC>(a, st);
 }
 
-// ws null: the workspace's bytes alone.
+// Key blocks are divided along the queries, so they may be wide whatever their number.
 template <typename T, int DC>
 cudaError_t rows_window_bwd_d(const ts_attn_bwd_params& bp, const WindowArgs& win, size_t* bytes, void* ws, cudaStream_t st) {
   using A = typename Elem<T>::acc;
   const ts_attn_params& p = bp.fwd;
   constexpr int kMost = sizeof(A) == 8 ? 1 : DC == 2 ? 4 : DC == 4 ? 2 : 1;  // row tiles that the registers hold
-  const size_t delta = (sizeof(A) * (size_t)p.batch * p.q_heads * p.q_len + 255) / 256 * 256;
-  const RowsWindowBwd a{bp, win, ws};
-  unsigned char* parts = ws ? reinterpret_cast<unsigned char*>(ws) + delta : nullptr;
-  if (ws) {
-    const int64_t rows = (int64_t)p.batch * p.q_heads * p.q_len;
-    cudaError_t e = launch_dependent(rows_delta_kernel<T>, dim3((unsigned)((rows * 32 + 255) / 256)), dim3(256), 0, st, bp,
-                                     reinterpret_cast<A*>(ws));
-    if (e != cudaSuccess) return e;
+  if constexpr (kMost > 1) {
+    if (p.kv_len <= 16) return rows_window_bwd_t<T, 1, 1, DC>(bp, win, bytes, ws, st);
     const int rt = rows_rt(p.q_len, (int64_t)p.q_heads * p.batch, kMost);
-    if (rt == 1) e = rows_window_dq_t<T, 1, DC>(a, st);
-    if constexpr (kMost >= 2)
-      if (rt == 2) e = rows_window_dq_t<T, 2, DC>(a, st);
-    if constexpr (kMost >= 4)
-      if (rt == 4) e = rows_window_dq_t<T, 4, DC>(a, st);
-    if (e != cudaSuccess) return e;
+    if constexpr (kMost == 4)
+      if (rt == 4) return rows_window_bwd_t<T, 4, kMost, DC>(bp, win, bytes, ws, st);
+    if (rt == 2) return rows_window_bwd_t<T, 2, kMost, DC>(bp, win, bytes, ws, st);
   }
-  // Key blocks are divided along the queries, so they may be wide whatever their number.
-  const cudaError_t e = p.kv_len > 16 ? rows_window_dkv_t<T, kMost, DC>(a, bytes, parts, st)
-                                      : rows_window_dkv_t<T, 1, DC>(a, bytes, parts, st);
-  *bytes += delta;
-  return e;
+  return rows_window_bwd_t<T, 1, kMost, DC>(bp, win, bytes, ws, st);
 }
 
 template <typename T, int DC>

@@ -523,8 +523,9 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) token_logprobs_bwd_kerne
   let_next_start();
   const int64_t group = kGroup == kBlock ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kBlock / kGroup) + threadIdx.x / kGroup;
   const int id = threadIdx.x % kGroup;
-  const int64_t row = group / a.parts;
-  if (row >= p.rows) return;
+  if (group >= p.rows * a.parts) return;
+  // From the last row on: those that a forward has just read are still in L2.
+  const int64_t row = p.rows - 1 - group / a.parts;
   const int part = (int)(group % a.parts);
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
   T* out = reinterpret_cast<T*>(a.grad) + row * a.grad_stride;
