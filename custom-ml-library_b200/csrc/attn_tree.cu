@@ -97,15 +97,20 @@ __global__ void __launch_bounds__(384, 1)
     ptx::tmem_alloc(&bars->tmem_base, 512);
     ptx::tmem_relinquish();
   }
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tm_k);
+    ptx::prefetch_tensormap(&tm_v);
+  }
   wait_for_previous();
   let_next_start();
   const TreeLine line(args, kBN, kUnitPlaces);
   if (warp == 0) {
+    const bool faulted = fault_set(args.fault);  // under way during the planning
     LinePlace ends[2];
     line_share(line, lane, blockIdx.x, args.ctas, ends);
     if (lane == 0) {
       bars->from = ends[0];
-      bars->tiles = fault_set(args.fault) ? 0 : ends[1].tiles - ends[0].tiles;
+      bars->tiles = faulted ? 0 : ends[1].tiles - ends[0].tiles;
     }
   }
   ptx::tc_fence_before();
@@ -122,8 +127,6 @@ __global__ void __launch_bounds__(384, 1)
     if (warp == 0) {
       // ---------------------------- producer ------------------------------
       if (lane == 0 && n_tiles > 0) {
-        ptx::prefetch_tensormap(&tm_k);
-        ptx::prefetch_tensormap(&tm_v);
         // K is a tile ahead of V: they walk along the share by themselves.
         struct Stream {
           LineWalk walk;
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(kMergeThreads)
   const ts_attn_params& p = a.p;
   __shared__ int64_t s_first, s_total;
   __shared__ int s_tiles;
-  __shared__ float2 s_row[kBM];  // the reference and 1 / sum of every row
+  __shared__ float2 s_row[kMergeThreads];  // reference and sum of every row, of several slices of its results first
   __shared__ float4 s_sum[kMergeThreads];
   const TreeLine line(a, tile_keys, start_places, true);
   const int unit = blockIdx.x % line.units, b = blockIdx.x / line.units;
@@ -582,42 +585,68 @@ __global__ void __launch_bounds__(kMergeThreads)
     }
     return;
   }
-  // A warp a row, lanes over its results.
-  for (int row = warp; row < rows; row += kMergeThreads / 32) {
+  // Threads over an item's results; the first of them are under way while the rows' numbers are found.
+  const int split = max(1, min(parts, kMergeThreads / mine)), lanes = kMergeThreads / split;
+  const int slot = threadIdx.x % lanes, s = threadIdx.x / lanes;
+  float4 o[kMergeParts];
+  auto load = [&](int x, int i0) {
+    const int row = (first + x) % rows, quad = (first + x) / rows;
+#pragma unroll
+    for (int u = 0; u < kMergeParts; ++u)
+      if (i0 + u * split < parts)
+        o[u] = from[(int64_t)(i0 + u * split) * a.part_rows * quads + (int64_t)quad * a.part_rows + row];
+  };
+  if (slot < mine && s < split) load(slot, s);
+  const int slices = kMergeThreads / rows, row_slice = threadIdx.x / rows;
+  if (row_slice < slices) {
+    const int row = threadIdx.x % rows;
     float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml[(int64_t)i * a.part_rows + row].x);
+    for (int i0 = row_slice; i0 < parts; i0 += slices * kFewParts) {
+      float2 v[kFewParts];
+      float top = m;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    for (int i = lane; i < parts; i += 32) {
-      const float2 v = ml[(int64_t)i * a.part_rows + row];
-      if (v.x != -INFINITY) l = fmaf(ptx::ex2(v.x - m), v.y, l);
+      for (int u = 0; u < kFewParts; ++u) {
+        const int i = i0 + u * slices;
+        v[u] = i < parts ? ml[(int64_t)i * a.part_rows + row] : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < kFewParts; ++u) top = fmaxf(top, v[u].x);
+      l = m == -INFINITY ? 0.f : l * ptx::ex2(m - top);
+#pragma unroll
+      for (int u = 0; u < kFewParts; ++u)
+        if (v[u].x != -INFINITY) l = fmaf(ptx::ex2(v[u].x - top), v[u].y, l);
+      m = top;
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    if (lane != 0) continue;
-    s_row[row] = make_float2(m, l > 0.f ? 1.f / l : l);
-    if (blockIdx.y == 0 && p.lse) write_lse(row, m, l);
+    s_row[threadIdx.x] = make_float2(m, l);
   }
   __syncthreads();
-  const int split = max(1, min(parts, kMergeThreads / mine)), lanes = kMergeThreads / split;
+  for (int n = slices; n > 1;) {  // the slices' numbers, upper halves into lower ones
+    const int half = (n + 1) / 2;
+    if (row_slice < n - half) {
+      const float2 x = s_row[threadIdx.x], y = s_row[threadIdx.x + half * rows];
+      const float m = fmaxf(x.x, y.x);
+      float l = x.x == -INFINITY ? 0.f : ptx::ex2(x.x - m) * x.y;
+      if (y.x != -INFINITY) l = fmaf(ptx::ex2(y.x - m), y.y, l);
+      s_row[threadIdx.x] = make_float2(m, l);
+    }
+    __syncthreads();
+    n = half;
+  }
+  if (blockIdx.y == 0 && p.lse && row_slice == 0) write_lse(threadIdx.x, s_row[threadIdx.x].x, s_row[threadIdx.x].y);
   for (int x0 = 0; x0 < mine; x0 += lanes) {
-    const int x = x0 + threadIdx.x % lanes, s = threadIdx.x / lanes;
+    const int x = x0 + slot;
     const bool live = x < mine && s < split;
-    const int row = live ? (first + x) % rows : 0, quad = live ? (first + x) / rows : 0;
+    const float2 total = s_row[live ? (first + x) % rows : 0];
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float m = s_row[row].x;
-    if (live && m != -INFINITY) {
+    if (live && total.x != -INFINITY) {
+      const int row = (first + x) % rows;
       for (int i0 = s; i0 < parts; i0 += split * kMergeParts) {
-        float4 o[kMergeParts];
+        if (x0 > 0 || i0 > s) load(x, i0);
         float w[kMergeParts];
 #pragma unroll
         for (int u = 0; u < kMergeParts; ++u) {
           const int i = i0 + u * split;
-          w[u] = 0.f;
-          if (i < parts) {
-            w[u] = ptx::ex2(ml[(int64_t)i * a.part_rows + row].x - m);  // 0 where the part has seen nothing
-            o[u] = from[(int64_t)i * a.part_rows * quads + (int64_t)quad * a.part_rows + row];
-          }
+          w[u] = i < parts ? ptx::ex2(ml[(int64_t)i * a.part_rows + row].x - total.x) : 0.f;  // 0 where it has seen nothing
         }
 #pragma unroll
         for (int u = 0; u < kMergeParts; ++u) add(sum, w[u], o[u]);
@@ -628,15 +657,15 @@ __global__ void __launch_bounds__(kMergeThreads)
       __syncthreads();
       if (live && s == 0)
         for (int i = 1; i < split; ++i) {
-          const float4 o = s_sum[i * lanes + threadIdx.x];
-          sum.x += o.x;
-          sum.y += o.y;
-          sum.z += o.z;
-          sum.w += o.w;
+          const float4 y = s_sum[i * lanes + threadIdx.x];
+          sum.x += y.x;
+          sum.y += y.y;
+          sum.z += y.z;
+          sum.w += y.w;
         }
       __syncthreads();
     }
-    if (live && s == 0) write(row, quad, sum, s_row[row].y);
+    if (live && s == 0) write((first + x) % rows, (first + x) / rows, sum, total.y > 0.f ? 1.f / total.y : total.y);
   }
 }
 
@@ -698,9 +727,12 @@ size_t tc_tree_workspace(const ts_attn_params& p) {
 }
 
 cudaError_t tree_merge(const TreeArgs& a, int tile_keys, int start_places, cudaStream_t st) {
-  // Shares of 64 items at least, and blocks for the SMs two or three times over where there are that many.
+  // Blocks for the SMs two or three times over, with shares of 64 items at least, or of so few that a thread reads all
+  // that it takes of an item at once.
   const int units = a.p.batch * a.p.kv_heads * a.row_tiles, items = a.part_rows * part_quads(a.p);
-  const int share = max(64, ceil_div(items, max(1, 600 / units)));
+  const int parts = ceil_div(a.ctas, units) + 1;  // of a unit of ordinary length
+  const int least = max(8, min(64, kMergeThreads * kMergeParts / parts));
+  const int share = max(least, ceil_div(items, max(1, 600 / units)));
   const dim3 grid((unsigned)units, (unsigned)ceil_div(items, share)), block(kMergeThreads);
   switch (a.p.dtype) {
     case TS_F32: return launch_dependent(tree_merge_kernel<float>, grid, block, 0, st, a, tile_keys, start_places, share);
