@@ -11,12 +11,15 @@
 // (value, lower index).  Rows built so that too many elements reach the bound (constant ones, say) find the k-th value
 // by bisection and take its first holders in order.
 // Rows of up to 4096 logits are a warp's each, longer ones a block's, or a cluster's where there are few of them.
-// Bounded by memory: one read of the logits.  Backward: one read and one write.
+// Bounded by memory: one read of the logits.  Backward: one read and one write, from the last row on, which the forward
+// has read last (L2).  bf16, 4096 rows of 128256: 177 us, 5.9 TB/s of 6.5 that a copy reaches; with 5 alternatives 222;
+// 4095 rows of 50257: 89 us, 4.6 TB/s (6 short waves of blocks), its gradient 130 us, 6.3 TB/s.
 #include <cooperative_groups.h>
 
 #include "dependent.cuh"
 #include "tc_util.cuh"
 #include "token_logprobs.cuh"
+#include "tree.cuh"
 
 namespace tsa {
 
@@ -28,7 +31,11 @@ constexpr int kCandidates = 256;
 constexpr int kPeakBytes = 64 * 1024;
 constexpr int kWarpRow = 4096;  // longest row of a warp
 constexpr int kMaxCluster = 8;
-constexpr int kBlocksPerSm = 5;  // of the row kernels (launch bounds)
+constexpr int kBlocksPerSm = 5;  // of the row kernel (launch bounds)
+// Warps' rows and the gradient, whose parts are independent, run in smaller blocks (4095 rows of 50257 with gradients:
+// 219 against 226 us; 4756 of 182: 10.8 against 11.8); a row's block or cluster in larger ones (one row of 260000 with
+// 20 alternatives: 14.7 against 18.8 us, 300 of 128256 30.6 against 40.6).
+constexpr int kSmallBlock = 128, kSmallWarps = kSmallBlock / 32, kSmallPerSm = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1.0e6f;  // stands for differences below it: e^kFar is 0, and 0 * kFar is too
 constexpr float kLowest = -3.402823466e38f;
@@ -157,6 +164,10 @@ __device__ __forceinline__ void scan(const Span<T>& span, int id, int threads, i
     a.t += t0 + t1;
     s2 = t2 = 0;
   };
+  // At most 2 (N - 1) elements outside vectors, one a thread at most.  Under way during the pass, but for alternatives,
+  // whose kernel the register costs more (4096 rows of 128256: 226 against 222 us without, 180 against 177 with none).
+  const bool edge = id < span.edges();
+  float edge_x = !kTop && edge ? span.at(span.edge_index(id)) : -INFINITY;
   for (int v0 = id, step = 0; v0 < span.vectors; v0 += threads * kUnroll, ++step) {
     uint4 raw[kUnroll];
     float top = -INFINITY;
@@ -192,11 +203,11 @@ __device__ __forceinline__ void scan(const Span<T>& span, int id, int threads, i
     }
   }
   fold();
-  for (int i = id; i < span.edges(); i += threads) {
-    const float x = span.at(span.edge_index(i));
-    if (x > a.m) rebase(a, x);
-    add(a, x);
-    if (kTop) peak = max_nan(peak, x);
+  if (edge) {
+    if (kTop) edge_x = span.at(span.edge_index(id));
+    if (edge_x > a.m) rebase(a, edge_x);
+    add(a, edge_x);
+    if (kTop) peak = max_nan(peak, edge_x);
   }
 }
 
@@ -369,16 +380,16 @@ template <typename T, int kGroup> struct Select {
 
 // Rows of up to kWarpRow logits: a warp each.
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kBlock) token_logprobs_warp_kernel(const __grid_constant__ ts_token_logprobs p) {
+__global__ void __launch_bounds__(kSmallBlock) token_logprobs_warp_kernel(const __grid_constant__ ts_token_logprobs p) {
   constexpr int kPeaks = kTop ? (kWarpRow / Vec<T>::kN + 32 * kUnroll - 1) / (32 * kUnroll) * 32 : 1;
-  __shared__ float s_peaks[kWarps][kPeaks];
-  __shared__ uint64_t s_found[kWarps][kTop ? kCandidates : 1];
-  __shared__ int s_list[kWarps][kTop ? kCandidates : 1];
-  __shared__ uint32_t s_count[kWarps], s_listed[kWarps];
+  __shared__ float s_peaks[kSmallWarps][kPeaks];
+  __shared__ uint64_t s_found[kSmallWarps][kTop ? kCandidates : 1];
+  __shared__ int s_list[kSmallWarps][kTop ? kCandidates : 1];
+  __shared__ uint32_t s_count[kSmallWarps], s_listed[kSmallWarps];
   wait_for_previous();
   let_next_start();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t row = (int64_t)blockIdx.x * kSmallWarps + warp;
   if (row >= p.rows) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.stride;
   const Span<T> span(x, 0, p.vocab);
@@ -473,7 +484,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
       }
       if constexpr (kTop) {
         n = parts * p.top;  // at most kMaxCluster * kMaxTopTokens
-        if (id < (int)n) s_found[id] = cluster.map_shared_rank(s_best, id / p.top)[id % p.top];
+        for (int i = id; i < (int)n; i += kBlock) s_found[i] = cluster.map_shared_rank(s_best, i / p.top)[i % p.top];
       }
     }
     cluster.sync();  // the other blocks' memory has been read
@@ -516,12 +527,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 }  // namespace
 
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(kBlock, kBlocksPerSm) token_logprobs_bwd_kernel(const __grid_constant__ BwdArgs a) {
+__global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_kernel(const __grid_constant__ BwdArgs a) {
   constexpr int N = Vec<T>::kN;
   const ts_token_logprobs& p = a.p;
   wait_for_previous();
   let_next_start();
-  const int64_t group = kGroup == kBlock ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kBlock / kGroup) + threadIdx.x / kGroup;
+  const int64_t group = (int64_t)blockIdx.x * (kSmallBlock / kGroup) + threadIdx.x / kGroup;
   const int id = threadIdx.x % kGroup;
   if (group >= p.rows * a.parts) return;
   // From the last row on: those that a forward has just read are still in L2.
@@ -616,11 +627,11 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) token_logprobs_bwd_kerne
 template <typename T, bool kTop>
 static cudaError_t forward_t(const ts_token_logprobs& p, cudaStream_t st) {
   if (p.vocab <= kWarpRow)
-    return launch_dependent(token_logprobs_warp_kernel<T, kTop>, dim3((unsigned)ceil_div(p.rows, kWarps)), dim3(kBlock), 0,
-                            st, p);
+    return launch_dependent(token_logprobs_warp_kernel<T, kTop>, dim3((unsigned)ceil_div(p.rows, kSmallWarps)),
+                            dim3(kSmallBlock), 0, st, p);
   // A cluster a row while there are fewer rows than blocks that the SMs hold, in parts of 4096 logits at least.
   int parts = 1;
-  while (parts < kMaxCluster && (int64_t)p.rows * parts <= 2 * 148 && p.vocab / (2 * parts) >= 4096) parts *= 2;
+  while (parts < kMaxCluster && (int64_t)p.rows * parts <= 2 * device_sms() && p.vocab / (2 * parts) >= 4096) parts *= 2;
   auto kern = token_logprobs_kernel<T, kTop>;
   int shift = 0;
   size_t peaks = 0;
@@ -663,14 +674,14 @@ static cudaError_t backward_t(BwdArgs a, cudaStream_t st) {
   if (vectors <= 32 * kUnroll * 2) {  // a warp a row
     a.parts = 1;
     a.part = vectors;
-    return launch_dependent(token_logprobs_bwd_kernel<T, 32>, dim3((unsigned)ceil_div(a.p.rows, kBlock / 32)), dim3(kBlock),
-                            0, st, a);
+    return launch_dependent(token_logprobs_bwd_kernel<T, 32>, dim3((unsigned)ceil_div(a.p.rows, kSmallWarps)),
+                            dim3(kSmallBlock), 0, st, a);
   }
-  a.part = kBlock * kUnroll * 2;
+  a.part = kSmallBlock * kUnroll * 2;
   a.parts = ceil_div(vectors, a.part);
   a.part = ceil_div(vectors, a.parts);
-  return launch_dependent(token_logprobs_bwd_kernel<T, kBlock>, dim3((unsigned)(a.p.rows * (int64_t)a.parts)), dim3(kBlock), 0,
-                          st, a);
+  return launch_dependent(token_logprobs_bwd_kernel<T, kSmallBlock>, dim3((unsigned)(a.p.rows * (int64_t)a.parts)),
+                          dim3(kSmallBlock), 0, st, a);
 }
 
 cudaError_t token_logprobs_bwd(const ts_token_logprobs& p, const float* grad_logprob, const float* grad_entropy,
