@@ -612,9 +612,10 @@ int check_window(const ts_attn_params* p, const ts_window* w) {
   const int st = check_params(p);
   if (st != TS_OK) return st;
   if (!w || w->window < 1 || w->sinks < 0 || !p->is_causal) return TS_ERR_INVALID_ARGUMENT;
+  if (p->causal_offset > (int64_t)1 << 62) return TS_ERR_INVALID_ARGUMENT;  // positions behind it stay 64-bit numbers
   if (p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
   if (p->q_heads > kGridMax || p->batch > kGridMax || (int64_t)p->kv_heads * p->batch > 0x7fffffff ||
-      p->kv_len > 16 * kGridMax)
+      p->kv_len > 1 << 30)
     return TS_ERR_UNSUPPORTED;
   return TS_OK;
 }
@@ -630,7 +631,7 @@ int check_window_bwd(const ts_attn_bwd_params* bp, const ts_window* w) {
   const int st = check_window(&bp->fwd, w);
   if (st != TS_OK) return st;
   if (!bp->fwd.lse || !bp->dout.data || !bp->dq.data || !bp->dk.data || !bp->dv.data) return TS_ERR_INVALID_ARGUMENT;
-  if ((int64_t)bp->fwd.batch * bp->fwd.q_heads > 0x7fffffff ||
+  if (bp->fwd.kv_len > 64 * kGridMax || (int64_t)bp->fwd.batch * bp->fwd.q_heads > 0x7fffffff ||
       (int64_t)bp->fwd.batch * bp->fwd.q_heads * bp->fwd.q_len > (int64_t)1 << 33)
     return TS_ERR_UNSUPPORTED;
   return TS_OK;

@@ -566,8 +566,8 @@ size_t tc_bwd_workspace(const ts_attn_bwd_params& bp) {
 }
 
 // How the key tiles with sinks are divided.  A CTA's time is its number of (query tile, head) pairs; undivided, a tile
-// with sinks takes those of all queries.  Parts of half an SM's even share of all pairs (16 at least) end no later
-// than the rest (16000 queries, 4 heads on one KV head of 128, a window of 500, 4 sinks: 131 us, 1668 undivided).
+// with sinks takes those of all queries.  Parts of three quarters of an SM's even share of all pairs (16 at least) end
+// no later than the rest (16000 queries, 4 heads on one KV head of 128, a window of 500, 4 sinks: 131 us, 1668 undivided).
 struct SinkParts {
   int tiles, parts;
 };
@@ -578,7 +578,7 @@ static SinkParts sink_parts(const ts_attn_params& p, const WindowArgs& win) {
   const int64_t all = rep * ceil_div(p.q_len, kBM);
   const int64_t near = rep * i64min(ceil_div(p.q_len, kBM), ((int64_t)win.window + kBN) / kBM + 1);
   const int64_t share = heads * (with_sinks * all + (tiles - with_sinks) * near) / device_sms();
-  const int64_t parts = (all + i64max(16, share / 2) - 1) / i64max(16, share / 2);
+  const int64_t most = i64max(16, share * 3 / 4), parts = (all + most - 1) / most;
   return SinkParts{(int)with_sinks, (int)i64max(1, i64min(64, parts))};
 }
 

@@ -193,6 +193,8 @@ def _window_params(q, k, v, o, lse, scale, causal_offset, kv_lens) -> tuple:
     hkv, tk = k.shape[1], k.shape[2]
     if k.shape != (b, hkv, tk, d) or v.shape[:3] != (b, hkv, tk) or o.shape != (b, hq, tq, v.shape[3]):
         raise ValueError("query, key, value and output shapes do not match")
+    if o.dtype != q.dtype:
+        raise TypeError("the output must have the dtype of the inputs")
     if kv_lens is not None and kv_lens.dtype != torch.int32:
         kv_lens = kv_lens.to(torch.int32)
     if kv_lens is not None and (kv_lens.shape != (b,) or not kv_lens.is_contiguous() or not kv_lens.is_cuda):
@@ -839,13 +841,15 @@ def kv_keep(caches, base, path, counts):
 
     ``path`` (int32 [B, N]) holds the accepted nodes in ascending order, ``base`` and ``counts`` int32 vectors.  All
     layers share their shapes, strides and dtype (int8 storage too; the scales of an int8 cache are caches of one
-    channel)."""
+    channel) and lie in memory of their own."""
     keys, values = [], []
     for key, value in caches:
         keys.append(key)
         values.append(value)
     if not keys:
         raise ValueError("caches must be (keys, values) pairs")
+    if len({t.data_ptr() for t in keys + values}) < 2 * len(keys):
+        raise ValueError("a cache may be given only once")
     key, value = keys[0], values[0]
     index = key.get_device()
     if index < 0 or key.dim() != 4 or value.dim() != 4 or value.shape[:3] != key.shape[:3]:

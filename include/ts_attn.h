@@ -457,8 +457,8 @@ TS_ATTN_API int ts_rope_at(ts_view4 x, ts_view4 y, int32_t dtype, int32_t batch,
                            int32_t inverse, void* stream);
 
 /* Closes caches behind the accepted path: slot base[b] + path[b, k] moves to slot base[b] + k for k < counts[b], in
- * the key and value caches of every layer.  path ascends (nodes of one root-to-leaf path do); entries that would read
- * past the capacity are skipped. */
+ * the key and value caches of every layer, each in memory of its own.  path ascends (nodes of one root-to-leaf path do);
+ * entries that would read past the capacity are skipped. */
 typedef struct ts_kv_keep_params {
   void* const* keys; /* host arrays of `layers` device pointers, all with the strides below */
   void* const* values;

@@ -225,6 +225,23 @@ def test_gradients_against_differences():
     assert abs(float((d.double() * step).sum()) - slope) < 1e-4
 
 
+@pytest.mark.parametrize("vocab", [999, 20011])
+def test_far_rows(vocab):
+    """Rows more than 2^31 elements apart."""
+    far = 2**31 + 5
+    store = torch.empty(far + vocab, dtype=torch.float16, device="cuda")
+    x = store.as_strided((2, vocab), (far, 1))
+    x.copy_(torch.randn(2, vocab, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda"))
+    t, g = torch.tensor([3, vocab - 1], device="cuda"), torch.ones(2, device="cuda")
+    near = x.contiguous()
+    a, b = engine.token_logprobs(x, t, top=5), engine.token_logprobs(near, t, top=5)
+    # the two layouts start at other offsets from a vector's boundary, and sum in another order
+    assert torch.equal(a.top_indices, b.top_indices) and torch.allclose(a.logprob, b.logprob, atol=1e-5)
+    da = engine.token_logprobs_backward(x, t, a, g, g)
+    db = engine.token_logprobs_backward(near, t, a, g, g)
+    assert torch.equal(da, db)
+
+
 def test_streams_and_graphs():
     x, t = make(50, 7001, "bf16")
     g = torch.ones(50, device="cuda")

@@ -247,6 +247,30 @@ def test_keep(dtype, dim, value_dim, layers):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_far_addresses(dtype):
+    """Heads and rows that lie more than 2^31 elements apart, read by the attention and closed up behind a path."""
+    far, nodes, dim, room = 2**31 + 64, 6, 64, 700
+    store = torch.empty(far + 4 * room * dim, dtype=DTYPES[dtype], device="cuda")
+    k = store.as_strided((1, 2, room, dim), (far, far, dim, 1))
+    v = store[2 * room * dim :].as_strided((1, 2, room, dim), (far, far, dim, 1))
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for x in (k, v):
+        x.copy_(torch.randn(1, 2, room, dim, generator=gen, device="cuda"))
+    q = torch.randn(1, 4, nodes, dim, generator=gen, device="cuda").to(k.dtype)
+    cuda = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    lens, parents = cuda([650]), cuda([[-1, 0, 0, 1, 3, 2]])
+    out, lse = engine.attention_tree(q, k, v, lens, parents, need_lse=True)
+    near, near_lse = engine.attention_tree(q, k.contiguous(), v.contiguous(), lens, parents, need_lse=True)
+    assert torch.equal(out, near) and torch.equal(lse, near_lse)
+    rows = [x.transpose(0, 1) for x in (k, v)]  # the heads as rows of a batch
+    want = [x.contiguous() for x in rows]
+    path, counts, base = cuda([[1, 3, 4], [0, 2, 5]]), cuda([3, 2]), cuda([644, 644])
+    keep_reference([want], [644, 644], path.tolist(), [3, 2])
+    engine.kv_keep([rows], base, path, counts)
+    assert all(torch.equal(a, b) for a, b in zip(rows, want))
+
+
 def test_keep_stays_inside():
     """Counts and entries that no tree gives move nothing outside the cache."""
     room = torch.arange(4 * 2 * 10 * 8, device="cuda", dtype=torch.float32).view(4, 2, 10, 8)
@@ -285,6 +309,11 @@ def test_refusals():
         engine.tree_positions(tree.long(), lens)
     with pytest.raises(ValueError):
         engine.tree_positions(tree, lens[:1])
+    v, layer = torch.zeros_like(k), (k.clone(), k.clone())
+    engine.kv_keep([(k, v), layer], lens, tree, lens)
+    for caches in ([(k, k)], [(k, v), (v, k)], [layer, layer]):  # two walks along one memory
+        with pytest.raises(ValueError, match="once"):
+            engine.kv_keep(caches, lens, tree, lens)
     for args in (([], lens, tree, lens), ([(k, k[:1])], lens, tree, lens), ([(k, k.half())], lens, tree, lens),
                  ([(k, k), (k[:, :, :8], k)], lens, tree, lens), ([(k, k)], lens.long(), tree, lens),
                  ([(k, k)], lens, tree[:1], lens), ([(k, k)], lens, tree, lens[:1]),

@@ -85,6 +85,30 @@ def test_cuda_cores(dtype, dim, tokens, window, sinks):
     run(dtype, 2, 4, 2, tokens, dim, window, sinks, path="simt")
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 32), ("f16", 256)])
+def test_many_keys(dtype, dim):
+    """A few queries behind more than a million keys: what the sinks and the last keys alone give, gradients of zero
+    everywhere else."""
+    tokens, window, sinks, keys = 5, 300, 3, 1_200_001
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    make = lambda h, t: torch.randn(1, h, t, dim, generator=gen, device="cuda").to(DTYPES[dtype])  # noqa: E731
+    q, k, v, g = make(2, tokens), make(1, keys), make(1, keys), make(2, tokens)
+    rule = dict(is_causal=True, window=window, sinks=sinks, causal_offset=keys - tokens)
+    out, lse = engine.forward(q, k, v, **rule)
+    dq, dk, dv = engine.backward(q, k, v, out, lse, g, **rule)
+    seen = torch.cat([torch.arange(sinks), torch.arange(keys - tokens - window + 1, keys)]).cuda()
+    ref = Attention(q, k[:, :, seen], v[:, :, seen],
+                    window_seen(1, tokens, len(seen), window, sinks, len(seen) - tokens),
+                    cubic=engine.window_path(q, k, v, window=window, sinks=sinks) == "tcgen05")
+    ref.check(out, lse)
+    want, bounds = ref.backward(g)
+    for x, y, bound, name in zip((dq, dk[:, :, seen], dv[:, :, seen]), want, bounds, ("dq", "dk", "dv")):
+        within(x, y, bound, name)
+    dk[:, :, seen] = 0
+    dv[:, :, seen] = 0
+    assert not dk.any() and not dv.any()
+
+
 def test_value_dimension_and_scale():
     run("f32", 1, 2, 2, 100, 48, 30, 2, value_dim=80, path="simt")
     run("bf16", 1, 2, 2, 100, 64, 30, 2, value_dim=32, path="simt")

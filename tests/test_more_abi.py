@@ -59,7 +59,8 @@ def test_window_refusals():
              (problem(q_heads=3, kv_heads=2), good, BAD), (problem(causal_offset=-1), good, BAD),
              (problem(scale=float("nan")), good, BAD), (problem(dtype=7), good, UNSUPPORTED),
              (problem(head_dim=257), good, UNSUPPORTED), (problem(mask_kind=1, mask=FAKE), good, UNSUPPORTED),
-             (problem(batch=70000), good, UNSUPPORTED)]
+             (problem(batch=70000), good, UNSUPPORTED), (problem(kv_len=(1 << 30) + 1), good, UNSUPPORTED),
+             (problem(causal_offset=(1 << 62) + 1), good, BAD)]
     for p, w, status in cases:
         assert lib.ts_attn_fwd_window(ctypes.byref(p), ctypes.byref(w), FAKE, 1 << 40, None) == status
         assert lib.ts_attn_fwd_window_workspace_size(ctypes.byref(p), ctypes.byref(w)) == 0
