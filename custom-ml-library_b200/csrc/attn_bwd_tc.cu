@@ -566,8 +566,9 @@ size_t tc_bwd_workspace(const ts_attn_bwd_params& bp) {
 }
 
 // How the key tiles with sinks are divided.  A CTA's time is its number of (query tile, head) pairs; undivided, a tile
-// with sinks takes those of all queries.  Parts of three quarters of an SM's even share of all pairs (16 at least) end
-// no later than the rest (16000 queries, 4 heads on one KV head of 128, a window of 500, 4 sinks: 131 us, 1668 undivided).
+// with sinks takes those of all queries.  That is no more than an SM's even share of all pairs,
+// or it is divided into parts of half a share (16 pairs at least), which end no later than the rest (16000 queries, 4
+// heads on one KV head of 128, a window of 500, 4 sinks: 131 us, 1668 undivided).
 struct SinkParts {
   int tiles, parts;
 };
@@ -578,7 +579,7 @@ static SinkParts sink_parts(const ts_attn_params& p, const WindowArgs& win) {
   const int64_t all = rep * ceil_div(p.q_len, kBM);
   const int64_t near = rep * i64min(ceil_div(p.q_len, kBM), ((int64_t)win.window + kBN) / kBM + 1);
   const int64_t share = heads * (with_sinks * all + (tiles - with_sinks) * near) / device_sms();
-  const int64_t most = i64max(16, share * 3 / 4), parts = (all + most - 1) / most;
+  const int64_t most = i64max(16, share / 2), parts = all <= share ? 1 : (all + most - 1) / most;
   return SinkParts{(int)with_sinks, (int)i64max(1, i64min(64, parts))};
 }
 
@@ -656,18 +657,19 @@ __global__ void bwd_stats_kernel(ts_attn_bwd_params bp, float* stats, int t_pad)
 }
 
 // The same under a window: 8 or 16 lanes a row with 16-byte loads, four rows of each in flight (16 heads of 16384
-// rows of 128: 42 us, where a warp a row with loads of one element takes 95).
+// rows of 128: 41 us, where a warp a row with loads of one element takes 95).
 template <typename T>
 __global__ void __launch_bounds__(256)
     window_stats_kernel(const __grid_constant__ ts_attn_bwd_params bp, float* stats, int t_pad, int lanes) {
   constexpr int kRows = 4;
   const ts_attn_params& p = bp.fwd;
-  const int64_t total = (int64_t)p.batch * p.q_heads * t_pad;
   const int c = threadIdx.x % lanes;
-  const int64_t row0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes * kRows;
-  // t_pad is a multiple of 64, so the rows of a thread belong to one head.
-  const int64_t bh = row0 / t_pad;
-  const int i0 = (int)(row0 - bh * t_pad), b = (int)(bh / p.q_heads), h = (int)(bh - (int64_t)b * p.q_heads);
+  // Heads fastest: the projections give a token's heads side by side.  t_pad is a multiple of 64.
+  const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int h = (int)(group % p.q_heads), b = (int)(group / p.q_heads / (t_pad / kRows));
+  const int i0 = (int)(group / p.q_heads % (t_pad / kRows)) * kRows;
+  const int64_t bh = (int64_t)b * p.q_heads + h;
+  const bool live = b < p.batch;
   uint4 g[kRows], o[kRows];
   float lse[kRows];
 #pragma unroll
@@ -675,7 +677,7 @@ __global__ void __launch_bounds__(256)
     const int64_t i = i0 + u;
     g[u] = o[u] = make_uint4(0u, 0u, 0u, 0u);
     lse[u] = -INFINITY;
-    if (row0 < total && i < p.q_len) {
+    if (live && i < p.q_len) {
       if (8 * c < p.value_dim) {
         g[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(bp.dout.data) + b * bp.dout.stride[0] +
                                                h * bp.dout.stride[1] + i * bp.dout.stride[2] + 8 * c);
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1)
       if (off < lanes) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    if (c == 0 && row0 < total) {
+    if (c == 0 && live) {
       stats[bh * 2 * t_pad + i0 + u] = lse[u] == -INFINITY ? -INFINITY : -lse[u] * kLog2e;
       stats[bh * 2 * t_pad + t_pad + i0 + u] = -acc;
     }
