@@ -550,21 +550,34 @@ __global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_k
       if (v0 + u * kGroup < v_last) raw[u] = __ldcs(body + v0 + u * kGroup);
   };
   load(v_first + id);  // under way while the row's numbers are read
-  const float m = p.norm[2 * row], log_s = p.norm[2 * row + 1], entropy = p.entropy[row];
+  float m = p.norm[2 * row], log_s = p.norm[2 * row + 1];
+  const float entropy = p.entropy[row];
   const int64_t target = p.targets[row];
   const bool real = target != p.ignore_index;
   const float g_target = real && a.grad_logprob ? a.grad_logprob[row] : 0.f;
-  const float g_entropy = a.grad_entropy ? a.grad_entropy[row] : 0.f;
+  float g_entropy = a.grad_entropy ? a.grad_entropy[row] : 0.f;
   float g_all = g_target;
   if (a.grad_top)
     for (int j = 0; j < p.top; ++j) g_all += a.grad_top[row * p.top + j];
   // A target outside the vocabulary has no log probability: its row's gradient is NaN, as that is.
   if (real && a.grad_logprob && (target < 0 || target >= p.vocab)) g_all = __int_as_float(0x7fc00000);
-  const bool none = log_s == -INFINITY;  // a row without a distribution has no gradient
+  const bool none = log_s == -INFINITY;  // a row without a distribution (every logit -inf) has no gradient
+  if (none) m = log_s = g_entropy = g_all = 0.f;
+  const uint64_t minus_m = ptx::f2pack(-m, -m), minus_s = ptx::f2pack(-log_s, -log_s);
+  const uint64_t log2e2 = ptx::f2pack(kLog2e, kLog2e), entropy2 = ptx::f2pack(entropy, entropy);
+  const uint64_t g_entropy2 = ptx::f2pack(-g_entropy, -g_entropy), g_all2 = ptx::f2pack(-g_all, -g_all);
+  auto grads_of = [&](uint64_t v, float& g0, float& g1) {
+    float d0, d1, e0, e1;
+    ptx::f2unpack(ptx::add2(ptx::add2(v, minus_m), minus_s), d0, d1);
+    const uint64_t d = ptx::f2pack(max_nan(d0, kFar), max_nan(d1, kFar));
+    ptx::f2unpack(ptx::fma2(d, log2e2, 0ull), e0, e1);
+    const uint64_t g = ptx::fma2(g_entropy2, ptx::add2(d, entropy2), g_all2);
+    ptx::f2unpack(ptx::fma2(ptx::f2pack(ex2(e0), ex2(e1)), g, 0ull), g0, g1);
+  };
   auto grad_of = [&](float v) {
-    if (none) return 0.f;
-    const float d = max_nan((v - m) - log_s, kFar);
-    return -ex2(d * kLog2e) * fmaf(g_entropy, d + entropy, g_all);
+    float g0, g1;
+    grads_of(ptx::f2pack(v, v), g0, g1);
+    return g0;
   };
   // Where the gradient's rows lie otherwise than the logits', elements are stored one by one.
   const bool aligned = (reinterpret_cast<uintptr_t>(out + span.head) & 15) == 0;
@@ -575,12 +588,7 @@ __global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_k
       if (v >= v_last) break;
       float g[N];
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        float x0, x1;
-        ptx::f2unpack(pair_of<T>(raw[u], i), x0, x1);
-        g[2 * i] = grad_of(x0);
-        g[2 * i + 1] = grad_of(x1);
-      }
+      for (int i = 0; i < N / 2; ++i) grads_of(pair_of<T>(raw[u], i), g[2 * i], g[2 * i + 1]);
       T* to = out + span.head + (int64_t)v * N;
       if (aligned) {
         uint4 w;
