@@ -9,10 +9,11 @@
 // exact in the accumulation type (fp32, or fp64 for fp64), exponentials in base 2.
 // Which columns a row sees is a 32-bit word a row and 32 columns (tree.cuh, window.cuh).
 //
-// Bound by the shared memory's reads of large problems, by the latency of a block's tiles of small ones.  Measured in
-// fp32, D 64 (the products that the mask needs, not the tiles'): 2 x 2000 queries, 8 heads, forward 428 us (19 TFLOP/s of
-// 74), with a window of 500 195 us; forward and backward 1402 and 749 us; 2 x 511 queries, 4 heads on 2, a window of
-// 128 and 3 sinks, forward and backward 107 us.
+// Bound by fixed latencies at two warps a scheduler, which registers and shared memory leave (half of the issue slots and
+// of the multiply-add pipe in use; with half the rows a block and three or four warps the reads cost more: gradients of
+// 2 x 2000 queries 1170 us against 940), and by a block's chain of tiles in small calls.  fp32, D 64, counting the pairs
+// that are seen: 2 x 2000 queries, 8 heads, forward 428 us (19 TFLOP/s of 74), with a window of 500 195 us; forward and
+// backward, on 4 KV heads, 1390 and 749 us; 2 x 511 queries, 4 heads on 2, a window of 128, 3 sinks, both 107 us.
 #pragma once
 #include "dependent.cuh"
 #include "simt_kernels.cuh"
@@ -757,7 +758,7 @@ __device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const Ro
 
 // Both in one launch, dK and dV first (a pair costs them four products, dQ three): small calls keep the SMs busy with
 // either, and larger ones have one tail.  In launches one behind the other (dQ, blocks with sinks, other blocks) the
-// gradients of the last example above took 105 us, now 70; of 2 x 2000 queries 1400, now 970.
+// last example above took 156 us with its forward, now 107; 2 x 2000 queries 1829, now 1390.
 template <typename T, int RTQ, int RTK, int DC>
 __global__ void __launch_bounds__(kRowsThreads)
     rows_window_bwd_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks, int dkv_blocks) {

@@ -12,8 +12,13 @@
 //               running maximum, sum and accumulator of their own, thread r on row r; joined at a unit's end
 // S is a tile ahead, so a V tile waits in the ring for its own P alone and the rest of the ring is in flight.
 // (Groups on alternate whole tiles hold two V tiles back, and the ring then keeps too little in flight: 198
-// against 150 us for 32 rows of 500 to 8192 keys, 16 nodes; with six slots instead of five, the queries of up to 64 rows
-// in half the room, 122.)
+// against 150 us for 32 rows of 500 to 8192 keys, 16 nodes; six slots instead of five, with the queries of up to 64
+// rows in half the room, 125.)
+// Bounded by memory for long caches: those 32 rows read 578 MB, 89 us at the rate of a copy, in 116 us of this kernel,
+// 14 of them until the first tile has come and 10 for the spread of the CTAs' ends; the join takes the other 9.  Few
+// rows and short caches are a chain of latencies: 2.5 us to plan, 2 for the first keys, 2.5 for the first softmax
+// (instructions come from L2), 1.8 a tile, 9 to join 37 parts (28 us for 2 rows of 32768 visible keys on 2 heads, 12 for
+// 37 keys on 4).
 // P is rounded to the type of V, as in the prefill kernels; scores, sums and accumulators are fp32.
 #include <type_traits>
 

@@ -13,7 +13,7 @@
 // Rows of up to 4096 logits are a warp's each, longer ones a block's, or a cluster's where there are few of them.
 // Bounded by memory: one read of the logits.  Backward: one read and one write, from the last row on, which the forward
 // has read last (L2).  bf16, 4096 rows of 128256: 177 us, 5.9 TB/s of 6.5 that a copy reaches; with 5 alternatives 222;
-// 4095 rows of 50257: 89 us, 4.6 TB/s (6 short waves of blocks), its gradient 130 us, 6.3 TB/s.
+// 4095 rows of 50257: 80 us, 5.2 TB/s (5.7 a wave of blocks, and 8 us to start and end), the gradient 121 us, 6.8 TB/s.
 #include <cooperative_groups.h>
 
 #include "dependent.cuh"
@@ -168,12 +168,12 @@ __device__ __forceinline__ void scan(const Span<T>& span, int id, int threads, i
   // whose kernel the register costs more (4096 rows of 128256: 226 against 222 us without, 180 against 177 with none).
   const bool edge = id < span.edges();
   float edge_x = !kTop && edge ? span.at(span.edge_index(id)) : -INFINITY;
-  for (int v0 = id, step = 0; v0 < span.vectors; v0 += threads * kUnroll, ++step) {
-    uint4 raw[kUnroll];
-    float top = -INFINITY;
+  uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (v0 + u * threads < span.vectors) raw[u] = body[v0 + u * threads];
+  for (int u = 0; u < kUnroll; ++u)
+    if (id + u * threads < span.vectors) raw[u] = body[id + u * threads];
+  for (int v0 = id, step = 0; v0 < span.vectors; v0 += threads * kUnroll, ++step) {
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (v0 + u * threads < span.vectors) top = max_nan(top, peak_of(raw[u], T()));
@@ -200,6 +200,8 @@ __device__ __forceinline__ void scan(const Span<T>& span, int id, int threads, i
         s2 = ptx::add2(s2, e);
         t2 = ptx::fma2(d, e, t2);
       }
+      const int next = v0 + (kUnroll + u) * threads;  // under way while the others are added
+      if (next < span.vectors) raw[u] = body[next];
     }
   }
   fold();
