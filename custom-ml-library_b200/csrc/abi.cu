@@ -694,7 +694,7 @@ bool window_split_faster(const ts_attn_params& p, const tsa::WindowArgs& win, bo
   const int dim = p.head_dim > p.value_dim ? p.head_dim : p.value_dim, sms = tsa::device_sms();
   const int group = p.q_heads / p.kv_heads, keys = tc ? 128 : dim <= 64 ? 64 : 32, line_rows = tc ? 128 : 64;
   const int64_t heads = (int64_t)p.q_heads * p.batch;
-  const int widest = dim <= 128 ? 4 : 2, rt = tc ? 8 : tsa::rows_rt(p.q_len, heads, widest);
+  const int rt = tc ? 8 : tsa::rows_rt(p.q_len, heads, tsa::rows_widest(dim));
   const int64_t rows = (int64_t)group * p.q_len, units = (rows + line_rows - 1) / line_rows * p.kv_heads * p.batch;
   // Key tiles of a block of `queries` tokens.
   auto tiles = [&](int64_t queries) {

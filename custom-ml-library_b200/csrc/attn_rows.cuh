@@ -13,7 +13,7 @@
 // of the multiply-add pipe in use; with half the rows a block and three or four warps the reads cost more: gradients of
 // 2 x 2000 queries 1170 us against 940), and by a block's chain of tiles in small calls.  fp32, D 64, counting the pairs
 // that are seen: 2 x 2000 queries, 8 heads, forward 428 us (19 TFLOP/s of 74), with a window of 500 195 us; forward and
-// backward, on 4 KV heads, 1390 and 749 us; 2 x 511 queries, 4 heads on 2, a window of 128, 3 sinks, both 107 us.
+// backward, on 4 KV heads, 1396 and 710 us; 2 x 511 queries, 4 heads on 2, a window of 128, 3 sinks, both 101 us.
 #pragma once
 #include "dependent.cuh"
 #include "simt_kernels.cuh"
@@ -543,9 +543,9 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) delta[row] = sum;
 }
 
-// Key blocks [first, first + count) whose queries are divided into parts of `queries`, a multiple of a tile.
+// Key blocks [first, first + count) whose tiles of queries, of all heads of the group, are divided into parts.
 struct RowsKeySet {
-  int first, count, parts, queries;
+  int first, count, parts;
   void* part;
 };
 struct RowsKeyBlocks {
@@ -639,7 +639,7 @@ __device__ __forceinline__ void rows_window_dq(const RowsWindowBwd& a, unsigned 
   }
 }
 
-// dK and dV of (KV head and row, key block, part of the queries).  With one part they are written at once; with more,
+// dK and dV of (KV head and row, key block, part of its tiles of queries).  With one part they are written at once; with more,
 // each part leaves its sums in `part` and rows_dkv_sum_kernel adds them in order.
 template <typename T, int RT, int DC>
 __device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const RowsKeyBlocks& blocks, unsigned char* smem_raw,
@@ -671,17 +671,15 @@ __device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const Ro
   clear(dv);
   const A scale = (A)p.scale, scale2 = (A)(p.scale * kLog2eD);
   // Queries that see some of the block's keys, and this part's of them.
-  int64_t first = i64min(p.q_len, i64max(0, j0 - offset) / kCols * kCols), stop = p.q_len;
+  const int64_t first = i64min(p.q_len, i64max(0, j0 - offset) / kCols * kCols);
+  int64_t stop = p.q_len;
   if (j0 >= a.win.sinks) stop = i64min(stop, (int64_t)min(j0 + C::kRows, kv_end) - 1 - offset + a.win.window);
   if (j0 >= kv_end) stop = 0;
-  if (set.parts > 1) {
-    const int64_t from = first + (int64_t)part * set.queries;
-    stop = i64min(stop, from + set.queries);
-    first = from;
-  }
-  const int tiles_a_head = first < stop ? (int)((stop - first + kCols - 1) / kCols) : 0, n = rep * tiles_a_head;
+  const int tiles_a_head = first < stop ? (int)((stop - first + kCols - 1) / kCols) : 0;
+  const int64_t all = (int64_t)rep * tiles_a_head, it0 = part * all / set.parts;
+  const int n = (int)((part + 1) * all / set.parts - it0);
   auto stage = [&](int it) {
-    const int h = hk * rep + it / tiles_a_head, i0 = (int)first + it % tiles_a_head * kCols;
+    const int h = hk * rep + (int)((it0 + it) / tiles_a_head), i0 = (int)(first + (it0 + it) % tiles_a_head * kCols);
     A* q = tiles + it % kBufs * 2 * kCols * C::kStride;
     stage_tile<T, A>(q, C::kStride, p.q, b, h, i0, kCols, p.q_len, p.head_dim);
     stage_tile<T, A>(q + kCols * C::kStride, C::kStride, a.bp.dout, b, h, i0, kCols, p.q_len, p.value_dim);
@@ -694,7 +692,7 @@ __device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const Ro
   };
   if (n > 0) stage(0);
   for (int it = 0; it < n; ++it) {
-    const int i0 = (int)first + it % tiles_a_head * kCols;
+    const int i0 = (int)(first + (it0 + it) % tiles_a_head * kCols);
     const A *q = tiles + it % kBufs * 2 * kCols * C::kStride, *g = q + kCols * C::kStride;
     const A *lse2 = s_lse2[it % kBufs], *delta = s_delta[it % kBufs];
     ptx::copies_done();
@@ -758,7 +756,7 @@ __device__ __forceinline__ void rows_window_dkv(const RowsWindowBwd& a, const Ro
 
 // Both in one launch, dK and dV first (a pair costs them four products, dQ three): small calls keep the SMs busy with
 // either, and larger ones have one tail.  In launches one behind the other (dQ, blocks with sinks, other blocks) the
-// last example above took 156 us with its forward, now 107; 2 x 2000 queries 1829, now 1390.
+// last example above took 156 us with its forward, then 107; 2 x 2000 queries 1829, then 1402.
 template <typename T, int RTQ, int RTK, int DC>
 __global__ void __launch_bounds__(kRowsThreads)
     rows_window_bwd_kernel(const __grid_constant__ RowsWindowBwd a, const __grid_constant__ RowsKeyBlocks blocks, int dkv_blocks) {
@@ -815,21 +813,24 @@ cudaError_t rows_window_fwd_t(const RowsWindow& a, cudaStream_t st) {
   return launch_rows(rows_window_fwd_kernel<T, RT, DC>, grid, C::kFwdSmem, st, a);
 }
 
-// The key blocks with sinks, which all the queries behind them see, and the others, each divided until the SMs have
-// work for several blocks (at most 64 parts: a part's sums are written and read once more).
+// The key blocks with sinks, which all the queries behind them see, and the others, each divided into as many blocks as
+// the SMs hold at a time (and at most 64 parts): more of them cost more in copies of K and V and in sums that are written
+// and read once more than they even out (1000 queries, 4 heads of 128, a window of 300, 100 sinks, gradients: 295 us,
+// 342 with twice as many; 202 queries of 24 heads on 3 behind 501 keys 124 against 113).  Under a window of half the
+// queries or more the blocks' lengths differ, and three times as many even them out (2 x 2000 queries, 8 heads on 4 of
+// 64, no narrower window: 1396 us, 1511 undivided).
 template <typename A>
 RowsKeyBlocks rows_key_blocks(const ts_attn_params& p, const WindowArgs& win, int rows, int cols, unsigned char* ws,
                               size_t* bytes) {
   const int blocks = ceil_div(p.kv_len, rows), with_sinks = ceil_div(min(win.sinks, p.kv_len), rows);
-  const int64_t heads = (int64_t)p.kv_heads * p.batch, want = 6 * (int64_t)device_sms();
+  const int64_t heads = (int64_t)p.kv_heads * p.batch;
+  const int64_t want = (win.window < p.q_len / 2 ? 2 : 6) * (int64_t)device_sms();
   *bytes = 0;
   auto divide = [&](int first, int count, int64_t seen) {
-    RowsKeySet s{first, count, 0, 0, nullptr};
+    RowsKeySet s{first, count, 0, nullptr};
     if (count == 0) return s;
-    const int64_t tiles = (seen + cols - 1) / cols;
-    const int64_t parts = i64max(1, i64min(i64min(64, tiles), want / i64max(1, heads * count)));
-    s.queries = (int)((tiles + parts - 1) / parts) * cols;
-    s.parts = (int)((seen + s.queries - 1) / s.queries);
+    const int64_t tiles = p.q_heads / p.kv_heads * ((seen + cols - 1) / cols);
+    s.parts = (int)i64max(1, i64min(i64min(64, tiles), want / i64max(1, heads * count)));
     s.part = ws ? ws + *bytes : nullptr;
     if (s.parts > 1) *bytes += sizeof(A) * (size_t)s.parts * heads * count * rows * (p.head_dim + p.value_dim);
     return s;
@@ -883,8 +884,8 @@ cudaError_t rows_tree_t(TreeArgs& a, cudaStream_t st) {
 template <typename T, int DC>
 cudaError_t rows_window_fwd_d(const RowsWindow& a, cudaStream_t st) {
   using A = typename Elem<T>::acc;
-  const int rt = rows_rt(a.p.q_len, (int64_t)a.p.q_heads * a.p.batch, sizeof(A) == 8 ? (DC <= 4 ? 2 : 1) : DC <= 4 ? 4 : 2);
-  if constexpr (sizeof(A) == 4 && DC <= 4)
+  const int rt = rows_rt(a.p.q_len, (int64_t)a.p.q_heads * a.p.batch, sizeof(A) == 8 ? (DC <= 4 ? 2 : 1) : rows_widest(32 * DC));
+  if constexpr (sizeof(A) == 4 && DC == 2)
     if (rt == 4) return rows_window_fwd_t<T, 4, DC>(a, st);
   if constexpr (sizeof(A) == 4 || DC <= 4)
     if (rt == 2) return rows_window_fwd_t<T, 2, DC>(a, st);

@@ -17,6 +17,10 @@ struct RowsWindow {
   }
 };
 
+// Row tiles of a forward block: four for up to 64 channels (2 x 2000 queries, 8 heads of 64: 425 us, with two 449), two
+// for more (2 x 1500 of 128: 540 us, with four 600).
+inline int rows_widest(int dim) { return dim <= 64 ? 4 : 2; }
+
 // Row tiles of a block, at most `widest`.  A tile costs the reads of its columns, the same for any number of row tiles,
 // and those of its rows (about 8 to 1), and the blocks of an SM share what it can read.
 inline int rows_rt(int rows, int64_t slices, int widest) {
