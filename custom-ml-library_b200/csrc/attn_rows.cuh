@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_fwd_kernel(const __g
   for (int r = 0; r < RT; ++r) {
     const int i = i0 + f.ty + 16 * r;
     if (i >= p.q_len) continue;
-    const A inv = f.l[r] > A(0) ? A(1) / f.l[r] : A(0);
+    const A inv = f.l[r] == A(0) ? A(0) : A(1) / f.l[r];  // a sum that is NaN stays one
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_fwd_kernel(const __g
     if (p.lse && f.tx == 0)
       reinterpret_cast<A*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
                                   (int64_t)i * p.lse_stride[2]] =
-          f.l[r] > A(0) ? (f.m[r] + acc_log2(f.l[r])) * (A)kLn2D : neg_inf<A>();
+          f.l[r] == A(0) ? neg_inf<A>() : (f.m[r] + acc_log2(f.l[r])) * (A)kLn2D;
   }
 }
 
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
                 make_float4(f.acc[r][c][0], f.acc[r][c][1], f.acc[r][c][2], f.acc[r][c][3]);
       } else {
         const int h = hk * group + i / p.q_len, node = i % p.q_len;
-        const A inv = f.l[r] > A(0) ? A(1) / f.l[r] : A(0);
+        const A inv = f.l[r] == A(0) ? A(0) : A(1) / f.l[r];  // a sum that is NaN stays one
 #pragma unroll
         for (int c = 0; c < DC; ++c)
 #pragma unroll
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
         if (p.lse && f.tx == 0)
           reinterpret_cast<A*>(p.lse)[(int64_t)b * p.lse_stride[0] + (int64_t)h * p.lse_stride[1] +
                                       (int64_t)node * p.lse_stride[2]] =
-              f.l[r] > A(0) ? (f.m[r] + acc_log2(f.l[r])) * (A)kLn2D : neg_inf<A>();
+              f.l[r] == A(0) ? neg_inf<A>() : (f.m[r] + acc_log2(f.l[r])) * (A)kLn2D;
       }
     }
     if constexpr (!kSplit) break;

@@ -109,6 +109,21 @@ def test_many_keys(dtype, dim):
     assert not dk.any() and not dv.any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f64", "bf16"])
+def test_nan_stays_in_its_row(dtype):
+    """A query that is NaN, and a key that only two queries see: their outputs are NaN (on CUDA cores the LSE too)."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (heads(gen, 1, 200, 2, 64, dtype) for _ in range(3))
+    clean, clean_lse = engine.forward(q, k, v, is_causal=True, window=2)
+    q[0, 1, 17, 3] = float("nan")
+    k[0, 0, 90, 0] = float("nan")
+    out, lse = engine.forward(q, k, v, is_causal=True, window=2)
+    gone = torch.zeros(2, 200, dtype=torch.bool, device="cuda")
+    gone[1, 17] = gone[0, 90] = gone[0, 91] = True
+    assert out[0][gone].isnan().all() and (dtype == "bf16" or lse[0][gone].isnan().all())
+    assert torch.equal(out[0][~gone], clean[0][~gone]) and torch.equal(lse[0][~gone], clean_lse[0][~gone])
+
+
 def test_value_dimension_and_scale():
     run("f32", 1, 2, 2, 100, 48, 30, 2, value_dim=80, path="simt")
     run("bf16", 1, 2, 2, 100, 64, 30, 2, value_dim=32, path="simt")
