@@ -252,6 +252,54 @@ def test_refusals():
             nn.keep_drafts(caches, 1, [[0], [0]])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("captured", [False, True])
+def test_two_streams_at_once(dtype, captured):
+    """A decoding loop on each of two streams, eager or as graphs replayed side by side, gives what it gives alone."""
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def work(seed):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        make = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dtype)  # noqa: E731
+        q, k, v, x = make(3, 8, 6, 64), make(3, 2, 900, 64), make(3, 2, 900, 64), make(18, 20011)
+        lens, tree = ints([800, 77, 301]), ints([[-1, 0, 0, 1, 2, 2]] * 3)
+        path, counts = ints([[0, 2, 5], [0, 1, 3], [0, 0, 0]]), ints([3, 3, 1])
+        keys, values, goal = k.clone(), v.clone(), torch.arange(18, device="cuda")
+
+        def step():
+            keys.copy_(k)
+            values.copy_(v)
+            o, lse = engine.attention_tree(q, keys, values, lens, tree, need_lse=True)
+            w, _ = engine.forward(q, keys, values, is_causal=True, kv_lens=lens, window=200, sinks=3)
+            engine.kv_keep([(keys, values)], lens - 6, path, counts)
+            lp = engine.token_logprobs(x, goal, top=3)
+            return [o, lse, w, keys, values, *lp, engine.token_logprobs_backward(x, goal, lp, lp.logprob)]
+
+        return step
+
+    steps = [work(1), work(2)]
+    want = [[t.clone() for t in step()] for step in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    got = [None, None]
+    if captured:
+        graphs = [torch.cuda.CUDAGraph() for _ in steps]
+        for i, (graph, step) in enumerate(zip(graphs, steps)):
+            with torch.cuda.graph(graph, stream=streams[i]):
+                got[i] = step()
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                if captured:
+                    graphs[i].replay()
+                else:
+                    got[i] = steps[i]()
+    torch.cuda.synchronize()
+    engine.check_device_status()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_a_failed_step_gives_ragged_rows_back():
     """A layer that fails leaves every row of every cache at its own length."""
     lm = model()
