@@ -52,13 +52,14 @@ __device__ __forceinline__ void copy_row16(void* dst, const void* src, bool live
 }
 
 // Rows [t0, t0 + rows) of (b, h) into shared memory, a row every `stride` elements; zeros at and behind row `end` and
-// channel C (to a whole quad).  fp32 rows on 16-byte boundaries are under way when it returns (ptx::copies_done).
+// channel C (to a whole quad, which is what the products read: vectors alone serve where C ends with one, as a double's
+// two channels need not).  fp32 rows on 16-byte boundaries are under way when it returns (ptx::copies_done).
 template <typename T, typename A>
 __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& src, int b, int h, int64_t t0, int rows,
                                            int64_t end, int C) {
   constexpr int kVec = 16 / sizeof(T);
   const T* base = reinterpret_cast<const T*>(src.data) + (int64_t)b * src.stride[0] + (int64_t)h * src.stride[1];
-  const bool vec = src.stride[3] == 1 && C % kVec == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
+  const bool vec = src.stride[3] == 1 && C % kVec == 0 && C % 4 == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(base) % 16 == 0;
   if (vec) {
     const int per = C / kVec, n = rows * per;
@@ -115,7 +116,7 @@ __device__ __forceinline__ void stage_packed(A* dst, int stride, const ts_view4&
   constexpr int kVec = 16 / sizeof(T), kBatch = 4;
   const T* base = reinterpret_cast<const T*>(src.data) + (int64_t)b * src.stride[0];
   auto row_at = [&](int r) { return base + (int64_t)(h0 + r / tokens) * src.stride[1] + (int64_t)(r % tokens) * src.stride[2]; };
-  const bool vec = src.stride[3] == 1 && C % kVec == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
+  const bool vec = src.stride[3] == 1 && C % kVec == 0 && C % 4 == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
                    (src.stride[1] * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0;
   const int wide = ceil_div(C, 4) * 4, per = vec ? C / kVec : wide, n = rows * per;
   for (int x0 = threadIdx.x; x0 < n; x0 += kRowsThreads * kBatch) {
