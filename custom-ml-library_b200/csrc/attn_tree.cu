@@ -555,6 +555,9 @@ __global__ void __launch_bounds__(kMergeThreads)
         if (4 * quad + e < p.value_dim) out[e * p.o.stride[3]] = value[e];
     }
   };
+  // Of a result whose reference is x.  One without a reference has seen nothing, or NaN alone: 0 times its sum, 0 or
+  // NaN, is what it adds to the row's.
+  auto weight = [](float x, float m) { return x == -INFINITY ? 0.f : ptx::ex2(x - m); };
   auto add = [](float4& sum, float w, const float4& o) {
     if (w == 0.f) return;  // a part that has seen nothing may hold anything
     sum.x = fmaf(w, o.x, sum.x);
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(kMergeThreads)
       for (int i = 0; i < kFewParts; ++i) m = fmaxf(m, v[i].x);
 #pragma unroll
       for (int i = 0; i < kFewParts; ++i) {
-        const float w = v[i].x == -INFINITY ? 0.f : ptx::ex2(v[i].x - m);
+        const float w = weight(v[i].x, m);
         l = fmaf(w, v[i].y, l);
         add(sum, w, o[i]);
       }
@@ -616,10 +619,9 @@ __global__ void __launch_bounds__(kMergeThreads)
       }
 #pragma unroll
       for (int u = 0; u < kFewParts; ++u) top = fmaxf(top, v[u].x);
-      l = m == -INFINITY ? 0.f : l * ptx::ex2(m - top);
+      l *= weight(m, top);
 #pragma unroll
-      for (int u = 0; u < kFewParts; ++u)
-        if (v[u].x != -INFINITY) l = fmaf(ptx::ex2(v[u].x - top), v[u].y, l);
+      for (int u = 0; u < kFewParts; ++u) l = fmaf(weight(v[u].x, top), v[u].y, l);
       m = top;
     }
     s_row[threadIdx.x] = make_float2(m, l);
@@ -630,9 +632,7 @@ __global__ void __launch_bounds__(kMergeThreads)
     if (row_slice < n - half) {
       const float2 x = s_row[threadIdx.x], y = s_row[threadIdx.x + half * rows];
       const float m = fmaxf(x.x, y.x);
-      float l = x.x == -INFINITY ? 0.f : ptx::ex2(x.x - m) * x.y;
-      if (y.x != -INFINITY) l = fmaf(ptx::ex2(y.x - m), y.y, l);
-      s_row[threadIdx.x] = make_float2(m, l);
+      s_row[threadIdx.x] = make_float2(m, fmaf(weight(y.x, m), y.y, weight(x.x, m) * x.y));
     }
     __syncthreads();
     n = half;

@@ -1,4 +1,5 @@
-"""Windows and drafted trees where they can go wrong beside sizes and masks: head dimensions of half a quad."""
+"""Windows and drafted trees where they can go wrong beside sizes and masks: head dimensions of half a quad, NaN through
+the join of many partial results."""
 
 import random
 
@@ -14,6 +15,11 @@ torch = pytest.importorskip("torch")
 from tensorsmith_b200 import engine  # noqa: E402
 
 NAN = float("nan")
+
+
+def make(dtype, *shape, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=gen, device="cuda").to(DTYPES[dtype])
 
 
 def nan_everywhere(dtype, dim):
@@ -35,3 +41,41 @@ def test_f64_half_quads(dim, value_dim):
     rng = random.Random(dim)
     nan_everywhere("f64", room)
     check("f64", 4, 2, dim, [9, 200, 131], [random_tree(rng, 7, b) for b in range(3)], value_dim=value_dim, path="simt")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("keys", [300, 20011])
+@pytest.mark.parametrize("nodes,tree", [(1, False), (3, True)])
+def test_nan_through_the_join(dtype, keys, nodes, tree):
+    """A NaN query, and NaN keys in a part of a row: NaN in what sees them, output and LSE, with few partial results
+    and with many; nothing changes elsewhere, and a padded node and an empty row stay zero."""
+    q, k, v = make(dtype, 3, 2, nodes, 64), make(dtype, 3, 1, keys, 64, seed=1), make(dtype, 3, 1, keys, 64, seed=2)
+    lens = torch.tensor([keys, keys - 60, 0], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([[-1, 0, -2]] * 3, dtype=torch.int32, device="cuda") if tree else None
+    clean, clean_lse = engine.attention_tree(q, k, v, lens, parents, need_lse=True)
+    q[0, 1, 0, 5] = NAN
+    if tree:
+        q[0, 0, 2] = NAN  # of a padded node
+    k[1, 0, keys // 2 : keys // 2 + keys // 10] = NAN
+    out, lse = engine.attention_tree(q, k, v, lens, parents, need_lse=True)
+    gone = torch.zeros(3, 2, nodes, dtype=torch.bool, device="cuda")
+    gone[0, 1, 0] = True
+    gone[1, :, : 2 if tree else 1] = True
+    assert out[gone].isnan().all() and lse[gone].isnan().all()
+    assert torch.equal(out[~gone], clean[~gone]) and torch.equal(lse[~gone], clean_lse[~gone])
+    assert not clean[2].any() and (clean_lse[2] == -float("inf")).all()
+    if tree:
+        assert not clean[:, :, 2].any() and (clean_lse[:, :, 2] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_nan_through_a_split_window(dtype, monkeypatch):
+    monkeypatch.setenv("TS_WINDOW_KERNEL", "split")
+    q, k, v = make(dtype, 1, 2, 2, 64), make(dtype, 1, 1, 9001, 64, seed=1), make(dtype, 1, 1, 9001, 64, seed=2)
+    kw = dict(is_causal=True, window=8000, sinks=4, causal_offset=8999)
+    clean, clean_lse = engine.forward(q, k, v, **kw)
+    q[0, 1, 1, 0] = NAN
+    out, lse = engine.forward(q, k, v, **kw)
+    assert out[0, 1, 1].isnan().all() and lse[0, 1, 1].isnan()
+    out[0, 1, 1], lse[0, 1, 1] = clean[0, 1, 1], clean_lse[0, 1, 1]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
