@@ -51,12 +51,21 @@ __device__ __forceinline__ void copy_row16(void* dst, const void* src, bool live
                : "memory");
 }
 
-// Rows [t0, t0 + rows) of (b, h) into shared memory, a row every `stride` elements; zeros at and behind row `end` and
-// channel C (to a whole quad, which is what the products read: vectors alone serve where C ends with one, as a double's
-// two channels need not).  fp32 rows on 16-byte boundaries are under way when it returns (ptx::copies_done).
-template <typename T, typename A>
+// Which rows of a tile are zeros whatever memory holds: none, or those of a word's bits.
+struct NoneGone {
+  __device__ __forceinline__ bool operator()(int) const { return false; }
+};
+struct BitsGone {
+  uint64_t bits;
+  __device__ __forceinline__ bool operator()(int r) const { return bits >> r & 1u; }
+};
+
+// Rows [t0, t0 + rows) of (b, h) into shared memory, a row every `stride` elements; zeros in rows that are gone, at
+// and behind row `end`, and from channel C on (to a whole quad, which is what the products read: vectors alone serve
+// where C ends with one, as a double's two channels need not).  fp32 rows on 16-byte boundaries are under way when it returns (ptx::copies_done).
+template <typename T, typename A, typename Gone = NoneGone>
 __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& src, int b, int h, int64_t t0, int rows,
-                                           int64_t end, int C) {
+                                           int64_t end, int C, Gone gone = Gone()) {
   constexpr int kVec = 16 / sizeof(T);
   const T* base = reinterpret_cast<const T*>(src.data) + (int64_t)b * src.stride[0] + (int64_t)h * src.stride[1];
   const bool vec = src.stride[3] == 1 && C % kVec == 0 && C % 4 == 0 && (src.stride[2] * sizeof(T)) % 16 == 0 &&
@@ -66,7 +75,7 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
     if constexpr (sizeof(T) == 4) {
       for (int x = threadIdx.x; x < n; x += kRowsThreads) {
         const int r = x / per, c = x - r * per;
-        const bool live = t0 + r < end;
+        const bool live = t0 + r < end && !gone(r);
         copy_row16(dst + r * stride + c * kVec, live ? base + (t0 + r) * src.stride[2] + c * kVec : base, live);
       }
       return;
@@ -78,7 +87,8 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
       for (int u = 0; u < kBatch; ++u) {
         const int x = x0 + u * kRowsThreads, r = x / per, c = x % per;
         raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (x < n && t0 + r < end) raw[u] = *reinterpret_cast<const uint4*>(base + (t0 + r) * src.stride[2] + c * kVec);
+        if (x < n && t0 + r < end && !gone(r))
+          raw[u] = *reinterpret_cast<const uint4*>(base + (t0 + r) * src.stride[2] + c * kVec);
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
@@ -99,7 +109,8 @@ __device__ __forceinline__ void stage_tile(A* dst, int stride, const ts_view4& s
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int x = x0 + u * kRowsThreads, r = x / wide, c = x % wide;
-      raw[u] = x < n && c < C && t0 + r < end ? base[(t0 + r) * src.stride[2] + c * src.stride[3]] : Elem<T>::from_acc(A(0));
+      raw[u] = x < n && c < C && t0 + r < end && !gone(r) ? base[(t0 + r) * src.stride[2] + c * src.stride[3]]
+                                                          : Elem<T>::from_acc(A(0));
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -329,16 +340,17 @@ template <typename T, int RT, int DC> struct RowsForward {
     for (int r = 0; r < RT; ++r) m[r] = neg_inf<A>(), l[r] = A(0);
   }
   // n tiles, tile j at key key_of(j), of head hk; bits(r, slot): what row ty + 16 r sees of the 32 keys from `slot` on.
-  // Keys at and behind `end` are not read.  K of the next tile is under way during P.V, V during Q.K.
-  template <typename Key, typename Bits>
+  // Keys at and behind `end` are not read, nor the values of those of tile k0 that gone_of(k0) names.  K of the next tile
+  // is under way during P.V, V during Q.K.
+  template <typename Key, typename Bits, typename GoneOf>
   __device__ __forceinline__ void run(const ts_attn_params& p, int b, int hk, int n, int end, A scale2, Key key_of,
-                                      Bits bits) {
+                                      Bits bits, GoneOf gone_of) {
     if (n > 0) stage_tile<T, A>(k, C::kStride, p.k, b, hk, key_of(0), kCols, end, p.head_dim);
     for (int j = 0; j < n; ++j) {
       const int k0 = key_of(j);
       ptx::copies_done();
       __syncthreads();  // K(j) is there, V(j - 1) is used up
-      stage_tile<T, A>(v, C::kStride, p.v, b, hk, k0, kCols, end, p.value_dim);
+      stage_tile<T, A>(v, C::kStride, p.v, b, hk, k0, kCols, end, p.value_dim, gone_of(k0));
       A s[RT][kNC];
       dots<RT, kNC>(s, q, k, C::kStride, p.head_dim, ty, tx);
 #pragma unroll
@@ -407,7 +419,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_window_fwd_kernel(const __g
           const int64_t stop = i64min(kv_end, i + offset + 1);
           return range_bits(i + offset + 1 - a.win.window, stop, slot) |
                  range_bits(0, i64min(stop, a.win.sinks), slot);
-        });
+        },
+        [](int) { return NoneGone(); });
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int i = i0 + f.ty + 16 * r;
@@ -439,6 +452,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ LinePlace s_ends[2];
   __shared__ int s_parents[kTreeNodes];
+  __shared__ uint64_t s_hidden;
   const ts_attn_params& p = a.p;
   wait_for_previous();
   let_next_start();
@@ -469,6 +483,13 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
     const WindowTiles& wt = walk.list.tiles;
     __syncthreads();  // the unit before is used up
     if (a.parents && (int)threadIdx.x < p.q_len) s_parents[threadIdx.x] = a.parents[b * a.parents_stride + threadIdx.x];
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x, n = a.parents ? p.q_len : 0;  // a chain's slots are all seen
+      const int32_t* parents = a.parents + b * a.parents_stride;
+      const uint64_t hidden =
+          n ? hidden_nodes(n, base, lane < n ? parents[lane] : -1, lane + 32 < n ? parents[lane + 32] : -1, lane) : 0;
+      if (lane == 0) s_hidden = hidden;
+    }
     stage_packed<T, A>(f.q, F::C::kStride, p.q, b, hk * group, r0, F::C::kRows, a.rows, p.q_len, p.head_dim);
     __syncthreads();
     NodeView view[RT];
@@ -480,7 +501,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_tree_kernel(const __grid_co
     }
     f.start();
     f.run(p, b, hk, walk.count, len, scale2, [&](int j) { return wt.tile(walk.first + j) * F::kCols; },
-          [&](int r, int slot) { return view_bits(view[r], base, a.win.sinks, slot); });
+          [&](int r, int slot) { return view_bits(view[r], base, a.win.sinks, slot); },
+          [&](int k0) { return BitsGone{gone_bits(s_hidden, base, len, k0)}; });
     const int64_t part = (int64_t)b * line.units + walk.unit + blockIdx.x;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {

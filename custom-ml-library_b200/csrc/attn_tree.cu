@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(384, 1)
     const float qk_scale = (float)p.scale * kLog2e;
     int64_t i = 0;  // tile of the share
     NodeView view;
+    uint64_t hidden = 0;  // of row view_b
     int view_b = -1, view_r0 = -1;
     bool ok = true;
     for (int seg = 0; ok && walk.next(line); ++seg) {
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(384, 1)
       const bool live_warp = r0 + (warp & 3) * 32 < args.rows;  // some row of the warp is a query's
       const bool live = r0 + row < args.rows;
       if (b != view_b || r0 != view_r0) {  // the heads of a row share it
-        view = tree_node_of_warp((r0 + row) % p.q_len, p.q_len, base, args, b, lane);
+        view = tree_node_of_warp((r0 + row) % p.q_len, p.q_len, base, args, b, lane, &hidden);
         if (!live) {
           view.end = 0;
           view.drafted = 0;
@@ -382,8 +383,10 @@ __global__ void __launch_bounds__(384, 1)
           }
           ptx::tmem_wait_st();
         }
-        if (kh + kHalf > len) {
-          // The cache may hold anything behind its last key: its values there become zeros, as 0 * NaN is NaN.
+        const bool hides = hidden && kh + kHalf > base && kh < base + p.q_len;
+        if (kh + kHalf > len || hides) {
+          // The cache may hold anything behind its last key and in the slots of padded nodes: its values there become
+          // zeros, as 0 * NaN is NaN.
           const int64_t f = i64min(2 + 2 * i, 2 * n_tiles - 1);  // the fill that brought this tile's V
           unsigned char* v = sKV + (int)(f % S) * C::kTileBytes;
           if (!__all_sync(0xffffffffu,
@@ -391,11 +394,16 @@ __global__ void __launch_bounds__(384, 1)
             ok = false;
             break;
           }
-          const int gone = max(len - kh, 0);  // first row of the half to clear
-          for (int x = row; x < (kHalf - gone) * (D / 8); x += 128) {
-            const int vr = t * kHalf + gone + x / (D / 8), c = x % (D / 8);
-            *reinterpret_cast<uint4*>(v + (c >> 3) * kSlabBytes + vr * 128 + ((c & 7) << 4)) =
+          auto clear = [&](int hr, int c) {  // 8 channels of a row of the half
+            *reinterpret_cast<uint4*>(v + (c >> 3) * kSlabBytes + (t * kHalf + hr) * 128 + ((c & 7) << 4)) =
                 make_uint4(0u, 0u, 0u, 0u);
+          };
+          const int gone = max(len - kh, 0);  // first row behind the last key
+          for (int x = row; x < (kHalf - gone) * (D / 8); x += 128) clear(gone + x / (D / 8), x % (D / 8));
+          if (hides) {
+            const uint64_t bits = gone_bits(hidden, base, len, kh);
+            for (int x = row; x < kHalf * (D / 8); x += 128)
+              if ((bits >> (x / (D / 8))) & 1u) clear(x / (D / 8), x % (D / 8));
           }
           ptx::fence_proxy_async_smem();
         }

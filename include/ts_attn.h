@@ -410,7 +410,8 @@ typedef struct ts_window {
 } ts_window;
 
 /* ts_attn_fwd under a window: is_causal must be set, no explicit mask, no dropout.  Keys between the sinks and the
- * window of a block of queries are not read.  Half types with equal head dimensions that are multiples of 8 up to 128
+ * window of a block of queries are not read, but for those that share a tile (128 keys at most) with one that is seen:
+ * their values must be finite, as 0 * NaN is NaN.  Half types with equal head dimensions that are multiples of 8 up to 128
  * run on the tcgen05 kernels (P in q's type, as ts_attn_fwd), everything else on CUDA cores.  Chunks too short to give
  * every SM a block are shared along their keys as in ts_attn_tree and then need the workspace; the environment variable
  * TS_WINDOW_KERNEL = "split", "tile" or "pair" (a block for 128 or 256 queries), read at every call, forces one way where
@@ -433,7 +434,7 @@ TS_ATTN_API int ts_attn_bwd_window(const ts_attn_bwd_params* params, const ts_wi
 typedef struct ts_tree {
   const int32_t* parents; /* [batch, q_len] (device): node i's parent, a node before it, or -1: the committed tokens.
                              Any other value marks a padded node: it and its children give zeros (LSE -inf) and are
-                             seen by nobody.  NULL: a chain, node i's parent is node i - 1. */
+                             seen by nobody, whatever their slots hold.  NULL: a chain, node i's parent is node i - 1. */
   int64_t parents_stride; /* entries between rows */
   int32_t window, sinks;  /* ts_window; window 0: none */
 } ts_tree;
@@ -441,7 +442,7 @@ typedef struct ts_tree {
 
 /* Attention of q [batch, Hq, q_len, D] over the cache k, v: params as for ts_attn_decode with kv_lens required;
  * is_causal and causal_offset are ignored, no explicit mask.  Slots at and behind kv_lens[b] are not used, whatever
- * they hold.  Half types with equal head dimensions that are multiples of 8 up to 128 run on the tcgen05 kernel. */
+ * they hold; the values of the others must be finite (one that is not may reach nodes that do not see it).  Half types with equal head dimensions that are multiples of 8 up to 128 run on the tcgen05 kernel. */
 TS_ATTN_API int ts_attn_tree(const ts_attn_params* params, const ts_tree* tree, void* workspace,
                              size_t workspace_bytes, void* stream);
 TS_ATTN_API int ts_attn_tree_path(const ts_attn_params* params, const ts_tree* tree);

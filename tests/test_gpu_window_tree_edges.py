@@ -1,11 +1,11 @@
 """Windows and drafted trees where they can go wrong beside sizes and masks: head dimensions of half a quad, NaN through
-the join of many partial results."""
+the join of many partial results, slots that nobody sees."""
 
 import random
 
 import pytest
 
-from plain64 import DTYPES
+from plain64 import DTYPES, tree_seen
 from test_gpu_tree import check, random_tree
 from test_gpu_window import run
 
@@ -79,3 +79,32 @@ def test_nan_through_a_split_window(dtype, monkeypatch):
     assert out[0, 1, 1].isnan().all() and lse[0, 1, 1].isnan()
     out[0, 1, 1], lse[0, 1, 1] = clean[0, 1, 1], clean_lse[0, 1, 1]
     assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f16", 128), ("bf16", 96), ("f32", 64), ("f32", 33), ("f64", 64),
+                                       ("f64", 6), ("bf16", 256), ("f16", 20)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 200)])
+def test_slots_of_padded_nodes_may_hold_anything(dtype, dim, window, sinks):
+    """Slots below kv_lens that nobody sees: of padded nodes, of their children, of children of nodes before the cache."""
+    rng = random.Random(dim)
+    nodes = 40
+    odd = [-2, nodes, 2**31 - 1, -(2**31)]
+    trees = [random_tree(rng, nodes) for _ in range(6)]
+    for tree in trees[1:]:
+        for i in rng.sample(range(nodes), 6):
+            tree[i] = rng.choice([*odd, i])
+    lens = [170, 150, 128 + 20, 40, 25, 9000]  # nodes over a tile's border, at a row's start, of a row in many parts
+    q, k, v, kv_lens, parents, out, lse = check(dtype, 4, 2, dim, lens, trees, window=window, sinks=sinks,
+                                                capacity=9000)
+    hidden = ~tree_seen(trees, lens, 9000).any(2)[:, 0].cuda()  # no node sees the slot
+    for b, n in enumerate(lens):
+        hidden[b, : max(n - nodes, 0)] = hidden[b, n:] = False
+    assert hidden.any()
+    for fill in (NAN, float("inf"), -float("inf")):
+        for x in (k, v):
+            x.masked_fill_(hidden[:, None, :, None], fill)
+        again, again_lse = engine.attention_tree(q, k, v, kv_lens, parents, window=window or None, sinks=sinks,
+                                                 need_lse=True)
+        torch.cuda.synchronize()
+        engine.check_device_status()
+        assert torch.equal(again, out) and torch.equal(again_lse, lse)
