@@ -607,6 +607,7 @@ cudaError_t by_dtype(int dtype, F32 f32, F64 f64, F16 f16, BF16 bf16, A&&... a) 
 }
 
 constexpr int kGridMax = 65535;  // of a grid's second and third dimension
+constexpr int kMaxKeys = 1 << 30;  // tiles' ends behind the last key stay 32-bit numbers
 
 int check_window(const ts_attn_params* p, const ts_window* w) {
   const int st = check_params(p);
@@ -615,7 +616,7 @@ int check_window(const ts_attn_params* p, const ts_window* w) {
   if (p->causal_offset > (int64_t)1 << 62) return TS_ERR_INVALID_ARGUMENT;  // positions behind it stay 64-bit numbers
   if (p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
   if (p->q_heads > kGridMax || p->batch > kGridMax || (int64_t)p->kv_heads * p->batch > 0x7fffffff ||
-      p->kv_len > 1 << 30)
+      p->kv_len > kMaxKeys)
     return TS_ERR_UNSUPPORTED;
   return TS_OK;
 }
@@ -657,6 +658,7 @@ int check_tree(const ts_attn_params* p, const ts_tree* t) {
   if (t->window < 0 || t->sinks < 0) return TS_ERR_INVALID_ARGUMENT;
   if (p->mask_kind != TS_MASK_NONE) return TS_ERR_UNSUPPORTED;
   if (t->parents && p->q_len > TS_TREE_MAX_NODES) return TS_ERR_UNSUPPORTED;
+  if (p->kv_len > kMaxKeys) return TS_ERR_UNSUPPORTED;
   if ((int64_t)p->q_heads / p->kv_heads * p->q_len > 0x40000000 ||
       (int64_t)p->batch * p->q_heads * p->q_len > 0x40000000)
     return TS_ERR_UNSUPPORTED;

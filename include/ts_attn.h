@@ -441,7 +441,7 @@ typedef struct ts_tree {
 #define TS_TREE_MAX_NODES 64 /* q_len with parents; chains may be longer */
 
 /* Attention of q [batch, Hq, q_len, D] over the cache k, v: params as for ts_attn_decode with kv_lens required;
- * is_causal and causal_offset are ignored, no explicit mask.  Slots at and behind kv_lens[b] are not used, whatever
+ * is_causal and causal_offset are ignored, no explicit mask, kv_len is 2^30 at most.  Slots at and behind kv_lens[b] are not used, whatever
  * they hold; the values of the others must be finite (one that is not may reach nodes that do not see it).  Half types with equal head dimensions that are multiples of 8 up to 128 run on the tcgen05 kernel. */
 TS_ATTN_API int ts_attn_tree(const ts_attn_params* params, const ts_tree* tree, void* workspace,
                              size_t workspace_bytes, void* stream);
