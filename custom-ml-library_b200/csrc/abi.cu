@@ -632,6 +632,8 @@ int check_window_bwd(const ts_attn_bwd_params* bp, const ts_window* w) {
   const int st = check_window(&bp->fwd, w);
   if (st != TS_OK) return st;
   if (!bp->fwd.lse || !bp->dout.data || !bp->dq.data || !bp->dk.data || !bp->dv.data) return TS_ERR_INVALID_ARGUMENT;
+  // Tiles of 128 keys are a grid's second dimension on the tensor cores, those with sinks in up to 64 parts (only while
+  // there are fewer of them than SMs).
   if (bp->fwd.kv_len > 64 * kGridMax || (int64_t)bp->fwd.batch * bp->fwd.q_heads > 0x7fffffff ||
       (int64_t)bp->fwd.batch * bp->fwd.q_heads * bp->fwd.q_len > (int64_t)1 << 33)
     return TS_ERR_UNSUPPORTED;

@@ -505,13 +505,14 @@ __global__ void __launch_bounds__(512, 1)
 }
 
 // dq[b,h,i,:] = dq_acc (fp32, one channel-major [D][64] tile per 64 rows) converted
-// to the input dtype: one CTA per (tile, b*h) transposes its tile through
-// shared memory so both the read and the write are coalesced.
+// to the input dtype: one CTA per (tile, b*h), in the grid's first dimension,
+// which holds any number of tiles, transposes its tile through shared memory
+// so both the read and the write are coalesced.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) dq_convert_kernel(const float* __restrict__ acc, ts_view4 dq, int heads,
-                                                         int len, int n_tiles, int dim = D) {
+__global__ void __launch_bounds__(256) dq_convert_kernel(const float* __restrict__ acc, ts_view4 dq, int batch,
+                                                         int heads, int len, int n_tiles, int dim) {
   __shared__ float tile[kBM][D + 1];
-  const int bh = blockIdx.x, t = blockIdx.y;
+  const int bh = blockIdx.x % (batch * heads), t = blockIdx.x / (batch * heads);
   const float4* src = reinterpret_cast<const float4*>(acc + ((int64_t)bh * n_tiles + t) * (D * kBM));
   for (int idx = threadIdx.x; idx < D * (kBM / 4); idx += blockDim.x) {
     const int d = idx / (kBM / 4), j = (idx % (kBM / 4)) ^ (d & 7);
@@ -788,19 +789,15 @@ cudaError_t tc_backward(const ts_attn_bwd_params& bp, void* ws, size_t ws_bytes,
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  const dim3 cgrid((unsigned)(p.batch * p.q_heads), (unsigned)(t_pad / kBM));
   const int n_tiles = t_pad / kBM;
-  if (p.head_dim <= 64) {
-    if (bf)
-      dq_convert_kernel<__nv_bfloat16, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
-    else
-      dq_convert_kernel<__half, 64><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
-  } else {
-    if (bf)
-      dq_convert_kernel<__nv_bfloat16, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
-    else
-      dq_convert_kernel<__half, 128><<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.q_heads, p.q_len, n_tiles, p.head_dim);
-  }
+  const unsigned cgrid = (unsigned)((int64_t)p.batch * p.q_heads * n_tiles);
+  auto convert = [&](auto kern) {
+    kern<<<cgrid, 256, 0, st>>>(dq_acc, bp.dq, p.batch, p.q_heads, p.q_len, n_tiles, p.head_dim);
+  };
+  if (p.head_dim <= 64)
+    bf ? convert(dq_convert_kernel<__nv_bfloat16, 64>) : convert(dq_convert_kernel<__half, 64>);
+  else
+    bf ? convert(dq_convert_kernel<__nv_bfloat16, 128>) : convert(dq_convert_kernel<__half, 128>);
   return cudaGetLastError();
 }
 

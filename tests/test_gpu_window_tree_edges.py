@@ -1,11 +1,12 @@
 """Windows and drafted trees where they can go wrong beside sizes and masks: head dimensions of half a quad, NaN through
-the join of many partial results, slots that nobody sees."""
+the join of many partial results, slots that nobody sees, more
+queries than a grid's second dimension has tiles."""
 
 import random
 
 import pytest
 
-from plain64 import DTYPES, tree_seen
+from plain64 import DTYPES, Attention, tree_seen, window_seen, within
 from test_gpu_tree import check, random_tree
 from test_gpu_window import run
 
@@ -108,3 +109,24 @@ def test_slots_of_padded_nodes_may_hold_anything(dtype, dim, window, sinks):
         torch.cuda.synchronize()
         engine.check_device_status()
         assert torch.equal(again, out) and torch.equal(again_lse, lse)
+
+
+def test_more_queries_than_a_grid_has_rows_of_tiles():
+    """4.2 million queries, 65537 tiles of 64: the last of them, and keys that the first ones alone see."""
+    tokens, keys, dim, window, sinks, last = 65536 * 64 + 70, 200, 8, 40, 2, 100
+    q, g = make("bf16", 1, 1, tokens, dim), make("bf16", 1, 1, tokens, dim, seed=1)
+    k, v = make("bf16", 1, 1, keys, dim, seed=2), make("bf16", 1, 1, keys, dim, seed=3)
+    kw = dict(is_causal=True, window=window, sinks=sinks)
+    out, lse = engine.forward(q, k, v, **kw)
+    dq, dk, dv = engine.backward(q, k, v, out, lse, g, **kw)
+    torch.cuda.synchronize()
+    engine.check_device_status()
+    for first, n in ((0, 400), (tokens - last, last)):
+        some = slice(first, first + n)
+        ref = Attention(q[:, :, some], k, v, window_seen(1, n, keys, window, sinks, first))
+        ref.check(out[:, :, some], lse[:, :, some])
+        want, bounds = ref.backward(g[:, :, some])
+        within(dq[:, :, some], want[0], bounds[0], "dq")
+        if first == 0:  # behind the sinks, a key is seen by the window's queries alone
+            within(dk[:, :, sinks:], want[1][:, :, sinks:], bounds[1][:, :, sinks:], "dk")
+            within(dv[:, :, sinks:], want[2][:, :, sinks:], bounds[2][:, :, sinks:], "dv")
