@@ -969,8 +969,11 @@ def token_logprobs_backward(logits, targets, result, grad_logprob=None, grad_ent
                 raise ValueError("gradients must be fp32 of the shapes of what they belong to, on the logits' device")
             g = g.contiguous()
         given.append(g)
-    if result.logprob.shape != targets.shape or result.logprob.get_device() != index:
-        raise ValueError("the result belongs to other logits")
+    shape, fp32 = targets.shape, torch.float32
+    for t, want, dtype in ((result.logprob, shape, fp32), (result.entropy, shape, fp32), (result.norm, (*shape, 2), fp32),
+                           (result.top_logprobs, (*shape, top), fp32), (result.top_indices, (*shape, top), torch.int64)):
+        if t.shape != want or t.dtype != dtype or t.get_device() != index:
+            raise ValueError("the result belongs to other logits")
     rows, vocab = flat.shape
     grad = torch.empty((rows, vocab), dtype=flat.dtype, device=flat.device)
     if rows:
