@@ -559,8 +559,28 @@ __global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_k
   const float g_target = real && a.grad_logprob ? a.grad_logprob[row] : 0.f;
   float g_entropy = a.grad_entropy ? a.grad_entropy[row] : 0.f;
   float g_all = g_target;
+  bool idle = !real && g_entropy == 0.f;
   if (a.grad_top)
-    for (int j = 0; j < p.top; ++j) g_all += a.grad_top[row * p.top + j];
+    for (int j = 0; j < p.top; ++j) {
+      const float g = a.grad_top[row * p.top + j];
+      g_all += g;
+      idle = idle && g == 0.f;
+    }
+  // Where the gradient's rows lie otherwise than the logits', elements are stored one by one.
+  const bool aligned = (reinterpret_cast<uintptr_t>(out + span.head) & 15) == 0;
+  const bool last = part == a.parts - 1;
+  if (idle) {  // an ignored row that counts in nothing else has no gradient, whatever its logits are
+    for (int v = v_first + id; v < v_last; v += kGroup) {
+      T* to = out + span.head + (int64_t)v * N;
+      if (aligned)
+        *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+      else
+        for (int i = 0; i < N; ++i) to[i] = Elem<T>::from_acc(0.f);
+    }
+    if (last)
+      for (int i = id; i < span.edges(); i += kGroup) out[span.edge_index(i)] = Elem<T>::from_acc(0.f);
+    return;
+  }
   // A target outside the vocabulary has no log probability: its row's gradient is NaN, as that is.
   if (real && a.grad_logprob && (target < 0 || target >= p.vocab)) g_all = __int_as_float(0x7fc00000);
   const bool none = log_s == -INFINITY;  // a row without a distribution (every logit -inf) has no gradient
@@ -581,8 +601,6 @@ __global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_k
     grads_of(ptx::f2pack(v, v), g0, g1);
     return g0;
   };
-  // Where the gradient's rows lie otherwise than the logits', elements are stored one by one.
-  const bool aligned = (reinterpret_cast<uintptr_t>(out + span.head) & 15) == 0;
   for (int v0 = v_first + id; v0 < v_last;) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -607,7 +625,6 @@ __global__ void __launch_bounds__(kSmallBlock, kSmallPerSm) token_logprobs_bwd_k
     v0 += kGroup * kUnroll;
     load(v0);
   }
-  const bool last = part == a.parts - 1;
   if (last)
     for (int i = id; i < span.edges(); i += kGroup) out[span.edge_index(i)] = Elem<T>::from_acc(grad_of(span.at(span.edge_index(i))));
   // The target and the alternatives: their elements once more, with what they receive themselves.

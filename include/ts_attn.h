@@ -495,7 +495,8 @@ typedef struct ts_token_logprobs {
 #define TS_TOP_TOKENS_MAX 32
 TS_ATTN_API int ts_token_logprobs_fwd(const ts_token_logprobs* params, void* stream);
 /* grad_logits [rows, vocab] (dtype of the logits, another buffer) from the gradients of logprob, entropy and
- * top_logprobs (each optional, fp32, contiguous), given the forward's norm, entropy and top_indices. */
+ * top_logprobs (each optional, fp32, contiguous), given the forward's norm, entropy and top_indices.  A row with an
+ * ignored target, to which the latter two give 0 or nothing, has a gradient of 0 whatever its logits are. */
 TS_ATTN_API int ts_token_logprobs_bwd(const ts_token_logprobs* params, const float* grad_logprob,
                                       const float* grad_entropy, const float* grad_top, void* grad_logits,
                                       int64_t grad_stride, void* stream);

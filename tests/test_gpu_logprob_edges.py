@@ -1,4 +1,4 @@
-"""Log probabilities of tokens: results that do not belong to the call."""
+"""Log probabilities of tokens: results that do not belong to the call, ignored rows of anything."""
 
 import pytest
 
@@ -23,3 +23,28 @@ def test_results_of_another_call():
                 dict(logprob=less.logprob)):
         with pytest.raises(ValueError):
             engine.token_logprobs_backward(x, t, r._replace(**bad), g, g, torch.ones(6, 3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [70, 5003, 50257])
+def test_ignored_rows_may_hold_anything(dtype, vocab):
+    """A padded row has no gradient, whatever its logits are; one that an entropy or an alternative counts in has."""
+    x = torch.randn(6, vocab, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    t = torch.tensor([3, -100, 5, -100, -100, -100], device="cuda")
+    clean = engine.token_logprobs(x, t, top=2)
+    g = torch.randn(6, device="cuda")
+    weight = (t >= 0).float()
+    uses = ((g, None, None), (g, g * weight, None), (g, g * weight, torch.ones(6, 2, device="cuda") * weight[:, None]))
+    want = [engine.token_logprobs_backward(x, t, clean, *use) for use in uses]
+    x[1] = float("nan")
+    x[3, vocab // 2], x[4] = float("inf"), -float("inf")
+    got = engine.token_logprobs(x, t, top=2)
+    assert not got.logprob[[1, 3, 4]].any()
+    for use, ref in zip(uses, want):
+        d = engine.token_logprobs_backward(x, t, got, *use)
+        assert not d[[1, 3, 4, 5]].any() and torch.equal(d[[0, 2]], ref[[0, 2]])
+    ones = torch.ones(6, device="cuda")
+    d = engine.token_logprobs_backward(x, t, got, g, ones)
+    assert d[1].isnan().all() and d[3].isnan().any() and not d[4].any() and d[5].any()
+    d = engine.token_logprobs_backward(x, t, got, g, None, torch.ones(6, 2, device="cuda"))
+    assert d[1].isnan().all() and d[5].any()
