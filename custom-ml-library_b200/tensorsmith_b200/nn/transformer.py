@@ -76,6 +76,18 @@ class _AttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None, None
 
 
+class _DifferentiatedFn(torch.autograd.Function):
+    """A gradient that kernels made, as a function of what it was made from: its own derivative is an error."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("log probabilities of tokens have no second derivative")
+
+
 class _TokenLogprobsFn(torch.autograd.Function):
     """Log probabilities, entropies and alternatives of logits; their joint gradient in one pass."""
 
@@ -94,13 +106,16 @@ class _TokenLogprobsFn(torch.autograd.Function):
         grads = [None if g is None else g.float() for g in (g_logprob, g_entropy, g_top)]
         if all(g is None for g in grads):
             return None, None, None, None
-        return engine.token_logprobs_backward(logits, targets, engine.TokenLogprobs(*result), *grads,
-                                              ignore_index=ctx.ignore_index), None, None, None
+        grad = engine.token_logprobs_backward(logits, targets, engine.TokenLogprobs(*result), *grads,
+                                              ignore_index=ctx.ignore_index)
+        if torch.is_grad_enabled():  # create_graph: the gradient depends on all of these
+            grad = _DifferentiatedFn.apply(grad, logits, *grads)
+        return grad, None, None, None
 
 
 def token_logprobs(logits, targets, *, top: int = 0, ignore_index: int = -100) -> engine.TokenLogprobs:
     """Log probabilities of ``targets`` [...] under ``logits`` [..., V], entropies and the ``top`` most likely
-    alternatives (``engine.token_logprobs``), differentiable in ``logits``."""
+    alternatives (``engine.token_logprobs``), differentiable once in ``logits``."""
     return engine.TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, top, ignore_index))
 
 

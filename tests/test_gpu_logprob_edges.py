@@ -1,11 +1,12 @@
-"""Log probabilities of tokens: results that do not belong to the call, ignored rows of anything."""
+"""Log probabilities of tokens: results that do not belong to the call, ignored rows of anything, second
+derivatives."""
 
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from tensorsmith_b200 import engine  # noqa: E402
+from tensorsmith_b200 import engine, nn  # noqa: E402
 
 
 def test_results_of_another_call():
@@ -48,3 +49,12 @@ def test_ignored_rows_may_hold_anything(dtype, vocab):
     assert d[1].isnan().all() and d[3].isnan().any() and not d[4].any() and d[5].any()
     d = engine.token_logprobs_backward(x, t, got, g, None, torch.ones(6, 2, device="cuda"))
     assert d[1].isnan().all() and d[5].any()
+
+
+def test_no_second_derivative():
+    """Of a gradient that the kernels made there is none: asked for one, torch raises instead of leaving a term out."""
+    x = torch.randn(4, 30, device="cuda", requires_grad=True)
+    result = nn.token_logprobs(x, torch.arange(4, device="cuda"))
+    (g,) = torch.autograd.grad(result.logprob.sum() + result.entropy.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (g.square().sum() + x.sum()).backward()
