@@ -76,6 +76,9 @@ class _AttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None, None
 
 
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
 class _DifferentiatedFn(torch.autograd.Function):
     """A gradient that kernels made, as a function of what it was made from: its own derivative is an error."""
 
@@ -447,9 +450,13 @@ class TransformerLM(_Module):
         if parents is not None:
             if caches is None:
                 raise ValueError("drafted trees need caches")
-            parents = torch.as_tensor(parents).to(self.device, torch.int32).contiguous()
-            if parents.shape != tokens.shape:
+            parents = torch.as_tensor(parents)
+            if parents.shape != tokens.shape or parents.dtype not in _INTEGERS:
                 raise ValueError("parents must be one integer a token")
+            parents = parents.to(self.device)
+            if parents.dtype == torch.int64:  # entries beyond 32 bits mark padding as others do
+                parents = parents.clamp(-2, parents.shape[1])
+            parents = parents.int().contiguous()
         offset = 0
         if caches is not None:
             if len(caches) != len(self.blocks) or len({cache.length for cache in caches}) != 1:
