@@ -723,6 +723,15 @@ def attention_int4(q, pool, page_table, kv_lens, *, page_size, max_len=None, is_
 # -- drafted tokens over a cache -----------------------------------------------
 
 
+def check_tree(parents, rows: int, nodes: int, index: int) -> None:
+    """Raises unless ``parents`` are those of ``attention_tree`` for ``rows`` trees of ``nodes`` on device ``index``."""
+    if parents.dtype != torch.int32 or parents.shape != (rows, nodes) or parents.get_device() != index or (
+            parents.stride(1) != 1 and nodes > 1):
+        raise ValueError("parents must be int32 [batch, nodes] with contiguous rows on the query's device")
+    if nodes > _lib.TREE_MAX_NODES:
+        raise ValueError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes")
+
+
 def _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse):
     """(packed ts_attn_params, packed ts_tree, device index) of an attention_tree call after its checks."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -742,11 +751,7 @@ def _tree_args(q, k, v, kv_lens, parents, window, sinks, scale, out, lse):
     lens = _int32_vector(kv_lens, "kv_lens", rows, index)
     tree, stride = 0, 0
     if parents is not None:
-        if parents.dtype != torch.int32 or parents.shape != (rows, nodes) or parents.get_device() != index or (
-                parents.stride(1) != 1 and nodes > 1):
-            raise ValueError("parents must be int32 [batch, nodes] with contiguous rows on the query's device")
-        if nodes > _lib.TREE_MAX_NODES:
-            raise ValueError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes")
+        check_tree(parents, rows, nodes, index)
         tree, stride = parents.data_ptr(), parents.stride(0)
     if window is None:
         _no_window(sinks)

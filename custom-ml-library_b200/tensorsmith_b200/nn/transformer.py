@@ -283,6 +283,8 @@ class MultiHeadAttention(_Module):
                                     or isinstance(cache, PagedLayer)):
             raise ValueError("drafted trees need causal attention over a KVCache, without a mask")
         batch, steps, _ = input.shape
+        if parents is not None:  # before the cache takes the step
+            engine.check_tree(parents, batch, steps, input.get_device())
         offset = 0 if cache is None else cache.length
         if attn_mask is not None:
             expected = (batch, self.num_heads, steps, offset + source.shape[1])

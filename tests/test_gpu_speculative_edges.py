@@ -1,11 +1,12 @@
-"""Drafted trees through the models: entries of ``parents`` beyond 32 bits."""
+"""Drafted trees through the models: entries of ``parents`` beyond 32 bits, steps that are refused."""
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from tensorsmith_b200 import no_grad  # noqa: E402
+from tensorsmith_b200 import nn, no_grad  # noqa: E402
 from test_gpu_speculative import model  # noqa: E402
 
 
@@ -45,3 +46,21 @@ def test_parents_of_any_integer_type(dtype):
             lm(torch.tensor([[1, 2, 3]]), caches=caches)
             logits.append(lm(torch.tensor([[4, 5, 6, 7]]), caches=caches, parents=given))
     assert torch.equal(*logits)
+
+
+@pytest.mark.parametrize("rotary", [True, False])
+def test_a_refused_tree_leaves_the_module_s_cache(rotary):
+    np.random.seed(1)
+    attention = nn.MultiHeadAttention(64, 4, rotary=rotary, device="cuda").eval()
+    cache = nn.KVCache(1, 4, 16, 200)
+    x = torch.randn(1, 70, 64, device="cuda")
+    int32 = lambda *shape: torch.full(shape, -1, dtype=torch.int32, device="cuda")  # noqa: E731
+    with no_grad(), torch.no_grad():
+        attention(x[:, :5], cache=cache)
+        for steps, parents in ((70, int32(1, 70)), (3, int32(1, 4)), (3, int32(1, 3).long()), (3, int32(2, 3)),
+                               (3, int32(1, 3).cpu()), (3, int32(3))):
+            with pytest.raises(ValueError):
+                attention(x[:, :steps], cache=cache, parents=parents)
+            assert cache.length == 5
+        attention(x[:, :64], cache=cache, parents=int32(1, 64))
+        assert cache.length == 69
