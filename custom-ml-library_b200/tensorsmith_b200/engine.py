@@ -1125,8 +1125,8 @@ def rope_inv_freq(rotary_dim: int, base: float, device) -> torch.Tensor:
 
 def rope(x, *, offset=0, base=10000.0, rotary_dim=None, positions=None, inverse=False, out=None):
     """Interleaved-pair rotary embedding of a [B, H, T, C] view at positions offset + t
-    (or positions[b] + t; or positions[b, t], as ``tree_positions`` gives them); ``inverse`` applies the inverse
-    rotation (the VJP)."""
+    (or positions[b] + t, positions [B] or [B, 1]; or positions[b, t], as ``tree_positions`` gives them); ``inverse``
+    applies the inverse rotation (the VJP)."""
     _require_cuda(x)
     dim = x.shape[3] if rotary_dim is None else int(rotary_dim)
     out = torch.empty_like(x) if out is None else out
@@ -1134,6 +1134,8 @@ def rope(x, *, offset=0, base=10000.0, rotary_dim=None, positions=None, inverse=
     pos = None
     if positions is not None:
         pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
+        if pos.shape == (x.shape[0], 1):  # a row's, as [B]
+            pos = pos.reshape(-1).contiguous()
         if pos.dim() == 2:
             if pos.shape != (x.shape[0], x.shape[2]) or pos.device != x.device:
                 raise ValueError("positions of every token must be [B, T] on the input's device")

@@ -1,6 +1,6 @@
 """Windows and drafted trees where they can go wrong beside sizes and masks: head dimensions of half a quad, NaN through
 the join of many partial results, slots that nobody sees, more
-queries than a grid's second dimension has tiles."""
+queries than a grid's second dimension has tiles, positions in a column."""
 
 import random
 
@@ -130,3 +130,10 @@ def test_more_queries_than_a_grid_has_rows_of_tiles():
         if first == 0:  # behind the sinks, a key is seen by the window's queries alone
             within(dk[:, :, sinks:], want[1][:, :, sinks:], bounds[1][:, :, sinks:], "dk")
             within(dv[:, :, sinks:], want[2][:, :, sinks:], bounds[2][:, :, sinks:], "dv")
+
+
+def test_positions_of_one_column():
+    """Positions [B, 1] are a row's, as [B] are: token t stands at positions[b] + t."""
+    x = make("f32", 2, 3, 5, 64)
+    positions = torch.tensor([7, 300], dtype=torch.int32, device="cuda")
+    assert torch.equal(engine.rope(x, positions=positions[:, None]), engine.rope(x, positions=positions))
