@@ -1134,10 +1134,12 @@ def rope(x, *, offset=0, base=10000.0, rotary_dim=None, positions=None, inverse=
     pos = None
     if positions is not None:
         pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
+        if pos.get_device() != x.get_device() or pos.numel() < x.shape[0]:
+            raise ValueError("positions must be one a row or one a token, on the input's device")
         if pos.shape == (x.shape[0], 1):  # a row's, as [B]
             pos = pos.reshape(-1).contiguous()
         if pos.dim() == 2:
-            if pos.shape != (x.shape[0], x.shape[2]) or pos.device != x.device:
+            if pos.shape != (x.shape[0], x.shape[2]):
                 raise ValueError("positions of every token must be [B, T] on the input's device")
             pos = pos.contiguous()
             with _on(x.get_device()):

@@ -137,3 +137,13 @@ def test_positions_of_one_column():
     x = make("f32", 2, 3, 5, 64)
     positions = torch.tensor([7, 300], dtype=torch.int32, device="cuda")
     assert torch.equal(engine.rope(x, positions=positions[:, None]), engine.rope(x, positions=positions))
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_positions_that_are_refused(tokens):
+    x = make("f32", 2, 3, tokens, 64)
+    cuda = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")  # noqa: E731
+    for positions in (cuda(2, 1).cpu(), cuda(2, tokens).cpu(), cuda(2).cpu(), cuda(1), cuda(1, 1), cuda(2, tokens + 1),
+                      cuda(0)):
+        with pytest.raises(ValueError, match="positions"):
+            engine.rope(x, positions=positions)
