@@ -147,3 +147,22 @@ def test_positions_that_are_refused(tokens):
                       cuda(0)):
         with pytest.raises(ValueError, match="positions"):
             engine.rope(x, positions=positions)
+
+
+@pytest.mark.parametrize("nodes,group", [(2, 1), (5, 2), (20, 2), (31, 5), (32, 3), (33, 4), (64, 5)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_slots_of_padded_nodes_in_trees_of_any_size(dtype, nodes, group):
+    rng = random.Random(nodes)
+    trees = [random_tree(rng, nodes) for _ in range(5)]
+    for tree in trees:
+        for i in rng.sample(range(nodes), max(1, nodes // 6)):
+            tree[i] = rng.choice([-2, nodes, i])
+    lens = [nodes + 100, nodes - 1, 128, nodes + 3000, nodes + 127]
+    q, k, v, kv_lens, parents, out, lse = check(dtype, 2 * group, 2, 64, lens, trees, capacity=3100)
+    hidden = ~tree_seen(trees, lens, 3100).any(2)[:, 0].cuda()
+    for b, n in enumerate(lens):
+        hidden[b, : max(n - nodes, 0)] = hidden[b, n:] = False
+    assert hidden.any()
+    v.masked_fill_(hidden[:, None, :, None], NAN)
+    again, again_lse = engine.attention_tree(q, k, v, kv_lens, parents, need_lse=True)
+    assert torch.equal(again, out) and torch.equal(again_lse, lse)
