@@ -14,6 +14,7 @@
 // 2 x 2000 queries 1170 us against 940), and by a block's chain of tiles in small calls.  fp32, D 64, counting the pairs
 // that are seen: 2 x 2000 queries, 8 heads, forward 428 us (19 TFLOP/s of 74), with a window of 500 195 us; forward and
 // backward, on 4 KV heads, 1396 and 710 us; 2 x 511 queries, 4 heads on 2, a window of 128, 3 sinks, both 101 us.
+// bf16 of 256 channels, 4096 queries, 16 heads on 8, a window of 1024: forward 2.86 ms (21 TFLOP/s), backward 18.8 (8).
 #pragma once
 #include "dependent.cuh"
 #include "simt_kernels.cuh"
