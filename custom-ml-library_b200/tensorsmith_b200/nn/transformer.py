@@ -57,6 +57,18 @@ class _RopeFn(torch.autograd.Function):
         return engine.rope(g.contiguous(), offset=ctx.offset, inverse=True), None
 
 
+class _DifferentiatedFn(torch.autograd.Function):
+    """A gradient that kernels made, as a function of what it was made from: its own derivative is an error."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("windowed attention and log probabilities of tokens have no second derivative")
+
+
 class _AttentionFn(torch.autograd.Function):
     """Attention forward / recomputing backward on the engine (nn/attention.py:132-252)."""
 
@@ -72,23 +84,13 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = engine.backward(q, k, v, out, lse, g.contiguous(), **ctx.kw)
-        return dq, dk, dv, None, None, None, None, None, None
+        grads = engine.backward(q, k, v, out, lse, g.contiguous(), **ctx.kw)
+        if ctx.kw["window"] is not None and torch.is_grad_enabled():  # create_graph
+            grads = (_DifferentiatedFn.apply(x, q, k, v, g) for x in grads)
+        return *grads, None, None, None, None, None, None
 
 
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
-
-
-class _DifferentiatedFn(torch.autograd.Function):
-    """A gradient that kernels made, as a function of what it was made from: its own derivative is an error."""
-
-    @staticmethod
-    def forward(ctx, grad, *sources):
-        return grad.view_as(grad)
-
-    @staticmethod
-    def backward(ctx, g):
-        raise RuntimeError("log probabilities of tokens have no second derivative")
 
 
 class _TokenLogprobsFn(torch.autograd.Function):

@@ -64,3 +64,15 @@ def test_a_refused_tree_leaves_the_module_s_cache(rotary):
             assert cache.length == 5
         attention(x[:, :64], cache=cache, parents=int32(1, 64))
         assert cache.length == 69
+
+
+def test_windowed_attention_has_no_second_derivative():
+    """Asked for one, torch raises; a first derivative under create_graph is what it is without."""
+    np.random.seed(2)
+    attention = nn.MultiHeadAttention(64, 4, window=5, sinks=1, device="cuda").train()
+    x = torch.randn(2, 20, 64, device="cuda", requires_grad=True)
+    (plain,) = torch.autograd.grad(attention(x).square().sum(), x)
+    (g,) = torch.autograd.grad(attention(x).square().sum(), x, create_graph=True)
+    assert torch.equal(plain, g)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.square().sum().backward()
